@@ -26,6 +26,10 @@ ERRORS = {
 }
 QTYPE_Q8_0 = 8
 QTYPE_Q4_0 = 2
+F32, F16, BF16 = 0, 1, 30  # ggml type ids
+PLAN_BAD_LENGTH, PLAN_TABLE_FULL, PLAN_ROWS_FULL, PLAN_NO_PAGES = 1, 2, 4, 8
+ROPE_INTERLEAVED, ROPE_HALF = 0, 1
+ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_BANDS, ROPE_SCALE_YARN = 0, 1, 2, 3
 
 
 class TpShare(C.Structure):
@@ -69,6 +73,31 @@ class Timings(C.Structure):
 class SampleOpts(C.Structure):
     _fields_ = [("temperature", C.c_double), ("top_k", C.c_int32), ("top_p", C.c_double),
                 ("repeat_penalty", C.c_double), ("num_predict", C.c_int32), ("seed", C.c_uint64)]
+
+
+class PagedKV(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int32), ("n_pages", C.c_int32),
+                ("page_size", C.c_int32), ("nkv", C.c_int32), ("hd", C.c_int32), ("reserved", C.c_int32),
+                ("page_stride", C.c_int64), ("pos_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class RopeOpts(C.Structure):
+    _fields_ = [("rot_dim", C.c_int32), ("scaling", C.c_int32), ("theta", C.c_double), ("factor", C.c_double),
+                ("orig_ctx", C.c_double), ("low", C.c_double), ("high", C.c_double)]
+
+
+class RopeRows(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("nh", C.c_int32), ("nkv", C.c_int32), ("hd", C.c_int32),
+                ("rot_dim", C.c_int32), ("layout", C.c_int32), ("scale", C.c_float), ("reserved", C.c_int32),
+                ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64),
+                ("q_out_stride", C.c_int64), ("k_out_stride", C.c_int64)]
+
+
+class PagedAttnOpts(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("nh", C.c_int32), ("n_req", C.c_int32), ("max_pages", C.c_int32),
+                ("len_add", C.c_int32), ("window", C.c_int32), ("scale", C.c_float), ("softcap", C.c_float),
+                ("slopes", C.c_void_p), ("q_stride", C.c_int64), ("out_stride", C.c_int64),
+                ("table_stride", C.c_int64)]
 
 
 def build(verbose: bool = False) -> str:
@@ -122,6 +151,14 @@ SIGNATURES = {
     "b2_batch_use_graph": (C.c_int, [_P, _i32]),
     "b2_attention_decode": (C.c_int, [_P, _P, _P, _P, _i32, _i32, _i32, _i32, _i32, _P]),
     "b2_attention_decode_noalloc": (C.c_int, [_P, _P, _P, _P, _i32, _i32, _i32, _i32, _i32, _P]),
+    "b2_page_plan": (C.c_int, [_P, _P, _i32, _i32, _P, _P, _P, _i64, _i32, _P, _P, _P, _P, _P, _i32, _P, _P]),
+    "b2_rope_freqs": (C.c_int, [C.POINTER(RopeOpts), C.POINTER(C.c_double), C.POINTER(C.c_float)]),
+    "b2_rope": (C.c_int, [C.POINTER(RopeRows), _P, _P, _i32, _P, _P, _P, _P, _P]),
+    "b2_rope_append": (C.c_int, [C.POINTER(RopeRows), C.POINTER(PagedKV), _P, _P, _P, _i32, _P, _P, _P, _P, _P]),
+    "b2_attention_paged_scratch_bytes": (_i64, [_i32, _i32, _i32, _i32]),
+    "b2_attention_paged": (C.c_int, [C.POINTER(PagedKV), C.POINTER(PagedAttnOpts), _P, _P, _P, _P, _i32, _P, _P, _P,
+                                     _P]),
+    "b2_logprobs": (C.c_int, [_P, _i32, _i32, _i32, _i64, _P, _i32, _P, _P, _i32, _P, _P, _P]),
     "b2_device_status": (C.c_int, [_P]),
     "b2_stream_handle": (_P, [_P]),
     "b2_trace_step": (C.c_int, [_P, _i32, C.POINTER(_i64), _i64, _i32p, _i32p]),
@@ -425,3 +462,83 @@ def attention_decode_noalloc(q_ptr: int, k_ptr: int, v_ptr: int, out_ptr: int, b
                              hd: int, ctx: int, stream: int = 0) -> None:
     """attention_decode without device allocation (fixed in-library scratch)."""
     _check(lib().b2_attention_decode_noalloc(q_ptr, k_ptr, v_ptr, out_ptr, batch, nh, nkv, hd, ctx, stream or None))
+
+
+def paged_kv(k_ptr: int, v_ptr: int, dtype: int, n_pages: int, page_size: int, nkv: int, hd: int,
+             page_stride: int = 0, pos_stride: int = 0, head_stride: int = 0) -> PagedKV:
+    """A paged KV cache (b2_paged_kv): k and v at device addresses, dtype F16 or
+    BF16, strides in elements (all 0: dense [n_pages][page_size][nkv][hd])."""
+    return PagedKV(k_ptr, v_ptr, dtype, n_pages, page_size, nkv, hd, 0, page_stride, pos_stride, head_stride)
+
+
+def page_plan(cached: int, fresh: int, n_req: int, page_size: int, free_pages: int, n_free: int, table: int,
+              table_stride: int, max_pages: int, lens: int, starts: int, slots: int, positions: int, token_req: int,
+              max_tokens: int, info: int, stream: int = 0) -> None:
+    """b2_page_plan on device addresses: table entries, slots, positions and
+    requests of a step's tokens from the requests' lengths.  info[0] != 0
+    (PLAN_* bits) says that the step does not fit."""
+    _check(lib().b2_page_plan(cached, fresh, n_req, page_size, free_pages, n_free, table, table_stride, max_pages,
+                              lens, starts, slots, positions, token_req, max_tokens, info, stream or None))
+
+
+def rope_freqs(rot_dim: int, theta: float, scaling: int = ROPE_SCALE_NONE, factor: float = 1.0, orig_ctx: float = 0.0,
+               low: float = 0.0, high: float = 0.0) -> tuple:
+    """b2_rope_freqs: (radians per position of each pair as float64, the factor on cos and sin)."""
+    o = RopeOpts(int(rot_dim), int(scaling), float(theta), float(factor), float(orig_ctx), float(low), float(high))
+    out = np.empty(max(rot_dim // 2, 1), dtype=np.float64)
+    scale = C.c_float()
+    _check(lib().b2_rope_freqs(C.byref(o), out.ctypes.data_as(C.POINTER(C.c_double)), C.byref(scale)))
+    return out, scale.value
+
+
+def rope_rows(dtype: int, nh: int, nkv: int, hd: int, rot_dim: int, layout: int = ROPE_INTERLEAVED, scale: float = 1.0,
+              q_stride: int = 0, k_stride: int = 0, v_stride: int = 0, q_out_stride: int = 0,
+              k_out_stride: int = 0) -> RopeRows:
+    """The rows of a rotary call (b2_rope_rows); strides in elements, 0 = dense."""
+    return RopeRows(dtype, nh, nkv, hd, rot_dim, layout, scale, 0, q_stride, k_stride, v_stride, q_out_stride,
+                    k_out_stride)
+
+
+def rope(rows: RopeRows, freqs: int, positions: int, n_tok: int, q: int = 0, k: int = 0, q_out: int = 0,
+         k_out: int = 0, stream: int = 0) -> None:
+    """b2_rope on device addresses: q -> q_out and k -> k_out (either pair 0), in place allowed."""
+    _check(lib().b2_rope(C.byref(rows), freqs, positions, n_tok, q or None, k or None, q_out or None, k_out or None,
+                         stream or None))
+
+
+def rope_append(rows: RopeRows, kv: PagedKV, freqs: int, positions: int, slots: int, n_tok: int, q: int, k: int,
+                v: int, q_out: int, stream: int = 0) -> None:
+    """b2_rope_append on device addresses: q -> q_out, k (rotated) and v -> the cache at slots."""
+    _check(lib().b2_rope_append(C.byref(rows), C.byref(kv), freqs, positions, slots, n_tok, q or None, k, v,
+                                q_out or None, stream or None))
+
+
+def paged_attn_opts(dtype: int, nh: int, n_req: int, max_pages: int, len_add: int = 0, window: int = 0,
+                    scale: float = 0.0, softcap: float = 0.0, slopes: int = 0, q_stride: int = 0, out_stride: int = 0,
+                    table_stride: int = 0) -> PagedAttnOpts:
+    """Options of attention_paged (b2_paged_attn_opts); slopes: device address of nh floats or 0."""
+    return PagedAttnOpts(dtype, nh, n_req, max_pages, len_add, window, scale, softcap, slopes or None, q_stride,
+                         out_stride, table_stride)
+
+
+def attention_paged_scratch_bytes(batch: int, nh: int, nkv: int, hd: int) -> int:
+    """Device scratch attention_paged needs (on the current device)."""
+    n = int(lib().b2_attention_paged_scratch_bytes(batch, nh, nkv, hd))
+    if n < 0:
+        _check(n)
+    return n
+
+
+def attention_paged(kv: PagedKV, opts: PagedAttnOpts, q: int, table: int, lens: int, req: int, batch: int, out: int,
+                    lse: int, scratch: int, stream: int = 0) -> None:
+    """b2_attention_paged on device addresses (req and lse may be 0)."""
+    _check(lib().b2_attention_paged(C.byref(kv), C.byref(opts), q, table, lens, req or None, batch, out, lse or None,
+                                    scratch, stream or None))
+
+
+def logprobs(logits: int, dtype: int, n: int, rows: int, ld: int, ids: int, m: int, logprob: int, entropy: int,
+             k: int, top_ids: int, top_logprob: int, stream: int = 0) -> None:
+    """b2_logprobs on device addresses: log p of ids [rows][m], entropy [rows]
+    (0: not wanted), the k best alternatives [rows][k]."""
+    _check(lib().b2_logprobs(logits, dtype, n, rows, ld, ids or None, m, logprob or None, entropy or None, k,
+                             top_ids or None, top_logprob or None, stream or None))

@@ -6,11 +6,14 @@
 #include <chrono>
 #include <cmath>
 #include <cstring>
+#include <initializer_list>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "gemm.h"
 #include "model.h"
+#include "paged.h"
 #include "sample.h"
 
 int b2_load_impl(const char* path, const b2_load_opts* opts, b2_model** out, std::string* err);
@@ -27,6 +30,7 @@ int b2_batch_prefill_impl(b2_batch* bt, int slot, const int32_t* prompt, int n, 
 int b2_batch_step_impl(b2_batch* bt, const int32_t* tokens, int32_t* next_out, std::string* err);
 int b2_batch_logits_impl(const b2_batch* bt, float* out, std::string* err);
 int b2_batch_use_graph_impl(b2_batch* bt, int on);
+int b2_rope_freqs_impl(const b2_rope_opts& o, double* freqs, float* scale);
 int b2_attention_impl(const float* q, const uint16_t* k, const uint16_t* v, float* out, int batch, int nh, int nkv,
                       int hd, int ctx, cudaStream_t s, std::string* err);
 int b2_attention_noalloc_impl(const float* q, const uint16_t* k, const uint16_t* v, float* out, int batch, int nh,
@@ -39,6 +43,72 @@ thread_local std::string g_last_error;
 int ret(int code, const std::string& msg = "") {
     if (code != B2_OK) g_last_error = msg.empty() ? "error" : msg;
     return code;
+}
+
+// Runs an entry point's body: an exception becomes B2_ERR_OOM.
+template <typename F>
+auto guarded(F&& body) noexcept -> decltype(body()) {
+    try {
+        return body();
+    } catch (...) {
+        g_last_error.clear();  // (no message: even that may not fit)
+        return B2_ERR_OOM;
+    }
+}
+
+bool float_type(int32_t t) { return t == 0 || t == 1 || t == 30; }
+
+int on_device(const char* who, std::initializer_list<std::pair<const char*, const void*>> ptrs) {
+    std::string err;
+    for (const auto& p : ptrs) {
+        const int rc = b2::check_device_pointer(p.second, p.first, &err);
+        if (rc != B2_OK) return ret(rc, std::string(who) + ": " + err);
+    }
+    return B2_OK;
+}
+
+// Checks a paged cache's description and fills in dense strides.
+int paged_kv_args(const char* who, const b2_paged_kv* kv, b2_paged_kv* out) {
+    const std::string w(who);
+    if (!kv || !kv->k || !kv->v) return ret(B2_ERR_BAD_ARG, w + ": null cache");
+    if (kv->dtype != 1 && kv->dtype != 30)
+        return ret(B2_ERR_UNSUPPORTED_TYPE, w + ": the cache's type must be 1 (F16) or 30 (BF16)");
+    if (kv->n_pages <= 0 || kv->page_size <= 0 || kv->nkv <= 0 || kv->hd <= 0)
+        return ret(B2_ERR_BAD_ARG, w + ": the cache's sizes must be positive");
+    if (kv->hd % 8 || kv->hd > b2::kPagedMaxHd)
+        return ret(B2_ERR_BAD_ARG, w + ": head_dim must be a multiple of 8, at most 256");
+    *out = *kv;
+    if (!kv->page_stride && !kv->pos_stride && !kv->head_stride) {
+        out->head_stride = kv->hd;
+        out->pos_stride = (int64_t)kv->nkv * kv->hd;
+        out->page_stride = out->pos_stride * kv->page_size;
+    }
+    if (out->page_stride < 0 || out->pos_stride < 0 || out->head_stride < 0 ||
+        (out->page_stride | out->pos_stride | out->head_stride) % 8)
+        return ret(B2_ERR_BAD_ARG, w + ": the cache's strides must be multiples of 8, not negative");
+    if ((reinterpret_cast<uintptr_t>(kv->k) | reinterpret_cast<uintptr_t>(kv->v)) & 15)
+        return ret(B2_ERR_BAD_ARG, w + ": k and v must be 16-byte aligned");
+    return B2_OK;
+}
+
+int rope_rows_args(const char* who, const b2_rope_rows* r, b2_rope_rows* out) {
+    const std::string w(who);
+    if (!r) return ret(B2_ERR_BAD_ARG, w + ": null argument");
+    if (!float_type(r->dtype)) return ret(B2_ERR_UNSUPPORTED_TYPE, w + ": dtype must be 0 (F32), 1 (F16) or 30 (BF16)");
+    if (r->nh < 0 || r->nkv < 0 || r->hd <= 0 || r->hd % 2 || r->hd > b2::kPagedMaxHd ||
+        (int64_t)r->nh + 2 * (int64_t)r->nkv > (1 << 20))
+        return ret(B2_ERR_BAD_ARG, w + ": bad heads (head_dim even, at most 256)");
+    if (r->rot_dim < 0 || r->rot_dim > r->hd || r->rot_dim % 2)
+        return ret(B2_ERR_BAD_ARG, w + ": rot_dim must be even, 0 .. head_dim");
+    if (r->layout != B2_ROPE_INTERLEAVED && r->layout != B2_ROPE_HALF) return ret(B2_ERR_BAD_ARG, w + ": unknown layout");
+    if (r->q_stride < 0 || r->k_stride < 0 || r->v_stride < 0 || r->q_out_stride < 0 || r->k_out_stride < 0)
+        return ret(B2_ERR_BAD_ARG, w + ": negative stride");
+    if ((r->q_out_stride && r->q_out_stride < (int64_t)r->nh * r->hd) ||
+        (r->k_out_stride && r->k_out_stride < (int64_t)r->nkv * r->hd))
+        return ret(B2_ERR_BAD_ARG, w + ": output rows overlap");
+    *out = *r;
+    if (out->scale == 0.0f) out->scale = 1.0f;
+    return B2_OK;
 }
 
 bool cuda_ok(cudaError_t e, std::string* err) {
@@ -576,6 +646,148 @@ int b2_attention_decode(const float* q, const uint16_t* k, const uint16_t* v, fl
     std::string err;
     int rc = b2_attention_impl(q, k, v, out, batch, nh, nkv, hd, ctx, static_cast<cudaStream_t>(stream), &err);
     return ret(rc, err);
+}
+
+int b2_page_plan(const int32_t* cached, const int32_t* fresh, int32_t n_req, int32_t page_size,
+                 const int32_t* free_pages, const int32_t* n_free, int32_t* table, int64_t table_stride,
+                 int32_t max_pages, int32_t* lens, int32_t* starts, int64_t* slots, int32_t* positions,
+                 int32_t* token_req, int32_t max_tokens, int32_t* info, void* stream) {
+    return guarded([&] {
+        if (!cached || !fresh || !free_pages || !n_free || !table || !lens || !starts || !slots || !positions ||
+            !token_req || !info)
+            return ret(B2_ERR_BAD_ARG, "b2_page_plan: null argument");
+        if (n_req <= 0 || n_req > b2::kPlanMaxReq)
+            return ret(B2_ERR_BAD_ARG, "b2_page_plan: takes 1 to 16384 requests");
+        if (page_size <= 0 || max_pages <= 0 || max_tokens <= 0 || table_stride < max_pages)
+            return ret(B2_ERR_BAD_ARG, "b2_page_plan: page_size, max_pages and max_tokens must be positive, table_stride >= max_pages");
+        int rc = on_device("b2_page_plan", {{"cached", cached}, {"table", table}, {"slots", slots}});
+        if (rc != B2_OK) return rc;
+        const b2::PagePlanArgs a{cached, fresh,     free_pages, n_free,    table,     table_stride, lens,      starts,
+                                 slots,  positions, token_req,  info,      n_req,     page_size,    max_pages, max_tokens};
+        std::string err;
+        rc = b2::launch_page_plan(a, static_cast<cudaStream_t>(stream), &err);
+        return ret(rc, err);
+    });
+}
+
+int b2_rope_freqs(const b2_rope_opts* o, double* freqs, float* scale) {
+    return guarded([&] {
+        if (!o || !freqs) return ret(B2_ERR_BAD_ARG, "b2_rope_freqs: null argument");
+        if (o->rot_dim <= 0 || o->rot_dim % 2 || !(o->theta > 1.0) || !std::isfinite(o->theta))
+            return ret(B2_ERR_BAD_ARG, "b2_rope_freqs: rot_dim must be even and positive, theta > 1");
+        if (o->scaling < B2_ROPE_SCALE_NONE || o->scaling > B2_ROPE_SCALE_YARN)
+            return ret(B2_ERR_BAD_ARG, "b2_rope_freqs: unknown scaling");
+        if (o->scaling != B2_ROPE_SCALE_NONE && !(o->factor > 0.0 && std::isfinite(o->factor)))
+            return ret(B2_ERR_BAD_ARG, "b2_rope_freqs: factor must be positive");
+        if (o->scaling >= B2_ROPE_SCALE_BANDS && !(o->orig_ctx > 0.0 && std::isfinite(o->orig_ctx)))
+            return ret(B2_ERR_BAD_ARG, "b2_rope_freqs: orig_ctx must be positive");
+        return ret(b2_rope_freqs_impl(*o, freqs, scale), "b2_rope_freqs: high must be above low");
+    });
+}
+
+int b2_rope(const b2_rope_rows* rows, const double* freqs, const int32_t* positions, int32_t n_tok, const void* q,
+            const void* k, void* q_out, void* k_out, void* stream) {
+    return guarded([&] {
+        b2_rope_rows r;
+        int rc = rope_rows_args("b2_rope", rows, &r);
+        if (rc != B2_OK) return rc;
+        if (!positions || (!freqs && r.rot_dim) || n_tok <= 0 || !q != !q_out || !k != !k_out || (!q && !k))
+            return ret(B2_ERR_BAD_ARG, "b2_rope: null argument or no tokens");
+        if ((q && r.nh <= 0) || (k && r.nkv <= 0)) return ret(B2_ERR_BAD_ARG, "b2_rope: bad heads");
+        rc = on_device("b2_rope", {{"q", q}, {"k", k}, {"q_out", q_out}, {"k_out", k_out}, {"positions", positions}});
+        if (rc != B2_OK) return rc;
+        std::string err;
+        rc = b2::launch_rope(r, nullptr, freqs, positions, nullptr, n_tok, q, k, nullptr, q_out, k_out,
+                             static_cast<cudaStream_t>(stream), &err);
+        return ret(rc, err);
+    });
+}
+
+int b2_rope_append(const b2_rope_rows* rows, const b2_paged_kv* kv, const double* freqs, const int32_t* positions,
+                   const int64_t* slots, int32_t n_tok, const void* q, const void* k, const void* v, void* q_out,
+                   void* stream) {
+    return guarded([&] {
+        b2_rope_rows r;
+        int rc = rope_rows_args("b2_rope_append", rows, &r);
+        if (rc != B2_OK) return rc;
+        b2_paged_kv c;
+        rc = paged_kv_args("b2_rope_append", kv, &c);
+        if (rc != B2_OK) return rc;
+        if (!positions || !slots || (!freqs && r.rot_dim) || n_tok <= 0 || !q != !q_out || !k || !v)
+            return ret(B2_ERR_BAD_ARG, "b2_rope_append: null argument or no tokens");
+        if ((q && r.nh <= 0) || r.nkv != c.nkv || r.hd != c.hd)
+            return ret(B2_ERR_BAD_ARG, "b2_rope_append: the rows' heads do not match the cache's");
+        if (r.dtype != 0 && r.dtype != c.dtype)
+            return ret(B2_ERR_UNSUPPORTED_TYPE, "b2_rope_append: rows must be F32 or of the cache's type");
+        rc = on_device("b2_rope_append", {{"q", q}, {"k", k}, {"v", v}, {"q_out", q_out}, {"the cache", c.k}, {"slots", slots}});
+        if (rc != B2_OK) return rc;
+        std::string err;
+        rc = b2::launch_rope(r, &c, freqs, positions, slots, n_tok, q, k, v, q_out, nullptr,
+                             static_cast<cudaStream_t>(stream), &err);
+        return ret(rc, err);
+    });
+}
+
+int64_t b2_attention_paged_scratch_bytes(int32_t batch, int32_t nh, int32_t nkv, int32_t hd) {
+    return guarded([&]() -> int64_t {
+        if (batch <= 0 || nh <= 0 || nkv <= 0 || nh % nkv || hd <= 0 || hd > b2::kPagedMaxHd)
+            return ret(B2_ERR_BAD_ARG, "b2_attention_paged_scratch_bytes: bad sizes");
+        std::string err;
+        const int sms = b2::current_sms(&err);
+        if (!sms) return ret(B2_ERR_CUDA, err);
+        return (int64_t)b2::attention_paged_scratch(batch, nh, nkv, hd, sms);
+    });
+}
+
+int b2_attention_paged(const b2_paged_kv* kv, const b2_paged_attn_opts* opts, const void* q, const int32_t* table,
+                       const int32_t* lens, const int32_t* req, int32_t batch, void* out, float* lse,
+                       void* d_scratch, void* stream) {
+    return guarded([&] {
+        b2_paged_kv c;
+        int rc = paged_kv_args("b2_attention_paged", kv, &c);
+        if (rc != B2_OK) return rc;
+        if (!opts || !q || !table || !lens || !out || !d_scratch || batch <= 0)
+            return ret(B2_ERR_BAD_ARG, "b2_attention_paged: null argument or no rows");
+        const b2_paged_attn_opts& o = *opts;
+        if (o.dtype != 0 && o.dtype != c.dtype)
+            return ret(B2_ERR_UNSUPPORTED_TYPE, "b2_attention_paged: q must be F32 or of the cache's type");
+        if (o.nh <= 0 || o.nh % c.nkv || (int64_t)batch * o.nh > 0x7fffffff)
+            return ret(B2_ERR_BAD_ARG, "b2_attention_paged: the query heads must be a multiple of the cache's heads");
+        if (o.n_req <= 0 || o.max_pages <= 0 || (!req && batch > o.n_req) || o.len_add < 0)
+            return ret(B2_ERR_BAD_ARG, "b2_attention_paged: bad table (n_req, max_pages, len_add)");
+        const int64_t qd = (int64_t)o.nh * c.hd;
+        if (o.window < 0 || !(o.scale >= 0.0f) || !(o.softcap >= 0.0f) || std::isinf(o.scale) || std::isinf(o.softcap) ||
+            o.q_stride < 0 || (o.out_stride && o.out_stride < qd) || (o.table_stride && o.table_stride < o.max_pages))
+            return ret(B2_ERR_BAD_ARG, "b2_attention_paged: bad window, scale, softcap or stride");
+        if (reinterpret_cast<uintptr_t>(d_scratch) & 15)
+            return ret(B2_ERR_BAD_ARG, "b2_attention_paged: scratch must be 16-byte aligned");
+        rc = on_device("b2_attention_paged", {{"q", q}, {"the cache", c.k}, {"table", table}, {"out", out}, {"scratch", d_scratch}});
+        if (rc != B2_OK) return rc;
+        std::string err;
+        rc = b2::launch_attention_paged(c, o, q, table, lens, req, batch, out, lse, d_scratch,
+                                        static_cast<cudaStream_t>(stream), &err);
+        return ret(rc, err);
+    });
+}
+
+int b2_logprobs(const void* logits, int32_t dtype, int32_t n, int32_t rows, int64_t ld, const int32_t* ids, int32_t m,
+                float* logprob, float* entropy, int32_t k, int32_t* top_ids, float* top_logprob, void* stream) {
+    return guarded([&] {
+        if (!logits || n <= 0 || n > (1 << 30) || rows <= 0 || ld < n || m < 0 || k < 0)
+            return ret(B2_ERR_BAD_ARG, "b2_logprobs: bad argument");
+        if (!float_type(dtype)) return ret(B2_ERR_UNSUPPORTED_TYPE, "b2_logprobs: dtype must be 0 (F32), 1 (F16) or 30 (BF16)");
+        if (k > b2::kLogprobMaxTop || k > n) return ret(B2_ERR_BAD_ARG, "b2_logprobs: at most 64 alternatives, and n");
+        if ((m && (!ids || !logprob)) || (k && (!top_ids || !top_logprob)))
+            return ret(B2_ERR_BAD_ARG, "b2_logprobs: null argument");
+        if (!m && !k && !entropy) return B2_OK;
+        int rc = on_device("b2_logprobs", {{"logits", logits}, {"ids", m ? ids : nullptr}, {"logprob", m ? logprob : nullptr},
+                                           {"entropy", entropy}, {"top_ids", k ? top_ids : nullptr}});
+        if (rc != B2_OK) return rc;
+        std::string err;
+        rc = b2::launch_logprobs(logits, dtype, n, rows, ld, ids, m, logprob, entropy, k, top_ids, top_logprob,
+                                 static_cast<cudaStream_t>(stream), &err);
+        return ret(rc, err);
+    });
 }
 
 int b2_trace_step(b2_model* m, int32_t token, int64_t* out_ns, int64_t cap, int32_t* n_phases, int32_t* n_ctas) {

@@ -1,0 +1,383 @@
+// Log probabilities of given tokens, the entropy and the top alternatives of
+// rows of logits.
+//
+// With m = max x and d = x - m:  S = sum e^d,  T = sum d e^d,
+//   log p(i) = d_i - log S,   H = log S - T / S.
+// (Both terms of H are >= 0, so nothing cancels.)  One pass keeps (m, S, T)
+// per thread, rescaled when a thread's maximum grows:
+//   m -> m':  S' = S e^(m - m'),  T' = e^(m - m') (T + (m - m') S).
+//
+// Top k without a second pass over the row.  Every thread of the pass ends
+// with the largest logit it saw; the k-th largest of those maxima is a lower
+// bound of the k-th largest logit, and a logit at or above it can only be in
+// a thread whose maximum is.  About k of the threads' shares are read again
+// (from L2) for their candidates, which are ordered by counting.  Where very
+// many threads tie at the bound (a vocabulary masked with one value), the
+// logits above it come from fewer than k threads, and the ties are taken in
+// index order from the start of the row.
+//
+// A row's slices go to the CTAs of a cluster, so that few rows still fill the
+// machine; the lists and sums meet in the first CTA's hands over distributed
+// shared memory.  HBM-bound for fp32, close to the rate of the exponential
+// units for 16-bit logits.
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "dev.cuh"
+#include "paged.h"
+
+namespace b2 {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int kLpThreads = 512;
+constexpr int kLpWarps = kLpThreads / 32;
+constexpr int kLpMaxCluster = 8;
+constexpr int kLpRound = kLpThreads * 8;         // logits one collecting round may add
+constexpr int kLpCap = kLpRound + 1024;          // candidates held at once
+constexpr int kLpPlainThreads = 128;             // more threads at the bound than this: the ties path
+constexpr float kLog2eF = 1.4426950408889634f;
+constexpr float kLn2F = 0.6931471805599453f;
+
+struct LogprobArgs {
+    const void* x;
+    int64_t ld;
+    const int32_t* ids;
+    float *logprob, *entropy, *top_logprob;
+    int32_t* top_ids;
+    int n, m, k, cluster, wide;
+};
+
+__device__ __forceinline__ float lf(float x) { return x; }
+__device__ __forceinline__ float lf(__half x) { return __half2float(x); }
+__device__ __forceinline__ float lf(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+__device__ __forceinline__ float lex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// max that keeps a NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
+// Order of the alternatives: value down (-0 equals 0), then index up.
+__device__ __forceinline__ unsigned long long key_of(float x, int i) {
+    uint32_t b = __float_as_uint(x + 0.0f);
+    b = (b & 0x80000000u) ? ~b : b | 0x80000000u;
+    return ((unsigned long long)b << 32) | (uint32_t)~i;
+}
+__device__ __forceinline__ int key_index(unsigned long long k) { return (int)~(uint32_t)k; }
+
+struct Sums {
+    float m, S, T;  // T in units of log 2: sum (x - m) log2(e) 2^(..)
+};
+
+// b's sums added to a's
+__device__ __forceinline__ Sums join(Sums a, Sums b) {
+    Sums r;
+    r.m = fmaxf(a.m, b.m);
+    const float z = r.m == -INFINITY ? 0.0f : r.m;
+    const float da = max_nan((a.m - z) * kLog2eF, -150.0f), db = max_nan((b.m - z) * kLog2eF, -150.0f);
+    const float fa = lex2(da), fb = lex2(db);
+    r.S = a.S * fa + b.S * fb;
+    r.T = fa * fmaf(da, a.S, a.T) + fb * fmaf(db, b.S, b.T);
+    return r;
+}
+
+struct LpShared {
+    Sums part[kLpWarps];
+    Sums row;                                // this CTA's slice
+    float tmax[kLpThreads];
+    float thr;
+    int n_above, n_at, n_cand, found;
+    int wcount[kLpWarps];
+    unsigned short who[kLpThreads];
+    unsigned long long top[kLogprobMaxTop];  // this CTA's list, in order
+    unsigned long long cand[kLpCap];
+};
+
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) LpPack {
+    T v[VEC];
+};
+
+// The k largest of s.cand[0 .. cnt) into s.top in order (zeros past cnt).
+__device__ void order_top(LpShared& s, int cnt, int k) {
+    for (int i = threadIdx.x; i < k; i += kLpThreads)
+        if (i >= cnt) s.top[i] = 0;
+    for (int i = threadIdx.x; i < cnt; i += kLpThreads) {
+        const unsigned long long key = s.cand[i];
+        int above = 0;
+        for (int j = 0; j < cnt; j++) above += s.cand[j] > key;
+        if (above < k) s.top[above] = key;
+    }
+    __syncthreads();
+}
+
+// One CTA: the slice [v0, v1) of a row in chunks of VEC logits (the last one
+// cut at n).
+template <typename T, int VEC>
+__device__ __forceinline__ void slice_pass(const T* x, int n, int v0, int v1, Sums& t) {
+    constexpr int U = VEC == 1 ? 4 : 32 / (int)sizeof(T) / VEC * 2;  // chunks in flight
+    using P = LpPack<T, VEC>;
+    const int full = min(v1, n / VEC);  // chunks without a cut
+    auto add = [&](const float* f, int cnt) {
+        float bm = f[0];
+#pragma unroll
+        for (int i = 1; i < cnt; i++) bm = fmaxf(bm, f[i]);
+        const float nm = fmaxf(t.m, bm);
+        const float z = nm == -INFINITY ? 0.0f : nm;
+        const float df = max_nan((t.m - z) * kLog2eF, -150.0f);
+        const float g = lex2(df);
+        t.T = g * fmaf(df, t.S, t.T);
+        t.S *= g;
+        t.m = nm;
+#pragma unroll
+        for (int i = 0; i < cnt; i++) {
+            const float d = max_nan((f[i] - z) * kLog2eF, -150.0f);
+            const float e = lex2(d);
+            t.S += e;
+            t.T = fmaf(d, e, t.T);
+        }
+    };
+    int v = v0 + (int)threadIdx.x;
+    for (; v + (U - 1) * kLpThreads < full; v += U * kLpThreads) {
+        P p[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) p[u] = *reinterpret_cast<const P*>(x + (int64_t)(v + u * kLpThreads) * VEC);
+        float f[U * VEC];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int i = 0; i < VEC; i++) f[u * VEC + i] = lf(p[u].v[i]);
+        add(f, U * VEC);
+    }
+    for (; v < full; v += kLpThreads) {
+        const P p = *reinterpret_cast<const P*>(x + (int64_t)v * VEC);
+        float f[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; i++) f[i] = lf(p.v[i]);
+        add(f, VEC);
+    }
+    for (; v < v1; v += kLpThreads)  // the cut chunk
+        for (int i = v * VEC; i < n; i++) {
+            const float f = lf(x[i]);
+            add(&f, 1);
+        }
+}
+
+// The k largest of the slice into s.top, from the threads' maxima in s.tmax.
+template <typename T, int VEC>
+__device__ __forceinline__ void slice_top(const T* x, int n, int v0, int v1, int k, LpShared& s) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const float mine = s.tmax[tid];
+    if (tid == 0) s.n_above = s.n_at = s.n_cand = 0;
+    int above = 0;
+    for (int j = 0; j < kLpThreads; j++) {
+        const float o = s.tmax[j];
+        above += o > mine || (o == mine && j < tid);
+    }
+    if (above == min(k, kLpThreads) - 1) s.thr = mine;
+    __syncthreads();
+    const float thr = s.thr;
+    if (mine >= thr) {
+        if (mine > thr) atomicAdd(&s.n_above, 1);
+        atomicAdd(&s.n_at, 1);
+    }
+    __syncthreads();
+    const bool plain = s.n_at <= kLpPlainThreads && thr > -INFINITY;
+    const int n_who = plain ? s.n_at : s.n_above;
+    __syncthreads();
+    if (tid == 0) s.found = 0;
+    __syncthreads();
+    if (plain ? mine >= thr : mine > thr) s.who[atomicAdd(&s.found, 1)] = (unsigned short)tid;
+    __syncthreads();
+
+    // the candidates: chunk i of thread who[j] is v0 + who[j] + i * kLpThreads
+    const int per = (v1 - v0 + kLpThreads - 1) / kLpThreads;
+    const int total = n_who * per;
+    unsigned long long bound = 0;  // after a cut of the list: keys at or under it are out
+    for (int base = 0; base < total; base += kLpThreads) {
+        const int c = base + tid;
+        if (c < total) {
+            const int v = v0 + s.who[c / per] + (c % per) * kLpThreads;
+            if (v < v1) {
+                for (int i = v * VEC, e = min(n, v * VEC + VEC); i < e; i++) {
+                    const float f = lf(x[i]);
+                    if (plain ? f >= thr : f > thr) {
+                        const unsigned long long key = key_of(f, i);
+                        if (key > bound) s.cand[atomicAdd(&s.n_cand, 1)] = key;
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        const int cnt = s.n_cand;
+        if (cnt > kLpCap - kLpRound && base + kLpThreads < total) {
+            order_top(s, cnt, k);
+            for (int i = tid; i < k; i += kLpThreads) s.cand[i] = s.top[i];
+            bound = s.top[k - 1];
+            if (tid == 0) s.n_cand = k;
+        }
+        __syncthreads();
+    }
+    // ties at the bound, in index order
+    if (!plain) {
+        const int i1 = min(n, v1 * VEC);
+        int cnt = min(s.n_cand, k);  // (fewer than k logits lie above the bound, unless one thread has several)
+        order_top(s, s.n_cand, k);
+        for (int base = v0 * VEC; base < i1 && cnt < k; base += kLpThreads) {
+            const int i = base + tid;
+            const bool tie = i < i1 && lf(x[i]) == thr;
+            const unsigned bal = __ballot_sync(0xffffffffu, tie);
+            if (lane == 0) s.wcount[warp] = __popc(bal);
+            __syncthreads();
+            int at = cnt + __popc(bal & ((1u << lane) - 1)), all = 0;
+            for (int w = 0; w < kLpWarps; w++) {
+                if (w < warp) at += s.wcount[w];
+                all += s.wcount[w];
+            }
+            if (tie && at < k) s.top[at] = key_of(thr, i);
+            cnt = min(k, cnt + all);
+            __syncthreads();
+        }
+    } else {
+        order_top(s, s.n_cand, k);
+    }
+}
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kLpThreads) logprob_kernel(const __grid_constant__ LogprobArgs a) {
+    extern __shared__ __align__(16) uint8_t lp_raw[];
+    LpShared& s = *reinterpret_cast<LpShared*>(lp_raw);
+    pdl_trigger();
+    pdl_wait();
+    const int C = a.cluster, rank = C > 1 ? (int)cg::this_cluster().block_rank() : 0;
+    const int64_t row = blockIdx.x / C;
+    const T* x = static_cast<const T*>(a.x) + row * a.ld;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int nv = (a.n + VEC - 1) / VEC, per = (nv + C - 1) / C;
+    const int v0 = min(nv, rank * per), v1 = min(nv, v0 + per);
+
+    Sums t{-INFINITY, 0.0f, 0.0f};
+    slice_pass<T, VEC>(x, a.n, v0, v1, t);
+    s.tmax[tid] = t.m;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        const Sums p{__shfl_xor_sync(0xffffffffu, t.m, o), __shfl_xor_sync(0xffffffffu, t.S, o),
+                     __shfl_xor_sync(0xffffffffu, t.T, o)};
+        t = join(t, p);
+    }
+    if (lane == 0) s.part[warp] = t;
+    __syncthreads();
+    if (tid == 0) {
+        for (int w = 1; w < kLpWarps; w++) t = join(t, s.part[w]);
+        s.row = t;
+    }
+    if (a.k > 0) slice_top<T, VEC>(x, a.n, v0, v1, a.k, s);
+    __syncthreads();
+
+    if (C > 1) {
+        cg::cluster_group cl = cg::this_cluster();
+        cl.sync();
+        if (rank == 0) {
+            if (tid == 0)
+                for (int r = 1; r < C; r++) s.row = join(s.row, cl.map_shared_rank(&s, r)->row);
+            // the C lists as one, with no empty places
+            if (tid == 0) s.n_cand = 0;
+            __syncthreads();
+            for (int i = tid; i < C * a.k; i += kLpThreads) {
+                const unsigned long long key = cl.map_shared_rank(&s, i / a.k)->top[i % a.k];
+                if (key) s.cand[atomicAdd(&s.n_cand, 1)] = key;
+            }
+            __syncthreads();
+            if (a.k > 0) order_top(s, s.n_cand, a.k);
+            __syncthreads();
+        }
+        cl.sync();  // no CTA leaves while its lists are read
+        if (rank) return;
+    }
+    const Sums r = s.row;
+    const float lS = logf(r.S);
+    const float z = r.m == -INFINITY ? 0.0f : r.m;
+    auto lp = [&](float v) { return (v - z) - lS; };
+    const float nan = __int_as_float(0x7fc00000);
+    for (int i = tid; i < a.m; i += kLpThreads) {
+        const int id = a.ids[row * a.m + i];
+        a.logprob[row * a.m + i] = id >= 0 && id < a.n && r.m != -INFINITY ? lp(lf(x[id])) : nan;
+    }
+    if (tid == 0 && a.entropy) a.entropy[row] = lS - r.T / r.S * kLn2F;
+    for (int i = tid; i < a.k; i += kLpThreads) {
+        const unsigned long long key = s.top[i];
+        const int id = key ? key_index(key) : -1;
+        a.top_ids[row * a.k + i] = id;
+        a.top_logprob[row * a.k + i] = id >= 0 && r.m != -INFINITY ? lp(lf(x[id])) : nan;
+    }
+}
+
+template <typename T>
+cudaError_t go(const LogprobArgs& a, int rows, cudaStream_t s) {
+    constexpr int W = 16 / sizeof(T);
+    auto kern = a.wide ? logprob_kernel<T, W> : logprob_kernel<T, 1>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(LpShared));
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(rows * a.cluster));
+    cfg.blockDim = dim3(kLpThreads);
+    cfg.dynamicSmemBytes = sizeof(LpShared);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim = {(unsigned)a.cluster, 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = a.cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kern, a);
+}
+
+}  // namespace
+
+int launch_logprobs(const void* logits, int dtype, int n, int rows, int64_t ld, const int32_t* ids, int m,
+                    float* logprob, float* entropy, int k, int32_t* top_ids, float* top_logprob, cudaStream_t s,
+                    std::string* err) {
+    const int sms = current_sms(err);
+    if (!sms) return B2_ERR_CUDA;
+    const int es = dtype == 0 ? 4 : 2;
+    LogprobArgs a{};
+    a.x = logits;
+    a.ld = ld;
+    a.ids = ids;
+    a.logprob = logprob;
+    a.entropy = entropy;
+    a.top_ids = top_ids;
+    a.top_logprob = top_logprob;
+    a.n = n;
+    a.m = m;
+    a.k = k;
+    // 16-byte loads where every row starts on 16 bytes
+    a.wide = !((uintptr_t)logits & 15) && (rows == 1 || ld * es % 16 == 0);
+    // CTAs per row: while the rows do not fill the machine and a slice keeps 4096 logits
+    int c = 1;
+    while (c < kLpMaxCluster && rows * 2LL * c <= sms && n / (2 * c) >= 4096) c *= 2;
+    a.cluster = c;
+    const cudaError_t e = dtype == 0   ? go<float>(a, rows, s)
+                          : dtype == 1 ? go<__half>(a, rows, s)
+                                       : go<__nv_bfloat16>(a, rows, s);
+    if (e != cudaSuccess) {
+        *err = std::string("log probabilities launch: ") + cudaGetErrorString(e);
+        return B2_ERR_CUDA;
+    }
+    return B2_OK;
+}
+
+}  // namespace b2

@@ -302,6 +302,176 @@ int b2_batch_logits(const b2_batch* b, float* out);
  * stepping eagerly.  Off by default. */
 int b2_batch_use_graph(b2_batch* b, int32_t on);
 
+/* ---- paged serving step: plan, rotate + append, attend, score ----
+ *
+ * A server that keeps its KV cache in pages (blocks of page_size positions,
+ * handed out as sequences grow) runs a step in this order: b2_page_plan takes
+ * pages from the free list and says where every token of the step goes;
+ * b2_rope_append rotates q and k and writes k and v to those places;
+ * b2_attention_paged attends, one query row per token; b2_logprobs scores the
+ * logits.  Kernel-level entry points: DEVICE pointers unless said otherwise,
+ * on the current device (host memory, or another device's, fails with
+ * B2_ERR_BAD_ARG), asynchronous on `stream` (a cudaStream_t; NULL = the legacy
+ * default stream), no allocation, no state kept between calls, capturable in a
+ * CUDA graph.  Calls that overlap on the GPU must not share outputs or
+ * scratch.  Types are ggml type ids: 0 = F32, 1 = F16, 30 = BF16.  The Go
+ * engine has one contiguous cache per sequence (kvCache,
+ * transformer.go:61-92); these have no counterpart there beyond the
+ * arithmetic cited. */
+
+/* A paged KV cache: the element d of head h of position s of page p is at
+ * k[p * page_stride + s * pos_stride + h * head_stride + d], v alike.  Strides
+ * in elements; all three 0 = dense [n_pages][page_size][nkv][hd].  k and v on
+ * 16 bytes, strides multiples of 8, hd a multiple of 8 up to 256. */
+typedef struct {
+    void* k;
+    void* v;
+    int32_t dtype; /* 1 = F16, 30 = BF16 */
+    int32_t n_pages;
+    int32_t page_size;
+    int32_t nkv;
+    int32_t hd;
+    int32_t reserved;
+    int64_t page_stride;
+    int64_t pos_stride;
+    int64_t head_stride;
+} b2_paged_kv;
+
+/* Why a plan did not fit: bits of b2_page_plan's info[0]. */
+#define B2_PLAN_BAD_LENGTH 1 /* a negative length */
+#define B2_PLAN_TABLE_FULL 2 /* a request needs more than max_pages pages, or passes 2^31 - 1 positions */
+#define B2_PLAN_ROWS_FULL 4  /* more new tokens than max_tokens */
+#define B2_PLAN_NO_PAGES 8   /* more new pages than *n_free */
+
+/* Block tables and slot maps from request lengths.  Request r (of n_req, at
+ * most 16384) holds cached[r] positions in the first ceil(cached[r] /
+ * page_size) entries of its table row (table + r * table_stride, max_pages
+ * entries) and gets fresh[r] >= 0 more tokens.  New pages are taken from the
+ * front of free_pages (*n_free of them, a device word), in request order.
+ * Writes
+ *   table      the new entries, nothing else
+ *   lens[r]    cached[r] + fresh[r]
+ *   starts     [n_req + 1] first token row of each request, and the total
+ *   slots, positions, token_req  [max_tokens], for each token in request
+ *              order: page * page_size + place in the page, the position, the
+ *              request; the rows past the last token get -1, 0, -1
+ *   info       [4] {status, tokens, pages taken, 0}
+ * A step that does not fit (status != 0, B2_PLAN_* bits) leaves the table as
+ * it was and is an empty one otherwise: every token row -1, starts 0, lens =
+ * cached.  A token in a page whose table or list entry is negative gets slot
+ * -1.  No two requests may share a page that either still writes. */
+int b2_page_plan(const int32_t* cached, const int32_t* fresh, int32_t n_req, int32_t page_size,
+                 const int32_t* free_pages, const int32_t* n_free, int32_t* table, int64_t table_stride,
+                 int32_t max_pages, int32_t* lens, int32_t* starts, int64_t* slots, int32_t* positions,
+                 int32_t* token_req, int32_t max_tokens, int32_t* info, void* stream);
+
+#define B2_ROPE_INTERLEAVED 0 /* pairs (2i, 2i + 1), as transformer.go:935-955 rotates */
+#define B2_ROPE_HALF 1        /* pairs (i, i + rot_dim / 2) */
+
+#define B2_ROPE_SCALE_NONE 0
+#define B2_ROPE_SCALE_LINEAR 1 /* every frequency over factor */
+#define B2_ROPE_SCALE_BANDS 2  /* over factor where a pair turns at most `low` times in orig_ctx positions, kept
+                                  where it turns at least `high` times, blended linearly in the turns between */
+#define B2_ROPE_SCALE_YARN 3   /* the same ends, blended linearly in the pair's number; cos and sin times
+                                  0.1 log(factor) + 1 */
+
+typedef struct {
+    int32_t rot_dim; /* rotated elements of a head (even) */
+    int32_t scaling; /* B2_ROPE_SCALE_* */
+    double theta;    /* rope_theta, > 1 */
+    double factor;   /* context stretch, > 0 (ignored for NONE) */
+    double orig_ctx; /* positions the model was trained on, > 0 (BANDS, YARN) */
+    double low;      /* <= 0: 1 */
+    double high;     /* <= 0: 4 (BANDS) or 32 (YARN) */
+} b2_rope_opts;
+
+/* The frequencies of b2_rope, radians per position, freqs[rot_dim / 2] (HOST
+ * memory; a server uploads them once), and the factor on cos and sin (scale;
+ * may be NULL).  transformer.go:939-942 is theta^(-2i/hd), in float64. */
+int b2_rope_freqs(const b2_rope_opts* opts, double* freqs, float* scale);
+
+/* The rows of a step: q [n_tok] rows of nh heads, k and v [n_tok] rows of nkv
+ * heads, hd elements a head (even, at most 256), heads back to back in a row.
+ * Strides in elements from row to row; 0 = dense.  Any alignment; rows on 16
+ * bytes run fastest. */
+typedef struct {
+    int32_t dtype; /* q, k, v, q_out, k_out: 0 = F32, 1 = F16, 30 = BF16 */
+    int32_t nh;
+    int32_t nkv;
+    int32_t hd;
+    int32_t rot_dim; /* the first rot_dim elements of a head turn, the rest stays (even, 0 .. hd) */
+    int32_t layout;  /* B2_ROPE_INTERLEAVED or B2_ROPE_HALF */
+    float scale;     /* factor on cos and sin; 0 = 1 */
+    int32_t reserved;
+    int64_t q_stride;
+    int64_t k_stride;
+    int64_t v_stride;
+    int64_t q_out_stride;
+    int64_t k_out_stride;
+} b2_rope_rows;
+
+/* transformer.go:935-955 applyRoPE on rows at positions[n_tok]: pair i turns
+ * by positions * freqs[i] (freqs [rot_dim / 2] device doubles), the angle
+ * reduced in 64 bits, the rotation in fp32, rounded once.  q -> q_out, k ->
+ * k_out; either pair may be NULL; a row may be rotated in place (q_out = q
+ * with the same stride), other overlaps are not allowed. */
+int b2_rope(const b2_rope_rows* rows, const double* freqs, const int32_t* positions, int32_t n_tok, const void* q,
+            const void* k, void* q_out, void* k_out, void* stream);
+/* The same, with k (rotated) and v written to the cache at slots[n_tok] (page
+ * * page_size + place, as b2_page_plan gives them; a slot below 0 or past the
+ * cache writes nothing).  q and q_out may be NULL.  The cache's type is the
+ * rows', or F16 / BF16 for F32 rows.  No two tokens may share a slot. */
+int b2_rope_append(const b2_rope_rows* rows, const b2_paged_kv* kv, const double* freqs, const int32_t* positions,
+                   const int64_t* slots, int32_t n_tok, const void* q, const void* k, const void* v, void* q_out,
+                   void* stream);
+
+typedef struct {
+    int32_t dtype;     /* q and out: 0 = F32, or the cache's type */
+    int32_t nh;        /* query heads, a multiple of the cache's nkv */
+    int32_t n_req;     /* rows of the table */
+    int32_t max_pages; /* entries of a table row */
+    int32_t len_add;   /* added to every lens entry */
+    int32_t window;    /* > 0: a row sees its last `window` positions only */
+    float scale;       /* 0 = 1 / sqrt(hd) */
+    float softcap;     /* > 0: s -> softcap * tanh(s / softcap) */
+    const float* slopes; /* [nh] device, or NULL: s += slope * (position - last position) */
+    int64_t q_stride;     /* elements from row to row; 0 = nh * hd */
+    int64_t out_stride;   /* 0 = nh * hd */
+    int64_t table_stride; /* 0 = max_pages */
+} b2_paged_attn_opts;
+
+/* transformer.go:663-685 attention of `batch` query rows over the paged cache:
+ * row b of q ([batch] rows of nh * hd) attends over the first lens[b] +
+ * len_add positions of the sequence in table row req[b] (req NULL: b).  With
+ * lens = the plan's positions, len_add = 1 and req = its token_req the rows
+ * are a step's tokens, prompts included.  The order per score is scale,
+ * softcap, slope, mask; fp32 softmax.  Writes out and, when lse is not NULL,
+ * lse[b][nh] = log of the sum of e^score.  A row that sees nothing (length <=
+ * 0, req < 0) gets zeros and -inf; a row whose length passes its table, whose
+ * req is n_req or more, or whose visible pages are not all in 0 .. n_pages - 1
+ * gets NaN.  Keys and values that are not seen may hold anything; an infinite
+ * value that is seen makes its element infinite or NaN.  Pages outside the
+ * window are not looked at.  d_scratch:
+ * b2_attention_paged_scratch_bytes(batch, nh, nkv, hd) bytes of device memory
+ * on 16 bytes, no contents needed. */
+int64_t b2_attention_paged_scratch_bytes(int32_t batch, int32_t nh, int32_t nkv, int32_t hd);
+int b2_attention_paged(const b2_paged_kv* kv, const b2_paged_attn_opts* opts, const void* q, const int32_t* table,
+                       const int32_t* lens, const int32_t* req, int32_t batch, void* out, float* lse,
+                       void* d_scratch, void* stream);
+
+/* Log probabilities of given tokens, the entropy and the top alternatives of
+ * rows of n logits (row i at logits + i * ld, ld >= n; n up to 2^30): the
+ * softmax of transformer.go:1050-1067 kept as logarithms, fp32 sums.
+ * logprob[i][m] = log p(ids[i][m]) (an id outside 0 .. n - 1: NaN),
+ * entropy[i] in nats (may be NULL), top_ids / top_logprob[i][k] = the k
+ * largest logits in order, equal ones by lowest id (k up to 64 and n).  A
+ * logit of -inf is a token left out: log p = -inf, nothing added to the
+ * entropy.  A row with a NaN or +inf, or with -inf alone, gets NaN for all but
+ * top_ids; NaN logits are never alternatives (a place left empty for that
+ * gets id -1). */
+int b2_logprobs(const void* logits, int32_t dtype, int32_t n, int32_t rows, int64_t ld, const int32_t* ids, int32_t m,
+                float* logprob, float* entropy, int32_t k, int32_t* top_ids, float* top_logprob, void* stream);
+
 /* ---- tensor parallelism (engine.go LoadOptions.NumGPU; no counterpart in the
  * Go engine, which runs on CPU cores) ----
  *
