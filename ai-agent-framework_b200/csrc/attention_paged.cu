@@ -10,27 +10,32 @@
 // it, whatever the number of query heads that share it.
 //
 // Split.  The work of the whole batch is one line of units, a unit being one
-// tile of kTile positions of one (sequence, KV head, block of 16 query
-// heads), and CTA c of G takes the units [c W / G, (c + 1) W / G).  Ragged
+// step of kStep positions of one (sequence, KV head, block of 16 query heads),
+// and worker w of G, a warp, takes the units [w W / G, (w + 1) W / G).  Ragged
 // batches thus load every SM equally without the host knowing a length, and
-// a launch captured in a graph follows the lengths it finds.  A CTA whose
-// share starts or ends inside a (sequence, head) writes that piece's
-// unnormalised (o, m, l) to the scratch: at most two pieces a CTA, so the
+// a launch captured in a graph follows the lengths it finds.  Each row of
+// units starts with kOverhead empty ones, the price of starting and ending a
+// row in steps, so that a worker with many short sequences gets fewer bytes.
+// A worker whose share starts or ends inside a row writes that piece's
+// unnormalised (o, m, l) to the scratch: at most two pieces a worker, so the
 // scratch does not grow with the lengths.  A second launch joins the pieces of
-// the (sequence, head)s that were cut and fills the rows that see nothing.
+// the rows that were cut and fills the rows that see nothing.
 //
-// One CTA is 4 warps; each warp streams its own 16 positions of every tile
-// through its own cp.async ring (no barrier between warps until a piece
-// ends).  S = Q K^T and O = P V are mma.m16n8k16 with the group's query heads
-// as the 16 rows: the tensor work is a small part of the time the bytes need,
-// so the 128-row tcgen05 tile, which a group of 8 heads would leave 94 %
-// empty, has nothing to give here.
+// A warp streams its positions through a cp.async ring of its own and meets no
+// other warp: the ring runs on into the next row's K and V while a row ends.
+// S = Q K^T and O = P V are mma.m16n8k16 with the group's query heads as the
+// 16 rows: the tensor work is a small part of the time the bytes need, so the
+// 128-row tcgen05 tile, which a group of 8 heads would leave 94 % empty, has
+// nothing to give here.
 //
 // Rounding.  K and V enter the products as they are.  q (fp32) is scaled per
 // row by a power of two and split into 2 terms for an fp16 cache (22 bits) or
 // 3 for a bf16 cache (24 bits); the probabilities, times 2^14 so that small
 // ones keep their bits in fp16, into 2 terms (3 where the output is fp32 and
-// the cache bf16).  Sums, maxima and outputs are fp32, rounded once at the end.
+// the cache bf16).  A step's P V is summed on its own and added in fp32: the
+// tensor cores' accumulation cuts instead of rounding, which over a long row
+// would pull the output towards zero.  Sums, maxima and outputs are fp32,
+// rounded once at the end.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -46,11 +51,15 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreadsP = 32 * kWarps;
-constexpr int kStep = 16;             // positions of one warp step
-constexpr int kTile = kWarps * kStep; // positions of one unit
-constexpr int kRows = 16;             // query heads of one unit (rows of the mma)
+constexpr int kStep = 16;       // positions of one unit
+constexpr int kOverhead = 4;    // units' worth of starting and ending a row
+constexpr int kMinUnits = 6;    // a worker's share, at least (overhead counted)
+constexpr int kRows = 16;       // query heads of one unit (rows of the mma)
+constexpr int kJoinThreads = 256;
+constexpr int kJoinWarps = kJoinThreads / 32;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kPShift = 14.0f;      // probabilities are kept times 2^14
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kPScale = 16384.0f;  // probabilities enter P V times 2^14
 
 struct PagedArgs {
     const void* q;
@@ -58,11 +67,12 @@ struct PagedArgs {
     const int32_t *table, *lens, *req;
     void* out;
     float* lse;
-    float* part;   // [G][2][kRows][hd + 2]
-    int2* desc;    // [batch * nkv * rt]: first and last CTA of each unit row
+    float* part;   // [workers][2][kRows][hd + 2]: o, m (log2 units), l
+    int2* desc;    // [batch * nkv * rt]: first and last worker of each row of units
     const float* slopes;
     int64_t q_stride, out_stride, table_stride, page_stride, pos_stride, head_stride;
-    int batch, nh, nkv, grp, rt, hd, page_size, n_pages, max_pages, n_req, len_add, window, grid;
+    int batch, nh, nkv, grp, rt, hd, page_size, n_pages, max_pages, n_req, len_add, window, workers, sms;
+    int q_pairs;   // q's rows can be read two elements at a time
     float scale, softcap;
 };
 
@@ -83,7 +93,9 @@ __device__ __forceinline__ Seq seq_of(const PagedArgs& a, int b) {
     return s;
 }
 
-__device__ __forceinline__ int tiles_of(const Seq& s) { return s.len == 0 ? 0 : (s.len - 1) / kTile - s.lo / kTile + 1; }
+__device__ __forceinline__ int steps_of(const Seq& s) { return s.len == 0 ? 0 : (s.len - 1) / kStep - s.lo / kStep + 1; }
+// units of one row of sequence s: its steps behind the overhead
+__device__ __forceinline__ int units_of(const Seq& s) { return s.len == 0 ? 0 : steps_of(s) + kOverhead; }
 
 template <int HD>
 __device__ __forceinline__ uint32_t sw(int r, int c) {
@@ -160,15 +172,61 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+__device__ __forceinline__ float2 pair_of(const float* p, bool pairs) {
+    return pairs ? *reinterpret_cast<const float2*>(p) : make_float2(p[0], p[1]);
+}
+__device__ __forceinline__ float2 pair_of(const __half* p, bool pairs) {
+    return pairs ? __half22float2(*reinterpret_cast<const __half2*>(p)) : make_float2(__half2float(p[0]), __half2float(p[1]));
+}
+__device__ __forceinline__ float2 pair_of(const __nv_bfloat16* p, bool pairs) {
+    return pairs ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p))
+                 : make_float2(__bfloat162float(p[0]), __bfloat162float(p[1]));
+}
+
+// A worker's place in its units: step `step` of `ns` of row `hr` of sequence
+// b, `left` units after this row's, of which this row's share ends at `end`.
+struct Cursor {
+    Seq sq;
+    int b, hr, ns, step, end;
+    long long left;  // units of the worker behind this row
+
+    // takes the row's share of `left` units from unit x of the row on
+    __device__ __forceinline__ void enter(int x) {
+        const int row = ns + kOverhead;
+        const long long take = min((long long)(row - x), left);
+        left -= take;
+        step = max(0, x - kOverhead);
+        end = max(0, (int)(x + take) - kOverhead);
+    }
+    __device__ __forceinline__ bool done() const { return step >= end; }
+    // on to the worker's next step; false when there is none
+    __device__ __forceinline__ bool settle(const PagedArgs& a, int rpb) {
+        while (step >= end) {
+            if (left <= 0) return false;
+            if (++hr == rpb) {
+                hr = 0;
+                do {
+                    sq = seq_of(a, ++b);
+                    ns = steps_of(sq);
+                } while (ns == 0);
+            }
+            enter(0);
+        }
+        return true;
+    }
+};
+
 template <int HD, int QT>
 struct Sm {
     static constexpr int kRow = HD * 2;
-    static constexpr int kStages = HD == 64 ? 6 : 3;
-    static constexpr int kStage = 2 * kStep * kRow;              // a warp's K and V rows of one tile
-    static constexpr int kRing = kWarps * kStages * kStage;
-    static constexpr int kQ = kRows * kRow;                      // one term of q
-    static constexpr int kTotal = kRing + QT * kQ + kRows * 4;   // + the rows' 2^-e
-    static_assert(kWarps * kRows * (HD + 2) * 4 <= kRing, "the warps' merge fits over the ring");
+    static constexpr int kStages = HD == 64 ? 6 : HD == 128 ? 3 : 2;
+    static constexpr int kStage = 2 * kStep * kRow;  // a warp's K and V rows of one step
+    static constexpr int kRing = kStages * kStage;   // of one warp
+    // q's fragments stay in registers while O's leave room for them
+    static constexpr bool kQReg = QT * HD / 4 + HD / 2 <= 192;
+    static constexpr int kQ = kQReg ? 0 : QT * kRows * kRow;
+    static constexpr int kWarp = kRing + kQ;
+    static constexpr int kTotal = kWarps * kWarp;
 };
 
 // T: the type of q and out; C: the cache's; QT, PT: terms of q and of the
@@ -176,396 +234,483 @@ struct Sm {
 template <int HD, typename T, typename C, int QT, int PT>
 __global__ void __launch_bounds__(kThreadsP) paged_split_kernel(const __grid_constant__ PagedArgs a) {
     using SM = Sm<HD, QT>;
-    constexpr int KS = HD / 16, NT = HD / 8, ST = SM::kStages;
+    constexpr int KS = HD / 16, NT = HD / 8, ST = SM::kStages, RQ = SM::kQReg ? KS : 1;
     extern __shared__ __align__(1024) uint8_t psm[];
     __shared__ long long wsum[kWarps];
-    __shared__ int sh_b;
-    __shared__ long long sh_base;
-    uint8_t* qs = psm + SM::kRing;
-    float* qscale = reinterpret_cast<float*>(qs + QT * SM::kQ);
+    __shared__ long long chunk[kThreadsP];  // units before the end of each thread's sequences
     pdl_trigger();
     pdl_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gi = lane >> 2, ti = lane & 3;
     const int hd = a.hd, hc = hd / 8, rpb = a.nkv * a.rt;
+    uint8_t* const ring = psm + warp * SM::kWarp;
 
     // columns past hd stay zero: the copies never write them
     if (hd < HD)
-        for (int i = tid; i < SM::kRing / 16; i += kThreadsP) *reinterpret_cast<uint4*>(psm + 16 * i) = make_uint4(0, 0, 0, 0);
+        for (int i = lane; i < SM::kRing / 16; i += 32) *reinterpret_cast<uint4*>(ring + 16 * i) = make_uint4(0, 0, 0, 0);
 
-    // this CTA's units: the tiles of the sequences before each, by a scan
+    // the units before each sequence, by a scan over the lengths
     const int per = (a.batch + kThreadsP - 1) / kThreadsP;
-    const int b0 = min(a.batch, tid * per), b1 = min(a.batch, b0 + per);
-    long long mine = 0;
-    for (int b = b0; b < b1; b++) mine += tiles_of(seq_of(a, b));
-    long long inc = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += x;
-    }
-    if (lane == 31) wsum[warp] = inc;
-    __syncthreads();
-    long long total = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; w++) {
-        if (w == warp) inc += total;
-        total += wsum[w];
-    }
-    const long long W = total * rpb;
-    const long long G = min((long long)a.grid, W);
-    const int cta = blockIdx.x;
-    if (cta >= G) return;
-    long long u = cta * W / G;
-    const long long u1 = (cta + 1) * W / G;
     {
-        long long base = (inc - mine) * rpb;
-        if (u >= base && u < inc * rpb) {
-            for (int b = b0; b < b1; b++) {
-                const long long n = (long long)tiles_of(seq_of(a, b)) * rpb;
-                if (u < base + n) {
-                    sh_b = b;
-                    sh_base = base;
-                    break;
-                }
-                base += n;
-            }
+        const int b0 = min(a.batch, tid * per), b1 = min(a.batch, b0 + per);
+        long long inc = 0;
+        for (int b = b0; b < b1; b++) inc += units_of(seq_of(a, b));
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += x;
         }
+        if (lane == 31) wsum[warp] = inc;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kWarps; w++)
+            if (w < warp) inc += wsum[w];
+        chunk[tid] = inc * rpb;
     }
     __syncthreads();
-    int b = sh_b;
-    Seq sq = seq_of(a, b);
-    int nt = tiles_of(sq);
-    int hr = (int)((u - sh_base) / nt), tile = (int)((u - sh_base) - (long long)hr * nt);
+    const long long W = chunk[kThreadsP - 1];
+    const long long G = max(1LL, min((long long)a.workers, W / kMinUnits));
+    const int worker = warp * gridDim.x + blockIdx.x;  // neighbours on different SMs
+    if (worker >= G || W == 0) return;
+    const long long u0 = worker * W / G, u1 = (worker + 1) * W / G;
+    Cursor ld;
+    {
+        int c = 0;  // the thread whose sequences hold u0
+#pragma unroll
+        for (int j = 0; j < kThreadsP / 32; j++) c += __popc(__ballot_sync(0xffffffffu, chunk[j * 32 + lane] <= u0));
+        long long base = c ? chunk[c - 1] : 0;
+        int b = c * per;
+        while (true) {
+            ld.sq = seq_of(a, b);
+            const long long n = (long long)units_of(ld.sq) * rpb;
+            if (u0 < base + n) break;
+            base += n;
+            b++;
+        }
+        ld.b = b;
+        ld.ns = steps_of(ld.sq);
+        const int row = ld.ns + kOverhead;
+        ld.hr = (int)((u0 - base) / row);
+        ld.left = u1 - u0;
+        ld.enter((int)((u0 - base) - (long long)ld.hr * row));
+    }
+    bool more = ld.settle(a, rpb);  // the loading side has a step
+    if (!more) return;              // (overhead alone)
+    Cursor cu = ld;
 
-    uint8_t* ring = psm + warp * ST * SM::kStage;
-    const uint32_t ring_s = smem_u32(ring), qs_s = smem_u32(qs);
-    const int a_row = (lane & 7) + ((lane >> 3) & 1) * 8, a_kc = (lane >> 4) & 1;
+    const uint32_t ring_s = smem_u32(ring);
     const int bk_row = (lane & 7) + ((lane >> 4) & 1) * 8, bk_kc = (lane >> 3) & 1;
     const int bv_row = (lane & 7) + ((lane >> 3) & 1) * 8, bv_dc = (lane >> 4) & 1;
 
-    while (u < u1) {
-        const int h = hr / a.rt, row0 = (hr - h * a.rt) * kRows;  // KV head, first query head of the group
-        const int rows = min(kRows, a.grp - row0);
-        const int n = (int)min((long long)(nt - tile), u1 - u);
-        const bool from_start = tile == 0, to_end = tile + n == nt;
-        const int head0 = h * a.grp + row0;
-        const int t_first = sq.lo / kTile + tile;  // absolute tile
-        const int32_t* trow = a.table + (int64_t)sq.tr * a.table_stride;
-        bool bad = false;
-
-        // page of this lane's row (lane & 15) of tile i: -1 for a position that is not seen
-        auto fetch = [&](int i) {
-            const int p = (t_first + i) * kTile + warp * kStep + (lane & 15);
-            int id = -1;
-            if (i < n && p >= sq.lo && p < sq.len) {
-                id = __ldg(trow + p / a.page_size);
-                if (id < 0 || id >= a.n_pages) {
-                    bad = true;
-                    id = -1;
-                }
+    // The loading side: fetch looks up the page of this lane's row (lane & 15)
+    // of a step two steps before issue copies the step's rows.
+    struct Place {
+        int64_t off;  // the row's place in its page; -1: a position that is not seen
+        int page;
+        bool live;
+    };
+    auto fetch = [&]() {
+        Place f{-1, -1, more};
+        if (more) {
+            const int p = (ld.sq.lo / kStep + ld.step) * kStep + (lane & 15);
+            if (p >= ld.sq.lo && p < ld.sq.len) {
+                const int pg = p / a.page_size;
+                f.page = __ldg(a.table + (int64_t)ld.sq.tr * a.table_stride + pg);
+                f.off = (int64_t)(p - pg * a.page_size) * a.pos_stride + (int64_t)(ld.hr / a.rt) * a.head_stride;
             }
-            return id;
-        };
-        auto issue = [&](int i, int id) {
-            if (i < n) {
-                const int p = (t_first + i) * kTile + warp * kStep + (lane & 15);
-                const int64_t off = id < 0 ? 0 : id * a.page_stride + (p % a.page_size) * a.pos_stride + h * a.head_stride;
-                const uint32_t kt = ring_s + (i % ST) * SM::kStage, vt = kt + kStep * SM::kRow;
-                constexpr int LR = HD / 8 <= 32 ? 32 / (HD / 8) : 1;  // rows one warp copy covers
-                const int c = lane % (HD / 8), r0 = lane / (HD / 8);
+            ld.step++;
+            more = ld.settle(a, rpb);
+        }
+        return f;
+    };
+    uint32_t bad_slots = 0;
+    auto issue = [&](int slot, const Place& f) {
+        if (f.live) {
+            const bool seen = f.off >= 0;
+            const bool ok = seen && f.page >= 0 && f.page < a.n_pages;
+            const uint32_t bad = __ballot_sync(0xffffffffu, seen && !ok);
+            bad_slots = (bad_slots & ~(1u << slot)) | (bad ? 1u << slot : 0u);
+            const int64_t off = ok ? f.page * a.page_stride + f.off : -1;
+            const uint32_t kt = ring_s + slot * SM::kStage, vt = kt + kStep * SM::kRow;
+            constexpr int LR = 32 / (HD / 8);  // rows one warp copy covers
+            const int c = lane % (HD / 8), r0 = lane / (HD / 8);
 #pragma unroll
-                for (int j = 0; j < kStep / LR; j++) {
-                    const int r = r0 + j * LR;
-                    const int64_t o = __shfl_sync(0xffffffffu, off, r) + c * 8;
-                    const bool ok = __shfl_sync(0xffffffffu, id, r) >= 0;
-                    if (c < hc) {
-                        cp16(kt + sw<HD>(r, c), a.k + o, ok);
-                        cp16(vt + sw<HD>(r, c), a.v + o, ok);
-                    }
+            for (int j = 0; j < kStep / LR; j++) {
+                const int r = r0 + j * LR;
+                const int64_t o = __shfl_sync(0xffffffffu, off, r);
+                if (c < hc) {
+                    const int64_t at = (o < 0 ? 0 : o) + c * 8;
+                    cp16(kt + sw<HD>(r, c), a.k + at, o >= 0);
+                    cp16(vt + sw<HD>(r, c), a.v + at, o >= 0);
                 }
             }
-            cp_async_commit();
-        };
-        int id = fetch(0);
+        }
+        cp_async_commit();
+    };
+    Place f0 = fetch(), f1 = fetch();
 #pragma unroll 1
-        for (int i = 0; i < ST - 1; i++) {
-            const int nx = fetch(i + 1);
-            issue(i, id);
-            id = nx;
-        }
+    for (int i = 0; i < ST - 1; i++) {
+        const Place f2 = fetch();
+        issue(i, f0);
+        f0 = f1;
+        f1 = f2;
+    }
 
-        // q: warp w takes rows w, w + 4, ...
-        for (int r = warp; r < kRows; r += kWarps) {
-            const T* qr = static_cast<const T*>(a.q) + (int64_t)b * a.q_stride + (int64_t)(head0 + r) * hd;
-            float x[HD / 32];
-            float mx = 0.0f;
-#pragma unroll
-            for (int j = 0; j < HD / 64; j++) {
-                const int c = 2 * (lane + 32 * j);
-                x[2 * j] = x[2 * j + 1] = 0.0f;
-                if (r < rows && c < hd) {
-                    x[2 * j] = (float)qr[c];
-                    x[2 * j + 1] = (float)qr[c + 1];
+    int slot = 0;
+    while (true) {
+        // a row begins
+        const int h = cu.hr / a.rt, row0 = (cu.hr - h * a.rt) * kRows;  // KV head, first query head of the group
+        const int rows = min(kRows, a.grp - row0), head0 = h * a.grp + row0;
+        const int first = cu.step, lo = cu.sq.lo, len = cu.sq.len;
+        uint32_t qf[RQ][QT][4];
+        float sc0, sc1;
+        {
+            const T* q0 = static_cast<const T*>(a.q) + (int64_t)cu.b * a.q_stride + (int64_t)(head0 + gi) * hd;
+            const T* q1 = q0 + (int64_t)8 * hd;
+            const bool v0 = gi < rows, v1 = gi + 8 < rows, pairs = a.q_pairs;
+            auto el = [&](const T* p, bool v, int c) { return v && c < hd ? pair_of(p + c, pairs) : make_float2(0.0f, 0.0f); };
+            float up0 = 1.0f, up1 = 1.0f;
+            sc0 = sc1 = a.scale;
+            if (QT > 1) {  // the row's largest element to [2^10, 2^11); a single term is q itself
+                float m0 = 0.0f, m1 = 0.0f;
+#pragma unroll 4
+                for (int c = 2 * ti; c < HD; c += 8) {
+                    const float2 x = el(q0, v0, c), y = el(q1, v1, c);
+                    m0 = fmaxf(m0, fmaxf(fabsf(x.x), fabsf(x.y)));
+                    m1 = fmaxf(m1, fmaxf(fabsf(y.x), fabsf(y.y)));
                 }
-                mx = fmaxf(mx, fmaxf(fabsf(x[2 * j]), fabsf(x[2 * j + 1])));
-            }
-            float back = 1.0f;
-            if (QT > 1) {  // the largest element to [2^10, 2^11); one term is q itself
-                mx = warp_max(mx);
-                const int e = mx > 0.0f && mx < 3.0e38f ? min(100, max(-100, 10 - ilogbf(mx))) : 0;
-                const float f = __int_as_float((127 + e) << 23);
-                back = __int_as_float((127 - e) << 23);
 #pragma unroll
-                for (int j = 0; j < HD / 32; j++) x[j] *= f;
+                for (int o = 1; o < 4; o <<= 1) {
+                    m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
+                    m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
+                }
+                auto ex = [](float m) { return m > 0.0f && m < 3.0e38f ? min(100, max(-100, 10 - ilogbf(m))) : 0; };
+                const int e0 = ex(m0), e1 = ex(m1);
+                up0 = __int_as_float((127 + e0) << 23);
+                up1 = __int_as_float((127 + e1) << 23);
+                sc0 *= __int_as_float((127 - e0) << 23);
+                sc1 *= __int_as_float((127 - e1) << 23);
             }
+            auto frag = [&](int kk, uint32_t (*t)[4]) {
+                const int c = 16 * kk + 2 * ti;
+                const float2 x[4] = {el(q0, v0, c), el(q1, v1, c), el(q0, v0, c + 8), el(q1, v1, c + 8)};
 #pragma unroll
-            for (int j = 0; j < HD / 64; j++) {
-                const int c = 2 * (lane + 32 * j);
-                uint32_t t[QT];
-                split_terms<C, QT>(x[2 * j], x[2 * j + 1], t);
-                const uint32_t off = sw<HD>(r, c / 8) + (c % 8) * 2;
+                for (int j = 0; j < 4; j++) {
+                    uint32_t w[QT];
+                    const float f = (j & 1) ? up1 : up0;
+                    split_terms<C, QT>(x[j].x * f, x[j].y * f, w);
 #pragma unroll
-                for (int i = 0; i < QT; i++) *reinterpret_cast<uint32_t*>(qs + i * SM::kQ + off) = t[i];
+                    for (int i = 0; i < QT; i++) t[i][j] = w[i];
+                }
+            };
+            if constexpr (SM::kQReg) {
+#pragma unroll
+                for (int kk = 0; kk < KS; kk++) frag(kk, qf[kk]);
+            } else {  // [kk][term][lane] fragments of 16 bytes
+                __syncwarp();
+                uint4* qs = reinterpret_cast<uint4*>(ring + SM::kRing);
+#pragma unroll 2
+                for (int kk = 0; kk < KS; kk++) {
+                    uint32_t t[QT][4];
+                    frag(kk, t);
+#pragma unroll
+                    for (int i = 0; i < QT; i++) qs[(kk * QT + i) * 32 + lane] = make_uint4(t[i][0], t[i][1], t[i][2], t[i][3]);
+                }
+                __syncwarp();
             }
-            if (lane == 0) qscale[r] = back * a.scale;
         }
-        __syncthreads();
-        const float sc0 = qscale[gi], sc1 = qscale[gi + 8];
+        // scores in log2 units
+        const float cap = a.softcap;
+        const float k0 = cap > 0.0f ? sc0 / cap : sc0 * kLog2e, k1 = cap > 0.0f ? sc1 / cap : sc1 * kLog2e;
         float sl0 = 0.0f, sl1 = 0.0f;
         if (a.slopes) {
-            if (gi < rows) sl0 = __ldg(a.slopes + head0 + gi);
-            if (gi + 8 < rows) sl1 = __ldg(a.slopes + head0 + gi + 8);
+            if (gi < rows) sl0 = __ldg(a.slopes + head0 + gi) * kLog2e;
+            if (gi + 8 < rows) sl1 = __ldg(a.slopes + head0 + gi + 8) * kLog2e;
         }
 
         float o[NT][4];
 #pragma unroll
         for (int i = 0; i < NT; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
         float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;  // rows gi, gi + 8
+        bool bad = false;
 
 #pragma unroll 1
-        for (int i = 0; i < n; i++) {
-            const int nx = fetch(i + ST);
-            issue(i + ST - 1, id);
-            id = nx;
+        for (; cu.step < cu.end; cu.step++) {
+            const Place f2 = fetch();
+            issue(slot == 0 ? ST - 1 : slot - 1, f0);
+            f0 = f1;
+            f1 = f2;
             cp_wait<ST - 1>();
             __syncwarp();
-            const uint32_t kt = ring_s + (i % ST) * SM::kStage, vt = kt + kStep * SM::kRow;
-            const int p0 = (t_first + i) * kTile + warp * kStep;
-            if (p0 < sq.len && p0 + kStep > sq.lo) {
-                // one accumulator pair per term of q: short chains, and the terms below the
-                // first stay out of a score that an infinite key made infinite (0 * inf)
-                float s0[QT][4], s1[QT][4];
+            const uint32_t kt = ring_s + slot * SM::kStage, vt = kt + kStep * SM::kRow;
+            bad |= (bad_slots >> slot) & 1;
+            slot = slot == ST - 1 ? 0 : slot + 1;
+            const int p0 = (lo / kStep + cu.step) * kStep;
+            // one accumulator pair per term of q: short chains, and the terms below the
+            // first stay out of a score that an infinite key made infinite (0 * inf)
+            float s0[QT][4], s1[QT][4];
 #pragma unroll
-                for (int t = 0; t < QT; t++)
+            for (int t = 0; t < QT; t++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) s0[t][j] = s1[t][j] = 0.0f;
+                for (int j = 0; j < 4; j++) s0[t][j] = s1[t][j] = 0.0f;
 #pragma unroll
-                for (int kk = 0; kk < KS; kk++) {
-                    uint32_t bk[4];
-                    ldsm(kt + sw<HD>(bk_row, 2 * kk + bk_kc), bk);
+            for (int kk = 0; kk < KS; kk++) {
+                uint32_t bk[4];
+                ldsm(kt + sw<HD>(bk_row, 2 * kk + bk_kc), bk);
 #pragma unroll
-                    for (int t = 0; t < QT; t++) {
-                        uint32_t aq[4];
-                        ldsm(qs_s + t * SM::kQ + sw<HD>(a_row, 2 * kk + a_kc), aq);
+                for (int t = 0; t < QT; t++) {
+                    if constexpr (SM::kQReg) {
+                        Cvt<C>::mma(s0[t], qf[kk][t], bk[0], bk[1]);
+                        Cvt<C>::mma(s1[t], qf[kk][t], bk[2], bk[3]);
+                    } else {
+                        const uint4 w = reinterpret_cast<const uint4*>(ring + SM::kRing)[(kk * QT + t) * 32 + lane];
+                        const uint32_t aq[4] = {w.x, w.y, w.z, w.w};
                         Cvt<C>::mma(s0[t], aq, bk[0], bk[1]);
                         Cvt<C>::mma(s1[t], aq, bk[2], bk[3]);
                     }
                 }
-                // rows gi (values 0, 1) and gi + 8 (2, 3); positions p0 + 2 ti + {0, 1} (s0), + 8 (s1)
-                float s[8];
+            }
+            // rows gi (values 0, 1) and gi + 8 (2, 3); positions p0 + 2 ti + {0, 1} (s0), + 8 (s1)
+            float s[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float top = j < 4 ? s0[0][j] : s1[0][j - 4];
+                float low = 0.0f;
+#pragma unroll
+                for (int t = QT - 1; t > 0; t--) low += j < 4 ? s0[t][j] : s1[t][j - 4];
+                s[j] = (QT > 1 && fabsf(top) == INFINITY ? top : top + low) * ((j & 2) ? k1 : k0);
+            }
+            if (cap > 0.0f) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) s[j] = (cap * kLog2e) * tanhf(s[j]);
+            }
+            const int pj = p0 + 2 * ti;
+            if (a.slopes) {
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    s[j] = fmaf((j & 2) ? sl1 : sl0, (float)(pj + (j & 1) + (j & 4) * 2 - (len - 1)), s[j]);
+            }
+            if (p0 < lo || p0 + kStep > len) {
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    const float top = j < 4 ? s0[0][j] : s1[0][j - 4];
-                    float low = 0.0f;
-#pragma unroll
-                    for (int t = QT - 1; t > 0; t--) low += j < 4 ? s0[t][j] : s1[t][j - 4];
-                    s[j] = (QT > 1 && fabsf(top) == INFINITY ? top : top + low) * ((j & 2) ? sc1 : sc0);
+                    const int p = pj + (j & 1) + (j & 4) * 2;
+                    if (p < lo || p >= len) s[j] = -INFINITY;
                 }
-                if (a.softcap > 0.0f) {
+            }
+            float r0 = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[4], s[5])), r1 = fmaxf(fmaxf(s[2], s[3]), fmaxf(s[6], s[7]));
+            r0 = fmaxf(r0, __shfl_xor_sync(0xffffffffu, r0, 1));
+            r1 = fmaxf(r1, __shfl_xor_sync(0xffffffffu, r1, 1));
+            r0 = fmaxf(r0, __shfl_xor_sync(0xffffffffu, r0, 2));
+            r1 = fmaxf(r1, __shfl_xor_sync(0xffffffffu, r1, 2));
+            const float n0 = fmaxf(m0, r0), n1 = fmaxf(m1, r1);
+            // (a row whose scores are all -inf so far keeps weight zero)
+            const float z0 = n0 == -INFINITY ? 0.0f : n0, z1 = n1 == -INFINITY ? 0.0f : n1;
+            const float g0 = ex2(m0 - z0), g1 = ex2(m1 - z1);
+            m0 = n0;
+            m1 = n1;
+            float p[8];
 #pragma unroll
-                    for (int j = 0; j < 8; j++) s[j] = a.softcap * tanhf(s[j] / a.softcap);
-                }
-                const int pj = p0 + 2 * ti;
-                if (a.slopes) {
+            for (int j = 0; j < 8; j++) p[j] = ex2(s[j] - ((j & 2) ? z1 : z0)) * kPScale;
+            l0 = fmaf(l0, g0, (p[0] + p[1]) + (p[4] + p[5]));
+            l1 = fmaf(l1, g1, (p[2] + p[3]) + (p[6] + p[7]));
+            uint32_t pa[PT][4];
 #pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        s[j] = fmaf((j & 2) ? sl1 : sl0, (float)(pj + (j & 1) + (j & 4) * 2 - (sq.len - 1)), s[j]);
-                }
-                if (p0 < sq.lo || p0 + kStep > sq.len) {
+            for (int j = 0; j < 4; j++) {
+                uint32_t t[PT];
+                split_terms<C, PT>(p[2 * j], p[2 * j + 1], t);
 #pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const int p = pj + (j & 1) + (j & 4) * 2;
-                        if (p < sq.lo || p >= sq.len) s[j] = -INFINITY;
-                    }
-                }
-                float r0 = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[4], s[5])), r1 = fmaxf(fmaxf(s[2], s[3]), fmaxf(s[6], s[7]));
-                r0 = fmaxf(r0, __shfl_xor_sync(0xffffffffu, r0, 1));
-                r1 = fmaxf(r1, __shfl_xor_sync(0xffffffffu, r1, 1));
-                r0 = fmaxf(r0, __shfl_xor_sync(0xffffffffu, r0, 2));
-                r1 = fmaxf(r1, __shfl_xor_sync(0xffffffffu, r1, 2));
-                const float n0 = fmaxf(m0, r0), n1 = fmaxf(m1, r1);
-                // (a row whose scores are all -inf so far keeps weight zero)
-                const float z0 = n0 == -INFINITY ? 0.0f : n0, z1 = n1 == -INFINITY ? 0.0f : n1;
-                const float f0 = ex2((m0 - z0) * kLog2e), f1 = ex2((m1 - z1) * kLog2e);
-                m0 = n0;
-                m1 = n1;
-                float p[8];
+                for (int x = 0; x < PT; x++) pa[x][j] = t[x];
+            }
 #pragma unroll
-                for (int j = 0; j < 8; j++) p[j] = ex2(fmaf(s[j] - ((j & 2) ? z1 : z0), kLog2e, kPShift));
-                l0 = fmaf(l0, f0, (p[0] + p[1]) + (p[4] + p[5]));
-                l1 = fmaf(l1, f1, (p[2] + p[3]) + (p[6] + p[7]));
+            for (int j = 0; j < NT / 2; j++) {
+                uint32_t bv[4];
+                ldsm_t(vt + sw<HD>(bv_row, 2 * j + bv_dc), bv);
+                float t0[4] = {0.0f, 0.0f, 0.0f, 0.0f}, t1[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int j = 0; j < NT; j++) {
-                    o[j][0] *= f0;
-                    o[j][1] *= f0;
-                    o[j][2] *= f1;
-                    o[j][3] *= f1;
-                }
-                uint32_t pa[PT][4];
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    uint32_t t[PT];
-                    split_terms<C, PT>(p[2 * j], p[2 * j + 1], t);
-#pragma unroll
-                    for (int x = 0; x < PT; x++) pa[x][j] = t[x];
+                for (int x = PT - 1; x >= 0; x--) {
+                    Cvt<C>::mma(t0, pa[x], bv[0], bv[1]);
+                    Cvt<C>::mma(t1, pa[x], bv[2], bv[3]);
                 }
 #pragma unroll
-                for (int j = 0; j < NT / 2; j++) {
-                    uint32_t bv[4];
-                    ldsm_t(vt + sw<HD>(bv_row, 2 * j + bv_dc), bv);
-#pragma unroll
-                    for (int x = 0; x < PT; x++) {
-                        Cvt<C>::mma(o[2 * j], pa[x], bv[0], bv[1]);
-                        Cvt<C>::mma(o[2 * j + 1], pa[x], bv[2], bv[3]);
-                    }
+                for (int i = 0; i < 4; i++) {
+                    o[2 * j][i] = fmaf(o[2 * j][i], (i & 2) ? g1 : g0, t0[i]);
+                    o[2 * j + 1][i] = fmaf(o[2 * j + 1][i], (i & 2) ? g1 : g0, t1[i]);
                 }
             }
             __syncwarp();  // the slot is refilled by the next step's issue
         }
-        cp_wait<0>();
         l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
         l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
         l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
         l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-        if (__any_sync(0xffffffffu, bad)) m0 = m1 = l0 = l1 = __int_as_float(0x7fc00000);  // a page that is not there
-
-        // the warps' pieces meet over the ring: [warp][16][HD + 2]
-        __syncthreads();
-        float* mw = reinterpret_cast<float*>(psm);
-        float* wr = mw + warp * kRows * (HD + 2);
+        if (bad) m0 = m1 = l0 = l1 = __int_as_float(0x7fc00000);  // a page that is not there
+        const bool from_start = first == 0, to_end = cu.end == cu.ns;
+        if (from_start && to_end) {
+            const float i0 = l0 == 0.0f ? 0.0f : 1.0f / l0, i1 = l1 == 0.0f ? 0.0f : 1.0f / l1;
+            T* out = static_cast<T*>(a.out) + (int64_t)cu.b * a.out_stride + (int64_t)(head0 + gi) * hd;
 #pragma unroll
-        for (int j = 0; j < NT; j++) {
-            const int d = j * 8 + 2 * ti;
-            wr[gi * (HD + 2) + d] = o[j][0];
-            wr[gi * (HD + 2) + d + 1] = o[j][1];
-            wr[(gi + 8) * (HD + 2) + d] = o[j][2];
-            wr[(gi + 8) * (HD + 2) + d + 1] = o[j][3];
-        }
-        if (ti == 0) {
-            wr[gi * (HD + 2) + HD] = m0;
-            wr[gi * (HD + 2) + HD + 1] = l0;
-            wr[(gi + 8) * (HD + 2) + HD] = m1;
-            wr[(gi + 8) * (HD + 2) + HD + 1] = l1;
-        }
-        __syncthreads();
-        const bool whole = from_start && to_end;
-        float* part = a.part + (int64_t)(2 * cta + (from_start ? 1 : 0)) * kRows * (hd + 2);
-        for (int i = tid; i < rows * (hd + 1); i += kThreadsP) {
-            const int r = i / (hd + 1), d = i - r * (hd + 1);  // d == hd: the row's m and l
-            float M = -INFINITY;
-            bool nan = false;
+            for (int j = 0; j < NT; j++) {
+                const int d = j * 8 + 2 * ti;
+                if (d < hd) {
+                    if (gi < rows) {
+                        out[d] = (T)(o[j][0] * i0);
+                        out[d + 1] = (T)(o[j][1] * i0);
+                    }
+                    if (gi + 8 < rows) {
+                        out[(int64_t)8 * hd + d] = (T)(o[j][2] * i1);
+                        out[(int64_t)8 * hd + d + 1] = (T)(o[j][3] * i1);
+                    }
+                }
+            }
+            if (a.lse && ti == 0) {
+                float* lse = a.lse + (int64_t)cu.b * a.nh + head0 + gi;
+                if (gi < rows) lse[0] = l0 == 0.0f ? -INFINITY : (m0 + (log2f(l0) - 14.0f)) * kLn2;
+                if (gi + 8 < rows) lse[8] = l1 == 0.0f ? -INFINITY : (m1 + (log2f(l1) - 14.0f)) * kLn2;
+            }
+        } else {
+            float* part = a.part + ((int64_t)(2 * worker + (from_start ? 1 : 0)) * kRows + gi) * (hd + 2);
 #pragma unroll
-            for (int w = 0; w < kWarps; w++) {
-                const float m = mw[(w * kRows + r) * (HD + 2) + HD];
-                nan |= m != m;
-                M = fmaxf(M, m);
+            for (int j = 0; j < NT; j++) {
+                const int d = j * 8 + 2 * ti;
+                if (d < hd) {
+                    if (gi < rows) *reinterpret_cast<float2*>(part + d) = make_float2(o[j][0], o[j][1]);
+                    if (gi + 8 < rows) *reinterpret_cast<float2*>(part + 8 * (hd + 2) + d) = make_float2(o[j][2], o[j][3]);
+                }
             }
-            float val = 0.0f, L = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kWarps; w++) {
-                const float* pw = mw + (w * kRows + r) * (HD + 2);
-                const float f = pw[HD] == -INFINITY ? 0.0f : ex2((pw[HD] - M) * kLog2e);
-                if (d < hd) val = fmaf(pw[d], f, val);
-                L = fmaf(pw[HD + 1], f, L);
-            }
-            if (nan) M = L = val = __int_as_float(0x7fc00000);
-            if (!whole) {
-                part[r * (hd + 2) + d] = d < hd ? val : M;
-                if (d == hd) part[r * (hd + 2) + hd + 1] = L;
-            } else if (d < hd) {
-                static_cast<T*>(a.out)[(int64_t)b * a.out_stride + (int64_t)(head0 + r) * hd + d] =
-                    (T)(L == 0.0f ? 0.0f : val / L);
-            } else if (a.lse) {
-                a.lse[(int64_t)b * a.nh + head0 + r] = L == 0.0f ? -INFINITY : M + (log2f(L) - kPShift) * 0.6931471805599453f;
+            if (ti == 0) {
+                if (gi < rows) *reinterpret_cast<float2*>(part + hd) = make_float2(m0, l0);
+                if (gi + 8 < rows) *reinterpret_cast<float2*>(part + 8 * (hd + 2) + hd) = make_float2(m1, l1);
             }
         }
-        if (to_end && tid == 0) {
-            const long long first = u - tile;  // the unit row's first unit, and the CTA that holds it
-            a.desc[(int64_t)b * rpb + hr] = make_int2((int)(((first + 1) * G - 1) / W), cta);
-        }
-        __syncthreads();
-        if (hd < HD && u + n < u1) {  // the merge wrote over the ring's zero columns
-            for (int i = tid; i < SM::kRing / 16; i += kThreadsP)
-                *reinterpret_cast<uint4*>(psm + 16 * i) = make_uint4(0, 0, 0, 0);
-            __syncthreads();
-        }
-
-        u += n;
-        tile = 0;
-        if (to_end && ++hr == rpb) {
-            hr = 0;
-            while (u < u1) {
-                sq = seq_of(a, ++b);
-                nt = tiles_of(sq);
-                if (nt) break;
+        if (to_end && lane == 0) {
+            // the worker that holds the row's first step: floor(((u + 1) G - 1) / W) of its unit u
+            int c0 = worker;
+            if (!from_start) {
+                const long long u = u1 - cu.left - (cu.ns + kOverhead) + kOverhead;
+                c0 = (int)(((u + 1) * G - 1) / W);
             }
+            a.desc[(int64_t)cu.b * rpb + cu.hr] = make_int2(c0, worker);
         }
+        if (!cu.settle(a, rpb)) break;
     }
+    cp_wait<0>();
 }
 
-// One CTA per (sequence, query head): joins the pieces of a row that was cut,
-// and fills a row that sees nothing (zeros, lse -inf) or whose length passes
-// its table (NaN).
+// One CTA per row of units, or per query head of it (blockIdx.y): joins the
+// pieces of a row that was cut, and fills a row that sees nothing (zeros, lse
+// -inf) or whose length passes its table (NaN).  The 8 warps are 8 / pw heads
+// times pw shares of the pieces.
 template <typename T>
-__global__ void __launch_bounds__(kThreadsP) paged_join_kernel(const __grid_constant__ PagedArgs a) {
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedArgs a, int pw) {
+    __shared__ float red[kJoinWarps][kPagedMaxHd + 2];
     pdl_trigger();
     pdl_wait();
-    const int b = blockIdx.x / a.nh, head = blockIdx.x - b * a.nh, hd = a.hd;
+    const int rpb = a.nkv * a.rt, b = blockIdx.x / rpb, hr = blockIdx.x - b * rpb, hd = a.hd;
+    const int h = hr / a.rt, row0 = (hr - h * a.rt) * kRows, rows = min(kRows, a.grp - row0), head0 = h * a.grp + row0;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rw = kJoinWarps / pw, share = warp % pw;
+    const float nan = __int_as_float(0x7fc00000);
     const Seq sq = seq_of(a, b);
-    T* out = static_cast<T*>(a.out) + (int64_t)b * a.out_stride + (int64_t)head * hd;
-    float* lse = a.lse ? a.lse + (int64_t)b * a.nh + head : nullptr;
-    if (sq.len == 0) {
-        const float nan = __int_as_float(0x7fc00000);
-        for (int d = threadIdx.x; d < hd; d += kThreadsP) out[d] = (T)(sq.bad ? nan : 0.0f);
-        if (lse && threadIdx.x == 0) *lse = sq.bad ? nan : -INFINITY;
-        return;
+    int2 c = make_int2(0, 0);
+    if (sq.len) {
+        c = a.desc[blockIdx.x];
+        if (c.x == c.y) return;
     }
-    const int h = head / a.grp, rg = head - h * a.grp, hr = h * a.rt + rg / kRows;
-    const int2 c = a.desc[(int64_t)b * a.nkv * a.rt + hr];
-    if (c.x == c.y) return;
-    const float* row = a.part + (int64_t)(rg % kRows) * (hd + 2);
-    const int64_t ps = (int64_t)kRows * (hd + 2);
-    auto piece = [&](int i) { return row + (2 * (int64_t)i + (i == c.x ? 1 : 0)) * ps; };
-    float M = -INFINITY;
-    bool nan = false;
-    for (int i = c.x; i <= c.y; i++) {
-        const float m = piece(i)[hd];
-        nan |= m != m;
-        M = fmaxf(M, m);
+    for (int rb = blockIdx.y * rw; rb < rows; rb += gridDim.y * rw) {
+        const int r = rb + warp / pw;
+        const bool live = r < rows;
+        float o[kPagedMaxHd / 32], M = -INFINITY, L = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kPagedMaxHd / 32; j++) o[j] = 0.0f;
+        bool bad = false;
+        if (live && sq.len) {
+            const float* base = a.part + (int64_t)r * (hd + 2);
+            const int64_t ps = (int64_t)kRows * (hd + 2);
+            auto piece = [&](int i) { return base + (2 * (int64_t)i + (i == c.x ? 1 : 0)) * ps; };
+            for (int i0 = c.x + share; i0 <= c.y; i0 += 32 * pw) {
+                const int i = i0 + lane * pw;
+                const float m = i <= c.y ? piece(i)[hd] : -INFINITY;
+                bad |= m != m;
+                M = fmaxf(M, m);
+            }
+            M = warp_max(M);
+            bad = __any_sync(0xffffffffu, bad);
+#pragma unroll 4
+            for (int i = c.x + share; i <= c.y; i += pw) {
+                const float* p = piece(i);
+                const float2 ml = *reinterpret_cast<const float2*>(p + hd);
+                const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - M);
+                L = fmaf(ml.y, f, L);
+#pragma unroll
+                for (int j = 0; j < kPagedMaxHd / 64; j++) {
+                    const int d = 2 * lane + 64 * j;
+                    if (d < hd) {
+                        const float2 x = *reinterpret_cast<const float2*>(p + d);
+                        o[2 * j] = fmaf(x.x, f, o[2 * j]);
+                        o[2 * j + 1] = fmaf(x.y, f, o[2 * j + 1]);
+                    }
+                }
+            }
+            if (bad) M = L = nan;
+        }
+        if (pw > 1) {  // the shares of a head meet in its first warp
+#pragma unroll
+            for (int j = 0; j < kPagedMaxHd / 64; j++) {
+                const int d = 2 * lane + 64 * j;
+                if (d < hd) {
+                    red[warp][d] = o[2 * j];
+                    red[warp][d + 1] = o[2 * j + 1];
+                }
+            }
+            if (lane == 0) {
+                red[warp][kPagedMaxHd] = M;
+                red[warp][kPagedMaxHd + 1] = L;
+            }
+            __syncthreads();
+            if (share == 0) {
+                float N = M;
+                bool any = M != M;
+                for (int w = 1; w < pw; w++) {
+                    const float m = red[warp + w][kPagedMaxHd];
+                    any |= m != m;
+                    N = fmaxf(N, m);
+                }
+                float f = M == -INFINITY ? 0.0f : ex2(M - N);
+                L *= f;
+#pragma unroll
+                for (int j = 0; j < kPagedMaxHd / 32; j++) o[j] *= f;
+                for (int w = 1; w < pw; w++) {
+                    const float m = red[warp + w][kPagedMaxHd];
+                    f = m == -INFINITY ? 0.0f : ex2(m - N);
+                    L = fmaf(red[warp + w][kPagedMaxHd + 1], f, L);
+#pragma unroll
+                    for (int j = 0; j < kPagedMaxHd / 64; j++) {
+                        const int d = 2 * lane + 64 * j;
+                        if (d < hd) {
+                            o[2 * j] = fmaf(red[warp + w][d], f, o[2 * j]);
+                            o[2 * j + 1] = fmaf(red[warp + w][d + 1], f, o[2 * j + 1]);
+                        }
+                    }
+                }
+                M = any ? nan : N;
+                if (any) L = nan;
+            }
+            __syncthreads();
+        }
+        if (live && share == 0) {
+            if (sq.bad) M = L = nan;
+            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+            T* out = static_cast<T*>(a.out) + (int64_t)b * a.out_stride + (int64_t)(head0 + r) * hd;
+#pragma unroll
+            for (int j = 0; j < kPagedMaxHd / 64; j++) {
+                const int d = 2 * lane + 64 * j;
+                if (d < hd) {
+                    out[d] = (T)(o[2 * j] * inv);
+                    out[d + 1] = (T)(o[2 * j + 1] * inv);
+                }
+            }
+            if (a.lse && lane == 0)
+                a.lse[(int64_t)b * a.nh + head0 + r] = L == 0.0f ? -INFINITY : (M + (log2f(L) - 14.0f)) * kLn2;
+        }
     }
-    float L = 0.0f, o0 = 0.0f, o1 = 0.0f;
-    const int d0 = threadIdx.x, d1 = threadIdx.x + kThreadsP;
-    for (int i = c.x; i <= c.y; i++) {
-        const float* p = piece(i);
-        const float f = p[hd] == -INFINITY ? 0.0f : ex2((p[hd] - M) * kLog2e);
-        L = fmaf(p[hd + 1], f, L);
-        if (d0 < hd) o0 = fmaf(p[d0], f, o0);
-        if (d1 < hd) o1 = fmaf(p[d1], f, o1);
-    }
-    if (nan) M = L = o0 = o1 = __int_as_float(0x7fc00000);
-    if (d0 < hd) out[d0] = (T)(L == 0.0f ? 0.0f : o0 / L);
-    if (d1 < hd) out[d1] = (T)(L == 0.0f ? 0.0f : o1 / L);
-    if (lse && threadIdx.x == 0) *lse = L == 0.0f ? -INFINITY : M + (log2f(L) - kPShift) * 0.6931471805599453f;
 }
 
 constexpr int kMaxPagedDevices = 64;
@@ -583,9 +728,14 @@ cudaError_t go(const PagedArgs& a, cudaStream_t s) {
         if (e != cudaSuccess) return e;
         if (dev < kMaxPagedDevices) attr[dev] = true;
     }
-    e = launch_pdl(kern, dim3(a.grid), dim3(kThreadsP), smem, s, a);
+    e = launch_pdl(kern, dim3(a.workers / kWarps), dim3(kThreadsP), smem, s, a);
     if (e != cudaSuccess) return e;
-    return launch_pdl(paged_join_kernel<T>, dim3(a.batch * a.nh), dim3(kThreadsP), 0, s, a);
+    // few rows: a CTA per query head, its pieces over the 8 warps; many: a warp per head
+    const int rows = a.batch * a.nkv * a.rt;
+    const int heads = std::min(a.grp, kRows);
+    return rows * heads <= 2 * a.sms
+               ? launch_pdl(paged_join_kernel<T>, dim3(rows, heads), dim3(kJoinThreads), 0, s, a, kJoinWarps)
+               : launch_pdl(paged_join_kernel<T>, dim3(rows, 1), dim3(kJoinThreads), 0, s, a, 1);
 }
 
 template <int HD>
@@ -595,11 +745,11 @@ cudaError_t go_hd(const PagedArgs& a, int dtype, int cache, cudaStream_t s) {
     return cache == 1 ? go<HD, __half, __half, 1, 2>(a, s) : go<HD, __nv_bfloat16, __nv_bfloat16, 1, 2>(a, s);
 }
 
-// CTAs that fit the machine at once: two an SM, one for head dimensions past
-// 128 (their rings take most of the shared memory)
-int paged_grid(int hd, int sms) { return hd > 128 ? sms : 2 * sms; }
+// Warps that fit the machine at once: two CTAs an SM, one for head dimensions
+// past 128 (their rings take most of the shared memory).
+int paged_workers(int hd, int sms) { return (hd > 128 ? 1 : 2) * kWarps * sms; }
 
-size_t part_bytes(int hd, int sms) { return (size_t)paged_grid(hd, sms) * 2 * kRows * (hd + 2) * sizeof(float); }
+size_t part_bytes(int hd, int sms) { return (size_t)paged_workers(hd, sms) * 2 * kRows * (hd + 2) * sizeof(float); }
 
 }  // namespace
 
@@ -644,7 +794,10 @@ int launch_attention_paged(const b2_paged_kv& kv, const b2_paged_attn_opts& o, c
     a.n_req = o.n_req;
     a.len_add = o.len_add;
     a.window = o.window;
-    a.grid = paged_grid(kv.hd, sms);
+    a.workers = paged_workers(kv.hd, sms);
+    a.sms = sms;
+    const int es = o.dtype == 0 ? 4 : 2;
+    a.q_pairs = a.q_stride % 2 == 0 && !(reinterpret_cast<uintptr_t>(q) & (2 * es - 1));
     a.scale = o.scale > 0.0f ? o.scale : (float)(1.0 / sqrt((double)kv.hd));
     a.softcap = o.softcap;
     const cudaError_t e = kv.hd <= 64    ? go_hd<64>(a, o.dtype, kv.dtype, s)
