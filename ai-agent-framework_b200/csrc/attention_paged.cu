@@ -10,7 +10,7 @@
 // it, whatever the number of query heads that share it.
 //
 // Split.  The work of the whole batch is one line of units, a unit being one
-// step of kStep positions of one (sequence, KV head, block of 16 query heads),
+// step of kStep positions of one (sequence, KV head, block of query heads),
 // and worker w of G, a warp, takes the units [w W / G, (w + 1) W / G).  Ragged
 // batches thus load every SM equally without the host knowing a length, and
 // a launch captured in a graph follows the lengths it finds.  Each row of
@@ -23,10 +23,12 @@
 //
 // A warp streams its positions through a cp.async ring of its own and meets no
 // other warp: the ring runs on into the next row's K and V while a row ends.
-// S = Q K^T and O = P V are mma.m16n8k16 with the group's query heads as the
-// 16 rows: the tensor work is a small part of the time the bytes need, so the
-// 128-row tcgen05 tile, which a group of 8 heads would leave 94 % empty, has
-// nothing to give here.
+// The products are S^T = K Q^T and O^T = V^T P^T on mma.m16n8k16: 16 positions
+// (or dimensions) by 8 query heads, so a group of up to 8 heads fills the tile
+// (16 heads: two of them on the same K and V fragments), and P^T is S^T's
+// accumulator transposed by movmatrix.  With the heads as the 16 rows instead,
+// half of every product, exponential and rescaling of a group of 8 would be of
+// rows that do not exist; the 128-row tcgen05 tile would be 94 % empty.
 //
 // Rounding.  K and V enter the products as they are.  q (fp32) is scaled per
 // row by a power of two and split into 2 terms for an fp16 cache (22 bits) or
@@ -54,7 +56,6 @@ constexpr int kThreadsP = 32 * kWarps;
 constexpr int kStep = 16;       // positions of one unit
 constexpr int kOverhead = 4;    // units' worth of starting and ending a row
 constexpr int kMinUnits = 6;    // a worker's share, at least (overhead counted)
-constexpr int kRows = 16;       // query heads of one unit (rows of the mma)
 constexpr int kJoinThreads = 256;
 constexpr int kJoinWarps = kJoinThreads / 32;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -67,14 +68,16 @@ struct PagedArgs {
     const int32_t *table, *lens, *req;
     void* out;
     float* lse;
-    float* part;   // [workers][2][kRows][hd + 2]: o, m (log2 units), l
+    float* part;   // [workers][2][heads][hd + 2]: o, m (log2 units), l
     int2* desc;    // [batch * nkv * rt]: first and last worker of each row of units
     const float* slopes;
     int64_t q_stride, out_stride, table_stride, page_stride, pos_stride, head_stride;
-    int batch, nh, nkv, grp, rt, hd, page_size, n_pages, max_pages, n_req, len_add, window, workers, sms;
+    int batch, nh, nkv, grp, heads, rt, hd, page_size, page_shift, n_pages, max_pages, n_req, len_add, window, workers, sms;
     int q_pairs;   // q's rows can be read two elements at a time
     float scale, softcap;
 };
+// heads: query heads of one unit (8 or 16); rt: blocks of that many in a group.
+// page_shift: log2 of the page size, or -1.
 
 // A row's sequence: table row, visible positions [lo, len).  len 0: nothing.
 struct Seq {
@@ -216,25 +219,27 @@ struct Cursor {
     }
 };
 
-template <int HD, int QT>
+template <int HD>
 struct Sm {
     static constexpr int kRow = HD * 2;
-    static constexpr int kStages = HD == 64 ? 6 : HD == 128 ? 3 : 2;
+    static constexpr int kStages = HD == 64 ? 6 : 3;
     static constexpr int kStage = 2 * kStep * kRow;  // a warp's K and V rows of one step
-    static constexpr int kRing = kStages * kStage;   // of one warp
-    // q's fragments stay in registers while O's leave room for them
-    static constexpr bool kQReg = QT * HD / 4 + HD / 2 <= 192;
-    static constexpr int kQ = kQReg ? 0 : QT * kRows * kRow;
-    static constexpr int kWarp = kRing + kQ;
+    static constexpr int kWarp = kStages * kStage;
     static constexpr int kTotal = kWarps * kWarp;
 };
 
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
 // T: the type of q and out; C: the cache's; QT, PT: terms of q and of the
-// probabilities.
-template <int HD, typename T, typename C, int QT, int PT>
+// probabilities; NG: blocks of 8 query heads.
+template <int HD, typename T, typename C, int QT, int PT, int NG>
 __global__ void __launch_bounds__(kThreadsP) paged_split_kernel(const __grid_constant__ PagedArgs a) {
-    using SM = Sm<HD, QT>;
-    constexpr int KS = HD / 16, NT = HD / 8, ST = SM::kStages, RQ = SM::kQReg ? KS : 1;
+    using SM = Sm<HD>;
+    constexpr int KS = HD / 16, ST = SM::kStages, kHeads = 8 * NG;
     extern __shared__ __align__(1024) uint8_t psm[];
     __shared__ long long wsum[kWarps];
     __shared__ long long chunk[kThreadsP];  // units before the end of each thread's sequences
@@ -246,7 +251,7 @@ __global__ void __launch_bounds__(kThreadsP) paged_split_kernel(const __grid_con
 
     // columns past hd stay zero: the copies never write them
     if (hd < HD)
-        for (int i = lane; i < SM::kRing / 16; i += 32) *reinterpret_cast<uint4*>(ring + 16 * i) = make_uint4(0, 0, 0, 0);
+        for (int i = lane; i < SM::kWarp / 16; i += 32) *reinterpret_cast<uint4*>(ring + 16 * i) = make_uint4(0, 0, 0, 0);
 
     // the units before each sequence, by a scan over the lengths
     const int per = (a.batch + kThreadsP - 1) / kThreadsP;
@@ -298,8 +303,9 @@ __global__ void __launch_bounds__(kThreadsP) paged_split_kernel(const __grid_con
     Cursor cu = ld;
 
     const uint32_t ring_s = smem_u32(ring);
-    const int bk_row = (lane & 7) + ((lane >> 4) & 1) * 8, bk_kc = (lane >> 3) & 1;
-    const int bv_row = (lane & 7) + ((lane >> 3) & 1) * 8, bv_dc = (lane >> 4) & 1;
+    // ldmatrix rows and chunks of this lane: K as A (positions x dims), V^T as A (dims x positions)
+    const int k_row = (lane & 7) + ((lane >> 3) & 1) * 8, k_c = (lane >> 4) & 1;
+    const int v_row = (lane & 7) + ((lane >> 4) & 1) * 8, v_c = (lane >> 3) & 1;
 
     // The loading side: fetch looks up the page of this lane's row (lane & 15)
     // of a step two steps before issue copies the step's rows.
@@ -313,7 +319,7 @@ __global__ void __launch_bounds__(kThreadsP) paged_split_kernel(const __grid_con
         if (more) {
             const int p = (ld.sq.lo / kStep + ld.step) * kStep + (lane & 15);
             if (p >= ld.sq.lo && p < ld.sq.len) {
-                const int pg = p / a.page_size;
+                const int pg = a.page_shift >= 0 ? p >> a.page_shift : p / a.page_size;
                 f.page = __ldg(a.table + (int64_t)ld.sq.tr * a.table_stride + pg);
                 f.off = (int64_t)(p - pg * a.page_size) * a.pos_stride + (int64_t)(ld.hr / a.rt) * a.head_stride;
             }
@@ -358,79 +364,66 @@ __global__ void __launch_bounds__(kThreadsP) paged_split_kernel(const __grid_con
     int slot = 0;
     while (true) {
         // a row begins
-        const int h = cu.hr / a.rt, row0 = (cu.hr - h * a.rt) * kRows;  // KV head, first query head of the group
-        const int rows = min(kRows, a.grp - row0), head0 = h * a.grp + row0;
+        const int h = cu.hr / a.rt, row0 = (cu.hr - h * a.rt) * kHeads;  // KV head, first query head of the group
+        const int heads = min(kHeads, a.grp - row0), head0 = h * a.grp + row0;
         const int first = cu.step, lo = cu.sq.lo, len = cu.sq.len;
-        uint32_t qf[RQ][QT][4];
-        float sc0, sc1;
-        {
-            const T* q0 = static_cast<const T*>(a.q) + (int64_t)cu.b * a.q_stride + (int64_t)(head0 + gi) * hd;
-            const T* q1 = q0 + (int64_t)8 * hd;
-            const bool v0 = gi < rows, v1 = gi + 8 < rows, pairs = a.q_pairs;
-            auto el = [&](const T* p, bool v, int c) { return v && c < hd ? pair_of(p + c, pairs) : make_float2(0.0f, 0.0f); };
-            float up0 = 1.0f, up1 = 1.0f;
-            sc0 = sc1 = a.scale;
-            if (QT > 1) {  // the row's largest element to [2^10, 2^11); a single term is q itself
-                float m0 = 0.0f, m1 = 0.0f;
-#pragma unroll 4
-                for (int c = 2 * ti; c < HD; c += 8) {
-                    const float2 x = el(q0, v0, c), y = el(q1, v1, c);
-                    m0 = fmaxf(m0, fmaxf(fabsf(x.x), fabsf(x.y)));
-                    m1 = fmaxf(m1, fmaxf(fabsf(y.x), fabsf(y.y)));
-                }
-#pragma unroll
-                for (int o = 1; o < 4; o <<= 1) {
-                    m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
-                    m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
-                }
-                auto ex = [](float m) { return m > 0.0f && m < 3.0e38f ? min(100, max(-100, 10 - ilogbf(m))) : 0; };
-                const int e0 = ex(m0), e1 = ex(m1);
-                up0 = __int_as_float((127 + e0) << 23);
-                up1 = __int_as_float((127 + e1) << 23);
-                sc0 *= __int_as_float((127 - e0) << 23);
-                sc1 *= __int_as_float((127 - e1) << 23);
-            }
-            auto frag = [&](int kk, uint32_t (*t)[4]) {
-                const int c = 16 * kk + 2 * ti;
-                const float2 x[4] = {el(q0, v0, c), el(q1, v1, c), el(q0, v0, c + 8), el(q1, v1, c + 8)};
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    uint32_t w[QT];
-                    const float f = (j & 1) ? up1 : up0;
-                    split_terms<C, QT>(x[j].x * f, x[j].y * f, w);
-#pragma unroll
-                    for (int i = 0; i < QT; i++) t[i][j] = w[i];
-                }
-            };
-            if constexpr (SM::kQReg) {
-#pragma unroll
-                for (int kk = 0; kk < KS; kk++) frag(kk, qf[kk]);
-            } else {  // [kk][term][lane] fragments of 16 bytes
-                __syncwarp();
-                uint4* qs = reinterpret_cast<uint4*>(ring + SM::kRing);
-#pragma unroll 2
-                for (int kk = 0; kk < KS; kk++) {
-                    uint32_t t[QT][4];
-                    frag(kk, t);
-#pragma unroll
-                    for (int i = 0; i < QT; i++) qs[(kk * QT + i) * 32 + lane] = make_uint4(t[i][0], t[i][1], t[i][2], t[i][3]);
-                }
-                __syncwarp();
-            }
-        }
-        // scores in log2 units
+        uint32_t qf[NG][KS][QT][2];  // B fragments: head gi, dims 16 kk + 2 ti + {0, 1} and + 8
+        float ks[NG][2], sl[NG][2];  // heads 2 ti, 2 ti + 1 of each block: score factor, slope
         const float cap = a.softcap;
-        const float k0 = cap > 0.0f ? sc0 / cap : sc0 * kLog2e, k1 = cap > 0.0f ? sc1 / cap : sc1 * kLog2e;
-        float sl0 = 0.0f, sl1 = 0.0f;
-        if (a.slopes) {
-            if (gi < rows) sl0 = __ldg(a.slopes + head0 + gi) * kLog2e;
-            if (gi + 8 < rows) sl1 = __ldg(a.slopes + head0 + gi + 8) * kLog2e;
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            const bool v = 8 * g + gi < heads, pairs = a.q_pairs;
+            const T* q0 = static_cast<const T*>(a.q) + (int64_t)cu.b * a.q_stride + (int64_t)(head0 + (v ? 8 * g + gi : 0)) * hd;
+            float x[KS][4];
+#pragma unroll
+            for (int kk = 0; kk < KS; kk++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const int c = 16 * kk + 2 * ti + 8 * j;
+                    const float2 t = v && c < hd ? pair_of(q0 + c, pairs) : make_float2(0.0f, 0.0f);
+                    x[kk][2 * j] = t.x;
+                    x[kk][2 * j + 1] = t.y;
+                }
+            float up = 1.0f, factor = a.scale;
+            if (QT > 1) {  // the row's largest element to [2^10, 2^11); a single term is q itself
+                float m = 0.0f;
+#pragma unroll
+                for (int kk = 0; kk < KS; kk++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) m = fmaxf(m, fabsf(x[kk][j]));
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                // (the exponent field is enough: subnormal rows count as 2^-127)
+                const int e = m < 3.0e38f ? min(100, max(-100, 137 - (int)(__float_as_uint(m) >> 23))) : 0;
+                up = __int_as_float((127 + e) << 23);
+                factor *= __int_as_float((127 - e) << 23);
+            }
+#pragma unroll
+            for (int kk = 0; kk < KS; kk++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    uint32_t w[QT];
+                    split_terms<C, QT>(x[kk][2 * j] * up, x[kk][2 * j + 1] * up, w);
+#pragma unroll
+                    for (int i = 0; i < QT; i++) qf[g][kk][i][j] = w[i];
+                }
+            factor = cap > 0.0f ? factor / cap : factor * kLog2e;  // scores in log2 units
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                ks[g][j] = __shfl_sync(0xffffffffu, factor, 4 * (2 * ti + j));
+                sl[g][j] = a.slopes && 8 * g + 2 * ti + j < heads ? __ldg(a.slopes + head0 + 8 * g + 2 * ti + j) * kLog2e : 0.0f;
+            }
         }
 
-        float o[NT][4];
+        float o[NG][KS][4];  // dims 16 i + gi (values 0, 1) and + 8 (2, 3); heads 2 ti, 2 ti + 1
+        float m[NG][2], l[NG][2];
 #pragma unroll
-        for (int i = 0; i < NT; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;  // rows gi, gi + 8
+        for (int g = 0; g < NG; g++) {
+#pragma unroll
+            for (int i = 0; i < KS; i++) o[g][i][0] = o[g][i][1] = o[g][i][2] = o[g][i][3] = 0.0f;
+            m[g][0] = m[g][1] = -INFINITY;
+            l[g][0] = l[g][1] = 0.0f;
+        }
         bool bad = false;
 
 #pragma unroll 1
@@ -445,149 +438,129 @@ __global__ void __launch_bounds__(kThreadsP) paged_split_kernel(const __grid_con
             bad |= (bad_slots >> slot) & 1;
             slot = slot == ST - 1 ? 0 : slot + 1;
             const int p0 = (lo / kStep + cu.step) * kStep;
-            // one accumulator pair per term of q: short chains, and the terms below the
+            // one accumulator per term of q: short chains, and the terms below the
             // first stay out of a score that an infinite key made infinite (0 * inf)
-            float s0[QT][4], s1[QT][4];
+            float st[NG][QT][4];
 #pragma unroll
-            for (int t = 0; t < QT; t++)
+            for (int g = 0; g < NG; g++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) s0[t][j] = s1[t][j] = 0.0f;
+                for (int t = 0; t < QT; t++) st[g][t][0] = st[g][t][1] = st[g][t][2] = st[g][t][3] = 0.0f;
 #pragma unroll
             for (int kk = 0; kk < KS; kk++) {
-                uint32_t bk[4];
-                ldsm(kt + sw<HD>(bk_row, 2 * kk + bk_kc), bk);
+                uint32_t ak[4];
+                ldsm(kt + sw<HD>(k_row, 2 * kk + k_c), ak);
 #pragma unroll
-                for (int t = 0; t < QT; t++) {
-                    if constexpr (SM::kQReg) {
-                        Cvt<C>::mma(s0[t], qf[kk][t], bk[0], bk[1]);
-                        Cvt<C>::mma(s1[t], qf[kk][t], bk[2], bk[3]);
-                    } else {
-                        const uint4 w = reinterpret_cast<const uint4*>(ring + SM::kRing)[(kk * QT + t) * 32 + lane];
-                        const uint32_t aq[4] = {w.x, w.y, w.z, w.w};
-                        Cvt<C>::mma(s0[t], aq, bk[0], bk[1]);
-                        Cvt<C>::mma(s1[t], aq, bk[2], bk[3]);
+                for (int g = 0; g < NG; g++)
+#pragma unroll
+                    for (int t = 0; t < QT; t++) Cvt<C>::mma(st[g][t], ak, qf[g][kk][t][0], qf[g][kk][t][1]);
+            }
+            uint32_t pb[NG][PT][2];
+            float fo[NG][2];
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                // positions p0 + gi (values 0, 1) and + 8 (2, 3); heads 2 ti, 2 ti + 1
+                float s[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float top = st[g][0][j];
+                    float low = 0.0f;
+#pragma unroll
+                    for (int t = QT - 1; t > 0; t--) low += st[g][t][j];
+                    s[j] = (QT > 1 && fabsf(top) == INFINITY ? top : top + low) * ks[g][j & 1];
+                }
+                if (cap > 0.0f) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) s[j] = (cap * kLog2e) * tanhf(s[j]);
+                }
+                if (a.slopes) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        s[j] = fmaf(sl[g][j & 1], (float)(p0 + gi + (j & 2) * 4 - (len - 1)), s[j]);
+                }
+                if (p0 < lo || p0 + kStep > len) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int p = p0 + gi + (j & 2) * 4;
+                        if (p < lo || p >= len) s[j] = -INFINITY;
                     }
                 }
-            }
-            // rows gi (values 0, 1) and gi + 8 (2, 3); positions p0 + 2 ti + {0, 1} (s0), + 8 (s1)
-            float s[8];
+                float p[4];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float top = j < 4 ? s0[0][j] : s1[0][j - 4];
-                float low = 0.0f;
-#pragma unroll
-                for (int t = QT - 1; t > 0; t--) low += j < 4 ? s0[t][j] : s1[t][j - 4];
-                s[j] = (QT > 1 && fabsf(top) == INFINITY ? top : top + low) * ((j & 2) ? k1 : k0);
-            }
-            if (cap > 0.0f) {
-#pragma unroll
-                for (int j = 0; j < 8; j++) s[j] = (cap * kLog2e) * tanhf(s[j]);
-            }
-            const int pj = p0 + 2 * ti;
-            if (a.slopes) {
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-                    s[j] = fmaf((j & 2) ? sl1 : sl0, (float)(pj + (j & 1) + (j & 4) * 2 - (len - 1)), s[j]);
-            }
-            if (p0 < lo || p0 + kStep > len) {
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const int p = pj + (j & 1) + (j & 4) * 2;
-                    if (p < lo || p >= len) s[j] = -INFINITY;
-                }
-            }
-            float r0 = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[4], s[5])), r1 = fmaxf(fmaxf(s[2], s[3]), fmaxf(s[6], s[7]));
-            r0 = fmaxf(r0, __shfl_xor_sync(0xffffffffu, r0, 1));
-            r1 = fmaxf(r1, __shfl_xor_sync(0xffffffffu, r1, 1));
-            r0 = fmaxf(r0, __shfl_xor_sync(0xffffffffu, r0, 2));
-            r1 = fmaxf(r1, __shfl_xor_sync(0xffffffffu, r1, 2));
-            const float n0 = fmaxf(m0, r0), n1 = fmaxf(m1, r1);
-            // (a row whose scores are all -inf so far keeps weight zero)
-            const float z0 = n0 == -INFINITY ? 0.0f : n0, z1 = n1 == -INFINITY ? 0.0f : n1;
-            const float g0 = ex2(m0 - z0), g1 = ex2(m1 - z1);
-            m0 = n0;
-            m1 = n1;
-            float p[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) p[j] = ex2(s[j] - ((j & 2) ? z1 : z0)) * kPScale;
-            l0 = fmaf(l0, g0, (p[0] + p[1]) + (p[4] + p[5]));
-            l1 = fmaf(l1, g1, (p[2] + p[3]) + (p[6] + p[7]));
-            uint32_t pa[PT][4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                uint32_t t[PT];
-                split_terms<C, PT>(p[2 * j], p[2 * j + 1], t);
-#pragma unroll
-                for (int x = 0; x < PT; x++) pa[x][j] = t[x];
-            }
-#pragma unroll
-            for (int j = 0; j < NT / 2; j++) {
-                uint32_t bv[4];
-                ldsm_t(vt + sw<HD>(bv_row, 2 * j + bv_dc), bv);
-                float t0[4] = {0.0f, 0.0f, 0.0f, 0.0f}, t1[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int x = PT - 1; x >= 0; x--) {
-                    Cvt<C>::mma(t0, pa[x], bv[0], bv[1]);
-                    Cvt<C>::mma(t1, pa[x], bv[2], bv[3]);
+                for (int j = 0; j < 2; j++) {
+                    float r = fmaxf(s[j], s[j + 2]);
+                    r = fmaxf(r, __shfl_xor_sync(0xffffffffu, r, 4));
+                    r = fmaxf(r, __shfl_xor_sync(0xffffffffu, r, 8));
+                    r = fmaxf(r, __shfl_xor_sync(0xffffffffu, r, 16));
+                    const float n = fmaxf(m[g][j], r);
+                    const float z = n == -INFINITY ? 0.0f : n;  // (a row whose scores are all -inf so far keeps weight zero)
+                    fo[g][j] = ex2(m[g][j] - z);
+                    m[g][j] = n;
+                    p[j] = ex2(s[j] - z) * kPScale;
+                    p[j + 2] = ex2(s[j + 2] - z) * kPScale;
+                    l[g][j] = fmaf(l[g][j], fo[g][j], p[j] + p[j + 2]);
                 }
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    o[2 * j][i] = fmaf(o[2 * j][i], (i & 2) ? g1 : g0, t0[i]);
-                    o[2 * j + 1][i] = fmaf(o[2 * j + 1][i], (i & 2) ? g1 : g0, t1[i]);
+                for (int j = 0; j < 2; j++) {
+                    uint32_t t[PT];
+                    split_terms<C, PT>(p[2 * j], p[2 * j + 1], t);
+#pragma unroll
+                    for (int x = 0; x < PT; x++) pb[g][x][j] = transpose8x8(t[x]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < KS; i++) {
+                uint32_t av[4];
+                ldsm_t(vt + sw<HD>(v_row, 2 * i + v_c), av);
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int x = PT - 1; x >= 0; x--) Cvt<C>::mma(t, av, pb[g][x][0], pb[g][x][1]);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) o[g][i][j] = fmaf(o[g][i][j], fo[g][j & 1], t[j]);
                 }
             }
             __syncwarp();  // the slot is refilled by the next step's issue
         }
-        l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-        l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-        if (bad) m0 = m1 = l0 = l1 = __int_as_float(0x7fc00000);  // a page that is not there
-        const bool from_start = first == 0, to_end = cu.end == cu.ns;
-        if (from_start && to_end) {
-            const float i0 = l0 == 0.0f ? 0.0f : 1.0f / l0, i1 = l1 == 0.0f ? 0.0f : 1.0f / l1;
-            T* out = static_cast<T*>(a.out) + (int64_t)cu.b * a.out_stride + (int64_t)(head0 + gi) * hd;
+
+        const bool from_start = first == 0, to_end = cu.end == cu.ns, whole = from_start && to_end;
 #pragma unroll
-            for (int j = 0; j < NT; j++) {
-                const int d = j * 8 + 2 * ti;
-                if (d < hd) {
-                    if (gi < rows) {
-                        out[d] = (T)(o[j][0] * i0);
-                        out[d + 1] = (T)(o[j][1] * i0);
+        for (int g = 0; g < NG; g++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                float x = l[g][j], y = m[g][j];
+                x += __shfl_xor_sync(0xffffffffu, x, 4);
+                x += __shfl_xor_sync(0xffffffffu, x, 8);
+                x += __shfl_xor_sync(0xffffffffu, x, 16);
+                if (bad) x = y = __int_as_float(0x7fc00000);  // a page that is not there
+                const int head = 8 * g + 2 * ti + j;
+                if (head >= heads) continue;
+                if (whole) {
+                    const float inv = x == 0.0f ? 0.0f : 1.0f / x;
+                    T* out = static_cast<T*>(a.out) + (int64_t)cu.b * a.out_stride + (int64_t)(head0 + head) * hd;
+#pragma unroll
+                    for (int i = 0; i < KS; i++) {
+                        const int d = 16 * i + gi;
+                        if (d < hd) out[d] = (T)(o[g][i][j] * inv);
+                        if (d + 8 < hd) out[d + 8] = (T)(o[g][i][j + 2] * inv);
                     }
-                    if (gi + 8 < rows) {
-                        out[(int64_t)8 * hd + d] = (T)(o[j][2] * i1);
-                        out[(int64_t)8 * hd + d + 1] = (T)(o[j][3] * i1);
+                    if (a.lse && gi == 0)
+                        a.lse[(int64_t)cu.b * a.nh + head0 + head] = x == 0.0f ? -INFINITY : (y + (log2f(x) - 14.0f)) * kLn2;
+                } else {
+                    float* part = a.part + ((int64_t)(2 * worker + (from_start ? 1 : 0)) * kHeads + head) * (hd + 2);
+#pragma unroll
+                    for (int i = 0; i < KS; i++) {
+                        const int d = 16 * i + gi;
+                        if (d < hd) part[d] = o[g][i][j];
+                        if (d + 8 < hd) part[d + 8] = o[g][i][j + 2];
                     }
+                    if (gi == 0) *reinterpret_cast<float2*>(part + hd) = make_float2(y, x);
                 }
             }
-            if (a.lse && ti == 0) {
-                float* lse = a.lse + (int64_t)cu.b * a.nh + head0 + gi;
-                if (gi < rows) lse[0] = l0 == 0.0f ? -INFINITY : (m0 + (log2f(l0) - 14.0f)) * kLn2;
-                if (gi + 8 < rows) lse[8] = l1 == 0.0f ? -INFINITY : (m1 + (log2f(l1) - 14.0f)) * kLn2;
-            }
-        } else {
-            float* part = a.part + ((int64_t)(2 * worker + (from_start ? 1 : 0)) * kRows + gi) * (hd + 2);
-#pragma unroll
-            for (int j = 0; j < NT; j++) {
-                const int d = j * 8 + 2 * ti;
-                if (d < hd) {
-                    if (gi < rows) *reinterpret_cast<float2*>(part + d) = make_float2(o[j][0], o[j][1]);
-                    if (gi + 8 < rows) *reinterpret_cast<float2*>(part + 8 * (hd + 2) + d) = make_float2(o[j][2], o[j][3]);
-                }
-            }
-            if (ti == 0) {
-                if (gi < rows) *reinterpret_cast<float2*>(part + hd) = make_float2(m0, l0);
-                if (gi + 8 < rows) *reinterpret_cast<float2*>(part + 8 * (hd + 2) + hd) = make_float2(m1, l1);
-            }
-        }
         if (to_end && lane == 0) {
             // the worker that holds the row's first step: floor(((u + 1) G - 1) / W) of its unit u
             int c0 = worker;
-            if (!from_start) {
-                const long long u = u1 - cu.left - (cu.ns + kOverhead) + kOverhead;
-                c0 = (int)(((u + 1) * G - 1) / W);
-            }
+            if (!from_start) c0 = (int)(((u1 - cu.left - cu.ns + 1) * G - 1) / W);
             a.desc[(int64_t)cu.b * rpb + cu.hr] = make_int2(c0, worker);
         }
         if (!cu.settle(a, rpb)) break;
@@ -601,51 +574,63 @@ __global__ void __launch_bounds__(kThreadsP) paged_split_kernel(const __grid_con
 // times pw shares of the pieces.
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedArgs a, int pw) {
-    __shared__ float red[kJoinWarps][kPagedMaxHd + 2];
+    __shared__ __align__(8) float red[kJoinWarps][kPagedMaxHd + 2];
     pdl_trigger();
     pdl_wait();
     const int rpb = a.nkv * a.rt, b = blockIdx.x / rpb, hr = blockIdx.x - b * rpb, hd = a.hd;
-    const int h = hr / a.rt, row0 = (hr - h * a.rt) * kRows, rows = min(kRows, a.grp - row0), head0 = h * a.grp + row0;
+    const int h = hr / a.rt, row0 = (hr - h * a.rt) * a.heads, rows = min(a.heads, a.grp - row0), head0 = h * a.grp + row0;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rw = kJoinWarps / pw, share = warp % pw;
     const float nan = __int_as_float(0x7fc00000);
+    int2 c = a.desc[blockIdx.x];  // (not read before sq says that it was written)
     const Seq sq = seq_of(a, b);
-    int2 c = make_int2(0, 0);
-    if (sq.len) {
-        c = a.desc[blockIdx.x];
-        if (c.x == c.y) return;
-    }
+    if (sq.len && c.x == c.y) return;
     for (int rb = blockIdx.y * rw; rb < rows; rb += gridDim.y * rw) {
         const int r = rb + warp / pw;
         const bool live = r < rows;
-        float o[kPagedMaxHd / 32], M = -INFINITY, L = 0.0f;
-#pragma unroll
-        for (int j = 0; j < kPagedMaxHd / 32; j++) o[j] = 0.0f;
+        constexpr int ND = kPagedMaxHd / 64, NP = 4;  // float2 a lane; pieces in flight
+        float2 o[ND];
+        float M = -INFINITY, L = 0.0f;
         bool bad = false;
+#pragma unroll
+        for (int j = 0; j < ND; j++) o[j] = make_float2(0.0f, 0.0f);
         if (live && sq.len) {
             const float* base = a.part + (int64_t)r * (hd + 2);
-            const int64_t ps = (int64_t)kRows * (hd + 2);
-            auto piece = [&](int i) { return base + (2 * (int64_t)i + (i == c.x ? 1 : 0)) * ps; };
-            for (int i0 = c.x + share; i0 <= c.y; i0 += 32 * pw) {
-                const int i = i0 + lane * pw;
-                const float m = i <= c.y ? piece(i)[hd] : -INFINITY;
-                bad |= m != m;
-                M = fmaxf(M, m);
-            }
-            M = warp_max(M);
-            bad = __any_sync(0xffffffffu, bad);
-#pragma unroll 4
-            for (int i = c.x + share; i <= c.y; i += pw) {
-                const float* p = piece(i);
-                const float2 ml = *reinterpret_cast<const float2*>(p + hd);
-                const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - M);
-                L = fmaf(ml.y, f, L);
+            const int64_t ps = (int64_t)a.heads * (hd + 2);
+            for (int i0 = c.x + share; i0 <= c.y; i0 += NP * pw) {
+                float2 ml[NP], x[NP][ND];
 #pragma unroll
-                for (int j = 0; j < kPagedMaxHd / 64; j++) {
-                    const int d = 2 * lane + 64 * j;
-                    if (d < hd) {
-                        const float2 x = *reinterpret_cast<const float2*>(p + d);
-                        o[2 * j] = fmaf(x.x, f, o[2 * j]);
-                        o[2 * j + 1] = fmaf(x.y, f, o[2 * j + 1]);
+                for (int k = 0; k < NP; k++) {
+                    const int i = i0 + k * pw;
+                    const float* p = base + (2 * (int64_t)i + (i == c.x ? 1 : 0)) * ps;
+                    ml[k] = i <= c.y ? *reinterpret_cast<const float2*>(p + hd) : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+                    for (int j = 0; j < ND; j++) {
+                        const int d = 2 * lane + 64 * j;
+                        x[k][j] = i <= c.y && d < hd ? *reinterpret_cast<const float2*>(p + d) : make_float2(0.0f, 0.0f);
+                    }
+                }
+                float N = M;
+#pragma unroll
+                for (int k = 0; k < NP; k++) {
+                    bad |= ml[k].x != ml[k].x;
+                    N = fmaxf(N, ml[k].x);
+                }
+                const float z = N == -INFINITY ? 0.0f : N, f = ex2(M - z);
+                M = N;
+                L *= f;
+#pragma unroll
+                for (int j = 0; j < ND; j++) {
+                    o[j].x *= f;
+                    o[j].y *= f;
+                }
+#pragma unroll
+                for (int k = 0; k < NP; k++) {
+                    const float w = ex2(ml[k].x - z);
+                    L = fmaf(ml[k].y, w, L);
+#pragma unroll
+                    for (int j = 0; j < ND; j++) {
+                        o[j].x = fmaf(x[k][j].x, w, o[j].x);
+                        o[j].y = fmaf(x[k][j].y, w, o[j].y);
                     }
                 }
             }
@@ -653,17 +638,9 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
         }
         if (pw > 1) {  // the shares of a head meet in its first warp
 #pragma unroll
-            for (int j = 0; j < kPagedMaxHd / 64; j++) {
-                const int d = 2 * lane + 64 * j;
-                if (d < hd) {
-                    red[warp][d] = o[2 * j];
-                    red[warp][d + 1] = o[2 * j + 1];
-                }
-            }
-            if (lane == 0) {
-                red[warp][kPagedMaxHd] = M;
-                red[warp][kPagedMaxHd + 1] = L;
-            }
+            for (int j = 0; j < ND; j++)
+                if (2 * lane + 64 * j < hd) *reinterpret_cast<float2*>(&red[warp][2 * lane + 64 * j]) = o[j];
+            if (lane == 0) *reinterpret_cast<float2*>(&red[warp][kPagedMaxHd]) = make_float2(M, L);
             __syncthreads();
             if (share == 0) {
                 float N = M;
@@ -673,22 +650,24 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
                     any |= m != m;
                     N = fmaxf(N, m);
                 }
-                float f = M == -INFINITY ? 0.0f : ex2(M - N);
+                const float z = N == -INFINITY ? 0.0f : N, f = ex2(M - z);
                 L *= f;
 #pragma unroll
-                for (int j = 0; j < kPagedMaxHd / 32; j++) o[j] *= f;
+                for (int j = 0; j < ND; j++) {
+                    o[j].x *= f;
+                    o[j].y *= f;
+                }
                 for (int w = 1; w < pw; w++) {
-                    const float m = red[warp + w][kPagedMaxHd];
-                    f = m == -INFINITY ? 0.0f : ex2(m - N);
-                    L = fmaf(red[warp + w][kPagedMaxHd + 1], f, L);
+                    const float2 ml = *reinterpret_cast<const float2*>(&red[warp + w][kPagedMaxHd]);
+                    const float g = ex2(ml.x - z);
+                    L = fmaf(ml.y, g, L);
 #pragma unroll
-                    for (int j = 0; j < kPagedMaxHd / 64; j++) {
-                        const int d = 2 * lane + 64 * j;
-                        if (d < hd) {
-                            o[2 * j] = fmaf(red[warp + w][d], f, o[2 * j]);
-                            o[2 * j + 1] = fmaf(red[warp + w][d + 1], f, o[2 * j + 1]);
+                    for (int j = 0; j < ND; j++)
+                        if (2 * lane + 64 * j < hd) {
+                            const float2 x = *reinterpret_cast<const float2*>(&red[warp + w][2 * lane + 64 * j]);
+                            o[j].x = fmaf(x.x, g, o[j].x);
+                            o[j].y = fmaf(x.y, g, o[j].y);
                         }
-                    }
                 }
                 M = any ? nan : N;
                 if (any) L = nan;
@@ -700,11 +679,11 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
             const float inv = L == 0.0f ? 0.0f : 1.0f / L;
             T* out = static_cast<T*>(a.out) + (int64_t)b * a.out_stride + (int64_t)(head0 + r) * hd;
 #pragma unroll
-            for (int j = 0; j < kPagedMaxHd / 64; j++) {
+            for (int j = 0; j < ND; j++) {
                 const int d = 2 * lane + 64 * j;
                 if (d < hd) {
-                    out[d] = (T)(o[2 * j] * inv);
-                    out[d + 1] = (T)(o[2 * j + 1] * inv);
+                    out[d] = (T)(o[j].x * inv);
+                    out[d + 1] = (T)(o[j].y * inv);
                 }
             }
             if (a.lse && lane == 0)
@@ -715,11 +694,11 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
 
 constexpr int kMaxPagedDevices = 64;
 
-template <int HD, typename T, typename C, int QT, int PT>
+template <int HD, typename T, typename C, int QT, int PT, int NG>
 cudaError_t go(const PagedArgs& a, cudaStream_t s) {
     static std::atomic<bool> attr[kMaxPagedDevices] = {};  // the attribute belongs to a device
-    constexpr int smem = Sm<HD, QT>::kTotal;
-    auto kern = paged_split_kernel<HD, T, C, QT, PT>;
+    constexpr int smem = Sm<HD>::kTotal;
+    auto kern = paged_split_kernel<HD, T, C, QT, PT, NG>;
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
@@ -731,31 +710,43 @@ cudaError_t go(const PagedArgs& a, cudaStream_t s) {
     e = launch_pdl(kern, dim3(a.workers / kWarps), dim3(kThreadsP), smem, s, a);
     if (e != cudaSuccess) return e;
     // few rows: a CTA per query head, its pieces over the 8 warps; many: a warp per head
-    const int rows = a.batch * a.nkv * a.rt;
-    const int heads = std::min(a.grp, kRows);
+    const int rows = a.batch * a.nkv * a.rt, heads = std::min(a.grp, a.heads);
     return rows * heads <= 2 * a.sms
                ? launch_pdl(paged_join_kernel<T>, dim3(rows, heads), dim3(kJoinThreads), 0, s, a, kJoinWarps)
                : launch_pdl(paged_join_kernel<T>, dim3(rows, 1), dim3(kJoinThreads), 0, s, a, 1);
 }
 
+// Query heads of one unit: 16 for groups past 8, so that K and V are read
+// once for all of them, while the fragments of q and O fit the registers.
+int unit_heads(int hd, int grp, int dtype) { return grp > 8 && (hd <= 128 || dtype != 0) ? 16 : 8; }
+
+template <int HD, typename T, typename C, int QT, int PT>
+cudaError_t go_heads(const PagedArgs& a, cudaStream_t s) {
+    if constexpr (HD <= 128 || QT == 1) {
+        if (a.heads == 16) return go<HD, T, C, QT, PT, 2>(a, s);
+    }
+    return go<HD, T, C, QT, PT, 1>(a, s);
+}
+
 template <int HD>
 cudaError_t go_hd(const PagedArgs& a, int dtype, int cache, cudaStream_t s) {
     if (dtype == 0)
-        return cache == 1 ? go<HD, float, __half, 2, 2>(a, s) : go<HD, float, __nv_bfloat16, 3, 3>(a, s);
-    return cache == 1 ? go<HD, __half, __half, 1, 2>(a, s) : go<HD, __nv_bfloat16, __nv_bfloat16, 1, 2>(a, s);
+        return cache == 1 ? go_heads<HD, float, __half, 2, 2>(a, s) : go_heads<HD, float, __nv_bfloat16, 3, 3>(a, s);
+    return cache == 1 ? go_heads<HD, __half, __half, 1, 2>(a, s) : go_heads<HD, __nv_bfloat16, __nv_bfloat16, 1, 2>(a, s);
 }
 
 // Warps that fit the machine at once: two CTAs an SM, one for head dimensions
 // past 128 (their rings take most of the shared memory).
 int paged_workers(int hd, int sms) { return (hd > 128 ? 1 : 2) * kWarps * sms; }
 
-size_t part_bytes(int hd, int sms) { return (size_t)paged_workers(hd, sms) * 2 * kRows * (hd + 2) * sizeof(float); }
+size_t part_bytes(int hd, int heads, int sms) { return (size_t)paged_workers(hd, sms) * 2 * heads * (hd + 2) * sizeof(float); }
 
 }  // namespace
 
 size_t attention_paged_scratch(int batch, int nh, int nkv, int hd, int sms) {
-    const int rt = (nh / nkv + kRows - 1) / kRows;
-    return part_bytes(hd, sms) + (size_t)batch * nkv * rt * sizeof(int2);
+    // (the type of q is not known here: the larger of the two unit sizes)
+    const int grp = nh / nkv, heads = grp > 8 ? 16 : 8;
+    return part_bytes(hd, heads, sms) + (size_t)batch * nkv * ((grp + 7) / 8) * sizeof(int2);
 }
 
 int launch_attention_paged(const b2_paged_kv& kv, const b2_paged_attn_opts& o, const void* q, const int32_t* table,
@@ -773,7 +764,10 @@ int launch_attention_paged(const b2_paged_kv& kv, const b2_paged_attn_opts& o, c
     a.out = out;
     a.lse = lse;
     a.part = static_cast<float*>(scratch);
-    a.desc = reinterpret_cast<int2*>(static_cast<uint8_t*>(scratch) + part_bytes(kv.hd, sms));
+    a.grp = o.nh / kv.nkv;
+    a.heads = unit_heads(kv.hd, a.grp, o.dtype);
+    a.rt = (a.grp + a.heads - 1) / a.heads;
+    a.desc = reinterpret_cast<int2*>(static_cast<uint8_t*>(scratch) + part_bytes(kv.hd, a.heads, sms));
     a.slopes = o.slopes;
     const int64_t qd = (int64_t)o.nh * kv.hd;
     a.q_stride = o.q_stride ? o.q_stride : qd;
@@ -785,10 +779,9 @@ int launch_attention_paged(const b2_paged_kv& kv, const b2_paged_attn_opts& o, c
     a.batch = batch;
     a.nh = o.nh;
     a.nkv = kv.nkv;
-    a.grp = o.nh / kv.nkv;
-    a.rt = (a.grp + kRows - 1) / kRows;
     a.hd = kv.hd;
     a.page_size = kv.page_size;
+    a.page_shift = (kv.page_size & (kv.page_size - 1)) ? -1 : __builtin_ctz(kv.page_size);
     a.n_pages = kv.n_pages;
     a.max_pages = o.max_pages;
     a.n_req = o.n_req;
