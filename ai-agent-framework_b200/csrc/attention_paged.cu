@@ -100,11 +100,6 @@ __device__ __forceinline__ int steps_of(const Seq& s) { return s.len == 0 ? 0 : 
 // units of one row of sequence s: its steps behind the overhead
 __device__ __forceinline__ int units_of(const Seq& s) { return s.len == 0 ? 0 : steps_of(s) + kOverhead; }
 
-template <int HD>
-__device__ __forceinline__ uint32_t sw(int r, int c) {
-    return (uint32_t)(r * (HD * 2) + ((c ^ (r & 7)) << 4));
-}
-
 __device__ __forceinline__ void cp16(uint32_t smem, const void* gmem, bool valid) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(valid ? 16 : 0) : "memory");
 }
@@ -139,6 +134,12 @@ struct Cvt<__half> {
             "{%0, %1, %2, %3};"
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }    static __device__ __forceinline__ void mma0(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%10, %10, %10, %10};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
     }
 };
 template <>
@@ -154,6 +155,12 @@ struct Cvt<__nv_bfloat16> {
             "{%0, %1, %2, %3};"
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }    static __device__ __forceinline__ void mma0(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%10, %10, %10, %10};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
     }
 };
 
@@ -184,6 +191,12 @@ __device__ __forceinline__ float2 pair_of(const __half* p, bool pairs) {
 __device__ __forceinline__ float2 pair_of(const __nv_bfloat16* p, bool pairs) {
     return pairs ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p))
                  : make_float2(__bfloat162float(p[0]), __bfloat162float(p[1]));
+}
+
+// x * y / z, exact; in 32 bits where they do (a 64-bit division is some 100 instructions)
+__device__ __forceinline__ long long mul_div(long long x, long long y, long long z) {
+    const long long p = x * y;
+    return p <= 0xffffffffLL ? (long long)((unsigned)p / (unsigned)z) : p / z;
 }
 
 // A worker's place in its units: step `step` of `ns` of row `hr` of sequence
@@ -273,10 +286,10 @@ __global__ void __launch_bounds__(kThreadsP) paged_split_kernel(const __grid_con
     }
     __syncthreads();
     const long long W = chunk[kThreadsP - 1];
-    const long long G = max(1LL, min((long long)a.workers, W / kMinUnits));
+    const long long G = max(1LL, min((long long)a.workers, mul_div(W, 1, kMinUnits)));
     const int worker = warp * gridDim.x + blockIdx.x;  // neighbours on different SMs
     if (worker >= G || W == 0) return;
-    const long long u0 = worker * W / G, u1 = (worker + 1) * W / G;
+    const long long u0 = mul_div(worker, W, G), u1 = mul_div(worker + 1, W, G);
     Cursor ld;
     {
         int c = 0;  // the thread whose sequences hold u0
@@ -294,7 +307,7 @@ __global__ void __launch_bounds__(kThreadsP) paged_split_kernel(const __grid_con
         ld.b = b;
         ld.ns = steps_of(ld.sq);
         const int row = ld.ns + kOverhead;
-        ld.hr = (int)((u0 - base) / row);
+        ld.hr = (int)mul_div(u0 - base, 1, row);
         ld.left = u1 - u0;
         ld.enter((int)((u0 - base) - (long long)ld.hr * row));
     }
@@ -303,21 +316,30 @@ __global__ void __launch_bounds__(kThreadsP) paged_split_kernel(const __grid_con
     Cursor cu = ld;
 
     const uint32_t ring_s = smem_u32(ring);
-    // ldmatrix rows and chunks of this lane: K as A (positions x dims), V^T as A (dims x positions)
-    const int k_row = (lane & 7) + ((lane >> 3) & 1) * 8, k_c = (lane >> 4) & 1;
+    // ldmatrix places of this lane in a stage, K as A (positions x dims) and V^T as
+    // A (dims x positions): chunk 2 i + c of row r is at (place of chunk c) ^ 32 i
+    const int k_row = lane & 15, k_c = lane >> 4;
     const int v_row = (lane & 7) + ((lane >> 4) & 1) * 8, v_c = (lane >> 3) & 1;
+    const uint32_t k_at = k_row * SM::kRow + ((k_c ^ (k_row & 7)) << 4), v_at = v_row * SM::kRow + ((v_c ^ (v_row & 7)) << 4);
+    // copies: row r0 + j LR, chunk c of each; chunk c of row r goes to c ^ (r & 7)
+    constexpr int LR = 32 / (HD / 8);  // rows one warp copy covers
+    const int c_c = lane % (HD / 8), c_r = lane / (HD / 8);
+    const uint32_t c_at = c_r * SM::kRow + ((c_c ^ c_r) << 4);
+    const bool c_in = c_c < hc, one_page = a.page_size % kStep == 0;
+    const int64_t v_off = a.v - a.k;
 
     // The loading side: fetch looks up the page of this lane's row (lane & 15)
     // of a step two steps before issue copies the step's rows.
     struct Place {
         int64_t off;  // the row's place in its page; -1: a position that is not seen
         int page;
-        bool live;
+        bool live, full;  // a step; all of it seen and in one page
     };
     auto fetch = [&]() {
-        Place f{-1, -1, more};
+        Place f{-1, -1, more, false};
         if (more) {
-            const int p = (ld.sq.lo / kStep + ld.step) * kStep + (lane & 15);
+            const int first = (ld.sq.lo / kStep + ld.step) * kStep, p = first + (lane & (kStep - 1));
+            f.full = one_page && first >= ld.sq.lo && first + kStep <= ld.sq.len;
             if (p >= ld.sq.lo && p < ld.sq.len) {
                 const int pg = a.page_shift >= 0 ? p >> a.page_shift : p / a.page_size;
                 f.page = __ldg(a.table + (int64_t)ld.sq.tr * a.table_stride + pg);
@@ -332,21 +354,33 @@ __global__ void __launch_bounds__(kThreadsP) paged_split_kernel(const __grid_con
     auto issue = [&](int slot, const Place& f) {
         if (f.live) {
             const bool seen = f.off >= 0;
-            const bool ok = seen && f.page >= 0 && f.page < a.n_pages;
+            const bool ok = seen && (unsigned)f.page < (unsigned)a.n_pages;
             const uint32_t bad = __ballot_sync(0xffffffffu, seen && !ok);
             bad_slots = (bad_slots & ~(1u << slot)) | (bad ? 1u << slot : 0u);
+            const uint32_t kt = ring_s + slot * SM::kStage + c_at;
             const int64_t off = ok ? f.page * a.page_stride + f.off : -1;
-            const uint32_t kt = ring_s + slot * SM::kStage, vt = kt + kStep * SM::kRow;
-            constexpr int LR = 32 / (HD / 8);  // rows one warp copy covers
-            const int c = lane % (HD / 8), r0 = lane / (HD / 8);
+            if (f.full && !bad) {  // the rows follow each other by pos_stride
+                const uint16_t* k = a.k + (__shfl_sync(0xffffffffu, off, 0) + c_r * a.pos_stride + c_c * 8);
+                const int64_t next = LR * a.pos_stride;
+                if (c_in) {
 #pragma unroll
-            for (int j = 0; j < kStep / LR; j++) {
-                const int r = r0 + j * LR;
-                const int64_t o = __shfl_sync(0xffffffffu, off, r);
-                if (c < hc) {
-                    const int64_t at = (o < 0 ? 0 : o) + c * 8;
-                    cp16(kt + sw<HD>(r, c), a.k + at, o >= 0);
-                    cp16(vt + sw<HD>(r, c), a.v + at, o >= 0);
+                    for (int j = 0; j < kStep / LR; j++) {
+                        const uint32_t at = (kt ^ (((j * LR) & 7) << 4)) + j * LR * SM::kRow;
+                        cp16(at, k, true);
+                        cp16(at + kStep * SM::kRow, k + v_off, true);
+                        k += next;
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < kStep / LR; j++) {
+                    const int64_t o = __shfl_sync(0xffffffffu, off, c_r + j * LR);
+                    const uint32_t at = (kt ^ (((j * LR) & 7) << 4)) + j * LR * SM::kRow;
+                    if (c_in) {
+                        const uint16_t* k = a.k + ((o < 0 ? 0 : o) + c_c * 8);
+                        cp16(at, k, o >= 0);
+                        cp16(at + kStep * SM::kRow, k + v_off, o >= 0);
+                    }
                 }
             }
         }
@@ -415,12 +449,12 @@ __global__ void __launch_bounds__(kThreadsP) paged_split_kernel(const __grid_con
             }
         }
 
-        float o[NG][KS][4];  // dims 16 i + gi (values 0, 1) and + 8 (2, 3); heads 2 ti, 2 ti + 1
+        unsigned long long o[NG][KS][2];  // dims 16 i + gi and + 8; heads 2 ti, 2 ti + 1 as a pair
         float m[NG][2], l[NG][2];
 #pragma unroll
         for (int g = 0; g < NG; g++) {
 #pragma unroll
-            for (int i = 0; i < KS; i++) o[g][i][0] = o[g][i][1] = o[g][i][2] = o[g][i][3] = 0.0f;
+            for (int i = 0; i < KS; i++) o[g][i][0] = o[g][i][1] = 0;
             m[g][0] = m[g][1] = -INFINITY;
             l[g][0] = l[g][1] = 0.0f;
         }
@@ -442,20 +476,19 @@ __global__ void __launch_bounds__(kThreadsP) paged_split_kernel(const __grid_con
             // first stay out of a score that an infinite key made infinite (0 * inf)
             float st[NG][QT][4];
 #pragma unroll
-            for (int g = 0; g < NG; g++)
-#pragma unroll
-                for (int t = 0; t < QT; t++) st[g][t][0] = st[g][t][1] = st[g][t][2] = st[g][t][3] = 0.0f;
-#pragma unroll
             for (int kk = 0; kk < KS; kk++) {
                 uint32_t ak[4];
-                ldsm(kt + sw<HD>(k_row, 2 * kk + k_c), ak);
+                ldsm((kt + k_at) ^ (kk * 32), ak);
 #pragma unroll
                 for (int g = 0; g < NG; g++)
 #pragma unroll
-                    for (int t = 0; t < QT; t++) Cvt<C>::mma(st[g][t], ak, qf[g][kk][t][0], qf[g][kk][t][1]);
+                    for (int t = 0; t < QT; t++) {
+                        if (kk == 0) Cvt<C>::mma0(st[g][t], ak, qf[g][kk][t][0], qf[g][kk][t][1]);
+                        else Cvt<C>::mma(st[g][t], ak, qf[g][kk][t][0], qf[g][kk][t][1]);
+                    }
             }
             uint32_t pb[NG][PT][2];
-            float fo[NG][2];
+            unsigned long long fo2[NG];
 #pragma unroll
             for (int g = 0; g < NG; g++) {
                 // positions p0 + gi (values 0, 1) and + 8 (2, 3); heads 2 ti, 2 ti + 1
@@ -484,7 +517,7 @@ __global__ void __launch_bounds__(kThreadsP) paged_split_kernel(const __grid_con
                         if (p < lo || p >= len) s[j] = -INFINITY;
                     }
                 }
-                float p[4];
+                float p[4], fo[2];
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
                     float r = fmaxf(s[j], s[j + 2]);
@@ -493,12 +526,13 @@ __global__ void __launch_bounds__(kThreadsP) paged_split_kernel(const __grid_con
                     r = fmaxf(r, __shfl_xor_sync(0xffffffffu, r, 16));
                     const float n = fmaxf(m[g][j], r);
                     const float z = n == -INFINITY ? 0.0f : n;  // (a row whose scores are all -inf so far keeps weight zero)
-                    fo[g][j] = ex2(m[g][j] - z);
+                    fo[j] = ex2(m[g][j] - z);
                     m[g][j] = n;
                     p[j] = ex2(s[j] - z) * kPScale;
                     p[j + 2] = ex2(s[j + 2] - z) * kPScale;
-                    l[g][j] = fmaf(l[g][j], fo[g][j], p[j] + p[j + 2]);
+                    l[g][j] = fmaf(l[g][j], fo[j], p[j] + p[j + 2]);
                 }
+                fo2[g] = f2_pack(fo[0], fo[1]);
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
                     uint32_t t[PT];
@@ -510,20 +544,25 @@ __global__ void __launch_bounds__(kThreadsP) paged_split_kernel(const __grid_con
 #pragma unroll
             for (int i = 0; i < KS; i++) {
                 uint32_t av[4];
-                ldsm_t(vt + sw<HD>(v_row, 2 * i + v_c), av);
+                ldsm_t((vt + v_at) ^ (i * 32), av);
 #pragma unroll
                 for (int g = 0; g < NG; g++) {
-                    float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    float t[4];
+                    Cvt<C>::mma0(t, av, pb[g][PT - 1][0], pb[g][PT - 1][1]);
 #pragma unroll
-                    for (int x = PT - 1; x >= 0; x--) Cvt<C>::mma(t, av, pb[g][x][0], pb[g][x][1]);
-#pragma unroll
-                    for (int j = 0; j < 4; j++) o[g][i][j] = fmaf(o[g][i][j], fo[g][j & 1], t[j]);
+                    for (int x = PT - 2; x >= 0; x--) Cvt<C>::mma(t, av, pb[g][x][0], pb[g][x][1]);
+                    o[g][i][0] = f2_fma(o[g][i][0], fo2[g], f2_pack(t[0], t[1]));
+                    o[g][i][1] = f2_fma(o[g][i][1], fo2[g], f2_pack(t[2], t[3]));
                 }
             }
             __syncwarp();  // the slot is refilled by the next step's issue
         }
 
         const bool from_start = first == 0, to_end = cu.end == cu.ns, whole = from_start && to_end;
+        auto val = [&](int g, int i, int half, int j) {
+            const float2 x = f2_unpack(o[g][i][half]);
+            return j ? x.y : x.x;
+        };
 #pragma unroll
         for (int g = 0; g < NG; g++)
 #pragma unroll
@@ -541,8 +580,8 @@ __global__ void __launch_bounds__(kThreadsP) paged_split_kernel(const __grid_con
 #pragma unroll
                     for (int i = 0; i < KS; i++) {
                         const int d = 16 * i + gi;
-                        if (d < hd) out[d] = (T)(o[g][i][j] * inv);
-                        if (d + 8 < hd) out[d + 8] = (T)(o[g][i][j + 2] * inv);
+                        if (d < hd) out[d] = (T)(val(g, i, 0, j) * inv);
+                        if (d + 8 < hd) out[d + 8] = (T)(val(g, i, 1, j) * inv);
                     }
                     if (a.lse && gi == 0)
                         a.lse[(int64_t)cu.b * a.nh + head0 + head] = x == 0.0f ? -INFINITY : (y + (log2f(x) - 14.0f)) * kLn2;
@@ -551,8 +590,8 @@ __global__ void __launch_bounds__(kThreadsP) paged_split_kernel(const __grid_con
 #pragma unroll
                     for (int i = 0; i < KS; i++) {
                         const int d = 16 * i + gi;
-                        if (d < hd) part[d] = o[g][i][j];
-                        if (d + 8 < hd) part[d + 8] = o[g][i][j + 2];
+                        if (d < hd) part[d] = val(g, i, 0, j);
+                        if (d + 8 < hd) part[d + 8] = val(g, i, 1, j);
                     }
                     if (gi == 0) *reinterpret_cast<float2*>(part + hd) = make_float2(y, x);
                 }
@@ -571,8 +610,8 @@ __global__ void __launch_bounds__(kThreadsP) paged_split_kernel(const __grid_con
 // One CTA per row of units, or per query head of it (blockIdx.y): joins the
 // pieces of a row that was cut, and fills a row that sees nothing (zeros, lse
 // -inf) or whose length passes its table (NaN).  The 8 warps are 8 / pw heads
-// times pw shares of the pieces.
-template <typename T>
+// times pw shares of the pieces; a lane holds ND pairs of a head (hd <= 64 ND).
+template <typename T, int ND>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedArgs a, int pw) {
     __shared__ __align__(8) float red[kJoinWarps][kPagedMaxHd + 2];
     pdl_trigger();
@@ -587,7 +626,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     for (int rb = blockIdx.y * rw; rb < rows; rb += gridDim.y * rw) {
         const int r = rb + warp / pw;
         const bool live = r < rows;
-        constexpr int ND = kPagedMaxHd / 64, NP = 4;  // float2 a lane; pieces in flight
+        constexpr int NP = 4;  // pieces in flight
         float2 o[ND];
         float M = -INFINITY, L = 0.0f;
         bool bad = false;
@@ -712,8 +751,8 @@ cudaError_t go(const PagedArgs& a, cudaStream_t s) {
     // few rows: a CTA per query head, its pieces over the 8 warps; many: a warp per head
     const int rows = a.batch * a.nkv * a.rt, heads = std::min(a.grp, a.heads);
     return rows * heads <= 2 * a.sms
-               ? launch_pdl(paged_join_kernel<T>, dim3(rows, heads), dim3(kJoinThreads), 0, s, a, kJoinWarps)
-               : launch_pdl(paged_join_kernel<T>, dim3(rows, 1), dim3(kJoinThreads), 0, s, a, 1);
+               ? launch_pdl(paged_join_kernel<T, HD / 64>, dim3(rows, heads), dim3(kJoinThreads), 0, s, a, kJoinWarps)
+               : launch_pdl(paged_join_kernel<T, HD / 64>, dim3(rows, 1), dim3(kJoinThreads), 0, s, a, 1);
 }
 
 // Query heads of one unit: 16 for groups past 8, so that K and V are read
