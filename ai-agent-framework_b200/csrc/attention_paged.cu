@@ -9,20 +9,23 @@
 // HBM-bound: every visible K and V row is read once, from the page that holds
 // it, whatever the number of query heads that share it.
 //
-// Split.  The work of the whole batch is one line of units, a unit being one
-// step of kStep positions of one (sequence, KV head, block of query heads),
-// and worker w of G, a warp, takes the units [w W / G, (w + 1) W / G).  Ragged
-// batches thus load every SM equally without the host knowing a length, and
-// a launch captured in a graph follows the lengths it finds.  Each row of
-// units starts with kOverhead empty ones, the price of starting and ending a
-// row in steps, so that a worker with many short sequences gets fewer bytes.
-// A worker whose share starts or ends inside a row writes that piece's
+// Split.  The sequences of the batch, one after another, are a line of units,
+// a unit being one step of 16 or 32 positions.  Group g of G takes the units
+// [g W / G, (g + 1) W / G), and its workers, one warp for every (KV head, block
+// of query heads), walk that share side by side.  Ragged batches thus load
+// every SM equally without the host knowing a length, and a launch captured in
+// a graph follows the lengths it finds; and the heads of a position, neighbours
+// in memory, are read at about the same time (head dimension 112, 8 KV heads:
+// heads apart in time cost 1.3 times the bytes in half-used 128-byte lines).
+// Each sequence starts with kOverhead empty units, the price of starting and
+// ending it in steps, so that a group with many short ones gets fewer bytes.
+// A worker whose share starts or ends inside a sequence writes that piece's
 // unnormalised (o, m, l) to the scratch: at most two pieces a worker, so the
 // scratch does not grow with the lengths.  A second launch joins the pieces of
-// the rows that were cut and fills the rows that see nothing.
+// the sequences that were cut and fills the rows that see nothing.
 //
 // A warp streams its positions through a cp.async ring of its own and meets no
-// other warp: the ring runs on into the next row's K and V while a row ends.
+// other warp: the ring runs on into the next sequence while one ends.
 // The products are S^T = K Q^T and O^T = V^T P^T on mma.m16n8k16: 16 positions
 // (or dimensions) by 8 query heads, so a group of up to 8 heads fills the tile
 // (16 heads: two of them on the same K and V fragments), and P^T is S^T's
@@ -51,11 +54,8 @@
 namespace b2 {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreadsP = 32 * kWarps;
-constexpr int kStep = 16;       // positions of one unit
-constexpr int kOverhead = 4;    // units' worth of starting and ending a row
-constexpr int kMinUnits = 6;    // a worker's share, at least (overhead counted)
+constexpr int kOverhead = 4;    // units' worth of starting and ending a sequence
+constexpr int kMinUnits = 2;    // a group's share, at least (overhead counted)
 constexpr int kJoinThreads = 256;
 constexpr int kJoinWarps = kJoinThreads / 32;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -69,10 +69,10 @@ struct PagedArgs {
     void* out;
     float* lse;
     float* part;   // [workers][2][heads][hd + 2]: o, m (log2 units), l
-    int2* desc;    // [batch * nkv * rt]: first and last worker of each row of units
+    int2* desc;    // [batch]: first and last group of each sequence
     const float* slopes;
     int64_t q_stride, out_stride, table_stride, page_stride, pos_stride, head_stride;
-    int batch, nh, nkv, grp, heads, rt, hd, page_size, page_shift, n_pages, max_pages, n_req, len_add, window, workers, sms;
+    int batch, nh, nkv, grp, heads, rt, hd, page_size, page_shift, n_pages, max_pages, n_req, len_add, window, groups, sms;
     int q_pairs;   // q's rows can be read two elements at a time
     float scale, softcap;
 };
@@ -96,9 +96,15 @@ __device__ __forceinline__ Seq seq_of(const PagedArgs& a, int b) {
     return s;
 }
 
-__device__ __forceinline__ int steps_of(const Seq& s) { return s.len == 0 ? 0 : (s.len - 1) / kStep - s.lo / kStep + 1; }
-// units of one row of sequence s: its steps behind the overhead
-__device__ __forceinline__ int units_of(const Seq& s) { return s.len == 0 ? 0 : steps_of(s) + kOverhead; }
+template <int STEP>
+__device__ __forceinline__ int steps_of(const Seq& s) {
+    return s.len == 0 ? 0 : (s.len - 1) / STEP - s.lo / STEP + 1;
+}
+// units of sequence s: its steps behind the overhead
+template <int STEP>
+__device__ __forceinline__ int units_of(const Seq& s) {
+    return s.len == 0 ? 0 : steps_of<STEP>(s) + kOverhead;
+}
 
 __device__ __forceinline__ void cp16(uint32_t smem, const void* gmem, bool valid) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(valid ? 16 : 0) : "memory");
@@ -193,49 +199,58 @@ __device__ __forceinline__ float2 pair_of(const __nv_bfloat16* p, bool pairs) {
                  : make_float2(__bfloat162float(p[0]), __bfloat162float(p[1]));
 }
 
-// x * y / z, exact; in 32 bits where they do (a 64-bit division is some 100 instructions)
-__device__ __forceinline__ long long mul_div(long long x, long long y, long long z) {
-    const long long p = x * y;
+// (x * y + add) / z, exact; in 32 bits where they do (a 64-bit division is some 100 instructions)
+__device__ __forceinline__ long long mul_div(long long x, long long y, long long z, int add = 0) {
+    const long long p = x * y + add;
     return p <= 0xffffffffLL ? (long long)((unsigned)p / (unsigned)z) : p / z;
 }
 
-// A worker's place in its units: step `step` of `ns` of row `hr` of sequence
-// b, `left` units after this row's, of which this row's share ends at `end`.
+// A worker's place in its units: step `step` of the `ns` of row b, up to `end`
+// of which are its share; `left` units of its share lie behind this row.
+template <int STEP>
 struct Cursor {
     Seq sq;
-    int b, hr, ns, step, end;
-    long long left;  // units of the worker behind this row
+    int b, ns, step, end;
+    long long left;
 
-    // takes the row's share of `left` units from unit x of the row on
+    // takes this row's part of `left` units, from unit x of the row on
     __device__ __forceinline__ void enter(int x) {
-        const int row = ns + kOverhead;
-        const long long take = min((long long)(row - x), left);
+        const long long take = min((long long)(ns + kOverhead - x), left);
         left -= take;
         step = max(0, x - kOverhead);
         end = max(0, (int)(x + take) - kOverhead);
     }
-    __device__ __forceinline__ bool done() const { return step >= end; }
     // on to the worker's next step; false when there is none
-    __device__ __forceinline__ bool settle(const PagedArgs& a, int rpb) {
+    __device__ __forceinline__ bool settle(const PagedArgs& a) {
         while (step >= end) {
             if (left <= 0) return false;
-            if (++hr == rpb) {
-                hr = 0;
-                do {
-                    sq = seq_of(a, ++b);
-                    ns = steps_of(sq);
-                } while (ns == 0);
-            }
+            do {
+                sq = seq_of(a, ++b);
+                ns = steps_of<STEP>(sq);
+            } while (ns == 0);
             enter(0);
         }
         return true;
     }
 };
 
-template <int HD>
+template <int HD, int NG>
 struct Sm {
+    // 32 positions a step, as two products side by side, hide each other's
+    // latencies (8 x 32K of head dimension 64: 131 us with 16, 94 with 32); with
+    // head dimension 256 or 16 query heads the registers are better kept for two
+    // warps a scheduler (32K x 16 of 16 heads: 69 us with 32, 61 with 16).
+    static constexpr int kSub = HD > 128 || NG > 1 ? 1 : 2;
+    static constexpr int kStep = 16 * kSub;
+    // The copies in flight are what the ring holds beyond the step at work.
+    // 64 KB an SM is enough for the full rate, and more is worse: the SMs then
+    // get unequal shares of the bandwidth (8 x 32K with 128 KB: 178 us, the first
+    // SM done after 132, the last after 175; with 64 KB 162 us).
+    static constexpr int kStages = 2;
+    static constexpr int kWarps = 4;
+    static constexpr int kCtas = HD > 128 ? 1 : HD == 128 && NG == 1 ? 1 : 2;  // of an SM
+    static constexpr int kThreads = 32 * kWarps;
     static constexpr int kRow = HD * 2;
-    static constexpr int kStages = HD == 64 ? 6 : 3;
     static constexpr int kStage = 2 * kStep * kRow;  // a warp's K and V rows of one step
     static constexpr int kWarp = kStages * kStage;
     static constexpr int kTotal = kWarps * kWarp;
@@ -250,12 +265,13 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 // T: the type of q and out; C: the cache's; QT, PT: terms of q and of the
 // probabilities; NG: blocks of 8 query heads.
 template <int HD, typename T, typename C, int QT, int PT, int NG>
-__global__ void __launch_bounds__(kThreadsP) paged_split_kernel(const __grid_constant__ PagedArgs a) {
-    using SM = Sm<HD>;
-    constexpr int KS = HD / 16, ST = SM::kStages, kHeads = 8 * NG;
+__global__ void __launch_bounds__(Sm<HD, NG>::kThreads) paged_split_kernel(const __grid_constant__ PagedArgs a) {
+    using SM = Sm<HD, NG>;
+    constexpr int KS = HD / 16, ST = SM::kStages, SUB = SM::kSub, STEP = SM::kStep, kHeads = 8 * NG;
+    constexpr int kWarps = SM::kWarps, kThreads = SM::kThreads;
     extern __shared__ __align__(1024) uint8_t psm[];
     __shared__ long long wsum[kWarps];
-    __shared__ long long chunk[kThreadsP];  // units before the end of each thread's sequences
+    __shared__ long long chunk[kThreads];  // units before the end of each thread's sequences
     pdl_trigger();
     pdl_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gi = lane >> 2, ti = lane & 3;
@@ -267,11 +283,11 @@ __global__ void __launch_bounds__(kThreadsP) paged_split_kernel(const __grid_con
         for (int i = lane; i < SM::kWarp / 16; i += 32) *reinterpret_cast<uint4*>(ring + 16 * i) = make_uint4(0, 0, 0, 0);
 
     // the units before each sequence, by a scan over the lengths
-    const int per = (a.batch + kThreadsP - 1) / kThreadsP;
+    const int per = (a.batch + kThreads - 1) / kThreads;
     {
         const int b0 = min(a.batch, tid * per), b1 = min(a.batch, b0 + per);
         long long inc = 0;
-        for (int b = b0; b < b1; b++) inc += units_of(seq_of(a, b));
+        for (int b = b0; b < b1; b++) inc += units_of<STEP>(seq_of(a, b));
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const long long x = __shfl_up_sync(0xffffffffu, inc, o);
@@ -282,38 +298,40 @@ __global__ void __launch_bounds__(kThreadsP) paged_split_kernel(const __grid_con
 #pragma unroll
         for (int w = 0; w < kWarps; w++)
             if (w < warp) inc += wsum[w];
-        chunk[tid] = inc * rpb;
+        chunk[tid] = inc;
     }
     __syncthreads();
-    const long long W = chunk[kThreadsP - 1];
-    const long long G = max(1LL, min((long long)a.workers, mul_div(W, 1, kMinUnits)));
+    const long long W = chunk[kThreads - 1];
+    const long long G = max(1LL, min((long long)a.groups, mul_div(W, 1, kMinUnits)));
     const int worker = warp * gridDim.x + blockIdx.x;  // neighbours on different SMs
-    if (worker >= G || W == 0) return;
-    const long long u0 = mul_div(worker, W, G), u1 = mul_div(worker + 1, W, G);
-    Cursor ld;
+    const int group = worker / rpb, hr = worker - group * rpb;
+    if (group >= G || W == 0) return;
+    const long long u0 = mul_div(group, W, G), u1 = mul_div(group + 1, W, G);
+    Cursor<STEP> ld;
     {
         int c = 0;  // the thread whose sequences hold u0
 #pragma unroll
-        for (int j = 0; j < kThreadsP / 32; j++) c += __popc(__ballot_sync(0xffffffffu, chunk[j * 32 + lane] <= u0));
+        for (int j = 0; j < kThreads / 32; j++) c += __popc(__ballot_sync(0xffffffffu, chunk[j * 32 + lane] <= u0));
         long long base = c ? chunk[c - 1] : 0;
         int b = c * per;
         while (true) {
             ld.sq = seq_of(a, b);
-            const long long n = (long long)units_of(ld.sq) * rpb;
+            const int n = units_of<STEP>(ld.sq);
             if (u0 < base + n) break;
             base += n;
             b++;
         }
         ld.b = b;
-        ld.ns = steps_of(ld.sq);
-        const int row = ld.ns + kOverhead;
-        ld.hr = (int)mul_div(u0 - base, 1, row);
+        ld.ns = steps_of<STEP>(ld.sq);
         ld.left = u1 - u0;
-        ld.enter((int)((u0 - base) - (long long)ld.hr * row));
+        ld.enter((int)(u0 - base));
     }
-    bool more = ld.settle(a, rpb);  // the loading side has a step
+    const int h = hr / a.rt, row0 = (hr - h * a.rt) * kHeads;  // KV head, first query head of the group
+    const int heads = min(kHeads, a.grp - row0), head0 = h * a.grp + row0;
+    const int64_t h_off = (int64_t)h * a.head_stride;
+    bool more = ld.settle(a);  // the loading side has a step
     if (!more) return;              // (overhead alone)
-    Cursor cu = ld;
+    Cursor<STEP> cu = ld;
 
     const uint32_t ring_s = smem_u32(ring);
     // ldmatrix places of this lane in a stage, K as A (positions x dims) and V^T as
@@ -325,7 +343,7 @@ __global__ void __launch_bounds__(kThreadsP) paged_split_kernel(const __grid_con
     constexpr int LR = 32 / (HD / 8);  // rows one warp copy covers
     const int c_c = lane % (HD / 8), c_r = lane / (HD / 8);
     const uint32_t c_at = c_r * SM::kRow + ((c_c ^ c_r) << 4);
-    const bool c_in = c_c < hc, one_page = a.page_size % kStep == 0;
+    const bool c_in = c_c < hc, one_page = a.page_size % 16 == 0;
     const int64_t v_off = a.v - a.k;
 
     // The loading side: fetch looks up the page of this lane's row (lane & 15)
@@ -333,20 +351,20 @@ __global__ void __launch_bounds__(kThreadsP) paged_split_kernel(const __grid_con
     struct Place {
         int64_t off;  // the row's place in its page; -1: a position that is not seen
         int page;
-        bool live, full;  // a step; all of it seen and in one page
+        bool live, full;  // a step; all of it seen, every 16 rows in one page
     };
     auto fetch = [&]() {
         Place f{-1, -1, more, false};
         if (more) {
-            const int first = (ld.sq.lo / kStep + ld.step) * kStep, p = first + (lane & (kStep - 1));
-            f.full = one_page && first >= ld.sq.lo && first + kStep <= ld.sq.len;
+            const int first = (ld.sq.lo / STEP + ld.step) * STEP, p = first + (lane & (STEP - 1));
+            f.full = one_page && first >= ld.sq.lo && first + STEP <= ld.sq.len;
             if (p >= ld.sq.lo && p < ld.sq.len) {
                 const int pg = a.page_shift >= 0 ? p >> a.page_shift : p / a.page_size;
                 f.page = __ldg(a.table + (int64_t)ld.sq.tr * a.table_stride + pg);
-                f.off = (int64_t)(p - pg * a.page_size) * a.pos_stride + (int64_t)(ld.hr / a.rt) * a.head_stride;
+                f.off = (int64_t)(p - pg * a.page_size) * a.pos_stride + h_off;
             }
             ld.step++;
-            more = ld.settle(a, rpb);
+            more = ld.settle(a);
         }
         return f;
     };
@@ -359,27 +377,30 @@ __global__ void __launch_bounds__(kThreadsP) paged_split_kernel(const __grid_con
             bad_slots = (bad_slots & ~(1u << slot)) | (bad ? 1u << slot : 0u);
             const uint32_t kt = ring_s + slot * SM::kStage + c_at;
             const int64_t off = ok ? f.page * a.page_stride + f.off : -1;
-            if (f.full && !bad) {  // the rows follow each other by pos_stride
-                const uint16_t* k = a.k + (__shfl_sync(0xffffffffu, off, 0) + c_r * a.pos_stride + c_c * 8);
-                const int64_t next = LR * a.pos_stride;
-                if (c_in) {
+            if (f.full && !bad) {  // 16 rows follow each other by pos_stride
+                const int64_t at0 = c_r * a.pos_stride + c_c * 8, next = LR * a.pos_stride;
 #pragma unroll
-                    for (int j = 0; j < kStep / LR; j++) {
-                        const uint32_t at = (kt ^ (((j * LR) & 7) << 4)) + j * LR * SM::kRow;
-                        cp16(at, k, true);
-                        cp16(at + kStep * SM::kRow, k + v_off, true);
-                        k += next;
+                for (int sub = 0; sub < SUB; sub++) {
+                    const uint16_t* k = a.k + (__shfl_sync(0xffffffffu, off, 16 * sub) + at0);
+                    if (c_in) {
+#pragma unroll
+                        for (int j = 0; j < 16 / LR; j++) {
+                            const uint32_t at = (kt ^ (((j * LR) & 7) << 4)) + (16 * sub + j * LR) * SM::kRow;
+                            cp16(at, k, true);
+                            cp16(at + STEP * SM::kRow, k + v_off, true);
+                            k += next;
+                        }
                     }
                 }
             } else {
 #pragma unroll
-                for (int j = 0; j < kStep / LR; j++) {
+                for (int j = 0; j < STEP / LR; j++) {
                     const int64_t o = __shfl_sync(0xffffffffu, off, c_r + j * LR);
                     const uint32_t at = (kt ^ (((j * LR) & 7) << 4)) + j * LR * SM::kRow;
                     if (c_in) {
                         const uint16_t* k = a.k + ((o < 0 ? 0 : o) + c_c * 8);
                         cp16(at, k, o >= 0);
-                        cp16(at + kStep * SM::kRow, k + v_off, o >= 0);
+                        cp16(at + STEP * SM::kRow, k + v_off, o >= 0);
                     }
                 }
             }
@@ -397,9 +418,7 @@ __global__ void __launch_bounds__(kThreadsP) paged_split_kernel(const __grid_con
 
     int slot = 0;
     while (true) {
-        // a row begins
-        const int h = cu.hr / a.rt, row0 = (cu.hr - h * a.rt) * kHeads;  // KV head, first query head of the group
-        const int heads = min(kHeads, a.grp - row0), head0 = h * a.grp + row0;
+        // a sequence begins
         const int first = cu.step, lo = cu.sq.lo, len = cu.sq.len;
         uint32_t qf[NG][KS][QT][2];  // B fragments: head gi, dims 16 kk + 2 ti + {0, 1} and + 8
         float ks[NG][2], sl[NG][2];  // heads 2 ti, 2 ti + 1 of each block: score factor, slope
@@ -468,91 +487,116 @@ __global__ void __launch_bounds__(kThreadsP) paged_split_kernel(const __grid_con
             f1 = f2;
             cp_wait<ST - 1>();
             __syncwarp();
-            const uint32_t kt = ring_s + slot * SM::kStage, vt = kt + kStep * SM::kRow;
+            const uint32_t kt = ring_s + slot * SM::kStage, vt = kt + STEP * SM::kRow;
             bad |= (bad_slots >> slot) & 1;
             slot = slot == ST - 1 ? 0 : slot + 1;
-            const int p0 = (lo / kStep + cu.step) * kStep;
+            const int p0 = (lo / STEP + cu.step) * STEP;
             // one accumulator per term of q: short chains, and the terms below the
             // first stay out of a score that an infinite key made infinite (0 * inf)
-            float st[NG][QT][4];
+            float st[SUB][NG][QT][4];
 #pragma unroll
-            for (int kk = 0; kk < KS; kk++) {
-                uint32_t ak[4];
-                ldsm((kt + k_at) ^ (kk * 32), ak);
+            for (int kk = 0; kk < KS; kk++)
 #pragma unroll
-                for (int g = 0; g < NG; g++)
+                for (int sub = 0; sub < SUB; sub++) {
+                    uint32_t ak[4];
+                    ldsm(((kt + k_at) ^ (kk * 32)) + sub * 16 * SM::kRow, ak);
 #pragma unroll
-                    for (int t = 0; t < QT; t++) {
-                        if (kk == 0) Cvt<C>::mma0(st[g][t], ak, qf[g][kk][t][0], qf[g][kk][t][1]);
-                        else Cvt<C>::mma(st[g][t], ak, qf[g][kk][t][0], qf[g][kk][t][1]);
-                    }
-            }
-            uint32_t pb[NG][PT][2];
+                    for (int g = 0; g < NG; g++)
+#pragma unroll
+                        for (int t = 0; t < QT; t++) {
+                            if (kk == 0) Cvt<C>::mma0(st[sub][g][t], ak, qf[g][kk][t][0], qf[g][kk][t][1]);
+                            else Cvt<C>::mma(st[sub][g][t], ak, qf[g][kk][t][0], qf[g][kk][t][1]);
+                        }
+                }
+            uint32_t pb[SUB][NG][PT][2];
             unsigned long long fo2[NG];
 #pragma unroll
             for (int g = 0; g < NG; g++) {
-                // positions p0 + gi (values 0, 1) and + 8 (2, 3); heads 2 ti, 2 ti + 1
-                float s[4];
+                // positions p0 + 16 sub + gi (values 0, 1) and + 8 (2, 3); heads 2 ti, 2 ti + 1
+                float s[SUB][4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const float top = st[g][0][j];
-                    float low = 0.0f;
+                for (int sub = 0; sub < SUB; sub++)
 #pragma unroll
-                    for (int t = QT - 1; t > 0; t--) low += st[g][t][j];
-                    s[j] = (QT > 1 && fabsf(top) == INFINITY ? top : top + low) * ks[g][j & 1];
-                }
+                    for (int j = 0; j < 4; j++) {
+                        const float top = st[sub][g][0][j];
+                        float low = 0.0f;
+#pragma unroll
+                        for (int t = QT - 1; t > 0; t--) low += st[sub][g][t][j];
+                        s[sub][j] = (QT > 1 && fabsf(top) == INFINITY ? top : top + low) * ks[g][j & 1];
+                    }
                 if (cap > 0.0f) {
 #pragma unroll
-                    for (int j = 0; j < 4; j++) s[j] = (cap * kLog2e) * tanhf(s[j]);
+                    for (int sub = 0; sub < SUB; sub++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) s[sub][j] = (cap * kLog2e) * tanhf(s[sub][j]);
                 }
                 if (a.slopes) {
 #pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        s[j] = fmaf(sl[g][j & 1], (float)(p0 + gi + (j & 2) * 4 - (len - 1)), s[j]);
-                }
-                if (p0 < lo || p0 + kStep > len) {
+                    for (int sub = 0; sub < SUB; sub++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const int p = p0 + gi + (j & 2) * 4;
-                        if (p < lo || p >= len) s[j] = -INFINITY;
-                    }
+                        for (int j = 0; j < 4; j++)
+                            s[sub][j] = fmaf(sl[g][j & 1], (float)(p0 + 16 * sub + gi + (j & 2) * 4 - (len - 1)), s[sub][j]);
                 }
-                float p[4], fo[2];
+                if (p0 < lo || p0 + STEP > len) {
+#pragma unroll
+                    for (int sub = 0; sub < SUB; sub++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const int p = p0 + 16 * sub + gi + (j & 2) * 4;
+                            if (p < lo || p >= len) s[sub][j] = -INFINITY;
+                        }
+                }
+                float fo[2], z[2];
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    float r = fmaxf(s[j], s[j + 2]);
+                    float r = fmaxf(s[0][j], s[0][j + 2]);
+#pragma unroll
+                    for (int sub = 1; sub < SUB; sub++) r = fmaxf(r, fmaxf(s[sub][j], s[sub][j + 2]));
                     r = fmaxf(r, __shfl_xor_sync(0xffffffffu, r, 4));
                     r = fmaxf(r, __shfl_xor_sync(0xffffffffu, r, 8));
                     r = fmaxf(r, __shfl_xor_sync(0xffffffffu, r, 16));
                     const float n = fmaxf(m[g][j], r);
-                    const float z = n == -INFINITY ? 0.0f : n;  // (a row whose scores are all -inf so far keeps weight zero)
-                    fo[j] = ex2(m[g][j] - z);
+                    z[j] = n == -INFINITY ? 0.0f : n;  // (a row whose scores are all -inf so far keeps weight zero)
+                    fo[j] = ex2(m[g][j] - z[j]);
                     m[g][j] = n;
-                    p[j] = ex2(s[j] - z) * kPScale;
-                    p[j + 2] = ex2(s[j + 2] - z) * kPScale;
-                    l[g][j] = fmaf(l[g][j], fo[j], p[j] + p[j + 2]);
+                    l[g][j] *= fo[j];
                 }
                 fo2[g] = f2_pack(fo[0], fo[1]);
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    uint32_t t[PT];
-                    split_terms<C, PT>(p[2 * j], p[2 * j + 1], t);
+                for (int sub = 0; sub < SUB; sub++) {
+                    float p[4];
 #pragma unroll
-                    for (int x = 0; x < PT; x++) pb[g][x][j] = transpose8x8(t[x]);
+                    for (int j = 0; j < 4; j++) p[j] = ex2(s[sub][j] - z[j & 1]) * kPScale;
+                    l[g][0] += p[0] + p[2];
+                    l[g][1] += p[1] + p[3];
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        uint32_t t[PT];
+                        split_terms<C, PT>(p[2 * j], p[2 * j + 1], t);
+#pragma unroll
+                        for (int x = 0; x < PT; x++) pb[sub][g][x][j] = transpose8x8(t[x]);
+                    }
                 }
             }
 #pragma unroll
             for (int i = 0; i < KS; i++) {
-                uint32_t av[4];
-                ldsm_t((vt + v_at) ^ (i * 32), av);
+                float t[NG][4];
+#pragma unroll
+                for (int sub = 0; sub < SUB; sub++) {
+                    uint32_t av[4];
+                    ldsm_t(((vt + v_at) ^ (i * 32)) + sub * 16 * SM::kRow, av);
+#pragma unroll
+                    for (int g = 0; g < NG; g++)
+#pragma unroll
+                        for (int x = PT - 1; x >= 0; x--) {
+                            if (sub == 0 && x == PT - 1) Cvt<C>::mma0(t[g], av, pb[sub][g][x][0], pb[sub][g][x][1]);
+                            else Cvt<C>::mma(t[g], av, pb[sub][g][x][0], pb[sub][g][x][1]);
+                        }
+                }
 #pragma unroll
                 for (int g = 0; g < NG; g++) {
-                    float t[4];
-                    Cvt<C>::mma0(t, av, pb[g][PT - 1][0], pb[g][PT - 1][1]);
-#pragma unroll
-                    for (int x = PT - 2; x >= 0; x--) Cvt<C>::mma(t, av, pb[g][x][0], pb[g][x][1]);
-                    o[g][i][0] = f2_fma(o[g][i][0], fo2[g], f2_pack(t[0], t[1]));
-                    o[g][i][1] = f2_fma(o[g][i][1], fo2[g], f2_pack(t[2], t[3]));
+                    o[g][i][0] = f2_fma(o[g][i][0], fo2[g], f2_pack(t[g][0], t[g][1]));
+                    o[g][i][1] = f2_fma(o[g][i][1], fo2[g], f2_pack(t[g][2], t[g][3]));
                 }
             }
             __syncwarp();  // the slot is refilled by the next step's issue
@@ -596,19 +640,19 @@ __global__ void __launch_bounds__(kThreadsP) paged_split_kernel(const __grid_con
                     if (gi == 0) *reinterpret_cast<float2*>(part + hd) = make_float2(y, x);
                 }
             }
-        if (to_end && lane == 0) {
-            // the worker that holds the row's first step: floor(((u + 1) G - 1) / W) of its unit u
-            int c0 = worker;
-            if (!from_start) c0 = (int)(((u1 - cu.left - cu.ns + 1) * G - 1) / W);
-            a.desc[(int64_t)cu.b * rpb + cu.hr] = make_int2(c0, worker);
+        if (to_end && hr == 0 && lane == 0) {
+            // the group that holds the first step's unit u: floor(((u + 1) G - 1) / W)
+            int c0 = group;
+            if (!from_start) c0 = (int)mul_div(u1 - cu.left - cu.ns + 1, G, W, -1);
+            a.desc[cu.b] = make_int2(c0, group);
         }
-        if (!cu.settle(a, rpb)) break;
+        if (!cu.settle(a)) break;
     }
     cp_wait<0>();
 }
 
-// One CTA per row of units, or per query head of it (blockIdx.y): joins the
-// pieces of a row that was cut, and fills a row that sees nothing (zeros, lse
+// One CTA per (row, KV head, block of query heads), or per query head of it
+// (blockIdx.y): joins the pieces of a row that was cut, and fills a row that sees nothing (zeros, lse
 // -inf) or whose length passes its table (NaN).  The 8 warps are 8 / pw heads
 // times pw shares of the pieces; a lane holds ND pairs of a head (hd <= 64 ND).
 template <typename T, int ND>
@@ -620,7 +664,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     const int h = hr / a.rt, row0 = (hr - h * a.rt) * a.heads, rows = min(a.heads, a.grp - row0), head0 = h * a.grp + row0;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rw = kJoinWarps / pw, share = warp % pw;
     const float nan = __int_as_float(0x7fc00000);
-    int2 c = a.desc[blockIdx.x];  // (not read before sq says that it was written)
+    int2 c = a.desc[b];  // (not used before sq says that it was written)
     const Seq sq = seq_of(a, b);
     if (sq.len && c.x == c.y) return;
     for (int rb = blockIdx.y * rw; rb < rows; rb += gridDim.y * rw) {
@@ -633,14 +677,14 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
 #pragma unroll
         for (int j = 0; j < ND; j++) o[j] = make_float2(0.0f, 0.0f);
         if (live && sq.len) {
-            const float* base = a.part + (int64_t)r * (hd + 2);
-            const int64_t ps = (int64_t)a.heads * (hd + 2);
+            const float* base = a.part + ((int64_t)2 * hr * a.heads + r) * (hd + 2);
+            const int64_t ps = (int64_t)a.heads * (hd + 2);  // of a piece; a group's are 2 rpb apart
             for (int i0 = c.x + share; i0 <= c.y; i0 += NP * pw) {
                 float2 ml[NP], x[NP][ND];
 #pragma unroll
                 for (int k = 0; k < NP; k++) {
                     const int i = i0 + k * pw;
-                    const float* p = base + (2 * (int64_t)i + (i == c.x ? 1 : 0)) * ps;
+                    const float* p = base + (2 * (int64_t)i * rpb + (i == c.x ? 1 : 0)) * ps;
                     ml[k] = i <= c.y ? *reinterpret_cast<const float2*>(p + hd) : make_float2(-INFINITY, 0.0f);
 #pragma unroll
                     for (int j = 0; j < ND; j++) {
@@ -736,7 +780,8 @@ constexpr int kMaxPagedDevices = 64;
 template <int HD, typename T, typename C, int QT, int PT, int NG>
 cudaError_t go(const PagedArgs& a, cudaStream_t s) {
     static std::atomic<bool> attr[kMaxPagedDevices] = {};  // the attribute belongs to a device
-    constexpr int smem = Sm<HD>::kTotal;
+    using SM = Sm<HD, NG>;
+    constexpr int smem = SM::kTotal;
     auto kern = paged_split_kernel<HD, T, C, QT, PT, NG>;
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -746,7 +791,7 @@ cudaError_t go(const PagedArgs& a, cudaStream_t s) {
         if (e != cudaSuccess) return e;
         if (dev < kMaxPagedDevices) attr[dev] = true;
     }
-    e = launch_pdl(kern, dim3(a.workers / kWarps), dim3(kThreadsP), smem, s, a);
+    e = launch_pdl(kern, dim3((a.groups * a.nkv * a.rt + SM::kWarps - 1) / SM::kWarps), dim3(SM::kThreads), smem, s, a);
     if (e != cudaSuccess) return e;
     // few rows: a CTA per query head, its pieces over the 8 warps; many: a warp per head
     const int rows = a.batch * a.nkv * a.rt, heads = std::min(a.grp, a.heads);
@@ -774,18 +819,28 @@ cudaError_t go_hd(const PagedArgs& a, int dtype, int cache, cudaStream_t s) {
     return cache == 1 ? go_heads<HD, __half, __half, 1, 2>(a, s) : go_heads<HD, __nv_bfloat16, __nv_bfloat16, 1, 2>(a, s);
 }
 
-// Warps that fit the machine at once: two CTAs an SM, one for head dimensions
-// past 128 (their rings take most of the shared memory).
-int paged_workers(int hd, int sms) { return (hd > 128 ? 1 : 2) * kWarps * sms; }
+// Groups of rpb workers each: as many as fit the machine at once.
+template <int HD, int NG>
+int groups_in(int rpb, int sms) {
+    return std::max(1, Sm<HD, NG>::kCtas * Sm<HD, NG>::kWarps * sms / rpb);
+}
+int groups_of(int hd, int heads, int rpb, int sms) {
+    if (heads == 16) return hd <= 64 ? groups_in<64, 2>(rpb, sms) : hd <= 128 ? groups_in<128, 2>(rpb, sms) : groups_in<256, 2>(rpb, sms);
+    return hd <= 64 ? groups_in<64, 1>(rpb, sms) : hd <= 128 ? groups_in<128, 1>(rpb, sms) : groups_in<256, 1>(rpb, sms);
+}
 
-size_t part_bytes(int hd, int heads, int sms) { return (size_t)paged_workers(hd, sms) * 2 * heads * (hd + 2) * sizeof(float); }
+size_t part_bytes(int hd, int heads, int rpb, int sms) {
+    return (size_t)groups_of(hd, heads, rpb, sms) * rpb * 2 * heads * (hd + 2) * sizeof(float);
+}
 
 }  // namespace
 
 size_t attention_paged_scratch(int batch, int nh, int nkv, int hd, int sms) {
     // (the type of q is not known here: the larger of the two unit sizes)
-    const int grp = nh / nkv, heads = grp > 8 ? 16 : 8;
-    return part_bytes(hd, heads, sms) + (size_t)batch * nkv * ((grp + 7) / 8) * sizeof(int2);
+    const int grp = nh / nkv;
+    size_t n = part_bytes(hd, 8, nkv * ((grp + 7) / 8), sms);
+    if (grp > 8) n = std::max(n, part_bytes(hd, 16, nkv * ((grp + 15) / 16), sms));
+    return n + (size_t)batch * sizeof(int2);
 }
 
 int launch_attention_paged(const b2_paged_kv& kv, const b2_paged_attn_opts& o, const void* q, const int32_t* table,
@@ -806,7 +861,7 @@ int launch_attention_paged(const b2_paged_kv& kv, const b2_paged_attn_opts& o, c
     a.grp = o.nh / kv.nkv;
     a.heads = unit_heads(kv.hd, a.grp, o.dtype);
     a.rt = (a.grp + a.heads - 1) / a.heads;
-    a.desc = reinterpret_cast<int2*>(static_cast<uint8_t*>(scratch) + part_bytes(kv.hd, a.heads, sms));
+    a.desc = reinterpret_cast<int2*>(static_cast<uint8_t*>(scratch) + part_bytes(kv.hd, a.heads, kv.nkv * a.rt, sms));
     a.slopes = o.slopes;
     const int64_t qd = (int64_t)o.nh * kv.hd;
     a.q_stride = o.q_stride ? o.q_stride : qd;
@@ -826,7 +881,7 @@ int launch_attention_paged(const b2_paged_kv& kv, const b2_paged_attn_opts& o, c
     a.n_req = o.n_req;
     a.len_add = o.len_add;
     a.window = o.window;
-    a.workers = paged_workers(kv.hd, sms);
+    a.groups = groups_of(kv.hd, a.heads, kv.nkv * a.rt, sms);
     a.sms = sms;
     const int es = o.dtype == 0 ? 4 : 2;
     a.q_pairs = a.q_stride % 2 == 0 && !(reinterpret_cast<uintptr_t>(q) & (2 * es - 1));
