@@ -8,10 +8,11 @@
 //   m -> m':  S' = S e^(m - m'),  T' = e^(m - m') (T + (m - m') S).
 //
 // Top k without a second pass over the row.  Every thread of the pass ends
-// with the largest logit it saw; the k-th largest of those maxima is a lower
-// bound of the k-th largest logit, and a logit at or above it can only be in
-// a thread whose maximum is.  About k of the threads' shares are read again
-// (from L2) for their candidates, which are ordered by counting.  Where very
+// with the largest logit it saw.  The k-th largest of the maxima of 64 groups
+// of threads is a lower bound of the k-th largest logit, and a logit at or
+// above it can only be in a thread whose maximum is.  A few more than k of the
+// threads' shares are read again (from L2) for their candidates, which are
+// ordered by counting.  Where very
 // many threads tie at the bound (a vocabulary masked with one value), the
 // logits above it come from fewer than k threads, and the ties are taken in
 // index order from the start of the row.
@@ -37,6 +38,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kLpThreads = 512;
 constexpr int kLpWarps = kLpThreads / 32;
+constexpr int kLpGroups = kLogprobMaxTop;         // groups of threads whose maxima give the bound
 constexpr int kLpMaxCluster = 8;
 constexpr int kLpRound = kLpThreads * 8;         // logits one collecting round may add
 constexpr int kLpCap = kLpRound + 1024;          // candidates held at once
@@ -78,7 +80,7 @@ __device__ __forceinline__ unsigned long long key_of(float x, int i) {
 __device__ __forceinline__ int key_index(unsigned long long k) { return (int)~(uint32_t)k; }
 
 struct Sums {
-    float m, S, T;  // T in units of log 2: sum (x - m) log2(e) 2^(..)
+    float m, S, T;  // T in units of log 2: sum (x - m) log2(e) e^(x - m)
 };
 
 // b's sums added to a's
@@ -92,11 +94,77 @@ __device__ __forceinline__ Sums join(Sums a, Sums b) {
     r.T = fa * fmaf(da, a.S, a.T) + fb * fmaf(db, b.S, b.T);
     return r;
 }
+__device__ __forceinline__ Sums join_lanes(Sums t, int lanes) {
+    for (int o = lanes / 2; o; o >>= 1) {
+        const Sums p{__shfl_xor_sync(0xffffffffu, t.m, o), __shfl_xor_sync(0xffffffffu, t.S, o),
+                     __shfl_xor_sync(0xffffffffu, t.T, o)};
+        t = join(t, p);
+    }
+    return t;
+}
+
+// A thread's sums, S and T as pairs (even and odd elements)
+struct Acc {
+    float m = -INFINITY;
+    unsigned long long S = 0, T = 0;
+
+    // the maximum grows to at least bm; returns the reference
+    __device__ __forceinline__ float grow(float bm) {
+        const float nm = fmaxf(m, bm);
+        const float z = nm == -INFINITY ? 0.0f : nm;
+        const float df = max_nan((m - z) * kLog2eF, -150.0f), g = lex2(df);
+        const unsigned long long g2 = f2_pack(g, g);
+        T = f2_mul(g2, f2_fma(f2_pack(df, df), S, T));
+        S = f2_mul(S, g2);
+        m = nm;
+        return z;
+    }
+    // two elements, x - z in `d`; `clamp`: they may be far below z, or -inf
+    template <bool CLAMP>
+    __device__ __forceinline__ void add(unsigned long long d) {
+        unsigned long long t = f2_mul(d, f2_pack(kLog2eF, kLog2eF));
+        float2 u = f2_unpack(t);
+        if (CLAMP) {  // (e^d is 0 there, and 0 * inf would not be)
+            u.x = max_nan(u.x, -150.0f);
+            u.y = max_nan(u.y, -150.0f);
+            t = f2_pack(u.x, u.y);
+        }
+        const unsigned long long e = f2_pack(lex2(u.x), lex2(u.y));
+        S = f2_add(S, e);
+        T = f2_fma(t, e, T);
+    }
+    __device__ __forceinline__ Sums sums() const {
+        const float2 s = f2_unpack(S), t = f2_unpack(T);
+        return Sums{m, s.x + s.y, t.x + t.y};
+    }
+};
+
+// 16-bit logits two at a time: the larger (a NaN loses), the larger (a NaN
+// stays), and as floats
+template <typename T>
+struct Two;
+template <>
+struct Two<__nv_bfloat16> {
+    using V = __nv_bfloat162;
+    static __device__ __forceinline__ V of(uint32_t u) { return *reinterpret_cast<const V*>(&u); }
+    static __device__ __forceinline__ V both(float x) { return __bfloat162bfloat162(__float2bfloat16_rd(x)); }
+    static __device__ __forceinline__ float2 floats(V v) {
+        const uint32_t u = *reinterpret_cast<const uint32_t*>(&v);
+        return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+    }
+};
+template <>
+struct Two<__half> {
+    using V = __half2;
+    static __device__ __forceinline__ V of(uint32_t u) { return *reinterpret_cast<const V*>(&u); }
+    static __device__ __forceinline__ V both(float x) { return __half2half2(__float2half_rd(x)); }
+    static __device__ __forceinline__ float2 floats(V v) { return __half22float2(v); }
+};
 
 struct LpShared {
     Sums part[kLpWarps];
     Sums row;                                // this CTA's slice
-    float tmax[kLpThreads];
+    float gmax[kLpGroups];
     float thr;
     int n_above, n_at, n_cand, found;
     int wcount[kLpWarps];
@@ -123,70 +191,100 @@ __device__ void order_top(LpShared& s, int cnt, int k) {
     __syncthreads();
 }
 
+// N chunks of VEC logits added to the sums.
+template <typename T, int VEC, int N>
+__device__ __forceinline__ void add_chunks(const LpPack<T, VEC> (&p)[N], Acc& t) {
+    if constexpr (sizeof(T) == 2 && VEC == 8) {
+        using W = Two<T>;
+        typename W::V v[N * 4];
+#pragma unroll
+        for (int u = 0; u < N; u++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[u * 4 + i] = W::of(reinterpret_cast<const uint32_t*>(p[u].v)[i]);
+        typename W::V mx = v[0];
+#pragma unroll
+        for (int i = 1; i < N * 4; i++) mx = __hmax2(mx, v[i]);
+        const float2 f = W::floats(mx);
+        const float z = t.grow(fmaxf(f.x, f.y));
+        // logits that add nothing are raised to where they still add nothing (-inf among them)
+        const typename W::V low = W::both(z - fmaxf(256.0f, fabsf(z) * 0.015625f));
+        const unsigned long long z2 = f2_pack(-z, -z);
+        if (W::floats(low).x > -INFINITY) {
+#pragma unroll
+            for (int i = 0; i < N * 4; i++) {
+                const float2 x = W::floats(__hmax2_nan(v[i], low));
+                t.template add<false>(f2_add(f2_pack(x.x, x.y), z2));
+            }
+        } else {  // the largest so far is next to the type's lowest value
+#pragma unroll
+            for (int i = 0; i < N * 4; i++) {
+                const float2 x = W::floats(v[i]);
+                t.template add<true>(f2_add(f2_pack(x.x, x.y), z2));
+            }
+        }
+    } else {
+        float f[N * VEC];
+#pragma unroll
+        for (int u = 0; u < N; u++)
+#pragma unroll
+            for (int i = 0; i < VEC; i++) f[u * VEC + i] = lf(p[u].v[i]);
+        float bm = f[0];
+#pragma unroll
+        for (int i = 1; i < N * VEC; i++) bm = fmaxf(bm, f[i]);
+        const float z = t.grow(bm);
+        const unsigned long long z2 = f2_pack(-z, -z);
+#pragma unroll
+        for (int i = 0; i < N * VEC; i += 2)
+            t.template add<true>(f2_add(f2_pack(f[i], i + 1 < N * VEC ? f[i + 1] : -INFINITY), z2));
+    }
+}
+
 // One CTA: the slice [v0, v1) of a row in chunks of VEC logits (the last one
 // cut at n).
 template <typename T, int VEC>
-__device__ __forceinline__ void slice_pass(const T* x, int n, int v0, int v1, Sums& t) {
-    constexpr int U = VEC == 1 ? 4 : 32 / (int)sizeof(T) / VEC * 2;  // chunks in flight
+__device__ __forceinline__ void slice_pass(const T* x, int n, int v0, int v1, Acc& t) {
+    constexpr int U = 4;  // chunks in flight
     using P = LpPack<T, VEC>;
     const int full = min(v1, n / VEC);  // chunks without a cut
-    auto add = [&](const float* f, int cnt) {
-        float bm = f[0];
-#pragma unroll
-        for (int i = 1; i < cnt; i++) bm = fmaxf(bm, f[i]);
-        const float nm = fmaxf(t.m, bm);
-        const float z = nm == -INFINITY ? 0.0f : nm;
-        const float df = max_nan((t.m - z) * kLog2eF, -150.0f);
-        const float g = lex2(df);
-        t.T = g * fmaf(df, t.S, t.T);
-        t.S *= g;
-        t.m = nm;
-#pragma unroll
-        for (int i = 0; i < cnt; i++) {
-            const float d = max_nan((f[i] - z) * kLog2eF, -150.0f);
-            const float e = lex2(d);
-            t.S += e;
-            t.T = fmaf(d, e, t.T);
-        }
-    };
     int v = v0 + (int)threadIdx.x;
     for (; v + (U - 1) * kLpThreads < full; v += U * kLpThreads) {
         P p[U];
 #pragma unroll
         for (int u = 0; u < U; u++) p[u] = *reinterpret_cast<const P*>(x + (int64_t)(v + u * kLpThreads) * VEC);
-        float f[U * VEC];
-#pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-            for (int i = 0; i < VEC; i++) f[u * VEC + i] = lf(p[u].v[i]);
-        add(f, U * VEC);
+        add_chunks<T, VEC, U>(p, t);
     }
     for (; v < full; v += kLpThreads) {
-        const P p = *reinterpret_cast<const P*>(x + (int64_t)v * VEC);
-        float f[VEC];
-#pragma unroll
-        for (int i = 0; i < VEC; i++) f[i] = lf(p.v[i]);
-        add(f, VEC);
+        const P p[1] = {*reinterpret_cast<const P*>(x + (int64_t)v * VEC)};
+        add_chunks<T, VEC, 1>(p, t);
     }
     for (; v < v1; v += kLpThreads)  // the cut chunk
         for (int i = v * VEC; i < n; i++) {
-            const float f = lf(x[i]);
-            add(&f, 1);
+            const LpPack<T, 1> p[1] = {{x[i]}};
+            add_chunks<T, 1, 1>(p, t);
         }
 }
 
-// The k largest of the slice into s.top, from the threads' maxima in s.tmax.
+// The k largest of the slice into s.top, from the threads' maxima `mine`.
 template <typename T, int VEC>
-__device__ __forceinline__ void slice_top(const T* x, int n, int v0, int v1, int k, LpShared& s) {
+__device__ __forceinline__ void slice_top(const T* x, int n, int v0, int v1, int k, float mine, LpShared& s) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const float mine = s.tmax[tid];
+    // the k-th largest of kLpGroups maxima of eight threads each
+    float group = mine;
+#pragma unroll
+    for (int o = 1; o < kLpThreads / kLpGroups; o <<= 1) group = fmaxf(group, __shfl_xor_sync(0xffffffffu, group, o));
+    if (tid % (kLpThreads / kLpGroups) == 0) s.gmax[tid / (kLpThreads / kLpGroups)] = group;
     if (tid == 0) s.n_above = s.n_at = s.n_cand = 0;
-    int above = 0;
-    for (int j = 0; j < kLpThreads; j++) {
-        const float o = s.tmax[j];
-        above += o > mine || (o == mine && j < tid);
+    __syncthreads();
+    if (tid < kLpGroups) {
+        const float g = s.gmax[tid];
+        int above = 0;
+#pragma unroll 8
+        for (int j = 0; j < kLpGroups; j++) {
+            const float o = s.gmax[j];
+            above += o > g || (o == g && j < tid);
+        }
+        if (above == k - 1) s.thr = g;
     }
-    if (above == min(k, kLpThreads) - 1) s.thr = mine;
     __syncthreads();
     const float thr = s.thr;
     if (mine >= thr) {
@@ -268,30 +366,27 @@ __global__ void __launch_bounds__(kLpThreads) logprob_kernel(const __grid_consta
     const int nv = (a.n + VEC - 1) / VEC, per = (nv + C - 1) / C;
     const int v0 = min(nv, rank * per), v1 = min(nv, v0 + per);
 
-    Sums t{-INFINITY, 0.0f, 0.0f};
-    slice_pass<T, VEC>(x, a.n, v0, v1, t);
-    s.tmax[tid] = t.m;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        const Sums p{__shfl_xor_sync(0xffffffffu, t.m, o), __shfl_xor_sync(0xffffffffu, t.S, o),
-                     __shfl_xor_sync(0xffffffffu, t.T, o)};
-        t = join(t, p);
-    }
+    Acc acc;
+    slice_pass<T, VEC>(x, a.n, v0, v1, acc);
+    const Sums t = join_lanes(acc.sums(), 32);
     if (lane == 0) s.part[warp] = t;
     __syncthreads();
-    if (tid == 0) {
-        for (int w = 1; w < kLpWarps; w++) t = join(t, s.part[w]);
-        s.row = t;
+    if (warp == 0) {
+        const Sums u = join_lanes(lane < kLpWarps ? s.part[lane] : Sums{-INFINITY, 0.0f, 0.0f}, kLpWarps);
+        if (lane == 0) s.row = u;
     }
-    if (a.k > 0) slice_top<T, VEC>(x, a.n, v0, v1, a.k, s);
+    if (a.k > 0) slice_top<T, VEC>(x, a.n, v0, v1, a.k, acc.m, s);
     __syncthreads();
 
     if (C > 1) {
         cg::cluster_group cl = cg::this_cluster();
         cl.sync();
         if (rank == 0) {
-            if (tid == 0)
-                for (int r = 1; r < C; r++) s.row = join(s.row, cl.map_shared_rank(&s, r)->row);
+            if (warp == 0) {
+                const Sums u = join_lanes(lane < C ? cl.map_shared_rank(&s, lane)->row : Sums{-INFINITY, 0.0f, 0.0f}, kLpMaxCluster);
+                __syncwarp();
+                if (lane == 0) s.row = u;
+            }
             // the C lists as one, with no empty places
             if (tid == 0) s.n_cand = 0;
             __syncthreads();
@@ -328,8 +423,7 @@ template <typename T>
 cudaError_t go(const LogprobArgs& a, int rows, cudaStream_t s) {
     constexpr int W = 16 / sizeof(T);
     auto kern = a.wide ? logprob_kernel<T, W> : logprob_kernel<T, 1>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(LpShared));
-    if (e != cudaSuccess) return e;
+    static_assert(sizeof(LpShared) <= 48 * 1024, "fits without an attribute");
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(rows * a.cluster));
     cfg.blockDim = dim3(kLpThreads);

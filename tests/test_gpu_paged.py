@@ -632,7 +632,7 @@ def test_logprobs_many_rows():
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("kind", ["zeros", "signed zeros", "two levels", "lowest value", "few allowed", "one allowed", "ascending",
+@pytest.mark.parametrize("kind", ["zeros", "signed zeros", "two levels", "lowest value", "lowest and -inf", "few allowed", "one allowed", "ascending",
                                   "descending", "one thread", "large", "tail"])
 @pytest.mark.parametrize("n", [700, 20011, 131072])
 @pytest.mark.parametrize("rows", [1, 100])
@@ -650,6 +650,9 @@ def test_logprobs_ties_and_masks(dtype, kind, n, rows):
     elif kind == "lowest value":  # a mask of the type's lowest value, seven allowed
         x.fill_(torch.finfo(dt).min)
         x[1 if rows > 1 else 0:, some[:7]] = torch.randn(7, device="cuda", generator=g)  # (row 0 of many: nothing allowed)
+    elif kind == "lowest and -inf":
+        x.fill_(-math.inf)
+        x[:, some[:n // 2]] = torch.finfo(dt).min
     elif kind == "few allowed":
         x.fill_(-math.inf)
         x[:, some[:7]] = torch.randn(rows, 7, device="cuda", generator=g)
