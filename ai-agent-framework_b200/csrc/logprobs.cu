@@ -7,15 +7,14 @@
 // per thread, rescaled when a thread's maximum grows:
 //   m -> m':  S' = S e^(m - m'),  T' = e^(m - m') (T + (m - m') S).
 //
-// Top k without a second pass over the row.  Every thread of the pass ends
-// with the largest logit it saw.  The k-th largest of the maxima of 64 groups
-// of threads is a lower bound of the k-th largest logit, and a logit at or
-// above it can only be in a thread whose maximum is.  A few more than k of the
-// threads' shares are read again (from L2) for their candidates, which are
-// ordered by counting.  Where very
-// many threads tie at the bound (a vocabulary masked with one value), the
-// logits above it come from fewer than k threads, and the ties are taken in
-// index order from the start of the row.
+// Top k without a second pass over the row.  The pass leaves, besides each
+// thread's largest logit, the largest of every 32 that a thread took together
+// (in shared memory, rounded up to bf16).  The k-th largest of the maxima of 64
+// groups of threads is a lower bound of the k-th largest logit; only the 32s
+// whose maximum reaches it, a few more than k of them, are read again (from
+// L2), and their candidates are ordered by counting.  Where very many reach it
+// (a vocabulary masked with one value), the logits above the bound are taken
+// first and the ties in index order from the start of the row.
 //
 // A row's slices go to the CTAs of a cluster, so that few rows still fill the
 // machine; the lists and sums meet in the first CTA's hands over distributed
@@ -36,13 +35,14 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kLpThreads = 512;
+constexpr int kLpThreads = 256;
+constexpr int kLpBatch = 32;                     // logits a thread takes together
+constexpr int kLpEntries = 16;                   // maxima kept by a thread; longer slices: of several batches each
 constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kLpGroups = kLogprobMaxTop;         // groups of threads whose maxima give the bound
 constexpr int kLpMaxCluster = 8;
 constexpr int kLpRound = kLpThreads * 8;         // logits one collecting round may add
 constexpr int kLpCap = kLpRound + 1024;          // candidates held at once
-constexpr int kLpPlainThreads = 128;             // more threads at the bound than this: the ties path
 constexpr float kLog2eF = 1.4426950408889634f;
 constexpr float kLn2F = 0.6931471805599453f;
 
@@ -77,28 +77,35 @@ __device__ __forceinline__ unsigned long long key_of(float x, int i) {
     b = (b & 0x80000000u) ? ~b : b | 0x80000000u;
     return ((unsigned long long)b << 32) | (uint32_t)~i;
 }
+__device__ __forceinline__ float key_value(unsigned long long k) {
+    const uint32_t b = (uint32_t)(k >> 32);
+    return __uint_as_float((b & 0x80000000u) ? b & 0x7fffffffu : ~b);
+}
 __device__ __forceinline__ int key_index(unsigned long long k) { return (int)~(uint32_t)k; }
+
+// the warp's maximum (a NaN loses)
+__device__ __forceinline__ float max_lanes(float x) {
+    float y;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 struct Sums {
     float m, S, T;  // T in units of log 2: sum (x - m) log2(e) e^(x - m)
 };
 
-// b's sums added to a's
-__device__ __forceinline__ Sums join(Sums a, Sums b) {
-    Sums r;
-    r.m = fmaxf(a.m, b.m);
-    const float z = r.m == -INFINITY ? 0.0f : r.m;
-    const float da = max_nan((a.m - z) * kLog2eF, -150.0f), db = max_nan((b.m - z) * kLog2eF, -150.0f);
-    const float fa = lex2(da), fb = lex2(db);
-    r.S = a.S * fa + b.S * fb;
-    r.T = fa * fmaf(da, a.S, a.T) + fb * fmaf(db, b.S, b.T);
-    return r;
+// t with its maximum raised to m
+__device__ __forceinline__ Sums raise(Sums t, float m) {
+    const float d = max_nan((t.m - (m == -INFINITY ? 0.0f : m)) * kLog2eF, -150.0f), f = lex2(d);
+    return Sums{m, t.S * f, f * fmaf(d, t.S, t.T)};
 }
-__device__ __forceinline__ Sums join_lanes(Sums t, int lanes) {
-    for (int o = lanes / 2; o; o >>= 1) {
-        const Sums p{__shfl_xor_sync(0xffffffffu, t.m, o), __shfl_xor_sync(0xffffffffu, t.S, o),
-                     __shfl_xor_sync(0xffffffffu, t.T, o)};
-        t = join(t, p);
+// the warp's sums, in every lane
+__device__ __forceinline__ Sums join_lanes(Sums t) {
+    t = raise(t, max_lanes(t.m));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        t.S += __shfl_xor_sync(0xffffffffu, t.S, o);
+        t.T += __shfl_xor_sync(0xffffffffu, t.T, o);
     }
     return t;
 }
@@ -164,11 +171,12 @@ struct Two<__half> {
 struct LpShared {
     Sums part[kLpWarps];
     Sums row;                                // this CTA's slice
-    float gmax[kLpGroups];
+    __align__(16) float gmax[kLpGroups];
     float thr;
-    int n_above, n_at, n_cand, found;
+    int n_cand, n_list;
+    int list[kLpCap / kLpBatch];
     int wcount[kLpWarps];
-    unsigned short who[kLpThreads];
+    __nv_bfloat16 ent[kLpEntries][kLpThreads];
     unsigned long long top[kLogprobMaxTop];  // this CTA's list, in order
     unsigned long long cand[kLpCap];
 };
@@ -191,9 +199,9 @@ __device__ void order_top(LpShared& s, int cnt, int k) {
     __syncthreads();
 }
 
-// N chunks of VEC logits added to the sums.
+// N chunks of VEC logits added to the sums; returns their maximum.
 template <typename T, int VEC, int N>
-__device__ __forceinline__ void add_chunks(const LpPack<T, VEC> (&p)[N], Acc& t) {
+__device__ __forceinline__ float add_chunks(const LpPack<T, VEC> (&p)[N], Acc& t) {
     if constexpr (sizeof(T) == 2 && VEC == 8) {
         using W = Two<T>;
         typename W::V v[N * 4];
@@ -205,7 +213,7 @@ __device__ __forceinline__ void add_chunks(const LpPack<T, VEC> (&p)[N], Acc& t)
 #pragma unroll
         for (int i = 1; i < N * 4; i++) mx = __hmax2(mx, v[i]);
         const float2 f = W::floats(mx);
-        const float z = t.grow(fmaxf(f.x, f.y));
+        const float bm = fmaxf(f.x, f.y), z = t.grow(bm);
         // logits that add nothing are raised to where they still add nothing (-inf among them)
         const typename W::V low = W::both(z - fmaxf(256.0f, fabsf(z) * 0.015625f));
         const unsigned long long z2 = f2_pack(-z, -z);
@@ -222,6 +230,7 @@ __device__ __forceinline__ void add_chunks(const LpPack<T, VEC> (&p)[N], Acc& t)
                 t.template add<true>(f2_add(f2_pack(x.x, x.y), z2));
             }
         }
+        return bm;
     } else {
         float f[N * VEC];
 #pragma unroll
@@ -236,103 +245,187 @@ __device__ __forceinline__ void add_chunks(const LpPack<T, VEC> (&p)[N], Acc& t)
 #pragma unroll
         for (int i = 0; i < N * VEC; i += 2)
             t.template add<true>(f2_add(f2_pack(f[i], i + 1 < N * VEC ? f[i + 1] : -INFINITY), z2));
+        return bm;
     }
 }
 
-// One CTA: the slice [v0, v1) of a row in chunks of VEC logits (the last one
-// cut at n).
-template <typename T, int VEC>
-__device__ __forceinline__ void slice_pass(const T* x, int n, int v0, int v1, Acc& t) {
-    constexpr int U = 4;  // chunks in flight
-    using P = LpPack<T, VEC>;
-    const int full = min(v1, n / VEC);  // chunks without a cut
-    int v = v0 + (int)threadIdx.x;
-    for (; v + (U - 1) * kLpThreads < full; v += U * kLpThreads) {
-        P p[U];
-#pragma unroll
-        for (int u = 0; u < U; u++) p[u] = *reinterpret_cast<const P*>(x + (int64_t)(v + u * kLpThreads) * VEC);
-        add_chunks<T, VEC, U>(p, t);
+// How a thread's chunks (its i-th is v0 + tid + i kLpThreads) fall to its
+// entries: entry e has the chunks from e * len() on.
+template <int VEC>
+struct Entries {
+    static constexpr int U = kLpBatch / VEC;  // chunks of a batch
+    int agg;                                  // batches of an entry
+
+    __device__ __forceinline__ Entries(int v0, int v1) {
+        const int per = (v1 - v0 + kLpThreads - 1) / kLpThreads, batches = (per + U - 1) / U;
+        agg = max(1, (batches + kLpEntries - 1) / kLpEntries);
     }
+    __device__ __forceinline__ int len() const { return U * agg; }
+};
+
+// One CTA: the slice [v0, v1) of a row in chunks of VEC logits (the last one
+// cut at n).  Returns how many entries this thread wrote.
+template <typename T, int VEC>
+__device__ __forceinline__ int slice_pass(const T* x, int n, int v0, int v1, bool keep, Acc& t, LpShared& s) {
+    constexpr int U = Entries<VEC>::U;
+    using P = LpPack<T, VEC>;
+    const Entries<VEC> en(v0, v1);
+    const int full = min(v1, n / VEC);  // chunks without a cut
+    int left = en.agg, e = 0;
+    float em = -INFINITY;
+    auto put = [&]() { s.ent[e][threadIdx.x] = __float2bfloat16_ru(em); };
+    int v = v0 + (int)threadIdx.x;
+    constexpr int S = U * kLpThreads, B = S - kLpThreads;
+    auto load = [&](P (&p)[U], int at) {
+#pragma unroll
+        for (int u = 0; u < U; u++) p[u] = *reinterpret_cast<const P*>(x + (int64_t)(at + u * kLpThreads) * VEC);
+    };
+    auto work = [&](const P (&p)[U]) {
+        em = fmaxf(em, add_chunks<T, VEC, U>(p, t));
+        if (keep && --left == 0) {
+            put();
+            e++;
+            left = en.agg;
+            em = -INFINITY;
+        }
+    };
+    // (prefetching the next batch costs more in warps than it gains: 96 -> 103 us)
+    for (; v + B < full; v += S) {
+        P p[U];
+        load(p, v);
+        work(p);
+    }
+    const int tail = v;
     for (; v < full; v += kLpThreads) {
         const P p[1] = {*reinterpret_cast<const P*>(x + (int64_t)v * VEC)};
-        add_chunks<T, VEC, 1>(p, t);
+        em = fmaxf(em, add_chunks<T, VEC, 1>(p, t));
     }
     for (; v < v1; v += kLpThreads)  // the cut chunk
         for (int i = v * VEC; i < n; i++) {
             const LpPack<T, 1> p[1] = {{x[i]}};
-            add_chunks<T, 1, 1>(p, t);
+            em = fmaxf(em, add_chunks<T, 1, 1>(p, t));
         }
+    if (keep && (left != en.agg || v != tail)) {  // the last entry is a short one
+        put();
+        e++;
+    }
+    return e;
 }
 
-// The k largest of the slice into s.top, from the threads' maxima `mine`.
-template <typename T, int VEC>
-__device__ __forceinline__ void slice_top(const T* x, int n, int v0, int v1, int k, float mine, LpShared& s) {
+// The CTA's sums into s.part, and the k-th largest of kLpGroups maxima into s.thr.
+__device__ __forceinline__ void slice_sums(const Acc& acc, int k, LpShared& s) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    // the k-th largest of kLpGroups maxima of eight threads each
-    float group = mine;
+    constexpr int GL = kLpThreads / kLpGroups;  // lanes of a group
+    if (tid == 0) s.n_cand = s.n_list = 0;
+    if (k > 1) {
+        float g = acc.m;
 #pragma unroll
-    for (int o = 1; o < kLpThreads / kLpGroups; o <<= 1) group = fmaxf(group, __shfl_xor_sync(0xffffffffu, group, o));
-    if (tid % (kLpThreads / kLpGroups) == 0) s.gmax[tid / (kLpThreads / kLpGroups)] = group;
-    if (tid == 0) s.n_above = s.n_at = s.n_cand = 0;
+        for (int o = 1; o < GL; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+        if (tid % GL == 0) s.gmax[tid / GL] = g;
+    }
+    const Sums t = join_lanes(acc.sums());
+    if (lane == 0) s.part[warp] = t;
     __syncthreads();
-    if (tid < kLpGroups) {
+    if (k == 1 && tid == 0) {
+        float m = s.part[0].m;
+#pragma unroll
+        for (int w = 1; w < kLpWarps; w++) m = fmaxf(m, s.part[w].m);
+        s.thr = m;
+    }
+    if (k > 1 && tid < kLpGroups) {
         const float g = s.gmax[tid];
         int above = 0;
-#pragma unroll 8
-        for (int j = 0; j < kLpGroups; j++) {
-            const float o = s.gmax[j];
-            above += o > g || (o == g && j < tid);
+#pragma unroll
+        for (int j = 0; j < kLpGroups; j += 4) {
+            const float4 o = *reinterpret_cast<const float4*>(s.gmax + j);
+            above += (o.x > g || (o.x == g && j < tid)) + (o.y > g || (o.y == g && j + 1 < tid)) +
+                     (o.z > g || (o.z == g && j + 2 < tid)) + (o.w > g || (o.w == g && j + 3 < tid));
         }
         if (above == k - 1) s.thr = g;
     }
-    __syncthreads();
-    const float thr = s.thr;
-    if (mine >= thr) {
-        if (mine > thr) atomicAdd(&s.n_above, 1);
-        atomicAdd(&s.n_at, 1);
+    if (warp == kLpWarps - 1) {
+        const Sums u = join_lanes(lane < kLpWarps ? s.part[lane] : Sums{-INFINITY, 0.0f, 0.0f});
+        if (lane == 0) s.row = u;
     }
     __syncthreads();
-    const bool plain = s.n_at <= kLpPlainThreads && thr > -INFINITY;
-    const int n_who = plain ? s.n_at : s.n_above;
-    __syncthreads();
-    if (tid == 0) s.found = 0;
-    __syncthreads();
-    if (plain ? mine >= thr : mine > thr) s.who[atomicAdd(&s.found, 1)] = (unsigned short)tid;
-    __syncthreads();
+}
 
-    // the candidates: chunk i of thread who[j] is v0 + who[j] + i * kLpThreads
-    const int per = (v1 - v0 + kLpThreads - 1) / kLpThreads;
-    const int total = n_who * per;
-    unsigned long long bound = 0;  // after a cut of the list: keys at or under it are out
-    for (int base = 0; base < total; base += kLpThreads) {
-        const int c = base + tid;
-        if (c < total) {
-            const int v = v0 + s.who[c / per] + (c % per) * kLpThreads;
-            if (v < v1) {
-                for (int i = v * VEC, e = min(n, v * VEC + VEC); i < e; i++) {
-                    const float f = lf(x[i]);
-                    if (plain ? f >= thr : f > thr) {
-                        const unsigned long long key = key_of(f, i);
-                        if (key > bound) s.cand[atomicAdd(&s.n_cand, 1)] = key;
-                    }
-                }
+// The k largest of the slice into s.top, from the thread's maximum and its
+// `ne` entries.
+template <typename T, int VEC>
+__device__ __forceinline__ void slice_top(const T* x, int n, int v0, int v1, int k, float mine, int ne, LpShared& s) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const Entries<VEC> en(v0, v1);
+    const int most = kLpCap / (en.len() * VEC);  // entries that the list of candidates holds whatever is in them
+    const float thr = s.thr;
+    auto list = [&](bool ties) {  // the entries that reach the bound (or pass it), as first chunks
+        for (int e = 0; e < ne; e++) {
+            const float m = __bfloat162float(s.ent[e][tid]);
+            if (ties ? m >= thr : m > thr) {
+                const int at = atomicAdd(&s.n_list, 1);
+                if (at < most) s.list[at] = tid + e * en.len() * kLpThreads;
             }
         }
         __syncthreads();
-        const int cnt = s.n_cand;
-        if (cnt > kLpCap - kLpRound && base + kLpThreads < total) {
-            order_top(s, cnt, k);
-            for (int i = tid; i < k; i += kLpThreads) s.cand[i] = s.top[i];
-            bound = s.top[k - 1];
-            if (tid == 0) s.n_cand = k;
+        return s.n_list <= most;
+    };
+    const bool plain = list(true) && thr > -INFINITY;
+    bool few = plain;
+    if (!plain) {
+        __syncthreads();
+        if (tid == 0) s.n_list = 0;
+        __syncthreads();
+        few = list(false);
+    }
+    unsigned long long bound = 0;  // after a cut of the list: keys at or under it are out
+    auto take = [&](int v) {
+        if (v >= v1) return;
+        const int i0 = v * VEC;
+        if (i0 + VEC <= n) {
+            const LpPack<T, VEC> p = *reinterpret_cast<const LpPack<T, VEC>*>(x + i0);
+#pragma unroll
+            for (int i = 0; i < VEC; i++) {
+                const float f = lf(p.v[i]);
+                if (plain ? f >= thr : f > thr) {
+                    const unsigned long long key = key_of(f, i0 + i);
+                    if (key > bound) s.cand[atomicAdd(&s.n_cand, 1)] = key;
+                }
+            }
+        } else {
+            for (int i = i0; i < n; i++) {
+                const float f = lf(x[i]);
+                if (plain ? f >= thr : f > thr) {
+                    const unsigned long long key = key_of(f, i);
+                    if (key > bound) s.cand[atomicAdd(&s.n_cand, 1)] = key;
+                }
+            }
+        }
+    };
+    if (few) {  // their chunks, one to a thread
+        for (int i = tid; i < s.n_list * en.len(); i += kLpThreads) {
+            const int q = i / en.len();
+            take(v0 + s.list[q] + (i - q * en.len()) * kLpThreads);
         }
         __syncthreads();
+    } else {  // chunk by chunk, the list cut to the k largest whenever the next might not fit
+        for (int v = v0; v < v1; v += kLpThreads) {
+            if (mine > thr) take(v + tid);
+            __syncthreads();
+            const int cnt = s.n_cand;
+            if (cnt > kLpCap - kLpRound) {
+                order_top(s, cnt, k);
+                for (int i = tid; i < k; i += kLpThreads) s.cand[i] = s.top[i];
+                bound = s.top[k - 1];
+                if (tid == 0) s.n_cand = k;
+            }
+            __syncthreads();
+        }
     }
-    // ties at the bound, in index order
-    if (!plain) {
+    const int cnt0 = s.n_cand;
+    order_top(s, cnt0, k);
+    if (!plain) {  // ties at the bound, in index order
         const int i1 = min(n, v1 * VEC);
-        int cnt = min(s.n_cand, k);  // (fewer than k logits lie above the bound, unless one thread has several)
-        order_top(s, s.n_cand, k);
+        int cnt = min(cnt0, k);
         for (int base = v0 * VEC; base < i1 && cnt < k; base += kLpThreads) {
             const int i = base + tid;
             const bool tie = i < i1 && lf(x[i]) == thr;
@@ -348,8 +441,6 @@ __device__ __forceinline__ void slice_top(const T* x, int n, int v0, int v1, int
             cnt = min(k, cnt + all);
             __syncthreads();
         }
-    } else {
-        order_top(s, s.n_cand, k);
     }
 }
 
@@ -366,24 +457,27 @@ __global__ void __launch_bounds__(kLpThreads) logprob_kernel(const __grid_consta
     const int nv = (a.n + VEC - 1) / VEC, per = (nv + C - 1) / C;
     const int v0 = min(nv, rank * per), v1 = min(nv, v0 + per);
 
-    Acc acc;
-    slice_pass<T, VEC>(x, a.n, v0, v1, acc);
-    const Sums t = join_lanes(acc.sums(), 32);
-    if (lane == 0) s.part[warp] = t;
-    __syncthreads();
-    if (warp == 0) {
-        const Sums u = join_lanes(lane < kLpWarps ? s.part[lane] : Sums{-INFINITY, 0.0f, 0.0f}, kLpWarps);
-        if (lane == 0) s.row = u;
+    // the given tokens' logits, on their way during the pass
+    constexpr int kIds = 2;
+    float given[kIds];
+#pragma unroll
+    for (int j = 0; j < kIds; j++) {
+        const int i = tid + j * kLpThreads;
+        const int id = rank == 0 && i < a.m ? a.ids[row * a.m + i] : -1;
+        given[j] = id >= 0 && id < a.n ? lf(x[id]) : __int_as_float(0x7fc00000);
     }
-    if (a.k > 0) slice_top<T, VEC>(x, a.n, v0, v1, a.k, acc.m, s);
-    __syncthreads();
+
+    Acc acc;
+    const int ne = slice_pass<T, VEC>(x, a.n, v0, v1, a.k > 0, acc, s);
+    slice_sums(acc, a.k, s);
+    if (a.k > 0) slice_top<T, VEC>(x, a.n, v0, v1, a.k, acc.m, ne, s);
 
     if (C > 1) {
         cg::cluster_group cl = cg::this_cluster();
         cl.sync();
         if (rank == 0) {
             if (warp == 0) {
-                const Sums u = join_lanes(lane < C ? cl.map_shared_rank(&s, lane)->row : Sums{-INFINITY, 0.0f, 0.0f}, kLpMaxCluster);
+                const Sums u = join_lanes(lane < C ? cl.map_shared_rank(&s, lane)->row : Sums{-INFINITY, 0.0f, 0.0f});
                 __syncwarp();
                 if (lane == 0) s.row = u;
             }
@@ -406,16 +500,21 @@ __global__ void __launch_bounds__(kLpThreads) logprob_kernel(const __grid_consta
     const float z = r.m == -INFINITY ? 0.0f : r.m;
     auto lp = [&](float v) { return (v - z) - lS; };
     const float nan = __int_as_float(0x7fc00000);
-    for (int i = tid; i < a.m; i += kLpThreads) {
-        const int id = a.ids[row * a.m + i];
-        a.logprob[row * a.m + i] = id >= 0 && id < a.n && r.m != -INFINITY ? lp(lf(x[id])) : nan;
+    for (int i = tid, j = 0; i < a.m; i += kLpThreads, j++) {
+        float v = nan;
+        if (j < kIds) {
+            v = j ? given[kIds - 1] : given[0];
+        } else {
+            const int id = a.ids[row * a.m + i];
+            if (id >= 0 && id < a.n) v = lf(x[id]);
+        }
+        a.logprob[row * a.m + i] = r.m != -INFINITY ? lp(v) : nan;
     }
     if (tid == 0 && a.entropy) a.entropy[row] = lS - r.T / r.S * kLn2F;
     for (int i = tid; i < a.k; i += kLpThreads) {
         const unsigned long long key = s.top[i];
-        const int id = key ? key_index(key) : -1;
-        a.top_ids[row * a.k + i] = id;
-        a.top_logprob[row * a.k + i] = id >= 0 && r.m != -INFINITY ? lp(lf(x[id])) : nan;
+        a.top_ids[row * a.k + i] = key ? key_index(key) : -1;
+        a.top_logprob[row * a.k + i] = key && r.m != -INFINITY ? lp(key_value(key)) : nan;
     }
 }
 
@@ -423,7 +522,8 @@ template <typename T>
 cudaError_t go(const LogprobArgs& a, int rows, cudaStream_t s) {
     constexpr int W = 16 / sizeof(T);
     auto kern = a.wide ? logprob_kernel<T, W> : logprob_kernel<T, 1>;
-    static_assert(sizeof(LpShared) <= 48 * 1024, "fits without an attribute");
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(LpShared));
+    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(rows * a.cluster));
     cfg.blockDim = dim3(kLpThreads);
