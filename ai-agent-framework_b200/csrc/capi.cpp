@@ -662,8 +662,9 @@ int b2_page_plan(const int32_t* cached, const int32_t* fresh, int32_t n_req, int
             return ret(B2_ERR_BAD_ARG, "b2_page_plan: page_size, max_pages and max_tokens must be positive, table_stride >= max_pages");
         int rc = on_device("b2_page_plan", {{"cached", cached}, {"table", table}, {"slots", slots}});
         if (rc != B2_OK) return rc;
-        const b2::PagePlanArgs a{cached, fresh,     free_pages, n_free,    table,     table_stride, lens,      starts,
-                                 slots,  positions, token_req,  info,      n_req,     page_size,    max_pages, max_tokens};
+        const b2::PagePlanArgs a{cached, fresh,     free_pages, n_free, table, table_stride, lens,      starts,
+                                 slots,  positions, token_req,  info,   n_req, page_size,    max_pages, max_tokens,
+                                 0,      0};
         std::string err;
         rc = b2::launch_page_plan(a, static_cast<cudaStream_t>(stream), &err);
         return ret(rc, err);

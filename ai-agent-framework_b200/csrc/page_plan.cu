@@ -24,14 +24,27 @@
 namespace b2 {
 namespace {
 
-constexpr int kPlanThreads = 256;
-constexpr int kPlanWarps = kPlanThreads / 32;
+// Tokens of one lane, 32 apart, so that a warp's stores are whole lines: eight
+// where there are enough to fill the machine, one for a decode step.
+constexpr int kManyTokens = 8;
 
-__device__ __forceinline__ int pages_of(int len, int P) { return len / P + (len % P != 0); }
+constexpr unsigned kSumMax = 0x7fffffffu;
+// sums that stop at kSumMax (which no valid step reaches)
+__device__ __forceinline__ unsigned sat_add(unsigned a, unsigned b) { return min(a + b, kSumMax); }
 
-// The last index r of a[0 .. n] (ascending, a[0] = 0) with a[r] <= x.
-__device__ __forceinline__ int last_le(const int* a, int n, int x) {
-    int lo = 0, hi = n;
+// n / P for 0 <= n < 2^31 (Granlund and Montgomery, "Division by invariant
+// integers using multiplication", 1994): with s = ceil(log2 P) and mul =
+// floor(2^32 (2^s - P) / P) + 1, n / P = (mulhi(mul, n) + n) >> s.
+__device__ __forceinline__ int div_page(const PagePlanArgs& a, int n) {
+    return (int)((__umulhi(a.page_mul, (unsigned)n) + (unsigned)n) >> a.page_shift);
+}
+__device__ __forceinline__ int pages_of(const PagePlanArgs& a, int len) {
+    const int q = div_page(a, len);
+    return q + (q * a.page_size != len);
+}
+
+// The last index r of a[lo .. hi] (ascending, a[lo] <= x) with a[r] <= x.
+__device__ __forceinline__ int last_le(const int* a, int lo, int hi, int x) {
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (a[mid] <= x) lo = mid;
@@ -40,42 +53,54 @@ __device__ __forceinline__ int last_le(const int* a, int n, int x) {
     return lo;
 }
 
+template <int kPlanThreads, int J>
 __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const __grid_constant__ PagePlanArgs a) {
+    constexpr int kPlanWarps = kPlanThreads / 32;
     extern __shared__ int plan_sm[];
     int* start = plan_sm;                // [n_req + 1]
     int* taken = plan_sm + a.n_req + 1;  // [n_req + 1]
-    __shared__ long long wsum[2][kPlanWarps];
+    __shared__ unsigned wsum[2][kPlanWarps];
     __shared__ int wbad[kPlanWarps];
     pdl_trigger();
     pdl_wait();
-    const int R = a.n_req, P = a.page_size, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int R = a.n_req, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per = (R + kPlanThreads - 1) / kPlanThreads;
     const int r0 = min(R, tid * per), r1 = min(R, r0 + per);
+    const int n_free = max(0, *a.n_free);
 
-    // this thread's requests: their tokens and pages (64-bit: the sums of bad lengths must not wrap)
-    long long tok = 0, pg = 0;
-    int bad = 0;
-    for (int r = r0; r < r1; r++) {
-        const int c = a.cached[r], f = a.fresh[r];
-        if (c < 0 || f < 0) {
-            bad |= B2_PLAN_BAD_LENGTH;
-            continue;
+    // this thread's requests: their tokens and pages
+    unsigned tok = 0, pg = 0;
+    int bad = 0, c0 = 0, f0 = 0;  // (the first one's lengths stay at hand)
+    const long long most = min(0x7fffffffLL, (long long)a.max_pages * a.page_size);
+    for (int r = r0; r < r1; r += 4) {
+        int c[4], f[4];  // four requests' loads at once
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            c[k] = r + k < r1 ? a.cached[r + k] : 0;
+            f[k] = r + k < r1 ? a.fresh[r + k] : 0;
         }
-        const long long len = (long long)c + f;
-        if (len > 0x7fffffffLL || (len + P - 1) / P > a.max_pages) {
-            bad |= B2_PLAN_TABLE_FULL;
-            continue;
+        if (r == r0) {
+            c0 = c[0];
+            f0 = f[0];
         }
-        tok += f;
-        pg += pages_of((int)len, P) - pages_of(c, P);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const long long len = (long long)c[k] + f[k];
+            const bool neg = c[k] < 0 || f[k] < 0, wide = len > most;
+            bad |= neg ? B2_PLAN_BAD_LENGTH : wide ? B2_PLAN_TABLE_FULL : 0;
+            if (!neg && !wide) {
+                tok = sat_add(tok, f[k]);
+                pg = sat_add(pg, pages_of(a, (int)len) - pages_of(a, c[k]));
+            }
+        }
     }
-    long long it = tok, ip = pg;  // inclusive over the warp, then over the CTA
+    unsigned it = tok, ip = pg;  // inclusive over the warp, then over the CTA
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long t = __shfl_up_sync(0xffffffffu, it, o), p = __shfl_up_sync(0xffffffffu, ip, o);
+        const unsigned t = __shfl_up_sync(0xffffffffu, it, o), p = __shfl_up_sync(0xffffffffu, ip, o);
         if (lane >= o) {
-            it += t;
-            ip += p;
+            it = sat_add(it, t);
+            ip = sat_add(ip, p);
         }
     }
     if (lane == 31) {
@@ -86,19 +111,19 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const __grid_co
     if (lane == 0) wbad[warp] = bad;
     __syncthreads();
     int status = 0;
-    long long total_tok = 0, total_pg = 0;
+    unsigned total_tok = 0, total_pg = 0;
 #pragma unroll
     for (int w = 0; w < kPlanWarps; w++) {
         if (w == warp) {
-            it += total_tok;
-            ip += total_pg;
+            it = sat_add(it, total_tok);
+            ip = sat_add(ip, total_pg);
         }
-        total_tok += wsum[0][w];
-        total_pg += wsum[1][w];
+        total_tok = sat_add(total_tok, wsum[0][w]);
+        total_pg = sat_add(total_pg, wsum[1][w]);
         status |= wbad[w];
     }
-    if (total_tok > a.max_tokens) status |= B2_PLAN_ROWS_FULL;
-    if (total_pg > max(0, *a.n_free)) status |= B2_PLAN_NO_PAGES;
+    if (total_tok > (unsigned)a.max_tokens || total_tok == kSumMax) status |= B2_PLAN_ROWS_FULL;
+    if (total_pg > (unsigned)n_free || total_pg == kSumMax) status |= B2_PLAN_NO_PAGES;
     const bool ok = status == 0;
     const int T = ok ? (int)total_tok : 0, N = ok ? (int)total_pg : 0;
     if (ok) {
@@ -106,9 +131,9 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const __grid_co
         for (int r = r0; r < r1; r++) {
             start[r] = t;
             taken[r] = p;
-            const int c = a.cached[r], f = a.fresh[r];
+            const int c = r == r0 ? c0 : a.cached[r], f = r == r0 ? f0 : a.fresh[r];
             t += f;
-            p += pages_of(c + f, P) - pages_of(c, P);
+            p += pages_of(a, c + f) - pages_of(a, c);
         }
         if (tid == 0) {
             start[R] = T;
@@ -129,42 +154,75 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const __grid_co
         if (r < R) a.lens[r] = ok ? a.cached[r] + a.fresh[r] : a.cached[r];
     }
     for (int e = gtid; e < N; e += gsize) {
-        const int r = last_le(taken, R, e);
-        a.table[(int64_t)r * a.table_stride + pages_of(a.cached[r], P) + (e - taken[r])] = a.free_pages[e];
+        const int r = last_le(taken, 0, R, e);
+        a.table[(int64_t)r * a.table_stride + pages_of(a, a.cached[r]) + (e - taken[r])] = a.free_pages[e];
     }
-    for (int t = gtid; t < a.max_tokens; t += gsize) {
-        int64_t slot = -1;
-        int pos = 0, req = -1;
-        if (t < T) {
-            req = last_le(start, R, t);
-            const int c = a.cached[req], have = pages_of(c, P);
-            pos = c + (t - start[req]);
-            const int idx = pos / P;
-            // (a page of this step comes from the list: its table entry may be another CTA's to write)
-            const int page = idx < have ? a.table[(int64_t)req * a.table_stride + idx] : a.free_pages[taken[req] + idx - have];
-            if (page >= 0) slot = (int64_t)page * P + pos % P;
+    // a warp: J runs of 32 tokens
+    const long long wstep = (long long)(gsize / 32) * (32 * J);
+    for (long long t0 = (long long)(gtid / 32) * (32 * J); t0 < a.max_tokens; t0 += wstep) {
+        int lo = 0, hi = R;
+        if (J > 1 && t0 < T) {  // the requests of its first and last token bound the others'
+            const int t = (int)min(lane ? t0 + 32 * J - 1 : t0, (long long)T - 1);
+            const int r = lane < 2 ? last_le(start, 0, R, t) : 0;
+            lo = __shfl_sync(0xffffffffu, r, 0);
+            hi = __shfl_sync(0xffffffffu, r, 1);
         }
-        a.slots[t] = slot;
-        a.positions[t] = pos;
-        a.token_req[t] = req;
+        int pos[J], req[J], in[J], page[J];
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+            const long long t = t0 + 32 * j + lane;
+            pos[j] = in[j] = 0;
+            req[j] = page[j] = -1;
+            if (t < T) {
+                const int r = last_le(start, lo, hi, (int)t), c = a.cached[r];
+                pos[j] = c + ((int)t - start[r]);
+                const int idx = div_page(a, pos[j]), have = pages_of(a, c);
+                in[j] = pos[j] - idx * a.page_size;
+                req[j] = r;
+                // (a page of this step comes from the list: its table entry may be another CTA's to write)
+                page[j] = *(idx < have ? a.table + ((int64_t)r * a.table_stride + idx) : a.free_pages + (taken[r] + idx - have));
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+            const long long t = t0 + 32 * j + lane;
+            if (t < a.max_tokens) {
+                a.slots[t] = page[j] >= 0 ? (int64_t)page[j] * a.page_size + in[j] : -1;
+                a.positions[t] = pos[j];
+                a.token_req[t] = req[j];
+            }
+        }
     }
 }
 
 }  // namespace
 
-int launch_page_plan(const PagePlanArgs& a, cudaStream_t s, std::string* err) {
+template <int THREADS, int J>
+static cudaError_t go_plan(const PagePlanArgs& a, int sms, cudaStream_t s) {
+    const int smem = (int)(2 * sizeof(int) * ((size_t)a.n_req + 1));
+    if (smem > 47 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(page_plan_kernel<THREADS, J>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   (int)(2 * sizeof(int) * (kPlanMaxReq + 1)));
+        if (e != cudaSuccess) return e;
+    }
+    const long long work = std::max<long long>(((long long)a.max_tokens + J - 1) / J, a.n_req);
+    const int grid = (int)std::max<long long>(1, std::min<long long>(1024 / THREADS * sms, (work + THREADS - 1) / THREADS));
+    return launch_pdl(page_plan_kernel<THREADS, J>, dim3(grid), dim3(THREADS), smem, s, a);
+}
+
+int launch_page_plan(const PagePlanArgs& args, cudaStream_t s, std::string* err) {
+    PagePlanArgs a = args;
     const int sms = current_sms(err);
     if (!sms) return B2_ERR_CUDA;
-    const int smem = (int)(2 * sizeof(int) * ((size_t)a.n_req + 1));
-    if (smem > 48 * 1024 &&
-        cudaFuncSetAttribute(page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)(2 * sizeof(int) * (kPlanMaxReq + 1))) != cudaSuccess) {
-        *err = "page plan: shared memory attribute";
-        return B2_ERR_CUDA;
-    }
-    const long long work = std::max<long long>(a.max_tokens, a.n_req);
-    const int grid = (int)std::max<long long>(1, std::min<long long>(2 * sms, (work + kPlanThreads - 1) / kPlanThreads));
-    const cudaError_t e = launch_pdl(page_plan_kernel, dim3(grid), dim3(kPlanThreads), smem, s, a);
+    const unsigned P = (unsigned)a.page_size;
+    int sh = 0;
+    while ((1ull << sh) < P) sh++;
+    a.page_shift = sh;
+    a.page_mul = (unsigned)((((1ull << sh) - P) << 32) / P + 1);
+    // every CTA scans all requests: more threads for many of them
+    const bool many = a.max_tokens > 512 * sms;
+    const cudaError_t e = a.n_req > 1024 ? (many ? go_plan<1024, kManyTokens>(a, sms, s) : go_plan<1024, 1>(a, sms, s))
+                                         : (many ? go_plan<256, kManyTokens>(a, sms, s) : go_plan<256, 1>(a, sms, s));
     if (e != cudaSuccess) {
         *err = std::string("page plan launch: ") + cudaGetErrorString(e);
         return B2_ERR_CUDA;

@@ -33,6 +33,9 @@ struct PagePlanArgs {
     int32_t* token_req;        // [max_tokens]
     int32_t* info;             // [4]
     int32_t n_req, page_size, max_pages, max_tokens;
+    // set by launch_page_plan: division by the page size
+    uint32_t page_mul;
+    int32_t page_shift;
 };
 
 int launch_page_plan(const PagePlanArgs& a, cudaStream_t s, std::string* err);
