@@ -890,11 +890,7 @@ int launch_attention_paged(const b2_paged_kv& kv, const b2_paged_attn_opts& o, c
     const cudaError_t e = kv.hd <= 64    ? go_hd<64>(a, o.dtype, kv.dtype, s)
                           : kv.hd <= 128 ? go_hd<128>(a, o.dtype, kv.dtype, s)
                                          : go_hd<256>(a, o.dtype, kv.dtype, s);
-    if (e != cudaSuccess) {
-        *err = std::string("paged attention launch: ") + cudaGetErrorString(e);
-        return B2_ERR_CUDA;
-    }
-    return B2_OK;
+    return e == cudaSuccess ? B2_OK : cuda_failed("paged attention launch", e, err);
 }
 
 }  // namespace b2

@@ -58,14 +58,13 @@ auto guarded(F&& body) noexcept -> decltype(body()) {
 
 bool float_type(int32_t t) { return t == 0 || t == 1 || t == 30; }
 
-int on_device(const char* who, std::initializer_list<std::pair<const char*, const void*>> ptrs) {
+int on_device(const char* who, std::initializer_list<b2::DevicePtr> ptrs) {
     std::string err;
-    for (const auto& p : ptrs) {
-        const int rc = b2::check_device_pointer(p.second, p.first, &err);
-        if (rc != B2_OK) return ret(rc, std::string(who) + ": " + err);
-    }
-    return B2_OK;
+    const int rc = b2::check_device_pointers(ptrs.begin(), (int)ptrs.size(), &err);
+    return rc == B2_OK ? rc : ret(rc, std::string(who) + ": " + err);
 }
+
+size_t type_bytes(int32_t t) { return t == 0 ? 4 : 2; }
 
 // Checks a paged cache's description and fills in dense strides.
 int paged_kv_args(const char* who, const b2_paged_kv* kv, b2_paged_kv* out) {
@@ -86,8 +85,6 @@ int paged_kv_args(const char* who, const b2_paged_kv* kv, b2_paged_kv* out) {
     if (out->page_stride < 0 || out->pos_stride < 0 || out->head_stride < 0 ||
         (out->page_stride | out->pos_stride | out->head_stride) % 8)
         return ret(B2_ERR_BAD_ARG, w + ": the cache's strides must be multiples of 8, not negative");
-    if ((reinterpret_cast<uintptr_t>(kv->k) | reinterpret_cast<uintptr_t>(kv->v)) & 15)
-        return ret(B2_ERR_BAD_ARG, w + ": k and v must be 16-byte aligned");
     return B2_OK;
 }
 
@@ -660,7 +657,10 @@ int b2_page_plan(const int32_t* cached, const int32_t* fresh, int32_t n_req, int
             return ret(B2_ERR_BAD_ARG, "b2_page_plan: takes 1 to 16384 requests");
         if (page_size <= 0 || max_pages <= 0 || max_tokens <= 0 || table_stride < max_pages)
             return ret(B2_ERR_BAD_ARG, "b2_page_plan: page_size, max_pages and max_tokens must be positive, table_stride >= max_pages");
-        int rc = on_device("b2_page_plan", {{"cached", cached}, {"table", table}, {"slots", slots}});
+        int rc = on_device("b2_page_plan", {{"cached", cached, 4}, {"fresh", fresh, 4}, {"free_pages", free_pages, 4},
+                                            {"n_free", n_free, 4}, {"table", table, 4}, {"lens", lens, 4},
+                                            {"starts", starts, 4}, {"slots", slots, 8}, {"positions", positions, 4},
+                                            {"token_req", token_req, 4}, {"info", info, 4}});
         if (rc != B2_OK) return rc;
         const b2::PagePlanArgs a{cached, fresh,     free_pages, n_free, table, table_stride, lens,      starts,
                                  slots,  positions, token_req,  info,   n_req, page_size,    max_pages, max_tokens,
@@ -695,7 +695,9 @@ int b2_rope(const b2_rope_rows* rows, const double* freqs, const int32_t* positi
         if (!positions || (!freqs && r.rot_dim) || n_tok <= 0 || !q != !q_out || !k != !k_out || (!q && !k))
             return ret(B2_ERR_BAD_ARG, "b2_rope: null argument or no tokens");
         if ((q && r.nh <= 0) || (k && r.nkv <= 0)) return ret(B2_ERR_BAD_ARG, "b2_rope: bad heads");
-        rc = on_device("b2_rope", {{"q", q}, {"k", k}, {"q_out", q_out}, {"k_out", k_out}, {"positions", positions}});
+        const size_t es = type_bytes(r.dtype);
+        rc = on_device("b2_rope", {{"q", q, es}, {"k", k, es}, {"q_out", q_out, es}, {"k_out", k_out, es},
+                                   {"positions", positions, 4}, {"freqs", r.rot_dim ? freqs : nullptr, 8}});
         if (rc != B2_OK) return rc;
         std::string err;
         rc = b2::launch_rope(r, nullptr, freqs, positions, nullptr, n_tok, q, k, nullptr, q_out, k_out,
@@ -720,7 +722,10 @@ int b2_rope_append(const b2_rope_rows* rows, const b2_paged_kv* kv, const double
             return ret(B2_ERR_BAD_ARG, "b2_rope_append: the rows' heads do not match the cache's");
         if (r.dtype != 0 && r.dtype != c.dtype)
             return ret(B2_ERR_UNSUPPORTED_TYPE, "b2_rope_append: rows must be F32 or of the cache's type");
-        rc = on_device("b2_rope_append", {{"q", q}, {"k", k}, {"v", v}, {"q_out", q_out}, {"the cache", c.k}, {"slots", slots}});
+        const size_t es = type_bytes(r.dtype);
+        rc = on_device("b2_rope_append", {{"q", q, es}, {"k", k, es}, {"v", v, es}, {"q_out", q_out, es},
+                                          {"the cache's k", c.k, 16}, {"the cache's v", c.v, 16}, {"slots", slots, 8},
+                                          {"positions", positions, 4}, {"freqs", r.rot_dim ? freqs : nullptr, 8}});
         if (rc != B2_OK) return rc;
         std::string err;
         rc = b2::launch_rope(r, &c, freqs, positions, slots, n_tok, q, k, v, q_out, nullptr,
@@ -760,9 +765,10 @@ int b2_attention_paged(const b2_paged_kv* kv, const b2_paged_attn_opts* opts, co
         if (o.window < 0 || !(o.scale >= 0.0f) || !(o.softcap >= 0.0f) || std::isinf(o.scale) || std::isinf(o.softcap) ||
             o.q_stride < 0 || (o.out_stride && o.out_stride < qd) || (o.table_stride && o.table_stride < o.max_pages))
             return ret(B2_ERR_BAD_ARG, "b2_attention_paged: bad window, scale, softcap or stride");
-        if (reinterpret_cast<uintptr_t>(d_scratch) & 15)
-            return ret(B2_ERR_BAD_ARG, "b2_attention_paged: scratch must be 16-byte aligned");
-        rc = on_device("b2_attention_paged", {{"q", q}, {"the cache", c.k}, {"table", table}, {"out", out}, {"scratch", d_scratch}});
+        const size_t es = type_bytes(o.dtype);
+        rc = on_device("b2_attention_paged", {{"q", q, es}, {"the cache's k", c.k, 16}, {"the cache's v", c.v, 16},
+                                              {"table", table, 4}, {"lens", lens, 4}, {"req", req, 4}, {"out", out, es},
+                                              {"lse", lse, 4}, {"slopes", o.slopes, 4}, {"scratch", d_scratch, 16}});
         if (rc != B2_OK) return rc;
         std::string err;
         rc = b2::launch_attention_paged(c, o, q, table, lens, req, batch, out, lse, d_scratch,
@@ -781,8 +787,9 @@ int b2_logprobs(const void* logits, int32_t dtype, int32_t n, int32_t rows, int6
         if ((m && (!ids || !logprob)) || (k && (!top_ids || !top_logprob)))
             return ret(B2_ERR_BAD_ARG, "b2_logprobs: null argument");
         if (!m && !k && !entropy) return B2_OK;
-        int rc = on_device("b2_logprobs", {{"logits", logits}, {"ids", m ? ids : nullptr}, {"logprob", m ? logprob : nullptr},
-                                           {"entropy", entropy}, {"top_ids", k ? top_ids : nullptr}});
+        int rc = on_device("b2_logprobs", {{"logits", logits, type_bytes(dtype)}, {"ids", m ? ids : nullptr, 4},
+                                           {"logprob", m ? logprob : nullptr, 4}, {"entropy", entropy, 4},
+                                           {"top_ids", k ? top_ids : nullptr, 4}, {"top_logprob", k ? top_logprob : nullptr, 4}});
         if (rc != B2_OK) return rc;
         std::string err;
         rc = b2::launch_logprobs(logits, dtype, n, rows, ld, ids, m, logprob, entropy, k, top_ids, top_logprob,

@@ -567,11 +567,7 @@ int launch_logprobs(const void* logits, int dtype, int n, int rows, int64_t ld, 
     const cudaError_t e = dtype == 0   ? go<float>(a, rows, s)
                           : dtype == 1 ? go<__half>(a, rows, s)
                                        : go<__nv_bfloat16>(a, rows, s);
-    if (e != cudaSuccess) {
-        *err = std::string("log probabilities launch: ") + cudaGetErrorString(e);
-        return B2_ERR_CUDA;
-    }
-    return B2_OK;
+    return e == cudaSuccess ? B2_OK : cuda_failed("log probabilities launch", e, err);
 }
 
 }  // namespace b2

@@ -223,11 +223,7 @@ int launch_page_plan(const PagePlanArgs& args, cudaStream_t s, std::string* err)
     const bool many = a.max_tokens > 512 * sms;
     const cudaError_t e = a.n_req > 1024 ? (many ? go_plan<1024, kManyTokens>(a, sms, s) : go_plan<1024, 1>(a, sms, s))
                                          : (many ? go_plan<256, kManyTokens>(a, sms, s) : go_plan<256, 1>(a, sms, s));
-    if (e != cudaSuccess) {
-        *err = std::string("page plan launch: ") + cudaGetErrorString(e);
-        return B2_ERR_CUDA;
-    }
-    return B2_OK;
+    return e == cudaSuccess ? B2_OK : cuda_failed("page plan launch", e, err);
 }
 
 }  // namespace b2

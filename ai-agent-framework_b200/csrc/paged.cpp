@@ -28,20 +28,32 @@ int current_sms(std::string* err) {
     return n;
 }
 
-int check_device_pointer(const void* p, const char* what, std::string* err) {
-    if (!p) return B2_OK;
-    cudaPointerAttributes at{};
+int check_device_pointers(const DevicePtr* p, int n, std::string* err) {
+    for (int i = 0; i < n; i++)
+        if (reinterpret_cast<uintptr_t>(p[i].p) & (p[i].align - 1)) {
+            *err = std::string(p[i].name) + " must be " + std::to_string(p[i].align) + "-byte aligned";
+            return B2_ERR_BAD_ARG;
+        }
     int dev = -1;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaPointerGetAttributes(&at, p) != cudaSuccess) {
-        cudaGetLastError();
-        *err = "no CUDA device";
-        return B2_ERR_CUDA;
+    cudaError_t e = cudaGetDevice(&dev);
+    for (int i = 0; i < n && e == cudaSuccess; i++) {
+        if (!p[i].p) continue;
+        cudaPointerAttributes at{};
+        e = cudaPointerGetAttributes(&at, p[i].p);
+        if (e != cudaSuccess) break;
+        if (at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeDevice && at.device == dev)) continue;
+        *err = std::string(p[i].name) + (at.type == cudaMemoryTypeDevice
+                                             ? " is on device " + std::to_string(at.device) + ", the current device is " + std::to_string(dev)
+                                             : std::string(" is not device memory"));
+        return B2_ERR_BAD_ARG;
     }
-    if (at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeDevice && at.device == dev)) return B2_OK;
-    *err = std::string(what) + (at.type == cudaMemoryTypeDevice ? " is on device " + std::to_string(at.device) +
-                                                                      ", the current device is " + std::to_string(dev)
-                                                                : std::string(" is not device memory"));
-    return B2_ERR_BAD_ARG;
+    return e == cudaSuccess ? B2_OK : cuda_failed("no CUDA device", e, err);
+}
+
+int cuda_failed(const char* what, cudaError_t e, std::string* err) {
+    cudaGetLastError();  // reported here: not again to the caller's next CUDA call
+    *err = std::string(what) + ": " + cudaGetErrorString(e);
+    return B2_ERR_CUDA;
 }
 
 }  // namespace b2

@@ -1,9 +1,8 @@
 // Kernels of a paged serving step: block tables and slot maps (page_plan.cu),
 // rotary positions and cache writes (rope.cu), attention over the paged cache
-// (attention_paged.cu), log probabilities (logprobs.cu).  Each function
-// checks what only the device can tell (alignment, pointers' device), launches
-// on `s` and returns a B2_* code; the arguments' ranges are checked by the
-// exported entry points.
+// (attention_paged.cu), log probabilities (logprobs.cu).  Each launch_*
+// function works on `s` and returns a B2_* code; the exported entry points
+// check the arguments first.
 #pragma once
 #include <cuda_runtime.h>
 #include <stddef.h>
@@ -57,9 +56,18 @@ int launch_logprobs(const void* logits, int dtype, int n, int rows, int64_t ld, 
 // The current device's SM count, looked up once per device; 0 without one.
 int current_sms(std::string* err);
 
-// B2_OK when p is null or memory that kernels on the current device may
-// address (its own, or managed); B2_ERR_BAD_ARG for host memory and for
-// another device's.
-int check_device_pointer(const void* p, const char* what, std::string* err);
+// A pointer argument: its name in messages and its alignment (a power of two).
+struct DevicePtr {
+    const char* name;
+    const void* p;
+    size_t align;
+};
+// B2_OK when every pointer is null or aligned memory that kernels on the
+// current device may address (its own, or managed); B2_ERR_BAD_ARG otherwise,
+// for host memory and another device's among them.
+int check_device_pointers(const DevicePtr* p, int n, std::string* err);
+
+// The message of a failed CUDA call; returns B2_ERR_CUDA.
+int cuda_failed(const char* what, cudaError_t e, std::string* err);
 
 }  // namespace b2

@@ -261,11 +261,7 @@ int launch_rope(const b2_rope_rows& d, const b2_paged_kv* kv, const double* freq
         e = go<__half, __half>(a, wide, sms, s);
     else
         e = go<__nv_bfloat16, __nv_bfloat16>(a, wide, sms, s);
-    if (e != cudaSuccess) {
-        *err = std::string("rope launch: ") + cudaGetErrorString(e);
-        return B2_ERR_CUDA;
-    }
-    return B2_OK;
+    return e == cudaSuccess ? B2_OK : cuda_failed("rope launch", e, err);
 }
 
 }  // namespace b2

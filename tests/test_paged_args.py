@@ -102,6 +102,31 @@ def test_attention_paged_null_refusals(built_lib):
         refused(-8, "scratch", b2.attention_paged_scratch_bytes, *a)
 
 
+ODD = P + 1
+
+
+def test_misaligned_pointers(built_lib):
+    """Addresses that the element types do not allow, told before any of them is used."""
+    for name in ("cached", "fresh", "free_pages", "n_free", "table", "lens", "starts", "slots", "positions", "token_req", "info"):
+        refused(-8, "aligned", b2.page_plan, **{**PLAN, name: ODD})
+    refused(-8, "aligned", b2.page_plan, **{**PLAN, "slots": P + 4})
+    for name in ("freqs", "positions", "q", "k", "q_out", "k_out"):
+        a = dict(freqs=P, positions=P, n_tok=3, q=P, k=P, q_out=P, k_out=P)
+        refused(-8, "aligned", b2.rope, b2.rope_rows(**ROWS), **{**a, name: ODD})
+    refused(-8, "aligned", b2.rope, b2.rope_rows(**{**ROWS, "dtype": b2.F32}), P, P, 3, q=P + 2, q_out=P)
+    for i in (2, 3, 4, 6, 7, 8, 9):
+        a = [b2.rope_rows(**ROWS), kv(), P, P, P, 3, P, P, P, P]
+        a[i] = ODD
+        refused(-8, "aligned", b2.rope_append, *a)
+    for i in (2, 3, 4, 5, 7, 8, 9):
+        a = [kv(), b2.paged_attn_opts(**OPTS), P, P, P, P, 4, P, P, P]
+        a[i] = ODD
+        refused(-8, "aligned", b2.attention_paged, *a)
+    refused(-8, "aligned", b2.attention_paged, kv(), b2.paged_attn_opts(**OPTS, slopes=ODD), P, P, P, 0, 4, P, 0, P)
+    for name in ("logits", "ids", "logprob", "entropy", "top_ids", "top_logprob"):
+        refused(-8, "aligned", b2.logprobs, **{**LOGP, name: ODD})
+
+
 LOGP = dict(logits=P, dtype=b2.F32, n=100, rows=2, ld=100, ids=P, m=1, logprob=P, entropy=P, k=5, top_ids=P, top_logprob=P)
 
 
