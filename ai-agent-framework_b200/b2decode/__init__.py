@@ -148,6 +148,7 @@ SIGNATURES = {
     "b2_batch_prefill": (C.c_int, [_P, _i32, _i32p, _i32, C.POINTER(_i32)]),
     "b2_batch_step": (C.c_int, [_P, _i32p, _i32p]),
     "b2_batch_logits": (C.c_int, [_P, _f32p]),
+    "b2_batch_logprobs": (C.c_int, [_P, _i32, _i32p, _i32, _f32p, _f32p, _i32, _i32p, _f32p]),
     "b2_batch_use_graph": (C.c_int, [_P, _i32]),
     "b2_attention_decode": (C.c_int, [_P, _P, _P, _P, _i32, _i32, _i32, _i32, _i32, _P]),
     "b2_attention_decode_noalloc": (C.c_int, [_P, _P, _P, _P, _i32, _i32, _i32, _i32, _i32, _P]),
@@ -429,6 +430,21 @@ class Batch:
         out = np.empty((self.batch, self.vocab), dtype=np.float32)
         _check(lib().b2_batch_logits(self._h, out.ctypes.data_as(_f32p)))
         return out
+
+    def logprobs(self, ids, top: int = 0) -> tuple:
+        """Scores of the last forward's rows (b2_batch_logprobs): ids [rows][m],
+        one row per slot after a step, one row after a prefill.  Returns (log p
+        of the ids, entropy, the `top` best ids, their log p)."""
+        a = np.ascontiguousarray(np.asarray(ids, dtype=np.int32))
+        if a.ndim != 2:
+            raise ValueError("ids: one row of ids per row of logits")
+        rows, m = a.shape
+        lp, ent = np.empty((rows, m), np.float32), np.empty(rows, np.float32)
+        ti, tl = np.empty((rows, top), np.int32), np.empty((rows, top), np.float32)
+        _check(lib().b2_batch_logprobs(self._h, rows, a.ctypes.data_as(_i32p), m, lp.ctypes.data_as(_f32p),
+                                       ent.ctypes.data_as(_f32p), int(top), ti.ctypes.data_as(_i32p),
+                                       tl.ctypes.data_as(_f32p)))
+        return lp, ent, ti, tl
 
     def close(self) -> None:
         if self._h:

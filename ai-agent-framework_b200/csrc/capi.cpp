@@ -30,6 +30,9 @@ int b2_batch_prefill_impl(b2_batch* bt, int slot, const int32_t* prompt, int n, 
 int b2_batch_step_impl(b2_batch* bt, const int32_t* tokens, int32_t* next_out, std::string* err);
 int b2_batch_logits_impl(const b2_batch* bt, float* out, std::string* err);
 int b2_batch_use_graph_impl(b2_batch* bt, int on);
+int b2_batch_logprobs_impl(const b2_batch* bt, int rows, const int32_t* ids, int m, float* logprob, float* entropy, int k,
+                           int32_t* top_ids, float* top_logprob, std::string* err);
+int b2_batch_size(const b2_batch* bt);
 int b2_rope_freqs_impl(const b2_rope_opts& o, double* freqs, float* scale);
 int b2_attention_impl(const float* q, const uint16_t* k, const uint16_t* v, float* out, int batch, int nh, int nkv,
                       int hd, int ctx, cudaStream_t s, std::string* err);
@@ -634,6 +637,18 @@ int b2_batch_logits(const b2_batch* b, float* out) {
     if (!out) return ret(B2_ERR_BAD_ARG, "null argument");
     std::string err;
     return ret(b2_batch_logits_impl(b, out, &err), err);
+}
+
+int b2_batch_logprobs(const b2_batch* b, int32_t rows, const int32_t* ids, int32_t m, float* logprob, float* entropy,
+                      int32_t k, int32_t* top_ids, float* top_logprob) {
+    return guarded([&] {
+        if (!b) return ret(B2_ERR_NOT_LOADED, "no batch");
+        if (rows <= 0 || rows > b2_batch_size(b) || m < 0 || k < 0 || k > b2::kLogprobMaxTop || (m && (!ids || !logprob)) ||
+            (k && (!top_ids || !top_logprob)))
+            return ret(B2_ERR_BAD_ARG, "b2_batch_logprobs: bad argument");
+        std::string err;
+        return ret(b2_batch_logprobs_impl(b, rows, ids, m, logprob, entropy, k, top_ids, top_logprob, &err), err);
+    });
 }
 
 int b2_attention_decode(const float* q, const uint16_t* k, const uint16_t* v, float* out, int32_t batch, int32_t nh,

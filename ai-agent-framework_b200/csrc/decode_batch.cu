@@ -23,7 +23,9 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
+#include <cstring>
 #include <string>
 #include <vector>
 
@@ -31,6 +33,7 @@
 #include "dev.cuh"
 #include "gemm.h"
 #include "model.h"
+#include "paged.h"
 
 int b2_tiled_matvec_batch_impl(int qtype, const void* base, int64_t rp, int64_t row0, int rows, int cols,
                                const float* x, float* y, int nvec, cudaStream_t s, std::string* err);
@@ -946,6 +949,8 @@ int b2_batch_use_graph_impl(b2_batch* bt, int on) {
     return B2_OK;
 }
 
+int b2_batch_size(const b2_batch* bt) { return bt->B; }
+
 // Logits of the last step, [B][vocab] floats.
 int b2_batch_logits_impl(const b2_batch* bt, float* out, std::string* err) {
     const size_t n = (size_t)bt->B * bt->m->dev.V;
@@ -953,5 +958,42 @@ int b2_batch_logits_impl(const b2_batch* bt, float* out, std::string* err) {
             "logits") ||
         !ok(cudaStreamSynchronize(bt->m->stream), err, "logits"))
         return B2_ERR_CUDA;
+    return B2_OK;
+}
+
+// Scores of the first `rows` rows of the last forward's logits: host arrays in
+// and out, the work on the model's stream, with a buffer allocated on the
+// stream for the call (the ids, then the four results).
+int b2_batch_logprobs_impl(const b2_batch* bt, int rows, const int32_t* ids, int m, float* logprob, float* entropy, int k,
+                           int32_t* top_ids, float* top_logprob, std::string* err) {
+    cudaStream_t s = bt->m->stream;
+    const size_t nm = (size_t)rows * m, nk = (size_t)rows * k, n = 2 * nm + rows + 2 * nk;
+    if (k > bt->m->dev.V) {
+        *err = "more alternatives than the vocabulary has";
+        return B2_ERR_BAD_ARG;
+    }
+    std::vector<int32_t> host(n);
+    std::copy(ids, ids + nm, host.begin());
+    int32_t* d = nullptr;
+    if (!ok(cudaMallocAsync(&d, n * sizeof(int32_t), s), err, "scores buffer")) return B2_ERR_OOM;
+    float* d_lp = reinterpret_cast<float*>(d + nm);
+    float* d_ent = d_lp + nm;
+    int32_t* d_ti = reinterpret_cast<int32_t*>(d_ent + rows);
+    float* d_tl = reinterpret_cast<float*>(d_ti + nk);
+    int rc = nm && !ok(cudaMemcpyAsync(d, host.data(), nm * sizeof(int32_t), cudaMemcpyHostToDevice, s), err, "ids") ? B2_ERR_CUDA : B2_OK;
+    if (rc == B2_OK)
+        rc = launch_logprobs(bt->logits, 0, bt->m->dev.V, rows, bt->m->dev.V, d, m, d_lp, d_ent, k, d_ti, d_tl, s, err);
+    if (rc == B2_OK && !ok(cudaMemcpyAsync(host.data() + nm, d + nm, (n - nm) * sizeof(int32_t), cudaMemcpyDeviceToHost, s), err, "scores"))
+        rc = B2_ERR_CUDA;
+    cudaFreeAsync(d, s);
+    if (!ok(cudaStreamSynchronize(s), err, "scores") && rc == B2_OK) rc = B2_ERR_CUDA;
+    if (rc != B2_OK) return rc;
+    const int32_t* h = host.data() + nm;
+    if (nm) memcpy(logprob, h, nm * sizeof(float));
+    if (entropy) memcpy(entropy, h + nm, rows * sizeof(float));
+    if (nk) {
+        memcpy(top_ids, h + nm + rows, nk * sizeof(int32_t));
+        memcpy(top_logprob, h + nm + rows + nk, nk * sizeof(float));
+    }
     return B2_OK;
 }

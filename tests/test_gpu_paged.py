@@ -708,6 +708,33 @@ def test_logprobs_outputs_left_out_and_graph():
         logp_check(x, 9000, ids, 5, lp, H, ti, tl)
 
 
+@pytest.mark.parametrize("graph", [False, True])
+def test_batch_scores(built_lib, write_model, graph):
+    """The batched decode's own logits, scored in place: equal to the scores of the copied logits."""
+    from b2decode import gguf_writer as gw
+    shape = gw.ModelShape("qwen2", 256, 2, 4, 2, 512, 512, 256, 1e-6, 1e6, True, True, "q8_0", 1, 2)
+    m = b2.Model(write_model("qwen2-hd64-q8", shape), num_ctx=64)
+    bt = b2.Batch(m, 3)
+    bt.use_graph(graph)
+    nxt = [bt.prefill(i, [1, 5 + i, 9]) for i in range(3)]
+    first = bt.logprobs([[nxt[2], 3]], 5)  # after a prefill: its last token
+    x = torch.from_numpy(bt.logits()[:1]).cuda()
+    check = lambda x, ids, r: logp_check(x, 512, i32(ids), r[2].shape[1], *(torch.from_numpy(t).cuda() for t in r))  # noqa: E731
+    check(x, [[nxt[2], 3]], first)
+    assert first[2][0, 0] == nxt[2]
+    for _ in range(4):
+        nxt = bt.step(nxt)
+        got = bt.logprobs(np.asarray(nxt)[:, None], 4)
+        check(torch.from_numpy(bt.logits()).cuda(), np.asarray(nxt)[:, None], got)
+        assert np.array_equal(got[2][:, 0], nxt) and np.array_equal(got[0][:, 0], got[3][:, 0])
+    assert bt.logprobs(np.zeros((3, 0)), 0)[1].shape == (3,)
+    for rows, top in ((4, 1), (3, 65)):
+        with pytest.raises(b2.B2Error, match="b2_batch_logprobs"):
+            bt.logprobs(np.zeros((rows, 1)), top)
+    bt.close()
+    m.close()
+
+
 # ---------------------------------------------------------------------------
 # refusals that need a device, and a run of all of them
 # ---------------------------------------------------------------------------

@@ -138,6 +138,10 @@ def test_logprobs_refusals(built_lib, change, code):
     refused(code, "b2_logprobs", b2.logprobs, **{**LOGP, **change})
 
 
+def test_batch_logprobs_without_a_batch(built_lib):
+    assert built_lib.b2_batch_logprobs(None, 1, None, 0, None, None, 0, None, None) == -10
+
+
 @pytest.mark.skipif(has_gpu(), reason="checks the no-GPU error path")
 def test_no_gpu_is_an_error(built_lib):
     refused(-5, "no CUDA device", b2.page_plan, **PLAN)
