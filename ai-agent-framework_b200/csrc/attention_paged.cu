@@ -493,7 +493,7 @@ __global__ void __launch_bounds__(Sm<HD, NG>::kThreads) paged_split_kernel(const
             const int p0 = (lo / STEP + cu.step) * STEP;
             // one accumulator per term of q: short chains, and the terms below the
             // first stay out of a score that an infinite key made infinite (0 * inf)
-            float st[SUB][NG][QT][4];
+            float st[SUB][NG][QT][4], sp[SUB][NG][4];
 #pragma unroll
             for (int kk = 0; kk < KS; kk++)
 #pragma unroll
@@ -504,8 +504,16 @@ __global__ void __launch_bounds__(Sm<HD, NG>::kThreads) paged_split_kernel(const
                     for (int g = 0; g < NG; g++)
 #pragma unroll
                         for (int t = 0; t < QT; t++) {
-                            if (kk == 0) Cvt<C>::mma0(st[sub][g][t], ak, qf[g][kk][t][0], qf[g][kk][t][1]);
-                            else Cvt<C>::mma(st[sub][g][t], ak, qf[g][kk][t][0], qf[g][kk][t][1]);
+                            // (fp32 rows: the first term is summed 64 dimensions at a time, the sums
+                            // added in fp32, which rounds where the tensor cores' accumulation cuts)
+                            const bool parts = QT > 1 && t == 0 && kk >= 4;
+                            float* d = parts ? sp[sub][g] : st[sub][g][t];
+                            if (kk == 0 || (parts && kk % 4 == 0)) Cvt<C>::mma0(d, ak, qf[g][kk][t][0], qf[g][kk][t][1]);
+                            else Cvt<C>::mma(d, ak, qf[g][kk][t][0], qf[g][kk][t][1]);
+                            if (parts && (kk % 4 == 3 || kk == KS - 1)) {
+#pragma unroll
+                                for (int j = 0; j < 4; j++) st[sub][g][0][j] += sp[sub][g][j];
+                            }
                         }
                 }
             uint32_t pb[SUB][NG][PT][2];
