@@ -43,7 +43,6 @@ constexpr int kLpGroups = kLogprobMaxTop;         // groups of threads whose max
 constexpr int kLpMaxCluster = 8;
 constexpr int kLpRound = kLpThreads * 8;         // logits one collecting round may add
 constexpr int kLpCap = kLpRound + 1024;          // candidates held at once
-constexpr int kLpStages = 2;                     // batches of 16-bit logits in shared memory, all but one on their way
 constexpr float kLog2eF = 1.4426950408889634f;
 constexpr float kLn2F = 0.6931471805599453f;
 
@@ -179,10 +178,7 @@ struct LpShared {
     int wcount[kLpWarps];
     __nv_bfloat16 ent[kLpEntries][kLpThreads];
     unsigned long long top[kLogprobMaxTop];  // this CTA's list, in order
-    union {
-        unsigned long long cand[kLpCap];
-        uint4 ring[kLpStages][kLpBatch / 8][kLpThreads];  // of the pass over 16-bit logits
-    };
+    unsigned long long cand[kLpCap];
 };
 
 template <typename T, int VEC>
@@ -293,37 +289,11 @@ __device__ __forceinline__ int slice_pass(const T* x, int n, int v0, int v1, boo
             em = -INFINITY;
         }
     };
-    if constexpr (sizeof(T) == 2 && VEC == 8) {
-        // Each thread's next batches are on their way to places of its own in
-        // shared memory while one is added: no register waits for them, and no
-        // other thread.
-        const int nb = full > v + B ? (full - v - B - 1) / S + 1 : 0;
-        const T* src = x + (int64_t)v * VEC;
-        auto issue = [&](int j) {
-            if (j < nb) {
-#pragma unroll
-                for (int u = 0; u < U; u++)
-                    cp_async16(&s.ring[j % kLpStages][u][threadIdx.x], src + ((int64_t)j * S + u * kLpThreads) * VEC);
-            }
-            cp_async_commit();
-        };
-#pragma unroll
-        for (int j = 0; j < kLpStages - 1; j++) issue(j);
-        for (int j = 0; j < nb; j++) {
-            issue(j + kLpStages - 1);
-            asm volatile("cp.async.wait_group %0;" ::"n"(kLpStages - 1) : "memory");
-            P p[U];
-#pragma unroll
-            for (int u = 0; u < U; u++) p[u] = *reinterpret_cast<const P*>(&s.ring[j % kLpStages][u][threadIdx.x]);
-            work(p);
-        }
-        v += nb * S;
-    } else {
-        for (; v + B < full; v += S) {
-            P p[U];
-            load(p, v);
-            work(p);
-        }
+    // (prefetching the next batch costs more in warps than it gains: 96 -> 103 us)
+    for (; v + B < full; v += S) {
+        P p[U];
+        load(p, v);
+        work(p);
     }
     const int tail = v;
     for (; v < full; v += kLpThreads) {
