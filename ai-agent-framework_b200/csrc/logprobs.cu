@@ -10,7 +10,7 @@
 // Top k without a second pass over the row.  The pass leaves, besides each
 // thread's largest logit, the largest of every 32 that a thread took together
 // (in shared memory, rounded up to bf16).  The k-th largest of the maxima of 64
-// groups of threads is a lower bound of the k-th largest logit; only the 32s
+// groups of threads (of all threads for k past 32) is a lower bound of the k-th largest logit; only the 32s
 // whose maximum reaches it, a few more than k of them, are read again (from
 // L2), and their candidates are ordered by counting.  Where very many reach it
 // (a vocabulary masked with one value), the logits above the bound are taken
@@ -46,7 +46,8 @@ constexpr int kLpThreads = 256;
 constexpr int kLpBatch = 32;                     // logits a thread takes together
 constexpr int kLpEntries = 16;                   // maxima kept by a thread; longer slices: of several batches each
 constexpr int kLpWarps = kLpThreads / 32;
-constexpr int kLpGroups = kLogprobMaxTop;         // groups of threads whose maxima give the bound
+constexpr int kLpGroups = 64;                    // groups of threads whose maxima give the bound (k up to half of them)
+constexpr int kLpList = 256;                     // batches at the bound, at most, for their candidates to be taken directly
 constexpr int kLpMaxCluster = 8;
 constexpr int kLpRound = kLpThreads * 8;         // logits one collecting round may add
 constexpr int kLpCap = kLpRound + 1024;          // candidates held at once
@@ -178,10 +179,10 @@ struct Two<__half> {
 struct LpShared {
     Sums part[kLpWarps];
     Sums row;                                // this CTA's slice
-    __align__(16) float gmax[kLpGroups];
+    __align__(16) float gmax[kLpThreads];
     float thr;
     int n_cand, n_list;
-    int list[kLpCap / kLpBatch];
+    int list[kLpList];
     int wcount[kLpWarps];
     __nv_bfloat16 ent[kLpEntries][kLpThreads];
     unsigned long long top[kLogprobMaxTop];  // this CTA's list, in order
@@ -322,13 +323,12 @@ __device__ __forceinline__ int slice_pass(const T* x, int n, int v0, int v1, boo
 // The CTA's sums into s.part, and the k-th largest of kLpGroups maxima into s.thr.
 __device__ __forceinline__ void slice_sums(const Acc& acc, int k, LpShared& s) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    constexpr int GL = kLpThreads / kLpGroups;  // lanes of a group
+    const int groups = k <= kLpGroups / 2 ? kLpGroups : kLpThreads, gl = kLpThreads / groups;  // lanes of a group
     if (tid == 0) s.n_cand = s.n_list = 0;
     if (k > 1) {
         float g = acc.m;
-#pragma unroll
-        for (int o = 1; o < GL; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
-        if (tid % GL == 0) s.gmax[tid / GL] = g;
+        for (int o = 1; o < gl; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+        if (tid % gl == 0) s.gmax[tid / gl] = g;
     }
     const Sums t = join_lanes(acc.sums());
     if (lane == 0) s.part[warp] = t;
@@ -339,11 +339,11 @@ __device__ __forceinline__ void slice_sums(const Acc& acc, int k, LpShared& s) {
         for (int w = 1; w < kLpWarps; w++) m = fmaxf(m, s.part[w].m);
         s.thr = m;
     }
-    if (k > 1 && tid < kLpGroups) {
+    if (k > 1 && tid < groups) {
         const float g = s.gmax[tid];
         int above = 0;
-#pragma unroll
-        for (int j = 0; j < kLpGroups; j += 4) {
+#pragma unroll 4
+        for (int j = 0; j < groups; j += 4) {
             const float4 o = *reinterpret_cast<const float4*>(s.gmax + j);
             above += (o.x > g || (o.x == g && j < tid)) + (o.y > g || (o.y == g && j + 1 < tid)) +
                      (o.z > g || (o.z == g && j + 2 < tid)) + (o.w > g || (o.w == g && j + 3 < tid));
@@ -363,18 +363,17 @@ template <typename T, int VEC>
 __device__ __forceinline__ void slice_top(const T* x, int n, int v0, int v1, int k, float mine, int ne, LpShared& s) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const Entries<VEC> en(v0, v1);
-    const int most = kLpCap / (en.len() * VEC);  // entries that the list of candidates holds whatever is in them
     const float thr = s.thr;
     auto list = [&](bool ties) {  // the entries that reach the bound (or pass it), as first chunks
         for (int e = 0; e < ne; e++) {
             const float m = __bfloat162float(s.ent[e][tid]);
             if (ties ? m >= thr : m > thr) {
                 const int at = atomicAdd(&s.n_list, 1);
-                if (at < most) s.list[at] = tid + e * en.len() * kLpThreads;
+                if (at < kLpList) s.list[at] = tid + e * en.len() * kLpThreads;
             }
         }
         __syncthreads();
-        return s.n_list <= most;
+        return s.n_list <= kLpList;
     };
     const bool plain = list(true) && thr > -INFINITY;
     bool few = plain;
@@ -385,6 +384,11 @@ __device__ __forceinline__ void slice_top(const T* x, int n, int v0, int v1, int
         few = list(false);
     }
     unsigned long long bound = 0;  // after a cut of the list: keys at or under it are out
+    auto push = [&](unsigned long long key) {
+        if (key <= bound) return;
+        const int at = atomicAdd(&s.n_cand, 1);
+        if (at < kLpCap) s.cand[at] = key;
+    };
     auto take = [&](int v) {
         if (v >= v1) return;
         const int i0 = v * VEC;
@@ -394,16 +398,14 @@ __device__ __forceinline__ void slice_top(const T* x, int n, int v0, int v1, int
             for (int i = 0; i < VEC; i++) {
                 const float f = lf(p.v[i]);
                 if (plain ? f >= thr : f > thr) {
-                    const unsigned long long key = key_of(f, i0 + i);
-                    if (key > bound) s.cand[atomicAdd(&s.n_cand, 1)] = key;
+                    push(key_of(f, i0 + i));
                 }
             }
         } else {
             for (int i = i0; i < n; i++) {
                 const float f = lf(x[i]);
                 if (plain ? f >= thr : f > thr) {
-                    const unsigned long long key = key_of(f, i);
-                    if (key > bound) s.cand[atomicAdd(&s.n_cand, 1)] = key;
+                    push(key_of(f, i));
                 }
             }
         }
@@ -414,9 +416,16 @@ __device__ __forceinline__ void slice_top(const T* x, int n, int v0, int v1, int
             take(v0 + s.list[q] + (i - q * en.len()) * kLpThreads);
         }
         __syncthreads();
-    } else {  // chunk by chunk, the list cut to the k largest whenever the next might not fit
+        if (s.n_cand > kLpCap) {  // they hold more candidates than the list
+            __syncthreads();
+            if (tid == 0) s.n_cand = 0;
+            __syncthreads();
+            few = false;
+        }
+    }
+    if (!few) {  // chunk by chunk, the list cut to the k largest whenever the next might not fit
         for (int v = v0; v < v1; v += kLpThreads) {
-            if (mine > thr) take(v + tid);
+            if (plain ? mine >= thr : mine > thr) take(v + tid);
             __syncthreads();
             const int cnt = s.n_cand;
             if (cnt > kLpCap - kLpRound) {

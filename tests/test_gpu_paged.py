@@ -633,8 +633,8 @@ def test_logprobs_many_rows():
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("kind", ["zeros", "signed zeros", "two levels", "lowest value", "lowest and -inf", "few allowed", "one allowed", "ascending",
-                                  "descending", "one thread", "large", "tail"])
-@pytest.mark.parametrize("n", [700, 20011, 131072])
+                                  "descending", "one thread", "runs", "large", "tail"])
+@pytest.mark.parametrize("n", [700, 20011, 131072, 300001])
 @pytest.mark.parametrize("rows", [1, 100])
 def test_logprobs_ties_and_masks(dtype, kind, n, rows):
     """Alternatives where very many logits are equal, masked, in order, or in one thread's hands."""
@@ -663,6 +663,8 @@ def test_logprobs_ties_and_masks(dtype, kind, n, rows):
         x[:] = (i if kind == "ascending" else n - i).float() / n * 20
     elif kind == "one thread":  # large logits 4096 apart and in long runs
         x[:, (i // 8) % 512 == 5] = 4.0 + torch.rand(int(((i // 8) % 512 == 5).sum()), device="cuda", generator=g)
+    elif kind == "runs":  # a few batches of a thread hold many logits over the bound each
+        x[:, (i // 8) % 256 < 40] = 4.0 + torch.rand(int(((i // 8) % 256 < 40).sum()), device="cuda", generator=g)
     elif kind == "large":
         x[:] = 30000.0 * torch.randn(rows, n, device="cuda", generator=g).clamp(-2, 2)
     elif kind == "tail":
