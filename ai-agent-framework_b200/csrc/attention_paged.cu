@@ -41,6 +41,11 @@
 // tensor cores' accumulation cuts instead of rounding, which over a long row
 // would pull the output towards zero.  Sums, maxima and outputs are fp32,
 // rounded once at the end.
+//
+// Measured (8 KV heads of 128, HBM copies run at 6.5 TB/s): 8 x 32K, fp32 rows,
+// 32 heads: 162 us, 6.6 TB/s; 64 sequences of 16 .. 16384, bf16, 64 heads: 112 us,
+// 5.8 TB/s, the ragged ends and 4 us of joining being the rest; 1 x 4K: 13.5 us,
+// two launches and a chain of dependent loads (lengths, pages, K and V, pieces).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -56,6 +61,7 @@ namespace {
 
 constexpr int kOverhead = 4;    // units' worth of starting and ending a sequence
 constexpr int kMinUnits = 2;    // a group's share, at least (overhead counted)
+constexpr long long kMaxLen = 0x7fffffffLL - 63;  // so that a step's positions are ints
 constexpr int kJoinThreads = 256;
 constexpr int kJoinWarps = kJoinThreads / 32;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -73,16 +79,16 @@ struct PagedArgs {
     const float* slopes;
     int64_t q_stride, out_stride, table_stride, page_stride, pos_stride, head_stride;
     int batch, nh, nkv, grp, heads, rt, hd, page_size, page_shift, n_pages, max_pages, n_req, len_add, window, groups, sms;
+    // heads: query heads of one unit (8 or 16); rt: blocks of that many in a group;
+    // page_shift: log2 of the page size, or -1
     int q_pairs;   // q's rows can be read two elements at a time
     float scale, softcap;
 };
-// heads: query heads of one unit (8 or 16); rt: blocks of that many in a group.
-// page_shift: log2 of the page size, or -1.
 
 // A row's sequence: table row, visible positions [lo, len).  len 0: nothing.
 struct Seq {
     int tr, lo, len;
-    bool bad;  // the length passes the table
+    bool bad;  // the length passes the table, or the row has none
 };
 
 __device__ __forceinline__ Seq seq_of(const PagedArgs& a, int b) {
@@ -90,7 +96,7 @@ __device__ __forceinline__ Seq seq_of(const PagedArgs& a, int b) {
     s.tr = a.req ? __ldg(a.req + b) : b;
     const long long len = (long long)__ldg(a.lens + b) + a.len_add;
     const bool none = s.tr < 0 || len <= 0;
-    s.bad = !none && (s.tr >= a.n_req || len > (long long)a.max_pages * a.page_size || len > 0x7fffffffLL);
+    s.bad = !none && (s.tr >= a.n_req || len > (long long)a.max_pages * a.page_size || len > kMaxLen);
     s.len = none || s.bad ? 0 : (int)len;
     s.lo = a.window > 0 ? max(0, s.len - a.window) : 0;
     return s;
@@ -134,13 +140,16 @@ struct Cvt<__half> {
         back = __half22float2(h);
         return *reinterpret_cast<const uint32_t*>(&h);
     }
+    // d += a b
     static __device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
         asm volatile(
             "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
             "{%0, %1, %2, %3};"
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    }    static __device__ __forceinline__ void mma0(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    }
+    // d = a b
+    static __device__ __forceinline__ void mma0(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
         asm volatile(
             "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
             "{%10, %10, %10, %10};"
@@ -155,13 +164,16 @@ struct Cvt<__nv_bfloat16> {
         back = __bfloat1622float2(h);
         return *reinterpret_cast<const uint32_t*>(&h);
     }
+    // d += a b
     static __device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
         asm volatile(
             "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
             "{%0, %1, %2, %3};"
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    }    static __device__ __forceinline__ void mma0(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    }
+    // d = a b
+    static __device__ __forceinline__ void mma0(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
         asm volatile(
             "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
             "{%10, %10, %10, %10};"
@@ -330,7 +342,7 @@ __global__ void __launch_bounds__(Sm<HD, NG>::kThreads) paged_split_kernel(const
     const int heads = min(kHeads, a.grp - row0), head0 = h * a.grp + row0;
     const int64_t h_off = (int64_t)h * a.head_stride;
     bool more = ld.settle(a);  // the loading side has a step
-    if (!more) return;              // (overhead alone)
+    if (!more) return;         // (overhead alone)
     Cursor<STEP> cu = ld;
 
     const uint32_t ring_s = smem_u32(ring);

@@ -453,11 +453,11 @@ typedef struct {
  * are a step's tokens, prompts included.  The order per score is scale,
  * softcap, slope, mask; fp32 softmax.  Writes out and, when lse is not NULL,
  * lse[b][nh] = log of the sum of e^score.  A row that sees nothing (length <=
- * 0, req < 0) gets zeros and -inf; a row whose length passes its table, whose
- * req is n_req or more, or whose visible pages are not all in 0 .. n_pages - 1
- * gets NaN.  Keys and values that are not seen may hold anything; an infinite
- * value that is seen makes its element infinite or NaN.  Pages outside the
- * window are not looked at.  d_scratch:
+ * 0, req < 0) gets zeros and -inf.  A row whose length passes its table or
+ * 2^31 - 64, whose req is n_req or more, or whose visible pages are not all in
+ * 0 .. n_pages - 1 gets NaN.  Keys and values that are not seen may hold
+ * anything; an infinite value that is seen makes its element infinite or NaN.
+ * Pages outside the window are not looked at.  d_scratch:
  * b2_attention_paged_scratch_bytes(batch, nh, nkv, hd) bytes of device memory
  * on 16 bytes, no contents needed. */
 int64_t b2_attention_paged_scratch_bytes(int32_t batch, int32_t nh, int32_t nkv, int32_t hd);
