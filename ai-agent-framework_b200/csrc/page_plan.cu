@@ -16,8 +16,9 @@
 // writes, so a step that does not fit changes nothing in the table.
 //
 // Bound by latency: 3.1 us for 16 tokens (a launch, the lengths, a search, a
-// page), 12.2 us for a million tokens of 2048 requests, of which the 17 MB
-// written need 2.7.
+// page), 10.0 us for a million tokens of 2048 requests, of which the 17 MB
+// written need 2.7 (the issue slots of the scan, the searches and the table's
+// entries, one after another).
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -29,7 +30,7 @@ namespace b2 {
 namespace {
 
 // Tokens of one lane, 32 apart, so that a warp's stores are whole lines: eight
-// where there are enough to fill the machine (a million tokens: 12 us, 32 with
+// where there are enough to fill the machine (a million tokens: 10 us, 32 with
 // one), one for a decode step (16 tokens: 3.1 us, 5.5 with four, one after
 // another's search).
 constexpr int kManyTokens = 8;
@@ -78,10 +79,11 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const __grid_co
     unsigned tok = 0, pg = 0;
     int bad = 0, c0 = 0, f0 = 0;  // (the first one's lengths stay at hand)
     const long long most = min(0x7fffffffLL, (long long)a.max_pages * a.page_size);
-    for (int r = r0; r < r1; r += 4) {
-        int c[4], f[4];  // four requests' loads at once
+    constexpr int B = kPlanThreads > 512 ? 2 : 4;  // requests whose loads go out at once
+    for (int r = r0; r < r1; r += B) {
+        int c[B], f[B];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < B; k++) {
             c[k] = r + k < r1 ? a.cached[r + k] : 0;
             f[k] = r + k < r1 ? a.fresh[r + k] : 0;
         }
@@ -90,7 +92,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const __grid_co
             f0 = f[0];
         }
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < B; k++) {
             const long long len = (long long)c[k] + f[k];
             const bool neg = c[k] < 0 || f[k] < 0, wide = len > most;
             bad |= neg ? B2_PLAN_BAD_LENGTH : wide ? B2_PLAN_TABLE_FULL : 0;
@@ -116,18 +118,23 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const __grid_co
     bad = __reduce_or_sync(0xffffffffu, bad);
     if (lane == 0) wbad[warp] = bad;
     __syncthreads();
-    int status = 0;
-    unsigned total_tok = 0, total_pg = 0;
+    // the warps before this one, and all of them: a scan by every warp
+    unsigned wt = lane < kPlanWarps ? wsum[0][lane] : 0, wp = lane < kPlanWarps ? wsum[1][lane] : 0;
 #pragma unroll
-    for (int w = 0; w < kPlanWarps; w++) {
-        if (w == warp) {
-            it = sat_add(it, total_tok);
-            ip = sat_add(ip, total_pg);
+    for (int o = 1; o < kPlanWarps; o <<= 1) {
+        const unsigned t = __shfl_up_sync(0xffffffffu, wt, o), p = __shfl_up_sync(0xffffffffu, wp, o);
+        if (lane >= o) {
+            wt = sat_add(wt, t);
+            wp = sat_add(wp, p);
         }
-        total_tok = sat_add(total_tok, wsum[0][w]);
-        total_pg = sat_add(total_pg, wsum[1][w]);
-        status |= wbad[w];
     }
+    const unsigned total_tok = __shfl_sync(0xffffffffu, wt, kPlanWarps - 1), total_pg = __shfl_sync(0xffffffffu, wp, kPlanWarps - 1);
+    const unsigned bt = __shfl_sync(0xffffffffu, wt, max(warp - 1, 0)), bp = __shfl_sync(0xffffffffu, wp, max(warp - 1, 0));
+    if (warp) {
+        it = sat_add(it, bt);
+        ip = sat_add(ip, bp);
+    }
+    int status = __reduce_or_sync(0xffffffffu, lane < kPlanWarps ? wbad[lane] : 0);
     if (total_tok > (unsigned)a.max_tokens || total_tok == kSumMax) status |= B2_PLAN_ROWS_FULL;
     if (total_pg > (unsigned)n_free || total_pg == kSumMax) status |= B2_PLAN_NO_PAGES;
     const bool ok = status == 0;
@@ -163,23 +170,23 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const __grid_co
         const int r = last_le(taken, 0, R, e);
         a.table[(int64_t)r * a.table_stride + pages_of(a, a.cached[r]) + (e - taken[r])] = a.free_pages[e];
     }
-    // a warp: J runs of 32 tokens
-    const long long wstep = (long long)(gsize / 32) * (32 * J);
-    for (long long t0 = (long long)(gtid / 32) * (32 * J); t0 < a.max_tokens; t0 += wstep) {
+    // a warp: J runs of 32 tokens (unsigned: the last run may pass 2^31)
+    const unsigned cap = a.max_tokens, wstep = (unsigned)(gsize / 32) * (32 * J);
+    for (unsigned t0 = (unsigned)(gtid / 32) * (32 * J); t0 < cap; t0 = t0 + wstep < t0 ? cap : t0 + wstep) {
         int lo = 0, hi = R;
-        if (J > 1 && t0 < T) {  // the requests of its first and last token bound the others'
-            const int t = (int)min(lane ? t0 + 32 * J - 1 : t0, (long long)T - 1);
-            const int r = lane < 2 ? last_le(start, 0, R, t) : 0;
+        if (J > 1 && t0 < (unsigned)T) {  // the requests of its first and last token bound the others'
+            const unsigned t = min(lane ? t0 + 32 * J - 1 : t0, (unsigned)T - 1);
+            const int r = lane < 2 ? last_le(start, 0, R, (int)t) : 0;
             lo = __shfl_sync(0xffffffffu, r, 0);
             hi = __shfl_sync(0xffffffffu, r, 1);
         }
         int pos[J], req[J], in[J], page[J];
 #pragma unroll
         for (int j = 0; j < J; j++) {
-            const long long t = t0 + 32 * j + lane;
+            const unsigned t = t0 + 32 * j + lane;
             pos[j] = in[j] = 0;
             req[j] = page[j] = -1;
-            if (t < T) {
+            if (t < (unsigned)T) {
                 const int r = last_le(start, lo, hi, (int)t), c = a.cached[r];
                 pos[j] = c + ((int)t - start[r]);
                 const int idx = div_page(a, pos[j]), have = pages_of(a, c);
@@ -189,15 +196,15 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const __grid_co
                 page[j] = *(idx < have ? a.table + ((int64_t)r * a.table_stride + idx) : a.free_pages + (taken[r] + idx - have));
             }
         }
+        int64_t* slots = a.slots + t0 + lane;
+        int32_t *positions = a.positions + t0 + lane, *token_req = a.token_req + t0 + lane;
 #pragma unroll
-        for (int j = 0; j < J; j++) {
-            const long long t = t0 + 32 * j + lane;
-            if (t < a.max_tokens) {
-                a.slots[t] = page[j] >= 0 ? (int64_t)page[j] * a.page_size + in[j] : -1;
-                a.positions[t] = pos[j];
-                a.token_req[t] = req[j];
+        for (int j = 0; j < J; j++)
+            if (t0 + 32 * j + lane < cap) {
+                slots[32 * j] = page[j] >= 0 ? (int64_t)page[j] * a.page_size + in[j] : -1;
+                positions[32 * j] = pos[j];
+                token_req[32 * j] = req[j];
             }
-        }
     }
 }
 

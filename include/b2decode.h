@@ -322,7 +322,7 @@ int b2_batch_use_graph(b2_batch* b, int32_t on);
  * CUDA graph.  Calls that overlap on the GPU must not share outputs or
  * scratch.  Types are ggml type ids: 0 = F32, 1 = F16, 30 = BF16.  The Go
  * engine has one contiguous cache per sequence (kvCache,
- * transformer.go:61-92); these have no counterpart there beyond the
+ * transformer.go:88-92); these have no counterpart there beyond the
  * arithmetic cited. */
 
 /* A paged KV cache: the element d of head h of position s of page p is at
@@ -371,7 +371,7 @@ int b2_page_plan(const int32_t* cached, const int32_t* fresh, int32_t n_req, int
                  int32_t max_pages, int32_t* lens, int32_t* starts, int64_t* slots, int32_t* positions,
                  int32_t* token_req, int32_t max_tokens, int32_t* info, void* stream);
 
-#define B2_ROPE_INTERLEAVED 0 /* pairs (2i, 2i + 1), as transformer.go:935-955 rotates */
+#define B2_ROPE_INTERLEAVED 0 /* pairs (2i, 2i + 1), as transformer.go:936-951 rotates */
 #define B2_ROPE_HALF 1        /* pairs (i, i + rot_dim / 2) */
 
 #define B2_ROPE_SCALE_NONE 0
@@ -416,7 +416,7 @@ typedef struct {
     int64_t k_out_stride;
 } b2_rope_rows;
 
-/* transformer.go:935-955 applyRoPE on rows at positions[n_tok]: pair i turns
+/* transformer.go:936-951 applyRoPE on rows at positions[n_tok]: pair i turns
  * by positions * freqs[i] (freqs [rot_dim / 2] device doubles), the angle
  * reduced in 64 bits, the rotation in fp32, rounded once.  q -> q_out, k ->
  * k_out; either pair may be NULL; a row may be rotated in place (q_out = q
@@ -467,7 +467,7 @@ int b2_attention_paged(const b2_paged_kv* kv, const b2_paged_attn_opts* opts, co
 
 /* Log probabilities of given tokens, the entropy and the top alternatives of
  * rows of n logits (row i at logits + i * ld, ld >= n; n up to 2^30): the
- * softmax of transformer.go:1050-1067 kept as logarithms, fp32 sums.
+ * softmax of transformer.go:959-974 kept as logarithms, fp32 sums.
  * logprob[i][m] = log p(ids[i][m]) (an id outside 0 .. n - 1: NaN),
  * entropy[i] in nats (may be NULL), top_ids / top_logprob[i][k] = the k
  * largest logits in order, equal ones by lowest id (k up to 64 and n).  A
