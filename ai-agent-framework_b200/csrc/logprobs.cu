@@ -42,15 +42,11 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kLpThreads = 256;
 constexpr int kLpBatch = 32;                     // logits a thread takes together
 constexpr int kLpEntries = 16;                   // maxima kept by a thread; longer slices: of several batches each
-constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kLpGroups = 64;                    // groups of threads whose maxima give the bound (k up to half of them)
 constexpr int kLpList = 256;                     // batches at the bound, at most, for their candidates to be taken directly
 constexpr int kLpMaxCluster = 8;
-constexpr int kLpRound = kLpThreads * 8;         // logits one collecting round may add
-constexpr int kLpCap = kLpRound + 1024;          // candidates held at once
 constexpr float kLog2eF = 1.4426950408889634f;
 constexpr float kLn2F = 0.6931471805599453f;
 
@@ -176,17 +172,28 @@ struct Two<__half> {
     static __device__ __forceinline__ float2 floats(V v) { return __half22float2(v); }
 };
 
+// Threads of a CTA: 256, or 128 for rows of up to kLpShortRow logits, whose
+// fixed steps weigh more than their reading (4096 rows of 1000 fp32: 31 us with
+// 256, 19 with 128; of 16384 bf16: 47 and 41; of 32000: 69 both; 2048 of 128256:
+// 96 and 109).
+constexpr int kLpShortRow = 24576;
+
+template <int NT>
 struct LpShared {
-    Sums part[kLpWarps];
+    static constexpr int kWarps = NT / 32;
+    static constexpr int kRound = NT * 8;         // logits one collecting round may add
+    static constexpr int kCap = kRound + 1024;    // candidates held at once
+
+    Sums part[kWarps];
     Sums row;                                // this CTA's slice
-    __align__(16) float gmax[kLpThreads];
+    __align__(16) float gmax[NT];
     float thr;
     int n_cand, n_list;
     int list[kLpList];
-    int wcount[kLpWarps];
-    __nv_bfloat16 ent[kLpEntries][kLpThreads];
+    int wcount[kWarps];
+    __nv_bfloat16 ent[kLpEntries][NT];
     unsigned long long top[kLogprobMaxTop];  // this CTA's list, in order
-    unsigned long long cand[kLpCap];
+    unsigned long long cand[kCap];
 };
 
 template <typename T, int VEC>
@@ -195,10 +202,11 @@ struct alignas(sizeof(T) * VEC) LpPack {
 };
 
 // The k largest of s.cand[0 .. cnt) into s.top in order (zeros past cnt).
-__device__ void order_top(LpShared& s, int cnt, int k) {
-    for (int i = threadIdx.x; i < k; i += kLpThreads)
+template <int NT>
+__device__ void order_top(LpShared<NT>& s, int cnt, int k) {
+    for (int i = threadIdx.x; i < k; i += NT)
         if (i >= cnt) s.top[i] = 0;
-    for (int i = threadIdx.x; i < cnt; i += kLpThreads) {
+    for (int i = threadIdx.x; i < cnt; i += NT) {
         const unsigned long long key = s.cand[i];
         int above = 0;
         for (int j = 0; j < cnt; j++) above += s.cand[j] > key;
@@ -257,15 +265,15 @@ __device__ __forceinline__ float add_chunks(const LpPack<T, VEC> (&p)[N], Acc& t
     }
 }
 
-// How a thread's chunks (its i-th is v0 + tid + i kLpThreads) fall to its
+// How a thread's chunks (its i-th is v0 + tid + i NT) fall to its
 // entries: entry e has the chunks from e * len() on.
-template <int VEC>
+template <int VEC, int NT>
 struct Entries {
     static constexpr int U = kLpBatch / VEC;  // chunks of a batch
     int agg;                                  // batches of an entry
 
     __device__ __forceinline__ Entries(int v0, int v1) {
-        const int per = (v1 - v0 + kLpThreads - 1) / kLpThreads, batches = (per + U - 1) / U;
+        const int per = (v1 - v0 + NT - 1) / NT, batches = (per + U - 1) / U;
         agg = max(1, (batches + kLpEntries - 1) / kLpEntries);
     }
     __device__ __forceinline__ int len() const { return U * agg; }
@@ -273,20 +281,20 @@ struct Entries {
 
 // One CTA: the slice [v0, v1) of a row in chunks of VEC logits (the last one
 // cut at n).  Returns how many entries this thread wrote.
-template <typename T, int VEC>
-__device__ __forceinline__ int slice_pass(const T* x, int n, int v0, int v1, bool keep, Acc& t, LpShared& s) {
-    constexpr int U = Entries<VEC>::U;
+template <typename T, int VEC, int NT>
+__device__ __forceinline__ int slice_pass(const T* x, int n, int v0, int v1, bool keep, Acc& t, LpShared<NT>& s) {
+    constexpr int U = Entries<VEC, NT>::U;
     using P = LpPack<T, VEC>;
-    const Entries<VEC> en(v0, v1);
+    const Entries<VEC, NT> en(v0, v1);
     const int full = min(v1, n / VEC);  // chunks without a cut
     int left = en.agg, e = 0;
     float em = -INFINITY;
     auto put = [&]() { s.ent[e][threadIdx.x] = __float2bfloat16_ru(em); };
     int v = v0 + (int)threadIdx.x;
-    constexpr int S = U * kLpThreads, B = S - kLpThreads;
+    constexpr int S = U * NT, B = S - NT;
     auto load = [&](P (&p)[U], int at) {
 #pragma unroll
-        for (int u = 0; u < U; u++) p[u] = *reinterpret_cast<const P*>(x + (int64_t)(at + u * kLpThreads) * VEC);
+        for (int u = 0; u < U; u++) p[u] = *reinterpret_cast<const P*>(x + (int64_t)(at + u * NT) * VEC);
     };
     auto work = [&](const P (&p)[U]) {
         em = fmaxf(em, add_chunks<T, VEC, U>(p, t));
@@ -304,11 +312,11 @@ __device__ __forceinline__ int slice_pass(const T* x, int n, int v0, int v1, boo
         work(p);
     }
     const int tail = v;
-    for (; v < full; v += kLpThreads) {
+    for (; v < full; v += NT) {
         const P p[1] = {*reinterpret_cast<const P*>(x + (int64_t)v * VEC)};
         em = fmaxf(em, add_chunks<T, VEC, 1>(p, t));
     }
-    for (; v < v1; v += kLpThreads)  // the cut chunk
+    for (; v < v1; v += NT)  // the cut chunk
         for (int i = v * VEC; i < n; i++) {
             const LpPack<T, 1> p[1] = {{x[i]}};
             em = fmaxf(em, add_chunks<T, 1, 1>(p, t));
@@ -321,9 +329,11 @@ __device__ __forceinline__ int slice_pass(const T* x, int n, int v0, int v1, boo
 }
 
 // The CTA's sums into s.part, and the k-th largest of kLpGroups maxima into s.thr.
-__device__ __forceinline__ void slice_sums(const Acc& acc, int k, LpShared& s) {
+template <int NT>
+__device__ __forceinline__ void slice_sums(const Acc& acc, int k, LpShared<NT>& s) {
+    constexpr int kWarps = LpShared<NT>::kWarps;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int groups = k <= kLpGroups / 2 ? kLpGroups : kLpThreads, gl = kLpThreads / groups;  // lanes of a group
+    const int groups = k <= kLpGroups / 2 ? kLpGroups : NT, gl = NT / groups;  // lanes of a group
     if (tid == 0) s.n_cand = s.n_list = 0;
     if (k > 1) {
         float g = acc.m;
@@ -336,7 +346,7 @@ __device__ __forceinline__ void slice_sums(const Acc& acc, int k, LpShared& s) {
     if (k == 1 && tid == 0) {
         float m = s.part[0].m;
 #pragma unroll
-        for (int w = 1; w < kLpWarps; w++) m = fmaxf(m, s.part[w].m);
+        for (int w = 1; w < kWarps; w++) m = fmaxf(m, s.part[w].m);
         s.thr = m;
     }
     if (k > 1 && tid < groups) {
@@ -350,8 +360,8 @@ __device__ __forceinline__ void slice_sums(const Acc& acc, int k, LpShared& s) {
         }
         if (above == k - 1) s.thr = g;
     }
-    if (warp == kLpWarps - 1) {
-        const Sums u = join_lanes(lane < kLpWarps ? s.part[lane] : Sums{-INFINITY, 0.0f, 0.0f});
+    if (warp == kWarps - 1) {
+        const Sums u = join_lanes(lane < kWarps ? s.part[lane] : Sums{-INFINITY, 0.0f, 0.0f});
         if (lane == 0) s.row = u;
     }
     __syncthreads();
@@ -359,17 +369,18 @@ __device__ __forceinline__ void slice_sums(const Acc& acc, int k, LpShared& s) {
 
 // The k largest of the slice into s.top, from the thread's maximum and its
 // `ne` entries.
-template <typename T, int VEC>
-__device__ __forceinline__ void slice_top(const T* x, int n, int v0, int v1, int k, float mine, int ne, LpShared& s) {
+template <typename T, int VEC, int NT>
+__device__ __forceinline__ void slice_top(const T* x, int n, int v0, int v1, int k, float mine, int ne, LpShared<NT>& s) {
+    constexpr int kWarps = LpShared<NT>::kWarps, kRound = LpShared<NT>::kRound, kCap = LpShared<NT>::kCap;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const Entries<VEC> en(v0, v1);
+    const Entries<VEC, NT> en(v0, v1);
     const float thr = s.thr;
     auto list = [&](bool ties) {  // the entries that reach the bound (or pass it), as first chunks
         for (int e = 0; e < ne; e++) {
             const float m = __bfloat162float(s.ent[e][tid]);
             if (ties ? m >= thr : m > thr) {
                 const int at = atomicAdd(&s.n_list, 1);
-                if (at < kLpList) s.list[at] = tid + e * en.len() * kLpThreads;
+                if (at < kLpList) s.list[at] = tid + e * en.len() * NT;
             }
         }
         __syncthreads();
@@ -387,7 +398,7 @@ __device__ __forceinline__ void slice_top(const T* x, int n, int v0, int v1, int
     auto push = [&](unsigned long long key) {
         if (key <= bound) return;
         const int at = atomicAdd(&s.n_cand, 1);
-        if (at < kLpCap) s.cand[at] = key;
+        if (at < kCap) s.cand[at] = key;
     };
     auto take = [&](int v) {
         if (v >= v1) return;
@@ -411,12 +422,12 @@ __device__ __forceinline__ void slice_top(const T* x, int n, int v0, int v1, int
         }
     };
     if (few) {  // their chunks, one to a thread
-        for (int i = tid; i < s.n_list * en.len(); i += kLpThreads) {
+        for (int i = tid; i < s.n_list * en.len(); i += NT) {
             const int q = i / en.len();
-            take(v0 + s.list[q] + (i - q * en.len()) * kLpThreads);
+            take(v0 + s.list[q] + (i - q * en.len()) * NT);
         }
         __syncthreads();
-        if (s.n_cand > kLpCap) {  // they hold more candidates than the list
+        if (s.n_cand > kCap) {  // they hold more candidates than the list
             __syncthreads();
             if (tid == 0) s.n_cand = 0;
             __syncthreads();
@@ -424,13 +435,13 @@ __device__ __forceinline__ void slice_top(const T* x, int n, int v0, int v1, int
         }
     }
     if (!few) {  // chunk by chunk, the list cut to the k largest whenever the next might not fit
-        for (int v = v0; v < v1; v += kLpThreads) {
+        for (int v = v0; v < v1; v += NT) {
             if (plain ? mine >= thr : mine > thr) take(v + tid);
             __syncthreads();
             const int cnt = s.n_cand;
-            if (cnt > kLpCap - kLpRound) {
+            if (cnt > kCap - kRound) {
                 order_top(s, cnt, k);
-                for (int i = tid; i < k; i += kLpThreads) s.cand[i] = s.top[i];
+                for (int i = tid; i < k; i += NT) s.cand[i] = s.top[i];
                 bound = s.top[k - 1];
                 if (tid == 0) s.n_cand = k;
             }
@@ -442,14 +453,14 @@ __device__ __forceinline__ void slice_top(const T* x, int n, int v0, int v1, int
     if (!plain) {  // ties at the bound, in index order
         const int i1 = min(n, v1 * VEC);
         int cnt = min(cnt0, k);
-        for (int base = v0 * VEC; base < i1 && cnt < k; base += kLpThreads) {
+        for (int base = v0 * VEC; base < i1 && cnt < k; base += NT) {
             const int i = base + tid;
             const bool tie = i < i1 && lf(x[i]) == thr;
             const unsigned bal = __ballot_sync(0xffffffffu, tie);
             if (lane == 0) s.wcount[warp] = __popc(bal);
             __syncthreads();
             int at = cnt + __popc(bal & ((1u << lane) - 1)), all = 0;
-            for (int w = 0; w < kLpWarps; w++) {
+            for (int w = 0; w < kWarps; w++) {
                 if (w < warp) at += s.wcount[w];
                 all += s.wcount[w];
             }
@@ -460,10 +471,11 @@ __device__ __forceinline__ void slice_top(const T* x, int n, int v0, int v1, int
     }
 }
 
-template <typename T, int VEC>
-__global__ void __launch_bounds__(kLpThreads) logprob_kernel(const __grid_constant__ LogprobArgs a) {
+template <typename T, int VEC, int NT>
+__global__ void __launch_bounds__(NT) logprob_kernel(const __grid_constant__ LogprobArgs a) {
     extern __shared__ __align__(16) uint8_t lp_raw[];
-    LpShared& s = *reinterpret_cast<LpShared*>(lp_raw);
+    LpShared<NT>& s = *reinterpret_cast<LpShared<NT>*>(lp_raw);
+    constexpr int kWarps = LpShared<NT>::kWarps;
     pdl_trigger();
     pdl_wait();
     const int C = a.cluster, rank = C > 1 ? (int)cg::this_cluster().block_rank() : 0;
@@ -478,15 +490,15 @@ __global__ void __launch_bounds__(kLpThreads) logprob_kernel(const __grid_consta
     float given[kIds];
 #pragma unroll
     for (int j = 0; j < kIds; j++) {
-        const int i = tid + j * kLpThreads;
+        const int i = tid + j * NT;
         const int id = rank == 0 && i < a.m ? a.ids[row * a.m + i] : -1;
         given[j] = id >= 0 && id < a.n ? lf(x[id]) : __int_as_float(0x7fc00000);
     }
 
     Acc acc;
-    const int ne = slice_pass<T, VEC>(x, a.n, v0, v1, a.k > 0, acc, s);
+    const int ne = slice_pass<T, VEC, NT>(x, a.n, v0, v1, a.k > 0, acc, s);
     slice_sums(acc, a.k, s);
-    if (a.k > 0) slice_top<T, VEC>(x, a.n, v0, v1, a.k, acc.m, ne, s);
+    if (a.k > 0) slice_top<T, VEC, NT>(x, a.n, v0, v1, a.k, acc.m, ne, s);
 
     if (C > 1) {
         cg::cluster_group cl = cg::this_cluster();
@@ -500,7 +512,7 @@ __global__ void __launch_bounds__(kLpThreads) logprob_kernel(const __grid_consta
             // the C lists as one, with no empty places
             if (tid == 0) s.n_cand = 0;
             __syncthreads();
-            for (int i = tid; i < C * a.k; i += kLpThreads) {
+            for (int i = tid; i < C * a.k; i += NT) {
                 const unsigned long long key = cl.map_shared_rank(&s, i / a.k)->top[i % a.k];
                 if (key) s.cand[atomicAdd(&s.n_cand, 1)] = key;
             }
@@ -516,7 +528,7 @@ __global__ void __launch_bounds__(kLpThreads) logprob_kernel(const __grid_consta
     const float z = r.m == -INFINITY ? 0.0f : r.m;
     auto lp = [&](float v) { return (v - z) - lS; };
     const float nan = __int_as_float(0x7fc00000);
-    for (int i = tid, j = 0; i < a.m; i += kLpThreads, j++) {
+    for (int i = tid, j = 0; i < a.m; i += NT, j++) {
         float v = nan;
         if (j < kIds) {
             v = j ? given[kIds - 1] : given[0];
@@ -527,23 +539,23 @@ __global__ void __launch_bounds__(kLpThreads) logprob_kernel(const __grid_consta
         a.logprob[row * a.m + i] = r.m != -INFINITY ? lp(v) : nan;
     }
     if (tid == 0 && a.entropy) a.entropy[row] = lS - r.T / r.S * kLn2F;
-    for (int i = tid; i < a.k; i += kLpThreads) {
+    for (int i = tid; i < a.k; i += NT) {
         const unsigned long long key = s.top[i];
         a.top_ids[row * a.k + i] = key ? key_index(key) : -1;
         a.top_logprob[row * a.k + i] = key && r.m != -INFINITY ? lp(key_value(key)) : nan;
     }
 }
 
-template <typename T>
-cudaError_t go(const LogprobArgs& a, int rows, cudaStream_t s) {
+template <typename T, int NT>
+cudaError_t go_threads(const LogprobArgs& a, int rows, cudaStream_t s) {
     constexpr int W = 16 / sizeof(T);
-    auto kern = a.wide ? logprob_kernel<T, W> : logprob_kernel<T, 1>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(LpShared));
+    auto kern = a.wide ? logprob_kernel<T, W, NT> : logprob_kernel<T, 1, NT>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(LpShared<NT>));
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(rows * a.cluster));
-    cfg.blockDim = dim3(kLpThreads);
-    cfg.dynamicSmemBytes = sizeof(LpShared);
+    cfg.blockDim = dim3(NT);
+    cfg.dynamicSmemBytes = sizeof(LpShared<NT>);
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -553,6 +565,11 @@ cudaError_t go(const LogprobArgs& a, int rows, cudaStream_t s) {
     cfg.attrs = attr;
     cfg.numAttrs = a.cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kern, a);
+}
+
+template <typename T>
+cudaError_t go(const LogprobArgs& a, int rows, cudaStream_t s) {
+    return a.n <= kLpShortRow ? go_threads<T, 128>(a, rows, s) : go_threads<T, 256>(a, rows, s);
 }
 
 }  // namespace

@@ -430,6 +430,20 @@ def test_attention_paged_long_and_many(lens, dtype, cache):
     p.check(*p.call())
 
 
+def test_attention_paged_thousands_of_rows():
+    """More rows than threads in the scan; a wider table than it needs; no lse."""
+    g = np.random.default_rng(0)
+    lens = [int(n) for n in g.integers(0, 40, 3000)]
+    p = Paged(lens, 4, 2, 64, 16, "bf16", "bf16")
+    wide = torch.full((p.R, p.max_pages + 5), 10**9, dtype=torch.int32, device="cuda")
+    wide[:, :p.max_pages] = p.table
+    want = p.call()
+    p.check(*want)
+    p.table = wide
+    out, ls = p.call(lse=False, table_stride=wide.stride(0))
+    assert torch.equal(out, want[0]) and bool((ls == 5).all())
+
+
 def test_attention_paged_window_ignores_freed_pages():
     p = Paged([1000, 130], 4, 2, 64, 16, "f16", "f16")
     want = p.call(window=100)
