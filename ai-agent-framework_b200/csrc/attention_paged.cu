@@ -43,8 +43,8 @@
 // rounded once at the end.
 //
 // Measured (8 KV heads of 128, HBM copies run at 6.5 TB/s): 8 x 32K, fp32 rows,
-// 32 heads: 162 us, 6.6 TB/s; 64 sequences of 16 .. 16384, bf16, 64 heads: 112 us,
-// 5.8 TB/s, the ragged ends and 4 us of joining being the rest; 1 x 4K: 13.5 us,
+// 32 heads: 160 us, 6.7 TB/s; 64 sequences of 16 .. 16384, bf16, 64 heads: 110 us,
+// 5.9 TB/s, the ragged ends and 4 us of joining being the rest; 1 x 4K: 11.5 us,
 // two launches and a chain of dependent loads (lengths, pages, K and V, pieces).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -75,7 +75,6 @@ struct PagedArgs {
     void* out;
     float* lse;
     float* part;   // [workers][2][heads][hd + 2]: o, m (log2 units), l
-    int2* desc;    // [batch]: first and last group of each sequence
     const float* slopes;
     int64_t q_stride, out_stride, table_stride, page_stride, pos_stride, head_stride;
     int batch, nh, nkv, grp, heads, rt, hd, page_size, page_shift, n_pages, max_pages, n_req, len_add, window, groups, sms;
@@ -102,15 +101,13 @@ __device__ __forceinline__ Seq seq_of(const PagedArgs& a, int b) {
     return s;
 }
 
-template <int STEP>
-__device__ __forceinline__ int steps_of(const Seq& s) {
-    return s.len == 0 ? 0 : (s.len - 1) / STEP - s.lo / STEP + 1;
+// steps of sequence s, positions [lo, len), of `step` positions (16 or 32)
+__device__ __forceinline__ int steps_of(const Seq& s, int step) {
+    const int sh = step == 16 ? 4 : 5;
+    return s.len == 0 ? 0 : ((s.len - 1) >> sh) - (s.lo >> sh) + 1;
 }
 // units of sequence s: its steps behind the overhead
-template <int STEP>
-__device__ __forceinline__ int units_of(const Seq& s) {
-    return s.len == 0 ? 0 : steps_of<STEP>(s) + kOverhead;
-}
+__device__ __forceinline__ int units_of(const Seq& s, int step) { return s.len == 0 ? 0 : steps_of(s, step) + kOverhead; }
 
 __device__ __forceinline__ void cp16(uint32_t smem, const void* gmem, bool valid) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(valid ? 16 : 0) : "memory");
@@ -217,6 +214,11 @@ __device__ __forceinline__ long long mul_div(long long x, long long y, long long
     return p <= 0xffffffffLL ? (long long)((unsigned)p / (unsigned)z) : p / z;
 }
 
+// How many groups share W units; group g has the units from mul_div(g, W, G) on.
+__device__ __forceinline__ long long groups_for(const PagedArgs& a, long long W) {
+    return max(1LL, min((long long)a.groups, mul_div(W, 1, kMinUnits)));
+}
+
 // A worker's place in its units: step `step` of the `ns` of row b, up to `end`
 // of which are its share; `left` units of its share lie behind this row.
 template <int STEP>
@@ -238,7 +240,7 @@ struct Cursor {
             if (left <= 0) return false;
             do {
                 sq = seq_of(a, ++b);
-                ns = steps_of<STEP>(sq);
+                ns = steps_of(sq, STEP);
             } while (ns == 0);
             enter(0);
         }
@@ -284,8 +286,8 @@ __global__ void __launch_bounds__(Sm<HD, NG>::kThreads) paged_split_kernel(const
     extern __shared__ __align__(1024) uint8_t psm[];
     __shared__ long long wsum[kWarps];
     __shared__ long long chunk[kThreads];  // units before the end of each thread's sequences
-    pdl_trigger();
     pdl_wait();
+    pdl_trigger();  // (behind the wait: the joining launch reads the lengths before its own)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gi = lane >> 2, ti = lane & 3;
     const int hd = a.hd, hc = hd / 8, rpb = a.nkv * a.rt;
     uint8_t* const ring = psm + warp * SM::kWarp;
@@ -299,7 +301,7 @@ __global__ void __launch_bounds__(Sm<HD, NG>::kThreads) paged_split_kernel(const
     {
         const int b0 = min(a.batch, tid * per), b1 = min(a.batch, b0 + per);
         long long inc = 0;
-        for (int b = b0; b < b1; b++) inc += units_of<STEP>(seq_of(a, b));
+        for (int b = b0; b < b1; b++) inc += units_of(seq_of(a, b), STEP);
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const long long x = __shfl_up_sync(0xffffffffu, inc, o);
@@ -314,7 +316,7 @@ __global__ void __launch_bounds__(Sm<HD, NG>::kThreads) paged_split_kernel(const
     }
     __syncthreads();
     const long long W = chunk[kThreads - 1];
-    const long long G = max(1LL, min((long long)a.groups, mul_div(W, 1, kMinUnits)));
+    const long long G = groups_for(a, W);
     const int worker = warp * gridDim.x + blockIdx.x;  // neighbours on different SMs
     const int group = worker / rpb, hr = worker - group * rpb;
     if (group >= G || W == 0) return;
@@ -328,13 +330,13 @@ __global__ void __launch_bounds__(Sm<HD, NG>::kThreads) paged_split_kernel(const
         int b = c * per;
         while (true) {
             ld.sq = seq_of(a, b);
-            const int n = units_of<STEP>(ld.sq);
+            const int n = units_of(ld.sq, STEP);
             if (u0 < base + n) break;
             base += n;
             b++;
         }
         ld.b = b;
-        ld.ns = steps_of<STEP>(ld.sq);
+        ld.ns = steps_of(ld.sq, STEP);
         ld.left = u1 - u0;
         ld.enter((int)(u0 - base));
     }
@@ -660,50 +662,83 @@ __global__ void __launch_bounds__(Sm<HD, NG>::kThreads) paged_split_kernel(const
                     if (gi == 0) *reinterpret_cast<float2*>(part + hd) = make_float2(y, x);
                 }
             }
-        if (to_end && hr == 0 && lane == 0) {
-            // the group that holds the first step's unit u: floor(((u + 1) G - 1) / W)
-            int c0 = group;
-            if (!from_start) c0 = (int)mul_div(u1 - cu.left - cu.ns + 1, G, W, -1);
-            a.desc[cu.b] = make_int2(c0, group);
-        }
         if (!cu.settle(a)) break;
     }
     cp_wait<0>();
 }
 
-// One CTA per (row, KV head, block of query heads), or per query head of it
-// (blockIdx.y): joins the pieces of a row that was cut, and fills a row that sees nothing (zeros, lse
-// -inf) or whose length passes its table (NaN).  The 8 warps are 8 / pw heads
-// times pw shares of the pieces; a lane holds ND pairs of a head (hd <= 64 ND).
-template <typename T, int ND>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedArgs a, int pw) {
+// CTAs (row, blockIdx.y), the y shares taking the row's query heads in turn:
+// join the pieces of a row that was cut, and fill a row that sees nothing
+// (zeros, lse -inf) or whose length passes its table (NaN).  The 8 warps are 8 /
+// PW heads times PW shares of the pieces; a lane holds ND pairs of a head (hd <=
+// 64 ND).  PW = 8 is for few heads, one to a CTA, PW = 1 for many.  Which groups hold the row's pieces follows from the
+// lengths, worked out while the split kernel still runs.
+template <typename T, int ND, int PW>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedArgs a, int step) {
     __shared__ __align__(8) float red[kJoinWarps][kPagedMaxHd + 2];
+    __shared__ long long sums[2][kJoinWarps];
     pdl_trigger();
-    pdl_wait();
-    const int rpb = a.nkv * a.rt, b = blockIdx.x / rpb, hr = blockIdx.x - b * rpb, hd = a.hd;
-    const int h = hr / a.rt, row0 = (hr - h * a.rt) * a.heads, rows = min(a.heads, a.grp - row0), head0 = h * a.grp + row0;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rw = kJoinWarps / pw, share = warp % pw;
+    const int rpb = a.nkv * a.rt, b = blockIdx.x, hd = a.hd, nh = a.nh;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, share = warp % PW;
+    constexpr int rw = kJoinWarps / PW;
     const float nan = __int_as_float(0x7fc00000);
-    int2 c = a.desc[b];  // (not used before sq says that it was written)
+    // the lengths are older than the split kernel, which has seen its predecessor end before it let this one start
     const Seq sq = seq_of(a, b);
+    int2 c = make_int2(0, 0);  // first and last group of the row
+    {
+        long long before = 0, all = 0;
+        for (int i = threadIdx.x; i < a.batch; i += kJoinThreads) {
+            const int n = units_of(seq_of(a, i), step);
+            all += n;
+            if (i < b) before += n;
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            before += __shfl_xor_sync(0xffffffffu, before, o);
+            all += __shfl_xor_sync(0xffffffffu, all, o);
+        }
+        if (lane == 0) {
+            sums[0][warp] = before;
+            sums[1][warp] = all;
+        }
+        __syncthreads();
+        before = all = 0;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; w++) {
+            before += sums[0][w];
+            all += sums[1][w];
+        }
+        if (sq.len) {  // the group of unit u: floor(((u + 1) G - 1) / W)
+            const long long G = groups_for(a, all);
+            c.x = (int)mul_div(before + kOverhead + 1, G, all, -1);
+            c.y = (int)mul_div(before + units_of(sq, step), G, all, -1);
+        }
+    }
+    // a head's place among the workers: KV head, block of its group, row of the block
+    const int64_t ps = (int64_t)a.heads * (hd + 2);  // floats of a piece; a group's are 2 rpb pieces apart
+    auto place = [&](int head) {
+        const int h = head / a.grp, in = head - h * a.grp, blk = in / a.heads;
+        return a.part + (int64_t)2 * (h * a.rt + blk) * ps + (in - blk * a.heads) * (hd + 2);
+    };
+    int first = blockIdx.y * rw;
+    const float* base = place(first + warp / PW);  // (worked out before the wait)
+    pdl_wait();
     if (sq.len && c.x == c.y) return;
-    for (int rb = blockIdx.y * rw; rb < rows; rb += gridDim.y * rw) {
-        const int r = rb + warp / pw;
-        const bool live = r < rows;
-        constexpr int NP = 4;  // pieces in flight
+    for (; first < nh; first += gridDim.y * rw, base = place(first + warp / PW)) {  // (once where PW > 1)
+        const int head = first + warp / PW;
+        const bool live = head < nh;
+        constexpr int NP = ND <= 2 ? 8 : 4;  // pieces in flight
         float2 o[ND];
         float M = -INFINITY, L = 0.0f;
         bool bad = false;
 #pragma unroll
         for (int j = 0; j < ND; j++) o[j] = make_float2(0.0f, 0.0f);
         if (live && sq.len) {
-            const float* base = a.part + ((int64_t)2 * hr * a.heads + r) * (hd + 2);
-            const int64_t ps = (int64_t)a.heads * (hd + 2);  // of a piece; a group's are 2 rpb apart
-            for (int i0 = c.x + share; i0 <= c.y; i0 += NP * pw) {
+            for (int i0 = c.x + share; i0 <= c.y; i0 += NP * PW) {
                 float2 ml[NP], x[NP][ND];
 #pragma unroll
                 for (int k = 0; k < NP; k++) {
-                    const int i = i0 + k * pw;
+                    const int i = i0 + k * PW;
                     const float* p = base + (2 * (int64_t)i * rpb + (i == c.x ? 1 : 0)) * ps;
                     ml[k] = i <= c.y ? *reinterpret_cast<const float2*>(p + hd) : make_float2(-INFINITY, 0.0f);
 #pragma unroll
@@ -739,7 +774,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
             }
             if (bad) M = L = nan;
         }
-        if (pw > 1) {  // the shares of a head meet in its first warp
+        if constexpr (PW > 1) {  // the shares of a head meet in its first warp
 #pragma unroll
             for (int j = 0; j < ND; j++)
                 if (2 * lane + 64 * j < hd) *reinterpret_cast<float2*>(&red[warp][2 * lane + 64 * j]) = o[j];
@@ -748,7 +783,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
             if (share == 0) {
                 float N = M;
                 bool any = M != M;
-                for (int w = 1; w < pw; w++) {
+                for (int w = 1; w < PW; w++) {
                     const float m = red[warp + w][kPagedMaxHd];
                     any |= m != m;
                     N = fmaxf(N, m);
@@ -760,7 +795,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
                     o[j].x *= f;
                     o[j].y *= f;
                 }
-                for (int w = 1; w < pw; w++) {
+                for (int w = 1; w < PW; w++) {
                     const float2 ml = *reinterpret_cast<const float2*>(&red[warp + w][kPagedMaxHd]);
                     const float g = ex2(ml.x - z);
                     L = fmaf(ml.y, g, L);
@@ -780,7 +815,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
         if (live && share == 0) {
             if (sq.bad) M = L = nan;
             const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-            T* out = static_cast<T*>(a.out) + (int64_t)b * a.out_stride + (int64_t)(head0 + r) * hd;
+            T* out = static_cast<T*>(a.out) + (int64_t)b * a.out_stride + (int64_t)head * hd;
 #pragma unroll
             for (int j = 0; j < ND; j++) {
                 const int d = 2 * lane + 64 * j;
@@ -790,8 +825,9 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
                 }
             }
             if (a.lse && lane == 0)
-                a.lse[(int64_t)b * a.nh + head0 + r] = L == 0.0f ? -INFINITY : (M + (log2f(L) - 14.0f)) * kLn2;
+                a.lse[(int64_t)b * nh + head] = L == 0.0f ? -INFINITY : (M + (log2f(L) - 14.0f)) * kLn2;
         }
+        if (PW > 1) break;
     }
 }
 
@@ -813,11 +849,12 @@ cudaError_t go(const PagedArgs& a, cudaStream_t s) {
     }
     e = launch_pdl(kern, dim3((a.groups * a.nkv * a.rt + SM::kWarps - 1) / SM::kWarps), dim3(SM::kThreads), smem, s, a);
     if (e != cudaSuccess) return e;
-    // few rows: a CTA per query head, its pieces over the 8 warps; many: a warp per head
-    const int rows = a.batch * a.nkv * a.rt, heads = std::min(a.grp, a.heads);
-    return rows * heads <= 2 * a.sms
-               ? launch_pdl(paged_join_kernel<T, HD / 64>, dim3(rows, heads), dim3(kJoinThreads), 0, s, a, kJoinWarps)
-               : launch_pdl(paged_join_kernel<T, HD / 64>, dim3(rows, 1), dim3(kJoinThreads), 0, s, a, 1);
+    // few heads in all: a CTA for each, its pieces over the 8 warps; many: a warp
+    // for each, as many CTAs as the machine holds beside the split kernel
+    if ((long long)a.batch * a.nh <= 2 * a.sms)
+        return launch_pdl(paged_join_kernel<T, HD / 64, kJoinWarps>, dim3(a.batch, a.nh), dim3(kJoinThreads), 0, s, a, SM::kStep);
+    const int y = std::max(1, std::min((a.nh + kJoinWarps - 1) / kJoinWarps, 4 * a.sms / a.batch));
+    return launch_pdl(paged_join_kernel<T, HD / 64, 1>, dim3(a.batch, y), dim3(kJoinThreads), 0, s, a, SM::kStep);
 }
 
 // Query heads of one unit: 16 for groups past 8, so that K and V are read
@@ -860,7 +897,8 @@ size_t attention_paged_scratch(int batch, int nh, int nkv, int hd, int sms) {
     const int grp = nh / nkv;
     size_t n = part_bytes(hd, 8, nkv * ((grp + 7) / 8), sms);
     if (grp > 8) n = std::max(n, part_bytes(hd, 16, nkv * ((grp + 15) / 16), sms));
-    return n + (size_t)batch * sizeof(int2);
+    (void)batch;  // (the pieces are the workers', whatever the batch)
+    return n;
 }
 
 int launch_attention_paged(const b2_paged_kv& kv, const b2_paged_attn_opts& o, const void* q, const int32_t* table,
@@ -881,7 +919,6 @@ int launch_attention_paged(const b2_paged_kv& kv, const b2_paged_attn_opts& o, c
     a.grp = o.nh / kv.nkv;
     a.heads = unit_heads(kv.hd, a.grp, o.dtype);
     a.rt = (a.grp + a.heads - 1) / a.heads;
-    a.desc = reinterpret_cast<int2*>(static_cast<uint8_t*>(scratch) + part_bytes(kv.hd, a.heads, kv.nkv * a.rt, sms));
     a.slopes = o.slopes;
     const int64_t qd = (int64_t)o.nh * kv.hd;
     a.q_stride = o.q_stride ? o.q_stride : qd;
