@@ -77,7 +77,8 @@ struct PagedArgs {
     float* part;   // [workers][2][heads][hd + 2]: o, m (log2 units), l
     const float* slopes;
     int64_t q_stride, out_stride, table_stride, page_stride, pos_stride, head_stride;
-    int batch, nh, nkv, grp, heads, rt, hd, page_size, page_shift, n_pages, max_pages, n_req, len_add, window, groups, sms;
+    int batch, nh, nkv, grp, heads, rt, hd, page_size, page_shift, n_pages, max_pages, n_req;
+    int len_add, window, groups, sms;
     // heads: query heads of one unit (8 or 16); rt: blocks of that many in a group;
     // page_shift: log2 of the page size, or -1
     int q_pairs;   // q's rows can be read two elements at a time
@@ -440,7 +441,8 @@ __global__ void __launch_bounds__(Sm<HD, NG>::kThreads) paged_split_kernel(const
 #pragma unroll
         for (int g = 0; g < NG; g++) {
             const bool v = 8 * g + gi < heads, pairs = a.q_pairs;
-            const T* q0 = static_cast<const T*>(a.q) + (int64_t)cu.b * a.q_stride + (int64_t)(head0 + (v ? 8 * g + gi : 0)) * hd;
+            const T* q0 = static_cast<const T*>(a.q) + (int64_t)cu.b * a.q_stride +
+                          (int64_t)(head0 + (v ? 8 * g + gi : 0)) * hd;
             float x[KS][4];
 #pragma unroll
             for (int kk = 0; kk < KS; kk++)
@@ -478,7 +480,8 @@ __global__ void __launch_bounds__(Sm<HD, NG>::kThreads) paged_split_kernel(const
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 ks[g][j] = __shfl_sync(0xffffffffu, factor, 4 * (2 * ti + j));
-                sl[g][j] = a.slopes && 8 * g + 2 * ti + j < heads ? __ldg(a.slopes + head0 + 8 * g + 2 * ti + j) * kLog2e : 0.0f;
+                const int head = 8 * g + 2 * ti + j;
+                sl[g][j] = a.slopes && head < heads ? __ldg(a.slopes + head0 + head) * kLog2e : 0.0f;
             }
         }
 
@@ -852,7 +855,8 @@ cudaError_t go(const PagedArgs& a, cudaStream_t s) {
     // few heads in all: a CTA for each, its pieces over the 8 warps; many: a warp
     // for each, as many CTAs as the machine holds beside the split kernel
     if ((long long)a.batch * a.nh <= 2 * a.sms)
-        return launch_pdl(paged_join_kernel<T, HD / 64, kJoinWarps>, dim3(a.batch, a.nh), dim3(kJoinThreads), 0, s, a, SM::kStep);
+        return launch_pdl(paged_join_kernel<T, HD / 64, kJoinWarps>, dim3(a.batch, a.nh), dim3(kJoinThreads), 0, s, a,
+                          SM::kStep);
     const int y = std::max(1, std::min((a.nh + kJoinWarps - 1) / kJoinWarps, 4 * a.sms / a.batch));
     return launch_pdl(paged_join_kernel<T, HD / 64, 1>, dim3(a.batch, y), dim3(kJoinThreads), 0, s, a, SM::kStep);
 }
@@ -882,8 +886,10 @@ int groups_in(int rpb, int sms) {
     return std::max(1, Sm<HD, NG>::kCtas * Sm<HD, NG>::kWarps * sms / rpb);
 }
 int groups_of(int hd, int heads, int rpb, int sms) {
-    if (heads == 16) return hd <= 64 ? groups_in<64, 2>(rpb, sms) : hd <= 128 ? groups_in<128, 2>(rpb, sms) : groups_in<256, 2>(rpb, sms);
-    return hd <= 64 ? groups_in<64, 1>(rpb, sms) : hd <= 128 ? groups_in<128, 1>(rpb, sms) : groups_in<256, 1>(rpb, sms);
+    const bool two = heads == 16;
+    if (hd <= 64) return two ? groups_in<64, 2>(rpb, sms) : groups_in<64, 1>(rpb, sms);
+    if (hd <= 128) return two ? groups_in<128, 2>(rpb, sms) : groups_in<128, 1>(rpb, sms);
+    return two ? groups_in<256, 2>(rpb, sms) : groups_in<256, 1>(rpb, sms);
 }
 
 size_t part_bytes(int hd, int heads, int rpb, int sms) {

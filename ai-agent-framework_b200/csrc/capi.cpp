@@ -671,7 +671,8 @@ int b2_page_plan(const int32_t* cached, const int32_t* fresh, int32_t n_req, int
         if (n_req <= 0 || n_req > b2::kPlanMaxReq)
             return ret(B2_ERR_BAD_ARG, "b2_page_plan: takes 1 to 16384 requests");
         if (page_size <= 0 || max_pages <= 0 || max_tokens <= 0 || table_stride < max_pages)
-            return ret(B2_ERR_BAD_ARG, "b2_page_plan: page_size, max_pages and max_tokens must be positive, table_stride >= max_pages");
+            return ret(B2_ERR_BAD_ARG,
+                       "b2_page_plan: page_size, max_pages and max_tokens must be positive, table_stride >= max_pages");
         int rc = on_device("b2_page_plan", {{"cached", cached, 4}, {"fresh", fresh, 4}, {"free_pages", free_pages, 4},
                                             {"n_free", n_free, 4}, {"table", table, 4}, {"lens", lens, 4},
                                             {"starts", starts, 4}, {"slots", slots, 8}, {"positions", positions, 4},
@@ -797,14 +798,16 @@ int b2_logprobs(const void* logits, int32_t dtype, int32_t n, int32_t rows, int6
     return guarded([&] {
         if (!logits || n <= 0 || n > (1 << 30) || rows <= 0 || ld < n || m < 0 || k < 0)
             return ret(B2_ERR_BAD_ARG, "b2_logprobs: bad argument");
-        if (!float_type(dtype)) return ret(B2_ERR_UNSUPPORTED_TYPE, "b2_logprobs: dtype must be 0 (F32), 1 (F16) or 30 (BF16)");
+        if (!float_type(dtype))
+            return ret(B2_ERR_UNSUPPORTED_TYPE, "b2_logprobs: dtype must be 0 (F32), 1 (F16) or 30 (BF16)");
         if (k > b2::kLogprobMaxTop || k > n) return ret(B2_ERR_BAD_ARG, "b2_logprobs: at most 64 alternatives, and n");
         if ((m && (!ids || !logprob)) || (k && (!top_ids || !top_logprob)))
             return ret(B2_ERR_BAD_ARG, "b2_logprobs: null argument");
         if (!m && !k && !entropy) return B2_OK;
         int rc = on_device("b2_logprobs", {{"logits", logits, type_bytes(dtype)}, {"ids", m ? ids : nullptr, 4},
                                            {"logprob", m ? logprob : nullptr, 4}, {"entropy", entropy, 4},
-                                           {"top_ids", k ? top_ids : nullptr, 4}, {"top_logprob", k ? top_logprob : nullptr, 4}});
+                                           {"top_ids", k ? top_ids : nullptr, 4},
+                                           {"top_logprob", k ? top_logprob : nullptr, 4}});
         if (rc != B2_OK) return rc;
         std::string err;
         rc = b2::launch_logprobs(logits, dtype, n, rows, ld, ids, m, logprob, entropy, k, top_ids, top_logprob,

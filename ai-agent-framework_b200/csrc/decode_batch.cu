@@ -980,10 +980,13 @@ int b2_batch_logprobs_impl(const b2_batch* bt, int rows, const int32_t* ids, int
     float* d_ent = d_lp + nm;
     int32_t* d_ti = reinterpret_cast<int32_t*>(d_ent + rows);
     float* d_tl = reinterpret_cast<float*>(d_ti + nk);
-    int rc = nm && !ok(cudaMemcpyAsync(d, host.data(), nm * sizeof(int32_t), cudaMemcpyHostToDevice, s), err, "ids") ? B2_ERR_CUDA : B2_OK;
+    int rc = B2_OK;
+    if (nm && !ok(cudaMemcpyAsync(d, host.data(), nm * sizeof(int32_t), cudaMemcpyHostToDevice, s), err, "ids"))
+        rc = B2_ERR_CUDA;
     if (rc == B2_OK)
         rc = launch_logprobs(bt->logits, 0, bt->m->dev.V, rows, bt->m->dev.V, d, m, d_lp, d_ent, k, d_ti, d_tl, s, err);
-    if (rc == B2_OK && !ok(cudaMemcpyAsync(host.data() + nm, d + nm, (n - nm) * sizeof(int32_t), cudaMemcpyDeviceToHost, s), err, "scores"))
+    const size_t back = (n - nm) * sizeof(int32_t);
+    if (rc == B2_OK && !ok(cudaMemcpyAsync(host.data() + nm, d + nm, back, cudaMemcpyDeviceToHost, s), err, "scores"))
         rc = B2_ERR_CUDA;
     cudaFreeAsync(d, s);
     if (!ok(cudaStreamSynchronize(s), err, "scores") && rc == B2_OK) rc = B2_ERR_CUDA;

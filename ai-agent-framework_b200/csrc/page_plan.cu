@@ -128,8 +128,10 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const __grid_co
             wp = sat_add(wp, p);
         }
     }
-    const unsigned total_tok = __shfl_sync(0xffffffffu, wt, kPlanWarps - 1), total_pg = __shfl_sync(0xffffffffu, wp, kPlanWarps - 1);
-    const unsigned bt = __shfl_sync(0xffffffffu, wt, max(warp - 1, 0)), bp = __shfl_sync(0xffffffffu, wp, max(warp - 1, 0));
+    const unsigned total_tok = __shfl_sync(0xffffffffu, wt, kPlanWarps - 1);
+    const unsigned total_pg = __shfl_sync(0xffffffffu, wp, kPlanWarps - 1);
+    const unsigned bt = __shfl_sync(0xffffffffu, wt, max(warp - 1, 0));
+    const unsigned bp = __shfl_sync(0xffffffffu, wp, max(warp - 1, 0));
     if (warp) {
         it = sat_add(it, bt);
         ip = sat_add(ip, bp);
@@ -193,7 +195,8 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const __grid_co
                 in[j] = pos[j] - idx * a.page_size;
                 req[j] = r;
                 // (a page of this step comes from the list: its table entry may be another CTA's to write)
-                page[j] = *(idx < have ? a.table + ((int64_t)r * a.table_stride + idx) : a.free_pages + (taken[r] + idx - have));
+                page[j] = *(idx < have ? a.table + ((int64_t)r * a.table_stride + idx)
+                                       : a.free_pages + (taken[r] + idx - have));
             }
         }
         int64_t* slots = a.slots + t0 + lane;

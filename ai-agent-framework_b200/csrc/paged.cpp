@@ -42,9 +42,11 @@ int check_device_pointers(const DevicePtr* p, int n, std::string* err) {
         e = cudaPointerGetAttributes(&at, p[i].p);
         if (e != cudaSuccess) break;
         if (at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeDevice && at.device == dev)) continue;
-        *err = std::string(p[i].name) + (at.type == cudaMemoryTypeDevice
-                                             ? " is on device " + std::to_string(at.device) + ", the current device is " + std::to_string(dev)
-                                             : std::string(" is not device memory"));
+        *err = p[i].name;
+        if (at.type == cudaMemoryTypeDevice)
+            *err += " is on device " + std::to_string(at.device) + ", the current device is " + std::to_string(dev);
+        else
+            *err += " is not device memory";
         return B2_ERR_BAD_ARG;
     }
     return e == cudaSuccess ? B2_OK : cuda_failed("no CUDA device", e, err);
@@ -71,7 +73,8 @@ int cuda_failed(const char* what, cudaError_t e, std::string* err) {
 int b2_rope_freqs_impl(const b2_rope_opts& o, double* freqs, float* scale) {
     const int rot = o.rot_dim;
     const double two_pi = 6.283185307179586476925;
-    const double low = o.low > 0 ? o.low : 1.0, high = o.high > 0 ? o.high : (o.scaling == B2_ROPE_SCALE_YARN ? 32.0 : 4.0);
+    const double low = o.low > 0 ? o.low : 1.0;
+    const double high = o.high > 0 ? o.high : (o.scaling == B2_ROPE_SCALE_YARN ? 32.0 : 4.0);
     if (!(high > low)) return B2_ERR_BAD_ARG;
     auto pair = [&](double turns) { return rot * std::log(o.orig_ctx / (turns * two_pi)) / (2 * std::log(o.theta)); };
     double lo = 0, hi = 0;

@@ -30,7 +30,8 @@
 namespace b2 {
 namespace {
 
-constexpr int kRopeThreads = 128;  // (32768 rows back to back: 219 us; 226 with 256, 266 with 512: a CTA waits for its sines first)
+// (32768 rows back to back: 219 us; 226 with 256, 266 with 512: a CTA waits for its sines first)
+constexpr int kRopeThreads = 128;
 
 struct RopeArgs {
     const double* freqs;
