@@ -209,10 +209,11 @@ __device__ __forceinline__ float2 pair_of(const __nv_bfloat16* p, bool pairs) {
                  : make_float2(__bfloat162float(p[0]), __bfloat162float(p[1]));
 }
 
-// (x * y + add) / z, exact; in 32 bits where they do (a 64-bit division is some 100 instructions)
+// (x * y + add) / z, none negative, exact; in 32 bits where they do (a 64-bit
+// division is some 100 instructions)
 __device__ __forceinline__ long long mul_div(long long x, long long y, long long z, int add = 0) {
     const long long p = x * y + add;
-    return p <= 0xffffffffLL ? (long long)((unsigned)p / (unsigned)z) : p / z;
+    return (p | z) <= 0xffffffffLL ? (long long)((unsigned)p / (unsigned)z) : p / z;
 }
 
 // How many groups share W units; group g has the units from mul_div(g, W, G) on.
