@@ -22,7 +22,6 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <atomic>
 
 #include "dev.cuh"
 #include "paged.h"
