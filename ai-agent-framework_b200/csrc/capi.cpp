@@ -13,6 +13,7 @@
 
 #include "gemm.h"
 #include "model.h"
+#include "overlap.h"
 #include "paged.h"
 #include "sample.h"
 
@@ -681,7 +682,8 @@ int b2_page_plan(const int32_t* cached, const int32_t* fresh, int32_t n_req, int
         const b2::PagePlanArgs a{cached, fresh,     free_pages, n_free, table, table_stride, lens,      starts,
                                  slots,  positions, token_req,  info,   n_req, page_size,    max_pages, max_tokens,
                                  0,      0};
-        std::string err;
+        std::string err = b2::page_plan_overlap(a);
+        if (!err.empty()) return ret(B2_ERR_BAD_ARG, "b2_page_plan: " + err);
         rc = b2::launch_page_plan(a, static_cast<cudaStream_t>(stream), &err);
         return ret(rc, err);
     });

@@ -320,7 +320,8 @@ int b2_batch_use_graph(b2_batch* b, int32_t on);
  * B2_ERR_BAD_ARG), asynchronous on `stream` (a cudaStream_t; NULL = the legacy
  * default stream), no allocation, no state kept between calls, capturable in a
  * CUDA graph.  Calls that overlap on the GPU must not share outputs or
- * scratch.  Types are ggml type ids: 0 = F32, 1 = F16, 30 = BF16.  The Go
+ * scratch.  An output shares no memory with an input or another output, unless
+ * its entry point says that it may.  Types are ggml type ids: 0 = F32, 1 = F16, 30 = BF16.  The Go
  * engine has one contiguous cache per sequence (kvCache,
  * transformer.go:88-92); these have no counterpart there beyond the
  * arithmetic cited. */
@@ -365,7 +366,12 @@ typedef struct {
  * A step that does not fit (status != 0, B2_PLAN_* bits) leaves the table as
  * it was and is an empty one otherwise: every token row -1, starts 0, lens =
  * cached.  A token in a page whose table or list entry is negative gets slot
- * -1.  No two requests may share a page that either still writes. */
+ * -1.  No two requests may share a page that either still writes.  The outputs
+ * and the table share no memory with cached, fresh, n_free, free_pages or one
+ * another (the lengths are read again while others are written, so lens is no
+ * update of cached in place): a call whose output meets an input or the table
+ * fails with B2_ERR_BAD_ARG, for free_pages as far as its first entry, its
+ * length being on the device. */
 int b2_page_plan(const int32_t* cached, const int32_t* fresh, int32_t n_req, int32_t page_size,
                  const int32_t* free_pages, const int32_t* n_free, int32_t* table, int64_t table_stride,
                  int32_t max_pages, int32_t* lens, int32_t* starts, int64_t* slots, int32_t* positions,
