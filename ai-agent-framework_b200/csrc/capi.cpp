@@ -62,9 +62,17 @@ auto guarded(F&& body) noexcept -> decltype(body()) {
 
 bool float_type(int32_t t) { return t == 0 || t == 1 || t == 30; }
 
-int on_device(const char* who, std::initializer_list<b2::DevicePtr> ptrs) {
+int aligned(const char* who, std::initializer_list<b2::DevicePtr> ptrs) {
     std::string err;
-    const int rc = b2::check_device_pointers(ptrs.begin(), (int)ptrs.size(), &err);
+    const int rc = b2::check_alignment(ptrs.begin(), (int)ptrs.size(), &err);
+    return rc == B2_OK ? rc : ret(rc, std::string(who) + ": " + err);
+}
+
+int on_device(const char* who, std::initializer_list<b2::DevicePtr> ptrs) {
+    int rc = aligned(who, ptrs);
+    if (rc != B2_OK) return rc;
+    std::string err;
+    rc = b2::check_device_pointers(ptrs.begin(), (int)ptrs.size(), &err);
     return rc == B2_OK ? rc : ret(rc, std::string(who) + ": " + err);
 }
 
@@ -741,9 +749,15 @@ int b2_rope_append(const b2_rope_rows* rows, const b2_paged_kv* kv, const double
         if (r.dtype != 0 && r.dtype != c.dtype)
             return ret(B2_ERR_UNSUPPORTED_TYPE, "b2_rope_append: rows must be F32 or of the cache's type");
         const size_t es = type_bytes(r.dtype);
-        rc = on_device("b2_rope_append", {{"q", q, es}, {"k", k, es}, {"v", v, es}, {"q_out", q_out, es},
-                                          {"the cache's k", c.k, 16}, {"the cache's v", c.v, 16}, {"slots", slots, 8},
-                                          {"positions", positions, 4}, {"freqs", r.rot_dim ? freqs : nullptr, 8}});
+        const std::initializer_list<b2::DevicePtr> ptrs = {
+            {"q", q, es}, {"k", k, es}, {"v", v, es}, {"q_out", q_out, es}, {"the cache's k", c.k, 16},
+            {"the cache's v", c.v, 16}, {"slots", slots, 8}, {"positions", positions, 4},
+            {"freqs", r.rot_dim ? freqs : nullptr, 8}};
+        rc = aligned("b2_rope_append", ptrs);
+        if (rc != B2_OK) return rc;
+        if (!b2::kv_places_apart(c))
+            return ret(B2_ERR_BAD_ARG, "b2_rope_append: the cache's strides, or k and v, place elements on one another");
+        rc = on_device("b2_rope_append", ptrs);
         if (rc != B2_OK) return rc;
         std::string err;
         rc = b2::launch_rope(r, &c, freqs, positions, slots, n_tok, q, k, v, q_out, nullptr,

@@ -46,4 +46,25 @@ inline std::string page_plan_overlap(const PagePlanArgs& a) {
     return "";
 }
 
+// Whether the places of a cache are apart: pages, positions and heads, and k
+// and v, each taken with its distance, from the smallest distance up; every
+// distance has to pass the extent of the ones before it.  (Distances that
+// interleave without meeting in any other way are refused too.)
+inline bool kv_places_apart(const b2_paged_kv& kv) {
+    struct Dim {
+        __int128 step, n;
+    };
+    const __int128 k = (uintptr_t)kv.k, v = (uintptr_t)kv.v;
+    Dim d[] = {{(__int128)2 * kv.page_stride, kv.n_pages}, {(__int128)2 * kv.pos_stride, kv.page_size},
+               {(__int128)2 * kv.head_stride, kv.nkv}, {k < v ? v - k : k - v, 2}};
+    std::sort(d, d + 4, [](const Dim& a, const Dim& b) { return a.step < b.step; });
+    __int128 extent = 2 * kv.hd;
+    for (const Dim& x : d) {
+        if (x.n == 1) continue;
+        if (x.step < extent) return false;
+        extent += (x.n - 1) * x.step;
+    }
+    return true;
+}
+
 }  // namespace b2

@@ -28,12 +28,16 @@ int current_sms(std::string* err) {
     return n;
 }
 
-int check_device_pointers(const DevicePtr* p, int n, std::string* err) {
+int check_alignment(const DevicePtr* p, int n, std::string* err) {
     for (int i = 0; i < n; i++)
         if (reinterpret_cast<uintptr_t>(p[i].p) & (p[i].align - 1)) {
             *err = std::string(p[i].name) + " must be " + std::to_string(p[i].align) + "-byte aligned";
             return B2_ERR_BAD_ARG;
         }
+    return B2_OK;
+}
+
+int check_device_pointers(const DevicePtr* p, int n, std::string* err) {
     int dev = -1;
     cudaError_t e = cudaGetDevice(&dev);
     for (int i = 0; i < n && e == cudaSuccess; i++) {

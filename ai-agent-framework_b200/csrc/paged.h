@@ -62,9 +62,12 @@ struct DevicePtr {
     const void* p;
     size_t align;
 };
-// B2_OK when every pointer is null or aligned memory that kernels on the
-// current device may address (its own, or managed); B2_ERR_BAD_ARG otherwise,
-// for host memory and another device's among them.
+// B2_OK when every pointer is null or on its alignment; B2_ERR_BAD_ARG
+// otherwise.
+int check_alignment(const DevicePtr* p, int n, std::string* err);
+// B2_OK when every pointer is null or memory that kernels on the current
+// device may address (its own, or managed); B2_ERR_BAD_ARG otherwise, for host
+// memory and another device's among them.
 int check_device_pointers(const DevicePtr* p, int n, std::string* err);
 
 // The message of a failed CUDA call; returns B2_ERR_CUDA.

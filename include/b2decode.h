@@ -432,7 +432,10 @@ int b2_rope(const b2_rope_rows* rows, const double* freqs, const int32_t* positi
 /* The same, with k (rotated) and v written to the cache at slots[n_tok] (page
  * * page_size + place, as b2_page_plan gives them; a slot below 0 or past the
  * cache writes nothing).  q and q_out may be NULL.  The cache's type is the
- * rows', or F16 / BF16 for F32 rows.  No two tokens may share a slot. */
+ * rows', or F16 / BF16 for F32 rows.  No two tokens may share a slot, and no
+ * two places of the cache an element: taken from the smallest up, each of the
+ * strides, and the distance of k and v, passes the extent of the ones before
+ * (B2_ERR_BAD_ARG otherwise; attention only reads, and takes any strides). */
 int b2_rope_append(const b2_rope_rows* rows, const b2_paged_kv* kv, const double* freqs, const int32_t* positions,
                    const int64_t* slots, int32_t n_tok, const void* q, const void* k, const void* v, void* q_out,
                    void* stream);

@@ -73,6 +73,53 @@ def test_between_the_rows_of_a_table(check):
     assert plan(check, **{**kw, "info": kw["table"] + 2 * row + 4 * 13}) == "info overlaps table"
 
 
+PTR = 1 << 20  # an address that no refused call reads
+
+
+def append(**kw):
+    a = dict(k_ptr=PTR, v_ptr=PTR + (1 << 30), dtype=b2.F16, n_pages=4, page_size=16, nkv=2, hd=64)
+    a.update(kw)
+    kv = b2.paged_kv(**a)
+    rows = b2.rope_rows(b2.F16, 4, kv.nkv, kv.hd, kv.hd)
+    with pytest.raises(b2.B2Error) as e:
+        b2.rope_append(rows, kv, PTR, PTR, PTR, 3, PTR, PTR, PTR, PTR)
+    return "place elements on one another" in str(e.value)
+
+
+E = 16 * 2 * 64  # elements of a dense page
+
+
+@pytest.mark.parametrize("change", [
+    dict(v_ptr=PTR),  # k and v the same memory
+    dict(v_ptr=PTR + 2 * E),  # v one page into k's four
+    dict(v_ptr=PTR + 16),
+    dict(page_stride=E, pos_stride=128, head_stride=0),  # heads on one another
+    dict(page_stride=E, pos_stride=128, head_stride=56),
+    dict(page_stride=E, pos_stride=120, head_stride=64),  # positions
+    dict(page_stride=E - 8, pos_stride=128, head_stride=64),  # pages
+    dict(page_stride=0, pos_stride=128, head_stride=64),
+    dict(page_stride=E, pos_stride=64, head_stride=64 * 15),  # heads in a page of 15 positions
+    dict(page_stride=E, pos_stride=128, head_stride=64, v_ptr=PTR + 2 * E),  # k and v alternate by pages of a stride for one
+])
+def test_cache_places_on_one_another_are_refused(built_lib, change):
+    assert append(**change)
+
+
+@pytest.mark.parametrize("change", [
+    dict(), dict(v_ptr=PTR + 4 * 2 * E), dict(k_ptr=PTR + 4 * 2 * E, v_ptr=PTR),
+    dict(page_stride=E, pos_stride=64, head_stride=64 * 16),  # head-major
+    dict(page_stride=2 * E, pos_stride=128, head_stride=64, v_ptr=PTR + 2 * E),  # k and v of a page together
+    dict(page_stride=2 * E, pos_stride=256, head_stride=64, v_ptr=PTR + 2 * 128),  # of a position
+    dict(page_stride=2 * E, pos_stride=256, head_stride=128, v_ptr=PTR + 2 * 64),  # of a head
+    dict(page_stride=128, pos_stride=512, head_stride=64),  # pages inside positions
+    dict(n_pages=1, page_stride=8, pos_stride=128, head_stride=64), dict(nkv=1, head_stride=8, pos_stride=64, page_stride=1024),
+    dict(n_pages=1, nkv=1, page_size=1, page_stride=8, v_ptr=PTR + 128),
+])
+def test_cache_layouts_that_stay_accepted(built_lib, change):
+    """(They fail later: the addresses are no memory.)"""
+    assert not append(**change)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("out,inp", [("lens", "cached"), ("lens", "fresh"), ("starts", "cached"), ("info", "n_free"),
                                      ("positions", "table"), ("table", "free_pages")])
