@@ -966,6 +966,7 @@ int b2_batch_logits_impl(const b2_batch* bt, float* out, std::string* err) {
 // stream for the call (the ids, then the four results).
 int b2_batch_logprobs_impl(const b2_batch* bt, int rows, const int32_t* ids, int m, float* logprob, float* entropy, int k,
                            int32_t* top_ids, float* top_logprob, std::string* err) {
+    if (!device_current(bt->m, err)) return B2_ERR_BAD_ARG;
     cudaStream_t s = bt->m->stream;
     const size_t nm = (size_t)rows * m, nk = (size_t)rows * k, n = 2 * nm + rows + 2 * nk;
     if (k > bt->m->dev.V) {

@@ -751,6 +751,23 @@ def test_batch_scores(built_lib, write_model, graph):
     m.close()
 
 
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs a second device to be current")
+def test_batch_scores_with_another_device_current(built_lib, write_model):
+    """Refused as a step and a prefill are, before anything is launched."""
+    from b2decode import gguf_writer as gw
+    shape = gw.ModelShape("qwen2", 256, 2, 4, 2, 512, 512, 256, 1e-6, 1e6, True, True, "q8_0", 1, 2)
+    m = b2.Model(write_model("qwen2-hd64-q8", shape), num_ctx=64)
+    bt = b2.Batch(m, 1)
+    first = bt.prefill(0, [1, 5, 9])
+    with torch.cuda.device(1):
+        with pytest.raises(b2.B2Error, match="must be the current device") as e:
+            bt.logprobs([[first]], 1)
+        assert e.value.code == -8
+    assert bt.logprobs([[first]], 1)[2][0, 0] == first
+    bt.close()
+    m.close()
+
+
 # ---------------------------------------------------------------------------
 # refusals that need a device, and a run of all of them
 # ---------------------------------------------------------------------------
