@@ -66,6 +66,7 @@ struct b2_batch {
     int* arg_i = nullptr;
     int* h_io = nullptr;                                        // pinned [3 * kBatchMax]
     std::vector<int> pos;                                       // positions (host copy)
+    int scored = 0;  // rows of logits of the last forward: 1 of a prompt, B of a step, 0 without one
     bool use_graph = false;                  // replay steps from a captured CUDA graph
     cudaGraphExec_t exec = nullptr;          // the step's launches (tokens and ids copied outside)
     unsigned long long exec_gen = 0;         // scratch generation it captured (scratch_generation)
@@ -796,6 +797,7 @@ int b2_batch_prefill_impl(b2_batch* bt, int slot, const int32_t* prompt, int n, 
     }
     if (!device_current(m, err)) return B2_ERR_BAD_ARG;
     cudaStream_t s = m->stream;
+    bt->scored = 0;
     // chunks of equal size (no one-token tail off the tensor-core path)
     const int cmax = prefill_chunk(d), nchunks = (n + cmax - 1) / cmax, chunk = (n + nchunks - 1) / nchunks;
     for (int p0 = 0; p0 < n; p0 += chunk) {
@@ -819,6 +821,7 @@ int b2_batch_prefill_impl(b2_batch* bt, int slot, const int32_t* prompt, int n, 
         return st;
     }
     *next_out = bt->h_io[2 * kBatchMax];
+    bt->scored = 1;
     return B2_OK;
 }
 
@@ -890,6 +893,7 @@ int b2_batch_step_impl(b2_batch* bt, const int32_t* tokens, int32_t* next_out, s
         }
         max_len = std::max(max_len, bt->pos[b] + 1);
     }
+    bt->scored = 0;
     for (int b = 0; b < B; b++) bt->h_io[b] = tokens[b];
     if (!ok(cudaMemcpyAsync(bt->d_tok, bt->h_io, sizeof(int) * B, cudaMemcpyHostToDevice, s), err, "tokens"))
         return B2_ERR_CUDA;
@@ -937,6 +941,7 @@ int b2_batch_step_impl(b2_batch* bt, const int32_t* tokens, int32_t* next_out, s
         next_out[b] = bt->h_io[B + b];
         bt->pos[b] += 1;
     }
+    bt->scored = B;
     return B2_OK;
 }
 
@@ -967,6 +972,10 @@ int b2_batch_logits_impl(const b2_batch* bt, float* out, std::string* err) {
 int b2_batch_logprobs_impl(const b2_batch* bt, int rows, const int32_t* ids, int m, float* logprob, float* entropy, int k,
                            int32_t* top_ids, float* top_logprob, std::string* err) {
     if (!device_current(bt->m, err)) return B2_ERR_BAD_ARG;
+    if (rows > bt->scored) {
+        *err = "b2_batch_logprobs: the last forward left " + std::to_string(bt->scored) + " rows of logits";
+        return B2_ERR_BAD_ARG;
+    }
     cudaStream_t s = bt->m->stream;
     const size_t nm = (size_t)rows * m, nk = (size_t)rows * k, n = 2 * nm + rows + 2 * nk;
     if (k > bt->m->dev.V) {

@@ -297,7 +297,8 @@ int b2_batch_prefill(b2_batch* b, int32_t slot, const int32_t* prompt, int32_t n
 int b2_batch_step(b2_batch* b, const int32_t* tokens, int32_t* next_out);
 int b2_batch_logits(const b2_batch* b, float* out);
 /* b2_logprobs on those logits where they are, in device memory: rows (at most
- * the batch; 1 after a b2_batch_prefill) rows, ids [rows][m] and the results
+ * the batch after a b2_batch_step, 1 after a b2_batch_prefill; more, or any
+ * without a forward before, fail with B2_ERR_BAD_ARG) rows, ids [rows][m] and the results
  * ([rows][m], [rows], [rows][k] twice) in HOST memory, entropy may be NULL.
  * Returns when the results are there.  The Go engine returns no scores. */
 int b2_batch_logprobs(const b2_batch* b, int32_t rows, const int32_t* ids, int32_t m, float* logprob, float* entropy,

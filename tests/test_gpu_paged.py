@@ -751,6 +751,33 @@ def test_batch_scores(built_lib, write_model, graph):
     m.close()
 
 
+def test_batch_scores_of_rows_that_no_forward_left(built_lib, write_model):
+    """More rows than the last forward's logits: refused, not scores of an older step."""
+    from b2decode import gguf_writer as gw
+    shape = gw.ModelShape("qwen2", 256, 2, 4, 2, 512, 512, 256, 1e-6, 1e6, True, True, "q8_0", 1, 2)
+    m = b2.Model(write_model("qwen2-hd64-q8", shape), num_ctx=16)
+    bt = b2.Batch(m, 2)
+
+    def refused(rows, left):
+        with pytest.raises(b2.B2Error, match="b2_batch_logprobs: the last forward left %d rows" % left) as e:
+            bt.logprobs(np.zeros((rows, 1)), 1)
+        assert e.value.code == -8
+
+    refused(1, 0)
+    nxt = [bt.prefill(i, [1, 5 + i]) for i in range(2)]
+    refused(2, 1)
+    assert bt.logprobs([[nxt[1]]], 1)[2][0, 0] == nxt[1]
+    nxt = bt.step(nxt)
+    assert np.array_equal(bt.logprobs(np.zeros((2, 1)), 1)[2][:, 0], nxt)
+    with pytest.raises(b2.B2Error):  # a prompt that is refused leaves the step's logits
+        bt.prefill(0, list(range(1, 17)))
+    assert np.array_equal(bt.logprobs(np.zeros((2, 1)), 1)[2][:, 0], nxt)
+    bt.prefill(0, [1, 5, 6])
+    refused(2, 1)
+    bt.close()
+    m.close()
+
+
 @pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs a second device to be current")
 def test_batch_scores_with_another_device_current(built_lib, write_model):
     """Refused as a step and a prefill are, before anything is launched."""
