@@ -91,10 +91,21 @@ struct Seq {
     bool bad;  // the length passes the table, or the row has none
 };
 
+// Lengths, requests and table entries are usually the work of the launches
+// just before (a page plan on the same stream, whose grid may still run when
+// this one's CTAs start), so they take no read-only loads: plain ones behind
+// pdl_wait, and with EARLY, ahead of it, loads from L2, where the words of a
+// grid that has ended are.
+template <bool EARLY>
+__device__ __forceinline__ int word(const int32_t* p) {
+    return EARLY ? __ldcg(p) : *p;
+}
+
+template <bool EARLY = false>
 __device__ __forceinline__ Seq seq_of(const PagedArgs& a, int b) {
     Seq s;
-    s.tr = a.req ? __ldg(a.req + b) : b;
-    const long long len = (long long)__ldg(a.lens + b) + a.len_add;
+    s.tr = a.req ? word<EARLY>(a.req + b) : b;
+    const long long len = (long long)word<EARLY>(a.lens + b) + a.len_add;
     const bool none = s.tr < 0 || len <= 0;
     s.bad = !none && (s.tr >= a.n_req || len > (long long)a.max_pages * a.page_size || len > kMaxLen);
     s.len = none || s.bad ? 0 : (int)len;
@@ -289,7 +300,7 @@ __global__ void __launch_bounds__(Sm<HD, NG>::kThreads) paged_split_kernel(const
     __shared__ long long wsum[kWarps];
     __shared__ long long chunk[kThreads];  // units before the end of each thread's sequences
     pdl_wait();
-    pdl_trigger();  // (behind the wait: the joining launch reads the lengths before its own)
+    pdl_trigger();  // (behind the wait, in every thread: the joining launch reads the lengths before its own)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gi = lane >> 2, ti = lane & 3;
     const int hd = a.hd, hc = hd / 8, rpb = a.nkv * a.rt;
     uint8_t* const ring = psm + warp * SM::kWarp;
@@ -376,7 +387,7 @@ __global__ void __launch_bounds__(Sm<HD, NG>::kThreads) paged_split_kernel(const
             f.full = one_page && first >= ld.sq.lo && first + STEP <= ld.sq.len;
             if (p >= ld.sq.lo && p < ld.sq.len) {
                 const int pg = a.page_shift >= 0 ? p >> a.page_shift : p / a.page_size;
-                f.page = __ldg(a.table + (int64_t)ld.sq.tr * a.table_stride + pg);
+                f.page = a.table[(int64_t)ld.sq.tr * a.table_stride + pg];
                 f.off = (int64_t)(p - pg * a.page_size) * a.pos_stride + h_off;
             }
             ld.step++;
@@ -686,13 +697,13 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, share = warp % PW;
     constexpr int rw = kJoinWarps / PW;
     const float nan = __int_as_float(0x7fc00000);
-    // the lengths are older than the split kernel, which has seen its predecessor end before it let this one start
-    const Seq sq = seq_of(a, b);
+    // (the lengths' writer has ended: the split kernel waited for it before it let this one start)
+    const Seq sq = seq_of<true>(a, b);
     int2 c = make_int2(0, 0);  // first and last group of the row
     {
         long long before = 0, all = 0;
         for (int i = threadIdx.x; i < a.batch; i += kJoinThreads) {
-            const int n = units_of(seq_of(a, i), step);
+            const int n = units_of(seq_of<true>(a, i), step);
             all += n;
             if (i < b) before += n;
         }

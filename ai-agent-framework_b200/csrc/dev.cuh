@@ -499,7 +499,12 @@ __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.lau
 // grid launched without the attribute.  A kernel launched by launch_pdl
 // calls it before its first global read or write, in every thread, so its
 // own completion still implies its predecessor's (the chain of launches
-// stays ordered for the kernels after it).
+// stays ordered for the kernels after it).  One kernel reads before it: the
+// joining launch of the paged attention, words that were written before the
+// launch it follows, which triggers behind its own wait in every thread; it
+// reads them from L2 (__ldcg).  No kernel that may start before its data's
+// writer has ended reads that data with __ldg: those loads want words that
+// stay as they are from the kernel's start.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Launches kern<<<grid, block, smem, s>>>(args...) as a programmatic

@@ -550,6 +550,75 @@ def test_attention_paged_streams_and_graph():
         a.check(out, ls)
 
 
+def test_attention_paged_behind_its_plan_in_one_graph():
+    """Plan, append and attention in one captured graph that also moves the lengths, the free list and the rows on:
+    each replay's attention follows the lengths, requests and table entries written just before it."""
+    R, P, nh, nkv, hd, cap, steps, n_pages, mp = 5, 16, 8, 2, 64, 12, 40, 64, 20
+    g = torch.Generator(device="cuda").manual_seed(9)
+    bank = torch.randn(steps, cap, (nh + 2 * nkv) * hd, device="cuda", generator=g).half()
+    turns = [[1, 3, 0, 2, 1], [0, 1, 1, 1, 1], [2, 2, 2, 2, 2]]
+    fresh_bank = i32([turns[i % 3] for i in range(steps)])
+    free_all = torch.randperm(n_pages, device="cuda", generator=g).to(torch.int32)
+    new = lambda *n, t=torch.int32: torch.zeros(*n, dtype=t, device="cuda")  # noqa: E731
+    cached, fresh, used, at, n_free, table = new(R), new(R), new(1, t=torch.int64), new(1, t=torch.int64), new(1), new(R, mp)
+    lens, starts, slots, pos, req, info = new(R), new(R + 1), new(cap, t=torch.int64), new(cap), new(cap), new(4)
+    free, rows_in = new(n_pages), new(cap, (nh + 2 * nkv) * hd, t=torch.float16)
+    kc, vc = (torch.full((n_pages, P, nkv, hd), math.nan, device="cuda", dtype=torch.float16) for _ in range(2))
+    q, out, ls = new(cap, nh, hd, t=torch.float16), new(cap, nh, hd, t=torch.float16), new(cap, nh, t=torch.float32)
+    kv = b2.paged_kv(kc.data_ptr(), vc.data_ptr(), b2.F16, n_pages, P, nkv, hd)
+    rr = b2.rope_rows(b2.F16, nh, nkv, hd, 0, 0, 1.0, *[rows_in.stride(0)] * 3)
+    opts = b2.paged_attn_opts(b2.F16, nh, R, mp, len_add=1)
+    scratch = torch.empty(b2.attention_paged_scratch_bytes(cap, nh, nkv, hd), dtype=torch.uint8, device="cuda")
+    table.fill_(-1)
+    lane = torch.arange(n_pages, device="cuda")
+
+    def step():
+        fresh.copy_(fresh_bank.index_select(0, at)[0])
+        rows_in.copy_(bank.index_select(0, at)[0])
+        free.copy_(free_all[(lane + used).clamp(max=n_pages - 1)])
+        n_free.copy_(n_pages - used)
+        b2.page_plan(cached.data_ptr(), fresh.data_ptr(), R, P, free.data_ptr(), n_free.data_ptr(), table.data_ptr(), mp, mp,
+                     lens.data_ptr(), starts.data_ptr(), slots.data_ptr(), pos.data_ptr(), req.data_ptr(), cap, info.data_ptr(), stream())
+        e = rows_in.data_ptr()
+        b2.rope_append(rr, kv, 0, pos.data_ptr(), slots.data_ptr(), cap, e, e + 2 * nh * hd, e + 2 * (nh + nkv) * hd, q.data_ptr(), stream())
+        b2.attention_paged(kv, opts, q.data_ptr(), table.data_ptr(), pos.data_ptr(), req.data_ptr(), cap, out.data_ptr(), ls.data_ptr(),
+                           scratch.data_ptr(), stream())
+        cached.copy_(lens)
+        used.add_(info[2].long())
+        at.add_(1)
+
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        step()  # (what the allocator needs, before the capture)
+    torch.cuda.synchronize()
+    for t in (cached, used, at):
+        t.zero_()
+    table.fill_(-1)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    held = [[] for _ in range(R)]
+    for i in range(steps):
+        graph.replay()
+        rows, owner, length = bank[i].view(cap, nh + 2 * nkv, hd), [], []
+        for r in range(R):
+            for _ in range(turns[i % 3][r]):
+                held[r].append(rows[len(owner), nh:])
+                owner.append(r)
+                length.append(len(held[r]))
+        T = len(owner)
+        assert info.tolist()[:2] == [0, T] and lens.tolist() == [len(h) for h in held]
+        assert bool((out[T:] == 0).all()) and bool((ls[T:] == -math.inf).all())
+        for r in range(R):
+            if held[r]:
+                p = torch.arange(len(held[r]), device="cuda")
+                page, have = table[r, p // P].long(), torch.stack(held[r])
+                assert torch.equal(kc[page, p % P], have[:, :nkv]) and torch.equal(vc[page, p % P], have[:, nkv:])
+        p = Paged.__new__(Paged)
+        p.q, p.kc, p.vc, p.table, p.lens, p.req, p.P, p.hd, p.dt = rows[:T, :nh], kc, vc, table, length, owner, P, hd, torch.float16
+        p.check(out[:T], ls[:T])
+
+
 def test_attention_paged_same_bits_again():
     p = Paged([5000, 77, 0, 900], 8, 2, 128, 16, "f32", "f16")
     first = p.call()
