@@ -64,6 +64,7 @@ constexpr int kMinUnits = 2;    // a group's share, at least (overhead counted)
 constexpr long long kMaxLen = 0x7fffffffLL - 63;  // so that a step's positions are ints
 constexpr int kJoinThreads = 256;
 constexpr int kJoinWarps = kJoinThreads / 32;
+constexpr int kJoinRows = 1024;  // rows of one joining CTA, at most
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kPScale = 16384.0f;  // probabilities enter P V times 2^14
@@ -682,52 +683,57 @@ __global__ void __launch_bounds__(Sm<HD, NG>::kThreads) paged_split_kernel(const
     cp_wait<0>();
 }
 
-// CTAs (row, blockIdx.y), the y shares taking the row's query heads in turn:
-// join the pieces of a row that was cut, and fill a row that sees nothing
+// CTAs (rows, blockIdx.y): each has a run of neighbouring rows (one row while
+// there are no more rows than CTAs), the y shares taking the query heads in
+// turn: join the pieces of a row that was cut, and fill a row that sees nothing
 // (zeros, lse -inf) or whose length passes its table (NaN).  The 8 warps are 8 /
 // PW heads times PW shares of the pieces; a lane holds ND pairs of a head (hd <=
-// 64 ND).  PW = 8 is for few heads, one to a CTA, PW = 1 for many.  Which groups hold the row's pieces follows from the
-// lengths, worked out while the split kernel still runs.
+// 64 ND).  PW = 8 is for few heads, one to a CTA, PW = 1 for many.  Which groups
+// hold a row's pieces follows from the lengths, worked out while the split
+// kernel still runs: every CTA walks all lengths once, so their number is
+// bounded (16 sequences of 2001 among 65536 rows: 7.5 ms with a CTA for each
+// row, 0.71 with 8 an SM; the same among 1024: 43 us, 50 with 4 an SM, which
+// puts two of them in one CTA; 20000 short rows: 218 us, 258 with 16 an SM).
 template <typename T, int ND, int PW>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedArgs a, int step) {
     __shared__ __align__(8) float red[kJoinWarps][kPagedMaxHd + 2];
     __shared__ long long sums[2][kJoinWarps];
+    struct Todo {
+        int row, first, last, kind;  // the row's groups; what it is
+    };
+    enum { kCut, kEmpty, kBad };
+    __shared__ Todo todo[kJoinRows];
+    __shared__ int n_todo;
     pdl_trigger();
-    const int rpb = a.nkv * a.rt, b = blockIdx.x, hd = a.hd, nh = a.nh;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, share = warp % PW;
+    if (threadIdx.x == 0) n_todo = 0;
+    const int rpb = a.nkv * a.rt, hd = a.hd, nh = a.nh;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, share = warp % PW;
     constexpr int rw = kJoinWarps / PW;
     const float nan = __int_as_float(0x7fc00000);
+    const unsigned rows = a.batch, run = rows / gridDim.x, more = rows - run * gridDim.x;
+    const unsigned b0 = blockIdx.x * run + min(blockIdx.x, more), b1 = b0 + run + (blockIdx.x < more);
     // (the lengths' writer has ended: the split kernel waited for it before it let this one start)
-    const Seq sq = seq_of<true>(a, b);
-    int2 c = make_int2(0, 0);  // first and last group of the row
-    {
-        long long before = 0, all = 0;
-        for (int i = threadIdx.x; i < a.batch; i += kJoinThreads) {
-            const int n = units_of(seq_of<true>(a, i), step);
-            all += n;
-            if (i < b) before += n;
-        }
+    long long before = 0, all = 0;  // units before row b0, and of all rows
+    for (unsigned i = tid; i < rows; i += kJoinThreads) {
+        const int n = units_of(seq_of<true>(a, i), step);
+        all += n;
+        if (i < b0) before += n;
+    }
 #pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            before += __shfl_xor_sync(0xffffffffu, before, o);
-            all += __shfl_xor_sync(0xffffffffu, all, o);
-        }
-        if (lane == 0) {
-            sums[0][warp] = before;
-            sums[1][warp] = all;
-        }
-        __syncthreads();
-        before = all = 0;
+    for (int o = 16; o; o >>= 1) {
+        before += __shfl_xor_sync(0xffffffffu, before, o);
+        all += __shfl_xor_sync(0xffffffffu, all, o);
+    }
+    if (lane == 0) {
+        sums[0][warp] = before;
+        sums[1][warp] = all;
+    }
+    __syncthreads();
+    before = all = 0;
 #pragma unroll
-        for (int w = 0; w < kJoinWarps; w++) {
-            before += sums[0][w];
-            all += sums[1][w];
-        }
-        if (sq.len) {  // the group of unit u: floor(((u + 1) G - 1) / W)
-            const long long G = groups_for(a, all);
-            c.x = (int)mul_div(before + kOverhead + 1, G, all, -1);
-            c.y = (int)mul_div(before + units_of(sq, step), G, all, -1);
-        }
+    for (int w = 0; w < kJoinWarps; w++) {
+        before += sums[0][w];
+        all += sums[1][w];
     }
     // a head's place among the workers: KV head, block of its group, row of the block
     const int64_t ps = (int64_t)a.heads * (hd + 2);  // floats of a piece; a group's are 2 rpb pieces apart
@@ -735,114 +741,156 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
         const int h = head / a.grp, in = head - h * a.grp, blk = in / a.heads;
         return a.part + (int64_t)2 * (h * a.rt + blk) * ps + (in - blk * a.heads) * (hd + 2);
     };
-    int first = blockIdx.y * rw;
-    const float* base = place(first + warp / PW);  // (worked out before the wait)
+    const int first0 = blockIdx.y * rw;
+    const float* const base0 = place(first0 + warp / PW);  // (worked out before the wait)
+
+#pragma unroll 1
+    for (unsigned at = b0; at < b1; at += kJoinThreads) {
+        // a row to a thread: its units, those before it, its groups
+        const unsigned b = at + tid;
+        Seq sq{};
+        if (b < b1) sq = seq_of<true>(a, b);
+        const int n = units_of(sq, step);
+        long long end = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long t = __shfl_up_sync(0xffffffffu, end, o);
+            if (lane >= o) end += t;
+        }
+        __syncthreads();  // (the sums were read)
+        if (lane == 31) sums[0][warp] = end;
+        __syncthreads();
+        long long rows_units = 0;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; w++) {
+            if (w < warp) end += sums[0][w];
+            rows_units += sums[0][w];
+        }
+        if (b < b1) {
+            Todo t{(int)b, 0, 0, sq.bad ? kBad : kEmpty};
+            if (sq.len) {  // the group of unit u: floor(((u + 1) G - 1) / W)
+                const long long G = groups_for(a, all), u = before + end - n;
+                t.first = (int)mul_div(u + kOverhead + 1, G, all, -1);
+                t.last = (int)mul_div(u + n, G, all, -1);
+                t.kind = kCut;
+            }
+            if (t.kind != kCut || t.first != t.last) todo[atomicAdd(&n_todo, 1)] = t;
+        }
+        before += rows_units;
+    }
+    __syncthreads();
     pdl_wait();
-    if (sq.len && c.x == c.y) return;
-    for (; first < nh; first += gridDim.y * rw, base = place(first + warp / PW)) {  // (once where PW > 1)
-        const int head = first + warp / PW;
-        const bool live = head < nh;
-        constexpr int NP = ND <= 2 ? 8 : 4;  // pieces in flight
-        float2 o[ND];
-        float M = -INFINITY, L = 0.0f;
-        bool bad = false;
+#pragma unroll 1
+    for (int e = 0; e < n_todo; e++) {
+        const Todo t = todo[e];
+        const float* base = base0;
+        // (once where PW > 1)
+#pragma unroll 1
+        for (int first = first0; first < nh; first += gridDim.y * rw, base = place(first + warp / PW)) {
+            const int head = first + warp / PW;
+            const bool live = head < nh;
+            constexpr int NP = ND <= 2 ? 8 : 4;  // pieces in flight
+            float2 o[ND];
+            float M = -INFINITY, L = 0.0f;
+            bool bad = false;
 #pragma unroll
-        for (int j = 0; j < ND; j++) o[j] = make_float2(0.0f, 0.0f);
-        if (live && sq.len) {
-            for (int i0 = c.x + share; i0 <= c.y; i0 += NP * PW) {
-                float2 ml[NP], x[NP][ND];
+            for (int j = 0; j < ND; j++) o[j] = make_float2(0.0f, 0.0f);
+            if (live && t.kind == kCut) {
+                for (int i0 = t.first + share; i0 <= t.last; i0 += NP * PW) {
+                    float2 ml[NP], x[NP][ND];
 #pragma unroll
-                for (int k = 0; k < NP; k++) {
-                    const int i = i0 + k * PW;
-                    const float* p = base + (2 * (int64_t)i * rpb + (i == c.x ? 1 : 0)) * ps;
-                    ml[k] = i <= c.y ? *reinterpret_cast<const float2*>(p + hd) : make_float2(-INFINITY, 0.0f);
+                    for (int k = 0; k < NP; k++) {
+                        const int i = i0 + k * PW;
+                        const float* p = base + (2 * (int64_t)i * rpb + (i == t.first ? 1 : 0)) * ps;
+                        ml[k] = i <= t.last ? *reinterpret_cast<const float2*>(p + hd) : make_float2(-INFINITY, 0.0f);
 #pragma unroll
-                    for (int j = 0; j < ND; j++) {
-                        const int d = 2 * lane + 64 * j;
-                        x[k][j] = i <= c.y && d < hd ? *reinterpret_cast<const float2*>(p + d) : make_float2(0.0f, 0.0f);
-                    }
-                }
-                float N = M;
-#pragma unroll
-                for (int k = 0; k < NP; k++) {
-                    bad |= ml[k].x != ml[k].x;
-                    N = fmaxf(N, ml[k].x);
-                }
-                const float z = N == -INFINITY ? 0.0f : N, f = ex2(M - z);
-                M = N;
-                L *= f;
-#pragma unroll
-                for (int j = 0; j < ND; j++) {
-                    o[j].x *= f;
-                    o[j].y *= f;
-                }
-#pragma unroll
-                for (int k = 0; k < NP; k++) {
-                    const float w = ex2(ml[k].x - z);
-                    L = fmaf(ml[k].y, w, L);
-#pragma unroll
-                    for (int j = 0; j < ND; j++) {
-                        o[j].x = fmaf(x[k][j].x, w, o[j].x);
-                        o[j].y = fmaf(x[k][j].y, w, o[j].y);
-                    }
-                }
-            }
-            if (bad) M = L = nan;
-        }
-        if constexpr (PW > 1) {  // the shares of a head meet in its first warp
-#pragma unroll
-            for (int j = 0; j < ND; j++)
-                if (2 * lane + 64 * j < hd) *reinterpret_cast<float2*>(&red[warp][2 * lane + 64 * j]) = o[j];
-            if (lane == 0) *reinterpret_cast<float2*>(&red[warp][kPagedMaxHd]) = make_float2(M, L);
-            __syncthreads();
-            if (share == 0) {
-                float N = M;
-                bool any = M != M;
-                for (int w = 1; w < PW; w++) {
-                    const float m = red[warp + w][kPagedMaxHd];
-                    any |= m != m;
-                    N = fmaxf(N, m);
-                }
-                const float z = N == -INFINITY ? 0.0f : N, f = ex2(M - z);
-                L *= f;
-#pragma unroll
-                for (int j = 0; j < ND; j++) {
-                    o[j].x *= f;
-                    o[j].y *= f;
-                }
-                for (int w = 1; w < PW; w++) {
-                    const float2 ml = *reinterpret_cast<const float2*>(&red[warp + w][kPagedMaxHd]);
-                    const float g = ex2(ml.x - z);
-                    L = fmaf(ml.y, g, L);
-#pragma unroll
-                    for (int j = 0; j < ND; j++)
-                        if (2 * lane + 64 * j < hd) {
-                            const float2 x = *reinterpret_cast<const float2*>(&red[warp + w][2 * lane + 64 * j]);
-                            o[j].x = fmaf(x.x, g, o[j].x);
-                            o[j].y = fmaf(x.y, g, o[j].y);
+                        for (int j = 0; j < ND; j++) {
+                            const int d = 2 * lane + 64 * j;
+                            x[k][j] = i <= t.last && d < hd ? *reinterpret_cast<const float2*>(p + d) : make_float2(0.0f, 0.0f);
                         }
-                }
-                M = any ? nan : N;
-                if (any) L = nan;
-            }
-            __syncthreads();
-        }
-        if (live && share == 0) {
-            if (sq.bad) M = L = nan;
-            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-            T* out = static_cast<T*>(a.out) + (int64_t)b * a.out_stride + (int64_t)head * hd;
+                    }
+                    float N = M;
 #pragma unroll
-            for (int j = 0; j < ND; j++) {
-                const int d = 2 * lane + 64 * j;
-                if (d < hd) {
-                    out[d] = (T)(o[j].x * inv);
-                    out[d + 1] = (T)(o[j].y * inv);
+                    for (int k = 0; k < NP; k++) {
+                        bad |= ml[k].x != ml[k].x;
+                        N = fmaxf(N, ml[k].x);
+                    }
+                    const float z = N == -INFINITY ? 0.0f : N, f = ex2(M - z);
+                    M = N;
+                    L *= f;
+#pragma unroll
+                    for (int j = 0; j < ND; j++) {
+                        o[j].x *= f;
+                        o[j].y *= f;
+                    }
+#pragma unroll
+                    for (int k = 0; k < NP; k++) {
+                        const float w = ex2(ml[k].x - z);
+                        L = fmaf(ml[k].y, w, L);
+#pragma unroll
+                        for (int j = 0; j < ND; j++) {
+                            o[j].x = fmaf(x[k][j].x, w, o[j].x);
+                            o[j].y = fmaf(x[k][j].y, w, o[j].y);
+                        }
+                    }
                 }
+                if (bad) M = L = nan;
             }
-            if (a.lse && lane == 0)
-                a.lse[(int64_t)b * nh + head] = L == 0.0f ? -INFINITY : (M + (log2f(L) - 14.0f)) * kLn2;
+            if constexpr (PW > 1) {  // the shares of a head meet in its first warp
+#pragma unroll
+                for (int j = 0; j < ND; j++)
+                    if (2 * lane + 64 * j < hd) *reinterpret_cast<float2*>(&red[warp][2 * lane + 64 * j]) = o[j];
+                if (lane == 0) *reinterpret_cast<float2*>(&red[warp][kPagedMaxHd]) = make_float2(M, L);
+                __syncthreads();
+                if (share == 0) {
+                    float N = M;
+                    bool any = M != M;
+                    for (int w = 1; w < PW; w++) {
+                        const float m = red[warp + w][kPagedMaxHd];
+                        any |= m != m;
+                        N = fmaxf(N, m);
+                    }
+                    const float z = N == -INFINITY ? 0.0f : N, f = ex2(M - z);
+                    L *= f;
+#pragma unroll
+                    for (int j = 0; j < ND; j++) {
+                        o[j].x *= f;
+                        o[j].y *= f;
+                    }
+                    for (int w = 1; w < PW; w++) {
+                        const float2 ml = *reinterpret_cast<const float2*>(&red[warp + w][kPagedMaxHd]);
+                        const float g = ex2(ml.x - z);
+                        L = fmaf(ml.y, g, L);
+#pragma unroll
+                        for (int j = 0; j < ND; j++)
+                            if (2 * lane + 64 * j < hd) {
+                                const float2 x = *reinterpret_cast<const float2*>(&red[warp + w][2 * lane + 64 * j]);
+                                o[j].x = fmaf(x.x, g, o[j].x);
+                                o[j].y = fmaf(x.y, g, o[j].y);
+                            }
+                    }
+                    M = any ? nan : N;
+                    if (any) L = nan;
+                }
+                __syncthreads();
+            }
+            if (live && share == 0) {
+                if (t.kind == kBad) M = L = nan;
+                const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+                T* out = static_cast<T*>(a.out) + (int64_t)t.row * a.out_stride + (int64_t)head * hd;
+#pragma unroll
+                for (int j = 0; j < ND; j++) {
+                    const int d = 2 * lane + 64 * j;
+                    if (d < hd) {
+                        out[d] = (T)(o[j].x * inv);
+                        out[d + 1] = (T)(o[j].y * inv);
+                    }
+                }
+                if (a.lse && lane == 0)
+                    a.lse[(int64_t)t.row * nh + head] = L == 0.0f ? -INFINITY : (M + (log2f(L) - 14.0f)) * kLn2;
+            }
+            if (PW > 1) break;
         }
-        if (PW > 1) break;
     }
 }
 
@@ -865,12 +913,13 @@ cudaError_t go(const PagedArgs& a, cudaStream_t s) {
     e = launch_pdl(kern, dim3((a.groups * a.nkv * a.rt + SM::kWarps - 1) / SM::kWarps), dim3(SM::kThreads), smem, s, a);
     if (e != cudaSuccess) return e;
     // few heads in all: a CTA for each, its pieces over the 8 warps; many: a warp
-    // for each, as many CTAs as the machine holds beside the split kernel
+    // for each, a CTA for each row while there are up to 8 an SM of them
     if ((long long)a.batch * a.nh <= 2 * a.sms)
         return launch_pdl(paged_join_kernel<T, HD / 64, kJoinWarps>, dim3(a.batch, a.nh), dim3(kJoinThreads), 0, s, a,
                           SM::kStep);
-    const int y = std::max(1, std::min((a.nh + kJoinWarps - 1) / kJoinWarps, 4 * a.sms / a.batch));
-    return launch_pdl(paged_join_kernel<T, HD / 64, 1>, dim3(a.batch, y), dim3(kJoinThreads), 0, s, a, SM::kStep);
+    const int ctas = std::min(a.batch, std::max(8 * a.sms, (a.batch - 1) / kJoinRows + 1));
+    const int y = std::max(1, std::min((a.nh + kJoinWarps - 1) / kJoinWarps, 4 * a.sms / ctas));
+    return launch_pdl(paged_join_kernel<T, HD / 64, 1>, dim3(ctas, y), dim3(kJoinThreads), 0, s, a, SM::kStep);
 }
 
 // Query heads of one unit: 16 for groups past 8, so that K and V are read

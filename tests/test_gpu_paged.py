@@ -444,6 +444,92 @@ def test_attention_paged_thousands_of_rows():
     assert torch.equal(out, want[0]) and bool((ls == 5).all())
 
 
+def test_attention_paged_rows_of_a_fixed_step():
+    """A step of a fixed number of rows: long, short, empty, padding and bad ones side by side, more of them than
+    the joining launch has CTAs."""
+    g = np.random.default_rng(3)
+    lens = [int(n) for n in g.integers(0, 30, 2600)]
+    lens[:12] = [4000, 0, 700, 33, 2500, 0, 1, 900, 64, 0, 5, 1200]
+    lens[1300:1304] = [3000, 0, 1500, 1500]
+    p = Paged(lens, 12, 4, 64, 16, "bf16", "bf16", extra=0)
+    good, lse = p.call()
+    p.check(good, lse)
+    p.req = [b if b % 3 else -1 for b in range(2600)]
+    p.lens[4] = 4001 + p.max_pages * 16
+    p.table[1300, 100] = p.total
+    out, ls = p.call()
+    live = torch.tensor([b % 3 > 0 for b in range(2600)], device="cuda")
+    bad = torch.zeros_like(live)
+    bad[[4, 1300]] = True
+    assert bool(out[bad].isnan().all()) and bool(ls[bad].isnan().all())
+    assert bool((out[~live] == 0).all()) and bool((ls[~live] == -math.inf).all())
+    rest = torch.nonzero(live & ~bad)[:, 0]
+    # (the shares are cut elsewhere: sums in another order)
+    assert torch.equal(torch.isinf(ls[rest]), torch.isinf(lse[rest]))
+    q = Paged.__new__(Paged)
+    q.__dict__.update(p.__dict__)
+    keep = rest.tolist()
+    q.q, q.lens, q.req = p.q[rest], [lens[b] for b in keep], keep
+    q.check(out[rest], ls[rest])
+
+
+def test_attention_paged_a_million_rows():
+    """More rows than the joining launch's CTAs list at once; three positions at most, so the whole of it is one
+    tensor expression in 64 bits."""
+    B, R, hd = 1_300_000, 50, 8
+    g = torch.Generator(device="cuda").manual_seed(11)
+    k, v = (torch.randn(R, 16, 1, hd, device="cuda", generator=g).bfloat16() for _ in range(2))
+    q = torch.randn(B, 1, hd, device="cuda", generator=g).bfloat16()
+    req = torch.randint(0, R, (B,), device="cuda", generator=g).to(torch.int32)
+    n = (torch.randint(0, 10, (B,), device="cuda", generator=g) - 6).clamp(min=0).to(torch.int32)
+    table = torch.arange(R, device="cuda", dtype=torch.int32)
+    out, ls = torch.full_like(q, 5.0), torch.full((B, 1), 5.0, device="cuda")
+    kv = b2.paged_kv(k.data_ptr(), v.data_ptr(), b2.BF16, R, 16, 1, hd)
+    scratch = torch.full((b2.attention_paged_scratch_bytes(B, 1, 1, hd),), 255, dtype=torch.uint8, device="cuda")
+    b2.attention_paged(kv, b2.paged_attn_opts(b2.BF16, 1, R, 1), q.data_ptr(), table.data_ptr(), n.data_ptr(), req.data_ptr(), B,
+                       out.data_ptr(), ls.data_ptr(), scratch.data_ptr(), stream())
+    kk, vv = (t[req.long(), :3, 0].double() for t in (k, v))
+    s = torch.einsum("bd,bjd->bj", q[:, 0].double(), kk) * hd ** -0.5
+    mag = torch.einsum("bd,bjd->bj", q[:, 0].double().abs(), kk.abs()).amax(1) * hd ** -0.5
+    s = s.masked_fill(torch.arange(3, device="cuda")[None] >= n[:, None], -math.inf)
+    lse = torch.logsumexp(s, 1)
+    w = torch.where(n[:, None] > 0, torch.exp(s - lse[:, None]), 0.0)
+    D = mag * (2.0 ** -22 + 32 * E32)  # (as in attend64)
+    assert_within(out[:, 0], torch.einsum("bj,bjd->bd", w, vv), (2 * (D + 2.0 ** -20) * vv.abs().amax((1, 2)))[:, None].expand(B, hd),
+                  torch.bfloat16)
+    some = n > 0
+    assert bool((ls[~some] == -math.inf).all())
+    assert bool(((ls[:, 0].double() - lse).abs() <= D + 2.0 ** -20 + 4 * E32 * lse.abs())[some].all())
+
+
+def test_attention_paged_cost_of_padding_rows():
+    """16 sequences in calls of 8192 and 65536 rows, the rest padding: eight times the rows cost no more than some
+    eight times as long (a joining launch whose CTAs, one to a row, each walk all rows takes 37 times)."""
+    p = Paged([2001] * 16, 8, 2, 64, 16, "bf16", "bf16")
+
+    def us(rows):
+        lens, req = i32([2001] * 16 + [0] * (rows - 16)), i32(list(range(16)) + [-1] * (rows - 16))
+        q = torch.zeros(rows, 8, 64, device="cuda", dtype=torch.bfloat16)
+        out = torch.empty_like(q)
+        kv = b2.paged_kv(p.kc.data_ptr(), p.vc.data_ptr(), p.cid, p.total, 16, 2, 64)
+        o = b2.paged_attn_opts(b2.BF16, 8, 16, p.max_pages)
+        scratch = torch.empty(b2.attention_paged_scratch_bytes(rows, 8, 2, 64), dtype=torch.uint8, device="cuda")
+        best = math.inf
+        for _ in range(8):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            for _ in range(4):
+                b2.attention_paged(kv, o, q.data_ptr(), p.table.data_ptr(), lens.data_ptr(), req.data_ptr(), rows, out.data_ptr(), 0,
+                                   scratch.data_ptr(), stream())
+            b.record()
+            b.synchronize()
+            best = min(best, a.elapsed_time(b) * 250)
+        return best
+
+    few, many = us(8192), us(65536)
+    assert many < 16 * few, (few, many)
+
+
 def test_attention_paged_window_ignores_freed_pages():
     p = Paged([1000, 130], 4, 2, 64, 16, "f16", "f16")
     want = p.call(window=100)
