@@ -475,8 +475,9 @@ __global__ void __launch_bounds__(Sm<HD, NG>::kThreads) paged_split_kernel(const
                     for (int j = 0; j < 4; j++) m = fmaxf(m, fabsf(x[kk][j]));
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                // (the exponent field is enough: subnormal rows count as 2^-127)
-                const int e = m < 3.0e38f ? min(100, max(-100, 137 - (int)(__float_as_uint(m) >> 23))) : 0;
+                // (the exponent field is enough: subnormal rows count as 2^-127; down to
+                // -117 for the largest finite row, so that both factors stay normal)
+                const int e = m < INFINITY ? min(100, 137 - (int)(__float_as_uint(m) >> 23)) : 0;
                 up = __int_as_float((127 + e) << 23);
                 factor *= __int_as_float((127 - e) << 23);
             }

@@ -585,6 +585,17 @@ def test_attention_paged_range_of_q(size, cache):
     p.check(*p.call())
 
 
+@pytest.mark.parametrize("size", [1e30, 1e36, 2e37])
+@pytest.mark.parametrize("cache", ["f16", "bf16"])
+def test_attention_paged_largest_q(size, cache):
+    """fp32 queries next to the type's largest value, with a scale that brings their scores back."""
+    p = Paged([300, 17], 4, 2, 64, 16, "f32", cache, spread=0.1)
+    p.q *= size
+    assert bool(torch.isfinite(p.q).all())
+    scale = float(np.float32(1.0 / size))
+    p.check(*p.call(scale=scale), scale=scale)
+
+
 def test_attention_paged_infinite_scores():
     """Keys of -inf score -inf: the others carry the row; a row of them alone is an empty one."""
     p = Paged([200, 130], 2, 1, 64, 16, "f32", "f16")
