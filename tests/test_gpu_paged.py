@@ -413,6 +413,34 @@ def test_attention_paged(dtype, cache, nh, nkv, hd, lens, P):
 
 
 @pytest.mark.parametrize("dtype,cache", COMBOS)
+@pytest.mark.parametrize("nh,nkv,hd", [(16, 1, 64), (20, 1, 32), (26, 2, 40), (16, 1, 256), (20, 1, 192), (32, 2, 192), (40, 2, 256), (34, 2, 136)])
+@pytest.mark.parametrize("lens,P", [([0, 1, 2, 15, 16, 17, 63, 64, 65, 0], 16), ([130, 5, 700, 1, 64], 24), ([5000, 3], 16)])
+def test_attention_paged_wide_groups(dtype, cache, nh, nkv, hd, lens, P):
+    """More than 8 and more than 16 query heads a KV head, below and past head dimensions of 64 and 128."""
+    p = Paged(lens, nh, nkv, hd, P, dtype, cache, seed=nh + hd)
+    p.check(*p.call())
+
+
+@pytest.mark.parametrize("dtype,cache", COMBOS)
+@pytest.mark.parametrize("nh,nkv,hd", [(16, 2, 192), (16, 2, 256), (24, 2, 256), (48, 2, 64), (24, 2, 128)])
+def test_attention_paged_many_wide_heads(dtype, cache, nh, nkv, hd):
+    """More heads in all than the joining launch gives a CTA each, with rows that are cut and rows that see nothing."""
+    p = Paged([3000, 0, 1, 700, 40, 2000, 0] + [64, 5] * 14, nh, nkv, hd, 16, dtype, cache, seed=hd)
+    p.check(*p.call())
+
+
+@pytest.mark.parametrize("dtype,cache", COMBOS)
+@pytest.mark.parametrize("nh,nkv,hd", [(12, 3, 128), (4, 2, 256), (14, 2, 200), (12, 1, 64), (20, 1, 128), (18, 1, 256)])
+@pytest.mark.parametrize("window,softcap,alibi", [(0, 30.0, False), (1, 0.0, True), (100, 5.0, True), (333, 0.0, False)])
+def test_attention_paged_masks_of_wide_heads(dtype, cache, nh, nkv, hd, window, softcap, alibi):
+    """Window, cap and slopes with steps of 16 positions, tiles of 16 heads and several tiles a group."""
+    p = Paged([1, 99, 100, 101, 600, 64, 0, 1500], nh, nkv, hd, 40, dtype, cache, "fused kv", seed=window + hd)
+    slopes = 2.0 ** -(8.0 * torch.arange(1, nh + 1, device="cuda", dtype=torch.float32) / nh) if alibi else None
+    kw = dict(window=window, softcap=softcap, slopes=slopes, scale=0.07)
+    p.check(*p.call(**kw), **kw)
+
+
+@pytest.mark.parametrize("dtype,cache", COMBOS)
 @pytest.mark.parametrize("layout", ["head-major", "fused kv"])
 @pytest.mark.parametrize("window,softcap,alibi", [(0, 30.0, False), (1, 0.0, False), (64, 0.0, True), (100, 5.0, True), (5000, 0.0, True)])
 def test_attention_paged_masks(dtype, cache, layout, window, softcap, alibi):
@@ -803,6 +831,38 @@ def test_logprobs(dtype, n, rows, pad):
     for k, m in ((min(20, n), 2), (min(64, n), 0), (0, 1), (1, 8)):
         ids = torch.randint(0, n, (rows, m), device="cuda", generator=g).to(torch.int32)
         logp_check(x, n, ids, k, *logp_call(x, dtype, n, ids, k))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", [1000, 40000])
+def test_logprobs_many_given_tokens(dtype, n):
+    """More given tokens than two for each thread, the last ones out of range."""
+    dt, _ = DT[dtype]
+    g = torch.Generator(device="cuda").manual_seed(n)
+    x = torch.randn(3, n, device="cuda", generator=g).to(dt)
+    for m in (257, 513, 1400):
+        ids = torch.randint(0, n, (3, m), device="cuda", generator=g).to(torch.int32)
+        lp, H, ti, tl = logp_call(x, dtype, n, ids, 5)
+        logp_check(x, n, ids, 5, lp, H, ti, tl)
+        ids[:, -1], ids[0, m // 2] = n, -1
+        out = logp_call(x, dtype, n, ids, 5)[0]
+        bad = (ids < 0) | (ids >= n)
+        assert bool(out[bad].isnan().all()) and torch.equal(out[~bad], lp[~bad])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", [5, 4097, 50257, 128256])
+@pytest.mark.parametrize("rows", [1, 3])
+def test_logprobs_rows_off_16_bytes(dtype, n, rows):
+    """Logits that start at any element: one row and several, in a leading dimension of any width."""
+    dt, _ = DT[dtype]
+    g = torch.Generator(device="cuda").manual_seed(n + rows)
+    for off, pad in ((1, 0), (2, 8), (3, 3)):
+        mem = torch.full((off + rows * (n + pad) + 9,), math.nan, device="cuda", dtype=dt)
+        x = mem[off:off + rows * (n + pad)].view(rows, n + pad)
+        x[:, :n] = (3 * torch.randn(rows, n, device="cuda", generator=g)).to(dt)
+        ids = torch.randint(0, n, (rows, 2), device="cuda", generator=g).to(torch.int32)
+        logp_check(x, n, ids, min(5, n), *logp_call(x, dtype, n, ids, min(5, n)))
 
 
 def test_logprobs_many_rows():
