@@ -6,8 +6,10 @@
 //   out = sum_j e^(s_j - M) v_j / sum_j e^(s_j - M) over the positions
 //   max(0, len - window) <= j < len;  lse = M + log of the sum.
 //
-// HBM-bound: every visible K and V row is read once, from the page that holds
-// it, whatever the number of query heads that share it.
+// HBM-bound: every visible K and V row is read from the page that holds it once
+// for each block of query heads that share it, 8 or 16 of them; the blocks of a
+// larger group walk the rows side by side, so HBM gives them once and L2 the
+// other times.
 //
 // Split.  The sequences of the batch, one after another, are a line of units,
 // a unit being one step of 16 or 32 positions.  Group g of G takes the units
@@ -923,13 +925,16 @@ cudaError_t go(const PagedArgs& a, cudaStream_t s) {
     return launch_pdl(paged_join_kernel<T, HD / 64, 1>, dim3(ctas, y), dim3(kJoinThreads), 0, s, a, SM::kStep);
 }
 
-// Query heads of one unit: 16 for groups past 8, so that K and V are read
-// once for all of them, while the fragments of q and O fit the registers.
-int unit_heads(int hd, int grp, int dtype) { return grp > 8 && (hd <= 128 || dtype != 0) ? 16 : 8; }
+// Query heads of one unit: 16 for groups past 8, so that one pass over K and V
+// serves them (32K x 16 of 16 heads of 128: 68 us with two units of 8, 57 with
+// one of 16), up to head dimension 128.  Past that the fragments of q and O of
+// 16 heads are more than the registers hold, and two units, whose rows meet in
+// L2, are faster (16K x 16 of 16 heads of 256, 16-bit rows: 79 us; 88 with one).
+int unit_heads(int hd, int grp) { return grp > 8 && hd <= 128 ? 16 : 8; }
 
 template <int HD, typename T, typename C, int QT, int PT>
 cudaError_t go_heads(const PagedArgs& a, cudaStream_t s) {
-    if constexpr (HD <= 128 || QT == 1) {
+    if constexpr (HD <= 128) {
         if (a.heads == 16) return go<HD, T, C, QT, PT, 2>(a, s);
     }
     return go<HD, T, C, QT, PT, 1>(a, s);
@@ -951,7 +956,7 @@ int groups_of(int hd, int heads, int rpb, int sms) {
     const bool two = heads == 16;
     if (hd <= 64) return two ? groups_in<64, 2>(rpb, sms) : groups_in<64, 1>(rpb, sms);
     if (hd <= 128) return two ? groups_in<128, 2>(rpb, sms) : groups_in<128, 1>(rpb, sms);
-    return two ? groups_in<256, 2>(rpb, sms) : groups_in<256, 1>(rpb, sms);
+    return groups_in<256, 1>(rpb, sms);
 }
 
 size_t part_bytes(int hd, int heads, int rpb, int sms) {
@@ -961,12 +966,9 @@ size_t part_bytes(int hd, int heads, int rpb, int sms) {
 }  // namespace
 
 size_t attention_paged_scratch(int batch, int nh, int nkv, int hd, int sms) {
-    // (the type of q is not known here: the larger of the two unit sizes)
-    const int grp = nh / nkv;
-    size_t n = part_bytes(hd, 8, nkv * ((grp + 7) / 8), sms);
-    if (grp > 8) n = std::max(n, part_bytes(hd, 16, nkv * ((grp + 15) / 16), sms));
+    const int grp = nh / nkv, heads = unit_heads(hd, grp);
     (void)batch;  // (the pieces are the workers', whatever the batch)
-    return n;
+    return part_bytes(hd, heads, nkv * ((grp + heads - 1) / heads), sms);
 }
 
 int launch_attention_paged(const b2_paged_kv& kv, const b2_paged_attn_opts& o, const void* q, const int32_t* table,
@@ -985,7 +987,7 @@ int launch_attention_paged(const b2_paged_kv& kv, const b2_paged_attn_opts& o, c
     a.lse = lse;
     a.part = static_cast<float*>(scratch);
     a.grp = o.nh / kv.nkv;
-    a.heads = unit_heads(kv.hd, a.grp, o.dtype);
+    a.heads = unit_heads(kv.hd, a.grp);
     a.rt = (a.grp + a.heads - 1) / a.heads;
     a.slopes = o.slopes;
     const int64_t qd = (int64_t)o.nh * kv.hd;
