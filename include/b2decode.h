@@ -460,8 +460,10 @@ typedef struct {
  * row b of q ([batch] rows of nh * hd) attends over the first lens[b] +
  * len_add positions of the sequence in table row req[b] (req NULL: b).  With
  * lens = the plan's positions, len_add = 1 and req = its token_req the rows
- * are a step's tokens, prompts included.  The order per score is scale,
- * softcap, slope, mask; fp32 softmax.  Writes out and, when lse is not NULL,
+ * are a step's tokens, prompts included (each row reads its positions for
+ * itself, so a long prompt costs its length squared in reads).  The order per
+ * score is scale, softcap, slope, mask; fp32 softmax.  Writes out and, when
+ * lse is not NULL,
  * lse[b][nh] = log of the sum of e^score.  A row that sees nothing (length <=
  * 0, req < 0) gets zeros and -inf.  A row whose length passes its table or
  * 2^31 - 64, whose req is n_req or more, or whose visible pages are not all in
