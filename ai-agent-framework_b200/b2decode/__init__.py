@@ -28,6 +28,7 @@ QTYPE_Q8_0 = 8
 QTYPE_Q4_0 = 2
 F32, F16, BF16 = 0, 1, 30  # ggml type ids
 PLAN_BAD_LENGTH, PLAN_TABLE_FULL, PLAN_ROWS_FULL, PLAN_NO_PAGES = 1, 2, 4, 8
+FORK_BAD_PARENT = 16
 ROPE_INTERLEAVED, ROPE_HALF = 0, 1
 ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_BANDS, ROPE_SCALE_YARN = 0, 1, 2, 3
 
@@ -160,6 +161,18 @@ SIGNATURES = {
     "b2_attention_paged": (C.c_int, [C.POINTER(PagedKV), C.POINTER(PagedAttnOpts), _P, _P, _P, _P, _i32, _P, _P, _P,
                                      _P]),
     "b2_logprobs": (C.c_int, [_P, _i32, _i32, _i32, _i64, _P, _i32, _P, _P, _i32, _P, _P, _P]),
+    "b2_beam_select_scratch_bytes": (_i64, [_i32, _i32, _i32, _i32]),
+    "b2_beam_select": (C.c_int, [_P, _i32, _i32, _i32, _i32, _i64, _P, _i32, _i32, _P, _P, _P, _P, _P, _P]),
+    "b2_beam_reorder": (C.c_int, [_P, _i32, _i64, _P, _i32, _i64, _i64, _P, _P, _P, _P, _P]),
+    "b2_page_fork": (C.c_int, [_P, _i32, _P, _i64, _P, _i32, _i32, _P, _i32, _P, _P, _P, _i64, _i32, _P, _P, _P, _P]),
+    "b2_page_copy": (C.c_int, [C.POINTER(PagedKV), _i32, _i64, _P, _P, _i32, _P]),
+    "b2_page_pool_scratch_bytes": (_i64, [_i32]),
+    "b2_page_pool": (C.c_int, [_P, _i64, _P, _i32, _i32, _i32, _P, _i32, _P, _P, _P, _P]),
+    "b2_page_compact_scratch_bytes": (_i64, [_i32]),
+    "b2_page_compact": (C.c_int, [_P, _i64, _P, _i32, _i32, _i32, _P, _i32, _P, _i32, _P, _P, _P]),
+    "b2_attention_shared_scratch_bytes": (_i64, [_i32, _i32, _i32, _i32]),
+    "b2_attention_shared": (C.c_int, [C.POINTER(PagedKV), C.POINTER(PagedAttnOpts), _P, _P, _P, _P, _i32, _P, _P, _i32,
+                                      _P, _P, _P, _P]),
     "b2_device_status": (C.c_int, [_P]),
     "b2_stream_handle": (_P, [_P]),
     "b2_trace_step": (C.c_int, [_P, _i32, C.POINTER(_i64), _i64, _i32p, _i32p]),
@@ -558,3 +571,86 @@ def logprobs(logits: int, dtype: int, n: int, rows: int, ld: int, ids: int, m: i
     (0: not wanted), the k best alternatives [rows][k]."""
     _check(lib().b2_logprobs(logits, dtype, n, rows, ld, ids or None, m, logprob or None, entropy or None, k,
                              top_ids or None, top_logprob or None, stream or None))
+
+
+def _bytes(n: int) -> int:
+    if n < 0:
+        _check(n)
+    return n
+
+
+def beam_select_scratch_bytes(n: int, n_groups: int, width: int, k: int) -> int:
+    """Device scratch beam_select needs."""
+    return _bytes(int(lib().b2_beam_select_scratch_bytes(n, n_groups, width, k)))
+
+
+def beam_select(logits: int, dtype: int, n: int, n_groups: int, width: int, ld: int, scores: int, k: int, eos: int,
+                parent: int, token: int, score: int, eos_score: int, scratch: int, stream: int = 0) -> None:
+    """b2_beam_select on device addresses: the k best continuations (row, token,
+    score) of each request's `width` beams; eos < 0: no end token, scores 0: all
+    0, eos_score 0: not wanted."""
+    _check(lib().b2_beam_select(logits, dtype, n, n_groups, width, ld, scores or None, k, eos, parent, token, score,
+                                eos_score or None, scratch, stream or None))
+
+
+def beam_reorder(src: int, n_src: int, src_stride: int, dst: int, n_dst: int, dst_stride: int, row_words: int,
+                 parent: int, lens: int = 0, token: int = 0, new_lens: int = 0, stream: int = 0) -> None:
+    """b2_beam_reorder on device addresses: row r of dst = row parent[r] of src
+    (its first lens words, token[r] behind them), sizes in 32-bit words."""
+    _check(lib().b2_beam_reorder(src, n_src, src_stride, dst, n_dst, dst_stride, row_words, parent, lens or None,
+                                 token or None, new_lens or None, stream or None))
+
+
+def page_fork(parent: int, n_req: int, table: int, table_stride: int, lens: int, n_src: int, page_size: int, refs: int,
+              n_pages: int, free_pages: int, n_free: int, new_table: int, new_stride: int, max_pages: int,
+              new_lens: int, pairs: int, info: int, stream: int = 0) -> None:
+    """b2_page_fork on device addresses: block tables of rows that continue rows
+    `parent`, and the pages to copy (page_copy with info + 4 bytes as their
+    number).  info[0] != 0 (PLAN_* and FORK_* bits): nothing was written."""
+    _check(lib().b2_page_fork(parent, n_req, table, table_stride, lens, n_src, page_size, refs or None, n_pages,
+                              free_pages, n_free, new_table, new_stride, max_pages, new_lens, pairs, info,
+                              stream or None))
+
+
+def page_copy(kv: PagedKV, layers: int, layer_stride: int, pairs: int, n_pairs: int, max_pairs: int,
+              stream: int = 0) -> None:
+    """b2_page_copy on device addresses: pages to pages in `layers` layers, layer_stride elements apart."""
+    _check(lib().b2_page_copy(C.byref(kv), layers, layer_stride, pairs, n_pairs, max_pairs, stream or None))
+
+
+def page_pool_scratch_bytes(n_pages: int) -> int:
+    """Device scratch page_pool needs."""
+    return _bytes(int(lib().b2_page_pool_scratch_bytes(n_pages)))
+
+
+def page_pool(table: int, table_stride: int, lens: int, n_req: int, page_size: int, max_pages: int, refs: int,
+              n_pages: int, free_pages: int, n_free: int, scratch: int, stream: int = 0) -> None:
+    """b2_page_pool on device addresses: holders of every page, and the pages without one, ascending."""
+    _check(lib().b2_page_pool(table, table_stride, lens, n_req, page_size, max_pages, refs, n_pages, free_pages, n_free,
+                              scratch, stream or None))
+
+
+def page_compact_scratch_bytes(n_pages: int) -> int:
+    """Device scratch page_compact needs."""
+    return _bytes(int(lib().b2_page_compact_scratch_bytes(n_pages)))
+
+
+def page_compact(table: int, table_stride: int, lens: int, n_req: int, page_size: int, max_pages: int, refs: int,
+                 n_pages: int, pairs: int, max_pairs: int, info: int, scratch: int, stream: int = 0) -> None:
+    """b2_page_compact on device addresses: the pages in use to the front of the
+    pool, the table in place, the moves for page_copy (info + 4 bytes: their number)."""
+    _check(lib().b2_page_compact(table, table_stride, lens, n_req, page_size, max_pages, refs, n_pages, pairs, max_pairs,
+                                 info, scratch, stream or None))
+
+
+def attention_shared_scratch_bytes(batch: int, nh: int, nkv: int, hd: int) -> int:
+    """Device scratch attention_shared needs (on the current device)."""
+    return _bytes(int(lib().b2_attention_shared_scratch_bytes(batch, nh, nkv, hd)))
+
+
+def attention_shared(kv: PagedKV, opts: PagedAttnOpts, q: int, table: int, lens: int, req: int, batch: int, starts: int,
+                     prefix: int, n_groups: int, out: int, lse: int, scratch: int, stream: int = 0) -> None:
+    """b2_attention_shared on device addresses: attention_paged of rows whose
+    groups (starts [n_groups + 1]) share their first prefix [n_groups] positions."""
+    _check(lib().b2_attention_shared(C.byref(kv), C.byref(opts), q, table, lens, req or None, batch, starts, prefix,
+                                     n_groups, out, lse or None, scratch, stream or None))

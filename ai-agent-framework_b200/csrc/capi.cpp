@@ -60,6 +60,8 @@ auto guarded(F&& body) noexcept -> decltype(body()) {
     }
 }
 
+constexpr int64_t kBeamMaxRows = 1 << 27;  // rows of one beam selection
+
 bool float_type(int32_t t) { return t == 0 || t == 1 || t == 30; }
 
 int aligned(const char* who, std::initializer_list<b2::DevicePtr> ptrs) {
@@ -98,6 +100,36 @@ int paged_kv_args(const char* who, const b2_paged_kv* kv, b2_paged_kv* out) {
         (out->page_stride | out->pos_stride | out->head_stride) % 8)
         return ret(B2_ERR_BAD_ARG, w + ": the cache's strides must be multiples of 8, not negative");
     return B2_OK;
+}
+
+// Checks what the attentions over a paged cache have in common.
+int paged_attn_args(const char* who, const b2_paged_kv& c, const b2_paged_attn_opts* opts, const void* q,
+                    const int32_t* table, const int32_t* lens, const int32_t* req, int32_t batch, const void* out,
+                    const void* scratch) {
+    const std::string w(who);
+    if (!opts || !q || !table || !lens || !out || !scratch || batch <= 0)
+        return ret(B2_ERR_BAD_ARG, w + ": null argument or no rows");
+    const b2_paged_attn_opts& o = *opts;
+    if (o.dtype != 0 && o.dtype != c.dtype)
+        return ret(B2_ERR_UNSUPPORTED_TYPE, w + ": q must be F32 or of the cache's type");
+    if (o.nh <= 0 || o.nh % c.nkv || (int64_t)batch * o.nh > 0x7fffffff)
+        return ret(B2_ERR_BAD_ARG, w + ": the query heads must be a multiple of the cache's heads");
+    if (o.n_req <= 0 || o.max_pages <= 0 || (!req && batch > o.n_req) || o.len_add < 0)
+        return ret(B2_ERR_BAD_ARG, w + ": bad table (n_req, max_pages, len_add)");
+    const int64_t qd = (int64_t)o.nh * c.hd;
+    if (o.window < 0 || !(o.scale >= 0.0f) || !(o.softcap >= 0.0f) || std::isinf(o.scale) || std::isinf(o.softcap) ||
+        o.q_stride < 0 || (o.out_stride && o.out_stride < qd) || (o.table_stride && o.table_stride < o.max_pages))
+        return ret(B2_ERR_BAD_ARG, w + ": bad window, scale, softcap or stride");
+    return B2_OK;
+}
+
+int paged_attn_pointers(const char* who, const b2_paged_kv& c, const b2_paged_attn_opts& o, const void* q,
+                        const int32_t* table, const int32_t* lens, const int32_t* req, const void* out, const float* lse,
+                        const void* scratch, const int32_t* starts, const int32_t* prefix) {
+    const size_t es = type_bytes(o.dtype);
+    return on_device(who, {{"q", q, es}, {"the cache's k", c.k, 16}, {"the cache's v", c.v, 16}, {"table", table, 4},
+                           {"lens", lens, 4}, {"req", req, 4}, {"out", out, es}, {"lse", lse, 4}, {"slopes", o.slopes, 4},
+                           {"scratch", scratch, 16}, {"starts", starts, 4}, {"prefix", prefix, 4}});
 }
 
 int rope_rows_args(const char* who, const b2_rope_rows* r, b2_rope_rows* out) {
@@ -784,26 +816,12 @@ int b2_attention_paged(const b2_paged_kv* kv, const b2_paged_attn_opts* opts, co
         b2_paged_kv c;
         int rc = paged_kv_args("b2_attention_paged", kv, &c);
         if (rc != B2_OK) return rc;
-        if (!opts || !q || !table || !lens || !out || !d_scratch || batch <= 0)
-            return ret(B2_ERR_BAD_ARG, "b2_attention_paged: null argument or no rows");
-        const b2_paged_attn_opts& o = *opts;
-        if (o.dtype != 0 && o.dtype != c.dtype)
-            return ret(B2_ERR_UNSUPPORTED_TYPE, "b2_attention_paged: q must be F32 or of the cache's type");
-        if (o.nh <= 0 || o.nh % c.nkv || (int64_t)batch * o.nh > 0x7fffffff)
-            return ret(B2_ERR_BAD_ARG, "b2_attention_paged: the query heads must be a multiple of the cache's heads");
-        if (o.n_req <= 0 || o.max_pages <= 0 || (!req && batch > o.n_req) || o.len_add < 0)
-            return ret(B2_ERR_BAD_ARG, "b2_attention_paged: bad table (n_req, max_pages, len_add)");
-        const int64_t qd = (int64_t)o.nh * c.hd;
-        if (o.window < 0 || !(o.scale >= 0.0f) || !(o.softcap >= 0.0f) || std::isinf(o.scale) || std::isinf(o.softcap) ||
-            o.q_stride < 0 || (o.out_stride && o.out_stride < qd) || (o.table_stride && o.table_stride < o.max_pages))
-            return ret(B2_ERR_BAD_ARG, "b2_attention_paged: bad window, scale, softcap or stride");
-        const size_t es = type_bytes(o.dtype);
-        rc = on_device("b2_attention_paged", {{"q", q, es}, {"the cache's k", c.k, 16}, {"the cache's v", c.v, 16},
-                                              {"table", table, 4}, {"lens", lens, 4}, {"req", req, 4}, {"out", out, es},
-                                              {"lse", lse, 4}, {"slopes", o.slopes, 4}, {"scratch", d_scratch, 16}});
+        rc = paged_attn_args("b2_attention_paged", c, opts, q, table, lens, req, batch, out, d_scratch);
+        if (rc != B2_OK) return rc;
+        rc = paged_attn_pointers("b2_attention_paged", c, *opts, q, table, lens, req, out, lse, d_scratch, nullptr, nullptr);
         if (rc != B2_OK) return rc;
         std::string err;
-        rc = b2::launch_attention_paged(c, o, q, table, lens, req, batch, out, lse, d_scratch,
+        rc = b2::launch_attention_paged(c, *opts, q, table, lens, req, batch, out, lse, d_scratch,
                                         static_cast<cudaStream_t>(stream), &err);
         return ret(rc, err);
     });
@@ -828,6 +846,233 @@ int b2_logprobs(const void* logits, int32_t dtype, int32_t n, int32_t rows, int6
         std::string err;
         rc = b2::launch_logprobs(logits, dtype, n, rows, ld, ids, m, logprob, entropy, k, top_ids, top_logprob,
                                  static_cast<cudaStream_t>(stream), &err);
+        return ret(rc, err);
+    });
+}
+
+int64_t b2_beam_select_scratch_bytes(int32_t n, int32_t n_groups, int32_t width, int32_t k) {
+    return guarded([&]() -> int64_t {
+        if (n <= 0 || n_groups <= 0 || width <= 0 || width > b2::kBeamMaxWidth || k <= 0 || k > b2::kLogprobMaxTop ||
+            (int64_t)n_groups * width > kBeamMaxRows)
+            return ret(B2_ERR_BAD_ARG, "b2_beam_select_scratch_bytes: bad sizes");
+        return (int64_t)b2::beam_select_scratch(n, n_groups * width, k);
+    });
+}
+
+int b2_beam_select(const void* logits, int32_t dtype, int32_t n, int32_t n_groups, int32_t width, int64_t ld,
+                   const float* scores, int32_t k, int32_t eos, int32_t* parent, int32_t* token, float* score,
+                   float* eos_score, void* d_scratch, void* stream) {
+    return guarded([&] {
+        if (!logits || !parent || !token || !score || !d_scratch) return ret(B2_ERR_BAD_ARG, "b2_beam_select: null argument");
+        if (n <= 0 || n > (1 << 30) || ld < n || n_groups <= 0 || width <= 0 || width > b2::kBeamMaxWidth ||
+            (int64_t)n_groups * width > kBeamMaxRows)
+            return ret(B2_ERR_BAD_ARG, "b2_beam_select: bad rows (1 to 64 beams of a request, ld >= n)");
+        if (!float_type(dtype))
+            return ret(B2_ERR_UNSUPPORTED_TYPE, "b2_beam_select: dtype must be 0 (F32), 1 (F16) or 30 (BF16)");
+        if (k <= 0 || k > b2::kLogprobMaxTop || k > n)
+            return ret(B2_ERR_BAD_ARG, "b2_beam_select: 1 to 64 candidates, at most n");
+        if (eos >= n) return ret(B2_ERR_BAD_ARG, "b2_beam_select: eos must be below n");
+        const __int128 rows = (__int128)n_groups * width, es = type_bytes(dtype), best = (__int128)n_groups * k * 4;
+        const b2::Region in[] = {{"logits", logits, es * n, rows, es * ld}, {"scores", scores, 4 * rows}};
+        const b2::Region out[] = {{"parent", parent, best}, {"token", token, best}, {"score", score, best},
+                                  {"eos_score", eos >= 0 ? eos_score : nullptr, 4 * rows},
+                                  {"scratch", d_scratch, (__int128)b2::beam_select_scratch(n, (int)rows, k)}};
+        int rc = aligned("b2_beam_select", {{"logits", logits, type_bytes(dtype)}, {"scores", scores, 4}, {"parent", parent, 4},
+                                            {"token", token, 4}, {"score", score, 4}, {"eos_score", eos_score, 4},
+                                            {"scratch", d_scratch, 16}});
+        if (rc != B2_OK) return rc;
+        std::string err = b2::outputs_overlap(in, 2, out, 5);
+        if (!err.empty()) return ret(B2_ERR_BAD_ARG, "b2_beam_select: " + err);
+        rc = on_device("b2_beam_select", {{"logits", logits, 1}, {"scores", scores, 1}, {"parent", parent, 1}, {"token", token, 1},
+                                          {"score", score, 1}, {"eos_score", eos >= 0 ? eos_score : nullptr, 1},
+                                          {"scratch", d_scratch, 1}});
+        if (rc != B2_OK) return rc;
+        rc = b2::launch_beam_select(logits, dtype, n, n_groups, width, ld, scores, k, eos, parent, token, score, eos_score,
+                                    d_scratch, static_cast<cudaStream_t>(stream), &err);
+        return ret(rc, err);
+    });
+}
+
+int b2_beam_reorder(const void* src, int32_t n_src, int64_t src_stride, void* dst, int32_t n_dst, int64_t dst_stride,
+                    int64_t row_words, const int32_t* parent, const int32_t* lens, const int32_t* token,
+                    int32_t* new_lens, void* stream) {
+    return guarded([&] {
+        if (!src || !dst || !parent) return ret(B2_ERR_BAD_ARG, "b2_beam_reorder: null argument");
+        if (n_src <= 0 || n_dst <= 0 || row_words <= 0 || src_stride < row_words || dst_stride < row_words)
+            return ret(B2_ERR_BAD_ARG, "b2_beam_reorder: rows and words must be positive, strides >= row_words");
+        if (row_words > ((int64_t)1 << 40) || src_stride > ((int64_t)1 << 40) || dst_stride > ((int64_t)1 << 40))
+            return ret(B2_ERR_BAD_ARG, "b2_beam_reorder: at most 2^40 words a row");
+        const b2::Region in[] = {{"src", src, (__int128)4 * row_words, n_src, (__int128)4 * src_stride},
+                                 {"parent", parent, (__int128)4 * n_dst}, {"lens", lens, (__int128)4 * n_src},
+                                 {"token", token, (__int128)4 * n_dst}};
+        const b2::Region out[] = {{"dst", dst, (__int128)4 * row_words, n_dst, (__int128)4 * dst_stride},
+                                  {"new_lens", new_lens, (__int128)4 * n_dst}};
+        const std::initializer_list<b2::DevicePtr> ptrs = {{"src", src, 4}, {"dst", dst, 4}, {"parent", parent, 4},
+                                                           {"lens", lens, 4}, {"token", token, 4}, {"new_lens", new_lens, 4}};
+        int rc = aligned("b2_beam_reorder", ptrs);
+        if (rc != B2_OK) return rc;
+        std::string err = b2::outputs_overlap(in, 4, out, 2);
+        if (!err.empty()) return ret(B2_ERR_BAD_ARG, "b2_beam_reorder: " + err);
+        rc = on_device("b2_beam_reorder", ptrs);
+        if (rc != B2_OK) return rc;
+        rc = b2::launch_beam_reorder(src, n_src, src_stride, dst, n_dst, dst_stride, row_words, parent, lens, token, new_lens,
+                                     static_cast<cudaStream_t>(stream), &err);
+        return ret(rc, err);
+    });
+}
+
+int b2_page_fork(const int32_t* parent, int32_t n_req, const int32_t* table, int64_t table_stride, const int32_t* lens,
+                 int32_t n_src, int32_t page_size, const int32_t* refs, int32_t n_pages, const int32_t* free_pages,
+                 const int32_t* n_free, int32_t* new_table, int64_t new_stride, int32_t max_pages, int32_t* new_lens,
+                 int32_t* pairs, int32_t* info, void* stream) {
+    return guarded([&] {
+        if (!parent || !table || !lens || !free_pages || !n_free || !new_table || !new_lens || !pairs || !info)
+            return ret(B2_ERR_BAD_ARG, "b2_page_fork: null argument");
+        if (n_req <= 0 || n_req > b2::kPlanMaxReq || n_src <= 0 || n_src > b2::kPlanMaxReq)
+            return ret(B2_ERR_BAD_ARG, "b2_page_fork: takes 1 to 16384 rows");
+        if (page_size <= 0 || max_pages <= 0 || n_pages <= 0 || table_stride < max_pages || new_stride < max_pages)
+            return ret(B2_ERR_BAD_ARG, "b2_page_fork: page_size, n_pages and max_pages must be positive, strides >= max_pages");
+        const __int128 w = 4, row = w * max_pages;
+        const b2::Region in[] = {{"parent", parent, w * n_req}, {"table", table, row, n_src, w * table_stride},
+                                 {"lens", lens, w * n_src}, {"refs", refs, w * n_pages}, {"free_pages", free_pages, w},
+                                 {"n_free", n_free, w}};
+        const b2::Region out[] = {{"new_table", new_table, row, n_req, w * new_stride}, {"new_lens", new_lens, w * n_req},
+                                  {"pairs", pairs, 3 * w * n_req}, {"info", info, 4 * w}};
+        const std::initializer_list<b2::DevicePtr> ptrs = {
+            {"parent", parent, 4}, {"table", table, 4}, {"lens", lens, 4}, {"refs", refs, 4}, {"free_pages", free_pages, 4},
+            {"n_free", n_free, 4}, {"new_table", new_table, 4}, {"new_lens", new_lens, 4}, {"pairs", pairs, 4}, {"info", info, 4}};
+        int rc = aligned("b2_page_fork", ptrs);
+        if (rc != B2_OK) return rc;
+        std::string err = b2::outputs_overlap(in, 6, out, 4);
+        if (!err.empty()) return ret(B2_ERR_BAD_ARG, "b2_page_fork: " + err);
+        rc = on_device("b2_page_fork", ptrs);
+        if (rc != B2_OK) return rc;
+        const b2::PageForkArgs a{parent, table, lens, refs, free_pages, n_free, new_table, new_lens, pairs, info,
+                                 table_stride, new_stride, n_req, n_src, page_size, n_pages, max_pages};
+        rc = b2::launch_page_fork(a, static_cast<cudaStream_t>(stream), &err);
+        return ret(rc, err);
+    });
+}
+
+int b2_page_copy(const b2_paged_kv* kv, int32_t layers, int64_t layer_stride, const int32_t* pairs,
+                 const int32_t* n_pairs, int32_t max_pairs, void* stream) {
+    return guarded([&] {
+        b2_paged_kv c;
+        int rc = paged_kv_args("b2_page_copy", kv, &c);
+        if (rc != B2_OK) return rc;
+        if (!pairs || !n_pairs) return ret(B2_ERR_BAD_ARG, "b2_page_copy: null argument");
+        if (layers <= 0 || layer_stride < 0 || layer_stride % 8 || max_pairs <= 0)
+            return ret(B2_ERR_BAD_ARG, "b2_page_copy: layers and max_pairs must be positive, layer_stride a multiple of 8");
+        const std::initializer_list<b2::DevicePtr> ptrs = {{"the cache's k", c.k, 16}, {"the cache's v", c.v, 16},
+                                                           {"pairs", pairs, 4}, {"n_pairs", n_pairs, 4}};
+        rc = aligned("b2_page_copy", ptrs);
+        if (rc != B2_OK) return rc;
+        if (!b2::kv_places_apart(c, layers, layer_stride))
+            return ret(B2_ERR_BAD_ARG, "b2_page_copy: the cache's strides, k and v, or the layers, place elements on one another");
+        rc = on_device("b2_page_copy", ptrs);
+        if (rc != B2_OK) return rc;
+        std::string err;
+        rc = b2::launch_page_copy(c, layers, layer_stride, pairs, n_pairs, max_pairs, static_cast<cudaStream_t>(stream), &err);
+        return ret(rc, err);
+    });
+}
+
+int64_t b2_page_pool_scratch_bytes(int32_t n_pages) {
+    return guarded([&]() -> int64_t {
+        if (n_pages <= 0) return ret(B2_ERR_BAD_ARG, "b2_page_pool_scratch_bytes: n_pages must be positive");
+        return (int64_t)b2::page_pool_scratch(n_pages);
+    });
+}
+
+int b2_page_pool(const int32_t* table, int64_t table_stride, const int32_t* lens, int32_t n_req, int32_t page_size,
+                 int32_t max_pages, int32_t* refs, int32_t n_pages, int32_t* free_pages, int32_t* n_free,
+                 void* d_scratch, void* stream) {
+    return guarded([&] {
+        if (!table || !lens || !refs || !free_pages || !n_free || !d_scratch)
+            return ret(B2_ERR_BAD_ARG, "b2_page_pool: null argument");
+        if (n_req <= 0 || n_req > b2::kPlanMaxReq) return ret(B2_ERR_BAD_ARG, "b2_page_pool: takes 1 to 16384 rows");
+        if (page_size <= 0 || max_pages <= 0 || n_pages <= 0 || table_stride < max_pages)
+            return ret(B2_ERR_BAD_ARG, "b2_page_pool: page_size, n_pages and max_pages must be positive, table_stride >= max_pages");
+        const __int128 w = 4;
+        const b2::Region in[] = {{"table", table, w * max_pages, n_req, w * table_stride}, {"lens", lens, w * n_req}};
+        const b2::Region out[] = {{"refs", refs, w * n_pages}, {"free_pages", free_pages, w * n_pages}, {"n_free", n_free, w},
+                                  {"scratch", d_scratch, (__int128)b2::page_pool_scratch(n_pages)}};
+        const std::initializer_list<b2::DevicePtr> ptrs = {{"table", table, 4}, {"lens", lens, 4}, {"refs", refs, 4},
+                                                           {"free_pages", free_pages, 4}, {"n_free", n_free, 4},
+                                                           {"scratch", d_scratch, 16}};
+        int rc = aligned("b2_page_pool", ptrs);
+        if (rc != B2_OK) return rc;
+        std::string err = b2::outputs_overlap(in, 2, out, 4);
+        if (!err.empty()) return ret(B2_ERR_BAD_ARG, "b2_page_pool: " + err);
+        rc = on_device("b2_page_pool", ptrs);
+        if (rc != B2_OK) return rc;
+        rc = b2::launch_page_pool(table, table_stride, lens, n_req, page_size, max_pages, refs, n_pages, free_pages, n_free,
+                                  d_scratch, static_cast<cudaStream_t>(stream), &err);
+        return ret(rc, err);
+    });
+}
+
+int64_t b2_page_compact_scratch_bytes(int32_t n_pages) {
+    return guarded([&]() -> int64_t {
+        if (n_pages <= 0) return ret(B2_ERR_BAD_ARG, "b2_page_compact_scratch_bytes: n_pages must be positive");
+        return (int64_t)b2::page_compact_scratch(n_pages);
+    });
+}
+
+int b2_page_compact(int32_t* table, int64_t table_stride, const int32_t* lens, int32_t n_req, int32_t page_size,
+                    int32_t max_pages, const int32_t* refs, int32_t n_pages, int32_t* pairs, int32_t max_pairs,
+                    int32_t* info, void* d_scratch, void* stream) {
+    return guarded([&] {
+        if (!table || !lens || !refs || !pairs || !info || !d_scratch)
+            return ret(B2_ERR_BAD_ARG, "b2_page_compact: null argument");
+        if (n_req <= 0 || n_req > b2::kPlanMaxReq) return ret(B2_ERR_BAD_ARG, "b2_page_compact: takes 1 to 16384 rows");
+        if (page_size <= 0 || max_pages <= 0 || n_pages <= 0 || max_pairs <= 0 || table_stride < max_pages)
+            return ret(B2_ERR_BAD_ARG,
+                       "b2_page_compact: page_size, n_pages, max_pages and max_pairs must be positive, table_stride >= max_pages");
+        const __int128 w = 4;
+        const b2::Region in[] = {{"lens", lens, w * n_req}, {"refs", refs, w * n_pages}};
+        const b2::Region out[] = {{"table", table, w * max_pages, n_req, w * table_stride}, {"pairs", pairs, 3 * w * max_pairs},
+                                  {"info", info, 4 * w}, {"scratch", d_scratch, (__int128)b2::page_compact_scratch(n_pages)}};
+        const std::initializer_list<b2::DevicePtr> ptrs = {{"table", table, 4}, {"lens", lens, 4}, {"refs", refs, 4},
+                                                           {"pairs", pairs, 4}, {"info", info, 4}, {"scratch", d_scratch, 16}};
+        int rc = aligned("b2_page_compact", ptrs);
+        if (rc != B2_OK) return rc;
+        std::string err = b2::outputs_overlap(in, 2, out, 4);
+        if (!err.empty()) return ret(B2_ERR_BAD_ARG, "b2_page_compact: " + err);
+        rc = on_device("b2_page_compact", ptrs);
+        if (rc != B2_OK) return rc;
+        rc = b2::launch_page_compact(table, table_stride, lens, n_req, page_size, max_pages, refs, n_pages, pairs, max_pairs,
+                                     info, d_scratch, static_cast<cudaStream_t>(stream), &err);
+        return ret(rc, err);
+    });
+}
+
+int64_t b2_attention_shared_scratch_bytes(int32_t batch, int32_t nh, int32_t nkv, int32_t hd) {
+    return guarded([&]() -> int64_t {
+        if (batch <= 0 || nh <= 0 || nkv <= 0 || nh % nkv || hd <= 0 || hd > b2::kPagedMaxHd || (int64_t)batch * nh > 0x7fffffff)
+            return ret(B2_ERR_BAD_ARG, "b2_attention_shared_scratch_bytes: bad sizes");
+        std::string err;
+        const int sms = b2::current_sms(&err);
+        if (!sms) return ret(B2_ERR_CUDA, err);
+        return (int64_t)b2::attention_shared_scratch(batch, nh, nkv, hd, sms);
+    });
+}
+
+int b2_attention_shared(const b2_paged_kv* kv, const b2_paged_attn_opts* opts, const void* q, const int32_t* table,
+                        const int32_t* lens, const int32_t* req, int32_t batch, const int32_t* starts,
+                        const int32_t* prefix, int32_t n_groups, void* out, float* lse, void* d_scratch, void* stream) {
+    return guarded([&] {
+        b2_paged_kv c;
+        int rc = paged_kv_args("b2_attention_shared", kv, &c);
+        if (rc != B2_OK) return rc;
+        rc = paged_attn_args("b2_attention_shared", c, opts, q, table, lens, req, batch, out, d_scratch);
+        if (rc != B2_OK) return rc;
+        if (!starts || !prefix || n_groups <= 0) return ret(B2_ERR_BAD_ARG, "b2_attention_shared: null argument or no groups");
+        rc = paged_attn_pointers("b2_attention_shared", c, *opts, q, table, lens, req, out, lse, d_scratch, starts, prefix);
+        if (rc != B2_OK) return rc;
+        std::string err;
+        rc = b2::launch_attention_shared(c, *opts, q, table, lens, req, batch, starts, prefix, n_groups, out, lse, d_scratch,
+                                         static_cast<cudaStream_t>(stream), &err);
         return ret(rc, err);
     });
 }

@@ -46,18 +46,46 @@ inline std::string page_plan_overlap(const PagePlanArgs& a) {
     return "";
 }
 
-// Whether the places of a cache are apart: pages, positions and heads, and k
-// and v, each taken with its distance, from the smallest distance up; every
-// distance has to pass the extent of the ones before it.  (Distances that
-// interleave without meeting in any other way are refused too.)
-inline bool kv_places_apart(const b2_paged_kv& kv) {
+// Whether a row of a meets a row of b.  Rows of one distance are taken modulo
+// it (the halves of a pair of tables laid row beside row are apart); rows of
+// different distances meet where their extents do.
+inline bool rows_meet(const Region& a, const Region& b) {
+    if (a.rows == 1) return regions_meet(a, b);
+    if (b.rows == 1) return regions_meet(b, a);
+    if (a.bytes <= 0 || b.bytes <= 0) return false;
+    const __int128 pa = (uintptr_t)a.p, pb = (uintptr_t)b.p;
+    const __int128 ea = pa + (a.rows - 1) * a.stride + a.bytes, eb = pb + (b.rows - 1) * b.stride + b.bytes;
+    if (ea <= pb || eb <= pa) return false;
+    if (a.stride != b.stride) return true;
+    const __int128 off = ((pb - pa) % a.stride + a.stride) % a.stride;  // b's rows behind the start of a's
+    return off < a.bytes || off + b.bytes > a.stride;
+}
+
+// "<output> overlaps <input>" where an output meets an input or another output.
+inline std::string outputs_overlap(const Region* in, int n_in, const Region* out, int n_out) {
+    for (int i = 0; i < n_out; i++) {
+        if (!out[i].p) continue;
+        for (int j = 0; j < n_in; j++)
+            if (in[j].p && rows_meet(out[i], in[j])) return std::string(out[i].name) + " overlaps " + in[j].name;
+        for (int j = 0; j < i; j++)
+            if (out[j].p && rows_meet(out[i], out[j])) return std::string(out[i].name) + " overlaps " + out[j].name;
+    }
+    return "";
+}
+
+// Whether the places of a cache (of `layers` layers) are apart: pages,
+// positions, heads and layers, and k and v, each taken with its distance, from
+// the smallest distance up; every distance has to pass the extent of the ones
+// before it.  (Distances that interleave without meeting in any other way are
+// refused too.)
+inline bool kv_places_apart(const b2_paged_kv& kv, int layers = 1, int64_t layer_stride = 0) {
     struct Dim {
         __int128 step, n;
     };
     const __int128 k = (uintptr_t)kv.k, v = (uintptr_t)kv.v;
     Dim d[] = {{(__int128)2 * kv.page_stride, kv.n_pages}, {(__int128)2 * kv.pos_stride, kv.page_size},
-               {(__int128)2 * kv.head_stride, kv.nkv}, {k < v ? v - k : k - v, 2}};
-    std::sort(d, d + 4, [](const Dim& a, const Dim& b) { return a.step < b.step; });
+               {(__int128)2 * kv.head_stride, kv.nkv}, {k < v ? v - k : k - v, 2}, {(__int128)2 * layer_stride, layers}};
+    std::sort(d, d + 5, [](const Dim& a, const Dim& b) { return a.step < b.step; });
     __int128 extent = 2 * kv.hd;
     for (const Dim& x : d) {
         if (x.n == 1) continue;

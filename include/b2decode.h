@@ -490,6 +490,130 @@ int b2_attention_paged(const b2_paged_kv* kv, const b2_paged_attn_opts* opts, co
 int b2_logprobs(const void* logits, int32_t dtype, int32_t n, int32_t rows, int64_t ld, const int32_t* ids, int32_t m,
                 float* logprob, float* entropy, int32_t k, int32_t* top_ids, float* top_logprob, void* stream);
 
+/* ---- beam search over the paged cache: choose, fork, attend ----
+ *
+ * A server that keeps several continuations (beams) of each request runs, per
+ * step: b2_beam_select picks the best continuations from the step's logits and
+ * b2_beam_reorder brings the token histories into their order; b2_page_fork
+ * gives every new beam the block table of the beam that it continues, b2_page_copy
+ * copies the pages that the two must not share, in all layers at once, and
+ * b2_page_pool lists the pages that no row holds any longer; b2_page_plan and
+ * b2_rope_append place the new tokens; b2_attention_shared attends, reading what
+ * the rows of a request share once.  b2_page_compact, now and then, moves the
+ * pages in use to the front of the pool.  Conventions as for the paged serving
+ * step above: device pointers on the current device, asynchronous, no
+ * allocation, no state between calls, capturable; outputs share no memory with
+ * inputs or one another unless said otherwise.  The Go engine runs one
+ * sequence with one continuation: no counterpart there. */
+
+/* The k best continuations of each of n_groups requests.  The logits have
+ * n_groups * width rows of n (row i at logits + i * ld, ld >= n; dtype 0, 1 or
+ * 30), the beams of a request one after another; scores[row] is the sum of a
+ * beam's log probabilities so far (NULL: all 0).  The candidate (row, v) has
+ *   scores[row] + logits[row][v] - log(sum of e^logits[row]),
+ * taken in 64 bits; parent / token / score [n_groups][k] get the k largest in
+ * order, equal ones by lowest row, then lowest v (parent: the row, counted
+ * over all requests; score rounded once).  Nothing continues with a logit of
+ * -inf, from a beam whose score is -inf, +inf or NaN, whose logits hold a NaN
+ * or +inf or are all -inf; places that are left get -1, -1, -inf.  eos >= 0
+ * (below n): no candidate has that token; its own score in every row goes to
+ * eos_score[rows] (may be NULL; -inf where the row offers none).  width, k up to 64, k up to
+ * n, n up to 2^30.  d_scratch: b2_beam_select_scratch_bytes(...) bytes on 16
+ * bytes, no contents needed. */
+int64_t b2_beam_select_scratch_bytes(int32_t n, int32_t n_groups, int32_t width, int32_t k);
+int b2_beam_select(const void* logits, int32_t dtype, int32_t n, int32_t n_groups, int32_t width, int64_t ld,
+                   const float* scores, int32_t k, int32_t eos, int32_t* parent, int32_t* token, float* score,
+                   float* eos_score, void* d_scratch, void* stream);
+
+/* Rows of state in the order of the beams that go on: row r of dst (of n_dst)
+ * becomes row parent[r] of src (n_src rows), row_words 32-bit words, rows
+ * strides words apart.  lens [n_src] (may be NULL): only the first
+ * min(lens[parent[r]], row_words) words are copied, and token [n_dst] (may be
+ * NULL) is written behind them where there is room.  new_lens [n_dst] (may be
+ * NULL): the words that row r then holds.  A parent outside 0 .. n_src - 1:
+ * the row is left as it was, its length 0. */
+int b2_beam_reorder(const void* src, int32_t n_src, int64_t src_stride, void* dst, int32_t n_dst, int64_t dst_stride,
+                    int64_t row_words, const int32_t* parent, const int32_t* lens, const int32_t* token,
+                    int32_t* new_lens, void* stream);
+
+#define B2_FORK_BAD_PARENT 16 /* info[0] of b2_page_fork: a parent of n_src or more */
+
+/* Block tables of rows that continue other rows.  Row s (of n_src, at most
+ * 16384) of table holds lens[s] positions in its first ceil(lens[s] /
+ * page_size) entries; new row r (of n_req, at most 16384) continues row
+ * parent[r] (below 0: it is empty).  Full pages are shared.  A page that is
+ * partly filled is written next, so it may have one holder: the first new row
+ * of its parent keeps it where refs[page] (NULL: 1 for all) is at most 1,
+ * every other gets the next page from the front of free_pages (*n_free of
+ * them), in the order of the new rows.  Writes
+ *   new_table  [n_req] rows, new_stride apart: the entries in use, nothing else
+ *   new_lens   [n_req]
+ *   pairs      [n_req][3]: page, copy, positions to copy, one for every page
+ *              taken, for b2_page_copy
+ *   info       [4] {status, pages taken (pairs), 0, 0}
+ * What does not fit (status: B2_PLAN_BAD_LENGTH a negative length,
+ * B2_PLAN_TABLE_FULL one past max_pages pages, B2_PLAN_NO_PAGES,
+ * B2_FORK_BAD_PARENT) writes nothing but info. */
+int b2_page_fork(const int32_t* parent, int32_t n_req, const int32_t* table, int64_t table_stride, const int32_t* lens,
+                 int32_t n_src, int32_t page_size, const int32_t* refs, int32_t n_pages, const int32_t* free_pages,
+                 const int32_t* n_free, int32_t* new_table, int64_t new_stride, int32_t max_pages, int32_t* new_lens,
+                 int32_t* pairs, int32_t* info, void* stream);
+
+/* Copies pages of a cache of `layers` layers (layer l's k and v lie l *
+ * layer_stride elements behind kv's, layer_stride a multiple of 8): for each
+ * of the first min(*n_pairs, max_pairs) triples of pairs the first pairs[i][2]
+ * positions of page pairs[i][0] to page pairs[i][1].  A triple with a page
+ * outside the cache, or of one page twice, copies nothing.  No page is written
+ * twice, or read and written.  The cache's places must be apart, as for
+ * b2_rope_append, and the layers too. */
+int b2_page_copy(const b2_paged_kv* kv, int32_t layers, int64_t layer_stride, const int32_t* pairs,
+                 const int32_t* n_pairs, int32_t max_pairs, void* stream);
+
+/* Who holds the pool's pages: refs[n_pages] = how many of the n_req rows (at
+ * most 16384) hold each page among their first ceil(lens / page_size) entries
+ * (at most max_pages; an id outside the pool counts nowhere), free_pages (room for n_pages) = the
+ * pages that none holds, ascending, *n_free of them, nothing written past
+ * those.  A row is freed by a length of 0; a prefix is kept for later by a row
+ * of its own.  d_scratch: b2_page_pool_scratch_bytes(n_pages) bytes on 16
+ * bytes. */
+int64_t b2_page_pool_scratch_bytes(int32_t n_pages);
+int b2_page_pool(const int32_t* table, int64_t table_stride, const int32_t* lens, int32_t n_req, int32_t page_size,
+                 int32_t max_pages, int32_t* refs, int32_t n_pages, int32_t* free_pages, int32_t* n_free,
+                 void* d_scratch, void* stream);
+
+/* Moves the pages in use to the front of the pool.  With U pages in use (refs
+ * > 0, as b2_page_pool leaves them), the i-th highest page of those at U or
+ * above goes to the i-th lowest free page below U, for the first min(moves,
+ * max_pairs) of them.  The entries in use of the table's rows are changed in
+ * place; pairs [max_pairs][3] = page, new page, page_size, for b2_page_copy;
+ * info [4] = {0, pairs, U, one past the last page in use afterwards}.  refs
+ * stays as it was: b2_page_pool again counts the new pages. */
+int64_t b2_page_compact_scratch_bytes(int32_t n_pages);
+int b2_page_compact(int32_t* table, int64_t table_stride, const int32_t* lens, int32_t n_req, int32_t page_size,
+                    int32_t max_pages, const int32_t* refs, int32_t n_pages, int32_t* pairs, int32_t max_pairs,
+                    int32_t* info, void* d_scratch, void* stream);
+
+/* b2_attention_paged for rows that share what they read.  The rows starts[g]
+ * .. starts[g + 1] - 1 (starts [n_groups + 1] ascending, on the device) are
+ * group g, and the tables of the rows of a group that see anything hold the
+ * same pages for the positions below prefix[g] (device): the beams of a
+ * request, requests behind one system prompt, or, with b2_page_plan's starts
+ * and lens as starts and prefix, the tokens of each request, prompts included.
+ * Such positions are read once for all the rows of a group (for every 128 (row, query
+ * head) pairs of a KV head), the positions behind them row by row.  Every row
+ * sees what it sees in b2_attention_paged, whose other arguments and results
+ * these are: lengths, windows, slopes, rows that see nothing (zeros and -inf),
+ * rows that get NaN; no row is touched by another's pages, lengths or values.
+ * Rows in no group attend alone.  Groups whose starts do not ascend give rows
+ * without meaning, no access out of range.  Head dimensions past 128 run as
+ * b2_attention_paged, every row for itself.  d_scratch:
+ * b2_attention_shared_scratch_bytes(batch, nh, nkv, hd) bytes on 16 bytes, no
+ * contents needed. */
+int64_t b2_attention_shared_scratch_bytes(int32_t batch, int32_t nh, int32_t nkv, int32_t hd);
+int b2_attention_shared(const b2_paged_kv* kv, const b2_paged_attn_opts* opts, const void* q, const int32_t* table,
+                        const int32_t* lens, const int32_t* req, int32_t batch, const int32_t* starts,
+                        const int32_t* prefix, int32_t n_groups, void* out, float* lse, void* d_scratch, void* stream);
+
 /* ---- tensor parallelism (engine.go LoadOptions.NumGPU; no counterpart in the
  * Go engine, which runs on CPU cores) ----
  *
