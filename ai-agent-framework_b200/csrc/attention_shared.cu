@@ -1,20 +1,1135 @@
-// Attention of rows that share a prefix of a paged KV cache.
+// Attention of rows that share a prefix of a paged KV cache: what b2_attention_paged
+// computes (attention_paged.cu has the formulas), with the positions that the
+// rows of a group have in common read once for all of them.
+//
+// Items.  A group's shared positions times up to 128 (row, query head) pairs of
+// one KV head are an item, and so are the positions of one row behind its
+// prefix, times its own heads.  A tile is 128 positions of an item:
+//   S = Q K^T (128 x 128),  m = max s, p = e^(s - m), l = sum p,  T = P V,
+// each tile with a maximum of its own, so tiles do not wait for one another; O
+// and L take them up in fp32 registers,
+//   M' = max(M, m),  O <- O e^(M - M') + T e^(m - M').
+// Items need not share a maximum either, so a row's pieces (shared, own, and
+// those of an item that was cut) meet in one joining launch.
+//
+// Split.  The items of the batch, one after another, are a line of units, a
+// tile being one (and an item's start another).  Share s of G takes the units
+// [s W / G, (s + 1) W / G) for every KV head side by side, so the machine is
+// evenly loaded whatever the lengths, the host knows none of them, and a graph
+// follows the lengths that it finds.  A first launch of one CTA lays the line.
+//
+// One CTA an SM, its roles warp by warp:
+//   16-19  K and V rows by cp.async into a ring of tiles in the 128-byte swizzle
+//          that the products read (pages may have any size), Q at an item's start
+//   20     tcgen05.mma, one thread: S = Q K^T of tile j + 1, then T = P V of tile
+//          j, P being read from tensor memory
+//   0-7    two warpgroups taking tiles in turn: S out of tensor memory, a row to
+//          a thread, the exponentials, P back over S
+//   8-15   O: T out of tensor memory, added in fp32 (the tensor cores' own
+//          accumulation cuts instead of rounding, which over a long row pulls
+//          towards zero); at an item's end the result or the piece
+//
+// Rounding.  As in attention_paged.cu: K and V as they are; fp32 rows scaled per
+// row by a power of two and split into 2 fp16 or 3 bf16 terms; probabilities
+// times 2^14 in 2 terms (3 for fp32 rows over a bf16 cache); sums, maxima and
+// O in fp32, rounded once.
+//
+// A value that one row of an item sees and another does not meets a weight of 0
+// there, and 0 times infinity or NaN is NaN: a row whose result is not finite is
+// computed again by the joining launch, alone, from its own positions.
 #include <cuda_runtime.h>
 
+#include <algorithm>
+#include <atomic>
+
+#include "attention_common.cuh"
+#include "dev.cuh"
 #include "paged.h"
+#include "tcgen05.cuh"
 
 namespace b2 {
+namespace {
+
+constexpr int kTile = 128;       // positions of a tile, rows of a product
+constexpr int kItemUnits = 1;    // units' worth of starting an item
+constexpr int kMinShare = 3;     // a share's units, at least
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanItems = 2 * kPlanThreads;  // items whose units stay in shared memory
+constexpr uint64_t kSharedWaitNs = 2000000000ull;
+constexpr int kNoLimit = 0x7fffffff;
+
+struct Item {
+    long long u0;      // units before it
+    int row0, rows;    // its rows
+    int lo, hi;        // positions
+    int tr, limit;     // table row; positions from limit on are not its own (kNoLimit: a row's own positions)
+};
+static_assert(sizeof(Item) == 32, "two 16-byte loads");
+
+struct Line {
+    long long units;
+    int items, shares;
+};
+
+struct SharedArgs {
+    const void* q;
+    const uint16_t *k, *v;
+    const int32_t *table, *lens, *req, *starts, *prefix;
+    void* out;
+    float* lse;
+    const float* slopes;
+    int64_t q_stride, out_stride, table_stride, page_stride, pos_stride, head_stride;
+    int batch, nh, nkv, grp, hd, page_size, page_shift, n_pages, max_pages, n_req, len_add, window, n_groups;
+    int hb, blocks, rows;  // query heads of an item, such blocks of a group of heads, rows of an item
+    int shares;            // at most
+    int q_wide, out_wide;  // 16-byte accesses
+    float scale, softcap;
+    // scratch
+    Line* line;
+    int* first;    // [shares] the item in which the share starts
+    int* redo;     // [batch]
+    int4* row;     // [batch] {first visible position, length, shared item, own item}: -1 none, -2 a row of NaN
+    Item* item;    // [2 batch]
+    float* whole;  // [2][batch][nh][hd + 4] results of whole items of rows that have two: o, m (log2 units), l
+    float* part;   // [CTAs][2][128][hd + 4] pieces of items that were cut
+};
+
+__device__ __forceinline__ int tiles_of(const Item& it) { return (it.hi - it.lo + kTile - 1) / kTile; }
+
+// The last i of a[0 .. n) (ascending, a[0] <= x) with a[i] <= x.
+template <typename F>
+__device__ __forceinline__ int last_at(int n, F&& le) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (le(mid)) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+// ---------------------------------------------------------------------------
+// the line of items, by one CTA
+// ---------------------------------------------------------------------------
+
+__global__ void __launch_bounds__(kPlanThreads) shared_line_kernel(const __grid_constant__ SharedArgs a) {
+    constexpr int W = kPlanThreads / 32;
+    __shared__ int v_lo[kPlanThreads + kTile], v_hi[kPlanThreads + kTile], v_tr[kPlanThreads + kTile];
+    __shared__ int owner_item[kTile + kPlanThreads];  // the item that starts at a row, also of the 128 rows before
+    __shared__ long long w_units[W], u_item[kPlanItems];
+    __shared__ int w_items[W];
+    pdl_trigger();
+    pdl_wait();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, R = a.rows;
+
+    struct Group {
+        int start, end, prefix;  // end <= start: in none
+    };
+    auto group_of = [&](int b) {
+        const int g = last_at(a.n_groups, [&](int i) { return a.starts[i] <= b; });
+        Group r{max(a.starts[g], 0), a.starts[g + 1], max(a.prefix[g], 0)};
+        if (a.starts[g] > b || r.end <= b) r = Group{b, b, 0};
+        return r;
+    };
+
+    int items = 0;
+    long long units = 0;
+    for (int base = 0; base < a.batch; base += kPlanThreads) {
+        Group gr{0, 0, 0};
+        Seq me{};
+        for (int i = tid; i < kPlanThreads + R - 1; i += kPlanThreads) {
+            const int b = base + i;
+            int lo = 0, hi = 0, tr = 0;
+            if (b < a.batch) {
+                const Group g = group_of(b);
+                const Seq s = seq_of(a, b);
+                lo = s.lo;
+                hi = min(s.len, g.prefix);
+                tr = s.tr;
+                if (i == tid) {
+                    gr = g;
+                    me = s;
+                }
+            }
+            v_lo[i] = lo;
+            v_hi[i] = hi;
+            v_tr[i] = tr;
+        }
+        __syncthreads();
+        const int b = base + tid;
+        const bool in = b < a.batch;
+        Item sh{}, own{};
+        if (in && gr.end > gr.start && (b - gr.start) % R == 0) {
+            sh.row0 = b;
+            sh.rows = min(R, min(gr.end, a.batch) - b);
+            sh.lo = kNoLimit;
+            sh.tr = -1;
+            for (int r = 0; r < sh.rows; r++)
+                if (v_hi[tid + r] > v_lo[tid + r]) {
+                    if (sh.tr < 0) sh.tr = v_tr[tid + r];
+                    sh.lo = min(sh.lo, v_lo[tid + r]);
+                    sh.hi = max(sh.hi, v_hi[tid + r]);
+                }
+            sh.limit = gr.prefix;
+        }
+        if (in) {
+            own = Item{0, b, 1, max(me.lo, gr.prefix), me.len, me.tr, kNoLimit};
+            a.redo[b] = 0;
+        }
+        const bool has_sh = sh.hi > sh.lo, has_own = own.hi > own.lo;
+        const int n = has_sh + has_own;
+        const int u_sh = has_sh ? tiles_of(sh) + kItemUnits : 0, u = u_sh + (has_own ? tiles_of(own) + kItemUnits : 0);
+        int ni = n;
+        long long nu = u;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, ni, o);
+            const long long y = __shfl_up_sync(0xffffffffu, nu, o);
+            if (lane >= o) {
+                ni += x;
+                nu += y;
+            }
+        }
+        if (lane == 31) {
+            w_items[warp] = ni;
+            w_units[warp] = nu;
+        }
+        if (tid < kTile) owner_item[tid] = base ? owner_item[kPlanThreads + tid] : -1;
+        __syncthreads();
+        int at = items + ni - n;
+        long long u0 = units + nu - u;
+#pragma unroll 4
+        for (int w = 0; w < W; w++) {
+            if (w < warp) {
+                at += w_items[w];
+                u0 += w_units[w];
+            }
+            items += w_items[w];
+            units += w_units[w];
+        }
+        const int i_sh = has_sh ? at : -1, i_own = has_own ? at + has_sh : -1;
+        owner_item[kTile + tid] = i_sh;
+        if (has_sh) {
+            sh.u0 = u0;
+            a.item[i_sh] = sh;
+            if (i_sh < kPlanItems) u_item[i_sh] = u0;
+        }
+        if (has_own) {
+            own.u0 = u0 + u_sh;
+            a.item[i_own] = own;
+            if (i_own < kPlanItems) u_item[i_own] = own.u0;
+        }
+        __syncthreads();
+        if (in) {
+            int mine = -1;
+            if (v_hi[tid] > v_lo[tid]) {  // (the item starts at most 127 rows before)
+                const int o = gr.start + (b - gr.start) / R * R - base + kTile;
+                mine = o >= 0 ? owner_item[o] : -1;
+            }
+            a.row[b] = me.bad ? make_int4(0, 0, -2, -2) : make_int4(me.lo, me.len, mine, i_own);
+        }
+        __syncthreads();
+    }
+    const int G = (int)max(1LL, min((long long)a.shares, units / kMinShare));
+    if (tid == 0) *a.line = Line{units, items, G};
+    if (units == 0) return;
+    for (int s = tid; s < G; s += kPlanThreads) {
+        const long long u = mul_div(s, units, G);
+        a.first[s] = last_at(items, [&](int i) { return (items <= kPlanItems ? u_item[i] : a.item[i].u0) <= u; });
+    }
+}
+
+// A share's walk over its pieces of the items.
+struct Piece {
+    Item it;
+    int index, t0, t1, tiles;  // tiles [t0, t1) of `tiles`
+};
+
+struct Walk {
+    const Item* items;
+    int next_i, n;
+    long long left;
+    long long u;  // the unit that comes next
+    Item ahead;
+
+    __device__ __forceinline__ void start(const SharedArgs& a, const Line& line, int share) {
+        items = a.item;
+        n = line.items;
+        u = mul_div(share, line.units, line.shares);
+        left = mul_div(share + 1, line.units, line.shares) - u;
+        next_i = a.first[share];
+        load();
+    }
+    __device__ __forceinline__ void load() {
+        if (next_i < n) {
+            const int4* p = reinterpret_cast<const int4*>(items + next_i);
+            reinterpret_cast<int4*>(&ahead)[0] = p[0];
+            reinterpret_cast<int4*>(&ahead)[1] = p[1];
+        }
+    }
+    // the next piece with a tile; false when the share is done
+    __device__ __forceinline__ bool next(Piece& p) {
+        while (left > 0 && next_i < n) {
+            p.it = ahead;
+            p.index = next_i++;
+            load();
+            p.tiles = tiles_of(p.it);
+            const int x = (int)(u - p.it.u0), take = (int)min((long long)(p.tiles + kItemUnits - x), left);
+            left -= take;
+            u += take;
+            p.t0 = max(0, x - kItemUnits);
+            p.t1 = max(0, x + take - kItemUnits);
+            if (p.t1 > p.t0) return true;
+        }
+        return false;
+    }
+};
+
+// ---------------------------------------------------------------------------
+// the products
+// ---------------------------------------------------------------------------
+
+constexpr int kSoftWarps = 8, kSumWarps = 8, kLoadWarps = 4;
+constexpr int kSharedThreads = 32 * (kSoftWarps + kSumWarps + kLoadWarps + 1);
+constexpr int kSharedSmemMax = 232448;
+
+template <int HD, int QT, int PT>
+struct Tm {
+    static constexpr int kTileBytes = kTile * HD * 2;  // K or V rows of a tile, and one term of Q
+    static constexpr int kQBufs = QT == 1 ? 2 : 1;
+    static constexpr int kQ = kQBufs * QT * kTileBytes;
+    static constexpr int kFixed = 1024 + 8192;  // alignment, then barriers and small tables
+    static constexpr int kFit = (kSharedSmemMax - kFixed - kQ) / kTileBytes;
+    static constexpr int kStages = kFit > 8 ? 8 : kFit;
+    // copies that a loading thread leaves in flight behind the one it has just issued
+    static constexpr int kAhead = kStages > 4 ? 4 : kStages - 2;
+    static_assert(kStages >= 3, "three tiles must fit");
+    static constexpr int kTotal = kFixed + kQ + kStages * kTileBytes;
+    // tensor memory: two S (P over it, a third term behind it), then T
+    static constexpr int kSCols = PT == 3 ? 192 : 128;
+    static constexpr int kTBufs = 2 * kSCols + 2 * HD <= 512 ? 2 : 1;
+    static_assert(2 * kSCols + kTBufs * HD <= 512, "tensor memory plan");
+};
+
+struct SmallShared {
+    uint64_t full[8], empty[8], q_empty[2], s_full[2], p_full[2], t_full[2], t_empty[2];
+    uint32_t tmem;
+    int dead;               // a wait gave up
+    uint32_t bad[8][4];     // positions of a tile whose page does not exist
+    float2 stats[4][kTile]; // m (log2 units) and l of a tile's rows
+    float factor[4][kTile]; // what an accumulator of S is times for a score
+};
+static_assert(sizeof(SmallShared) <= 8192, "");
+
+__device__ __forceinline__ bool shared_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = global_ns();
+    while (true) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*dead) return false;
+        if (global_ns() - t0 > kSharedWaitNs) {
+            *dead = 1;
+            return false;
+        }
+    }
+}
+
+// The same by a warp: one answer for all lanes.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
+    return __all_sync(0xffffffffu, shared_wait(bar, parity, dead));
+}
+
+// V as the second operand: its rows are positions, the products' K, and its
+// dimensions lie in 128-byte runs, 64 of them, the next 64 a block on: 8
+// positions are 1024 bytes (stride), the blocks kTile * 128 apart (leading).
+__device__ __forceinline__ uint64_t v_desc(uint32_t saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((kTile * 128) >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) |
+           ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
+}
+
+template <typename C>
+__device__ __forceinline__ uint32_t idesc(int n, bool v) {
+    const uint32_t type = std::is_same<C, __half>::value ? 0u : 1u;
+    return (1u << 4) | (type << 7) | (type << 10) | ((v ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+          "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
+          "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+// 8 elements from p on
+__device__ __forceinline__ void load8(const float* p, bool wide, float* x) {
+    if (wide) {
+        const float4 u = reinterpret_cast<const float4*>(p)[0], v = reinterpret_cast<const float4*>(p)[1];
+        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+        x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = p[i];
+    }
+}
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, bool wide, float* x) {
+    alignas(16) T t[8];
+    if (wide) *reinterpret_cast<uint4*>(t) = *reinterpret_cast<const uint4*>(p);
+    else
+#pragma unroll
+        for (int i = 0; i < 8; i++) t[i] = p[i];
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = to_float(t[i]);
+}
+
+template <int HD, typename T, typename C, int QT, int PT>
+__global__ void __launch_bounds__(kSharedThreads, 1) shared_tiles_kernel(const __grid_constant__ SharedArgs a) {
+    using TM = Tm<HD, QT, PT>;
+    constexpr int NS = TM::kStages, NT = TM::kTBufs, QB = TM::kQBufs;
+    extern __shared__ __align__(1024) uint8_t ssm_raw[];
+    uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ssm_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* const q_sm = base;
+    uint8_t* const ring = base + TM::kQ;
+    SmallShared& s = *reinterpret_cast<SmallShared*>(ring + NS * TM::kTileBytes);
+    volatile int* dead = &s.dead;
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int heads = a.nkv * a.blocks;
+    const int share = blockIdx.x / heads, hr = blockIdx.x - share * heads;
+    const int h = hr / a.blocks, blk = hr - h * a.blocks;  // KV head, block of its query heads
+    const int head0 = h * a.grp + blk * a.hb, hn = min(a.hb, a.grp - blk * a.hb);
+    const int hd = a.hd;
+
+    if (tid == 0) {
+        for (int i = 0; i < 8; i++) {
+            mbar_init(&s.full[i], kLoadWarps);
+            mbar_init(&s.empty[i], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&s.q_empty[i], 1);
+            mbar_init(&s.s_full[i], 1);
+            mbar_init(&s.p_full[i], 4);
+            mbar_init(&s.t_full[i], 1);
+            mbar_init(&s.t_empty[i], kSumWarps);
+        }
+        s.dead = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 20) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s.tmem)), "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    // columns past hd stay zero: the copies never write them
+    if (hd < HD) {
+        for (int i = tid; i < (TM::kQ + NS * TM::kTileBytes) / 16; i += kSharedThreads)
+            *reinterpret_cast<uint4*>(base + 16 * i) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async();
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = s.tmem;
+    pdl_wait();
+    pdl_trigger();
+
+    const Line line = *a.line;
+    Walk walk;
+    Piece p;
+    const bool work = line.units > 0 && share < line.shares;
+    if (work) walk.start(a, line, share);
+
+    if (!work) {
+    } else if (warp < kSoftWarps) {
+        // ------------------------------------------------------------ exponentials
+        const int wg = warp >> 2, quad = warp & 3, m = quad * 32 + lane;
+        const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+        const uint32_t s_col = tmem + lanes + wg * TM::kSCols;
+        const int rr = m / a.hb, hh = m - rr * a.hb;
+        const float cap = a.softcap;
+        const bool plain = !(cap > 0.0f) && !a.slopes;
+        const float slope = a.slopes && hh < hn ? a.slopes[head0 + hh] * kLog2e : 0.0f;
+        int j = 0, piece = 0;
+        bool ok = true;
+        while (ok && walk.next(p)) {
+            const bool mine = rr < p.it.rows && hh < hn;
+            int lo = 0, hi = 0, len = 0;
+            if (mine) {
+                const int4 r = a.row[p.it.row0 + rr];
+                len = r.y;
+                lo = max(r.x, p.it.lo);
+                hi = min(r.y, p.it.limit);
+            }
+            const bool busy = __any_sync(0xffffffffu, mine);
+            for (int t = p.t0; t < p.t1; t++, j++) {
+                if ((j & 1) != wg) continue;
+                if (!warp_wait(&s.s_full[wg], (j >> 1) & 1, dead)) {
+                    ok = false;
+                    break;
+                }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (busy) {
+                    const int p0 = p.it.lo + t * kTile, c0 = lo - p0, c1 = hi - p0;
+                    const int chunks = (min(kTile, p.it.hi - p0) + 31) / 32;
+                    const bool mask = __any_sync(0xffffffffu, c0 > 0 || c1 < 32 * chunks);
+                    float f = QT == 1 ? (cap > 0.0f ? a.scale / cap : a.scale * kLog2e) : s.factor[piece & 3][m];
+                    float mx = -INFINITY;
+#pragma unroll 1
+                    for (int ch = 0; ch < chunks; ch++) {
+                        uint32_t r[32];
+                        tmem_ld32(s_col + 32 * ch, r);
+                        if (!plain) {
+#pragma unroll
+                            for (int i = 0; i < 32; i++) {
+                                float x = __uint_as_float(r[i]) * f;
+                                if (cap > 0.0f) x = (cap * kLog2e) * tanhf(x);
+                                x = fmaf(slope, (float)(p0 + 32 * ch + i - (len - 1)), x);
+                                r[i] = __float_as_uint(x);
+                            }
+                        }
+                        if (mask) {
+#pragma unroll
+                            for (int i = 0; i < 32; i++)
+                                if (32 * ch + i < c0 || 32 * ch + i >= c1) r[i] = __float_as_uint(-INFINITY);
+                        }
+                        if (!plain) {
+                            tmem_st16(s_col + 32 * ch, r);
+                            tmem_st16(s_col + 32 * ch + 16, r + 16);
+                        }
+                        float x0 = mx, x1 = -INFINITY;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            x0 = fmaxf(x0, __uint_as_float(r[i]));
+                            x1 = fmaxf(x1, __uint_as_float(r[i + 1]));
+                        }
+                        mx = fmaxf(x0, x1);
+                    }
+                    if (!plain) {
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                        f = 1.0f;
+                    }
+                    const float top = mx == -INFINITY ? -INFINITY : mx * f, z = (top == -INFINITY ? 0.0f : top) - 14.0f;
+                    float l0 = 0.0f, l1 = 0.0f;
+#pragma unroll 1
+                    for (int ch = 0; ch < chunks; ch++) {
+                        uint32_t r[32];
+                        tmem_ld32(s_col + 32 * ch, r);
+                        if (mask && plain) {
+#pragma unroll
+                            for (int i = 0; i < 32; i++)
+                                if (32 * ch + i < c0 || 32 * ch + i >= c1) r[i] = __float_as_uint(-INFINITY);
+                        }
+                        uint32_t w[PT][16];
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const float e0 = ex2(fmaf(__uint_as_float(r[2 * i]), f, -z));
+                            const float e1 = ex2(fmaf(__uint_as_float(r[2 * i + 1]), f, -z));
+                            l0 += e0;
+                            l1 += e1;
+                            uint32_t x[PT];
+                            split_terms<C, PT>(e0, e1, x);
+#pragma unroll
+                            for (int k = 0; k < PT; k++) w[k][i] = x[k];
+                        }
+                        if (PT == 1) {
+                            tmem_st16(s_col + 16 * ch, w[0]);
+                        } else {
+                            tmem_st16(s_col + 32 * ch, w[0]);
+                            tmem_st16(s_col + 32 * ch + 16, w[PT > 1 ? 1 : 0]);
+                            if (PT == 3) tmem_st16(s_col + 128 + 16 * ch, w[PT - 1]);
+                        }
+                    }
+                    float l = l0 + l1;
+                    const uint32_t* bad = s.bad[j & 7];
+                    if (bad[0] | bad[1] | bad[2] | bad[3]) {
+                        for (int c = max(c0, 0); c < min(c1, kTile); c++)
+                            if ((bad[c >> 5] >> (c & 31)) & 1) l = __int_as_float(0x7fc00000);
+                    }
+                    s.stats[j & 3][m] = make_float2(top, l);
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s.p_full[wg]);
+            }
+            piece++;
+        }
+    } else if (warp < kSoftWarps + kSumWarps) {
+        // ------------------------------------------------------------ O
+        constexpr int HC = HD / 2;  // columns of a warp
+        const int half = (warp - kSoftWarps) >> 2, quad = warp & 3, m = quad * 32 + lane;
+        const uint32_t t_col = tmem + ((uint32_t)(quad * 32) << 16) + 2 * TM::kSCols + half * HC;
+        const int rr = m / a.hb, hh = m - rr * a.hb;
+        const int d0 = half * HC, dn = min(HC, hd - d0);  // this warp's dimensions
+        int j = 0;
+        bool ok = true;
+        while (walk.next(p)) {
+            const bool mine = rr < p.it.rows && hh < hn;
+            const bool busy = __any_sync(0xffffffffu, mine);
+            unsigned long long o[HC / 2];
+            float M = -INFINITY, L = 0.0f;
+#pragma unroll
+            for (int i = 0; i < HC / 2; i++) o[i] = 0;
+#pragma unroll 1
+            for (int t = p.t0; t < p.t1; t++, j++) {
+                const int buf = j % NT;
+                ok = ok && warp_wait(&s.t_full[buf], (j / NT) & 1, dead);
+                if (!ok) continue;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (busy) {
+                    const float2 st = s.stats[j & 3][m];
+                    const float n = fmaxf(M, st.x), z = n == -INFINITY ? 0.0f : n;
+                    const float fo = ex2(M - z), ft = ex2(st.x - z);
+                    M = n;
+                    L = fmaf(L, fo, st.y * ft);
+                    const unsigned long long fo2 = f2_pack(fo, fo), ft2 = f2_pack(ft, ft);
+#pragma unroll
+                    for (int c = 0; c < HC; c += 16) {
+                        uint32_t r[16];
+                        tmem_ld16(t_col + buf * HD + c, r);
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            const unsigned long long x = f2_pack(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+                            o[c / 2 + i] = f2_fma(o[c / 2 + i], fo2, f2_mul(x, ft2));
+                        }
+                    }
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s.t_empty[buf]);
+            }
+            if (!ok) L = __int_as_float(0x7fc00000);  // (a wait gave up: no result)
+            if (!mine || dn <= 0) continue;
+            const int b = p.it.row0 + rr, head = head0 + hh;
+            const bool start = p.t0 == 0, whole = start && p.t1 == p.tiles;
+            const int4 row = a.row[b];
+            const bool own = p.it.limit == kNoLimit;
+            if (whole && (own ? row.z : row.w) < 0) {  // all that the row sees
+                const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+                T* out = static_cast<T*>(a.out) + (int64_t)b * a.out_stride + (int64_t)head * hd + d0;
+                float big = 0.0f;
+#pragma unroll
+                for (int i = 0; i < HC / 8; i++) {
+                    if (8 * i >= dn) break;
+                    alignas(16) T y[8];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const float2 x = f2_unpack(o[4 * i + k]);
+                        const float u = x.x * inv, v = x.y * inv;
+                        big = fmaxf(fmaxf(big, u - u != 0.0f ? INFINITY : 0.0f), v - v != 0.0f ? INFINITY : 0.0f);
+                        big = u != u || v != v ? INFINITY : big;
+                        y[2 * k] = (T)u;
+                        y[2 * k + 1] = (T)v;
+                    }
+                    if (a.out_wide) {
+#pragma unroll
+                        for (int k = 0; k < (int)sizeof(T) / 2; k++)
+                            reinterpret_cast<uint4*>(out + 8 * i)[k] = reinterpret_cast<const uint4*>(y)[k];
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 8; k++) out[8 * i + k] = y[k];
+                    }
+                }
+                if (a.lse && half == 0) a.lse[(int64_t)b * a.nh + head] = L == 0.0f ? -INFINITY : (M + (log2f(L) - 14.0f)) * kLn2;
+                if (big > 0.0f) a.redo[b] = 1;
+            } else {
+                const int64_t width = hd + 4;
+                float* to = whole ? a.whole + (((int64_t)(own ? 1 : 0) * a.batch + b) * a.nh + head) * width
+                                  : a.part + (((int64_t)blockIdx.x * 2 + (start ? 1 : 0)) * kTile + m) * width;
+#pragma unroll
+                for (int i = 0; i < HC / 4; i++) {
+                    if (4 * i >= dn) break;
+                    const float2 x = f2_unpack(o[2 * i]), y = f2_unpack(o[2 * i + 1]);
+                    *reinterpret_cast<float4*>(to + d0 + 4 * i) = make_float4(x.x, x.y, y.x, y.y);
+                }
+                if (half == 0) *reinterpret_cast<float2*>(to + hd) = make_float2(M, L);
+            }
+        }
+    } else if (warp < kSoftWarps + kSumWarps + kLoadWarps) {
+        // ------------------------------------------------------------ K, V and Q
+        const int lw = warp - kSoftWarps - kSumWarps, row = lw * 32 + lane;
+        constexpr int CH = HD / 8, LR = 32 / CH;  // chunks of a row, rows of a warp's copy
+        const int hc = hd / 8, c = lane % CH, r0 = lane / CH;
+        const uint32_t ring_s = smem_u32(ring);
+        const int64_t h_off = (int64_t)h * a.head_stride + c * 8;
+        int stage = 0, told = 0;  // stages issued, and those that the products know of
+        bool ok = true;
+        auto tell = [&](int upto) {  // the stages before `upto` have landed
+            fence_proxy_async();
+            __syncwarp();
+            for (; told < upto; told++)
+                if (lane == 0) mbar_arrive(&s.full[told % NS]);
+        };
+        // rows with off >= 0 are copied, with off == -1 set to zero, others left
+        auto issue = [&](const uint16_t* src, int64_t off) {
+            const int slot = stage % NS;
+            if (stage >= NS) ok = ok && warp_wait(&s.empty[slot], (stage / NS - 1) & 1, dead);
+            if (!ok) return;
+            const uint32_t at0 = ring_s + slot * TM::kTileBytes + (c >> 3) * (kTile * 128);
+#pragma unroll
+            for (int i = 0; i < 32 / LR; i++) {
+                const int r = i * LR + r0;
+                const int64_t o = __shfl_sync(0xffffffffu, off, r);
+                const int rt = lw * 32 + r;
+                const uint32_t at = at0 + rt * 128 + (((c & 7) ^ (rt & 7)) << 4);
+                if (c < hc && o >= -1) cp16(at, src + (o < 0 ? 0 : o + h_off), o >= 0);
+            }
+            cp_async_commit();
+            stage++;
+            if (stage > TM::kAhead) {
+                cp_wait<TM::kAhead>();
+                tell(stage - TM::kAhead);
+            }
+        };
+        // the place of this lane's row of tile t: its offset; -1: none there; -2: nor needed
+        struct Place {
+            int64_t off;
+            bool bad;
+        };
+        auto fetch = [&](const Item& it, int t) {
+            const int p0 = it.lo + t * kTile, n = min(kTile, it.hi - p0), pos = p0 + row;
+            Place f{row < ((n + 15) & ~15) ? -1 : -2, false};
+            if (row < n) {
+                const int pg = a.page_shift >= 0 ? pos >> a.page_shift : pos / a.page_size;
+                const int page = a.table[(int64_t)it.tr * a.table_stride + pg];
+                f.bad = (unsigned)page >= (unsigned)a.n_pages;
+                if (!f.bad) f.off = page * a.page_stride + (int64_t)(pos - pg * a.page_size) * a.pos_stride;
+            }
+            return f;
+        };
+        auto load_q = [&](const Item& it, int piece) {
+            if (piece >= QB) {
+                uint64_t* bar = &s.q_empty[piece % QB];
+                const uint32_t parity = (piece / QB - 1) & 1;
+                if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
+                    cp_wait<0>();  // (the products that free it may wait for what is on its way)
+                    tell(stage);
+                    ok = ok && warp_wait(bar, parity, dead);
+                }
+            }
+            if (!ok) return;
+            const int m = row, qr = m / a.hb, hh = m - qr * a.hb;
+            if (qr >= it.rows || hh >= hn) return;
+            const T* q = static_cast<const T*>(a.q) + (int64_t)(it.row0 + qr) * a.q_stride + (int64_t)(head0 + hh) * hd;
+            uint8_t* to = q_sm + (piece % QB) * QT * TM::kTileBytes + m * 128;
+            float up = 1.0f;
+            if (QT > 1) {  // the row's largest element to [2^10, 2^11)
+                float mx = 0.0f;
+                for (int i = 0; i < hc; i++) {
+                    float x[8];
+                    load8(q + 8 * i, a.q_wide, x);
+#pragma unroll
+                    for (int k = 0; k < 8; k++) mx = fmaxf(mx, fabsf(x[k]));
+                }
+                const int e = mx < INFINITY ? min(100, 137 - (int)(__float_as_uint(mx) >> 23)) : 0;
+                up = __int_as_float((127 + e) << 23);
+                const float f = a.scale * __int_as_float((127 - e) << 23);
+                s.factor[piece & 3][m] = a.softcap > 0.0f ? f / a.softcap : f * kLog2e;
+            }
+            for (int i = 0; i < hc; i++) {
+                float x[8];
+                load8(q + 8 * i, a.q_wide, x);
+                uint32_t w[QT][4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    uint32_t y[QT];
+                    split_terms<C, QT>(x[2 * k] * up, x[2 * k + 1] * up, y);
+#pragma unroll
+                    for (int u = 0; u < QT; u++) w[u][k] = y[u];
+                }
+#pragma unroll
+                for (int u = 0; u < QT; u++)
+                    *reinterpret_cast<uint4*>(to + u * TM::kTileBytes + (i >> 3) * (kTile * 128) + (((i & 7) ^ (m & 7)) << 4)) =
+                        make_uint4(w[u][0], w[u][1], w[u][2], w[u][3]);
+            }
+        };
+        int j = 0, piece = 0;
+        int64_t v_off = -2;
+        bool have = false, more = walk.next(p);
+        int t = p.t0;
+        Place nx = more ? fetch(p.it, t) : Place{-2, false};
+        while (ok && more) {
+            const Place f = nx;
+            if (t == p.t0) load_q(p.it, piece++);
+            const uint32_t bad = __ballot_sync(0xffffffffu, f.bad);
+            if (lane == 0) s.bad[j & 7][lw] = bad;
+            // the next tile's pages, on their way meanwhile
+            if (++t == p.t1) {
+                more = walk.next(p);
+                t = p.t0;
+            }
+            if (more) nx = fetch(p.it, t);
+            if (ok) issue(a.k, f.off < 0 ? -2 : f.off);
+            if (ok && have) issue(a.v, v_off);
+            v_off = f.off;
+            have = true;
+            j++;
+        }
+        if (ok && have) issue(a.v, v_off);
+        cp_wait<0>();
+        if (ok) tell(stage);
+    } else if (lane == 0) {
+        // ------------------------------------------------------------ products
+        const uint32_t ring_s = smem_u32(ring), q_s = smem_u32(q_sm);
+        const int ks = (hd + 15) / 16, n_v = ks * 16;
+        int stage = 0, j = 0, piece = 0, was = 0;  // was: positions of the tile before, in 16s
+        bool ok = true;
+        auto values = [&](int jj) {  // T = P V of tile jj
+            ok = ok && shared_wait(&s.p_full[jj & 1], (jj >> 1) & 1, dead);
+            ok = ok && shared_wait(&s.full[stage % NS], (stage / NS) & 1, dead);
+            if (jj >= NT) ok = ok && shared_wait(&s.t_empty[jj % NT], (jj / NT - 1) & 1, dead);
+            if (!ok) return;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t v = ring_s + (stage % NS) * TM::kTileBytes, id = idesc<C>(n_v, true);
+            const uint32_t pc = tmem + (jj & 1) * TM::kSCols, tc = tmem + 2 * TM::kSCols + (jj % NT) * HD;
+            uint32_t acc = 0;
+#pragma unroll
+            for (int x = PT - 1; x >= 0; x--)  // (small terms first)
+                for (int k = 0; k < was; k++) {
+                    const uint32_t col = PT == 1 ? 8 * k : x == 2 ? 128 + 8 * k : 32 * (k >> 1) + 16 * x + 8 * (k & 1);
+                    mma_f16_ts(tc, pc + col, v_desc(v + k * 2048), id, acc);
+                    acc = 1;
+                }
+            mma_commit(&s.empty[stage % NS]);
+            mma_commit(&s.t_full[jj % NT]);
+            stage++;
+        };
+        while (ok && walk.next(p)) {
+            const uint32_t q = q_s + (piece % QB) * QT * TM::kTileBytes;
+            for (int t = p.t0; t < p.t1 && ok; t++, j++) {
+                const int n16 = (min(kTile, p.it.hi - (p.it.lo + t * kTile)) + 15) / 16;
+                ok = ok && shared_wait(&s.full[stage % NS], (stage / NS) & 1, dead);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t k_sm = ring_s + (stage % NS) * TM::kTileBytes, id = idesc<C>(16 * n16, false);
+                const uint32_t sc = tmem + (j & 1) * TM::kSCols;
+                uint32_t acc = 0;
+#pragma unroll
+                for (int x = QT - 1; x >= 0; x--)
+                    for (int k = 0; k < ks; k++) {
+                        const uint32_t in = (k >> 2) * (kTile * 128) + (k & 3) * 32;
+                        mma_f16(sc, sw128_desc(q + x * TM::kTileBytes + in), sw128_desc(k_sm + in), id, acc);
+                        acc = 1;
+                    }
+                mma_commit(&s.empty[stage % NS]);
+                mma_commit(&s.s_full[j & 1]);
+                if (t == p.t1 - 1) mma_commit(&s.q_empty[piece % QB]);
+                stage++;
+                if (j > 0) values(j - 1);
+                was = n16;
+            }
+            piece++;
+        }
+        if (ok && j > 0) values(j - 1);
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 20) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+// ---------------------------------------------------------------------------
+// joining
+// ---------------------------------------------------------------------------
+
+constexpr int kSharedJoinThreads = 256;
+
+// o, M (log2 units), L of a row's head, four dimensions a lane
+struct Sum {
+    float4 o;
+    float M, L;
+    __device__ __forceinline__ void add(float4 x, float m, float l) {
+        const float n = fmaxf(M, m), z = n == -INFINITY ? 0.0f : n, f = ex2(M - z), g = ex2(m - z);
+        M = n;
+        L = fmaf(L, f, l * g);
+        o.x = fmaf(o.x, f, x.x * g);
+        o.y = fmaf(o.y, f, x.y * g);
+        o.z = fmaf(o.z, f, x.z * g);
+        o.w = fmaf(o.w, f, x.w * g);
+    }
+};
+
+// A row's head by one warp, from its own positions: 32 scores at a time, a
+// position to a lane, then the values, four dimensions to a lane.
+template <typename T, typename C>
+__device__ __noinline__ Sum row_alone(const SharedArgs& a, int b, int head) {
+    const int lane = threadIdx.x & 31, hd = a.hd, d = 4 * lane;
+    const Seq sq = seq_of(a, b);
+    const int64_t h_off = (int64_t)(head / a.grp) * a.head_stride;
+    const T* q = static_cast<const T*>(a.q) + (int64_t)b * a.q_stride + (int64_t)head * hd;
+    const float slope = a.slopes ? a.slopes[head] : 0.0f;
+    Sum r{make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
+    bool bad = false;
+    for (int p0 = sq.lo; p0 < sq.len; p0 += 32) {
+        const int pos = p0 + lane;
+        int64_t off = -1;
+        float x = -INFINITY;
+        if (pos < sq.len) {
+            const int pg = pos / a.page_size, page = a.table[(int64_t)sq.tr * a.table_stride + pg];
+            if ((unsigned)page < (unsigned)a.n_pages) {
+                off = page * a.page_stride + (int64_t)(pos - pg * a.page_size) * a.pos_stride + h_off;
+                const C* k = reinterpret_cast<const C*>(a.k) + off;
+                float dot = 0.0f;
+                for (int i = 0; i < hd; i++) dot = fmaf(to_float(q[i]), to_float(k[i]), dot);
+                x = dot * a.scale;
+                if (a.softcap > 0.0f) x = a.softcap * tanhf(x / a.softcap);
+                x = fmaf(slope, (float)(pos - (sq.len - 1)), x) * kLog2e;
+            } else {
+                bad = true;
+            }
+        }
+        float m = x;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float n = fmaxf(r.M, m), z = n == -INFINITY ? 0.0f : n, f = ex2(r.M - z);
+        const float e = pos < sq.len ? ex2(x - z + 14.0f) : 0.0f;
+        r.M = n;
+        float l = e;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        r.L = fmaf(r.L, f, l);
+        r.o = make_float4(r.o.x * f, r.o.y * f, r.o.z * f, r.o.w * f);
+        for (int j = 0; j < min(32, sq.len - p0); j++) {
+            const int64_t at = __shfl_sync(0xffffffffu, off, j);
+            const float w = __shfl_sync(0xffffffffu, e, j);
+            if (at >= 0 && d < hd) {
+                const C* v = reinterpret_cast<const C*>(a.v) + at + d;
+                r.o.x = fmaf(w, to_float(v[0]), r.o.x);
+                r.o.y = fmaf(w, to_float(v[1]), r.o.y);
+                r.o.z = fmaf(w, to_float(v[2]), r.o.z);
+                r.o.w = fmaf(w, to_float(v[3]), r.o.w);
+            }
+        }
+    }
+    if (__any_sync(0xffffffffu, bad)) r.L = __int_as_float(0x7fc00000);
+    return r;
+}
+
+// CTAs (rows in turn, heads in turn), a warp for a head.
+template <typename T, typename C>
+__global__ void __launch_bounds__(kSharedJoinThreads) shared_join_kernel(const __grid_constant__ SharedArgs a) {
+    pdl_trigger();
+    pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hd = a.hd, d = 4 * lane;
+    const Line line = *a.line;
+    const int64_t width = hd + 4;
+    for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
+        const int4 row = a.row[b];
+        const int redo = a.redo[b];
+        // the shares of the row's items
+        struct Part {
+            int first, last, base;  // base: the row's place among the item's (row, head) pairs
+        } part[2];
+        bool cut = false;
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const int i = k ? row.w : row.z;
+            part[k] = Part{0, -1, 0};
+            if (i < 0) continue;
+            const Item it = a.item[i];
+            const long long u = it.u0 + kItemUnits;
+            part[k].first = (int)mul_div(u + 1, line.shares, line.units, -1);
+            part[k].last = (int)mul_div(u + tiles_of(it), line.shares, line.units, -1);
+            part[k].base = (b - it.row0) * a.hb;
+            cut |= part[k].first != part[k].last;
+        }
+        const bool one = (row.z >= 0) != (row.w >= 0);
+        if (one && !cut && !redo) continue;  // written already
+        for (int head = blockIdx.y * (kSharedJoinThreads / 32) + warp; head < a.nh;
+             head += gridDim.y * (kSharedJoinThreads / 32)) {
+            Sum r{make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
+            if (row.z == -2) {
+                r.L = __int_as_float(0x7fc00000);
+            } else if (!redo) {
+                const int h = head / a.grp, in = head - h * a.grp, blk = in / a.hb, hh = in - blk * a.hb;
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const Part pt = part[k];
+                    constexpr int N = 4;  // pieces in flight
+                    for (int i0 = pt.first; i0 <= pt.last; i0 += N) {
+                        float4 x[N];
+                        float2 ml[N];
+#pragma unroll
+                        for (int n = 0; n < N; n++) {
+                            const int i = i0 + n;
+                            const float* from =
+                                pt.first == pt.last
+                                    ? a.whole + (((int64_t)k * a.batch + b) * a.nh + head) * width
+                                    : a.part + (((int64_t)(i * a.nkv * a.blocks + h * a.blocks + blk) * 2 + (i == pt.first ? 1 : 0)) * kTile +
+                                                pt.base + hh) * width;
+                            x[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            ml[n] = make_float2(-INFINITY, 0.0f);
+                            if (i <= pt.last) {
+                                ml[n] = *reinterpret_cast<const float2*>(from + hd);
+                                if (d < hd) x[n] = *reinterpret_cast<const float4*>(from + d);
+                            }
+                        }
+#pragma unroll
+                        for (int n = 0; n < N; n++) r.add(x[n], ml[n].x, ml[n].y);
+                    }
+                }
+                const float t = r.L == 0.0f ? 0.0f : (r.o.x + r.o.y + r.o.z + r.o.w) / r.L;
+                if (__any_sync(0xffffffffu, d < hd && t - t != 0.0f)) r = row_alone<T, C>(a, b, head);
+            } else {
+                r = row_alone<T, C>(a, b, head);
+            }
+            const float inv = r.L == 0.0f ? 0.0f : 1.0f / r.L;
+            T* out = static_cast<T*>(a.out) + (int64_t)b * a.out_stride + (int64_t)head * hd;
+            if (d < hd) {
+                out[d] = (T)(r.o.x * inv);
+                out[d + 1] = (T)(r.o.y * inv);
+                out[d + 2] = (T)(r.o.z * inv);
+                out[d + 3] = (T)(r.o.w * inv);
+            }
+            if (a.lse && lane == 0)
+                a.lse[(int64_t)b * a.nh + head] = r.L == 0.0f ? -INFINITY : (r.M + (log2f(r.L) - 14.0f)) * kLn2;
+        }
+    }
+}
+
+constexpr int kMaxSharedDevices = 64;
+
+template <int HD, typename T, typename C, int QT, int PT>
+cudaError_t go(const SharedArgs& a, int sms, cudaStream_t s) {
+    static std::atomic<bool> attr[kMaxSharedDevices] = {};  // the attribute belongs to a device
+    constexpr int smem = Tm<HD, QT, PT>::kTotal;
+    auto kern = shared_tiles_kernel<HD, T, C, QT, PT>;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= kMaxSharedDevices || !attr[dev]) {
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+        if (dev < kMaxSharedDevices) attr[dev] = true;
+    }
+    e = launch_pdl(shared_line_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
+    if (e != cudaSuccess) return e;
+    e = launch_pdl(kern, dim3((unsigned)(a.shares * a.nkv * a.blocks)), dim3(kSharedThreads), smem, s, a);
+    if (e != cudaSuccess) return e;
+    const int rows = std::min(a.batch, 8 * sms);
+    const int y = std::max(1, std::min((a.nh + 7) / 8, 8 * sms / rows));
+    return launch_pdl(shared_join_kernel<T, C>, dim3(rows, y), dim3(kSharedJoinThreads), 0, s, a);
+}
+
+template <int HD>
+cudaError_t go_hd(const SharedArgs& a, int dtype, int cache, int sms, cudaStream_t s) {
+    if (dtype == 0)
+        return cache == 1 ? go<HD, float, __half, 2, 2>(a, sms, s) : go<HD, float, __nv_bfloat16, 3, 3>(a, sms, s);
+    return cache == 1 ? go<HD, __half, __half, 1, 2>(a, sms, s) : go<HD, __nv_bfloat16, __nv_bfloat16, 1, 2>(a, sms, s);
+}
+
+// How a group of query heads falls to items, and the shares of the machine.
+struct Shape {
+    int hb, blocks, rows, shares;
+    Shape(int nh, int nkv, int sms) {
+        const int grp = nh / nkv;
+        hb = std::min(grp, kTile);
+        blocks = (grp + hb - 1) / hb;
+        rows = kTile / hb;
+        shares = std::max(1, sms / (nkv * blocks));
+    }
+};
+
+size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
+
+// The scratch of `batch` rows; where its parts start, if a is given.
+size_t layout(int batch, int nh, int nkv, int hd, int sms, uint8_t* base, SharedArgs* a) {
+    const Shape sh(nh, nkv, sms);
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        uint8_t* p = base + at;
+        at += up16(bytes);
+        return p;
+    };
+    uint8_t* line = take(sizeof(Line));
+    uint8_t* first = take(4 * (size_t)sh.shares);
+    uint8_t* redo = take(4 * (size_t)batch);
+    uint8_t* row = take(16 * (size_t)batch);
+    uint8_t* item = take(2 * sizeof(Item) * (size_t)batch);
+    uint8_t* whole = take((size_t)2 * batch * nh * (hd + 4) * 4);
+    uint8_t* part = take((size_t)sh.shares * nkv * sh.blocks * 2 * kTile * (hd + 4) * 4);
+    if (a) {
+        a->line = reinterpret_cast<Line*>(line);
+        a->first = reinterpret_cast<int*>(first);
+        a->redo = reinterpret_cast<int*>(redo);
+        a->row = reinterpret_cast<int4*>(row);
+        a->item = reinterpret_cast<Item*>(item);
+        a->whole = reinterpret_cast<float*>(whole);
+        a->part = reinterpret_cast<float*>(part);
+    }
+    return at;
+}
+
+}  // namespace
 
 size_t attention_shared_scratch(int batch, int nh, int nkv, int hd, int sms) {
-    return attention_paged_scratch(batch, nh, nkv, hd, sms);
+    if (hd > 128) return attention_paged_scratch(batch, nh, nkv, hd, sms);
+    return layout(batch, nh, nkv, hd, sms, nullptr, nullptr);
 }
 
 int launch_attention_shared(const b2_paged_kv& kv, const b2_paged_attn_opts& o, const void* q, const int32_t* table,
                             const int32_t* lens, const int32_t* req, int batch, const int32_t* starts,
                             const int32_t* prefix, int n_groups, void* out, float* lse, void* scratch, cudaStream_t s,
                             std::string* err) {
-    (void)starts, (void)prefix, (void)n_groups;
-    return launch_attention_paged(kv, o, q, table, lens, req, batch, out, lse, scratch, s, err);
+    if (kv.hd > 128) return launch_attention_paged(kv, o, q, table, lens, req, batch, out, lse, scratch, s, err);
+    const int sms = current_sms(err);
+    if (!sms) return B2_ERR_CUDA;
+    SharedArgs a{};
+    a.q = q;
+    a.k = static_cast<const uint16_t*>(kv.k);
+    a.v = static_cast<const uint16_t*>(kv.v);
+    a.table = table;
+    a.lens = lens;
+    a.req = req;
+    a.starts = starts;
+    a.prefix = prefix;
+    a.out = out;
+    a.lse = lse;
+    a.slopes = o.slopes;
+    const int64_t qd = (int64_t)o.nh * kv.hd;
+    a.q_stride = o.q_stride ? o.q_stride : qd;
+    a.out_stride = o.out_stride ? o.out_stride : qd;
+    a.table_stride = o.table_stride ? o.table_stride : o.max_pages;
+    a.page_stride = kv.page_stride;
+    a.pos_stride = kv.pos_stride;
+    a.head_stride = kv.head_stride;
+    a.batch = batch;
+    a.nh = o.nh;
+    a.nkv = kv.nkv;
+    a.grp = o.nh / kv.nkv;
+    a.hd = kv.hd;
+    a.page_size = kv.page_size;
+    a.page_shift = (kv.page_size & (kv.page_size - 1)) ? -1 : __builtin_ctz(kv.page_size);
+    a.n_pages = kv.n_pages;
+    a.max_pages = o.max_pages;
+    a.n_req = o.n_req;
+    a.len_add = o.len_add;
+    a.window = o.window;
+    a.n_groups = n_groups;
+    const Shape sh(o.nh, kv.nkv, sms);
+    a.hb = sh.hb;
+    a.blocks = sh.blocks;
+    a.rows = sh.rows;
+    a.shares = sh.shares;
+    const int es = o.dtype == 0 ? 4 : 2;
+    a.q_wide = !(reinterpret_cast<uintptr_t>(q) & 15) && a.q_stride * es % 16 == 0;
+    a.out_wide = !(reinterpret_cast<uintptr_t>(out) & 15) && a.out_stride * es % 16 == 0;
+    a.scale = o.scale > 0.0f ? o.scale : (float)(1.0 / sqrt((double)kv.hd));
+    a.softcap = o.softcap;
+    layout(batch, o.nh, kv.nkv, kv.hd, sms, static_cast<uint8_t*>(scratch), &a);
+    const cudaError_t e = kv.hd <= 64 ? go_hd<64>(a, o.dtype, kv.dtype, sms, s) : go_hd<128>(a, o.dtype, kv.dtype, sms, s);
+    return e == cudaSuccess ? B2_OK : cuda_failed("shared attention launch", e, err);
 }
 
 }  // namespace b2
