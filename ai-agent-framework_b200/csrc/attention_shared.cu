@@ -19,9 +19,10 @@
 // follows the lengths that it finds.  A first launch of one CTA lays the line.
 //
 // One CTA an SM, its roles warp by warp:
-//   16-19  K and V rows by cp.async into a ring of tiles in the 128-byte swizzle
-//          that the products read (pages may have any size), Q at an item's start
-//   20     tcgen05.mma, one thread: S = Q K^T of tile j + 1, then T = P V of tile
+//   16-17  K and V rows by cp.async into a ring of tiles in the 128-byte swizzle
+//          that the products read (pages may have any size)
+//   18     the share's pieces of the items, laid out ahead for the others, and Q
+//   19     tcgen05.mma, one thread: S = Q K^T of tile j + 1, then T = P V of tile
 //          j, P being read from tensor memory
 //   0-7    two warpgroups taking tiles in turn: S out of tensor memory, a row to
 //          a thread, the exponentials, P back over S
@@ -239,69 +240,28 @@ __global__ void __launch_bounds__(kPlanThreads) shared_line_kernel(const __grid_
     }
 }
 
-// A share's walk over its pieces of the items.
-struct Piece {
-    Item it;
-    int index, t0, t1, tiles;  // tiles [t0, t1) of `tiles`
-};
-
-struct Walk {
-    const Item* items;
-    int next_i, n;
-    long long left;
-    long long u;  // the unit that comes next
-    Item ahead;
-
-    __device__ __forceinline__ void start(const SharedArgs& a, const Line& line, int share) {
-        items = a.item;
-        n = line.items;
-        u = mul_div(share, line.units, line.shares);
-        left = mul_div(share + 1, line.units, line.shares) - u;
-        next_i = a.first[share];
-        load();
-    }
-    __device__ __forceinline__ void load() {
-        if (next_i < n) {
-            const int4* p = reinterpret_cast<const int4*>(items + next_i);
-            reinterpret_cast<int4*>(&ahead)[0] = p[0];
-            reinterpret_cast<int4*>(&ahead)[1] = p[1];
-        }
-    }
-    // the next piece with a tile; false when the share is done
-    __device__ __forceinline__ bool next(Piece& p) {
-        while (left > 0 && next_i < n) {
-            p.it = ahead;
-            p.index = next_i++;
-            load();
-            p.tiles = tiles_of(p.it);
-            const int x = (int)(u - p.it.u0), take = (int)min((long long)(p.tiles + kItemUnits - x), left);
-            left -= take;
-            u += take;
-            p.t0 = max(0, x - kItemUnits);
-            p.t1 = max(0, x + take - kItemUnits);
-            if (p.t1 > p.t0) return true;
-        }
-        return false;
-    }
-};
-
 // ---------------------------------------------------------------------------
 // the products
 // ---------------------------------------------------------------------------
 
-constexpr int kSoftWarps = 8, kSumWarps = 8, kLoadWarps = 4;
-constexpr int kSharedThreads = 32 * (kSoftWarps + kSumWarps + kLoadWarps + 1);
+constexpr int kSoftWarps = 8, kSumWarps = 8;  // then two warps that copy, one that plans and brings Q, one that multiplies
+constexpr int kCopyWarp = kSoftWarps + kSumWarps, kCopyWarps = 2, kQWarp = kCopyWarp + kCopyWarps, kMmaWarp = kQWarp + 1;
+constexpr int kSharedThreads = 32 * (kMmaWarp + 1);
 constexpr int kSharedSmemMax = 232448;
+constexpr int kPieces = 4;  // pieces known ahead
+// registers of a thread: 96 at the launch, of which the last four warps give some to O's
+constexpr int kSumRegs = 112, kLastRegs = 64;
+static_assert(kSharedThreads == 640 && 256 * 96 + 256 * kSumRegs + 128 * kLastRegs <= 640 * 96, "register split");
 
 template <int HD, int QT, int PT>
 struct Tm {
     static constexpr int kTileBytes = kTile * HD * 2;  // K or V rows of a tile, and one term of Q
     static constexpr int kQBufs = QT == 1 ? 2 : 1;
     static constexpr int kQ = kQBufs * QT * kTileBytes;
-    static constexpr int kFixed = 1024 + 8192;  // alignment, then barriers and small tables
+    static constexpr int kFixed = 1024 + 17408;  // alignment, then barriers and small tables
     static constexpr int kFit = (kSharedSmemMax - kFixed - kQ) / kTileBytes;
     static constexpr int kStages = kFit > 8 ? 8 : kFit;
-    // copies that a loading thread leaves in flight behind the one it has just issued
+    // copies that a copying thread leaves in flight behind the one it has just issued
     static constexpr int kAhead = kStages > 4 ? 4 : kStages - 2;
     static_assert(kStages >= 3, "three tiles must fit");
     static constexpr int kTotal = kFixed + kQ + kStages * kTileBytes;
@@ -311,25 +271,48 @@ struct Tm {
     static_assert(2 * kSCols + kTBufs * HD <= 512, "tensor memory plan");
 };
 
-struct SmallShared {
-    uint64_t full[8], empty[8], q_empty[2], s_full[2], p_full[2], t_full[2], t_empty[2];
-    uint32_t tmem;
-    int dead;               // a wait gave up
-    uint32_t bad[8][4];     // positions of a tile whose page does not exist
-    float2 stats[4][kTile]; // m (log2 units) and l of a tile's rows
-    float factor[4][kTile]; // what an accumulator of S is times for a score
+// Tiles [t0, t1) of an item, as the planning warp lays them out for the others.
+struct Piece {
+    int row0, rows, lo, hi, tr, t0, t1;
+    int kind;  // of the bits below
 };
-static_assert(sizeof(SmallShared) <= 8192, "");
+constexpr int kPieceStart = 1, kPieceWhole = 2, kPieceOwn = 4, kPieceLast = 8;  // kPieceLast: no piece, the share is done
 
+struct SmallShared {
+    uint64_t full[8], empty[8], q_full[2], q_empty[2], s_full[2], p_full[2], t_full[2], t_empty[2];
+    uint64_t piece_full[kPieces], piece_empty[kPieces];
+    uint32_t tmem;
+    int dead;                    // a wait gave up
+    uint32_t bad[8][4];          // positions of a tile whose page does not exist
+    Piece piece[kPieces];
+    int4 row[kPieces][kTile];    // of a row of the product: first and end position, length, 1 + (all of the row: 2); 0: no row
+    float2 stats[4][kTile];      // m (log2 units) and l of a tile's rows
+    float factor[kPieces][kTile];  // what an accumulator of S is times for a score
+};
+static_assert(sizeof(SmallShared) <= 17408, "");
+
+// Waits for a barrier's phase, asleep where the hardware can: a warp that
+// polls takes issue slots from the four others of its scheduler.
 __device__ __forceinline__ bool shared_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t t0 = global_ns();
-    while (true) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if (*dead) return false;
-        if (global_ns() - t0 > kSharedWaitNs) {
-            *dead = 1;
-            return false;
+    uint64_t t0 = 0;
+    for (unsigned n = 0;; n++) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity), "r"(10000000u)
+            : "memory");
+        if (ok) return true;
+        if (n % 64 == 63) {
+            if (*dead) return false;
+            const uint64_t t = global_ns();
+            if (!t0) t0 = t;
+            if (t - t0 > kSharedWaitNs) {
+                *dead = 1;
+                return false;
+            }
         }
     }
 }
@@ -365,31 +348,50 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+// One lane of a converged warp, chosen so that the compiler knows of it: the
+// products' descriptors live in the warp's uniform registers.  (With lane == 0
+// in place of this and unrolled loops, one product of eight got its
+// predecessor's descriptor.)
+__device__ __forceinline__ bool elected() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// 8 elements from p on
-__device__ __forceinline__ void load8(const float* p, bool wide, float* x) {
-    if (wide) {
-        const float4 u = reinterpret_cast<const float4*>(p)[0], v = reinterpret_cast<const float4*>(p)[1];
-        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-        x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = p[i];
-    }
+// 4 elements from p on
+__device__ __forceinline__ float4 load4(const float* p, bool wide) {
+    return wide ? *reinterpret_cast<const float4*>(p) : make_float4(p[0], p[1], p[2], p[3]);
 }
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool wide, float* x) {
-    alignas(16) T t[8];
-    if (wide) *reinterpret_cast<uint4*>(t) = *reinterpret_cast<const uint4*>(p);
+__device__ __forceinline__ float4 load4(const T* p, bool wide) {
+    alignas(8) T t[4];
+    if (wide) *reinterpret_cast<uint2*>(t) = *reinterpret_cast<const uint2*>(p);
     else
 #pragma unroll
-        for (int i = 0; i < 8; i++) t[i] = p[i];
-#pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = to_float(t[i]);
+        for (int i = 0; i < 4; i++) t[i] = p[i];
+    return make_float4(to_float(t[0]), to_float(t[1]), to_float(t[2]), to_float(t[3]));
 }
+
+// Where a warp is in the pieces.
+struct Pieces {
+    int n = 0;  // pieces taken
+    // the next one (of its slot), or null: no more, or a wait gave up
+    __device__ __forceinline__ const Piece* next(SmallShared& s) {
+        const int slot = n % kPieces;
+        if (!warp_wait(&s.piece_full[slot], (n / kPieces) & 1, &s.dead)) return nullptr;
+        n++;
+        return s.piece[slot].kind & kPieceLast ? nullptr : &s.piece[slot];
+    }
+    // the warp is done with the one taken last
+    __device__ __forceinline__ void done(SmallShared& s) const {
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(&s.piece_empty[(n - 1) % kPieces]);
+    }
+};
 
 template <int HD, typename T, typename C, int QT, int PT>
 __global__ void __launch_bounds__(kSharedThreads, 1) shared_tiles_kernel(const __grid_constant__ SharedArgs a) {
@@ -411,20 +413,25 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_tiles_kernel(const _
 
     if (tid == 0) {
         for (int i = 0; i < 8; i++) {
-            mbar_init(&s.full[i], kLoadWarps);
+            mbar_init(&s.full[i], kCopyWarps);
             mbar_init(&s.empty[i], 1);
         }
         for (int i = 0; i < 2; i++) {
+            mbar_init(&s.q_full[i], 1);
             mbar_init(&s.q_empty[i], 1);
             mbar_init(&s.s_full[i], 1);
             mbar_init(&s.p_full[i], 4);
             mbar_init(&s.t_full[i], 1);
             mbar_init(&s.t_empty[i], kSumWarps);
         }
+        for (int i = 0; i < kPieces; i++) {
+            mbar_init(&s.piece_full[i], 1);
+            mbar_init(&s.piece_empty[i], kSoftWarps + kSumWarps + kCopyWarps + 1);
+        }
         s.dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 20) {
+    if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s.tmem)), "r"(512)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -442,35 +449,23 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_tiles_kernel(const _
     pdl_wait();
     pdl_trigger();
 
-    const Line line = *a.line;
-    Walk walk;
-    Piece p;
-    const bool work = line.units > 0 && share < line.shares;
-    if (work) walk.start(a, line, share);
-
-    if (!work) {
-    } else if (warp < kSoftWarps) {
+    if (warp < kSoftWarps) {
         // ------------------------------------------------------------ exponentials
         const int wg = warp >> 2, quad = warp & 3, m = quad * 32 + lane;
-        const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-        const uint32_t s_col = tmem + lanes + wg * TM::kSCols;
-        const int rr = m / a.hb, hh = m - rr * a.hb;
+        const uint32_t s_col = tmem + ((uint32_t)(quad * 32) << 16) + wg * TM::kSCols;
         const float cap = a.softcap;
         const bool plain = !(cap > 0.0f) && !a.slopes;
-        const float slope = a.slopes && hh < hn ? a.slopes[head0 + hh] * kLog2e : 0.0f;
-        int j = 0, piece = 0;
-        bool ok = true;
-        while (ok && walk.next(p)) {
-            const bool mine = rr < p.it.rows && hh < hn;
-            int lo = 0, hi = 0, len = 0;
-            if (mine) {
-                const int4 r = a.row[p.it.row0 + rr];
-                len = r.y;
-                lo = max(r.x, p.it.lo);
-                hi = min(r.y, p.it.limit);
-            }
-            const bool busy = __any_sync(0xffffffffu, mine);
-            for (int t = p.t0; t < p.t1; t++, j++) {
+        float slope = 0.0f;
+        if (a.slopes && m % a.hb < hn) slope = a.slopes[head0 + m % a.hb] * kLog2e;
+        int j = 0;
+        Pieces pieces;
+        while (const Piece* p = pieces.next(s)) {
+            const int slot = (pieces.n - 1) % kPieces;
+            const int4 row = s.row[slot][m];
+            const int it_lo = p->lo, it_hi = p->hi, t1 = p->t1;
+            const bool busy = __any_sync(0xffffffffu, row.w != 0);
+            bool ok = true;
+            for (int t = p->t0; t < t1; t++, j++) {
                 if ((j & 1) != wg) continue;
                 if (!warp_wait(&s.s_full[wg], (j >> 1) & 1, dead)) {
                     ok = false;
@@ -478,10 +473,10 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_tiles_kernel(const _
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if (busy) {
-                    const int p0 = p.it.lo + t * kTile, c0 = lo - p0, c1 = hi - p0;
-                    const int chunks = (min(kTile, p.it.hi - p0) + 31) / 32;
+                    const int p0 = it_lo + t * kTile, c0 = row.x - p0, c1 = row.y - p0;
+                    const int chunks = (min(kTile, it_hi - p0) + 31) / 32;
                     const bool mask = __any_sync(0xffffffffu, c0 > 0 || c1 < 32 * chunks);
-                    float f = QT == 1 ? (cap > 0.0f ? a.scale / cap : a.scale * kLog2e) : s.factor[piece & 3][m];
+                    float f = QT == 1 ? (cap > 0.0f ? a.scale / cap : a.scale * kLog2e) : s.factor[slot][m];
                     float mx = -INFINITY;
 #pragma unroll 1
                     for (int ch = 0; ch < chunks; ch++) {
@@ -492,7 +487,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_tiles_kernel(const _
                             for (int i = 0; i < 32; i++) {
                                 float x = __uint_as_float(r[i]) * f;
                                 if (cap > 0.0f) x = (cap * kLog2e) * tanhf(x);
-                                x = fmaf(slope, (float)(p0 + 32 * ch + i - (len - 1)), x);
+                                x = fmaf(slope, (float)(p0 + 32 * ch + i - (row.z - 1)), x);
                                 r[i] = __float_as_uint(x);
                             }
                         }
@@ -561,26 +556,30 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_tiles_kernel(const _
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&s.p_full[wg]);
             }
-            piece++;
+            if (!ok) break;
+            pieces.done(s);
         }
     } else if (warp < kSoftWarps + kSumWarps) {
         // ------------------------------------------------------------ O
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
         constexpr int HC = HD / 2;  // columns of a warp
         const int half = (warp - kSoftWarps) >> 2, quad = warp & 3, m = quad * 32 + lane;
         const uint32_t t_col = tmem + ((uint32_t)(quad * 32) << 16) + 2 * TM::kSCols + half * HC;
-        const int rr = m / a.hb, hh = m - rr * a.hb;
+        const int rr = m / a.hb, head = head0 + m - rr * a.hb;
         const int d0 = half * HC, dn = min(HC, hd - d0);  // this warp's dimensions
         int j = 0;
         bool ok = true;
-        while (walk.next(p)) {
-            const bool mine = rr < p.it.rows && hh < hn;
-            const bool busy = __any_sync(0xffffffffu, mine);
+        Pieces pieces;
+        while (const Piece* p = pieces.next(s)) {
+            const int4 row = s.row[(pieces.n - 1) % kPieces][m];
+            const bool busy = __any_sync(0xffffffffu, row.w != 0);
             unsigned long long o[HC / 2];
             float M = -INFINITY, L = 0.0f;
 #pragma unroll
             for (int i = 0; i < HC / 2; i++) o[i] = 0;
+            const int t1 = p->t1;
 #pragma unroll 1
-            for (int t = p.t0; t < p.t1; t++, j++) {
+            for (int t = p->t0; t < t1; t++, j++) {
                 const int buf = j % NT;
                 ok = ok && warp_wait(&s.t_full[buf], (j / NT) & 1, dead);
                 if (!ok) continue;
@@ -608,15 +607,13 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_tiles_kernel(const _
                 if (lane == 0) mbar_arrive(&s.t_empty[buf]);
             }
             if (!ok) L = __int_as_float(0x7fc00000);  // (a wait gave up: no result)
-            if (!mine || dn <= 0) continue;
-            const int b = p.it.row0 + rr, head = head0 + hh;
-            const bool start = p.t0 == 0, whole = start && p.t1 == p.tiles;
-            const int4 row = a.row[b];
-            const bool own = p.it.limit == kNoLimit;
-            if (whole && (own ? row.z : row.w) < 0) {  // all that the row sees
+            const int b = p->row0 + rr, kind = p->kind;
+            pieces.done(s);
+            if (!row.w || dn <= 0) continue;
+            if ((kind & kPieceWhole) && (row.w & 2)) {  // all that the row sees
                 const float inv = L == 0.0f ? 0.0f : 1.0f / L;
                 T* out = static_cast<T*>(a.out) + (int64_t)b * a.out_stride + (int64_t)head * hd + d0;
-                float big = 0.0f;
+                bool odd = false;  // not finite
 #pragma unroll
                 for (int i = 0; i < HC / 8; i++) {
                     if (8 * i >= dn) break;
@@ -625,8 +622,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_tiles_kernel(const _
                     for (int k = 0; k < 4; k++) {
                         const float2 x = f2_unpack(o[4 * i + k]);
                         const float u = x.x * inv, v = x.y * inv;
-                        big = fmaxf(fmaxf(big, u - u != 0.0f ? INFINITY : 0.0f), v - v != 0.0f ? INFINITY : 0.0f);
-                        big = u != u || v != v ? INFINITY : big;
+                        odd |= u - u != 0.0f || v - v != 0.0f;
                         y[2 * k] = (T)u;
                         y[2 * k + 1] = (T)v;
                     }
@@ -640,11 +636,12 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_tiles_kernel(const _
                     }
                 }
                 if (a.lse && half == 0) a.lse[(int64_t)b * a.nh + head] = L == 0.0f ? -INFINITY : (M + (log2f(L) - 14.0f)) * kLn2;
-                if (big > 0.0f) a.redo[b] = 1;
+                if (odd) a.redo[b] = 1;
             } else {
                 const int64_t width = hd + 4;
-                float* to = whole ? a.whole + (((int64_t)(own ? 1 : 0) * a.batch + b) * a.nh + head) * width
-                                  : a.part + (((int64_t)blockIdx.x * 2 + (start ? 1 : 0)) * kTile + m) * width;
+                float* to = kind & kPieceWhole
+                                ? a.whole + (((int64_t)(kind & kPieceOwn ? 1 : 0) * a.batch + b) * a.nh + head) * width
+                                : a.part + (((int64_t)blockIdx.x * 2 + (kind & kPieceStart ? 1 : 0)) * kTile + m) * width;
 #pragma unroll
                 for (int i = 0; i < HC / 4; i++) {
                     if (4 * i >= dn) break;
@@ -654,186 +651,300 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_tiles_kernel(const _
                 if (half == 0) *reinterpret_cast<float2*>(to + hd) = make_float2(M, L);
             }
         }
-    } else if (warp < kSoftWarps + kSumWarps + kLoadWarps) {
-        // ------------------------------------------------------------ K, V and Q
-        const int lw = warp - kSoftWarps - kSumWarps, row = lw * 32 + lane;
-        constexpr int CH = HD / 8, LR = 32 / CH;  // chunks of a row, rows of a warp's copy
-        const int hc = hd / 8, c = lane % CH, r0 = lane / CH;
-        const uint32_t ring_s = smem_u32(ring);
-        const int64_t h_off = (int64_t)h * a.head_stride + c * 8;
-        int stage = 0, told = 0;  // stages issued, and those that the products know of
-        bool ok = true;
-        auto tell = [&](int upto) {  // the stages before `upto` have landed
-            fence_proxy_async();
-            __syncwarp();
-            for (; told < upto; told++)
-                if (lane == 0) mbar_arrive(&s.full[told % NS]);
-        };
-        // rows with off >= 0 are copied, with off == -1 set to zero, others left
-        auto issue = [&](const uint16_t* src, int64_t off) {
-            const int slot = stage % NS;
-            if (stage >= NS) ok = ok && warp_wait(&s.empty[slot], (stage / NS - 1) & 1, dead);
-            if (!ok) return;
-            const uint32_t at0 = ring_s + slot * TM::kTileBytes + (c >> 3) * (kTile * 128);
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLastRegs));
+        if (warp < kQWarp) {
+            // -------------------------------------------------------- K and V
+            constexpr int RW = kTile / kCopyWarps;  // rows of a warp
+            const int lw = warp - kCopyWarp, row0 = lw * RW + lane;
+            constexpr int CH = HD / 8, LR = 32 / CH;  // chunks of a row, rows of a warp's copy
+            const int hc = hd / 8, c = lane % CH, r0 = lane / CH;
+            const uint32_t at0 = smem_u32(ring) + (c >> 3) * (kTile * 128) + (lw * RW + r0) * 128;
+            const int64_t h_off = (int64_t)h * a.head_stride + c * 8;
+            int stage = 0, told = 0;  // stages issued, and those that the products know of
+            bool ok = true;
+            auto tell = [&](int upto) {  // the stages before `upto` have landed
+                fence_proxy_async();
+                __syncwarp();
+                for (; told < upto; told++)
+                    if (lane == 0) mbar_arrive(&s.full[told % NS]);
+            };
+            // the places of this lane's rows of a tile: their offset; -1: none there; -2: nor needed
+            struct Place {
+                int64_t off[RW / 32];
+            };
+            struct Look {  // looked up, not yet used
+                int page[RW / 32], pos, n;
+            };
+            // rows with off >= 0 are copied, with off == -1 set to zero, others left
+            auto issue = [&](const uint16_t* src, const Place& f, bool zero) {
+                const int slot = stage % NS;
+                if (stage >= NS) ok = ok && warp_wait(&s.empty[slot], (stage / NS - 1) & 1, dead);
+                if (!ok) return;
+                const uint32_t to = at0 + slot * TM::kTileBytes;
 #pragma unroll
-            for (int i = 0; i < 32 / LR; i++) {
-                const int r = i * LR + r0;
-                const int64_t o = __shfl_sync(0xffffffffu, off, r);
-                const int rt = lw * 32 + r;
-                const uint32_t at = at0 + rt * 128 + (((c & 7) ^ (rt & 7)) << 4);
-                if (c < hc && o >= -1) cp16(at, src + (o < 0 ? 0 : o + h_off), o >= 0);
-            }
-            cp_async_commit();
-            stage++;
-            if (stage > TM::kAhead) {
-                cp_wait<TM::kAhead>();
-                tell(stage - TM::kAhead);
-            }
-        };
-        // the place of this lane's row of tile t: its offset; -1: none there; -2: nor needed
-        struct Place {
-            int64_t off;
-            bool bad;
-        };
-        auto fetch = [&](const Item& it, int t) {
-            const int p0 = it.lo + t * kTile, n = min(kTile, it.hi - p0), pos = p0 + row;
-            Place f{row < ((n + 15) & ~15) ? -1 : -2, false};
-            if (row < n) {
-                const int pg = a.page_shift >= 0 ? pos >> a.page_shift : pos / a.page_size;
-                const int page = a.table[(int64_t)it.tr * a.table_stride + pg];
-                f.bad = (unsigned)page >= (unsigned)a.n_pages;
-                if (!f.bad) f.off = page * a.page_stride + (int64_t)(pos - pg * a.page_size) * a.pos_stride;
-            }
-            return f;
-        };
-        auto load_q = [&](const Item& it, int piece) {
-            if (piece >= QB) {
-                uint64_t* bar = &s.q_empty[piece % QB];
-                const uint32_t parity = (piece / QB - 1) & 1;
-                if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
-                    cp_wait<0>();  // (the products that free it may wait for what is on its way)
-                    tell(stage);
-                    ok = ok && warp_wait(bar, parity, dead);
+                for (int i = 0; i < RW / LR; i++) {
+                    const int r = i * LR + r0;
+                    const int64_t o = __shfl_sync(0xffffffffu, f.off[i * LR / 32], r & 31);
+                    const uint32_t at = to + i * LR * 128 + (((c & 7) ^ (r & 7)) << 4);  // (lw * RW is a multiple of 8)
+                    if (c < hc && (o >= 0 || (zero && o == -1))) cp16(at, src + (o < 0 ? 0 : o + h_off), o >= 0);
                 }
-            }
-            if (!ok) return;
-            const int m = row, qr = m / a.hb, hh = m - qr * a.hb;
-            if (qr >= it.rows || hh >= hn) return;
-            const T* q = static_cast<const T*>(a.q) + (int64_t)(it.row0 + qr) * a.q_stride + (int64_t)(head0 + hh) * hd;
-            uint8_t* to = q_sm + (piece % QB) * QT * TM::kTileBytes + m * 128;
-            float up = 1.0f;
-            if (QT > 1) {  // the row's largest element to [2^10, 2^11)
-                float mx = 0.0f;
-                for (int i = 0; i < hc; i++) {
-                    float x[8];
-                    load8(q + 8 * i, a.q_wide, x);
-#pragma unroll
-                    for (int k = 0; k < 8; k++) mx = fmaxf(mx, fabsf(x[k]));
-                }
-                const int e = mx < INFINITY ? min(100, 137 - (int)(__float_as_uint(mx) >> 23)) : 0;
-                up = __int_as_float((127 + e) << 23);
-                const float f = a.scale * __int_as_float((127 - e) << 23);
-                s.factor[piece & 3][m] = a.softcap > 0.0f ? f / a.softcap : f * kLog2e;
-            }
-            for (int i = 0; i < hc; i++) {
-                float x[8];
-                load8(q + 8 * i, a.q_wide, x);
-                uint32_t w[QT][4];
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    uint32_t y[QT];
-                    split_terms<C, QT>(x[2 * k] * up, x[2 * k + 1] * up, y);
-#pragma unroll
-                    for (int u = 0; u < QT; u++) w[u][k] = y[u];
-                }
-#pragma unroll
-                for (int u = 0; u < QT; u++)
-                    *reinterpret_cast<uint4*>(to + u * TM::kTileBytes + (i >> 3) * (kTile * 128) + (((i & 7) ^ (m & 7)) << 4)) =
-                        make_uint4(w[u][0], w[u][1], w[u][2], w[u][3]);
-            }
-        };
-        int j = 0, piece = 0;
-        int64_t v_off = -2;
-        bool have = false, more = walk.next(p);
-        int t = p.t0;
-        Place nx = more ? fetch(p.it, t) : Place{-2, false};
-        while (ok && more) {
-            const Place f = nx;
-            if (t == p.t0) load_q(p.it, piece++);
-            const uint32_t bad = __ballot_sync(0xffffffffu, f.bad);
-            if (lane == 0) s.bad[j & 7][lw] = bad;
-            // the next tile's pages, on their way meanwhile
-            if (++t == p.t1) {
-                more = walk.next(p);
-                t = p.t0;
-            }
-            if (more) nx = fetch(p.it, t);
-            if (ok) issue(a.k, f.off < 0 ? -2 : f.off);
-            if (ok && have) issue(a.v, v_off);
-            v_off = f.off;
-            have = true;
-            j++;
-        }
-        if (ok && have) issue(a.v, v_off);
-        cp_wait<0>();
-        if (ok) tell(stage);
-    } else if (lane == 0) {
-        // ------------------------------------------------------------ products
-        const uint32_t ring_s = smem_u32(ring), q_s = smem_u32(q_sm);
-        const int ks = (hd + 15) / 16, n_v = ks * 16;
-        int stage = 0, j = 0, piece = 0, was = 0;  // was: positions of the tile before, in 16s
-        bool ok = true;
-        auto values = [&](int jj) {  // T = P V of tile jj
-            ok = ok && shared_wait(&s.p_full[jj & 1], (jj >> 1) & 1, dead);
-            ok = ok && shared_wait(&s.full[stage % NS], (stage / NS) & 1, dead);
-            if (jj >= NT) ok = ok && shared_wait(&s.t_empty[jj % NT], (jj / NT - 1) & 1, dead);
-            if (!ok) return;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t v = ring_s + (stage % NS) * TM::kTileBytes, id = idesc<C>(n_v, true);
-            const uint32_t pc = tmem + (jj & 1) * TM::kSCols, tc = tmem + 2 * TM::kSCols + (jj % NT) * HD;
-            uint32_t acc = 0;
-#pragma unroll
-            for (int x = PT - 1; x >= 0; x--)  // (small terms first)
-                for (int k = 0; k < was; k++) {
-                    const uint32_t col = PT == 1 ? 8 * k : x == 2 ? 128 + 8 * k : 32 * (k >> 1) + 16 * x + 8 * (k & 1);
-                    mma_f16_ts(tc, pc + col, v_desc(v + k * 2048), id, acc);
-                    acc = 1;
-                }
-            mma_commit(&s.empty[stage % NS]);
-            mma_commit(&s.t_full[jj % NT]);
-            stage++;
-        };
-        while (ok && walk.next(p)) {
-            const uint32_t q = q_s + (piece % QB) * QT * TM::kTileBytes;
-            for (int t = p.t0; t < p.t1 && ok; t++, j++) {
-                const int n16 = (min(kTile, p.it.hi - (p.it.lo + t * kTile)) + 15) / 16;
-                ok = ok && shared_wait(&s.full[stage % NS], (stage / NS) & 1, dead);
-                if (!ok) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t k_sm = ring_s + (stage % NS) * TM::kTileBytes, id = idesc<C>(16 * n16, false);
-                const uint32_t sc = tmem + (j & 1) * TM::kSCols;
-                uint32_t acc = 0;
-#pragma unroll
-                for (int x = QT - 1; x >= 0; x--)
-                    for (int k = 0; k < ks; k++) {
-                        const uint32_t in = (k >> 2) * (kTile * 128) + (k & 3) * 32;
-                        mma_f16(sc, sw128_desc(q + x * TM::kTileBytes + in), sw128_desc(k_sm + in), id, acc);
-                        acc = 1;
-                    }
-                mma_commit(&s.empty[stage % NS]);
-                mma_commit(&s.s_full[j & 1]);
-                if (t == p.t1 - 1) mma_commit(&s.q_empty[piece % QB]);
+                cp_async_commit();
                 stage++;
-                if (j > 0) values(j - 1);
-                was = n16;
+                if (stage > TM::kAhead) {
+                    cp_wait<TM::kAhead>();
+                    tell(stage - TM::kAhead);
+                }
+            };
+            auto look = [&](const Piece* p, int t) {
+                const int p0 = p->lo + t * kTile;
+                Look f;
+                f.n = min(kTile, p->hi - p0);
+                f.pos = p0 + row0;
+#pragma unroll
+                for (int i = 0; i < RW / 32; i++) {
+                    f.page[i] = -1;
+                    if (row0 + 32 * i < f.n) {
+                        const int pos = f.pos + 32 * i, pg = a.page_shift >= 0 ? pos >> a.page_shift : pos / a.page_size;
+                        f.page[i] = a.table[(int64_t)p->tr * a.table_stride + pg];
+                    }
+                }
+                return f;
+            };
+            int j = 0;
+            Pieces pieces;
+            Place v{};
+            bool have = false;
+            const Piece* p = pieces.next(s);
+            int t = p ? p->t0 : 0;
+            Look nx{};
+            if (p) nx = look(p, t);
+            while (ok && p) {
+                const Look now = nx;
+                // the next tile's pages, on their way meanwhile
+                if (++t == p->t1) {
+                    pieces.done(s);
+                    // (the piece that comes may wait for what is on its way)
+                    if (!__all_sync(0xffffffffu, mbar_try_wait(&s.piece_full[pieces.n % kPieces], (pieces.n / kPieces) & 1))) {
+                        cp_wait<0>();
+                        tell(stage);
+                    }
+                    p = pieces.next(s);
+                    t = p ? p->t0 : 0;
+                }
+                if (p) nx = look(p, t);
+                Place f;
+#pragma unroll
+                for (int i = 0; i < RW / 32; i++) {
+                    const int r = row0 + 32 * i, pos = now.pos + 32 * i;
+                    f.off[i] = r < ((now.n + 15) & ~15) ? -1 : -2;
+                    const bool in = r < now.n, there = in && (unsigned)now.page[i] < (unsigned)a.n_pages;
+                    if (there) {
+                        const int pg = a.page_shift >= 0 ? pos >> a.page_shift : pos / a.page_size;
+                        f.off[i] = now.page[i] * a.page_stride + (int64_t)(pos - pg * a.page_size) * a.pos_stride;
+                    }
+                    const uint32_t bad = __ballot_sync(0xffffffffu, in && !there);
+                    if (lane == 0) s.bad[j & 7][lw * (RW / 32) + i] = bad;
+                }
+                issue(a.k, f, false);
+                if (ok && have) issue(a.v, v, true);
+                v = f;
+                have = true;
+                j++;
             }
-            piece++;
+            if (ok && have) issue(a.v, v, true);
+            cp_wait<0>();
+            if (ok) tell(stage);
+        } else if (warp == kQWarp) {
+            // -------------------------------------------------------- pieces and Q
+            const Line line = *a.line;
+            const bool work = line.units > 0 && share < line.shares;
+            long long u = 0, left = 0;  // the unit that comes next, units of this share that are left
+            int next = 0;
+            Item ahead{};
+            auto load = [&]() {
+                if (next < line.items) {
+                    const int4* from = reinterpret_cast<const int4*>(a.item + next);
+                    reinterpret_cast<int4*>(&ahead)[0] = from[0];
+                    reinterpret_cast<int4*>(&ahead)[1] = from[1];
+                }
+            };
+            if (work) {
+                u = mul_div(share, line.units, line.shares);
+                left = mul_div(share + 1, line.units, line.shares) - u;
+                next = a.first[share];
+                load();
+            }
+            bool ok = true;
+            // lays out piece n; false: there is none
+            auto plan = [&](int n) {
+                const int slot = n % kPieces;
+                if (n >= kPieces) ok = ok && warp_wait(&s.piece_empty[slot], (n / kPieces - 1) & 1, dead);
+                if (!ok) return false;
+                Piece p{};
+                p.kind = kPieceLast;
+                int limit = 0;
+                while (left > 0 && next < line.items) {
+                    const Item it = ahead;
+                    next++;
+                    load();
+                    const int tiles = tiles_of(it), x = (int)(u - it.u0), take = (int)min((long long)(tiles + kItemUnits - x), left);
+                    left -= take;
+                    u += take;
+                    p.t0 = max(0, x - kItemUnits);
+                    p.t1 = max(0, x + take - kItemUnits);
+                    if (p.t1 == p.t0) continue;
+                    p.row0 = it.row0;
+                    p.rows = it.rows;
+                    p.lo = it.lo;
+                    p.hi = it.hi;
+                    p.tr = it.tr;
+                    limit = it.limit;
+                    p.kind = (p.t0 == 0 ? kPieceStart : 0) | (p.t0 == 0 && p.t1 == tiles ? kPieceWhole : 0) |
+                             (it.limit == kNoLimit ? kPieceOwn : 0);
+                    break;
+                }
+                if (!(p.kind & kPieceLast)) {
+#pragma unroll
+                    for (int i = 0; i < kTile / 32; i++) {
+                        const int m = 32 * i + lane, rr = m / a.hb;
+                        int4 w = make_int4(0, 0, 0, 0);
+                        if (rr < p.rows && m - rr * a.hb < hn) {
+                            const int4 r = a.row[p.row0 + rr];
+                            const bool all = (p.kind & kPieceOwn ? r.z : r.w) < 0;
+                            w = make_int4(max(r.x, p.lo), min(r.y, limit), r.y, all ? 3 : 1);
+                        }
+                        s.row[slot][m] = w;
+                    }
+                }
+                if (lane == 0) s.piece[slot] = p;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s.piece_full[slot]);
+                return !(p.kind & kPieceLast);
+            };
+            constexpr int LN = HD / 4, RS = 32 / LN;  // lanes of a row, rows of a step
+            const int d = 4 * (lane % LN), rs = lane / LN;
+            auto bring = [&](int n) {  // Q of piece n
+                if (n >= QB) ok = ok && warp_wait(&s.q_empty[n % QB], (n / QB - 1) & 1, dead);
+                if (!ok) return;
+                const int slot = n % kPieces, row0 = s.piece[slot].row0, count = s.piece[slot].rows * a.hb;
+                uint8_t* to = q_sm + (n % QB) * QT * TM::kTileBytes;
+                const T* q = static_cast<const T*>(a.q) + (int64_t)row0 * a.q_stride + (int64_t)head0 * hd + d;
+                constexpr int U = 4;  // steps at once
+                for (int m0 = 0; m0 < count; m0 += U * RS) {
+                    float4 x[U];
+#pragma unroll
+                    for (int i = 0; i < U; i++) {
+                        const int m = m0 + i * RS + rs, qr = m / a.hb, hh = m - qr * a.hb;
+                        x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (m < count && hh < hn && d < hd) x[i] = load4(q + qr * a.q_stride + (int64_t)hh * hd, a.q_wide);
+                    }
+#pragma unroll
+                    for (int i = 0; i < U; i++) {
+                        const int m = m0 + i * RS + rs;
+                        if (QT > 1) {  // the row's largest element to [2^10, 2^11)
+                            float mx = fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
+#pragma unroll
+                            for (int o = LN / 2; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                            // (the exponent field is enough: subnormal rows count as 2^-127; down to
+                            // -117 for the largest finite row, so that both factors stay normal)
+                            const int e = mx < INFINITY ? min(100, 137 - (int)(__float_as_uint(mx) >> 23)) : 0;
+                            const float up = __int_as_float((127 + e) << 23), f = a.scale * __int_as_float((127 - e) << 23);
+                            if (d == 0 && m < count) s.factor[slot][m] = a.softcap > 0.0f ? f / a.softcap : f * kLog2e;
+                            x[i] = make_float4(x[i].x * up, x[i].y * up, x[i].z * up, x[i].w * up);
+                        }
+                        uint32_t w0[QT], w1[QT];
+                        split_terms<C, QT>(x[i].x, x[i].y, w0);
+                        split_terms<C, QT>(x[i].z, x[i].w, w1);
+                        if (m < count && d < hd) {
+                            uint8_t* at = to + m * 128 + (d >> 6) * (kTile * 128) + ((((d & 63) >> 3) ^ (m & 7)) << 4) + (d & 4) * 2;
+#pragma unroll
+                            for (int k = 0; k < QT; k++) *reinterpret_cast<uint2*>(at + k * TM::kTileBytes) = make_uint2(w0[k], w1[k]);
+                        }
+                    }
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s.q_full[n % QB]);
+            };
+            bool more = plan(0);
+            for (int n = 0; ok && more; n++) {
+                more = plan(n + 1);
+                if (ok) bring(n);
+            }
+        } else {
+            // -------------------------------------------------------- products
+            const uint32_t ring_s = smem_u32(ring), q_s = smem_u32(q_sm);
+            const int ks = (hd + 15) / 16, n_v = ks * 16;
+            const uint32_t id_v = idesc<C>(n_v, true);
+            int stage = 0, j = 0, was = 0;  // was: positions of the tile before, in 16s
+            bool ok = true;
+            auto values = [&](int jj) {  // T = P V of tile jj
+                ok = ok && warp_wait(&s.p_full[jj & 1], (jj >> 1) & 1, dead);
+                ok = ok && warp_wait(&s.full[stage % NS], (stage / NS) & 1, dead);
+                if (jj >= NT) ok = ok && warp_wait(&s.t_empty[jj % NT], (jj / NT - 1) & 1, dead);
+                if (!ok) return;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (elected()) {
+                    const uint64_t v = v_desc(ring_s + (stage % NS) * TM::kTileBytes);
+                    const uint32_t pc = tmem + (jj & 1) * TM::kSCols, tc = tmem + 2 * TM::kSCols + (jj % NT) * HD;
+                    uint32_t acc = 0;
+#pragma unroll
+                    for (int x = PT - 1; x >= 0; x--)  // (small terms first)
+#pragma unroll
+                        for (int k = 0; k < kTile / 16; k++) {
+                            if (k >= was) continue;
+                            const uint32_t col = PT == 1 ? 8 * k : x == 2 ? 128 + 8 * k : 32 * (k >> 1) + 16 * x + 8 * (k & 1);
+                            mma_f16_ts(tc, pc + col, v + k * (2048 >> 4), id_v, acc);
+                            acc = 1;
+                        }
+                    mma_commit(&s.empty[stage % NS]);
+                    mma_commit(&s.t_full[jj % NT]);
+                }
+                __syncwarp();
+                stage++;
+            };
+            Pieces pieces;
+            while (const Piece* p = pieces.next(s)) {
+                const int n = pieces.n - 1, lo = p->lo, hi = p->hi, t0 = p->t0, t1 = p->t1;
+                pieces.done(s);
+                const uint64_t q = sw128_desc(q_s + (n % QB) * QT * TM::kTileBytes);
+                ok = ok && warp_wait(&s.q_full[n % QB], (n / QB) & 1, dead);
+                for (int t = t0; t < t1 && ok; t++, j++) {
+                    const int n16 = (min(kTile, hi - (lo + t * kTile)) + 15) / 16;
+                    ok = ok && warp_wait(&s.full[stage % NS], (stage / NS) & 1, dead);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (elected()) {
+                        const uint64_t k_sm = sw128_desc(ring_s + (stage % NS) * TM::kTileBytes);
+                        const uint32_t sc = tmem + (j & 1) * TM::kSCols, id = idesc<C>(16 * n16, false);
+                        uint32_t acc = 0;
+#pragma unroll
+                        for (int x = QT - 1; x >= 0; x--)
+#pragma unroll
+                            for (int k = 0; k < HD / 16; k++) {
+                                if (k >= ks) continue;
+                                const uint32_t in = ((k >> 2) * (kTile * 128) + (k & 3) * 32) >> 4;
+                                mma_f16(sc, q + x * (TM::kTileBytes >> 4) + in, k_sm + in, id, acc);
+                                acc = 1;
+                            }
+                        mma_commit(&s.empty[stage % NS]);
+                        mma_commit(&s.s_full[j & 1]);
+                        if (t == t1 - 1) mma_commit(&s.q_empty[n % QB]);
+                    }
+                    __syncwarp();
+                    stage++;
+                    if (j > 0) values(j - 1);
+                    was = n16;
+                }
+                if (!ok) break;
+            }
+            if (ok && j > 0) values(j - 1);
         }
-        if (ok && j > 0) values(j - 1);
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (warp == 20) {
+    if (warp == kMmaWarp) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
