@@ -19,14 +19,15 @@
 // follows the lengths that it finds.  A first launch of one CTA lays the line.
 //
 // One CTA an SM, its roles warp by warp:
-//   16-17  K and V rows by cp.async into a ring of tiles in the 128-byte swizzle
-//          that the products read (pages may have any size)
-//   18     the share's pieces of the items, laid out ahead for the others, and Q
-//   19     tcgen05.mma, one thread: S = Q K^T of tile j + 1, then T = P V of tile
+//   12-13  K and V rows into a ring of tiles in the 128-byte swizzle that the
+//          products read: by TMA where pages are multiples of 8 positions, by
+//          cp.async row by row elsewhere and at the ends of what is seen
+//   14     the share's pieces of the items, laid out ahead for the others, and Q
+//   15     tcgen05.mma, one thread: S = Q K^T of tile j + 1, then T = P V of tile
 //          j, P being read from tensor memory
 //   0-7    two warpgroups taking tiles in turn: S out of tensor memory, a row to
 //          a thread, the exponentials, P back over S
-//   8-15   O: T out of tensor memory, added in fp32 (the tensor cores' own
+//   8-11   O: T out of tensor memory, added in fp32 (the tensor cores' own
 //          accumulation cuts instead of rounding, which over a long row pulls
 //          towards zero); at an item's end the result or the piece
 //
@@ -38,6 +39,7 @@
 // A value that one row of an item sees and another does not meets a weight of 0
 // there, and 0 times infinity or NaN is NaN: a row whose result is not finite is
 // computed again by the joining launch, alone, from its own positions.
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -47,6 +49,7 @@
 #include "dev.cuh"
 #include "paged.h"
 #include "tcgen05.cuh"
+#include "tensor_map.h"
 
 namespace b2 {
 namespace {
@@ -84,6 +87,7 @@ struct SharedArgs {
     int hb, blocks, rows;  // query heads of an item, such blocks of a group of heads, rows of an item
     int shares;            // at most
     int q_wide, out_wide;  // 16-byte accesses
+    int box;               // positions of a box of the tensor maps (16 or 8); 0: pages that they cannot tell
     float scale, softcap;
     // scratch
     Line* line;
@@ -95,7 +99,9 @@ struct SharedArgs {
     float* part;   // [CTAs][2][128][hd + 4] pieces of items that were cut
 };
 
-__device__ __forceinline__ int tiles_of(const Item& it) { return (it.hi - it.lo + kTile - 1) / kTile; }
+// tiles start on multiples of 16 positions
+__device__ __forceinline__ int base_of(const Item& it) { return it.lo & ~15; }
+__device__ __forceinline__ int tiles_of(const Item& it) { return (it.hi - base_of(it) + kTile - 1) / kTile; }
 
 // The last i of a[0 .. n) (ascending, a[0] <= x) with a[i] <= x.
 template <typename F>
@@ -244,27 +250,29 @@ __global__ void __launch_bounds__(kPlanThreads) shared_line_kernel(const __grid_
 // the products
 // ---------------------------------------------------------------------------
 
-constexpr int kSoftWarps = 8, kSumWarps = 8;  // then two warps that copy, one that plans and brings Q, one that multiplies
+constexpr int kSoftWarps = 8, kSumWarps = 4;  // then two warps that copy, one that plans and brings Q, one that multiplies
 constexpr int kCopyWarp = kSoftWarps + kSumWarps, kCopyWarps = 2, kQWarp = kCopyWarp + kCopyWarps, kMmaWarp = kQWarp + 1;
 constexpr int kSharedThreads = 32 * (kMmaWarp + 1);
 constexpr int kSharedSmemMax = 232448;
 constexpr int kPieces = 4;  // pieces known ahead
-// registers of a thread: 96 at the launch, of which the last four warps give some to O's
-constexpr int kSumRegs = 112, kLastRegs = 64;
-static_assert(kSharedThreads == 640 && 256 * 96 + 256 * kSumRegs + 128 * kLastRegs <= 640 * 96, "register split");
+constexpr int kGroup = 16;  // positions that one step of the products takes; tiles start on multiples
+// registers of a thread: 128 at the launch, of which the last four warps give some to O's
+constexpr int kSumRegs = 184, kLastRegs = 72;
+static_assert(kSharedThreads == 512 && 256 * 128 + 128 * kSumRegs + 128 * kLastRegs <= 512 * 128, "register split");
 
 template <int HD, int QT, int PT>
 struct Tm {
     static constexpr int kTileBytes = kTile * HD * 2;  // K or V rows of a tile, and one term of Q
     static constexpr int kQBufs = QT == 1 ? 2 : 1;
     static constexpr int kQ = kQBufs * QT * kTileBytes;
+    static constexpr int kRaw = QT == 1 ? 0 : 16384;  // fp32 rows of Q on their way
     static constexpr int kFixed = 1024 + 17408;  // alignment, then barriers and small tables
-    static constexpr int kFit = (kSharedSmemMax - kFixed - kQ) / kTileBytes;
+    static constexpr int kFit = (kSharedSmemMax - kFixed - kQ - kRaw) / kTileBytes;
     static constexpr int kStages = kFit > 8 ? 8 : kFit;
     // copies that a copying thread leaves in flight behind the one it has just issued
     static constexpr int kAhead = kStages > 4 ? 4 : kStages - 2;
     static_assert(kStages >= 3, "three tiles must fit");
-    static constexpr int kTotal = kFixed + kQ + kStages * kTileBytes;
+    static constexpr int kTotal = kFixed + kQ + kRaw + kStages * kTileBytes;
     // tensor memory: two S (P over it, a third term behind it), then T
     static constexpr int kSCols = PT == 3 ? 192 : 128;
     static constexpr int kTBufs = 2 * kSCols + 2 * HD <= 512 ? 2 : 1;
@@ -275,6 +283,7 @@ struct Tm {
 struct Piece {
     int row0, rows, lo, hi, tr, t0, t1;
     int kind;  // of the bits below
+    __device__ __forceinline__ int start(int t) const { return (lo & ~15) + t * kTile; }
 };
 constexpr int kPieceStart = 1, kPieceWhole = 2, kPieceOwn = 4, kPieceLast = 8;  // kPieceLast: no piece, the share is done
 
@@ -336,7 +345,9 @@ __device__ __forceinline__ uint32_t idesc(int n, bool v) {
     return (1u << 4) | (type << 7) | (type << 10) | ((v ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
 }
 
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+// 32 columns of this thread's lane, on their way until tmem_wait of the same
+// registers.
+__device__ __forceinline__ void tmem_get32(uint32_t taddr, uint32_t* r) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
         "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
@@ -345,8 +356,51 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
           "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
           "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void tmem_get16(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+        "[%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+// (the registers pass through, so that nothing reads them before)
+__device__ __forceinline__ void tmem_wait16(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+}
+__device__ __forceinline__ void tmem_wait32(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+                   "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                   "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+}
+
+// 16 bytes from global to shared memory where `go`; `valid` false: zeros.  No
+// branch, so that a run of them is issued back to back.
+__device__ __forceinline__ void cp16_if(uint32_t smem, const void* gmem, bool valid, bool go) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %3, 0;\n\t"
+        "@p cp.async.cg.shared.global [%0], [%1], 16, %2;\n\t}" ::"r"(smem),
+        "l"(gmem), "r"(valid ? 16 : 0), "r"((uint32_t)go)
+        : "memory");
+}
+
+// A box of a cache's tensor map to shared memory: 64 dimensions from x on, one
+// head, kGroup or 8 positions from pos on, one page.
+__device__ __forceinline__ void tma_rows(uint32_t smem, const CUtensorMap* map, int x, int head, int pos, int page, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::
+            "r"(smem),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(pos), "r"(page), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// tanh(x) = 1 - 2 / (1 + e^2x): off by about 2^-23, absolute
+__device__ __forceinline__ float tanh_of(float x) { return 1.0f - __fdividef(2.0f, 1.0f + ex2(x * (2.0f * kLog2e))); }
 
 // One lane of a converged warp, chosen so that the compiler knows of it: the
 // products' descriptors live in the warp's uniform registers.  (With lane == 0
@@ -394,14 +448,17 @@ struct Pieces {
 };
 
 template <int HD, typename T, typename C, int QT, int PT>
-__global__ void __launch_bounds__(kSharedThreads, 1) shared_tiles_kernel(const __grid_constant__ SharedArgs a) {
+__global__ void __launch_bounds__(kSharedThreads, 1)
+    shared_tiles_kernel(const __grid_constant__ SharedArgs a, const __grid_constant__ CUtensorMap map_k,
+                        const __grid_constant__ CUtensorMap map_v) {
     using TM = Tm<HD, QT, PT>;
     constexpr int NS = TM::kStages, NT = TM::kTBufs, QB = TM::kQBufs;
     extern __shared__ __align__(1024) uint8_t ssm_raw[];
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ssm_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* const q_sm = base;
     uint8_t* const ring = base + TM::kQ;
-    SmallShared& s = *reinterpret_cast<SmallShared*>(ring + NS * TM::kTileBytes);
+    uint8_t* const raw = ring + NS * TM::kTileBytes;
+    SmallShared& s = *reinterpret_cast<SmallShared*>(raw + TM::kRaw);
     volatile int* dead = &s.dead;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -462,7 +519,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_tiles_kernel(const _
         while (const Piece* p = pieces.next(s)) {
             const int slot = (pieces.n - 1) % kPieces;
             const int4 row = s.row[slot][m];
-            const int it_lo = p->lo, it_hi = p->hi, t1 = p->t1;
+            const int start = p->start(0), it_hi = p->hi, t1 = p->t1;
             const bool busy = __any_sync(0xffffffffu, row.w != 0);
             bool ok = true;
             for (int t = p->t0; t < t1; t++, j++) {
@@ -473,63 +530,66 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_tiles_kernel(const _
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if (busy) {
-                    const int p0 = it_lo + t * kTile, c0 = row.x - p0, c1 = row.y - p0;
+                    const int p0 = start + t * kTile, c0 = row.x - p0, c1 = row.y - p0;
                     const int chunks = (min(kTile, it_hi - p0) + 31) / 32;
                     const bool mask = __any_sync(0xffffffffu, c0 > 0 || c1 < 32 * chunks);
                     float f = QT == 1 ? (cap > 0.0f ? a.scale / cap : a.scale * kLog2e) : s.factor[slot][m];
-                    float mx = -INFINITY;
+                    if (mask || !plain) {  // the scores that are not seen to -inf; cap and slope
 #pragma unroll 1
-                    for (int ch = 0; ch < chunks; ch++) {
-                        uint32_t r[32];
-                        tmem_ld32(s_col + 32 * ch, r);
-                        if (!plain) {
+                        for (int c = 0; c < 32 * chunks; c += 16) {
+                            uint32_t r[16];
+                            tmem_ld16(s_col + c, r);
+                            const float p1 = (float)(p0 + c - (row.z - 1));
 #pragma unroll
-                            for (int i = 0; i < 32; i++) {
-                                float x = __uint_as_float(r[i]) * f;
-                                if (cap > 0.0f) x = (cap * kLog2e) * tanhf(x);
-                                x = fmaf(slope, (float)(p0 + 32 * ch + i - (row.z - 1)), x);
-                                r[i] = __float_as_uint(x);
+                            for (int i = 0; i < 16; i++) {
+                                float x = __uint_as_float(r[i]);
+                                if (!plain) {
+                                    x *= f;
+                                    if (cap > 0.0f) x = (cap * kLog2e) * tanh_of(x);
+                                    x = fmaf(slope, p1 + (float)i, x);
+                                }
+                                r[i] = c + i < c0 || c + i >= c1 ? 0xff800000u : __float_as_uint(x);
                             }
+                            tmem_st16(s_col + c, r);
                         }
-                        if (mask) {
-#pragma unroll
-                            for (int i = 0; i < 32; i++)
-                                if (32 * ch + i < c0 || 32 * ch + i >= c1) r[i] = __float_as_uint(-INFINITY);
-                        }
-                        if (!plain) {
-                            tmem_st16(s_col + 32 * ch, r);
-                            tmem_st16(s_col + 32 * ch + 16, r + 16);
-                        }
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                        if (!plain) f = 1.0f;
+                    }
+                    // 32 columns on their way while 32 are worked on
+                    uint32_t ra[32], rb[32];
+                    float mx = -INFINITY;
+                    auto largest = [&](const uint32_t* r) {
                         float x0 = mx, x1 = -INFINITY;
 #pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            x0 = fmaxf(x0, __uint_as_float(r[i]));
-                            x1 = fmaxf(x1, __uint_as_float(r[i + 1]));
+                        for (int i = 0; i < 32; i += 4) {
+                            x0 = fmaxf(fmaxf(x0, __uint_as_float(r[i])), __uint_as_float(r[i + 1]));
+                            x1 = fmaxf(fmaxf(x1, __uint_as_float(r[i + 2])), __uint_as_float(r[i + 3]));
                         }
                         mx = fmaxf(x0, x1);
-                    }
-                    if (!plain) {
-                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                        f = 1.0f;
-                    }
-                    const float top = mx == -INFINITY ? -INFINITY : mx * f, z = (top == -INFINITY ? 0.0f : top) - 14.0f;
-                    float l0 = 0.0f, l1 = 0.0f;
+                    };
+                    tmem_get32(s_col, ra);
 #pragma unroll 1
-                    for (int ch = 0; ch < chunks; ch++) {
-                        uint32_t r[32];
-                        tmem_ld32(s_col + 32 * ch, r);
-                        if (mask && plain) {
-#pragma unroll
-                            for (int i = 0; i < 32; i++)
-                                if (32 * ch + i < c0 || 32 * ch + i >= c1) r[i] = __float_as_uint(-INFINITY);
+                    for (int ch = 0; ch < chunks; ch += 2) {
+                        tmem_wait32(ra);
+                        if (ch + 1 < chunks) tmem_get32(s_col + 32 * ch + 32, rb);
+                        largest(ra);
+                        if (ch + 1 < chunks) {
+                            tmem_wait32(rb);
+                            if (ch + 2 < chunks) tmem_get32(s_col + 32 * ch + 64, ra);
+                            largest(rb);
                         }
+                    }
+                    tmem_get32(s_col, ra);
+                    const float top = mx == -INFINITY ? -INFINITY : mx * f, z = 14.0f - (top == -INFINITY ? 0.0f : top);
+                    const unsigned long long f2 = f2_pack(f, f), z2 = f2_pack(z, z);
+                    unsigned long long l2 = 0;
+                    auto weigh = [&](const uint32_t* r, int ch) {
                         uint32_t w[PT][16];
 #pragma unroll
                         for (int i = 0; i < 16; i++) {
-                            const float e0 = ex2(fmaf(__uint_as_float(r[2 * i]), f, -z));
-                            const float e1 = ex2(fmaf(__uint_as_float(r[2 * i + 1]), f, -z));
-                            l0 += e0;
-                            l1 += e1;
+                            const float2 d = f2_unpack(f2_fma(f2_pack(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), f2, z2));
+                            const float e0 = ex2(d.x), e1 = ex2(d.y);
+                            l2 = f2_add(l2, f2_pack(e0, e1));
                             uint32_t x[PT];
                             split_terms<C, PT>(e0, e1, x);
 #pragma unroll
@@ -542,8 +602,20 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_tiles_kernel(const _
                             tmem_st16(s_col + 32 * ch + 16, w[PT > 1 ? 1 : 0]);
                             if (PT == 3) tmem_st16(s_col + 128 + 16 * ch, w[PT - 1]);
                         }
+                    };
+#pragma unroll 1
+                    for (int ch = 0; ch < chunks; ch += 2) {
+                        tmem_wait32(ra);
+                        if (ch + 1 < chunks) tmem_get32(s_col + 32 * ch + 32, rb);
+                        weigh(ra, ch);
+                        if (ch + 1 < chunks) {
+                            tmem_wait32(rb);
+                            if (ch + 2 < chunks) tmem_get32(s_col + 32 * ch + 64, ra);
+                            weigh(rb, ch + 1);
+                        }
                     }
-                    float l = l0 + l1;
+                    const float2 ls = f2_unpack(l2);
+                    float l = ls.x + ls.y;
                     const uint32_t* bad = s.bad[j & 7];
                     if (bad[0] | bad[1] | bad[2] | bad[3]) {
                         for (int c = max(c0, 0); c < min(c1, kTile); c++)
@@ -562,21 +634,19 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_tiles_kernel(const _
     } else if (warp < kSoftWarps + kSumWarps) {
         // ------------------------------------------------------------ O
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
-        constexpr int HC = HD / 2;  // columns of a warp
-        const int half = (warp - kSoftWarps) >> 2, quad = warp & 3, m = quad * 32 + lane;
-        const uint32_t t_col = tmem + ((uint32_t)(quad * 32) << 16) + 2 * TM::kSCols + half * HC;
+        const int quad = warp & 3, m = quad * 32 + lane;
+        const uint32_t t_col = tmem + ((uint32_t)(quad * 32) << 16) + 2 * TM::kSCols;
         const int rr = m / a.hb, head = head0 + m - rr * a.hb;
-        const int d0 = half * HC, dn = min(HC, hd - d0);  // this warp's dimensions
         int j = 0;
         bool ok = true;
         Pieces pieces;
         while (const Piece* p = pieces.next(s)) {
             const int4 row = s.row[(pieces.n - 1) % kPieces][m];
             const bool busy = __any_sync(0xffffffffu, row.w != 0);
-            unsigned long long o[HC / 2];
+            unsigned long long o[HD / 2];
             float M = -INFINITY, L = 0.0f;
 #pragma unroll
-            for (int i = 0; i < HC / 2; i++) o[i] = 0;
+            for (int i = 0; i < HD / 2; i++) o[i] = 0;
             const int t1 = p->t1;
 #pragma unroll 1
             for (int t = p->t0; t < t1; t++, j++) {
@@ -591,15 +661,24 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_tiles_kernel(const _
                     M = n;
                     L = fmaf(L, fo, st.y * ft);
                     const unsigned long long fo2 = f2_pack(fo, fo), ft2 = f2_pack(ft, ft);
-#pragma unroll
-                    for (int c = 0; c < HC; c += 16) {
-                        uint32_t r[16];
-                        tmem_ld16(t_col + buf * HD + c, r);
+                    uint32_t ra[16], rb[16];
+                    auto add = [&](const uint32_t* r, int c) {
 #pragma unroll
                         for (int i = 0; i < 8; i++) {
                             const unsigned long long x = f2_pack(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
                             o[c / 2 + i] = f2_fma(o[c / 2 + i], fo2, f2_mul(x, ft2));
                         }
+                    };
+                    const uint32_t from = t_col + buf * HD;
+                    tmem_get16(from, ra);
+#pragma unroll
+                    for (int c = 0; c < HD; c += 32) {
+                        tmem_wait16(ra);
+                        tmem_get16(from + c + 16, rb);
+                        add(ra, c);
+                        tmem_wait16(rb);
+                        if (c + 32 < HD) tmem_get16(from + c + 32, ra);
+                        add(rb, c + 16);
                     }
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -609,14 +688,14 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_tiles_kernel(const _
             if (!ok) L = __int_as_float(0x7fc00000);  // (a wait gave up: no result)
             const int b = p->row0 + rr, kind = p->kind;
             pieces.done(s);
-            if (!row.w || dn <= 0) continue;
+            if (!row.w) continue;
             if ((kind & kPieceWhole) && (row.w & 2)) {  // all that the row sees
                 const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-                T* out = static_cast<T*>(a.out) + (int64_t)b * a.out_stride + (int64_t)head * hd + d0;
+                T* out = static_cast<T*>(a.out) + (int64_t)b * a.out_stride + (int64_t)head * hd;
                 bool odd = false;  // not finite
 #pragma unroll
-                for (int i = 0; i < HC / 8; i++) {
-                    if (8 * i >= dn) break;
+                for (int i = 0; i < HD / 8; i++) {
+                    if (8 * i >= hd) break;
                     alignas(16) T y[8];
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
@@ -635,7 +714,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_tiles_kernel(const _
                         for (int k = 0; k < 8; k++) out[8 * i + k] = y[k];
                     }
                 }
-                if (a.lse && half == 0) a.lse[(int64_t)b * a.nh + head] = L == 0.0f ? -INFINITY : (M + (log2f(L) - 14.0f)) * kLn2;
+                if (a.lse) a.lse[(int64_t)b * a.nh + head] = L == 0.0f ? -INFINITY : (M + (log2f(L) - 14.0f)) * kLn2;
                 if (odd) a.redo[b] = 1;
             } else {
                 const int64_t width = hd + 4;
@@ -643,118 +722,221 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_tiles_kernel(const _
                                 ? a.whole + (((int64_t)(kind & kPieceOwn ? 1 : 0) * a.batch + b) * a.nh + head) * width
                                 : a.part + (((int64_t)blockIdx.x * 2 + (kind & kPieceStart ? 1 : 0)) * kTile + m) * width;
 #pragma unroll
-                for (int i = 0; i < HC / 4; i++) {
-                    if (4 * i >= dn) break;
+                for (int i = 0; i < HD / 4; i++) {
+                    if (4 * i >= hd) break;
                     const float2 x = f2_unpack(o[2 * i]), y = f2_unpack(o[2 * i + 1]);
-                    *reinterpret_cast<float4*>(to + d0 + 4 * i) = make_float4(x.x, x.y, y.x, y.y);
+                    *reinterpret_cast<float4*>(to + 4 * i) = make_float4(x.x, x.y, y.x, y.y);
                 }
-                if (half == 0) *reinterpret_cast<float2*>(to + hd) = make_float2(M, L);
+                *reinterpret_cast<float2*>(to + hd) = make_float2(M, L);
             }
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLastRegs));
         if (warp < kQWarp) {
             // -------------------------------------------------------- K and V
-            constexpr int RW = kTile / kCopyWarps;  // rows of a warp
-            const int lw = warp - kCopyWarp, row0 = lw * RW + lane;
-            constexpr int CH = HD / 8, LR = 32 / CH;  // chunks of a row, rows of a warp's copy
-            const int hc = hd / 8, c = lane % CH, r0 = lane / CH;
-            const uint32_t at0 = smem_u32(ring) + (c >> 3) * (kTile * 128) + (lw * RW + r0) * 128;
-            const int64_t h_off = (int64_t)h * a.head_stride + c * 8;
-            int stage = 0, told = 0;  // stages issued, and those that the products know of
-            bool ok = true;
-            auto tell = [&](int upto) {  // the stages before `upto` have landed
-                fence_proxy_async();
-                __syncwarp();
-                for (; told < upto; told++)
-                    if (lane == 0) mbar_arrive(&s.full[told % NS]);
-            };
-            // the places of this lane's rows of a tile: their offset; -1: none there; -2: nor needed
-            struct Place {
-                int64_t off[RW / 32];
-            };
-            struct Look {  // looked up, not yet used
-                int page[RW / 32], pos, n;
-            };
-            // rows with off >= 0 are copied, with off == -1 set to zero, others left
-            auto issue = [&](const uint16_t* src, const Place& f, bool zero) {
-                const int slot = stage % NS;
-                if (stage >= NS) ok = ok && warp_wait(&s.empty[slot], (stage / NS - 1) & 1, dead);
-                if (!ok) return;
-                const uint32_t to = at0 + slot * TM::kTileBytes;
-#pragma unroll
-                for (int i = 0; i < RW / LR; i++) {
-                    const int r = i * LR + r0;
-                    const int64_t o = __shfl_sync(0xffffffffu, f.off[i * LR / 32], r & 31);
-                    const uint32_t at = to + i * LR * 128 + (((c & 7) ^ (r & 7)) << 4);  // (lw * RW is a multiple of 8)
-                    if (c < hc && (o >= 0 || (zero && o == -1))) cp16(at, src + (o < 0 ? 0 : o + h_off), o >= 0);
-                }
-                cp_async_commit();
-                stage++;
-                if (stage > TM::kAhead) {
-                    cp_wait<TM::kAhead>();
-                    tell(stage - TM::kAhead);
-                }
-            };
-            auto look = [&](const Piece* p, int t) {
-                const int p0 = p->lo + t * kTile;
-                Look f;
-                f.n = min(kTile, p->hi - p0);
-                f.pos = p0 + row0;
-#pragma unroll
-                for (int i = 0; i < RW / 32; i++) {
-                    f.page[i] = -1;
-                    if (row0 + 32 * i < f.n) {
-                        const int pos = f.pos + 32 * i, pg = a.page_shift >= 0 ? pos >> a.page_shift : pos / a.page_size;
-                        f.page[i] = a.table[(int64_t)p->tr * a.table_stride + pg];
-                    }
-                }
-                return f;
-            };
+            const int lw = warp - kCopyWarp, hc = hd / 8;
+            const uint32_t ring_s = smem_u32(ring);
             int j = 0;
             Pieces pieces;
-            Place v{};
-            bool have = false;
             const Piece* p = pieces.next(s);
             int t = p ? p->t0 : 0;
-            Look nx{};
-            if (p) nx = look(p, t);
-            while (ok && p) {
-                const Look now = nx;
-                // the next tile's pages, on their way meanwhile
-                if (++t == p->t1) {
-                    pieces.done(s);
-                    // (the piece that comes may wait for what is on its way)
-                    if (!__all_sync(0xffffffffu, mbar_try_wait(&s.piece_full[pieces.n % kPieces], (pieces.n / kPieces) & 1))) {
-                        cp_wait<0>();
-                        tell(stage);
-                    }
-                    p = pieces.next(s);
-                    t = p ? p->t0 : 0;
-                }
-                if (p) nx = look(p, t);
-                Place f;
+            bool ok = true, have = false;
+            int stage = 0;
+            auto page_at = [&](const Piece* q, int pos) {
+                const int pg = a.page_shift >= 0 ? pos >> a.page_shift : pos / a.page_size;
+                return a.table[(int64_t)q->tr * a.table_stride + pg];
+            };
+            auto place = [&](int pos) {  // in its page
+                return a.page_shift >= 0 ? pos & (a.page_size - 1) : pos - pos / a.page_size * a.page_size;
+            };
+            auto slot_free = [&]() {
+                if (stage >= NS) ok = ok && warp_wait(&s.empty[stage % NS], (stage / NS - 1) & 1, dead);
+                return ok;
+            };
+            if (a.box) {
+                // Groups of `box` positions that lie in one page: seen whole, a tensor map's
+                // box each, issued by the first warp; in part, or in no page, row by row by
+                // the second.  The products take 16 positions at a time, so rows of V up to
+                // there that nobody sees are zeros.
+                const int G = a.box, groups = kTile / G;
+                struct Tile {
+                    int page, pos, lo, hi, n;  // this lane's group: page, first position; the tile's seen rows, rows to fill
+                };
+                auto look = [&](const Piece* q, int tt) {
+                    Tile f;
+                    const int p0 = q->start(tt);
+                    f.lo = q->lo - p0;
+                    f.hi = min(kTile, q->hi - p0);
+                    f.n = (f.hi + kGroup - 1) & ~(kGroup - 1);
+                    f.pos = p0 + lane * G;
+                    f.page = -1;
+                    // (any position of the group that is seen names its page)
+                    if (lane < groups && lane * G < f.hi && lane * G + G > f.lo) f.page = page_at(q, max(f.pos, q->lo));
+                    return f;
+                };
+                constexpr int BL = HD / 64;  // boxes of a group
+                auto issue = [&](const CUtensorMap* map, const uint16_t* src, const Tile& f, bool value) {
+                    if (!slot_free()) return;
+                    const int slot = stage % NS;
+                    const uint32_t to = ring_s + slot * TM::kTileBytes;
+                    const int r0 = lane * G;
+                    const bool there = (unsigned)f.page < (unsigned)a.n_pages;
+                    const bool whole = lane < groups && there && r0 >= f.lo && r0 + G <= f.hi;
+                    const uint32_t by_box = __ballot_sync(0xffffffffu, whole);
+                    if (lw == 0) {
+                        if (lane == 0) mbar_arrive_expect_tx(&s.full[slot], __popc(by_box) * G * 128 * BL);
+                        __syncwarp();
+                        if (whole) {
+                            const int in = place(f.pos);
 #pragma unroll
-                for (int i = 0; i < RW / 32; i++) {
-                    const int r = row0 + 32 * i, pos = now.pos + 32 * i;
-                    f.off[i] = r < ((now.n + 15) & ~15) ? -1 : -2;
-                    const bool in = r < now.n, there = in && (unsigned)now.page[i] < (unsigned)a.n_pages;
-                    if (there) {
-                        const int pg = a.page_shift >= 0 ? pos >> a.page_shift : pos / a.page_size;
-                        f.off[i] = now.page[i] * a.page_stride + (int64_t)(pos - pg * a.page_size) * a.pos_stride;
+                            for (int x = 0; x < BL; x++)
+                                tma_rows(to + x * (kTile * 128) + r0 * 128, map, 64 * x, h, in, f.page, &s.full[slot]);
+                        }
+                        __syncwarp();
+                    } else {
+                        uint32_t rest = __ballot_sync(0xffffffffu, lane < groups && !whole && r0 < f.n);
+                        while (rest) {
+                            const int g = __ffs(rest) - 1;
+                            rest &= rest - 1;
+                            const int page = __shfl_sync(0xffffffffu, f.page, g), pos = __shfl_sync(0xffffffffu, f.pos, g);
+                            const bool in_pool = (unsigned)page < (unsigned)a.n_pages;
+                            const uint16_t* from = src + (in_pool ? page * a.page_stride + place(pos) * a.pos_stride : 0) + h * a.head_stride;
+#pragma unroll 4
+                            for (int i = lane; i < G * hc; i += 32) {
+                                const int r = i / hc, c = i - r * hc, row = g * G + r;
+                                const bool seen = in_pool && row >= f.lo && row < f.hi;
+                                const uint32_t at = to + (c >> 3) * (kTile * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+                                cp16_if(at, seen ? from + r * a.pos_stride + c * 8 : src, seen, seen || value);
+                            }
+                        }
+                        cp_async_commit();
+                        cp_wait<0>();
+                        fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&s.full[slot]);
                     }
-                    const uint32_t bad = __ballot_sync(0xffffffffu, in && !there);
-                    if (lane == 0) s.bad[j & 7][lw * (RW / 32) + i] = bad;
+                    stage++;
+                };
+                Tile nx{}, v{};
+                if (p) nx = look(p, t);
+                while (ok && p) {
+                    const Tile f = nx;
+                    if (++t == p->t1) {
+                        pieces.done(s);
+                        p = pieces.next(s);
+                        t = p ? p->t0 : 0;
+                    }
+                    if (p) nx = look(p, t);  // (the next tile's pages, on their way meanwhile)
+                    // positions seen whose page is not there
+                    const int lo = max(f.lo, lane * G), hi = min(f.hi, lane * G + G);
+                    const bool gone = lane < groups && lo < hi && (unsigned)f.page >= (unsigned)a.n_pages;
+                    uint32_t bits[4] = {0, 0, 0, 0};
+                    if (__any_sync(0xffffffffu, gone)) {
+                        const uint32_t mine = gone ? (hi - lo == 32 ? 0xffffffffu : ((1u << (hi - lo)) - 1)) << (lo & 31) : 0;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) bits[i] = __reduce_or_sync(0xffffffffu, (lo >> 5) == i ? mine : 0);
+                    }
+                    if (lw == 0 && lane < 4) s.bad[j & 7][lane] = lane == 0 ? bits[0] : lane == 1 ? bits[1] : lane == 2 ? bits[2] : bits[3];
+                    issue(&map_k, a.k, f, false);
+                    if (ok && have) issue(&map_v, a.v, v, true);
+                    v = f;
+                    have = true;
+                    j++;
                 }
-                issue(a.k, f, false);
+                if (ok && have) issue(&map_v, a.v, v, true);
+            } else {
+                // Pages of any size and place: row by row, half of the tile's rows to a warp.
+                constexpr int RW = kTile / kCopyWarps;
+                constexpr int CH = HD / 8, LR = 32 / CH;  // chunks of a row, rows of a warp's copy
+                const int row0 = lw * RW + lane, c = lane % CH, r0 = lane / CH;
+                const uint32_t at0 = ring_s + (c >> 3) * (kTile * 128) + (lw * RW + r0) * 128;
+                const int64_t h_off = (int64_t)h * a.head_stride + c * 8;
+                int told = 0;               // stages that the products know of
+                auto tell = [&](int upto) {  // the stages before `upto` have landed
+                    fence_proxy_async();
+                    __syncwarp();
+                    for (; told < upto; told++)
+                        if (lane == 0) mbar_arrive(&s.full[told % NS]);
+                };
+                // this lane's rows of a tile: their offset; -1: none there; -2: nor needed
+                struct Place {
+                    int64_t off[RW / 32];
+                };
+                struct Look {  // looked up, not yet used
+                    int page[RW / 32], pos, lo, hi;
+                };
+                auto look = [&](const Piece* q, int tt) {
+                    Look f;
+                    const int p0 = q->start(tt);
+                    f.lo = q->lo - p0;
+                    f.hi = min(kTile, q->hi - p0);
+                    f.pos = p0 + row0;
+#pragma unroll
+                    for (int i = 0; i < RW / 32; i++) {
+                        const int r = row0 + 32 * i;
+                        f.page[i] = r >= f.lo && r < f.hi ? page_at(q, f.pos + 32 * i) : -1;
+                    }
+                    return f;
+                };
+                auto issue = [&](const uint16_t* src, const Place& f, bool value) {
+                    if (!slot_free()) return;
+                    const uint32_t to = at0 + (stage % NS) * TM::kTileBytes;
+                    constexpr int U = 4;  // copies whose places are worked out together
+#pragma unroll
+                    for (int i0 = 0; i0 < RW / LR; i0 += U) {
+                        int64_t o[U];
+#pragma unroll
+                        for (int u = 0; u < U; u++) o[u] = __shfl_sync(0xffffffffu, f.off[(i0 + u) * LR / 32], ((i0 + u) * LR + r0) & 31);
+#pragma unroll
+                        for (int u = 0; u < U; u++) {
+                            const int r = (i0 + u) * LR + r0;
+                            const uint32_t at = to + (i0 + u) * LR * 128 + (((c & 7) ^ (r & 7)) << 4);  // (lw * RW is a multiple of 8)
+                            cp16_if(at, src + (o[u] < 0 ? 0 : o[u] + h_off), o[u] >= 0, c < hc && (o[u] >= 0 || (value && o[u] == -1)));
+                        }
+                    }
+                    cp_async_commit();
+                    stage++;
+                    if (stage > TM::kAhead) {
+                        cp_wait<TM::kAhead>();
+                        tell(stage - TM::kAhead);
+                    }
+                };
+                Place v{};
+                Look nx{};
+                if (p) nx = look(p, t);
+                while (ok && p) {
+                    const Look now = nx;
+                    if (++t == p->t1) {
+                        pieces.done(s);
+                        // (the piece that comes may wait for what is on its way)
+                        if (!__all_sync(0xffffffffu, mbar_try_wait(&s.piece_full[pieces.n % kPieces], (pieces.n / kPieces) & 1))) {
+                            cp_wait<0>();
+                            tell(stage);
+                        }
+                        p = pieces.next(s);
+                        t = p ? p->t0 : 0;
+                    }
+                    if (p) nx = look(p, t);
+                    Place f;
+#pragma unroll
+                    for (int i = 0; i < RW / 32; i++) {
+                        const int r = row0 + 32 * i;
+                        f.off[i] = r < ((now.hi + kGroup - 1) & ~(kGroup - 1)) ? -1 : -2;
+                        const bool in = r >= now.lo && r < now.hi, there = in && (unsigned)now.page[i] < (unsigned)a.n_pages;
+                        if (there) f.off[i] = now.page[i] * a.page_stride + (int64_t)place(now.pos + 32 * i) * a.pos_stride;
+                        const uint32_t bad = __ballot_sync(0xffffffffu, in && !there);
+                        if (lane == 0) s.bad[j & 7][lw * (RW / 32) + i] = bad;
+                    }
+                    issue(a.k, f, false);
+                    if (ok && have) issue(a.v, v, true);
+                    v = f;
+                    have = true;
+                    j++;
+                }
                 if (ok && have) issue(a.v, v, true);
-                v = f;
-                have = true;
-                j++;
+                cp_wait<0>();
+                if (ok) tell(stage);
             }
-            if (ok && have) issue(a.v, v, true);
-            cp_wait<0>();
-            if (ok) tell(stage);
         } else if (warp == kQWarp) {
             // -------------------------------------------------------- pieces and Q
             const Line line = *a.line;
@@ -824,42 +1006,106 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_tiles_kernel(const _
             };
             constexpr int LN = HD / 4, RS = 32 / LN;  // lanes of a row, rows of a step
             const int d = 4 * (lane % LN), rs = lane / LN;
+            // a row of the product, `at` its first 64 dimensions' line: this lane's four elements as terms
+            auto put = [&](uint8_t* to, int slot, int m, float4 x, bool go) {
+                if (QT > 1) {  // the row's largest element to [2^10, 2^11)
+                    float mx = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+#pragma unroll
+                    for (int o = LN / 2; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                    // (the exponent field is enough: subnormal rows count as 2^-127; down to
+                    // -117 for the largest finite row, so that both factors stay normal)
+                    const int e = mx < INFINITY ? min(100, 137 - (int)(__float_as_uint(mx) >> 23)) : 0;
+                    const float up = __int_as_float((127 + e) << 23), f = a.scale * __int_as_float((127 - e) << 23);
+                    if (d == 0 && go) s.factor[slot][m] = a.softcap > 0.0f ? f / a.softcap : f * kLog2e;
+                    x = make_float4(x.x * up, x.y * up, x.z * up, x.w * up);
+                }
+                uint32_t w0[QT], w1[QT];
+                split_terms<C, QT>(x.x, x.y, w0);
+                split_terms<C, QT>(x.z, x.w, w1);
+                if (go) {
+                    uint8_t* at = to + m * 128 + (d >> 6) * (kTile * 128) + ((((d & 63) >> 3) ^ (m & 7)) << 4) + (d & 4) * 2;
+#pragma unroll
+                    for (int k = 0; k < QT; k++) *reinterpret_cast<uint2*>(at + k * TM::kTileBytes) = make_uint2(w0[k], w1[k]);
+                }
+            };
             auto bring = [&](int n) {  // Q of piece n
-                if (n >= QB) ok = ok && warp_wait(&s.q_empty[n % QB], (n / QB - 1) & 1, dead);
-                if (!ok) return;
                 const int slot = n % kPieces, row0 = s.piece[slot].row0, count = s.piece[slot].rows * a.hb;
                 uint8_t* to = q_sm + (n % QB) * QT * TM::kTileBytes;
-                const T* q = static_cast<const T*>(a.q) + (int64_t)row0 * a.q_stride + (int64_t)head0 * hd + d;
-                constexpr int U = 4;  // steps at once
-                for (int m0 = 0; m0 < count; m0 += U * RS) {
-                    float4 x[U];
-#pragma unroll
-                    for (int i = 0; i < U; i++) {
-                        const int m = m0 + i * RS + rs, qr = m / a.hb, hh = m - qr * a.hb;
-                        x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        if (m < count && hh < hn && d < hd) x[i] = load4(q + qr * a.q_stride + (int64_t)hh * hd, a.q_wide);
-                    }
-#pragma unroll
-                    for (int i = 0; i < U; i++) {
-                        const int m = m0 + i * RS + rs;
-                        if (QT > 1) {  // the row's largest element to [2^10, 2^11)
-                            float mx = fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
-#pragma unroll
-                            for (int o = LN / 2; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                            // (the exponent field is enough: subnormal rows count as 2^-127; down to
-                            // -117 for the largest finite row, so that both factors stay normal)
-                            const int e = mx < INFINITY ? min(100, 137 - (int)(__float_as_uint(mx) >> 23)) : 0;
-                            const float up = __int_as_float((127 + e) << 23), f = a.scale * __int_as_float((127 - e) << 23);
-                            if (d == 0 && m < count) s.factor[slot][m] = a.softcap > 0.0f ? f / a.softcap : f * kLog2e;
-                            x[i] = make_float4(x[i].x * up, x[i].y * up, x[i].z * up, x[i].w * up);
+                const T* q = static_cast<const T*>(a.q) + (int64_t)row0 * a.q_stride + (int64_t)head0 * hd;
+                auto free_ = [&]() {
+                    if (n >= QB) ok = ok && warp_wait(&s.q_empty[n % QB], (n / QB - 1) & 1, dead);
+                    return ok;
+                };
+                if (QT == 1 && a.q_wide) {  // as it is: chunks of 8 elements straight to their places
+                    if (!free_()) return;
+                    constexpr int CH = HD / 8, CR = 32 / CH;
+                    const int c = lane % CH;
+                    int m = lane / CH, qr = m / a.hb, hh = m - qr * a.hb;
+#pragma unroll 4
+                    for (int i = 0; i < count; i += CR) {
+                        const bool go = m < count && hh < hn && 8 * c < hd;
+                        const T* from = q + qr * a.q_stride + hh * hd + 8 * c;
+                        cp16_if(smem_u32(to) + m * 128 + (c >> 3) * (kTile * 128) + (((c & 7) ^ (m & 7)) << 4), go ? (const void*)from : a.q,
+                                true, go);
+                        m += CR;
+                        hh += CR;
+                        while (hh >= a.hb) {
+                            hh -= a.hb;
+                            qr++;
                         }
-                        uint32_t w0[QT], w1[QT];
-                        split_terms<C, QT>(x[i].x, x[i].y, w0);
-                        split_terms<C, QT>(x[i].z, x[i].w, w1);
-                        if (m < count && d < hd) {
-                            uint8_t* at = to + m * 128 + (d >> 6) * (kTile * 128) + ((((d & 63) >> 3) ^ (m & 7)) << 4) + (d & 4) * 2;
-#pragma unroll
-                            for (int k = 0; k < QT; k++) *reinterpret_cast<uint2*>(at + k * TM::kTileBytes) = make_uint2(w0[k], w1[k]);
+                    }
+                    cp_async_commit();
+                    cp_wait<0>();
+                } else if (QT > 1 && a.q_wide) {
+                    // fp32 rows pass through two halves of `raw`, a lane's 16 bytes coming back to
+                    // itself, so that a run of them is on its way while one is split
+                    constexpr int U = 16;  // steps of a half
+                    int m = rs, qr = m / a.hb, hh = m - qr * a.hb;
+                    const uint32_t mine = smem_u32(raw) + lane * 16;
+                    auto fetch = [&](int half) {
+#pragma unroll 4
+                        for (int i = 0; i < U; i++) {
+                            const bool go = m < count && hh < hn && d < hd;
+                            const T* from = q + qr * a.q_stride + hh * hd + d;
+                            cp16_if(mine + (half * U + i) * 512, go ? (const void*)from : a.q, go, true);
+                            m += RS;
+                            hh += RS;
+                            while (hh >= a.hb) {
+                                hh -= a.hb;
+                                qr++;
+                            }
+                        }
+                        cp_async_commit();
+                    };
+                    fetch(0);
+                    if (!free_()) {
+                        cp_wait<0>();
+                        return;
+                    }
+                    for (int m0 = 0, half = 0; m0 < count; m0 += U * RS, half ^= 1) {
+                        fetch(half ^ 1);
+                        cp_wait<1>();
+#pragma unroll 2
+                        for (int i = 0; i < U; i++) {
+                            const int mm = m0 + i * RS + rs;
+                            const float4 x = *reinterpret_cast<const float4*>(raw + (half * U + i) * 512 + lane * 16);
+                            put(to, slot, mm, x, mm < count && d < hd);
+                        }
+                    }
+                    cp_wait<0>();
+                } else {  // rows off 16 bytes
+                    if (!free_()) return;
+                    int m = rs, qr = m / a.hb, hh = m - qr * a.hb;
+#pragma unroll 2
+                    for (int i = 0; i < count; i += RS) {
+                        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (m < count && hh < hn && d < hd) x = load4(q + qr * a.q_stride + hh * hd + d, false);
+                        put(to, slot, m, x, m < count && d < hd);
+                        m += RS;
+                        hh += RS;
+                        while (hh >= a.hb) {
+                            hh -= a.hb;
+                            qr++;
                         }
                     }
                 }
@@ -889,13 +1135,12 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_tiles_kernel(const _
                     const uint64_t v = v_desc(ring_s + (stage % NS) * TM::kTileBytes);
                     const uint32_t pc = tmem + (jj & 1) * TM::kSCols, tc = tmem + 2 * TM::kSCols + (jj % NT) * HD;
                     uint32_t acc = 0;
-#pragma unroll
+#pragma unroll 1
                     for (int x = PT - 1; x >= 0; x--)  // (small terms first)
-#pragma unroll
-                        for (int k = 0; k < kTile / 16; k++) {
-                            if (k >= was) continue;
+#pragma unroll 2
+                        for (int k = 0; k < was; k++) {
                             const uint32_t col = PT == 1 ? 8 * k : x == 2 ? 128 + 8 * k : 32 * (k >> 1) + 16 * x + 8 * (k & 1);
-                            mma_f16_ts(tc, pc + col, v + k * (2048 >> 4), id_v, acc);
+                            mma_f16_ts(tc, pc + col, v + (uint32_t)k * (2048 >> 4), id_v, acc);
                             acc = 1;
                         }
                     mma_commit(&s.empty[stage % NS]);
@@ -906,12 +1151,12 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_tiles_kernel(const _
             };
             Pieces pieces;
             while (const Piece* p = pieces.next(s)) {
-                const int n = pieces.n - 1, lo = p->lo, hi = p->hi, t0 = p->t0, t1 = p->t1;
+                const int n = pieces.n - 1, start = p->start(0), hi = p->hi, t0 = p->t0, t1 = p->t1;
                 pieces.done(s);
                 const uint64_t q = sw128_desc(q_s + (n % QB) * QT * TM::kTileBytes);
                 ok = ok && warp_wait(&s.q_full[n % QB], (n / QB) & 1, dead);
                 for (int t = t0; t < t1 && ok; t++, j++) {
-                    const int n16 = (min(kTile, hi - (lo + t * kTile)) + 15) / 16;
+                    const int n16 = (min(kTile, hi - (start + t * kTile)) + 15) / 16;
                     ok = ok && warp_wait(&s.full[stage % NS], (stage / NS) & 1, dead);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -919,13 +1164,12 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_tiles_kernel(const _
                         const uint64_t k_sm = sw128_desc(ring_s + (stage % NS) * TM::kTileBytes);
                         const uint32_t sc = tmem + (j & 1) * TM::kSCols, id = idesc<C>(16 * n16, false);
                         uint32_t acc = 0;
-#pragma unroll
+#pragma unroll 1
                         for (int x = QT - 1; x >= 0; x--)
-#pragma unroll
-                            for (int k = 0; k < HD / 16; k++) {
-                                if (k >= ks) continue;
-                                const uint32_t in = ((k >> 2) * (kTile * 128) + (k & 3) * 32) >> 4;
-                                mma_f16(sc, q + x * (TM::kTileBytes >> 4) + in, k_sm + in, id, acc);
+#pragma unroll 2
+                            for (int k = 0; k < ks; k++) {
+                                const uint32_t in = (uint32_t)(k >> 2) * ((kTile * 128) >> 4) + (k & 3) * 2;
+                                mma_f16(sc, q + (uint32_t)x * (TM::kTileBytes >> 4) + in, k_sm + in, id, acc);
                                 acc = 1;
                             }
                         mma_commit(&s.empty[stage % NS]);
@@ -942,6 +1186,8 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_tiles_kernel(const _
             if (ok && j > 0) values(j - 1);
         }
     }
+    if (*dead)  // (copies of a share that gave up may still be on their way here)
+        for (int i = 0; i < 1000; i++) __nanosleep(1000);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (warp == kMmaWarp) {
@@ -1112,7 +1358,7 @@ __global__ void __launch_bounds__(kSharedJoinThreads) shared_join_kernel(const _
 constexpr int kMaxSharedDevices = 64;
 
 template <int HD, typename T, typename C, int QT, int PT>
-cudaError_t go(const SharedArgs& a, int sms, cudaStream_t s) {
+cudaError_t go(const SharedArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, int sms, cudaStream_t s) {
     static std::atomic<bool> attr[kMaxSharedDevices] = {};  // the attribute belongs to a device
     constexpr int smem = Tm<HD, QT, PT>::kTotal;
     auto kern = shared_tiles_kernel<HD, T, C, QT, PT>;
@@ -1126,7 +1372,7 @@ cudaError_t go(const SharedArgs& a, int sms, cudaStream_t s) {
     }
     e = launch_pdl(shared_line_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
     if (e != cudaSuccess) return e;
-    e = launch_pdl(kern, dim3((unsigned)(a.shares * a.nkv * a.blocks)), dim3(kSharedThreads), smem, s, a);
+    e = launch_pdl(kern, dim3((unsigned)(a.shares * a.nkv * a.blocks)), dim3(kSharedThreads), smem, s, a, mk, mv);
     if (e != cudaSuccess) return e;
     const int rows = std::min(a.batch, 8 * sms);
     const int y = std::max(1, std::min((a.nh + 7) / 8, 8 * sms / rows));
@@ -1134,10 +1380,34 @@ cudaError_t go(const SharedArgs& a, int sms, cudaStream_t s) {
 }
 
 template <int HD>
-cudaError_t go_hd(const SharedArgs& a, int dtype, int cache, int sms, cudaStream_t s) {
+cudaError_t go_hd(const SharedArgs& a, int dtype, int cache, const CUtensorMap& mk, const CUtensorMap& mv, int sms,
+                  cudaStream_t s) {
     if (dtype == 0)
-        return cache == 1 ? go<HD, float, __half, 2, 2>(a, sms, s) : go<HD, float, __nv_bfloat16, 3, 3>(a, sms, s);
-    return cache == 1 ? go<HD, __half, __half, 1, 2>(a, sms, s) : go<HD, __nv_bfloat16, __nv_bfloat16, 1, 2>(a, sms, s);
+        return cache == 1 ? go<HD, float, __half, 2, 2>(a, mk, mv, sms, s) : go<HD, float, __nv_bfloat16, 3, 3>(a, mk, mv, sms, s);
+    return cache == 1 ? go<HD, __half, __half, 1, 2>(a, mk, mv, sms, s) : go<HD, __nv_bfloat16, __nv_bfloat16, 1, 2>(a, mk, mv, sms, s);
+}
+
+// The positions of a tensor map's box: 16, or 8, where pages are multiples of
+// it; 0 where the cache's sizes or strides are not what a map takes.
+int box_of(const b2_paged_kv& kv) {
+    const int64_t top = (int64_t)1 << 38;  // (strides below 2^40 bytes)
+    const bool apart = (kv.nkv == 1 || kv.head_stride > 0) && kv.pos_stride > 0 && (kv.n_pages == 1 || kv.page_stride > 0);
+    if (!apart || kv.head_stride >= top || kv.pos_stride >= top || kv.page_stride >= top) return 0;
+    return kv.page_size % 16 == 0 ? 16 : kv.page_size % 8 == 0 ? 8 : 0;
+}
+
+// Dimensions: of a head, heads, positions of a page, pages.  A box is 64
+// dimensions (those past hd read as zero) of one head by `box` positions.
+bool make_map(CUtensorMap* m, const b2_paged_kv& kv, const void* at, int box) {
+    const auto enc = tensor_map_encoder();
+    if (!enc) return false;
+    auto stride = [](int64_t elements) { return (cuuint64_t)std::max<int64_t>(16, 2 * elements); };
+    const cuuint64_t dims[4] = {(cuuint64_t)kv.hd, (cuuint64_t)kv.nkv, (cuuint64_t)kv.page_size, (cuuint64_t)kv.n_pages};
+    const cuuint64_t strides[3] = {stride(kv.head_stride), stride(kv.pos_stride), stride(kv.page_stride)};
+    const cuuint32_t boxes[4] = {64, 1, (cuuint32_t)box, 1}, steps[4] = {1, 1, 1, 1};
+    return enc(m, kv.dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(at), dims,
+               strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // How a group of query heads falls to items, and the shares of the machine.
@@ -1239,7 +1509,10 @@ int launch_attention_shared(const b2_paged_kv& kv, const b2_paged_attn_opts& o, 
     a.scale = o.scale > 0.0f ? o.scale : (float)(1.0 / sqrt((double)kv.hd));
     a.softcap = o.softcap;
     layout(batch, o.nh, kv.nkv, kv.hd, sms, static_cast<uint8_t*>(scratch), &a);
-    const cudaError_t e = kv.hd <= 64 ? go_hd<64>(a, o.dtype, kv.dtype, sms, s) : go_hd<128>(a, o.dtype, kv.dtype, sms, s);
+    CUtensorMap mk{}, mv{};
+    a.box = box_of(kv);
+    if (a.box && !(make_map(&mk, kv, kv.k, a.box) && make_map(&mv, kv, kv.v, a.box))) a.box = 0;
+    const cudaError_t e = kv.hd <= 64 ? go_hd<64>(a, o.dtype, kv.dtype, mk, mv, sms, s) : go_hd<128>(a, o.dtype, kv.dtype, mk, mv, sms, s);
     return e == cudaSuccess ? B2_OK : cuda_failed("shared attention launch", e, err);
 }
 

@@ -54,8 +54,9 @@
 
 #include "../../include/b2decode.h"
 #include "dev.cuh"
-#include "tcgen05.cuh"
 #include "gemm.h"
+#include "tcgen05.cuh"
+#include "tensor_map.h"
 
 namespace b2 {
 namespace {
@@ -491,24 +492,6 @@ __global__ void splitk_sum1_kernel(const float* __restrict__ part, int ks, size_
     }
 }
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn(std::string* err) {
-    static EncodeTiledFn fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiledFn>(p);
-    });
-    if (!fn) *err = "cuTensorMapEncodeTiled is not available from the driver";
-    return fn;
-}
-
 bool make_map_2d(EncodeTiledFn enc, CUtensorMap* m, CUtensorMapDataType dt, const void* base, uint64_t inner,
                  uint64_t outer, uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle sw) {
     const cuuint64_t dims[2] = {inner, outer};
@@ -616,10 +599,9 @@ int gemm_run(int qtype, const void* base, int64_t rp, int64_t row0, int rows, in
         *err = "x must be 16-byte aligned and y 4-byte aligned";
         return B2_ERR_BAD_ARG;
     }
-    std::string e2;
-    EncodeTiledFn enc = encode_fn(&e2);
+    const EncodeTiledFn enc = tensor_map_encoder();
     if (!enc) {
-        *err = e2;
+        *err = "cuTensorMapEncodeTiled is not available from the driver";
         return B2_ERR_CUDA;
     }
     int dev = 0;
