@@ -19,15 +19,15 @@
 // follows the lengths that it finds.  A first launch of one CTA lays the line.
 //
 // One CTA an SM, its roles warp by warp:
-//   12-13  K and V rows into a ring of tiles in the 128-byte swizzle that the
+//   16-17  K and V rows into a ring of tiles in the 128-byte swizzle that the
 //          products read: by TMA where pages are multiples of 8 positions, by
 //          cp.async row by row elsewhere and at the ends of what is seen
-//   14     the share's pieces of the items, laid out ahead for the others, and Q
-//   15     tcgen05.mma, one thread: S = Q K^T of tile j + 1, then T = P V of tile
+//   18     the share's pieces of the items, laid out ahead for the others, and Q
+//   19     tcgen05.mma, one thread: S = Q K^T of tile j + 1, then T = P V of tile
 //          j, P being read from tensor memory
 //   0-7    two warpgroups taking tiles in turn: S out of tensor memory, a row to
 //          a thread, the exponentials, P back over S
-//   8-11   O: T out of tensor memory, added in fp32 (the tensor cores' own
+//   8-15   O, a half of the dimensions each four: T out of tensor memory, added in fp32 (the tensor cores' own
 //          accumulation cuts instead of rounding, which over a long row pulls
 //          towards zero); at an item's end the result or the piece
 //
@@ -250,15 +250,15 @@ __global__ void __launch_bounds__(kPlanThreads) shared_line_kernel(const __grid_
 // the products
 // ---------------------------------------------------------------------------
 
-constexpr int kSoftWarps = 8, kSumWarps = 4;  // then two warps that copy, one that plans and brings Q, one that multiplies
+constexpr int kSoftWarps = 8, kSumWarps = 8;  // then two warps that copy, one that plans and brings Q, one that multiplies
 constexpr int kCopyWarp = kSoftWarps + kSumWarps, kCopyWarps = 2, kQWarp = kCopyWarp + kCopyWarps, kMmaWarp = kQWarp + 1;
 constexpr int kSharedThreads = 32 * (kMmaWarp + 1);
 constexpr int kSharedSmemMax = 232448;
 constexpr int kPieces = 4;  // pieces known ahead
 constexpr int kGroup = 16;  // positions that one step of the products takes; tiles start on multiples
-// registers of a thread: 128 at the launch, of which the last four warps give some to O's
-constexpr int kSumRegs = 184, kLastRegs = 72;
-static_assert(kSharedThreads == 512 && 256 * 128 + 128 * kSumRegs + 128 * kLastRegs <= 512 * 128, "register split");
+// registers of a thread: 96 at the launch, of which the last four warps give some to the others
+constexpr int kSoftRegs = 112, kSumRegs = 96, kLastRegs = 64;
+static_assert(kSharedThreads == 640 && 256 * kSoftRegs + 256 * kSumRegs + 128 * kLastRegs <= 640 * 96, "register split");
 
 template <int HD, int QT, int PT>
 struct Tm {
@@ -266,9 +266,10 @@ struct Tm {
     static constexpr int kQBufs = QT == 1 ? 2 : 1;
     static constexpr int kQ = kQBufs * QT * kTileBytes;
     static constexpr int kRaw = QT == 1 ? 0 : 16384;  // fp32 rows of Q on their way
-    static constexpr int kFixed = 1024 + 17408;  // alignment, then barriers and small tables
+    static constexpr int kFixed = 1024 + 15360;  // alignment, then barriers and small tables
     static constexpr int kFit = (kSharedSmemMax - kFixed - kQ - kRaw) / kTileBytes;
     static constexpr int kStages = kFit > 8 ? 8 : kFit;
+    static constexpr int kStagesK = (kStages + 1) / 2, kStagesV = kStages / 2;
     // copies that a copying thread leaves in flight behind the one it has just issued
     static constexpr int kAhead = kStages > 4 ? 4 : kStages - 2;
     static_assert(kStages >= 3, "three tiles must fit");
@@ -288,7 +289,7 @@ struct Piece {
 constexpr int kPieceStart = 1, kPieceWhole = 2, kPieceOwn = 4, kPieceLast = 8;  // kPieceLast: no piece, the share is done
 
 struct SmallShared {
-    uint64_t full[8], empty[8], q_full[2], q_empty[2], s_full[2], p_full[2], t_full[2], t_empty[2];
+    uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], q_full[2], q_empty[2], s_full[2], p_full[2], t_full[2], t_empty[2];
     uint64_t piece_full[kPieces], piece_empty[kPieces];
     uint32_t tmem;
     int dead;                    // a wait gave up
@@ -298,27 +299,29 @@ struct SmallShared {
     float2 stats[4][kTile];      // m (log2 units) and l of a tile's rows
     float factor[kPieces][kTile];  // what an accumulator of S is times for a score
 };
-static_assert(sizeof(SmallShared) <= 17408, "");
+static_assert(sizeof(SmallShared) <= 15360, "");
 
-// Waits for a barrier's phase, asleep where the hardware can: a warp that
-// polls takes issue slots from the four others of its scheduler.
-__device__ __forceinline__ bool shared_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
+__device__ __forceinline__ bool phase_over(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(10000000u)  // (asleep for as long as that, where the hardware can)
+        : "memory");
+    return ok;
+}
+
+__device__ __forceinline__ bool long_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
     uint64_t t0 = 0;
     for (unsigned n = 0;; n++) {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok)
-            : "r"(smem_u32(bar)), "r"(parity), "r"(10000000u)
-            : "memory");
-        if (ok) return true;
+        if (__all_sync(0xffffffffu, phase_over(bar, parity))) return true;
         if (n % 64 == 63) {
-            if (*dead) return false;
+            if (__any_sync(0xffffffffu, *dead)) return false;
             const uint64_t t = global_ns();
             if (!t0) t0 = t;
-            if (t - t0 > kSharedWaitNs) {
+            if (__any_sync(0xffffffffu, t - t0 > kSharedWaitNs)) {
                 *dead = 1;
                 return false;
             }
@@ -326,9 +329,10 @@ __device__ __forceinline__ bool shared_wait(uint64_t* bar, uint32_t parity, vola
     }
 }
 
-// The same by a warp: one answer for all lanes.
+// Waits for a barrier's phase; by a warp, one answer for all lanes.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
-    return __all_sync(0xffffffffu, shared_wait(bar, parity, dead));
+    if (__all_sync(0xffffffffu, phase_over(bar, parity))) return true;
+    return long_wait(bar, parity, dead);
 }
 
 // V as the second operand: its rows are positions, the products' K, and its
@@ -339,24 +343,20 @@ __device__ __forceinline__ uint64_t v_desc(uint32_t saddr) {
            ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
 }
 
+__device__ __forceinline__ uint64_t desc_of(uint32_t lo, uint32_t hi) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+    return d;
+}
+
 template <typename C>
 __device__ __forceinline__ uint32_t idesc(int n, bool v) {
     const uint32_t type = std::is_same<C, __half>::value ? 0u : 1u;
     return (1u << 4) | (type << 7) | (type << 10) | ((v ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
 }
 
-// 32 columns of this thread's lane, on their way until tmem_wait of the same
+// 16 columns of this thread's lane, on their way until tmem_wait16 of the same
 // registers.
-__device__ __forceinline__ void tmem_get32(uint32_t taddr, uint32_t* r) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
-          "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
-          "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
-}
 __device__ __forceinline__ void tmem_get16(uint32_t taddr, uint32_t* r) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
@@ -371,12 +371,10 @@ __device__ __forceinline__ void tmem_wait16(uint32_t* r) {
                  : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
                    "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
 }
-__device__ __forceinline__ void tmem_wait32(uint32_t* r) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
-                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
-                   "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
-                   "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(v[0]),
+                 "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
 }
 
 // 16 bytes from global to shared memory where `go`; `valid` false: zeros.  No
@@ -387,6 +385,10 @@ __device__ __forceinline__ void cp16_if(uint32_t smem, const void* gmem, bool va
         "@p cp.async.cg.shared.global [%0], [%1], 16, %2;\n\t}" ::"r"(smem),
         "l"(gmem), "r"(valid ? 16 : 0), "r"((uint32_t)go)
         : "memory");
+}
+
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
 
 // A box of a cache's tensor map to shared memory: 64 dimensions from x on, one
@@ -452,7 +454,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
     shared_tiles_kernel(const __grid_constant__ SharedArgs a, const __grid_constant__ CUtensorMap map_k,
                         const __grid_constant__ CUtensorMap map_v) {
     using TM = Tm<HD, QT, PT>;
-    constexpr int NS = TM::kStages, NT = TM::kTBufs, QB = TM::kQBufs;
+    constexpr int NS = TM::kStages, NK = TM::kStagesK, NV = TM::kStagesV, NT = TM::kTBufs, QB = TM::kQBufs;
     extern __shared__ __align__(1024) uint8_t ssm_raw[];
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ssm_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* const q_sm = base;
@@ -469,9 +471,11 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
     const int hd = a.hd;
 
     if (tid == 0) {
-        for (int i = 0; i < 8; i++) {
-            mbar_init(&s.full[i], kCopyWarps);
-            mbar_init(&s.empty[i], 1);
+        for (int i = 0; i < 4; i++) {
+            mbar_init(&s.k_full[i], a.box ? 1 : kCopyWarps);
+            mbar_init(&s.v_full[i], a.box ? 1 : kCopyWarps);
+            mbar_init(&s.k_empty[i], 1);
+            mbar_init(&s.v_empty[i], 1);
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&s.q_full[i], 1);
@@ -508,6 +512,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
 
     if (warp < kSoftWarps) {
         // ------------------------------------------------------------ exponentials
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
         const int wg = warp >> 2, quad = warp & 3, m = quad * 32 + lane;
         const uint32_t s_col = tmem + ((uint32_t)(quad * 32) << 16) + wg * TM::kSCols;
         const float cap = a.softcap;
@@ -555,65 +560,59 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                         if (!plain) f = 1.0f;
                     }
-                    // 32 columns on their way while 32 are worked on
-                    uint32_t ra[32], rb[32];
-                    float mx = -INFINITY;
+                    // 16 columns on their way while 16 are worked on, in loops that the instruction
+                    // cache next to the scheduler holds
+                    uint32_t ra[16], rb[16];
+                    float x0 = -INFINITY, x1 = -INFINITY;
                     auto largest = [&](const uint32_t* r) {
-                        float x0 = mx, x1 = -INFINITY;
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
+                        for (int i = 0; i < 16; i += 4) {
                             x0 = fmaxf(fmaxf(x0, __uint_as_float(r[i])), __uint_as_float(r[i + 1]));
                             x1 = fmaxf(fmaxf(x1, __uint_as_float(r[i + 2])), __uint_as_float(r[i + 3]));
                         }
-                        mx = fmaxf(x0, x1);
                     };
-                    tmem_get32(s_col, ra);
+                    const uint32_t end = s_col + 32 * chunks;
+                    tmem_get16(s_col, ra);
 #pragma unroll 1
-                    for (int ch = 0; ch < chunks; ch += 2) {
-                        tmem_wait32(ra);
-                        if (ch + 1 < chunks) tmem_get32(s_col + 32 * ch + 32, rb);
+                    for (uint32_t c = s_col; c < end; c += 32) {
+                        tmem_wait16(ra);
+                        tmem_get16(c + 16, rb);
                         largest(ra);
-                        if (ch + 1 < chunks) {
-                            tmem_wait32(rb);
-                            if (ch + 2 < chunks) tmem_get32(s_col + 32 * ch + 64, ra);
-                            largest(rb);
-                        }
+                        tmem_wait16(rb);
+                        tmem_get16(c + 32 < end ? c + 32 : s_col, ra);  // (at the end, the first columns again)
+                        largest(rb);
                     }
-                    tmem_get32(s_col, ra);
+                    const float mx = fmaxf(x0, x1);
                     const float top = mx == -INFINITY ? -INFINITY : mx * f, z = 14.0f - (top == -INFINITY ? 0.0f : top);
                     const unsigned long long f2 = f2_pack(f, f), z2 = f2_pack(z, z);
-                    unsigned long long l2 = 0;
-                    auto weigh = [&](const uint32_t* r, int ch) {
-                        uint32_t w[PT][16];
+                    unsigned long long l2 = 0, l3 = 0;
+                    auto weigh = [&](const uint32_t* r, uint32_t to, uint32_t third) {
+                        uint32_t w[PT][8];
 #pragma unroll
-                        for (int i = 0; i < 16; i++) {
+                        for (int i = 0; i < 8; i++) {
                             const float2 d = f2_unpack(f2_fma(f2_pack(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), f2, z2));
                             const float e0 = ex2(d.x), e1 = ex2(d.y);
-                            l2 = f2_add(l2, f2_pack(e0, e1));
+                            if (i & 1) l2 = f2_add(l2, f2_pack(e0, e1));
+                            else l3 = f2_add(l3, f2_pack(e0, e1));
                             uint32_t x[PT];
                             split_terms<C, PT>(e0, e1, x);
 #pragma unroll
                             for (int k = 0; k < PT; k++) w[k][i] = x[k];
                         }
-                        if (PT == 1) {
-                            tmem_st16(s_col + 16 * ch, w[0]);
-                        } else {
-                            tmem_st16(s_col + 32 * ch, w[0]);
-                            tmem_st16(s_col + 32 * ch + 16, w[PT > 1 ? 1 : 0]);
-                            if (PT == 3) tmem_st16(s_col + 128 + 16 * ch, w[PT - 1]);
-                        }
+                        tmem_st8(to, w[0]);
+                        if (PT > 1) tmem_st8(to + 8, w[PT > 1 ? 1 : 0]);
+                        if (PT == 3) tmem_st8(third, w[PT - 1]);
                     };
 #pragma unroll 1
-                    for (int ch = 0; ch < chunks; ch += 2) {
-                        tmem_wait32(ra);
-                        if (ch + 1 < chunks) tmem_get32(s_col + 32 * ch + 32, rb);
-                        weigh(ra, ch);
-                        if (ch + 1 < chunks) {
-                            tmem_wait32(rb);
-                            if (ch + 2 < chunks) tmem_get32(s_col + 32 * ch + 64, ra);
-                            weigh(rb, ch + 1);
-                        }
+                    for (uint32_t c = s_col, th = s_col + 128; c < end; c += 32, th += 16) {
+                        tmem_wait16(ra);
+                        tmem_get16(c + 16, rb);
+                        weigh(ra, c, th);
+                        tmem_wait16(rb);
+                        if (c + 32 < end) tmem_get16(c + 32, ra);
+                        weigh(rb, c + 16, th + 8);
                     }
+                    l2 = f2_add(l2, l3);
                     const float2 ls = f2_unpack(l2);
                     float l = ls.x + ls.y;
                     const uint32_t* bad = s.bad[j & 7];
@@ -633,20 +632,21 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
         }
     } else if (warp < kSoftWarps + kSumWarps) {
         // ------------------------------------------------------------ O
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
-        const int quad = warp & 3, m = quad * 32 + lane;
-        const uint32_t t_col = tmem + ((uint32_t)(quad * 32) << 16) + 2 * TM::kSCols;
+        constexpr int HC = HD / 2;  // columns of a warp
+        const int half = (warp - kSoftWarps) >> 2, quad = warp & 3, m = quad * 32 + lane;
+        const uint32_t t_col = tmem + ((uint32_t)(quad * 32) << 16) + 2 * TM::kSCols + half * HC;
         const int rr = m / a.hb, head = head0 + m - rr * a.hb;
+        const int d0 = half * HC, dn = min(HC, hd - d0);  // this warp's dimensions
         int j = 0;
         bool ok = true;
         Pieces pieces;
         while (const Piece* p = pieces.next(s)) {
             const int4 row = s.row[(pieces.n - 1) % kPieces][m];
             const bool busy = __any_sync(0xffffffffu, row.w != 0);
-            unsigned long long o[HD / 2];
+            unsigned long long o[HC / 2];
             float M = -INFINITY, L = 0.0f;
 #pragma unroll
-            for (int i = 0; i < HD / 2; i++) o[i] = 0;
+            for (int i = 0; i < HC / 2; i++) o[i] = 0;
             const int t1 = p->t1;
 #pragma unroll 1
             for (int t = p->t0; t < t1; t++, j++) {
@@ -661,24 +661,16 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                     M = n;
                     L = fmaf(L, fo, st.y * ft);
                     const unsigned long long fo2 = f2_pack(fo, fo), ft2 = f2_pack(ft, ft);
-                    uint32_t ra[16], rb[16];
-                    auto add = [&](const uint32_t* r, int c) {
+                    const uint32_t from = t_col + buf * HD;
+#pragma unroll
+                    for (int c = 0; c < HC; c += 16) {
+                        uint32_t r[16];
+                        tmem_ld16(from + c, r);
 #pragma unroll
                         for (int i = 0; i < 8; i++) {
                             const unsigned long long x = f2_pack(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
                             o[c / 2 + i] = f2_fma(o[c / 2 + i], fo2, f2_mul(x, ft2));
                         }
-                    };
-                    const uint32_t from = t_col + buf * HD;
-                    tmem_get16(from, ra);
-#pragma unroll
-                    for (int c = 0; c < HD; c += 32) {
-                        tmem_wait16(ra);
-                        tmem_get16(from + c + 16, rb);
-                        add(ra, c);
-                        tmem_wait16(rb);
-                        if (c + 32 < HD) tmem_get16(from + c + 32, ra);
-                        add(rb, c + 16);
                     }
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -688,14 +680,14 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
             if (!ok) L = __int_as_float(0x7fc00000);  // (a wait gave up: no result)
             const int b = p->row0 + rr, kind = p->kind;
             pieces.done(s);
-            if (!row.w) continue;
+            if (!row.w || dn <= 0) continue;
             if ((kind & kPieceWhole) && (row.w & 2)) {  // all that the row sees
                 const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-                T* out = static_cast<T*>(a.out) + (int64_t)b * a.out_stride + (int64_t)head * hd;
+                T* out = static_cast<T*>(a.out) + (int64_t)b * a.out_stride + (int64_t)head * hd + d0;
                 bool odd = false;  // not finite
 #pragma unroll
-                for (int i = 0; i < HD / 8; i++) {
-                    if (8 * i >= hd) break;
+                for (int i = 0; i < HC / 8; i++) {
+                    if (8 * i >= dn) break;
                     alignas(16) T y[8];
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
@@ -714,7 +706,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                         for (int k = 0; k < 8; k++) out[8 * i + k] = y[k];
                     }
                 }
-                if (a.lse) a.lse[(int64_t)b * a.nh + head] = L == 0.0f ? -INFINITY : (M + (log2f(L) - 14.0f)) * kLn2;
+                if (a.lse && half == 0) a.lse[(int64_t)b * a.nh + head] = L == 0.0f ? -INFINITY : (M + (log2f(L) - 14.0f)) * kLn2;
                 if (odd) a.redo[b] = 1;
             } else {
                 const int64_t width = hd + 4;
@@ -722,12 +714,12 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                                 ? a.whole + (((int64_t)(kind & kPieceOwn ? 1 : 0) * a.batch + b) * a.nh + head) * width
                                 : a.part + (((int64_t)blockIdx.x * 2 + (kind & kPieceStart ? 1 : 0)) * kTile + m) * width;
 #pragma unroll
-                for (int i = 0; i < HD / 4; i++) {
-                    if (4 * i >= hd) break;
+                for (int i = 0; i < HC / 4; i++) {
+                    if (4 * i >= dn) break;
                     const float2 x = f2_unpack(o[2 * i]), y = f2_unpack(o[2 * i + 1]);
-                    *reinterpret_cast<float4*>(to + 4 * i) = make_float4(x.x, x.y, y.x, y.y);
+                    *reinterpret_cast<float4*>(to + d0 + 4 * i) = make_float4(x.x, x.y, y.x, y.y);
                 }
-                *reinterpret_cast<float2*>(to + hd) = make_float2(M, L);
+                if (half == 0) *reinterpret_cast<float2*>(to + hd) = make_float2(M, L);
             }
         }
     } else {
@@ -735,13 +727,12 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
         if (warp < kQWarp) {
             // -------------------------------------------------------- K and V
             const int lw = warp - kCopyWarp, hc = hd / 8;
-            const uint32_t ring_s = smem_u32(ring);
+            const uint32_t ring_k = smem_u32(ring), ring_v = ring_k + NK * TM::kTileBytes;
             int j = 0;
             Pieces pieces;
             const Piece* p = pieces.next(s);
             int t = p ? p->t0 : 0;
-            bool ok = true, have = false;
-            int stage = 0;
+            bool ok = true;
             auto page_at = [&](const Piece* q, int pos) {
                 const int pg = a.page_shift >= 0 ? pos >> a.page_shift : pos / a.page_size;
                 return a.table[(int64_t)q->tr * a.table_stride + pg];
@@ -749,25 +740,27 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
             auto place = [&](int pos) {  // in its page
                 return a.page_shift >= 0 ? pos & (a.page_size - 1) : pos - pos / a.page_size * a.page_size;
             };
-            auto slot_free = [&]() {
-                if (stage >= NS) ok = ok && warp_wait(&s.empty[stage % NS], (stage / NS - 1) & 1, dead);
-                return ok;
-            };
             if (a.box) {
-                // Groups of `box` positions that lie in one page: seen whole, a tensor map's
-                // box each, issued by the first warp; in part, or in no page, row by row by
-                // the second.  The products take 16 positions at a time, so rows of V up to
-                // there that nobody sees are zeros.
+                // K by the first warp, V by the second.  Groups of `box` positions that lie in one
+                // page: seen whole, a tensor map's box each; in part, or in no page, row by row.
+                // The products take 16 positions at a time, so rows of V up to there that nobody
+                // sees are zeros.
                 const int G = a.box, groups = kTile / G;
+                const bool value = lw != 0;
+                const CUtensorMap* map = value ? &map_v : &map_k;
+                const uint16_t* src = value ? a.v : a.k;
+                const int slots = value ? NV : NK;
+                const uint32_t ring_s = value ? ring_v : ring_k;
+                uint64_t *full = value ? s.v_full : s.k_full, *empty = value ? s.v_empty : s.k_empty;
+                int slot = 0, lap = 0;
                 struct Tile {
-                    int page, pos, lo, hi, n;  // this lane's group: page, first position; the tile's seen rows, rows to fill
+                    int page, pos, lo, hi;  // this lane's group: page, first position; the tile's seen rows
                 };
                 auto look = [&](const Piece* q, int tt) {
                     Tile f;
                     const int p0 = q->start(tt);
                     f.lo = q->lo - p0;
                     f.hi = min(kTile, q->hi - p0);
-                    f.n = (f.hi + kGroup - 1) & ~(kGroup - 1);
                     f.pos = p0 + lane * G;
                     f.page = -1;
                     // (any position of the group that is seen names its page)
@@ -775,51 +768,10 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                     return f;
                 };
                 constexpr int BL = HD / 64;  // boxes of a group
-                auto issue = [&](const CUtensorMap* map, const uint16_t* src, const Tile& f, bool value) {
-                    if (!slot_free()) return;
-                    const int slot = stage % NS;
-                    const uint32_t to = ring_s + slot * TM::kTileBytes;
-                    const int r0 = lane * G;
-                    const bool there = (unsigned)f.page < (unsigned)a.n_pages;
-                    const bool whole = lane < groups && there && r0 >= f.lo && r0 + G <= f.hi;
-                    const uint32_t by_box = __ballot_sync(0xffffffffu, whole);
-                    if (lw == 0) {
-                        if (lane == 0) mbar_arrive_expect_tx(&s.full[slot], __popc(by_box) * G * 128 * BL);
-                        __syncwarp();
-                        if (whole) {
-                            const int in = place(f.pos);
-#pragma unroll
-                            for (int x = 0; x < BL; x++)
-                                tma_rows(to + x * (kTile * 128) + r0 * 128, map, 64 * x, h, in, f.page, &s.full[slot]);
-                        }
-                        __syncwarp();
-                    } else {
-                        uint32_t rest = __ballot_sync(0xffffffffu, lane < groups && !whole && r0 < f.n);
-                        while (rest) {
-                            const int g = __ffs(rest) - 1;
-                            rest &= rest - 1;
-                            const int page = __shfl_sync(0xffffffffu, f.page, g), pos = __shfl_sync(0xffffffffu, f.pos, g);
-                            const bool in_pool = (unsigned)page < (unsigned)a.n_pages;
-                            const uint16_t* from = src + (in_pool ? page * a.page_stride + place(pos) * a.pos_stride : 0) + h * a.head_stride;
-#pragma unroll 4
-                            for (int i = lane; i < G * hc; i += 32) {
-                                const int r = i / hc, c = i - r * hc, row = g * G + r;
-                                const bool seen = in_pool && row >= f.lo && row < f.hi;
-                                const uint32_t at = to + (c >> 3) * (kTile * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
-                                cp16_if(at, seen ? from + r * a.pos_stride + c * 8 : src, seen, seen || value);
-                            }
-                        }
-                        cp_async_commit();
-                        cp_wait<0>();
-                        fence_proxy_async();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&s.full[slot]);
-                    }
-                    stage++;
-                };
-                Tile nx{}, v{};
+                Tile nx{};
                 if (p) nx = look(p, t);
-                while (ok && p) {
+#pragma unroll 1
+                while (p) {
                     const Tile f = nx;
                     if (++t == p->t1) {
                         pieces.done(s);
@@ -827,36 +779,92 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                         t = p ? p->t0 : 0;
                     }
                     if (p) nx = look(p, t);  // (the next tile's pages, on their way meanwhile)
-                    // positions seen whose page is not there
-                    const int lo = max(f.lo, lane * G), hi = min(f.hi, lane * G + G);
-                    const bool gone = lane < groups && lo < hi && (unsigned)f.page >= (unsigned)a.n_pages;
-                    uint32_t bits[4] = {0, 0, 0, 0};
-                    if (__any_sync(0xffffffffu, gone)) {
-                        const uint32_t mine = gone ? (hi - lo == 32 ? 0xffffffffu : ((1u << (hi - lo)) - 1)) << (lo & 31) : 0;
+                    const int r0 = lane * G, in = place(f.pos);
+                    const bool there = (unsigned)f.page < (unsigned)a.n_pages;
+                    const bool whole = lane < groups && there && r0 >= f.lo && r0 + G <= f.hi;
+                    const uint32_t by_box = __ballot_sync(0xffffffffu, whole);
+                    uint32_t rest = __ballot_sync(0xffffffffu, lane < groups && !whole && r0 < ((f.hi + kGroup - 1) & ~(kGroup - 1)));
+                    if (!value) {  // positions seen whose page is not there
+                        const int lo = max(f.lo, r0), hi = min(f.hi, r0 + G);
+                        const bool gone = lane < groups && lo < hi && !there;
+                        uint32_t bits = 0;
+                        if (rest && __any_sync(0xffffffffu, gone)) {
+                            const uint32_t mine = gone ? ((1u << (hi - lo)) - 1) << (lo & 31) : 0;
 #pragma unroll
-                        for (int i = 0; i < 4; i++) bits[i] = __reduce_or_sync(0xffffffffu, (lo >> 5) == i ? mine : 0);
+                            for (int i = 0; i < 4; i++) {
+                                const uint32_t b = __reduce_or_sync(0xffffffffu, (lo >> 5) == i ? mine : 0);
+                                if (lane == i) bits = b;
+                            }
+                        }
+                        if (lane < 4) s.bad[j & 7][lane] = bits;
                     }
-                    if (lw == 0 && lane < 4) s.bad[j & 7][lane] = lane == 0 ? bits[0] : lane == 1 ? bits[1] : lane == 2 ? bits[2] : bits[3];
-                    issue(&map_k, a.k, f, false);
-                    if (ok && have) issue(&map_v, a.v, v, true);
-                    v = f;
-                    have = true;
+                    if (lap) ok = ok && warp_wait(&empty[slot], (lap - 1) & 1, dead);
+                    if (!ok) break;
+                    uint64_t* bar = &full[slot];
+                    const uint32_t to = ring_s + slot * TM::kTileBytes;
+                    if (lane == 0) {
+                        const uint32_t bytes = __popc(by_box) * G * 128 * BL;
+                        if (rest) mbar_expect_tx(bar, bytes);
+                        else mbar_arrive_expect_tx(bar, bytes);
+                    }
+                    __syncwarp();
+                    const bool one = elected();
+                    for (int g0 = 0; g0 < groups; g0 += 8)
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {  // (uniform over the warp)
+                            const int g = g0 + i, page = __shfl_sync(0xffffffffu, f.page, g), at = __shfl_sync(0xffffffffu, in, g);
+                            if ((by_box >> g) & 1 && one) {
+#pragma unroll
+                                for (int x = 0; x < BL; x++) tma_rows(to + x * (kTile * 128) + g * G * 128, map, 64 * x, h, at, page, bar);
+                            }
+                        }
+                    __syncwarp();
+                    if (rest) {
+                        while (rest) {
+                            const int g = __ffs(rest) - 1;
+                            rest &= rest - 1;
+                            const int page = __shfl_sync(0xffffffffu, f.page, g), at = __shfl_sync(0xffffffffu, in, g);
+                            const bool in_pool = (unsigned)page < (unsigned)a.n_pages;
+                            const uint16_t* from = src + (in_pool ? page * a.page_stride + at * a.pos_stride : 0) + h * a.head_stride;
+#pragma unroll 4
+                            for (int i = lane; i < G * hc; i += 32) {
+                                const int r = i / hc, c = i - r * hc, row = g * G + r;
+                                const bool seen = in_pool && row >= f.lo && row < f.hi;
+                                cp16_if(to + (c >> 3) * (kTile * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4),
+                                        seen ? from + r * a.pos_stride + c * 8 : src, seen, seen || value);
+                            }
+                        }
+                        cp_async_commit();
+                        cp_wait<0>();
+                        fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(bar);
+                    }
+                    if (++slot == slots) {
+                        slot = 0;
+                        lap++;
+                    }
                     j++;
                 }
-                if (ok && have) issue(&map_v, a.v, v, true);
             } else {
                 // Pages of any size and place: row by row, half of the tile's rows to a warp.
                 constexpr int RW = kTile / kCopyWarps;
                 constexpr int CH = HD / 8, LR = 32 / CH;  // chunks of a row, rows of a warp's copy
                 const int row0 = lw * RW + lane, c = lane % CH, r0 = lane / CH;
-                const uint32_t at0 = ring_s + (c >> 3) * (kTile * 128) + (lw * RW + r0) * 128;
+                const uint32_t at0 = ring_k + (c >> 3) * (kTile * 128) + (lw * RW + r0) * 128;
                 const int64_t h_off = (int64_t)h * a.head_stride + c * 8;
-                int told = 0;               // stages that the products know of
-                auto tell = [&](int upto) {  // the stages before `upto` have landed
+                int issued[2] = {0, 0}, told[2] = {0, 0};  // tiles of K, of V, and those that the products know of
+                int waiting = 0;                           // stages issued that they do not know of,
+                uint32_t kinds = 0;                        // and what these are (V: 1), the last in bit 0
+                bool have = false;
+                auto tell = [&](int leave) {  // all but the last `leave` stages have landed
                     fence_proxy_async();
                     __syncwarp();
-                    for (; told < upto; told++)
-                        if (lane == 0) mbar_arrive(&s.full[told % NS]);
+                    for (; waiting > leave; waiting--) {
+                        const bool v = (kinds >> (waiting - 1)) & 1;
+                        const int n = v ? told[1]++ : told[0]++;
+                        if (lane == 0) mbar_arrive(v ? &s.v_full[n % NV] : &s.k_full[n % NK]);
+                    }
                 };
                 // this lane's rows of a tile: their offset; -1: none there; -2: nor needed
                 struct Place {
@@ -879,8 +887,10 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                     return f;
                 };
                 auto issue = [&](const uint16_t* src, const Place& f, bool value) {
-                    if (!slot_free()) return;
-                    const uint32_t to = at0 + (stage % NS) * TM::kTileBytes;
+                    const int n = value ? issued[1]++ : issued[0]++, slots = value ? NV : NK, slot = n % slots;
+                    if (n >= slots) ok = ok && warp_wait(value ? &s.v_empty[slot] : &s.k_empty[slot], (n / slots - 1) & 1, dead);
+                    if (!ok) return;
+                    const uint32_t to = at0 + (slot + (value ? NK : 0)) * TM::kTileBytes;
                     constexpr int U = 4;  // copies whose places are worked out together
 #pragma unroll
                     for (int i0 = 0; i0 < RW / LR; i0 += U) {
@@ -895,10 +905,10 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                         }
                     }
                     cp_async_commit();
-                    stage++;
-                    if (stage > TM::kAhead) {
+                    kinds = kinds << 1 | (value ? 1 : 0);
+                    if (++waiting > TM::kAhead) {
                         cp_wait<TM::kAhead>();
-                        tell(stage - TM::kAhead);
+                        tell(TM::kAhead);
                     }
                 };
                 Place v{};
@@ -911,7 +921,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                         // (the piece that comes may wait for what is on its way)
                         if (!__all_sync(0xffffffffu, mbar_try_wait(&s.piece_full[pieces.n % kPieces], (pieces.n / kPieces) & 1))) {
                             cp_wait<0>();
-                            tell(stage);
+                            tell(0);
                         }
                         p = pieces.next(s);
                         t = p ? p->t0 : 0;
@@ -935,7 +945,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                 }
                 if (ok && have) issue(a.v, v, true);
                 cp_wait<0>();
-                if (ok) tell(stage);
+                if (ok) tell(0);
             }
         } else if (warp == kQWarp) {
             // -------------------------------------------------------- pieces and Q
@@ -1120,64 +1130,77 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
             }
         } else {
             // -------------------------------------------------------- products
-            const uint32_t ring_s = smem_u32(ring), q_s = smem_u32(q_sm);
-            const int ks = (hd + 15) / 16, n_v = ks * 16;
-            const uint32_t id_v = idesc<C>(n_v, true);
-            int stage = 0, j = 0, was = 0;  // was: positions of the tile before, in 16s
+            // (values that go into descriptors are shuffled from lane 0, which keeps them, and
+            // the sums with constants below, in the warp's uniform registers)
+            auto uniform = [](uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); };
+            const uint32_t ring_k = smem_u32(ring) >> 4, ring_v = ring_k + NK * (TM::kTileBytes >> 4), q_s = smem_u32(q_sm) >> 4;
+            const uint32_t hi_k = (uint32_t)(sw128_desc(0) >> 32), lo_k = (uint32_t)sw128_desc(0);
+            const uint32_t hi_v = (uint32_t)(v_desc(0) >> 32), lo_v = (uint32_t)v_desc(0);
+            const int ks = (hd + 15) / 16;
+            const uint32_t id_v = uniform(idesc<C>(ks * 16, true)), id_k = uniform(idesc<C>(0, false));
+            int j = 0, was = 0;  // was: positions of the tile before, in 16s
+            int k_slot = 0, k_lap = 0, v_slot = 0, v_lap = 0;
             bool ok = true;
             auto values = [&](int jj) {  // T = P V of tile jj
                 ok = ok && warp_wait(&s.p_full[jj & 1], (jj >> 1) & 1, dead);
-                ok = ok && warp_wait(&s.full[stage % NS], (stage / NS) & 1, dead);
+                ok = ok && warp_wait(&s.v_full[v_slot], v_lap & 1, dead);
                 if (jj >= NT) ok = ok && warp_wait(&s.t_empty[jj % NT], (jj / NT - 1) & 1, dead);
                 if (!ok) return;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t v = uniform(lo_v + ring_v + v_slot * (TM::kTileBytes >> 4));
+                const uint32_t pc = uniform(tmem + (jj & 1) * TM::kSCols), tc = uniform(tmem + 2 * TM::kSCols + (jj % NT) * HD);
+                const int n = (int)uniform(was);
                 if (elected()) {
-                    const uint64_t v = v_desc(ring_s + (stage % NS) * TM::kTileBytes);
-                    const uint32_t pc = tmem + (jj & 1) * TM::kSCols, tc = tmem + 2 * TM::kSCols + (jj % NT) * HD;
-                    uint32_t acc = 0;
-#pragma unroll 1
+#pragma unroll
                     for (int x = PT - 1; x >= 0; x--)  // (small terms first)
-#pragma unroll 2
-                        for (int k = 0; k < was; k++) {
-                            const uint32_t col = PT == 1 ? 8 * k : x == 2 ? 128 + 8 * k : 32 * (k >> 1) + 16 * x + 8 * (k & 1);
-                            mma_f16_ts(tc, pc + col, v + (uint32_t)k * (2048 >> 4), id_v, acc);
-                            acc = 1;
+#pragma unroll
+                        for (int k = 0; k < kTile / 16; k++) {
+                            if (k == n) break;
+                            mma_f16_ts(tc, pc + (x == 2 ? 128 + 8 * k : 16 * k + 8 * x),
+                                       desc_of(v + k * (2048 >> 4), hi_v), id_v, x < PT - 1 || k > 0);
                         }
-                    mma_commit(&s.empty[stage % NS]);
+                    mma_commit(&s.v_empty[v_slot]);
                     mma_commit(&s.t_full[jj % NT]);
                 }
                 __syncwarp();
-                stage++;
+                if (++v_slot == NV) {
+                    v_slot = 0;
+                    v_lap++;
+                }
             };
             Pieces pieces;
             while (const Piece* p = pieces.next(s)) {
                 const int n = pieces.n - 1, start = p->start(0), hi = p->hi, t0 = p->t0, t1 = p->t1;
                 pieces.done(s);
-                const uint64_t q = sw128_desc(q_s + (n % QB) * QT * TM::kTileBytes);
+                const uint32_t q = uniform(lo_k + q_s + (n % QB) * QT * (TM::kTileBytes >> 4));
                 ok = ok && warp_wait(&s.q_full[n % QB], (n / QB) & 1, dead);
+#pragma unroll 1
                 for (int t = t0; t < t1 && ok; t++, j++) {
                     const int n16 = (min(kTile, hi - (start + t * kTile)) + 15) / 16;
-                    ok = ok && warp_wait(&s.full[stage % NS], (stage / NS) & 1, dead);
+                    ok = ok && warp_wait(&s.k_full[k_slot], k_lap & 1, dead);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t k_sm = uniform(lo_k + ring_k + k_slot * (TM::kTileBytes >> 4));
+                    const uint32_t sc = uniform(tmem + (j & 1) * TM::kSCols), id = uniform(id_k | (uint32_t)(2 * n16) << 17);
                     if (elected()) {
-                        const uint64_t k_sm = sw128_desc(ring_s + (stage % NS) * TM::kTileBytes);
-                        const uint32_t sc = tmem + (j & 1) * TM::kSCols, id = idesc<C>(16 * n16, false);
-                        uint32_t acc = 0;
-#pragma unroll 1
+#pragma unroll
                         for (int x = QT - 1; x >= 0; x--)
-#pragma unroll 2
-                            for (int k = 0; k < ks; k++) {
+#pragma unroll
+                            for (int k = 0; k < HD / 16; k++) {
+                                if (k == ks) break;
                                 const uint32_t in = (uint32_t)(k >> 2) * ((kTile * 128) >> 4) + (k & 3) * 2;
-                                mma_f16(sc, q + (uint32_t)x * (TM::kTileBytes >> 4) + in, k_sm + in, id, acc);
-                                acc = 1;
+                                mma_f16(sc, desc_of(q + x * (TM::kTileBytes >> 4) + in, hi_k), desc_of(k_sm + in, hi_k), id,
+                                        x < QT - 1 || k > 0);
                             }
-                        mma_commit(&s.empty[stage % NS]);
+                        mma_commit(&s.k_empty[k_slot]);
                         mma_commit(&s.s_full[j & 1]);
                         if (t == t1 - 1) mma_commit(&s.q_empty[n % QB]);
                     }
                     __syncwarp();
-                    stage++;
+                    if (++k_slot == NK) {
+                        k_slot = 0;
+                        k_lap++;
+                    }
                     if (j > 0) values(j - 1);
                     was = n16;
                 }
@@ -1356,6 +1379,7 @@ __global__ void __launch_bounds__(kSharedJoinThreads) shared_join_kernel(const _
 }
 
 constexpr int kMaxSharedDevices = 64;
+constexpr int kTerms16 = 1;  // terms of the probabilities of 16-bit rows
 
 template <int HD, typename T, typename C, int QT, int PT>
 cudaError_t go(const SharedArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, int sms, cudaStream_t s) {
@@ -1384,7 +1408,8 @@ cudaError_t go_hd(const SharedArgs& a, int dtype, int cache, const CUtensorMap& 
                   cudaStream_t s) {
     if (dtype == 0)
         return cache == 1 ? go<HD, float, __half, 2, 2>(a, mk, mv, sms, s) : go<HD, float, __nv_bfloat16, 3, 3>(a, mk, mv, sms, s);
-    return cache == 1 ? go<HD, __half, __half, 1, 2>(a, mk, mv, sms, s) : go<HD, __nv_bfloat16, __nv_bfloat16, 1, 2>(a, mk, mv, sms, s);
+    return cache == 1 ? go<HD, __half, __half, 1, kTerms16>(a, mk, mv, sms, s)
+                      : go<HD, __nv_bfloat16, __nv_bfloat16, 1, kTerms16>(a, mk, mv, sms, s);
 }
 
 // The positions of a tensor map's box: 16, or 8, where pages are multiples of

@@ -62,6 +62,24 @@ class Shared(Paged):
         return out, ls
 
 
+    def check(self, out, ls, window=0, scale=0.0, softcap=0.0, slopes=None, q=None):
+        """As Paged.check, with the rounding of 16-bit rows' probabilities to one 16-bit term: each weight off by at
+        most half a step h, so out = sum w v / sum w by at most h max|v|.  (Averaged over a whole output that error
+        is as large as the rounding of the result, sqrt(2) together, well inside the half step that the 2-norm gets.)"""
+        want, lse, to, tl = attend64(self.q if q is None else q, self.kc, self.vc, self.table, self.lens, self.req, self.P,
+                                     window, scale or self.hd ** -0.5, softcap, slopes)
+        h = half_step(self.dt) if self.dt != torch.float32 else 0.0
+        to = to + h * float(torch.nan_to_num(self.vc.float(), 0.0, 0.0, 0.0).abs().max())
+        assert_within(out, want, to[..., None].expand_as(want), self.dt)
+        none = torch.isinf(lse)
+        assert torch.equal(torch.isinf(ls) & (ls < 0), none)
+        assert bool(((ls.double() - lse).abs() <= tl)[~none].all()), float((ls.double() - lse)[~none].abs().max())
+        seen = want[~none]
+        if seen.numel() > 1000:
+            rel = float((out[~none].double() - seen).norm() / seen.norm())
+            assert rel <= max(2.0 ** -19, half_step(self.dt)), rel
+
+
 @pytest.mark.parametrize("dtype,cache", COMBOS)
 @pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 64), (14, 2, 64), (32, 8, 128), (7, 7, 128), (4, 1, 32), (10, 2, 80), (20, 1, 96),
                                        (33, 1, 128), (2, 1, 8), (3, 1, 120), (6, 2, 256), (130, 1, 64), (256, 1, 72)])
@@ -156,6 +174,7 @@ def test_attention_shared_values_that_others_do_not_see():
         p.kc[page(120)][1] = math.nan
         o, ls = p.call()
         want, lse, to, tl = attend64(p.q, p.kc, p.vc, p.table, p.lens, p.req, 16, 0, 64 ** -0.5, 0.0, None)
+        to = to + half_step(p.dt) * float(torch.nan_to_num(p.vc.float(), 0.0, 0.0, 0.0).abs().max())
         for b in (0, 3):  # see none of it
             assert_within(o[b], want[b], to[b][:, None].expand_as(want[b]), p.dt)
         assert bool(torch.isfinite(ls[[0, 3]]).all())
@@ -352,7 +371,9 @@ def test_attention_shared_behind_its_plan():
     step()
     assert info.tolist()[0] == 0
     T = int(fresh.sum())
+    vmax = float(vc.float().abs().max())
     want, lse, to, tl = attend64(q, kc, vc, td, [x + 1 for x in pos.tolist()], req.tolist(), P, 0, hd ** -0.5, 0.0, None)
+    to = to + half_step(torch.bfloat16) * vmax  # (probabilities of one term)
     assert_within(out, want, to[..., None].expand_as(want), torch.bfloat16)
     assert bool((out[T:] == 0).all()) and bool((ls[T:] == -math.inf).all())
     assert float((out[:T].double() - want[:T]).norm() / want[:T].norm()) <= half_step(torch.bfloat16)
