@@ -16,13 +16,14 @@
 // tile being one (and an item's start another).  Share s of G takes the units
 // [s W / G, (s + 1) W / G) for every KV head side by side, so the machine is
 // evenly loaded whatever the lengths, the host knows none of them, and a graph
-// follows the lengths that it finds.  A first launch of one CTA lays the line.
+// follows the lengths that it finds.  A first launch lays the line, by one CTA.
 //
 // One CTA an SM, its roles warp by warp:
 //   16-17  K and V rows into a ring of tiles in the 128-byte swizzle that the
 //          products read: by TMA where pages are multiples of 8 positions, by
 //          cp.async row by row elsewhere and at the ends of what is seen
 //   18     the share's pieces of the items, laid out ahead for the others, and Q
+//          by TMA, whose 16-bit terms the first launch has made
 //   19     tcgen05.mma, one thread: S = Q K^T of tile j + 1, then T = P V of tile
 //          j, P being read from tensor memory
 //   0-7    two warpgroups taking tiles in turn: S out of tensor memory, a row to
@@ -75,6 +76,12 @@ struct Line {
     int items, shares;
 };
 
+// Where a share starts: item, its unit, units of the share.
+struct Share {
+    int item, at;
+    long long units;
+};
+
 struct SharedArgs {
     const void* q;
     const uint16_t *k, *v;
@@ -87,11 +94,14 @@ struct SharedArgs {
     int hb, blocks, rows;  // query heads of an item, such blocks of a group of heads, rows of an item
     int shares;            // at most
     int q_wide, out_wide;  // 16-byte accesses
+    int terms;             // of Q that the first launch makes; 0: the products read q as it is
     int box;               // positions of a box of the tensor maps (16 or 8); 0: pages that they cannot tell
     float scale, softcap;
     // scratch
     Line* line;
-    int* first;    // [shares] the item in which the share starts
+    Share* share;  // [shares]
+    uint16_t* term;  // [terms][batch][nh][hd] Q, scaled per row, as 16-bit terms
+    float* factor;   // [batch][nh] what a product with them is times for a score
     int* redo;     // [batch]
     int4* row;     // [batch] {first visible position, length, shared item, own item}: -1 none, -2 a row of NaN
     Item* item;    // [2 batch]
@@ -119,14 +129,12 @@ __device__ __forceinline__ int last_at(int n, F&& le) {
 // the line of items, by one CTA
 // ---------------------------------------------------------------------------
 
-__global__ void __launch_bounds__(kPlanThreads) shared_line_kernel(const __grid_constant__ SharedArgs a) {
+__device__ __forceinline__ void lay_line(const SharedArgs& a) {
     constexpr int W = kPlanThreads / 32;
     __shared__ int v_lo[kPlanThreads + kTile], v_hi[kPlanThreads + kTile], v_tr[kPlanThreads + kTile];
     __shared__ int owner_item[kTile + kPlanThreads];  // the item that starts at a row, also of the 128 rows before
     __shared__ long long w_units[W], u_item[kPlanItems];
     __shared__ int w_items[W];
-    pdl_trigger();
-    pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, R = a.rows;
 
     struct Group {
@@ -239,11 +247,87 @@ __global__ void __launch_bounds__(kPlanThreads) shared_line_kernel(const __grid_
     }
     const int G = (int)max(1LL, min((long long)a.shares, units / kMinShare));
     if (tid == 0) *a.line = Line{units, items, G};
-    if (units == 0) return;
+    if (units == 0) {
+        for (int s = tid; s < a.shares; s += kPlanThreads) a.share[s] = Share{0, 0, 0};
+        return;
+    }
+    for (int s = G + tid; s < a.shares; s += kPlanThreads) a.share[s] = Share{0, 0, 0};
     for (int s = tid; s < G; s += kPlanThreads) {
         const long long u = mul_div(s, units, G);
-        a.first[s] = last_at(items, [&](int i) { return (items <= kPlanItems ? u_item[i] : a.item[i].u0) <= u; });
+        const int i = last_at(items, [&](int x) { return (items <= kPlanItems ? u_item[x] : a.item[x].u0) <= u; });
+        const long long at = u - (items <= kPlanItems ? u_item[i] : a.item[i].u0);
+        a.share[s] = Share{i, (int)at, mul_div(s + 1, units, G) - u};
     }
+}
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+// 4 elements from p on
+__device__ __forceinline__ float4 load4(const float* p, bool wide) {
+    return wide ? *reinterpret_cast<const float4*>(p) : make_float4(p[0], p[1], p[2], p[3]);
+}
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p, bool wide) {
+    alignas(8) T t[4];
+    if (wide) *reinterpret_cast<uint2*>(t) = *reinterpret_cast<const uint2*>(p);
+    else
+#pragma unroll
+        for (int i = 0; i < 4; i++) t[i] = p[i];
+    return make_float4(to_float(t[0]), to_float(t[1]), to_float(t[2]), to_float(t[3]));
+}
+
+// A warp's rows of Q, one after another: largest element to [2^10, 2^11), then
+// 16-bit terms.  (A single term is q itself, copied for its alignment.)
+template <typename T, typename C, int QT>
+__device__ __forceinline__ void make_terms(const SharedArgs& a, long long first, long long step) {
+    const int lane = threadIdx.x & 31, d = 4 * lane;
+    const long long rows = (long long)a.batch * a.nh;
+    const bool in = d < a.hd;
+    constexpr int U = 4;
+    for (long long r0 = first; r0 < rows; r0 += U * step) {
+        float4 x[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const long long r = r0 + u * step;
+            x[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (r < rows && in) {
+                const int b = (int)(r / a.nh), head = (int)(r - (long long)b * a.nh);
+                x[u] = load4(static_cast<const T*>(a.q) + b * a.q_stride + (int64_t)head * a.hd + d, a.q_wide);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const long long r = r0 + u * step;
+            if (r >= rows) break;
+            if (QT > 1) {
+                const float mx = fmaxf(fmaxf(fabsf(x[u].x), fabsf(x[u].y)), fmaxf(fabsf(x[u].z), fabsf(x[u].w)));
+                const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(mx));  // (none negative: ordered as their bits)
+                // (the exponent field is enough: subnormal rows count as 2^-127; down to
+                // -117 for the largest finite row, so that both factors stay normal)
+                const int e = top < 0x7f800000u ? min(100, 137 - (int)(top >> 23)) : 0;
+                const float up = __int_as_float((127 + e) << 23), f = a.scale * __int_as_float((127 - e) << 23);
+                if (lane == 0) a.factor[r] = a.softcap > 0.0f ? f / a.softcap : f * kLog2e;
+                x[u] = make_float4(x[u].x * up, x[u].y * up, x[u].z * up, x[u].w * up);
+            }
+            uint32_t w0[QT], w1[QT];
+            split_terms<C, QT>(x[u].x, x[u].y, w0);
+            split_terms<C, QT>(x[u].z, x[u].w, w1);
+            if (in)
+#pragma unroll
+                for (int k = 0; k < QT; k++) *reinterpret_cast<uint2*>(a.term + (k * rows + r) * a.hd + d) = make_uint2(w0[k], w1[k]);
+        }
+    }
+}
+
+// The first launch: the line by one CTA, Q's terms by the others.
+template <typename T, typename C, int QT>
+__global__ void __launch_bounds__(kPlanThreads) shared_line_kernel(const __grid_constant__ SharedArgs a) {
+    pdl_trigger();
+    pdl_wait();
+    if (blockIdx.x == 0) lay_line(a);
+    else make_terms<T, C, QT>(a, (blockIdx.x - 1) * (kPlanThreads / 32) + threadIdx.x / 32, (gridDim.x - 1) * (kPlanThreads / 32));
 }
 
 // ---------------------------------------------------------------------------
@@ -265,15 +349,14 @@ struct Tm {
     static constexpr int kTileBytes = kTile * HD * 2;  // K or V rows of a tile, and one term of Q
     static constexpr int kQBufs = QT == 1 ? 2 : 1;
     static constexpr int kQ = kQBufs * QT * kTileBytes;
-    static constexpr int kRaw = QT == 1 ? 0 : 16384;  // fp32 rows of Q on their way
     static constexpr int kFixed = 1024 + 15360;  // alignment, then barriers and small tables
-    static constexpr int kFit = (kSharedSmemMax - kFixed - kQ - kRaw) / kTileBytes;
+    static constexpr int kFit = (kSharedSmemMax - kFixed - kQ) / kTileBytes;
     static constexpr int kStages = kFit > 8 ? 8 : kFit;
     static constexpr int kStagesK = (kStages + 1) / 2, kStagesV = kStages / 2;
     // copies that a copying thread leaves in flight behind the one it has just issued
     static constexpr int kAhead = kStages > 4 ? 4 : kStages - 2;
     static_assert(kStages >= 3, "three tiles must fit");
-    static constexpr int kTotal = kFixed + kQ + kRaw + kStages * kTileBytes;
+    static constexpr int kTotal = kFixed + kQ + kStages * kTileBytes;
     // tensor memory: two S (P over it, a third term behind it), then T
     static constexpr int kSCols = PT == 3 ? 192 : 128;
     static constexpr int kTBufs = 2 * kSCols + 2 * HD <= 512 ? 2 : 1;
@@ -391,8 +474,9 @@ __device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
     asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
 
-// A box of a cache's tensor map to shared memory: 64 dimensions from x on, one
-// head, kGroup or 8 positions from pos on, one page.
+// A box of a tensor map to shared memory: of a cache's, 64 dimensions from x on,
+// one head, kGroup or 8 positions from pos on, one page; of Q's, 64 dimensions,
+// an item's heads, its rows, one term.
 __device__ __forceinline__ void tma_rows(uint32_t smem, const CUtensorMap* map, int x, int head, int pos, int page, uint64_t* bar) {
     asm volatile(
         "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::
@@ -412,24 +496,6 @@ __device__ __forceinline__ bool elected() {
     uint32_t r;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
     return r != 0;
-}
-
-__device__ __forceinline__ float to_float(float x) { return x; }
-__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-
-// 4 elements from p on
-__device__ __forceinline__ float4 load4(const float* p, bool wide) {
-    return wide ? *reinterpret_cast<const float4*>(p) : make_float4(p[0], p[1], p[2], p[3]);
-}
-template <typename T>
-__device__ __forceinline__ float4 load4(const T* p, bool wide) {
-    alignas(8) T t[4];
-    if (wide) *reinterpret_cast<uint2*>(t) = *reinterpret_cast<const uint2*>(p);
-    else
-#pragma unroll
-        for (int i = 0; i < 4; i++) t[i] = p[i];
-    return make_float4(to_float(t[0]), to_float(t[1]), to_float(t[2]), to_float(t[3]));
 }
 
 // Where a warp is in the pieces.
@@ -452,15 +518,14 @@ struct Pieces {
 template <int HD, typename T, typename C, int QT, int PT>
 __global__ void __launch_bounds__(kSharedThreads, 1)
     shared_tiles_kernel(const __grid_constant__ SharedArgs a, const __grid_constant__ CUtensorMap map_k,
-                        const __grid_constant__ CUtensorMap map_v) {
+                        const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_q) {
     using TM = Tm<HD, QT, PT>;
     constexpr int NS = TM::kStages, NK = TM::kStagesK, NV = TM::kStagesV, NT = TM::kTBufs, QB = TM::kQBufs;
     extern __shared__ __align__(1024) uint8_t ssm_raw[];
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ssm_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* const q_sm = base;
     uint8_t* const ring = base + TM::kQ;
-    uint8_t* const raw = ring + NS * TM::kTileBytes;
-    SmallShared& s = *reinterpret_cast<SmallShared*>(raw + TM::kRaw);
+    SmallShared& s = *reinterpret_cast<SmallShared*>(ring + NS * TM::kTileBytes);
     volatile int* dead = &s.dead;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -724,6 +789,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLastRegs));
+        asm volatile("fence.proxy.async;" ::: "memory");  // what the launches before wrote, for the TMA copies
         if (warp < kQWarp) {
             // -------------------------------------------------------- K and V
             const int lw = warp - kCopyWarp, hc = hd / 8;
@@ -949,24 +1015,19 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
             }
         } else if (warp == kQWarp) {
             // -------------------------------------------------------- pieces and Q
-            const Line line = *a.line;
-            const bool work = line.units > 0 && share < line.shares;
-            long long u = 0, left = 0;  // the unit that comes next, units of this share that are left
-            int next = 0;
+            const Share mine = share < a.shares ? a.share[share] : Share{0, 0, 0};
+            const int items = a.line->items;
+            long long left = mine.units;  // units of this share that are left
+            int next = mine.item, at = mine.at;
             Item ahead{};
             auto load = [&]() {
-                if (next < line.items) {
+                if (next < items) {
                     const int4* from = reinterpret_cast<const int4*>(a.item + next);
                     reinterpret_cast<int4*>(&ahead)[0] = from[0];
                     reinterpret_cast<int4*>(&ahead)[1] = from[1];
                 }
             };
-            if (work) {
-                u = mul_div(share, line.units, line.shares);
-                left = mul_div(share + 1, line.units, line.shares) - u;
-                next = a.first[share];
-                load();
-            }
+            if (left > 0) load();
             bool ok = true;
             // lays out piece n; false: there is none
             auto plan = [&](int n) {
@@ -976,13 +1037,13 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                 Piece p{};
                 p.kind = kPieceLast;
                 int limit = 0;
-                while (left > 0 && next < line.items) {
+                while (left > 0 && next < items) {
                     const Item it = ahead;
                     next++;
                     load();
-                    const int tiles = tiles_of(it), x = (int)(u - it.u0), take = (int)min((long long)(tiles + kItemUnits - x), left);
+                    const int tiles = tiles_of(it), x = at, take = (int)min((long long)(tiles + kItemUnits - x), left);
                     left -= take;
-                    u += take;
+                    at = 0;
                     p.t0 = max(0, x - kItemUnits);
                     p.t1 = max(0, x + take - kItemUnits);
                     if (p.t1 == p.t0) continue;
@@ -1005,6 +1066,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                             const int4 r = a.row[p.row0 + rr];
                             const bool all = (p.kind & kPieceOwn ? r.z : r.w) < 0;
                             w = make_int4(max(r.x, p.lo), min(r.y, limit), r.y, all ? 3 : 1);
+                            if (QT > 1) s.factor[slot][m] = a.factor[(int64_t)(p.row0 + rr) * a.nh + head0 + m - rr * a.hb];
                         }
                         s.row[slot][m] = w;
                     }
@@ -1014,114 +1076,21 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                 if (lane == 0) mbar_arrive(&s.piece_full[slot]);
                 return !(p.kind & kPieceLast);
             };
-            constexpr int LN = HD / 4, RS = 32 / LN;  // lanes of a row, rows of a step
-            const int d = 4 * (lane % LN), rs = lane / LN;
-            // a row of the product, `at` its first 64 dimensions' line: this lane's four elements as terms
-            auto put = [&](uint8_t* to, int slot, int m, float4 x, bool go) {
-                if (QT > 1) {  // the row's largest element to [2^10, 2^11)
-                    float mx = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+            auto bring = [&](int n) {  // Q of piece n: rows that are not the item's come along, and are not looked at
+                if (n >= QB) ok = ok && warp_wait(&s.q_empty[n % QB], (n / QB - 1) & 1, dead);
+                if (!ok) return;
+                uint64_t* bar = &s.q_full[n % QB];
+                const uint32_t to = smem_u32(q_sm) + (n % QB) * QT * TM::kTileBytes;
+                const int row0 = s.piece[n % kPieces].row0;
+                if (elected()) {
+                    mbar_arrive_expect_tx(bar, a.hb * a.rows * 128 * (HD / 64) * QT);
 #pragma unroll
-                    for (int o = LN / 2; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                    // (the exponent field is enough: subnormal rows count as 2^-127; down to
-                    // -117 for the largest finite row, so that both factors stay normal)
-                    const int e = mx < INFINITY ? min(100, 137 - (int)(__float_as_uint(mx) >> 23)) : 0;
-                    const float up = __int_as_float((127 + e) << 23), f = a.scale * __int_as_float((127 - e) << 23);
-                    if (d == 0 && go) s.factor[slot][m] = a.softcap > 0.0f ? f / a.softcap : f * kLog2e;
-                    x = make_float4(x.x * up, x.y * up, x.z * up, x.w * up);
-                }
-                uint32_t w0[QT], w1[QT];
-                split_terms<C, QT>(x.x, x.y, w0);
-                split_terms<C, QT>(x.z, x.w, w1);
-                if (go) {
-                    uint8_t* at = to + m * 128 + (d >> 6) * (kTile * 128) + ((((d & 63) >> 3) ^ (m & 7)) << 4) + (d & 4) * 2;
+                    for (int x = 0; x < QT; x++)
 #pragma unroll
-                    for (int k = 0; k < QT; k++) *reinterpret_cast<uint2*>(at + k * TM::kTileBytes) = make_uint2(w0[k], w1[k]);
+                        for (int k = 0; k < HD / 64; k++)
+                            tma_rows(to + x * TM::kTileBytes + k * (kTile * 128), &map_q, 64 * k, head0, row0, x, bar);
                 }
-            };
-            auto bring = [&](int n) {  // Q of piece n
-                const int slot = n % kPieces, row0 = s.piece[slot].row0, count = s.piece[slot].rows * a.hb;
-                uint8_t* to = q_sm + (n % QB) * QT * TM::kTileBytes;
-                const T* q = static_cast<const T*>(a.q) + (int64_t)row0 * a.q_stride + (int64_t)head0 * hd;
-                auto free_ = [&]() {
-                    if (n >= QB) ok = ok && warp_wait(&s.q_empty[n % QB], (n / QB - 1) & 1, dead);
-                    return ok;
-                };
-                if (QT == 1 && a.q_wide) {  // as it is: chunks of 8 elements straight to their places
-                    if (!free_()) return;
-                    constexpr int CH = HD / 8, CR = 32 / CH;
-                    const int c = lane % CH;
-                    int m = lane / CH, qr = m / a.hb, hh = m - qr * a.hb;
-#pragma unroll 4
-                    for (int i = 0; i < count; i += CR) {
-                        const bool go = m < count && hh < hn && 8 * c < hd;
-                        const T* from = q + qr * a.q_stride + hh * hd + 8 * c;
-                        cp16_if(smem_u32(to) + m * 128 + (c >> 3) * (kTile * 128) + (((c & 7) ^ (m & 7)) << 4), go ? (const void*)from : a.q,
-                                true, go);
-                        m += CR;
-                        hh += CR;
-                        while (hh >= a.hb) {
-                            hh -= a.hb;
-                            qr++;
-                        }
-                    }
-                    cp_async_commit();
-                    cp_wait<0>();
-                } else if (QT > 1 && a.q_wide) {
-                    // fp32 rows pass through two halves of `raw`, a lane's 16 bytes coming back to
-                    // itself, so that a run of them is on its way while one is split
-                    constexpr int U = 16;  // steps of a half
-                    int m = rs, qr = m / a.hb, hh = m - qr * a.hb;
-                    const uint32_t mine = smem_u32(raw) + lane * 16;
-                    auto fetch = [&](int half) {
-#pragma unroll 4
-                        for (int i = 0; i < U; i++) {
-                            const bool go = m < count && hh < hn && d < hd;
-                            const T* from = q + qr * a.q_stride + hh * hd + d;
-                            cp16_if(mine + (half * U + i) * 512, go ? (const void*)from : a.q, go, true);
-                            m += RS;
-                            hh += RS;
-                            while (hh >= a.hb) {
-                                hh -= a.hb;
-                                qr++;
-                            }
-                        }
-                        cp_async_commit();
-                    };
-                    fetch(0);
-                    if (!free_()) {
-                        cp_wait<0>();
-                        return;
-                    }
-                    for (int m0 = 0, half = 0; m0 < count; m0 += U * RS, half ^= 1) {
-                        fetch(half ^ 1);
-                        cp_wait<1>();
-#pragma unroll 2
-                        for (int i = 0; i < U; i++) {
-                            const int mm = m0 + i * RS + rs;
-                            const float4 x = *reinterpret_cast<const float4*>(raw + (half * U + i) * 512 + lane * 16);
-                            put(to, slot, mm, x, mm < count && d < hd);
-                        }
-                    }
-                    cp_wait<0>();
-                } else {  // rows off 16 bytes
-                    if (!free_()) return;
-                    int m = rs, qr = m / a.hb, hh = m - qr * a.hb;
-#pragma unroll 2
-                    for (int i = 0; i < count; i += RS) {
-                        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        if (m < count && hh < hn && d < hd) x = load4(q + qr * a.q_stride + hh * hd + d, false);
-                        put(to, slot, m, x, m < count && d < hd);
-                        m += RS;
-                        hh += RS;
-                        while (hh >= a.hb) {
-                            hh -= a.hb;
-                            qr++;
-                        }
-                    }
-                }
-                fence_proxy_async();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&s.q_full[n % QB]);
             };
             bool more = plan(0);
             for (int n = 0; ok && more; n++) {
@@ -1382,7 +1351,7 @@ constexpr int kMaxSharedDevices = 64;
 constexpr int kTerms16 = 1;  // terms of the probabilities of 16-bit rows
 
 template <int HD, typename T, typename C, int QT, int PT>
-cudaError_t go(const SharedArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, int sms, cudaStream_t s) {
+cudaError_t go(const SharedArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, int sms, cudaStream_t s) {
     static std::atomic<bool> attr[kMaxSharedDevices] = {};  // the attribute belongs to a device
     constexpr int smem = Tm<HD, QT, PT>::kTotal;
     auto kern = shared_tiles_kernel<HD, T, C, QT, PT>;
@@ -1394,9 +1363,11 @@ cudaError_t go(const SharedArgs& a, const CUtensorMap& mk, const CUtensorMap& mv
         if (e != cudaSuccess) return e;
         if (dev < kMaxSharedDevices) attr[dev] = true;
     }
-    e = launch_pdl(shared_line_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
+    const long long q_rows = a.terms ? (long long)a.batch * a.nh : 0;  // (a warp takes four at a time)
+    const int ctas = 1 + (int)std::min<long long>(2 * sms - 1, (q_rows + kPlanThreads / 8 - 1) / (kPlanThreads / 8));
+    e = launch_pdl(shared_line_kernel<T, C, QT>, dim3(ctas), dim3(kPlanThreads), 0, s, a);
     if (e != cudaSuccess) return e;
-    e = launch_pdl(kern, dim3((unsigned)(a.shares * a.nkv * a.blocks)), dim3(kSharedThreads), smem, s, a, mk, mv);
+    e = launch_pdl(kern, dim3((unsigned)(a.shares * a.nkv * a.blocks)), dim3(kSharedThreads), smem, s, a, mk, mv, mq);
     if (e != cudaSuccess) return e;
     const int rows = std::min(a.batch, 8 * sms);
     const int y = std::max(1, std::min((a.nh + 7) / 8, 8 * sms / rows));
@@ -1404,12 +1375,12 @@ cudaError_t go(const SharedArgs& a, const CUtensorMap& mk, const CUtensorMap& mv
 }
 
 template <int HD>
-cudaError_t go_hd(const SharedArgs& a, int dtype, int cache, const CUtensorMap& mk, const CUtensorMap& mv, int sms,
-                  cudaStream_t s) {
+cudaError_t go_hd(const SharedArgs& a, int dtype, int cache, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq,
+                  int sms, cudaStream_t s) {
     if (dtype == 0)
-        return cache == 1 ? go<HD, float, __half, 2, 2>(a, mk, mv, sms, s) : go<HD, float, __nv_bfloat16, 3, 3>(a, mk, mv, sms, s);
-    return cache == 1 ? go<HD, __half, __half, 1, kTerms16>(a, mk, mv, sms, s)
-                      : go<HD, __nv_bfloat16, __nv_bfloat16, 1, kTerms16>(a, mk, mv, sms, s);
+        return cache == 1 ? go<HD, float, __half, 2, 2>(a, mk, mv, mq, sms, s) : go<HD, float, __nv_bfloat16, 3, 3>(a, mk, mv, mq, sms, s);
+    return cache == 1 ? go<HD, __half, __half, 1, kTerms16>(a, mk, mv, mq, sms, s)
+                      : go<HD, __nv_bfloat16, __nv_bfloat16, 1, kTerms16>(a, mk, mv, mq, sms, s);
 }
 
 // The positions of a tensor map's box: 16, or 8, where pages are multiples of
@@ -1421,18 +1392,23 @@ int box_of(const b2_paged_kv& kv) {
     return kv.page_size % 16 == 0 ? 16 : kv.page_size % 8 == 0 ? 8 : 0;
 }
 
-// Dimensions: of a head, heads, positions of a page, pages.  A box is 64
-// dimensions (those past hd read as zero) of one head by `box` positions.
-bool make_map(CUtensorMap* m, const b2_paged_kv& kv, const void* at, int box) {
+// A map of 16-bit elements: boxes of 64 of the first dimension (those past its
+// end read as zero), b1 and b2 of the next two, in the 128-byte swizzle.
+bool make_map(CUtensorMap* m, int dtype, const void* at, const int64_t (&n)[4], const int64_t (&stride)[3], int b1, int b2) {
     const auto enc = tensor_map_encoder();
     if (!enc) return false;
-    auto stride = [](int64_t elements) { return (cuuint64_t)std::max<int64_t>(16, 2 * elements); };
-    const cuuint64_t dims[4] = {(cuuint64_t)kv.hd, (cuuint64_t)kv.nkv, (cuuint64_t)kv.page_size, (cuuint64_t)kv.n_pages};
-    const cuuint64_t strides[3] = {stride(kv.head_stride), stride(kv.pos_stride), stride(kv.page_stride)};
-    const cuuint32_t boxes[4] = {64, 1, (cuuint32_t)box, 1}, steps[4] = {1, 1, 1, 1};
-    return enc(m, kv.dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(at), dims,
+    cuuint64_t dims[4], strides[3];
+    for (int i = 0; i < 4; i++) dims[i] = (cuuint64_t)n[i];
+    for (int i = 0; i < 3; i++) strides[i] = (cuuint64_t)std::max<int64_t>(16, 2 * stride[i]);
+    const cuuint32_t boxes[4] = {64, (cuuint32_t)b1, (cuuint32_t)b2, 1}, steps[4] = {1, 1, 1, 1};
+    return enc(m, dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(at), dims,
                strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// A cache's k or v: dimensions of a head, heads, positions of a page, pages.
+bool make_map(CUtensorMap* m, const b2_paged_kv& kv, const void* at, int box) {
+    return make_map(m, kv.dtype, at, {kv.hd, kv.nkv, kv.page_size, kv.n_pages}, {kv.head_stride, kv.pos_stride, kv.page_stride}, 1, box);
 }
 
 // How a group of query heads falls to items, and the shares of the machine.
@@ -1459,15 +1435,19 @@ size_t layout(int batch, int nh, int nkv, int hd, int sms, uint8_t* base, Shared
         return p;
     };
     uint8_t* line = take(sizeof(Line));
-    uint8_t* first = take(4 * (size_t)sh.shares);
+    uint8_t* share = take(sizeof(Share) * (size_t)sh.shares);
     uint8_t* redo = take(4 * (size_t)batch);
     uint8_t* row = take(16 * (size_t)batch);
     uint8_t* item = take(2 * sizeof(Item) * (size_t)batch);
+    uint8_t* factor = take(4 * (size_t)batch * nh);
+    uint8_t* term = take((size_t)6 * batch * nh * hd);  // (three terms at most)
     uint8_t* whole = take((size_t)2 * batch * nh * (hd + 4) * 4);
     uint8_t* part = take((size_t)sh.shares * nkv * sh.blocks * 2 * kTile * (hd + 4) * 4);
     if (a) {
         a->line = reinterpret_cast<Line*>(line);
-        a->first = reinterpret_cast<int*>(first);
+        a->share = reinterpret_cast<Share*>(share);
+        a->factor = reinterpret_cast<float*>(factor);
+        a->term = reinterpret_cast<uint16_t*>(term);
         a->redo = reinterpret_cast<int*>(redo);
         a->row = reinterpret_cast<int4*>(row);
         a->item = reinterpret_cast<Item*>(item);
@@ -1533,11 +1513,19 @@ int launch_attention_shared(const b2_paged_kv& kv, const b2_paged_attn_opts& o, 
     a.out_wide = !(reinterpret_cast<uintptr_t>(out) & 15) && a.out_stride * es % 16 == 0;
     a.scale = o.scale > 0.0f ? o.scale : (float)(1.0 / sqrt((double)kv.hd));
     a.softcap = o.softcap;
+    a.terms = o.dtype == 0 ? (kv.dtype == 1 ? 2 : 3) : a.q_wide && a.q_stride < ((int64_t)1 << 38) ? 0 : 1;
     layout(batch, o.nh, kv.nkv, kv.hd, sms, static_cast<uint8_t*>(scratch), &a);
-    CUtensorMap mk{}, mv{};
+    CUtensorMap mk{}, mv{}, mq{};
+    const bool q_map = a.terms ? make_map(&mq, kv.dtype, a.term, {kv.hd, o.nh, batch, a.terms}, {kv.hd, qd, qd * batch}, a.hb, a.rows)
+                               : make_map(&mq, kv.dtype, q, {kv.hd, o.nh, batch, 1}, {kv.hd, a.q_stride, 8}, a.hb, a.rows);
+    if (!q_map) {
+        *err = "shared attention: no tensor map of q";
+        return B2_ERR_CUDA;
+    }
     a.box = box_of(kv);
     if (a.box && !(make_map(&mk, kv, kv.k, a.box) && make_map(&mv, kv, kv.v, a.box))) a.box = 0;
-    const cudaError_t e = kv.hd <= 64 ? go_hd<64>(a, o.dtype, kv.dtype, mk, mv, sms, s) : go_hd<128>(a, o.dtype, kv.dtype, mk, mv, sms, s);
+    const cudaError_t e = kv.hd <= 64 ? go_hd<64>(a, o.dtype, kv.dtype, mk, mv, mq, sms, s)
+                                      : go_hd<128>(a, o.dtype, kv.dtype, mk, mv, mq, sms, s);
     return e == cudaSuccess ? B2_OK : cuda_failed("shared attention launch", e, err);
 }
 
