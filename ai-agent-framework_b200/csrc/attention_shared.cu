@@ -59,7 +59,8 @@ constexpr int kTile = 128;       // positions of a tile, rows of a product
 constexpr int kItemUnits = 1;    // units' worth of starting an item
 constexpr int kMinShare = 3;     // a share's units, at least
 constexpr int kPlanThreads = 1024;
-constexpr int kPlanItems = 2 * kPlanThreads;  // items whose units stay in shared memory
+constexpr int kPlanItems = 2 * kPlanThreads;  // items whose units stay in shared memory,
+constexpr int kLineGroups = 2048;               // and groups
 constexpr uint64_t kSharedWaitNs = 2000000000ull;
 constexpr int kNoLimit = 0x7fffffff;
 
@@ -129,71 +130,105 @@ __device__ __forceinline__ int last_at(int n, F&& le) {
 // the line of items, by one CTA
 // ---------------------------------------------------------------------------
 
-__device__ __forceinline__ void lay_line(const SharedArgs& a) {
-    constexpr int W = kPlanThreads / 32;
-    __shared__ int v_lo[kPlanThreads + kTile], v_hi[kPlanThreads + kTile], v_tr[kPlanThreads + kTile];
-    __shared__ int owner_item[kTile + kPlanThreads];  // the item that starts at a row, also of the 128 rows before
-    __shared__ long long w_units[W], u_item[kPlanItems];
-    __shared__ int w_items[W];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, R = a.rows;
+// Rows of one turn, RPT to a thread, and the 127 behind them that its items may
+// reach into.
+template <int RPT>
+struct LineShared {
+    static constexpr int kRows = RPT * kPlanThreads;
+    int lo[kRows + kTile], hi[kRows + kTile];  // a row's positions among its group's shared ones
+    int len[kRows + kTile], tr[kRows + kTile];  // len -1: a row of NaN
+    int group[kRows + kTile];
+    int owner[kTile + kRows];                  // the item that starts at a row, also of the 128 rows before
+    int starts[kLineGroups + 1], prefix[kLineGroups];
+    long long w_units[kPlanThreads / 32], u_item[kPlanItems];
+    int w_items[kPlanThreads / 32];
+};
 
-    struct Group {
-        int start, end, prefix;  // end <= start: in none
-    };
-    auto group_of = [&](int b) {
-        const int g = last_at(a.n_groups, [&](int i) { return a.starts[i] <= b; });
-        Group r{max(a.starts[g], 0), a.starts[g + 1], max(a.prefix[g], 0)};
-        if (a.starts[g] > b || r.end <= b) r = Group{b, b, 0};
-        return r;
-    };
+template <int RPT>
+__device__ __forceinline__ void lay_line(const SharedArgs& a) {
+    using LS = LineShared<RPT>;
+    extern __shared__ __align__(16) uint8_t line_raw[];
+    LS& s = *reinterpret_cast<LS*>(line_raw);
+    constexpr int W = kPlanThreads / 32, N = LS::kRows;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, R = a.rows;
+    const bool near = a.n_groups <= kLineGroups;  // the groups are in shared memory
+    if (near) {
+        for (int i = tid; i <= a.n_groups; i += kPlanThreads) s.starts[i] = a.starts[i];
+        for (int i = tid; i < a.n_groups; i += kPlanThreads) s.prefix[i] = a.prefix[i];
+    }
+    auto start_of = [&](int g) { return near ? s.starts[g] : a.starts[g]; };
 
     int items = 0;
     long long units = 0;
-    for (int base = 0; base < a.batch; base += kPlanThreads) {
-        Group gr{0, 0, 0};
-        Seq me{};
-        for (int i = tid; i < kPlanThreads + R - 1; i += kPlanThreads) {
-            const int b = base + i;
-            int lo = 0, hi = 0, tr = 0;
-            if (b < a.batch) {
-                const Group g = group_of(b);
-                const Seq s = seq_of(a, b);
-                lo = s.lo;
-                hi = min(s.len, g.prefix);
-                tr = s.tr;
-                if (i == tid) {
-                    gr = g;
-                    me = s;
-                }
-            }
-            v_lo[i] = lo;
-            v_hi[i] = hi;
-            v_tr[i] = tr;
+    for (int base = 0; base < a.batch; base += N) {
+        Seq sq[RPT + 1];
+#pragma unroll
+        for (int u = 0; u <= RPT; u++) {  // (their words, on their way together)
+            const int i = tid + u * kPlanThreads;
+            sq[u] = Seq{};
+            if (i < N + R - 1 && base + i < a.batch) sq[u] = seq_of(a, base + i);
         }
         __syncthreads();
-        const int b = base + tid;
-        const bool in = b < a.batch;
-        Item sh{}, own{};
-        if (in && gr.end > gr.start && (b - gr.start) % R == 0) {
-            sh.row0 = b;
-            sh.rows = min(R, min(gr.end, a.batch) - b);
-            sh.lo = kNoLimit;
-            sh.tr = -1;
-            for (int r = 0; r < sh.rows; r++)
-                if (v_hi[tid + r] > v_lo[tid + r]) {
-                    if (sh.tr < 0) sh.tr = v_tr[tid + r];
-                    sh.lo = min(sh.lo, v_lo[tid + r]);
-                    sh.hi = max(sh.hi, v_hi[tid + r]);
+#pragma unroll
+        for (int u = 0; u <= RPT; u++) {
+            const int i = tid + u * kPlanThreads, b = base + i;
+            if (i >= N + R - 1) continue;
+            int g = -1, prefix = 0;
+            if (b < a.batch) {
+                g = last_at(a.n_groups, [&](int x) { return start_of(x) <= b; });
+                if (start_of(g) > b || start_of(g + 1) <= b) g = -1;
+                else prefix = max(near ? s.prefix[g] : a.prefix[g], 0);
+            }
+            s.lo[i] = sq[u].lo;
+            s.hi[i] = min(sq[u].len, prefix);
+            s.len[i] = sq[u].bad ? -1 : sq[u].len;
+            s.tr[i] = sq[u].tr;
+            s.group[i] = g;
+        }
+        __syncthreads();
+        // this thread's rows: their items and units
+        Item sh[RPT], own[RPT];
+        int n = 0, first[RPT];  // first: the row's group's first row
+        long long u = 0;
+#pragma unroll
+        for (int k = 0; k < RPT; k++) {
+            const int i = tid * RPT + k, b = base + i;
+            sh[k] = own[k] = Item{};
+            first[k] = b;
+            if (b >= a.batch) continue;
+            const int g = s.group[i];
+            int prefix = 0;
+            if (g >= 0) {
+                first[k] = max(start_of(g), 0);
+                prefix = max(near ? s.prefix[g] : a.prefix[g], 0);
+                if ((b - first[k]) % R == 0) {
+                    Item x{};
+                    x.row0 = b;
+                    x.rows = min(R, min(start_of(g + 1), a.batch) - b);
+                    x.lo = kNoLimit;
+                    x.tr = -1;
+                    x.limit = prefix;
+#pragma unroll 4
+                    for (int r = 0; r < x.rows; r++)
+                        if (s.hi[i + r] > s.lo[i + r]) {
+                            if (x.tr < 0) x.tr = s.tr[i + r];
+                            x.lo = min(x.lo, s.lo[i + r]);
+                            x.hi = max(x.hi, s.hi[i + r]);
+                        }
+                    sh[k] = x;
                 }
-            sh.limit = gr.prefix;
-        }
-        if (in) {
-            own = Item{0, b, 1, max(me.lo, gr.prefix), me.len, me.tr, kNoLimit};
+            }
+            own[k] = Item{0, b, 1, max(s.lo[i], prefix), max(s.len[i], 0), s.tr[i], kNoLimit};
             a.redo[b] = 0;
+            if (sh[k].hi > sh[k].lo) {
+                n++;
+                u += tiles_of(sh[k]) + kItemUnits;
+            }
+            if (own[k].hi > own[k].lo) {
+                n++;
+                u += tiles_of(own[k]) + kItemUnits;
+            }
         }
-        const bool has_sh = sh.hi > sh.lo, has_own = own.hi > own.lo;
-        const int n = has_sh + has_own;
-        const int u_sh = has_sh ? tiles_of(sh) + kItemUnits : 0, u = u_sh + (has_own ? tiles_of(own) + kItemUnits : 0);
         int ni = n;
         long long nu = u;
 #pragma unroll
@@ -206,57 +241,67 @@ __device__ __forceinline__ void lay_line(const SharedArgs& a) {
             }
         }
         if (lane == 31) {
-            w_items[warp] = ni;
-            w_units[warp] = nu;
+            s.w_items[warp] = ni;
+            s.w_units[warp] = nu;
         }
-        if (tid < kTile) owner_item[tid] = base ? owner_item[kPlanThreads + tid] : -1;
+        if (tid < kTile) s.owner[tid] = base ? s.owner[N + tid] : -1;
         __syncthreads();
-        int at = items + ni - n;
-        long long u0 = units + nu - u;
-#pragma unroll 4
-        for (int w = 0; w < W; w++) {
-            if (w < warp) {
-                at += w_items[w];
-                u0 += w_units[w];
+        // the warps before this one, and all of them: a scan by every warp
+        int wi = lane < W ? s.w_items[lane] : 0;
+        long long wu = lane < W ? s.w_units[lane] : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, wi, o);
+            const long long y = __shfl_up_sync(0xffffffffu, wu, o);
+            if (lane >= o) {
+                wi += x;
+                wu += y;
             }
-            items += w_items[w];
-            units += w_units[w];
         }
-        const int i_sh = has_sh ? at : -1, i_own = has_own ? at + has_sh : -1;
-        owner_item[kTile + tid] = i_sh;
-        if (has_sh) {
-            sh.u0 = u0;
-            a.item[i_sh] = sh;
-            if (i_sh < kPlanItems) u_item[i_sh] = u0;
-        }
-        if (has_own) {
-            own.u0 = u0 + u_sh;
-            a.item[i_own] = own;
-            if (i_own < kPlanItems) u_item[i_own] = own.u0;
+        int at = items + ni - n + (warp ? __shfl_sync(0xffffffffu, wi, max(warp - 1, 0)) : 0);
+        long long u0 = units + nu - u + (warp ? __shfl_sync(0xffffffffu, wu, max(warp - 1, 0)) : 0);
+        items += __shfl_sync(0xffffffffu, wi, 31);
+        units += __shfl_sync(0xffffffffu, wu, 31);
+        int i_own[RPT];
+        auto put = [&](Item& x) {
+            if (x.hi <= x.lo) return -1;
+            x.u0 = u0;
+            u0 += tiles_of(x) + kItemUnits;
+            a.item[at] = x;
+            if (at < kPlanItems) s.u_item[at] = x.u0;
+            return at++;
+        };
+#pragma unroll
+        for (int k = 0; k < RPT; k++) {
+            s.owner[kTile + tid * RPT + k] = put(sh[k]);
+            i_own[k] = put(own[k]);
         }
         __syncthreads();
-        if (in) {
+#pragma unroll
+        for (int k = 0; k < RPT; k++) {
+            const int i = tid * RPT + k, b = base + i;
+            if (b >= a.batch) continue;
             int mine = -1;
-            if (v_hi[tid] > v_lo[tid]) {  // (the item starts at most 127 rows before)
-                const int o = gr.start + (b - gr.start) / R * R - base + kTile;
-                mine = o >= 0 ? owner_item[o] : -1;
+            if (s.hi[i] > s.lo[i]) {  // (the item starts at most 127 rows before)
+                const int o = first[k] + (b - first[k]) / R * R - base + kTile;
+                mine = o >= 0 ? s.owner[o] : -1;
             }
-            a.row[b] = me.bad ? make_int4(0, 0, -2, -2) : make_int4(me.lo, me.len, mine, i_own);
+            a.row[b] = s.len[i] < 0 ? make_int4(0, 0, -2, -2) : make_int4(s.lo[i], s.len[i], mine, i_own[k]);
         }
         __syncthreads();
     }
     const int G = (int)max(1LL, min((long long)a.shares, units / kMinShare));
     if (tid == 0) *a.line = Line{units, items, G};
     if (units == 0) {
-        for (int s = tid; s < a.shares; s += kPlanThreads) a.share[s] = Share{0, 0, 0};
+        for (int i = tid; i < a.shares; i += kPlanThreads) a.share[i] = Share{0, 0, 0};
         return;
     }
-    for (int s = G + tid; s < a.shares; s += kPlanThreads) a.share[s] = Share{0, 0, 0};
-    for (int s = tid; s < G; s += kPlanThreads) {
-        const long long u = mul_div(s, units, G);
-        const int i = last_at(items, [&](int x) { return (items <= kPlanItems ? u_item[x] : a.item[x].u0) <= u; });
-        const long long at = u - (items <= kPlanItems ? u_item[i] : a.item[i].u0);
-        a.share[s] = Share{i, (int)at, mul_div(s + 1, units, G) - u};
+    for (int i = G + tid; i < a.shares; i += kPlanThreads) a.share[i] = Share{0, 0, 0};
+    for (int h = tid; h < G; h += kPlanThreads) {
+        const long long u = mul_div(h, units, G);
+        const int i = last_at(items, [&](int x) { return (items <= kPlanItems ? s.u_item[x] : a.item[x].u0) <= u; });
+        const long long at = u - (items <= kPlanItems ? s.u_item[i] : a.item[i].u0);
+        a.share[h] = Share{i, (int)at, mul_div(h + 1, units, G) - u};
     }
 }
 
@@ -322,11 +367,11 @@ __device__ __forceinline__ void make_terms(const SharedArgs& a, long long first,
 }
 
 // The first launch: the line by one CTA, Q's terms by the others.
-template <typename T, typename C, int QT>
+template <typename T, typename C, int QT, int RPT>
 __global__ void __launch_bounds__(kPlanThreads) shared_line_kernel(const __grid_constant__ SharedArgs a) {
     pdl_trigger();
     pdl_wait();
-    if (blockIdx.x == 0) lay_line(a);
+    if (blockIdx.x == 0) lay_line<RPT>(a);
     else make_terms<T, C, QT>(a, (blockIdx.x - 1) * (kPlanThreads / 32) + threadIdx.x / 32, (gridDim.x - 1) * (kPlanThreads / 32));
 }
 
@@ -1265,76 +1310,92 @@ __device__ __noinline__ Sum row_alone(const SharedArgs& a, int b, int head) {
     return r;
 }
 
-// CTAs (rows in turn, heads in turn), a warp for a head.
+// CTAs (rows in turn, heads in turn): which of its rows there is something to
+// join of, a row to a thread; then a warp for each of their heads.
 template <typename T, typename C>
 __global__ void __launch_bounds__(kSharedJoinThreads) shared_join_kernel(const __grid_constant__ SharedArgs a) {
+    struct Todo {
+        int b, kind;               // kind: 0 pieces, 1 by itself, 2 NaN
+        int first[2], last[2], base[2];  // the shares of its items, its place among the item's (row, head) pairs
+    };
+    __shared__ Todo todo[kSharedJoinThreads];
+    __shared__ int n_todo;
+    constexpr int kWarps = kSharedJoinThreads / 32;
     pdl_trigger();
     pdl_wait();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hd = a.hd, d = 4 * lane;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hd = a.hd, d = 4 * lane;
     const Line line = *a.line;
     const int64_t width = hd + 4;
-    for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
-        const int4 row = a.row[b];
-        const int redo = a.redo[b];
-        // the shares of the row's items
-        struct Part {
-            int first, last, base;  // base: the row's place among the item's (row, head) pairs
-        } part[2];
-        bool cut = false;
+    const int mine = (a.batch - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;  // rows of this CTA
+#pragma unroll 1
+    for (int r0 = 0; r0 < mine; r0 += kSharedJoinThreads) {
+        if (tid == 0) n_todo = 0;
+        __syncthreads();
+        if (r0 + tid < mine) {
+            Todo t{};
+            t.b = (int)(blockIdx.x + (int64_t)(r0 + tid) * gridDim.x);
+            const int4 row = a.row[t.b];
+            const int redo = a.redo[t.b];
+            bool cut = false;
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
-            const int i = k ? row.w : row.z;
-            part[k] = Part{0, -1, 0};
-            if (i < 0) continue;
-            const Item it = a.item[i];
-            const long long u = it.u0 + kItemUnits;
-            part[k].first = (int)mul_div(u + 1, line.shares, line.units, -1);
-            part[k].last = (int)mul_div(u + tiles_of(it), line.shares, line.units, -1);
-            part[k].base = (b - it.row0) * a.hb;
-            cut |= part[k].first != part[k].last;
+            for (int k = 0; k < 2; k++) {
+                const int i = k ? row.w : row.z;
+                t.last[k] = -1;
+                if (i < 0) continue;
+                const Item it = a.item[i];
+                const long long u = it.u0 + kItemUnits;
+                t.first[k] = (int)mul_div(u + 1, line.shares, line.units, -1);
+                t.last[k] = (int)mul_div(u + tiles_of(it), line.shares, line.units, -1);
+                t.base[k] = (t.b - it.row0) * a.hb;
+                cut |= t.first[k] != t.last[k];
+            }
+            t.kind = row.z == -2 ? 2 : redo ? 1 : 0;
+            // (a row of one item that was not cut is written already)
+            if (t.kind || cut || (row.z >= 0) == (row.w >= 0)) todo[atomicAdd(&n_todo, 1)] = t;
         }
-        const bool one = (row.z >= 0) != (row.w >= 0);
-        if (one && !cut && !redo) continue;  // written already
-        for (int head = blockIdx.y * (kSharedJoinThreads / 32) + warp; head < a.nh;
-             head += gridDim.y * (kSharedJoinThreads / 32)) {
+        __syncthreads();
+        const int heads = (a.nh + (int)gridDim.y - 1) / (int)gridDim.y, h0 = blockIdx.y * heads, h1 = min(a.nh, h0 + heads);
+#pragma unroll 1
+        for (int x = warp; x < n_todo * heads; x += kWarps) {
+            const int e = x / heads, head = h0 + x - e * heads;
+            if (head >= h1) continue;
+            const Todo t = todo[e];
             Sum r{make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
-            if (row.z == -2) {
-                r.L = __int_as_float(0x7fc00000);
-            } else if (!redo) {
+            bool alone = t.kind == 1;
+            if (t.kind == 0) {
                 const int h = head / a.grp, in = head - h * a.grp, blk = in / a.hb, hh = in - blk * a.hb;
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
-                    const Part pt = part[k];
                     constexpr int N = 4;  // pieces in flight
-                    for (int i0 = pt.first; i0 <= pt.last; i0 += N) {
-                        float4 x[N];
+                    for (int i0 = t.first[k]; i0 <= t.last[k]; i0 += N) {
+                        float4 v[N];
                         float2 ml[N];
 #pragma unroll
                         for (int n = 0; n < N; n++) {
                             const int i = i0 + n;
                             const float* from =
-                                pt.first == pt.last
-                                    ? a.whole + (((int64_t)k * a.batch + b) * a.nh + head) * width
-                                    : a.part + (((int64_t)(i * a.nkv * a.blocks + h * a.blocks + blk) * 2 + (i == pt.first ? 1 : 0)) * kTile +
-                                                pt.base + hh) * width;
-                            x[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                                t.first[k] == t.last[k]
+                                    ? a.whole + (((int64_t)k * a.batch + t.b) * a.nh + head) * width
+                                    : a.part + (((int64_t)(i * a.nkv * a.blocks + h * a.blocks + blk) * 2 + (i == t.first[k] ? 1 : 0)) * kTile +
+                                                t.base[k] + hh) * width;
+                            v[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                             ml[n] = make_float2(-INFINITY, 0.0f);
-                            if (i <= pt.last) {
+                            if (i <= t.last[k]) {
                                 ml[n] = *reinterpret_cast<const float2*>(from + hd);
-                                if (d < hd) x[n] = *reinterpret_cast<const float4*>(from + d);
+                                if (d < hd) v[n] = *reinterpret_cast<const float4*>(from + d);
                             }
                         }
 #pragma unroll
-                        for (int n = 0; n < N; n++) r.add(x[n], ml[n].x, ml[n].y);
+                        for (int n = 0; n < N; n++) r.add(v[n], ml[n].x, ml[n].y);
                     }
                 }
-                const float t = r.L == 0.0f ? 0.0f : (r.o.x + r.o.y + r.o.z + r.o.w) / r.L;
-                if (__any_sync(0xffffffffu, d < hd && t - t != 0.0f)) r = row_alone<T, C>(a, b, head);
-            } else {
-                r = row_alone<T, C>(a, b, head);
+                const float f = r.L == 0.0f ? 0.0f : (r.o.x + r.o.y + r.o.z + r.o.w) / r.L;
+                alone = __any_sync(0xffffffffu, d < hd && f - f != 0.0f);
             }
+            if (alone) r = row_alone<T, C>(a, t.b, head);
+            if (t.kind == 2) r.L = __int_as_float(0x7fc00000);
             const float inv = r.L == 0.0f ? 0.0f : 1.0f / r.L;
-            T* out = static_cast<T*>(a.out) + (int64_t)b * a.out_stride + (int64_t)head * hd;
+            T* out = static_cast<T*>(a.out) + (int64_t)t.b * a.out_stride + (int64_t)head * hd;
             if (d < hd) {
                 out[d] = (T)(r.o.x * inv);
                 out[d + 1] = (T)(r.o.y * inv);
@@ -1342,13 +1403,19 @@ __global__ void __launch_bounds__(kSharedJoinThreads) shared_join_kernel(const _
                 out[d + 3] = (T)(r.o.w * inv);
             }
             if (a.lse && lane == 0)
-                a.lse[(int64_t)b * a.nh + head] = r.L == 0.0f ? -INFINITY : (r.M + (log2f(r.L) - 14.0f)) * kLn2;
+                a.lse[(int64_t)t.b * a.nh + head] = r.L == 0.0f ? -INFINITY : (r.M + (log2f(r.L) - 14.0f)) * kLn2;
         }
+        __syncthreads();
     }
 }
 
 constexpr int kMaxSharedDevices = 64;
 constexpr int kTerms16 = 1;  // terms of the probabilities of 16-bit rows
+
+cudaError_t launch_line(void (*kern)(SharedArgs), int smem, int ctas, const SharedArgs& a, cudaStream_t s) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    return e == cudaSuccess ? launch_pdl(kern, dim3(ctas), dim3(kPlanThreads), smem, s, a) : e;
+}
 
 template <int HD, typename T, typename C, int QT, int PT>
 cudaError_t go(const SharedArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, int sms, cudaStream_t s) {
@@ -1365,12 +1432,17 @@ cudaError_t go(const SharedArgs& a, const CUtensorMap& mk, const CUtensorMap& mv
     }
     const long long q_rows = a.terms ? (long long)a.batch * a.nh : 0;  // (a warp takes four at a time)
     const int ctas = 1 + (int)std::min<long long>(2 * sms - 1, (q_rows + kPlanThreads / 8 - 1) / (kPlanThreads / 8));
-    e = launch_pdl(shared_line_kernel<T, C, QT>, dim3(ctas), dim3(kPlanThreads), 0, s, a);
+    // (a row to a thread; four where there are more: 2048 rows 9 us, 14 in two turns)
+    if (a.batch <= kPlanThreads) {
+        e = launch_line(shared_line_kernel<T, C, QT, 1>, (int)sizeof(LineShared<1>), ctas, a, s);
+    } else {
+        e = launch_line(shared_line_kernel<T, C, QT, 4>, (int)sizeof(LineShared<4>), ctas, a, s);
+    }
     if (e != cudaSuccess) return e;
     e = launch_pdl(kern, dim3((unsigned)(a.shares * a.nkv * a.blocks)), dim3(kSharedThreads), smem, s, a, mk, mv, mq);
     if (e != cudaSuccess) return e;
-    const int rows = std::min(a.batch, 8 * sms);
-    const int y = std::max(1, std::min((a.nh + 7) / 8, 8 * sms / rows));
+    const int rows = std::min(a.batch, 4 * sms);
+    const int y = std::max(1, std::min((a.nh + 7) / 8, 16 * sms / rows));
     return launch_pdl(shared_join_kernel<T, C>, dim3(rows, y), dim3(kSharedJoinThreads), 0, s, a);
 }
 
