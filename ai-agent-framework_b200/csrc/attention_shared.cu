@@ -75,6 +75,7 @@ static_assert(sizeof(Item) == 32, "two 16-byte loads");
 struct Line {
     long long units;
     int items, shares;
+    int dead;  // a wait of the tiles' launch gave up: every row becomes NaN
 };
 
 // Where a share starts: item, its unit, units of the share.
@@ -97,6 +98,7 @@ struct SharedArgs {
     int q_wide, out_wide;  // 16-byte accesses
     int terms;             // of Q that the first launch makes; 0: the products read q as it is
     int box;               // positions of a box of the tensor maps (16 or 8); 0: pages that they cannot tell
+    int flat;              // pages follow one another as their positions do: one dimension
     float scale, softcap;
     // scratch
     Line* line;
@@ -291,7 +293,7 @@ __device__ __forceinline__ void lay_line(const SharedArgs& a) {
         __syncthreads();
     }
     const int G = (int)max(1LL, min((long long)a.shares, units / kMinShare));
-    if (tid == 0) *a.line = Line{units, items, G};
+    if (tid == 0) *a.line = Line{units, items, G, 0};
     if (units == 0) {
         for (int i = tid; i < a.shares; i += kPlanThreads) a.share[i] = Share{0, 0, 0};
         return;
@@ -397,11 +399,12 @@ struct Tm {
     static constexpr int kFixed = 1024 + 15360;  // alignment, then barriers and small tables
     static constexpr int kFit = (kSharedSmemMax - kFixed - kQ) / kTileBytes;
     static constexpr int kStages = kFit > 8 ? 8 : kFit;
-    static constexpr int kStagesK = (kStages + 1) / 2, kStagesV = kStages / 2;
+    // V's tiles share the barriers of the two P that they are multiplied with
+    static constexpr int kStagesV = kStages >= 4 ? 2 : 1, kStagesK = kStages - kStagesV > 4 ? 4 : kStages - kStagesV;
     // copies that a copying thread leaves in flight behind the one it has just issued
-    static constexpr int kAhead = kStages > 4 ? 4 : kStages - 2;
+    static constexpr int kAhead = kStages - 2 > 4 ? 4 : kStages - 2;
     static_assert(kStages >= 3, "three tiles must fit");
-    static constexpr int kTotal = kFixed + kQ + kStages * kTileBytes;
+    static constexpr int kTotal = kFixed + kQ + (kStagesK + kStagesV) * kTileBytes;
     // tensor memory: two S (P over it, a third term behind it), then T
     static constexpr int kSCols = PT == 3 ? 192 : 128;
     static constexpr int kTBufs = 2 * kSCols + 2 * HD <= 512 ? 2 : 1;
@@ -417,7 +420,10 @@ struct Piece {
 constexpr int kPieceStart = 1, kPieceWhole = 2, kPieceOwn = 4, kPieceLast = 8;  // kPieceLast: no piece, the share is done
 
 struct SmallShared {
-    uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], q_full[2], q_empty[2], s_full[2], p_full[2], t_full[2], t_empty[2];
+    uint64_t k_full[4], k_empty[4], q_full[2], q_empty[2];
+    uint64_t s_full[2];  // S of tiles j, j + 1 (and where there are two K, their places are free)
+    uint64_t ready[2];   // their P, V and a place for T
+    uint64_t t_full[2];  // their T (and V's places are free)
     uint64_t piece_full[kPieces], piece_empty[kPieces];
     uint32_t tmem;
     int dead;                    // a wait gave up
@@ -565,12 +571,12 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
     shared_tiles_kernel(const __grid_constant__ SharedArgs a, const __grid_constant__ CUtensorMap map_k,
                         const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_q) {
     using TM = Tm<HD, QT, PT>;
-    constexpr int NS = TM::kStages, NK = TM::kStagesK, NV = TM::kStagesV, NT = TM::kTBufs, QB = TM::kQBufs;
+    constexpr int NK = TM::kStagesK, NV = TM::kStagesV, NT = TM::kTBufs, QB = TM::kQBufs;
     extern __shared__ __align__(1024) uint8_t ssm_raw[];
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ssm_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* const q_sm = base;
     uint8_t* const ring = base + TM::kQ;
-    SmallShared& s = *reinterpret_cast<SmallShared*>(ring + NS * TM::kTileBytes);
+    SmallShared& s = *reinterpret_cast<SmallShared*>(ring + (NK + NV) * TM::kTileBytes);
     volatile int* dead = &s.dead;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -581,19 +587,17 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
     const int hd = a.hd;
 
     if (tid == 0) {
+        const int copies = a.box ? 1 : kCopyWarps;
         for (int i = 0; i < 4; i++) {
-            mbar_init(&s.k_full[i], a.box ? 1 : kCopyWarps);
-            mbar_init(&s.v_full[i], a.box ? 1 : kCopyWarps);
+            mbar_init(&s.k_full[i], copies);
             mbar_init(&s.k_empty[i], 1);
-            mbar_init(&s.v_empty[i], 1);
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&s.q_full[i], 1);
             mbar_init(&s.q_empty[i], 1);
             mbar_init(&s.s_full[i], 1);
-            mbar_init(&s.p_full[i], 4);
+            mbar_init(&s.ready[i], 4 + kSumWarps + copies);
             mbar_init(&s.t_full[i], 1);
-            mbar_init(&s.t_empty[i], kSumWarps);
         }
         for (int i = 0; i < kPieces; i++) {
             mbar_init(&s.piece_full[i], 1);
@@ -609,7 +613,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
     }
     // columns past hd stay zero: the copies never write them
     if (hd < HD) {
-        for (int i = tid; i < (TM::kQ + NS * TM::kTileBytes) / 16; i += kSharedThreads)
+        for (int i = tid; i < (TM::kQ + (NK + NV) * TM::kTileBytes) / 16; i += kSharedThreads)
             *reinterpret_cast<uint4*>(base + 16 * i) = make_uint4(0, 0, 0, 0);
         fence_proxy_async();
     }
@@ -735,7 +739,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&s.p_full[wg]);
+                if (lane == 0) mbar_arrive(&s.ready[wg]);
             }
             if (!ok) break;
             pieces.done(s);
@@ -747,6 +751,8 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
         const uint32_t t_col = tmem + ((uint32_t)(quad * 32) << 16) + 2 * TM::kSCols + half * HC;
         const int rr = m / a.hb, head = head0 + m - rr * a.hb;
         const int d0 = half * HC, dn = min(HC, hd - d0);  // this warp's dimensions
+        if (lane == 0)  // (T's places are free)
+            for (int i = 0; i < NT; i++) mbar_arrive(&s.ready[i]);
         int j = 0;
         bool ok = true;
         Pieces pieces;
@@ -761,7 +767,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
 #pragma unroll 1
             for (int t = p->t0; t < t1; t++, j++) {
                 const int buf = j % NT;
-                ok = ok && warp_wait(&s.t_full[buf], (j / NT) & 1, dead);
+                ok = ok && warp_wait(&s.t_full[j & 1], (j >> 1) & 1, dead);
                 if (!ok) continue;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if (busy) {
@@ -785,9 +791,8 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&s.t_empty[buf]);
+                if (lane == 0) mbar_arrive(&s.ready[(j + NT) & 1]);
             }
-            if (!ok) L = __int_as_float(0x7fc00000);  // (a wait gave up: no result)
             const int b = p->row0 + rr, kind = p->kind;
             pieces.done(s);
             if (!row.w || dn <= 0) continue;
@@ -862,8 +867,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                 const uint16_t* src = value ? a.v : a.k;
                 const int slots = value ? NV : NK;
                 const uint32_t ring_s = value ? ring_v : ring_k;
-                uint64_t *full = value ? s.v_full : s.k_full, *empty = value ? s.v_empty : s.k_empty;
-                int slot = 0, lap = 0;
+                int slot = 0;
                 struct Tile {
                     int page, pos, lo, hi;  // this lane's group: page, first position; the tile's seen rows
                 };
@@ -879,6 +883,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                     return f;
                 };
                 constexpr int BL = HD / 64;  // boxes of a group
+                const uint32_t all = (1u << groups) - 1;
                 Tile nx{};
                 if (p) nx = look(p, t);
 #pragma unroll 1
@@ -893,13 +898,15 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                     const int r0 = lane * G, in = place(f.pos);
                     const bool there = (unsigned)f.page < (unsigned)a.n_pages;
                     const bool whole = lane < groups && there && r0 >= f.lo && r0 + G <= f.hi;
+                    const int where = a.flat ? f.page * a.page_size + in : in;
                     const uint32_t by_box = __ballot_sync(0xffffffffu, whole);
-                    uint32_t rest = __ballot_sync(0xffffffffu, lane < groups && !whole && r0 < ((f.hi + kGroup - 1) & ~(kGroup - 1)));
+                    uint32_t rest = 0;
+                    if (by_box != all) rest = __ballot_sync(0xffffffffu, lane < groups && !whole && r0 < ((f.hi + kGroup - 1) & ~(kGroup - 1)));
                     if (!value) {  // positions seen whose page is not there
-                        const int lo = max(f.lo, r0), hi = min(f.hi, r0 + G);
-                        const bool gone = lane < groups && lo < hi && !there;
                         uint32_t bits = 0;
-                        if (rest && __any_sync(0xffffffffu, gone)) {
+                        if (rest) {
+                            const int lo = max(f.lo, r0), hi = min(f.hi, r0 + G);
+                            const bool gone = lane < groups && lo < hi && !there;
                             const uint32_t mine = gone ? ((1u << (hi - lo)) - 1) << (lo & 31) : 0;
 #pragma unroll
                             for (int i = 0; i < 4; i++) {
@@ -909,21 +916,26 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                         }
                         if (lane < 4) s.bad[j & 7][lane] = bits;
                     }
-                    if (lap) ok = ok && warp_wait(&empty[slot], (lap - 1) & 1, dead);
+                    // the tile's place is free once the one before in it was multiplied
+                    const int was = j - slots;
+                    if (was >= 0)
+                        ok = ok && (value      ? warp_wait(&s.t_full[was & 1], (was >> 1) & 1, dead)
+                                    : NK == 2 ? warp_wait(&s.s_full[was & 1], (was >> 1) & 1, dead)
+                                              : warp_wait(&s.k_empty[slot], (was / NK) & 1, dead));
                     if (!ok) break;
-                    uint64_t* bar = &full[slot];
-                    const uint32_t to = ring_s + slot * TM::kTileBytes;
-                    if (lane == 0) {
+                    uint64_t* bar = value ? &s.ready[j & 1] : &s.k_full[slot];
+                    const uint32_t to = __shfl_sync(0xffffffffu, ring_s + slot * TM::kTileBytes, 0);
+                    const bool one = elected();
+                    if (one) {
                         const uint32_t bytes = __popc(by_box) * G * 128 * BL;
                         if (rest) mbar_expect_tx(bar, bytes);
                         else mbar_arrive_expect_tx(bar, bytes);
                     }
-                    __syncwarp();
-                    const bool one = elected();
                     for (int g0 = 0; g0 < groups; g0 += 8)
 #pragma unroll
                         for (int i = 0; i < 8; i++) {  // (uniform over the warp)
-                            const int g = g0 + i, page = __shfl_sync(0xffffffffu, f.page, g), at = __shfl_sync(0xffffffffu, in, g);
+                            const int g = g0 + i, at = __shfl_sync(0xffffffffu, where, g);
+                            const int page = a.flat ? 0 : __shfl_sync(0xffffffffu, f.page, g);
                             if ((by_box >> g) & 1 && one) {
 #pragma unroll
                                 for (int x = 0; x < BL; x++) tma_rows(to + x * (kTile * 128) + g * G * 128, map, 64 * x, h, at, page, bar);
@@ -951,10 +963,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                         __syncwarp();
                         if (lane == 0) mbar_arrive(bar);
                     }
-                    if (++slot == slots) {
-                        slot = 0;
-                        lap++;
-                    }
+                    if (++slot == slots) slot = 0;
                     j++;
                 }
             } else {
@@ -974,7 +983,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                     for (; waiting > leave; waiting--) {
                         const bool v = (kinds >> (waiting - 1)) & 1;
                         const int n = v ? told[1]++ : told[0]++;
-                        if (lane == 0) mbar_arrive(v ? &s.v_full[n % NV] : &s.k_full[n % NK]);
+                        if (lane == 0) mbar_arrive(v ? &s.ready[n & 1] : &s.k_full[n % NK]);
                     }
                 };
                 // this lane's rows of a tile: their offset; -1: none there; -2: nor needed
@@ -998,8 +1007,16 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                     return f;
                 };
                 auto issue = [&](const uint16_t* src, const Place& f, bool value) {
-                    const int n = value ? issued[1]++ : issued[0]++, slots = value ? NV : NK, slot = n % slots;
-                    if (n >= slots) ok = ok && warp_wait(value ? &s.v_empty[slot] : &s.k_empty[slot], (n / slots - 1) & 1, dead);
+                    const int n = value ? issued[1]++ : issued[0]++, slots = value ? NV : NK, slot = n % slots, was = n - slots;
+                    if (was >= 0) {
+                        uint64_t* bar = value ? &s.t_full[was & 1] : NK == 2 ? &s.s_full[was & 1] : &s.k_empty[slot];
+                        const uint32_t parity = (value || NK == 2 ? was >> 1 : was / NK) & 1;
+                        if (!__all_sync(0xffffffffu, phase_over(bar, parity))) {
+                            cp_wait<0>();  // (what frees it may wait for what is on its way)
+                            tell(0);
+                            ok = ok && warp_wait(bar, parity, dead);
+                        }
+                    }
                     if (!ok) return;
                     const uint32_t to = at0 + (slot + (value ? NK : 0)) * TM::kTileBytes;
                     constexpr int U = 4;  // copies whose places are worked out together
@@ -1152,35 +1169,41 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
             const uint32_t hi_v = (uint32_t)(v_desc(0) >> 32), lo_v = (uint32_t)v_desc(0);
             const int ks = (hd + 15) / 16;
             const uint32_t id_v = uniform(idesc<C>(ks * 16, true)), id_k = uniform(idesc<C>(0, false));
+            const uint32_t tm = uniform(tmem);
             int j = 0, was = 0;  // was: positions of the tile before, in 16s
-            int k_slot = 0, k_lap = 0, v_slot = 0, v_lap = 0;
-            bool ok = true;
-            auto values = [&](int jj) {  // T = P V of tile jj
-                ok = ok && warp_wait(&s.p_full[jj & 1], (jj >> 1) & 1, dead);
-                ok = ok && warp_wait(&s.v_full[v_slot], v_lap & 1, dead);
-                if (jj >= NT) ok = ok && warp_wait(&s.t_empty[jj % NT], (jj / NT - 1) & 1, dead);
+            int k_slot = 0, k_lap = 0;
+            bool ok = true, k_there = false;  // k_there: the next tile's K was waited for
+            auto values = [&](int jj, bool more) {  // T = P V of tile jj
+                // (K first: it is there as a rule, and every wait takes its time)
+                if (more) ok = ok && warp_wait(&s.k_full[k_slot], k_lap & 1, dead);
+                k_there = more;
+                ok = ok && warp_wait(&s.ready[jj & 1], (jj >> 1) & 1, dead);
                 if (!ok) return;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t v = uniform(lo_v + ring_v + v_slot * (TM::kTileBytes >> 4));
-                const uint32_t pc = uniform(tmem + (jj & 1) * TM::kSCols), tc = uniform(tmem + 2 * TM::kSCols + (jj % NT) * HD);
-                const int n = (int)uniform(was);
+                const uint32_t b = uniform(jj & 1), n = uniform(was);
+                const uint32_t v = lo_v + ring_v + (NV == 2 ? b : 0) * (TM::kTileBytes >> 4);
+                const uint32_t pc = tm + b * TM::kSCols, tc = tm + 2 * TM::kSCols + (NT == 2 ? b : 0) * HD;
                 if (elected()) {
+                    if (n == kTile / 16) {
 #pragma unroll
-                    for (int x = PT - 1; x >= 0; x--)  // (small terms first)
+                        for (int x = PT - 1; x >= 0; x--)  // (small terms first)
 #pragma unroll
-                        for (int k = 0; k < kTile / 16; k++) {
-                            if (k == n) break;
-                            mma_f16_ts(tc, pc + (x == 2 ? 128 + 8 * k : 16 * k + 8 * x),
-                                       desc_of(v + k * (2048 >> 4), hi_v), id_v, x < PT - 1 || k > 0);
-                        }
-                    mma_commit(&s.v_empty[v_slot]);
-                    mma_commit(&s.t_full[jj % NT]);
+                            for (int k = 0; k < kTile / 16; k++)
+                                mma_f16_ts(tc, pc + (x == 2 ? 128 + 8 * k : 16 * k + 8 * x), desc_of(v + k * (2048 >> 4), hi_v), id_v,
+                                           x < PT - 1 || k > 0);
+                    } else {
+                        uint32_t acc = 0;
+#pragma unroll 1
+                        for (int x = PT - 1; x >= 0; x--)
+#pragma unroll 1
+                            for (uint32_t k = 0; k < n; k++) {
+                                mma_f16_ts(tc, pc + (x == 2 ? 128 + 8 * k : 16 * k + 8 * x), desc_of(v + k * (2048 >> 4), hi_v), id_v, acc);
+                                acc = 1;
+                            }
+                    }
+                    mma_commit(&s.t_full[jj & 1]);
                 }
                 __syncwarp();
-                if (++v_slot == NV) {
-                    v_slot = 0;
-                    v_lap++;
-                }
             };
             Pieces pieces;
             while (const Piece* p = pieces.next(s)) {
@@ -1191,23 +1214,34 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
 #pragma unroll 1
                 for (int t = t0; t < t1 && ok; t++, j++) {
                     const int n16 = (min(kTile, hi - (start + t * kTile)) + 15) / 16;
-                    ok = ok && warp_wait(&s.k_full[k_slot], k_lap & 1, dead);
+                    if (!k_there) ok = ok && warp_wait(&s.k_full[k_slot], k_lap & 1, dead);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t k_sm = uniform(lo_k + ring_k + k_slot * (TM::kTileBytes >> 4));
-                    const uint32_t sc = uniform(tmem + (j & 1) * TM::kSCols), id = uniform(id_k | (uint32_t)(2 * n16) << 17);
+                    const uint32_t b = uniform(j & 1), ksl = NK == 2 ? b : uniform(k_slot), id = uniform(id_k | (uint32_t)(2 * n16) << 17);
+                    const uint32_t k_sm = lo_k + ring_k + ksl * (TM::kTileBytes >> 4), sc = tm + b * TM::kSCols;
                     if (elected()) {
+                        if (ks == HD / 16) {
 #pragma unroll
-                        for (int x = QT - 1; x >= 0; x--)
+                            for (int x = QT - 1; x >= 0; x--)
 #pragma unroll
-                            for (int k = 0; k < HD / 16; k++) {
-                                if (k == ks) break;
-                                const uint32_t in = (uint32_t)(k >> 2) * ((kTile * 128) >> 4) + (k & 3) * 2;
-                                mma_f16(sc, desc_of(q + x * (TM::kTileBytes >> 4) + in, hi_k), desc_of(k_sm + in, hi_k), id,
-                                        x < QT - 1 || k > 0);
-                            }
-                        mma_commit(&s.k_empty[k_slot]);
+                                for (int k = 0; k < HD / 16; k++) {
+                                    const uint32_t in = (uint32_t)(k >> 2) * ((kTile * 128) >> 4) + (k & 3) * 2;
+                                    mma_f16(sc, desc_of(q + x * (TM::kTileBytes >> 4) + in, hi_k), desc_of(k_sm + in, hi_k), id,
+                                            x < QT - 1 || k > 0);
+                                }
+                        } else {
+                            uint32_t acc = 0;
+#pragma unroll 1
+                            for (int x = QT - 1; x >= 0; x--)
+#pragma unroll 1
+                                for (int k = 0; k < ks; k++) {
+                                    const uint32_t in = (uint32_t)(k >> 2) * ((kTile * 128) >> 4) + (k & 3) * 2;
+                                    mma_f16(sc, desc_of(q + x * (TM::kTileBytes >> 4) + in, hi_k), desc_of(k_sm + in, hi_k), id, acc);
+                                    acc = 1;
+                                }
+                        }
                         mma_commit(&s.s_full[j & 1]);
+                        if (NK != 2) mma_commit(&s.k_empty[k_slot]);
                         if (t == t1 - 1) mma_commit(&s.q_empty[n % QB]);
                     }
                     __syncwarp();
@@ -1215,16 +1249,18 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                         k_slot = 0;
                         k_lap++;
                     }
-                    if (j > 0) values(j - 1);
+                    if (j > 0) values(j - 1, t + 1 < t1);
                     was = n16;
                 }
                 if (!ok) break;
             }
-            if (ok && j > 0) values(j - 1);
+            if (ok && j > 0) values(j - 1, false);
         }
     }
-    if (*dead)  // (copies of a share that gave up may still be on their way here)
-        for (int i = 0; i < 1000; i++) __nanosleep(1000);
+    if (*dead) {
+        a.line->dead = 1;
+        for (int i = 0; i < 1000; i++) __nanosleep(1000);  // (copies of a share that gave up may still be on their way here)
+    }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (warp == kMmaWarp) {
@@ -1349,7 +1385,7 @@ __global__ void __launch_bounds__(kSharedJoinThreads) shared_join_kernel(const _
                 t.base[k] = (t.b - it.row0) * a.hb;
                 cut |= t.first[k] != t.last[k];
             }
-            t.kind = row.z == -2 ? 2 : redo ? 1 : 0;
+            t.kind = row.z == -2 || line.dead ? 2 : redo ? 1 : 0;
             // (a row of one item that was not cut is written already)
             if (t.kind || cut || (row.z >= 0) == (row.w >= 0)) todo[atomicAdd(&n_todo, 1)] = t;
         }
@@ -1478,8 +1514,11 @@ bool make_map(CUtensorMap* m, int dtype, const void* at, const int64_t (&n)[4], 
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// A cache's k or v: dimensions of a head, heads, positions of a page, pages.
-bool make_map(CUtensorMap* m, const b2_paged_kv& kv, const void* at, int box) {
+// A cache's k or v: dimensions of a head, heads, positions of a page, pages
+// (flat: one page of all positions).
+bool make_map(CUtensorMap* m, const b2_paged_kv& kv, const void* at, int box, bool flat) {
+    if (flat)
+        return make_map(m, kv.dtype, at, {kv.hd, kv.nkv, (int64_t)kv.page_size * kv.n_pages, 1}, {kv.head_stride, kv.pos_stride, 8}, 1, box);
     return make_map(m, kv.dtype, at, {kv.hd, kv.nkv, kv.page_size, kv.n_pages}, {kv.head_stride, kv.pos_stride, kv.page_stride}, 1, box);
 }
 
@@ -1595,7 +1634,8 @@ int launch_attention_shared(const b2_paged_kv& kv, const b2_paged_attn_opts& o, 
         return B2_ERR_CUDA;
     }
     a.box = box_of(kv);
-    if (a.box && !(make_map(&mk, kv, kv.k, a.box) && make_map(&mv, kv, kv.v, a.box))) a.box = 0;
+    a.flat = kv.page_stride == kv.page_size * kv.pos_stride && (int64_t)kv.page_size * kv.n_pages < ((int64_t)1 << 31);
+    if (a.box && !(make_map(&mk, kv, kv.k, a.box, a.flat) && make_map(&mv, kv, kv.v, a.box, a.flat))) a.box = 0;
     const cudaError_t e = kv.hd <= 64 ? go_hd<64>(a, o.dtype, kv.dtype, mk, mv, mq, sms, s)
                                       : go_hd<128>(a, o.dtype, kv.dtype, mk, mv, mq, sms, s);
     return e == cudaSuccess ? B2_OK : cuda_failed("shared attention launch", e, err);
