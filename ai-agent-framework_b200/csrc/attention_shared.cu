@@ -98,7 +98,7 @@ struct SharedArgs {
     int q_wide, out_wide;  // 16-byte accesses
     int terms;             // of Q that the first launch makes; 0: the products read q as it is
     int box;               // positions of a box of the tensor maps (16 or 8); 0: pages that they cannot tell
-    int flat;              // pages follow one another as their positions do: one dimension
+    int flat;              // pages follow one another as their positions do: one dimension; 2: boxes of whole heads
     float scale, softcap;
     // scratch
     Line* line;
@@ -469,12 +469,20 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
     return long_wait(bar, parity, dead);
 }
 
-// V as the second operand: its rows are positions, the products' K, and its
-// dimensions lie in 128-byte runs, 64 of them, the next 64 a block on: 8
-// positions are 1024 bytes (stride), the blocks kTile * 128 apart (leading).
-__device__ __forceinline__ uint64_t v_desc(uint32_t saddr) {
-    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((kTile * 128) >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) |
-           ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
+// K and V tiles: 8 positions by 64 dimensions are 1024 bytes in the 128-byte
+// swizzle, a position a line of 128; the 64-dimension blocks of 8 positions
+// follow one another, then the next 8 positions.  The byte of dimension 8 c
+// (c: its 16-byte chunk) of position row:
+template <int BL>
+__device__ __forceinline__ uint32_t kv_at(int row, int c) {
+    return (row >> 3) * (BL * 1024) + (c >> 3) * 1024 + (row & 7) * 128 + (((c & 7) ^ (row & 7)) << 4);
+}
+// K as the second operand: 8 positions are BL * 1024 bytes on (stride).  V: its
+// rows are the products' K, so that is again the stride, and the blocks of
+// dimensions are 1024 apart (leading).
+template <int BL>
+__device__ __forceinline__ uint64_t kv_desc() {
+    return ((uint64_t)(1024u >> 4) << 16) | ((uint64_t)((BL * 1024u) >> 4) << 32) | ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
 }
 
 __device__ __forceinline__ uint64_t desc_of(uint32_t lo, uint32_t hi) {
@@ -518,6 +526,16 @@ __device__ __forceinline__ void cp16_if(uint32_t smem, const void* gmem, bool va
         "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %3, 0;\n\t"
         "@p cp.async.cg.shared.global [%0], [%1], 16, %2;\n\t}" ::"r"(smem),
         "l"(gmem), "r"(valid ? 16 : 0), "r"((uint32_t)go)
+        : "memory");
+}
+
+// The same of a map over all positions of a pool, 8 by 8: all dimensions of a
+// head, positions from 8 * eight on.
+__device__ __forceinline__ void tma_eights(uint32_t smem, const CUtensorMap* map, int eight, int head, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %2, %2, %3, %4}], [%5];" ::
+            "r"(smem),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(eight), "r"(head), "r"(smem_u32(bar))
         : "memory");
 }
 
@@ -868,54 +886,55 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                 const int slots = value ? NV : NK;
                 const uint32_t ring_s = value ? ring_v : ring_k;
                 int slot = 0;
-                struct Tile {
-                    int page, pos, lo, hi;  // this lane's group: page, first position; the tile's seen rows
-                };
-                auto look = [&](const Piece* q, int tt) {
-                    Tile f;
-                    const int p0 = q->start(tt);
-                    f.lo = q->lo - p0;
-                    f.hi = min(kTile, q->hi - p0);
-                    f.pos = p0 + lane * G;
-                    f.page = -1;
-                    // (any position of the group that is seen names its page)
-                    if (lane < groups && lane * G < f.hi && lane * G + G > f.lo) f.page = page_at(q, max(f.pos, q->lo));
-                    return f;
-                };
                 constexpr int BL = HD / 64;  // boxes of a group
                 const uint32_t all = (1u << groups) - 1;
-                Tile nx{};
-                if (p) nx = look(p, t);
+                const int r0 = lane * G;
+                // the piece: first position of its next tile, seen positions, table row; this lane's place in it
+                int p0 = 0, p_lo = 0, p_hi = 0;
+                const int32_t* row = nullptr;
+                auto enter = [&]() {
+                    if (!p) return;
+                    t = p->t1 - p->t0;
+                    p0 = p->start(p->t0);
+                    p_lo = p->lo;
+                    p_hi = p->hi;
+                    row = a.table + (int64_t)p->tr * a.table_stride;
+                };
+                auto look = [&]() {  // this lane's group: its page (any position of it that is seen names it)
+                    const int at = max(p0 + r0, p_lo);
+                    if (lane >= groups || at >= p_hi || p0 + r0 + G <= p_lo) return -1;
+                    return row[a.page_shift >= 0 ? at >> a.page_shift : at / a.page_size];
+                };
+                enter();
+                int nx = p ? look() : -1;
 #pragma unroll 1
                 while (p) {
-                    const Tile f = nx;
-                    if (++t == p->t1) {
+                    const int page = nx, lo_t = p_lo - p0, hi_t = min(kTile, p_hi - p0), in = place(p0 + r0);
+                    p0 += kTile;
+                    if (--t == 0) {
                         pieces.done(s);
                         p = pieces.next(s);
-                        t = p ? p->t0 : 0;
+                        enter();
                     }
-                    if (p) nx = look(p, t);  // (the next tile's pages, on their way meanwhile)
-                    const int r0 = lane * G, in = place(f.pos);
-                    const bool there = (unsigned)f.page < (unsigned)a.n_pages;
-                    const bool whole = lane < groups && there && r0 >= f.lo && r0 + G <= f.hi;
-                    const int where = a.flat ? f.page * a.page_size + in : in;
+                    if (p) nx = look();  // (the next tile's pages, on their way meanwhile)
+                    const bool there = (unsigned)page < (unsigned)a.n_pages;
+                    const bool whole = lane < groups && there && r0 >= lo_t && r0 + G <= hi_t;
+                    const int where = a.flat ? page * a.page_size + in : in;
                     const uint32_t by_box = __ballot_sync(0xffffffffu, whole);
-                    uint32_t rest = 0;
-                    if (by_box != all) rest = __ballot_sync(0xffffffffu, lane < groups && !whole && r0 < ((f.hi + kGroup - 1) & ~(kGroup - 1)));
-                    if (!value) {  // positions seen whose page is not there
-                        uint32_t bits = 0;
-                        if (rest) {
-                            const int lo = max(f.lo, r0), hi = min(f.hi, r0 + G);
-                            const bool gone = lane < groups && lo < hi && !there;
-                            const uint32_t mine = gone ? ((1u << (hi - lo)) - 1) << (lo & 31) : 0;
-#pragma unroll
-                            for (int i = 0; i < 4; i++) {
-                                const uint32_t b = __reduce_or_sync(0xffffffffu, (lo >> 5) == i ? mine : 0);
-                                if (lane == i) bits = b;
-                            }
+                    uint32_t rest = 0, bits = 0;
+                    if (by_box != all) {
+                        rest = __ballot_sync(0xffffffffu, lane < groups && !whole && r0 < ((hi_t + kGroup - 1) & ~(kGroup - 1)));
+                        // positions seen whose page is not there
+                        const int lo = max(lo_t, r0), hi = min(hi_t, r0 + G);
+                        const bool gone = lane < groups && lo < hi && !there;
+                        const uint32_t mine = gone ? ((1u << (hi - lo)) - 1) << (lo & 31) : 0;
+#pragma unroll 1
+                        for (int i = 0; i < 4; i++) {
+                            const uint32_t b = __reduce_or_sync(0xffffffffu, (lo >> 5) == i ? mine : 0);
+                            if (lane == i) bits = b;
                         }
-                        if (lane < 4) s.bad[j & 7][lane] = bits;
                     }
+                    if (!value && lane < 4) s.bad[j & 7][lane] = bits;
                     // the tile's place is free once the one before in it was multiplied
                     const int was = j - slots;
                     if (was >= 0)
@@ -935,10 +954,20 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
 #pragma unroll
                         for (int i = 0; i < 8; i++) {  // (uniform over the warp)
                             const int g = g0 + i, at = __shfl_sync(0xffffffffu, where, g);
-                            const int page = a.flat ? 0 : __shfl_sync(0xffffffffu, f.page, g);
-                            if ((by_box >> g) & 1 && one) {
-#pragma unroll
-                                for (int x = 0; x < BL; x++) tma_rows(to + x * (kTile * 128) + g * G * 128, map, 64 * x, h, at, page, bar);
+                            const uint32_t put = to + g * (G * 128 * BL);
+                            if (a.flat == 2) {
+                                if ((by_box >> g) & 1 && one) tma_eights(put, map, at >> 3, h, bar);
+                            } else {
+                                const int pg = a.flat ? 0 : __shfl_sync(0xffffffffu, page, g);
+                                if ((by_box >> g) & 1 && one)
+#pragma unroll 1
+                                    for (int r = 0, x = 0; r < G; x++) {  // (a box: of 8 positions where there are blocks)
+                                        tma_rows(put + r * (128 * BL) + x * 1024, map, 64 * x, h, at + r, pg, bar);
+                                        if (x == BL - 1) {
+                                            r += BL == 1 ? G : 8;
+                                            x = -1;
+                                        }
+                                    }
                             }
                         }
                     __syncwarp();
@@ -946,15 +975,14 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                         while (rest) {
                             const int g = __ffs(rest) - 1;
                             rest &= rest - 1;
-                            const int page = __shfl_sync(0xffffffffu, f.page, g), at = __shfl_sync(0xffffffffu, in, g);
-                            const bool in_pool = (unsigned)page < (unsigned)a.n_pages;
-                            const uint16_t* from = src + (in_pool ? page * a.page_stride + at * a.pos_stride : 0) + h * a.head_stride;
-#pragma unroll 4
+                            const int pg = __shfl_sync(0xffffffffu, page, g), at = __shfl_sync(0xffffffffu, in, g);
+                            const bool in_pool = (unsigned)pg < (unsigned)a.n_pages;
+                            const uint16_t* from = src + (in_pool ? pg * a.page_stride + at * a.pos_stride : 0) + h * a.head_stride;
+#pragma unroll 2
                             for (int i = lane; i < G * hc; i += 32) {
-                                const int r = i / hc, c = i - r * hc, row = g * G + r;
-                                const bool seen = in_pool && row >= f.lo && row < f.hi;
-                                cp16_if(to + (c >> 3) * (kTile * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4),
-                                        seen ? from + r * a.pos_stride + c * 8 : src, seen, seen || value);
+                                const int r = i / hc, c = i - r * hc, rt = g * G + r;
+                                const bool seen = in_pool && rt >= lo_t && rt < hi_t;
+                                cp16_if(to + kv_at<BL>(rt, c), seen ? from + r * a.pos_stride + c * 8 : src, seen, seen || value);
                             }
                         }
                         cp_async_commit();
@@ -971,7 +999,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                 constexpr int RW = kTile / kCopyWarps;
                 constexpr int CH = HD / 8, LR = 32 / CH;  // chunks of a row, rows of a warp's copy
                 const int row0 = lw * RW + lane, c = lane % CH, r0 = lane / CH;
-                const uint32_t at0 = ring_k + (c >> 3) * (kTile * 128) + (lw * RW + r0) * 128;
+                const uint32_t at0 = ring_k + kv_at<HD / 64>(lw * RW, 0);
                 const int64_t h_off = (int64_t)h * a.head_stride + c * 8;
                 int issued[2] = {0, 0}, told[2] = {0, 0};  // tiles of K, of V, and those that the products know of
                 int waiting = 0;                           // stages issued that they do not know of,
@@ -1028,7 +1056,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
 #pragma unroll
                         for (int u = 0; u < U; u++) {
                             const int r = (i0 + u) * LR + r0;
-                            const uint32_t at = to + (i0 + u) * LR * 128 + (((c & 7) ^ (r & 7)) << 4);  // (lw * RW is a multiple of 8)
+                            const uint32_t at = to + kv_at<HD / 64>(r, c);  // (lw * RW is a multiple of 8)
                             cp16_if(at, src + (o[u] < 0 ? 0 : o[u] + h_off), o[u] >= 0, c < hc && (o[u] >= 0 || (value && o[u] == -1)));
                         }
                     }
@@ -1165,8 +1193,9 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
             // the sums with constants below, in the warp's uniform registers)
             auto uniform = [](uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); };
             const uint32_t ring_k = smem_u32(ring) >> 4, ring_v = ring_k + NK * (TM::kTileBytes >> 4), q_s = smem_u32(q_sm) >> 4;
-            const uint32_t hi_k = (uint32_t)(sw128_desc(0) >> 32), lo_k = (uint32_t)sw128_desc(0);
-            const uint32_t hi_v = (uint32_t)(v_desc(0) >> 32), lo_v = (uint32_t)v_desc(0);
+            constexpr int BL = HD / 64;
+            const uint32_t hi_q = (uint32_t)(sw128_desc(0) >> 32), lo_q = (uint32_t)sw128_desc(0);
+            const uint32_t hi_kv = (uint32_t)(kv_desc<BL>() >> 32), lo_kv = (uint32_t)kv_desc<BL>();
             const int ks = (hd + 15) / 16;
             const uint32_t id_v = uniform(idesc<C>(ks * 16, true)), id_k = uniform(idesc<C>(0, false));
             const uint32_t tm = uniform(tmem);
@@ -1181,7 +1210,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                 if (!ok) return;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t b = uniform(jj & 1), n = uniform(was);
-                const uint32_t v = lo_v + ring_v + (NV == 2 ? b : 0) * (TM::kTileBytes >> 4);
+                const uint32_t v = lo_kv + ring_v + (NV == 2 ? b : 0) * (TM::kTileBytes >> 4);
                 const uint32_t pc = tm + b * TM::kSCols, tc = tm + 2 * TM::kSCols + (NT == 2 ? b : 0) * HD;
                 if (elected()) {
                     if (n == kTile / 16) {
@@ -1189,7 +1218,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                         for (int x = PT - 1; x >= 0; x--)  // (small terms first)
 #pragma unroll
                             for (int k = 0; k < kTile / 16; k++)
-                                mma_f16_ts(tc, pc + (x == 2 ? 128 + 8 * k : 16 * k + 8 * x), desc_of(v + k * (2048 >> 4), hi_v), id_v,
+                                mma_f16_ts(tc, pc + (x == 2 ? 128 + 8 * k : 16 * k + 8 * x), desc_of(v + k * ((2 * BL * 1024) >> 4), hi_kv), id_v,
                                            x < PT - 1 || k > 0);
                     } else {
                         uint32_t acc = 0;
@@ -1197,7 +1226,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                         for (int x = PT - 1; x >= 0; x--)
 #pragma unroll 1
                             for (uint32_t k = 0; k < n; k++) {
-                                mma_f16_ts(tc, pc + (x == 2 ? 128 + 8 * k : 16 * k + 8 * x), desc_of(v + k * (2048 >> 4), hi_v), id_v, acc);
+                                mma_f16_ts(tc, pc + (x == 2 ? 128 + 8 * k : 16 * k + 8 * x), desc_of(v + k * ((2 * BL * 1024) >> 4), hi_kv), id_v, acc);
                                 acc = 1;
                             }
                     }
@@ -1209,7 +1238,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
             while (const Piece* p = pieces.next(s)) {
                 const int n = pieces.n - 1, start = p->start(0), hi = p->hi, t0 = p->t0, t1 = p->t1;
                 pieces.done(s);
-                const uint32_t q = uniform(lo_k + q_s + (n % QB) * QT * (TM::kTileBytes >> 4));
+                const uint32_t q = uniform(lo_q + q_s + (n % QB) * QT * (TM::kTileBytes >> 4));
                 ok = ok && warp_wait(&s.q_full[n % QB], (n / QB) & 1, dead);
 #pragma unroll 1
                 for (int t = t0; t < t1 && ok; t++, j++) {
@@ -1218,7 +1247,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t b = uniform(j & 1), ksl = NK == 2 ? b : uniform(k_slot), id = uniform(id_k | (uint32_t)(2 * n16) << 17);
-                    const uint32_t k_sm = lo_k + ring_k + ksl * (TM::kTileBytes >> 4), sc = tm + b * TM::kSCols;
+                    const uint32_t k_sm = lo_kv + ring_k + ksl * (TM::kTileBytes >> 4), sc = tm + b * TM::kSCols;
                     if (elected()) {
                         if (ks == HD / 16) {
 #pragma unroll
@@ -1226,8 +1255,8 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
 #pragma unroll
                                 for (int k = 0; k < HD / 16; k++) {
                                     const uint32_t in = (uint32_t)(k >> 2) * ((kTile * 128) >> 4) + (k & 3) * 2;
-                                    mma_f16(sc, desc_of(q + x * (TM::kTileBytes >> 4) + in, hi_k), desc_of(k_sm + in, hi_k), id,
-                                            x < QT - 1 || k > 0);
+                                    mma_f16(sc, desc_of(q + x * (TM::kTileBytes >> 4) + in, hi_q),
+                                            desc_of(k_sm + (k >> 2) * (1024 >> 4) + (k & 3) * 2, hi_kv), id, x < QT - 1 || k > 0);
                                 }
                         } else {
                             uint32_t acc = 0;
@@ -1236,7 +1265,8 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
 #pragma unroll 1
                                 for (int k = 0; k < ks; k++) {
                                     const uint32_t in = (uint32_t)(k >> 2) * ((kTile * 128) >> 4) + (k & 3) * 2;
-                                    mma_f16(sc, desc_of(q + x * (TM::kTileBytes >> 4) + in, hi_k), desc_of(k_sm + in, hi_k), id, acc);
+                                    mma_f16(sc, desc_of(q + x * (TM::kTileBytes >> 4) + in, hi_q),
+                                            desc_of(k_sm + (uint32_t)(k >> 2) * (1024 >> 4) + (k & 3) * 2, hi_kv), id, acc);
                                     acc = 1;
                                 }
                         }
@@ -1500,26 +1530,44 @@ int box_of(const b2_paged_kv& kv) {
     return kv.page_size % 16 == 0 ? 16 : kv.page_size % 8 == 0 ? 8 : 0;
 }
 
-// A map of 16-bit elements: boxes of 64 of the first dimension (those past its
-// end read as zero), b1 and b2 of the next two, in the 128-byte swizzle.
-bool make_map(CUtensorMap* m, int dtype, const void* at, const int64_t (&n)[4], const int64_t (&stride)[3], int b1, int b2) {
+// A map of 16-bit elements in the 128-byte swizzle: n elements, strides (in
+// elements) from the second dimension on, and the box of each dimension.
+template <int R>
+bool make_map(CUtensorMap* m, int dtype, const void* at, const int64_t (&n)[R], const int64_t (&stride)[R - 1], const int (&box)[R]) {
     const auto enc = tensor_map_encoder();
     if (!enc) return false;
-    cuuint64_t dims[4], strides[3];
-    for (int i = 0; i < 4; i++) dims[i] = (cuuint64_t)n[i];
-    for (int i = 0; i < 3; i++) strides[i] = (cuuint64_t)std::max<int64_t>(16, 2 * stride[i]);
-    const cuuint32_t boxes[4] = {64, (cuuint32_t)b1, (cuuint32_t)b2, 1}, steps[4] = {1, 1, 1, 1};
-    return enc(m, dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(at), dims,
+    cuuint64_t dims[R], strides[R - 1];
+    cuuint32_t boxes[R], steps[R];
+    for (int i = 0; i < R; i++) {
+        dims[i] = (cuuint64_t)n[i];
+        boxes[i] = (cuuint32_t)box[i];
+        steps[i] = 1;
+        if (i) strides[i - 1] = (cuuint64_t)std::max<int64_t>(16, 2 * stride[i - 1]);
+    }
+    return enc(m, dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, R, const_cast<void*>(at), dims,
                strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// A cache's k or v: dimensions of a head, heads, positions of a page, pages
-// (flat: one page of all positions).
-bool make_map(CUtensorMap* m, const b2_paged_kv& kv, const void* at, int box, bool flat) {
-    if (flat)
-        return make_map(m, kv.dtype, at, {kv.hd, kv.nkv, (int64_t)kv.page_size * kv.n_pages, 1}, {kv.head_stride, kv.pos_stride, 8}, 1, box);
-    return make_map(m, kv.dtype, at, {kv.hd, kv.nkv, kv.page_size, kv.n_pages}, {kv.head_stride, kv.pos_stride, kv.page_stride}, 1, box);
+// Whether the cache's pages follow one another as their positions do (1), and
+// then whether a box may take whole heads (2).
+int flat_of(const b2_paged_kv& kv) {
+    if (kv.page_stride != kv.page_size * kv.pos_stride || (int64_t)kv.page_size * kv.n_pages >= ((int64_t)1 << 31)) return 0;
+    return kv.hd % 64 == 0 ? 2 : 1;
+}
+
+// A cache's k or v.  Boxes of 64 dimensions (those past hd read as zero), one
+// head, `box` positions (8 where a head has two blocks) of one page; or of whole
+// heads, positions 8 by 8.
+bool make_map(CUtensorMap* m, const b2_paged_kv& kv, const void* at, int box, int flat) {
+    const int64_t all = (int64_t)kv.page_size * kv.n_pages;
+    if (flat == 2)
+        return make_map<5>(m, kv.dtype, at, {64, 8, kv.hd / 64, all / 8, kv.nkv}, {kv.pos_stride, 64, 8 * kv.pos_stride, kv.head_stride},
+                           {64, 8, kv.hd / 64, box / 8, 1});
+    const int rows = kv.hd <= 64 ? box : 8;
+    if (flat) return make_map<4>(m, kv.dtype, at, {kv.hd, kv.nkv, all, 1}, {kv.head_stride, kv.pos_stride, 8}, {64, 1, rows, 1});
+    return make_map<4>(m, kv.dtype, at, {kv.hd, kv.nkv, kv.page_size, kv.n_pages}, {kv.head_stride, kv.pos_stride, kv.page_stride},
+                       {64, 1, rows, 1});
 }
 
 // How a group of query heads falls to items, and the shares of the machine.
@@ -1627,14 +1675,15 @@ int launch_attention_shared(const b2_paged_kv& kv, const b2_paged_attn_opts& o, 
     a.terms = o.dtype == 0 ? (kv.dtype == 1 ? 2 : 3) : a.q_wide && a.q_stride < ((int64_t)1 << 38) ? 0 : 1;
     layout(batch, o.nh, kv.nkv, kv.hd, sms, static_cast<uint8_t*>(scratch), &a);
     CUtensorMap mk{}, mv{}, mq{};
-    const bool q_map = a.terms ? make_map(&mq, kv.dtype, a.term, {kv.hd, o.nh, batch, a.terms}, {kv.hd, qd, qd * batch}, a.hb, a.rows)
-                               : make_map(&mq, kv.dtype, q, {kv.hd, o.nh, batch, 1}, {kv.hd, a.q_stride, 8}, a.hb, a.rows);
+    const bool q_map =
+        a.terms ? make_map<4>(&mq, kv.dtype, a.term, {kv.hd, o.nh, batch, a.terms}, {kv.hd, qd, qd * batch}, {64, a.hb, a.rows, 1})
+                : make_map<4>(&mq, kv.dtype, q, {kv.hd, o.nh, batch, 1}, {kv.hd, a.q_stride, 8}, {64, a.hb, a.rows, 1});
     if (!q_map) {
         *err = "shared attention: no tensor map of q";
         return B2_ERR_CUDA;
     }
     a.box = box_of(kv);
-    a.flat = kv.page_stride == kv.page_size * kv.pos_stride && (int64_t)kv.page_size * kv.n_pages < ((int64_t)1 << 31);
+    a.flat = flat_of(kv);
     if (a.box && !(make_map(&mk, kv, kv.k, a.box, a.flat) && make_map(&mv, kv, kv.v, a.box, a.flat))) a.box = 0;
     const cudaError_t e = kv.hd <= 64 ? go_hd<64>(a, o.dtype, kv.dtype, mk, mv, mq, sms, s)
                                       : go_hd<128>(a, o.dtype, kv.dtype, mk, mv, mq, sms, s);
