@@ -61,7 +61,6 @@ constexpr int kMinShare = 3;     // a share's units, at least
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanItems = 2 * kPlanThreads;  // items whose units stay in shared memory,
 constexpr int kLineGroups = 2048;               // and groups
-constexpr uint64_t kSharedWaitNs = 2000000000ull;
 constexpr int kNoLimit = 0x7fffffff;
 
 struct Item {
@@ -92,7 +91,7 @@ struct SharedArgs {
     float* lse;
     const float* slopes;
     int64_t q_stride, out_stride, table_stride, page_stride, pos_stride, head_stride;
-    int batch, nh, nkv, grp, hd, page_size, page_shift, n_pages, max_pages, n_req, len_add, window, n_groups;
+    int batch, nh, nkv, grp, hd, page_size, n_pages, max_pages, n_req, len_add, window, n_groups;
     int hb, blocks, rows;  // query heads of an item, such blocks of a group of heads, rows of an item
     int shares;            // at most
     int q_wide, out_wide;  // 16-byte accesses
@@ -100,6 +99,8 @@ struct SharedArgs {
     int box;               // positions of a box of the tensor maps (16 or 8); 0: pages that they cannot tell
     int flat;              // pages follow one another as their positions do: one dimension; 2: boxes of whole heads
     float scale, softcap;
+    uint32_t page_mul;  // division by the page size
+    int page_shift;
     // scratch
     Line* line;
     Share* share;  // [shares]
@@ -111,6 +112,13 @@ struct SharedArgs {
     float* whole;  // [2][batch][nh][hd + 4] results of whole items of rows that have two: o, m (log2 units), l
     float* part;   // [CTAs][2][128][hd + 4] pieces of items that were cut
 };
+
+// n / page_size for 0 <= n < 2^31 (Granlund and Montgomery, "Division by
+// invariant integers using multiplication", 1994): with s = ceil(log2 P) and mul
+// = floor(2^32 (2^s - P) / P) + 1, n / P = (mulhi(mul, n) + n) >> s.
+__device__ __forceinline__ int page_of(const SharedArgs& a, int n) {
+    return (int)((__umulhi(a.page_mul, (unsigned)n) + (unsigned)n) >> a.page_shift);
+}
 
 // tiles start on multiples of 16 positions
 __device__ __forceinline__ int base_of(const Item& it) { return it.lo & ~15; }
@@ -435,38 +443,18 @@ struct SmallShared {
 };
 static_assert(sizeof(SmallShared) <= 15360, "");
 
-__device__ __forceinline__ bool phase_over(uint64_t* bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity), "r"(10000000u)  // (asleep for as long as that, where the hardware can)
-        : "memory");
-    return ok;
-}
-
-__device__ __forceinline__ bool long_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
-    uint64_t t0 = 0;
-    for (unsigned n = 0;; n++) {
-        if (__all_sync(0xffffffffu, phase_over(bar, parity))) return true;
-        if (n % 64 == 63) {
-            if (__any_sync(0xffffffffu, *dead)) return false;
-            const uint64_t t = global_ns();
-            if (!t0) t0 = t;
-            if (__any_sync(0xffffffffu, t - t0 > kSharedWaitNs)) {
-                *dead = 1;
-                return false;
-            }
-        }
-    }
-}
-
-// Waits for a barrier's phase; by a warp, one answer for all lanes.
+// Waits for a barrier's phase; by a warp, one answer for all lanes.  A wait that
+// does not end (some 0.1 s at least, 4 s where every try sleeps a microsecond)
+// gives up: `dead` is set, and the call's rows become NaN.  Small, as it stands
+// in every role: what the roles run per tile has to stay in the SM's instruction
+// cache (with the clock in this loop, and copies and pages unrolled, the GPC's
+// was 65 % busy and everything four times as slow).
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
-    if (__all_sync(0xffffffffu, phase_over(bar, parity))) return true;
-    return long_wait(bar, parity, dead);
+#pragma unroll 1
+    for (int n = 0; n < (1 << 22); n++)
+        if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    *dead = 1;
+    return false;
 }
 
 // K and V tiles: 8 positions by 64 dimensions are 1024 bytes in the 128-byte
@@ -867,13 +855,8 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
             const Piece* p = pieces.next(s);
             int t = p ? p->t0 : 0;
             bool ok = true;
-            auto page_at = [&](const Piece* q, int pos) {
-                const int pg = a.page_shift >= 0 ? pos >> a.page_shift : pos / a.page_size;
-                return a.table[(int64_t)q->tr * a.table_stride + pg];
-            };
-            auto place = [&](int pos) {  // in its page
-                return a.page_shift >= 0 ? pos & (a.page_size - 1) : pos - pos / a.page_size * a.page_size;
-            };
+            auto page_at = [&](const Piece* q, int pos) { return a.table[(int64_t)q->tr * a.table_stride + page_of(a, pos)]; };
+            auto place = [&](int pos) { return pos - page_of(a, pos) * a.page_size; };  // in its page
             if (a.box) {
                 // K by the first warp, V by the second.  Groups of `box` positions that lie in one
                 // page: seen whole, a tensor map's box each; in part, or in no page, row by row.
@@ -903,7 +886,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                 auto look = [&]() {  // this lane's group: its page (any position of it that is seen names it)
                     const int at = max(p0 + r0, p_lo);
                     if (lane >= groups || at >= p_hi || p0 + r0 + G <= p_lo) return -1;
-                    return row[a.page_shift >= 0 ? at >> a.page_shift : at / a.page_size];
+                    return row[page_of(a, at)];
                 };
                 enter();
                 int nx = p ? look() : -1;
@@ -950,26 +933,25 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                         if (rest) mbar_expect_tx(bar, bytes);
                         else mbar_arrive_expect_tx(bar, bytes);
                     }
-                    for (int g0 = 0; g0 < groups; g0 += 8)
-#pragma unroll
-                        for (int i = 0; i < 8; i++) {  // (uniform over the warp)
-                            const int g = g0 + i, at = __shfl_sync(0xffffffffu, where, g);
-                            const uint32_t put = to + g * (G * 128 * BL);
-                            if (a.flat == 2) {
-                                if ((by_box >> g) & 1 && one) tma_eights(put, map, at >> 3, h, bar);
-                            } else {
-                                const int pg = a.flat ? 0 : __shfl_sync(0xffffffffu, page, g);
-                                if ((by_box >> g) & 1 && one)
 #pragma unroll 1
-                                    for (int r = 0, x = 0; r < G; x++) {  // (a box: of 8 positions where there are blocks)
-                                        tma_rows(put + r * (128 * BL) + x * 1024, map, 64 * x, h, at + r, pg, bar);
-                                        if (x == BL - 1) {
-                                            r += BL == 1 ? G : 8;
-                                            x = -1;
-                                        }
+                    for (int g = 0; g < groups; g++) {  // (uniform over the warp)
+                        const int at = __shfl_sync(0xffffffffu, where, g);
+                        const uint32_t put = to + g * (G * 128 * BL);
+                        if (a.flat == 2) {
+                            if ((by_box >> g) & 1 && one) tma_eights(put, map, at >> 3, h, bar);
+                        } else {
+                            const int pg = a.flat ? 0 : __shfl_sync(0xffffffffu, page, g);
+                            if ((by_box >> g) & 1 && one)
+#pragma unroll 1
+                                for (int r = 0, x = 0; r < G; x++) {  // (a box: of 8 positions where there are blocks)
+                                    tma_rows(put + r * (128 * BL) + x * 1024, map, 64 * x, h, at + r, pg, bar);
+                                    if (x == BL - 1) {
+                                        r += BL == 1 ? G : 8;
+                                        x = -1;
                                     }
-                            }
+                                }
                         }
+                    }
                     __syncwarp();
                     if (rest) {
                         while (rest) {
@@ -1039,7 +1021,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                     if (was >= 0) {
                         uint64_t* bar = value ? &s.t_full[was & 1] : NK == 2 ? &s.s_full[was & 1] : &s.k_empty[slot];
                         const uint32_t parity = (value || NK == 2 ? was >> 1 : was / NK) & 1;
-                        if (!__all_sync(0xffffffffu, phase_over(bar, parity))) {
+                        if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
                             cp_wait<0>();  // (what frees it may wait for what is on its way)
                             tell(0);
                             ok = ok && warp_wait(bar, parity, dead);
@@ -1336,7 +1318,7 @@ __device__ __noinline__ Sum row_alone(const SharedArgs& a, int b, int head) {
         int64_t off = -1;
         float x = -INFINITY;
         if (pos < sq.len) {
-            const int pg = pos / a.page_size, page = a.table[(int64_t)sq.tr * a.table_stride + pg];
+            const int pg = page_of(a, pos), page = a.table[(int64_t)sq.tr * a.table_stride + pg];
             if ((unsigned)page < (unsigned)a.n_pages) {
                 off = page * a.page_stride + (int64_t)(pos - pg * a.page_size) * a.pos_stride + h_off;
                 const C* k = reinterpret_cast<const C*>(a.k) + off;
@@ -1655,7 +1637,8 @@ int launch_attention_shared(const b2_paged_kv& kv, const b2_paged_attn_opts& o, 
     a.grp = o.nh / kv.nkv;
     a.hd = kv.hd;
     a.page_size = kv.page_size;
-    a.page_shift = (kv.page_size & (kv.page_size - 1)) ? -1 : __builtin_ctz(kv.page_size);
+    while ((1ull << a.page_shift) < (unsigned)kv.page_size) a.page_shift++;
+    a.page_mul = (uint32_t)((((1ull << a.page_shift) - kv.page_size) << 32) / kv.page_size + 1);
     a.n_pages = kv.n_pages;
     a.max_pages = o.max_pages;
     a.n_req = o.n_req;
