@@ -659,7 +659,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                     const int chunks = (min(kTile, it_hi - p0) + 31) / 32;
                     const bool mask = __any_sync(0xffffffffu, c0 > 0 || c1 < 32 * chunks);
                     float f = QT == 1 ? (cap > 0.0f ? a.scale / cap : a.scale * kLog2e) : s.factor[slot][m];
-                    if (mask || !plain) {  // the scores that are not seen to -inf; cap and slope
+                    if (!plain) {  // cap and slope
 #pragma unroll 1
                         for (int c = 0; c < 32 * chunks; c += 16) {
                             uint32_t r[16];
@@ -667,18 +667,29 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                             const float p1 = (float)(p0 + c - (row.z - 1));
 #pragma unroll
                             for (int i = 0; i < 16; i++) {
-                                float x = __uint_as_float(r[i]);
-                                if (!plain) {
-                                    x *= f;
-                                    if (cap > 0.0f) x = (cap * kLog2e) * tanh_of(x);
-                                    x = fmaf(slope, p1 + (float)i, x);
-                                }
-                                r[i] = c + i < c0 || c + i >= c1 ? 0xff800000u : __float_as_uint(x);
+                                float x = __uint_as_float(r[i]) * f;
+                                if (cap > 0.0f) x = (cap * kLog2e) * tanh_of(x);
+                                r[i] = __float_as_uint(fmaf(slope, p1 + (float)i, x));
                             }
                             tmem_st16(s_col + c, r);
                         }
                         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                        if (!plain) f = 1.0f;
+                        f = 1.0f;
+                    }
+                    if (mask) {  // the scores that are not seen to -inf
+#pragma unroll 1
+                        for (int c = 0; c < 32 * chunks; c += 16) {
+                            const int lo = min(max(c0 - c, 0), 16), hi = min(max(c1 - c, 0), 16);
+                            const uint32_t seen = hi > lo ? ((1u << hi) - 1) & ~((1u << lo) - 1) : 0;
+                            if (__all_sync(0xffffffffu, seen == 0xffff)) continue;
+                            uint32_t r[16];
+                            tmem_ld16(s_col + c, r);
+#pragma unroll
+                            for (int i = 0; i < 16; i++)
+                                if (!(seen >> i & 1)) r[i] = 0xff800000u;
+                            tmem_st16(s_col + c, r);
+                        }
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     }
                     // 16 columns on their way while 16 are worked on, in loops that the instruction
                     // cache next to the scheduler holds
@@ -737,6 +748,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                     float l = ls.x + ls.y;
                     const uint32_t* bad = s.bad[j & 7];
                     if (bad[0] | bad[1] | bad[2] | bad[3]) {
+#pragma unroll 1
                         for (int c = max(c0, 0); c < min(c1, kTile); c++)
                             if ((bad[c >> 5] >> (c & 31)) & 1) l = __int_as_float(0x7fc00000);
                     }
