@@ -1612,16 +1612,37 @@ size_t layout(int batch, int nh, int nkv, int hd, int sms, uint8_t* base, Shared
 
 }  // namespace
 
+// When to read what the rows of a group have in common once, and when row by row
+// (attention_paged.cu).  The three launches here take 22-30 us however little
+// there is to do; row by row costs 10-13 us and then the bytes of all rows, most
+// of them from L2, at 8 TB/s (or, with more than 8 query heads to a KV head, the
+// products' time).  The two meet where the rows' positions times max(heads to a
+// KV head, 8) x KV heads x dimensions come to some 2^28 (134 MB at 8 heads), in us:
+//   heads, dims, type     rows   positions   of 2^28   row by row   shared
+//   32 / 8, 128, fp32     1 x 4   2080        1/4       14.5         29.5
+//   64 / 8, 128, bf16     1 x 16  2080        1         28.8         30.0
+//   32 / 8, 128, fp32     1 x 64   544        1         28.9         34.4
+//   64 / 1, 128, bf16     4 x 4   2080        1         28.8         28.8
+//   32 / 8, 128, fp32     8 x 8   2080        4         76.0         47.3
+//   64 / 8, 128, bf16     1 x 16  8224        4         71.6         37.0
+// With no more rows than groups there is nothing to share: 64 x 1 rows, 64 / 8
+// heads, 2080 positions take 97 us row by row and 129 shared.  What is held
+// against 2^28 is what the table has room for, since the lengths are on the device.
+bool row_by_row(const b2_paged_kv& kv, const b2_paged_attn_opts& o, int batch, int n_groups) {
+    const double positions = (double)batch * o.max_pages * kv.page_size;
+    return kv.hd > 128 || n_groups >= batch || positions * std::max(o.nh, 8 * kv.nkv) * kv.hd <= (double)(1 << 28);
+}
+
 size_t attention_shared_scratch(int batch, int nh, int nkv, int hd, int sms) {
-    if (hd > 128) return attention_paged_scratch(batch, nh, nkv, hd, sms);
-    return layout(batch, nh, nkv, hd, sms, nullptr, nullptr);
+    const size_t rows = attention_paged_scratch(batch, nh, nkv, hd, sms);
+    return hd > 128 ? rows : std::max(rows, layout(batch, nh, nkv, hd, sms, nullptr, nullptr));
 }
 
 int launch_attention_shared(const b2_paged_kv& kv, const b2_paged_attn_opts& o, const void* q, const int32_t* table,
                             const int32_t* lens, const int32_t* req, int batch, const int32_t* starts,
                             const int32_t* prefix, int n_groups, void* out, float* lse, void* scratch, cudaStream_t s,
                             std::string* err) {
-    if (kv.hd > 128) return launch_attention_paged(kv, o, q, table, lens, req, batch, out, lse, scratch, s, err);
+    if (row_by_row(kv, o, batch, n_groups)) return launch_attention_paged(kv, o, q, table, lens, req, batch, out, lse, scratch, s, err);
     const int sms = current_sms(err);
     if (!sms) return B2_ERR_CUDA;
     SharedArgs a{};

@@ -538,7 +538,7 @@ def test_a_beam_search(P, cap):
     wqkv = torch.randn(H, (nh + 2 * nkv) * hd, device="cuda", generator=g) / H ** 0.5
     head = 3.0 * torch.randn(H, V, device="cuda", generator=g) / H ** 0.5
     prompts = [[int(t) for t in np.random.default_rng(P + i).integers(0, V, n)] for i, n in enumerate((50, 1, 96))]
-    N, max_pages, hist = 90, 10, 160
+    N, max_pages, hist = 90, 22000 // P + 1, 160  # (a table with room for so much that the beams are attended together)
     kc, vc = torch.full((2, N, P, nkv, hd), math.nan, device="cuda", dtype=torch.float16)
     kv = b2.paged_kv(kc.data_ptr(), vc.data_ptr(), b2.F16, N, P, nkv, hd)
     new = lambda *s, t=torch.int32, v=0: torch.full(s, v, dtype=t, device="cuda")  # noqa: E731

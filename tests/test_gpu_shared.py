@@ -17,9 +17,10 @@ torch = pytest.importorskip("torch")
 class Shared(Paged):
     """Groups [(rows' lengths, shared positions)]; a length below 0 is a row without a sequence.  The rows of a
     group have table rows of their own (the pages of the shared positions the same) or, with `one`, are tokens of
-    one sequence.  NaN in every place that no row sees."""
+    one sequence.  NaN in every place that no row sees.  `wide`: a table with room for so many positions that the
+    rows are taken together (small calls run row by row)."""
 
-    def __init__(self, groups, nh, nkv, hd, P, dtype, cache, layout="dense", seed=0, one=False, alone=()):
+    def __init__(self, groups, nh, nkv, hd, P, dtype, cache, layout="dense", seed=0, one=False, alone=(), wide=True):
         lens = [max(n, 0) for ls, _ in groups for n in ls] + list(alone)
         at, req = 0, []
         for i, (ls, _) in enumerate(groups):
@@ -39,6 +40,12 @@ class Shared(Paged):
                         n = min(-(-min(lens[r], p) // P), -(-lens[first] // P))
                         self.table[r, :n] = self.table[first, :n]
                 at += len(ls)
+        if wide:
+            per = len(lens) * P * nkv * max(nh // nkv, 8) * hd
+            self.max_pages = max(self.max_pages, 2 ** 28 // per + 1)
+            table = torch.full((self.R, self.max_pages), -1, dtype=torch.int32, device="cuda")
+            table[:, :self.table.shape[1]] = self.table
+            self.table = table
 
     def call(self, window=0, scale=0.0, softcap=0.0, slopes=None, len_add=0, lse=True, q=None, out=None, scratch=None,
              starts=None, prefix=None, n_groups=None, **strides):
@@ -89,8 +96,9 @@ class Shared(Paged):
     ([([130, 131, 300, 129], 128), ([5], 0), ([0, 0], 0), ([64, 20, -1, 65], 64)], 24),
     ([([700] * 9, 700), ([333, 257, 256, 255, 1, 0], 256)], 1)])
 def test_attention_shared(dtype, cache, nh, nkv, hd, groups, P):
-    p = Shared(groups, nh, nkv, hd, P, dtype, cache, seed=nh + hd)
-    p.check(*p.call())
+    for wide in (True, False):
+        p = Shared(groups, nh, nkv, hd, P, dtype, cache, seed=nh + hd, wide=wide)
+        p.check(*p.call())
 
 
 @pytest.mark.parametrize("dtype,cache", COMBOS)
@@ -344,7 +352,7 @@ def test_attention_shared_behind_its_plan():
     g = np.random.default_rng(5)
     cached, fresh = np.array([0, 200, 37, 0, 513]), np.array([150, 1, 40, 0, 1])
     P, nh, nkv, hd, cap, R = 16, 8, 2, 64, 200, 5
-    mp = 40
+    mp = 100
     n_pages = 120
     ids = g.permutation(n_pages).astype(np.int32)
     table, at = np.full((R, mp), -1, np.int32), 0
