@@ -34,7 +34,7 @@ struct BeamArgs {
     float *score, *eos_score;
     double* log_z;             // [rows], NaN: the row offers nothing
     unsigned long long* keys;  // [rows][k1], the row's largest logits in order (0: no more)
-    int n, width, k, k1, eos, cluster, wide;
+    int n, width, k, k1, eos, cluster, wide, sms;
 };
 
 // A beam's score, NaN where it offers nothing.
@@ -100,9 +100,8 @@ __global__ void __launch_bounds__(NT) beam_rows_kernel(const __grid_constant__ B
     }
 }
 
-constexpr int kMergeThreads = 256;
+constexpr int kMergeThreads = 512;
 constexpr int kMergeHeads = 2 * kLogprobMaxTop;                  // entries that give the bound, at most
-constexpr int kMergeMax = kBeamMaxWidth * (kLogprobMaxTop + 1);  // a request's candidates, at most
 
 // How far the first launch's log Z may be off: fp32 terms off by 2 steps and
 // sums by a dozen roundings are 2^-20, the rounding of d (d steps of a term
@@ -124,33 +123,52 @@ struct MergeShared {
     double log_z[kBeamMaxWidth];
     double head[kMergeHeads];
     double part[kMergeThreads / 32];
+    double pow2[32];              // 2^(j/32)
     double bound;
     int fine[kBeamMaxWidth];      // log_z is in 64 bits; 2: it has to be
     int live, n, again;
     Cand best[kLogprobMaxTop + 1];  // in order
-    Cand cand[kMergeMax];
+    Cand cand[1];                   // width x k1 of them
 };
 
-// log Z of a row in 64 bits, by the CTA.
+// e^x for x <= 0, off by 2^-49 of itself to -40 and 2^-45 to -700 (Tang's table method: x = (32 n + j) log(2) / 32 + r,
+// e^x = 2^n 2^(j/32) e^r with e^r as its series to r^6 / 720, |r| <= log(2) / 64;
+// pow2[j] = 2^(j/32)).  In 64 bits that is 12 operations; exp() took twice the time.
+__device__ __forceinline__ double exp64(double x, const double* pow2) {
+    x = fmax(x, -700.0);  // (adds nothing to a sum that holds 1)
+    const double shift = 6755399441055744.0;  // 1.5 2^52: the sum's low bits are the rounded whole number
+    const double t = fma(x, 32.0 * 1.4426950408889634, shift);
+    const int k = __double2loint(t);
+    const double r = fma(t - shift, -0.6931471805599453 / 32.0, x);
+    double p = fma(r, 1.0 / 720.0, 1.0 / 120.0);
+    p = fma(p, r, 1.0 / 24.0);
+    p = fma(p, r, 1.0 / 6.0);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    const double b = pow2[k & 31];
+    p = fma(p * r, b, b);
+    return __hiloint2double(__double2hiint(p) + ((k >> 5) << 20), __double2loint(p));
+}
+
+// log Z of a row whose largest logit is m in 64 bits, by the CTA.
 template <typename T>
-__device__ double log_z64(const T* x, int n, double* part) {
+__device__ double log_z64(const T* x, int n, bool wide, double m, double* part, const double* pow2) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    float m = -INFINITY;
-    for (int i = tid; i < n; i += kMergeThreads) m = fmaxf(m, lf(x[i]));
-    m = max_lanes(m);
-    __syncthreads();
-    if (lane == 0) part[warp] = m;
-    __syncthreads();
-    double M = part[0];
-    for (int w = 1; w < kMergeThreads / 32; w++) M = fmax(M, part[w]);
     double z[4] = {0, 0, 0, 0};
-    for (int i = tid; i < n; i += 4 * kMergeThreads) {
-        double d[4];
+    constexpr int VEC = 16 / sizeof(T), U = 4;  // four 16-byte loads in flight (two rows of 128256 fp32 one by one: 113 us)
+    const int chunks = wide ? n / VEC : 0;
+    for (int c = tid; c < chunks; c += U * kMergeThreads) {
+        LpPack<T, VEC> p[U];
 #pragma unroll
-        for (int j = 0; j < 4; j++) d[j] = i + j * kMergeThreads < n ? (double)lf(x[i + j * kMergeThreads]) - M : -INFINITY;
+        for (int u = 0; u < U; u++)
+            if (c + u * kMergeThreads < chunks) p[u] = reinterpret_cast<const LpPack<T, VEC>*>(x)[c + u * kMergeThreads];
 #pragma unroll
-        for (int j = 0; j < 4; j++) z[j] += exp(d[j]);
+        for (int u = 0; u < U; u++)
+            if (c + u * kMergeThreads < chunks)
+#pragma unroll
+                for (int i = 0; i < VEC; i++) z[i & 3] += exp64((double)lf(p[u].v[i]) - m, pow2);
     }
+    for (int i = chunks * VEC + tid; i < n; i += kMergeThreads) z[0] += exp64((double)lf(x[i]) - m, pow2);
     double s = (z[0] + z[1]) + (z[2] + z[3]);
 #pragma unroll
     for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -159,7 +177,7 @@ __device__ double log_z64(const T* x, int n, double* part) {
     __syncthreads();
     s = 0;
     for (int w = 0; w < kMergeThreads / 32; w++) s += part[w];
-    return M + log(s);
+    return m + log(s);
 }
 
 // One CTA a request.
@@ -195,18 +213,20 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
     };
     // a lower bound of the k-th best: the k-th largest among the first few of every list
     // (one more of each where one of them may be the end token)
-    const int deep = s.live ? min(k1, (k + s.live - 1) / s.live + (a.eos >= 0)) : 0, heads = W * deep;
+    const int deep = s.live ? min(k1, max((k + s.live - 1) / s.live + (a.eos >= 0), kMergeHeads / W)) : 0, heads = W * deep;
     double bound = -INFINITY;
     if (heads <= kMergeHeads) {
-        for (int i = tid; i < heads; i += kMergeThreads) s.head[i] = entry(i / deep, i % deep).score;
+        if (tid < heads) s.head[tid] = entry(tid / deep, tid % deep).score;
         if (tid == 0) s.bound = -INFINITY;
         __syncthreads();
-        for (int i = tid; i < heads; i += kMergeThreads) {
-            const double v = s.head[i];
-            int above = 0;
-            for (int j = 0; j < heads; j++) above += s.head[j] > v || (s.head[j] == v && j < i);
-            if (above == k - 1) s.bound = v;
-        }
+        constexpr int kHelp = kMergeThreads / kMergeHeads;  // lanes that count for one of them
+        const int i = tid / kHelp;
+        const double v = i < heads ? s.head[i] : 0.0;
+        int above = 0;
+        for (int j = tid % kHelp; j < heads; j += kHelp) above += s.head[j] > v || (s.head[j] == v && j < i);
+#pragma unroll
+        for (int o = 1; o < kHelp; o <<= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
+        if (i < heads && above == k - 1) s.bound = v;
         __syncthreads();
         bound = s.bound - 2 * kClose;
     }
@@ -237,9 +257,12 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
         }
         __syncthreads();
         if (!s.again) break;
+        if (tid < 32) s.pow2[tid] = exp2(tid / 32.0);
+        __syncthreads();
         for (int w = 0; w < W; w++) {
             if (s.fine[w] != 2) continue;
-            const double z = log_z64(static_cast<const T*>(a.x) + (row0 + w) * a.ld, a.n, s.part);
+            const double z = log_z64(static_cast<const T*>(a.x) + (row0 + w) * a.ld, a.n, a.wide,
+                                     (double)key_value(a.keys[(row0 + w) * k1]), s.part, s.pow2);
             __syncthreads();
             if (tid == 0) {
                 s.log_z[w] = z;
@@ -278,14 +301,26 @@ cudaError_t go_rows(const BeamArgs& a, int rows, cudaStream_t s) {
     return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
+// 128 threads instead of 256 also where the CTAs of 256, 6 an SM, would go round
+// once and by up to a third again, and those of 128 fit at once (rows of 128256
+// bf16, 256 and 128 threads: 880 rows 70 and 72 us, 896 rows 80 and 72, 1184 rows 91
+// and 82, 1760 rows 113 and 124).  Not with fp32, 5 an SM: 960 rows of 50000 60 and 70.
+template <typename T>
+bool small_ctas(const BeamArgs& a, int rows) {
+    const int round = 6 * a.sms;
+    return a.n <= kLpShortRow || (sizeof(T) == 2 && rows > round && 3LL * rows <= 4LL * round);
+}
+
 template <typename T>
 cudaError_t go(const BeamArgs& a, int rows, cudaStream_t s) {
-    cudaError_t e = a.n <= kLpShortRow ? go_rows<T, 128>(a, rows, s) : go_rows<T, 256>(a, rows, s);
+    cudaError_t e = small_ctas<T>(a, rows) ? go_rows<T, 128>(a, rows, s) : go_rows<T, 256>(a, rows, s);
     if (e != cudaSuccess) return e;
     auto kern = beam_merge_kernel<T>;
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(MergeShared));
+    auto smem = [](int list) { return sizeof(MergeShared) + (size_t)list * sizeof(Cand); };
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)smem(kBeamMaxWidth * (kLogprobMaxTop + 1)));
     if (e != cudaSuccess) return e;
-    return launch_pdl(kern, dim3(rows / a.width), dim3(kMergeThreads), sizeof(MergeShared), s, a);
+    return launch_pdl(kern, dim3(rows / a.width), dim3(kMergeThreads), smem(a.width * a.k1), s, a);
 }
 
 // entries of a row's list: one more where one of them may be the end token
@@ -376,6 +411,7 @@ int launch_beam_select(const void* logits, int dtype, int n, int n_groups, int w
     int c = 1;
     while (c < kLpMaxCluster && rows * 2LL * c <= sms && n / (2 * c) >= 4096) c *= 2;
     a.cluster = c;
+    a.sms = sms;
     const cudaError_t e = dtype == 0   ? go<float>(a, rows, s)
                           : dtype == 1 ? go<__half>(a, rows, s)
                                        : go<__nv_bfloat16>(a, rows, s);

@@ -14,7 +14,7 @@ namespace {
 
 constexpr int kLpBatch = 32;                     // logits a thread takes together
 constexpr int kLpEntries = 16;                   // maxima kept by a thread; longer slices: of several batches each
-constexpr int kLpGroups = 64;                    // groups of threads whose maxima give the bound (k up to half of them)
+constexpr int kLpGroups = 64;                    // groups of threads whose maxima give the bound (twice as many for k past half)
 constexpr int kLpList = 256;                     // batches at the bound, at most, for their candidates to be taken directly
 constexpr int kLpMaxCluster = 8;
 constexpr float kLog2eF = 1.4426950408889634f;
@@ -77,6 +77,7 @@ __device__ __forceinline__ Sums join_lanes(Sums t) {
 
 // A thread's sums, S and T as pairs (even and odd elements)
 struct Acc {
+    static constexpr bool kClamp = true;  // (e^d is multiplied by d, which may be -inf)
     float m = -INFINITY;
     unsigned long long S = 0, T = 0;
 
@@ -117,6 +118,7 @@ struct Acc {
 // (a + b = s + e exactly, Knuth's two-sum), so a large element meets a handful
 // of roundings instead of one with every later element.
 struct AccZ {
+    static constexpr bool kClamp = false;
     float m = -INFINITY, S = 0.0f, rest = 0.0f;
     unsigned long long part[4] = {0, 0, 0, 0};
 
@@ -229,10 +231,10 @@ __device__ __forceinline__ float add_chunks(const LpPack<T, VEC> (&p)[N], A& t) 
         for (int i = 1; i < N * 4; i++) mx = __hmax2(mx, v[i]);
         const float2 f = W::floats(mx);
         const float bm = fmaxf(f.x, f.y), z = t.grow(bm);
+        const unsigned long long z2 = f2_pack(-z, -z);
         // logits that add nothing are raised to where they still add nothing (-inf among them)
         const typename W::V low = W::both(z - fmaxf(256.0f, fabsf(z) * 0.015625f));
-        const unsigned long long z2 = f2_pack(-z, -z);
-        if (W::floats(low).x > -INFINITY) {
+        if (A::kClamp && W::floats(low).x > -INFINITY) {
 #pragma unroll
             for (int i = 0; i < N * 4; i++) {
                 const float2 x = W::floats(__hmax2_nan(v[i], low));
@@ -242,7 +244,7 @@ __device__ __forceinline__ float add_chunks(const LpPack<T, VEC> (&p)[N], A& t) 
 #pragma unroll
             for (int i = 0; i < N * 4; i++) {
                 const float2 x = W::floats(v[i]);
-                t.template add<true>(f2_add(f2_pack(x.x, x.y), z2), i);
+                t.template add<A::kClamp>(f2_add(f2_pack(x.x, x.y), z2), i);
             }
         }
         t.flush();
@@ -260,7 +262,7 @@ __device__ __forceinline__ float add_chunks(const LpPack<T, VEC> (&p)[N], A& t) 
         const unsigned long long z2 = f2_pack(-z, -z);
 #pragma unroll
         for (int i = 0; i < N * VEC; i += 2)
-            t.template add<true>(f2_add(f2_pack(f[i], i + 1 < N * VEC ? f[i + 1] : -INFINITY), z2), i / 2);
+            t.template add<A::kClamp>(f2_add(f2_pack(f[i], i + 1 < N * VEC ? f[i + 1] : -INFINITY), z2), i / 2);
         t.flush();
         return bm;
     }
@@ -334,7 +336,7 @@ template <int NT, typename A>
 __device__ __forceinline__ void slice_sums(const A& acc, int k, LpShared<NT>& s) {
     constexpr int kWarps = LpShared<NT>::kWarps;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int groups = k <= kLpGroups / 2 ? kLpGroups : NT, gl = NT / groups;  // lanes of a group
+    const int groups = k <= kLpGroups / 2 ? kLpGroups : 2 * kLpGroups, gl = NT / groups;  // lanes of a group
     if (tid == 0) s.n_cand = s.n_list = 0;
     if (k > 1) {
         float g = acc.m;
