@@ -47,7 +47,8 @@ __device__ __forceinline__ int sum_before(int x, int* warps, int* all) {
 // ---------------------------------------------------------------------------
 
 constexpr int kForkThreads = 512;
-constexpr int kForkChunk = 256;  // table entries of one warp's turn
+constexpr int kWalk = 4;             // table entries of a lane in flight
+constexpr int kPiece = 32 * kWalk;   // those of one warp's turn
 
 // Every CTA works out for itself which rows take a page (the words are few and
 // stay in L2), so one launch does all; then the rows' entries, in pieces, go
@@ -102,27 +103,32 @@ __global__ void __launch_bounds__(kForkThreads) page_fork_kernel(const __grid_co
     }
     if (status) return;
     const int warp0 = (blockIdx.x * kForkThreads + tid) / 32, n_warps = gridDim.x * kForkThreads / 32;
-    const int chunks = (a.max_pages + kForkChunk - 1) / kForkChunk;
-    const long long items = (long long)R * chunks;
+    const int pieces = (a.max_pages + kPiece - 1) / kPiece;
+    const long long items = (long long)R * pieces;
     for (long long it = warp0; it < items; it += n_warps) {
         const int c = (int)(it / R), r = (int)(it - (long long)c * R);
         const int p = a.parent[r], len = p >= 0 ? a.lens[p] : 0, n = pages_of(len, P);
         if (c == 0 && lane == 0) a.new_lens[r] = len;
-        const int e0 = c * kForkChunk, e1 = min(n, e0 + kForkChunk);
-        if (e0 >= e1) continue;
+        const int e0 = c * kPiece + lane;
+        if (c * kPiece >= n) continue;
         const int32_t* src = a.table + (int64_t)p * a.table_stride;
         int32_t* dst = a.new_table + (int64_t)r * a.new_stride;
         const int swap = taken[r] >= 0 ? len / P : -1;
-        for (int e = e0 + lane; e < e1; e += 32) {
-            int page = src[e];
+        int page[kWalk];
+#pragma unroll
+        for (int j = 0; j < kWalk; j++)
+            if (e0 + 32 * j < n) page[j] = src[e0 + 32 * j];
+#pragma unroll
+        for (int j = 0; j < kWalk; j++) {
+            const int e = e0 + 32 * j;
             if (e == swap) {
                 const int t = taken[r], copy = a.free_pages[t];
-                a.pairs[3 * t] = page;
+                a.pairs[3 * t] = page[j];
                 a.pairs[3 * t + 1] = copy;
                 a.pairs[3 * t + 2] = len % P;
-                page = copy;
+                page[j] = copy;
             }
-            dst[e] = page;
+            if (e < n) dst[e] = page[j];
         }
     }
 }
@@ -140,33 +146,46 @@ struct PageCopyArgs {
 };
 
 constexpr int kCopyThreads = 128;
-constexpr int kCopyLoads = 4;  // 16-byte loads of a thread in flight
-constexpr int kCopyChunks = kCopyThreads * kCopyLoads;
 
-// One CTA's turn: kCopyChunks 16-byte chunks of one page's k or v in one layer.
+// One CTA's turn: 16-byte chunks of one page's k or v in one layer, LOADS to a
+// thread: 8, or 4 where a page is no more than 8 KB.  Bound by HBM: 1.17 GB read and
+// written for pages of 32 KB take 186 us, 6.3 TB/s (4 loads: 189), 130 MB of half
+// pages 25 us (27), 57 MB of pages of 4 KB 11.8 us (8 loads: 14.8).
+template <int LOADS>
 __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(const __grid_constant__ PageCopyArgs a) {
     pdl_trigger();
     pdl_wait();
     const int n = max(0, min(*a.n_pairs, a.max_pairs));
+    constexpr int kCopyChunks = kCopyThreads * LOADS;
     const int per_pos = a.nkv * a.hc;
     const int turns = (int)(((int64_t)a.page_size * per_pos + kCopyChunks - 1) / kCopyChunks);
     const int64_t items = (int64_t)n * 2 * a.layers * turns;
+    const bool narrow = items <= 0x7fffffff;  // divisions of 32 bits where they do
     for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
-        const int turn = (int)(it % turns);
-        int64_t rest = it / turns;
-        const int which = (int)(rest % (2 * a.layers));
-        const int pair = (int)(rest / (2 * a.layers));
+        int turn, which, pair;
+        if (narrow) {
+            const unsigned i = (unsigned)it, rest = i / (unsigned)turns;
+            turn = (int)(i - rest * turns);
+            pair = (int)(rest / (unsigned)(2 * a.layers));
+            which = (int)(rest - (unsigned)pair * (2 * a.layers));
+        } else {
+            const int64_t rest = it / turns;
+            turn = (int)(it - rest * turns);
+            pair = (int)(rest / (2 * a.layers));
+            which = (int)(rest - (int64_t)pair * (2 * a.layers));
+        }
         const int src = a.pairs[3 * (int64_t)pair], dst = a.pairs[3 * (int64_t)pair + 1];
         const int count = min(a.pairs[3 * (int64_t)pair + 2], a.page_size);
         if (src == dst || (unsigned)src >= (unsigned)a.n_pages || (unsigned)dst >= (unsigned)a.n_pages) continue;
         const int64_t chunks = (int64_t)max(count, 0) * per_pos;
+        if ((int64_t)turn * kCopyChunks >= chunks) continue;
         uint16_t* base = (which & 1 ? a.v : a.k) + (which >> 1) * a.layer_stride;
         const uint16_t* from = base + src * a.page_stride;
         uint16_t* to = base + dst * a.page_stride;
-        uint4 v[kCopyLoads];
-        int64_t off[kCopyLoads];
+        uint4 v[LOADS];
+        int64_t off[LOADS];
 #pragma unroll
-        for (int j = 0; j < kCopyLoads; j++) {
+        for (int j = 0; j < LOADS; j++) {
             const int64_t i = (int64_t)turn * kCopyChunks + j * kCopyThreads + threadIdx.x;
             off[j] = -1;
             if (i < chunks) {
@@ -180,7 +199,7 @@ __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(const __grid_co
             }
         }
 #pragma unroll
-        for (int j = 0; j < kCopyLoads; j++)
+        for (int j = 0; j < LOADS; j++)
             if (off[j] >= 0) *reinterpret_cast<uint4*>(to + off[j]) = v[j];
     }
 }
@@ -188,6 +207,28 @@ __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(const __grid_co
 // ---------------------------------------------------------------------------
 // holders, free list
 // ---------------------------------------------------------------------------
+
+// f(page, its place) for the table entries that the lengths hold, a piece of a
+// row at a time, by the warps from `warp` on in steps of `n_warps`.
+template <typename A, typename F>
+__device__ __forceinline__ void walk_table(const A& a, int warp, int n_warps, F f) {
+    const int lane = threadIdx.x & 31, pieces = (a.max_pages + kPiece - 1) / kPiece;
+    const long long items = (long long)a.n_req * pieces;
+    for (long long it = warp; it < items; it += n_warps) {
+        const int c = (int)(it / a.n_req), r = (int)(it - (long long)c * a.n_req);
+        const int n = min(pages_of(a.lens[r], a.page_size), a.max_pages);
+        auto* row = a.table + (int64_t)r * a.table_stride;
+        int page[kWalk];
+#pragma unroll
+        for (int j = 0; j < kWalk; j++) {
+            const int e = c * kPiece + 32 * j + lane;
+            page[j] = e < n ? row[e] : -1;
+        }
+#pragma unroll
+        for (int j = 0; j < kWalk; j++)
+            if (page[j] >= 0) f(page[j], row + c * kPiece + 32 * j + lane);
+    }
+}
 
 constexpr int kPoolThreads = 512;
 constexpr int kPoolBlock = 4 * kPoolThreads;  // pages of one CTA
@@ -208,19 +249,36 @@ __global__ void __launch_bounds__(kPoolThreads) pool_zero_kernel(const __grid_co
 __global__ void __launch_bounds__(kPoolThreads) pool_count_kernel(const __grid_constant__ PoolArgs a) {
     pdl_trigger();
     pdl_wait();
-    const int lane = threadIdx.x & 31;
     const int warp0 = (blockIdx.x * kPoolThreads + threadIdx.x) / 32, n_warps = gridDim.x * kPoolThreads / 32;
-    const int chunks = (a.max_pages + kForkChunk - 1) / kForkChunk;
-    const long long items = (long long)a.n_req * chunks;
-    for (long long it = warp0; it < items; it += n_warps) {
-        const int c = (int)(it / a.n_req), r = (int)(it - (long long)c * a.n_req);
-        const int n = min(pages_of(a.lens[r], a.page_size), a.max_pages);
-        const int32_t* row = a.table + (int64_t)r * a.table_stride;
-        for (int e = c * kForkChunk + lane; e < min(n, (c + 1) * kForkChunk); e += 32) {
-            const int page = row[e];
-            if ((unsigned)page < (unsigned)a.n_pages) atomicAdd(&a.refs[page], 1);
-        }
-    }
+    walk_table(a, warp0, n_warps, [&](int page, const int32_t*) {
+        if (page < a.n_pages) atomicAdd(&a.refs[page], 1);
+    });
+}
+
+// The four launches in one, by a CTA that keeps the counts in its shared memory.
+constexpr int kSmallThreads = 1024;
+constexpr int kSmallPages = 4096;
+constexpr int kSmallEntries = 4096;
+
+__global__ void __launch_bounds__(kSmallThreads) pool_small_kernel(const __grid_constant__ PoolArgs a) {
+    __shared__ int count[kSmallPages], warps[kSmallThreads / 32];
+    pdl_trigger();
+    const int tid = threadIdx.x, per = (a.n_pages + kSmallThreads - 1) / kSmallThreads;
+    for (int i = tid; i < a.n_pages; i += kSmallThreads) count[i] = 0;
+    pdl_wait();
+    __syncthreads();
+    walk_table(a, tid / 32, kSmallThreads / 32, [&](int page, const int32_t*) {
+        if (page < a.n_pages) atomicAdd(&count[page], 1);
+    });
+    __syncthreads();
+    for (int i = tid; i < a.n_pages; i += kSmallThreads) a.refs[i] = count[i];
+    const int i0 = tid * per, i1 = min(a.n_pages, i0 + per);
+    int n = 0, all;
+    for (int i = i0; i < i1; i++) n += count[i] == 0;
+    int at = sum_before<kSmallThreads>(n, warps, &all);
+    for (int i = i0; i < i1; i++)
+        if (count[i] == 0) a.free_pages[at++] = i;
+    if (tid == 0) *a.n_free = all;
 }
 
 // how many pages of each block are free
@@ -287,7 +345,21 @@ struct CompactArgs {
 };
 
 // holes[i]: the i-th lowest free page below U; movers[i]: the i-th highest
-// page in use at U or above, rank[movers[i]] = i.
+// page in use at U or above, rank[movers[i]] = i.  Page p, with `before` free
+// pages before it, into them; the free pages up to it.
+__device__ __forceinline__ int place(const CompactArgs& a, int p, bool free_, int U, int before) {
+    if (free_) {
+        if (p < U) a.holes[before] = p;
+        before++;
+    } else if (p >= U) {
+        const int i = U - 1 - (p - before);  // pages in use above p
+        a.movers[i] = p;
+        a.rank[p] = i;
+    }
+    if (p == U - 1) *a.moves = before;  // the holes below U
+    return before;
+}
+
 __global__ void __launch_bounds__(kPoolThreads) compact_rank_kernel(const __grid_constant__ CompactArgs a) {
     __shared__ int warps[kPoolThreads / 32];
     pdl_trigger();
@@ -306,62 +378,49 @@ __global__ void __launch_bounds__(kPoolThreads) compact_rank_kernel(const __grid
     int all;
     before += sum_before<kPoolThreads>(n, warps, &all);
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const int p = p0 + j;
-        if (p >= a.n_pages) break;
-        if (free_[j]) {
-            if (p < U) a.holes[before] = p;
-            before++;
-        } else if (p >= U) {
-            const int i = U - 1 - (p - before);  // pages in use above p
-            a.movers[i] = p;
-            a.rank[p] = i;
-        }
-        if (p == U - 1) *a.moves = before;  // the holes below U
-    }
+    for (int j = 0; j < 4; j++)
+        if (p0 + j < a.n_pages) before = place(a, p0 + j, free_[j], U, before);
     if (blockIdx.x == 0 && threadIdx.x == 0) {
-        a.info[0] = 0;
         a.info[2] = U;
         if (U == 0) *a.moves = 0;
     }
 }
 
-__global__ void __launch_bounds__(kPoolThreads) compact_apply_kernel(const __grid_constant__ CompactArgs a) {
-    pdl_trigger();
-    pdl_wait();
-    const int tid = blockIdx.x * kPoolThreads + threadIdx.x, n_threads = gridDim.x * kPoolThreads, lane = threadIdx.x & 31;
-    const int U = a.info[2], moves = *a.moves, done = min(moves, a.max_pairs);
+// A table entry that is in use, given its new page if it has one.
+__device__ __forceinline__ void moved(const CompactArgs& a, int page, int32_t* at, int U, int done) {
+    if (page < U || page >= a.n_pages) return;
+    const int refs = a.refs[page], i = __ldcg(a.rank + page);
+    if (refs > 0 && i < done) *at = __ldcg(a.holes + i);
+}
+
+// The moves, and the table entries that they change, by n_threads threads.
+__device__ __forceinline__ void apply(const CompactArgs& a, int tid, int n_threads, int U) {
+    const int moves = __ldcg(a.moves), done = min(moves, a.max_pairs);
     for (int i = tid; i < done; i += n_threads) {
-        a.pairs[3 * (int64_t)i] = a.movers[i];
-        a.pairs[3 * (int64_t)i + 1] = a.holes[i];
+        a.pairs[3 * (int64_t)i] = __ldcg(a.movers + i);
+        a.pairs[3 * (int64_t)i + 1] = __ldcg(a.holes + i);
         a.pairs[3 * (int64_t)i + 2] = a.page_size;
     }
     if (tid == 0) {
+        a.info[0] = 0;
         a.info[1] = done;
-        a.info[3] = done < moves ? a.movers[done] + 1 : U;
+        a.info[3] = done < moves ? __ldcg(a.movers + done) + 1 : U;
     }
-    const int chunks = (a.max_pages + kForkChunk - 1) / kForkChunk;
-    const long long items = (long long)a.n_req * chunks;
-    for (long long it = tid / 32; it < items; it += n_threads / 32) {
-        const int c = (int)(it / a.n_req), r = (int)(it - (long long)c * a.n_req);
-        const int n = min(pages_of(a.lens[r], a.page_size), a.max_pages);
-        int32_t* row = a.table + (int64_t)r * a.table_stride;
-        for (int e = c * kForkChunk + lane; e < min(n, (c + 1) * kForkChunk); e += 32) {
-            const int page = row[e];
-            if (page >= U && page < a.n_pages && a.refs[page] > 0) {
-                const int i = a.rank[page];
-                if (i < done) row[e] = a.holes[i];
-            }
-        }
-    }
+    walk_table(a, tid / 32, n_threads / 32, [&](int page, int32_t* at) { moved(a, page, at, U, done); });
+}
+
+__global__ void __launch_bounds__(kPoolThreads) compact_apply_kernel(const __grid_constant__ CompactArgs a) {
+    pdl_trigger();
+    pdl_wait();
+    apply(a, blockIdx.x * kPoolThreads + threadIdx.x, gridDim.x * kPoolThreads, a.info[2]);
 }
 
 int pool_blocks(int n_pages) { return (n_pages + kPoolBlock - 1) / kPoolBlock; }
 size_t words16(size_t n) { return (n + 3) & ~(size_t)3; }
 
-// CTAs for the rows' entries: a warp for every kForkChunk of them
+// CTAs for the rows' entries: a warp for every kPiece of them
 int entry_ctas(int n_req, int max_pages, int threads, int sms) {
-    const long long items = (long long)n_req * ((max_pages + kForkChunk - 1) / kForkChunk);
+    const long long items = (long long)n_req * ((max_pages + kPiece - 1) / kPiece);
     return (int)std::max<long long>(1, std::min<long long>(2048 / threads * sms, (items + threads / 32 - 1) / (threads / 32)));
 }
 
@@ -400,10 +459,12 @@ int launch_page_copy(const b2_paged_kv& kv, int layers, int64_t layer_stride, co
     a.layers = layers;
     a.max_pairs = max_pairs;
     a.dense = kv.head_stride == kv.hd && kv.pos_stride == (int64_t)kv.nkv * kv.hd;
-    const int64_t turns = ((int64_t)a.page_size * a.nkv * a.hc + kCopyChunks - 1) / kCopyChunks;
+    const int64_t chunks = (int64_t)a.page_size * a.nkv * a.hc;
+    const int loads = chunks <= 4 * kCopyThreads ? 4 : 8;
+    const int64_t turns = (chunks + kCopyThreads * loads - 1) / (kCopyThreads * loads);
     const __int128 items = (__int128)max_pairs * 2 * layers * turns;
-    const cudaError_t e = launch_pdl(page_copy_kernel, dim3((unsigned)std::min<__int128>(items, 16 * sms)),
-                                     dim3(kCopyThreads), 0, s, a);
+    const cudaError_t e = launch_pdl(loads == 4 ? page_copy_kernel<4> : page_copy_kernel<8>,
+                                     dim3((unsigned)std::min<__int128>(items, 16 * sms)), dim3(kCopyThreads), 0, s, a);
     return e == cudaSuccess ? B2_OK : cuda_failed("page copy launch", e, err);
 }
 
@@ -416,6 +477,12 @@ int launch_page_pool(const int32_t* table, int64_t table_stride, const int32_t* 
     if (!sms) return B2_ERR_CUDA;
     const PoolArgs a{table, lens, table_stride, refs, free_pages, n_free, static_cast<int32_t*>(scratch),
                      n_req, page_size, max_pages, n_pages};
+    // (256 pages, 128 entries: 4.2 us, by four launches 6.2; 4096 pages, 4096 entries: 6.2 and 8.3; 8192 pages of
+    // as many entries: 10.3 and 8.3)
+    if (n_pages <= kSmallPages && (int64_t)n_req * max_pages <= kSmallEntries) {
+        const cudaError_t e = launch_pdl(pool_small_kernel, dim3(1), dim3(kSmallThreads), 0, s, a);
+        return e == cudaSuccess ? B2_OK : cuda_failed("page pool launch", e, err);
+    }
     const int blocks = pool_blocks(n_pages);
     cudaError_t e = launch_pdl(pool_zero_kernel, dim3(std::min(4 * sms, (n_pages + kPoolThreads - 1) / kPoolThreads)),
                                dim3(kPoolThreads), 0, s, a);
