@@ -945,23 +945,17 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                         if (rest) mbar_expect_tx(bar, bytes);
                         else mbar_arrive_expect_tx(bar, bytes);
                     }
+                    __syncwarp();
+                    if (a.flat == 2) {
+                        if (whole) tma_eights(to + lane * (G * 128 * BL), map, where >> 3, h, bar);
+                    } else if (whole) {
 #pragma unroll 1
-                    for (int g = 0; g < groups; g++) {  // (uniform over the warp)
-                        const int at = __shfl_sync(0xffffffffu, where, g);
-                        const uint32_t put = to + g * (G * 128 * BL);
-                        if (a.flat == 2) {
-                            if ((by_box >> g) & 1 && one) tma_eights(put, map, at >> 3, h, bar);
-                        } else {
-                            const int pg = a.flat ? 0 : __shfl_sync(0xffffffffu, page, g);
-                            if ((by_box >> g) & 1 && one)
-#pragma unroll 1
-                                for (int r = 0, x = 0; r < G; x++) {  // (a box: of 8 positions where there are blocks)
-                                    tma_rows(put + r * (128 * BL) + x * 1024, map, 64 * x, h, at + r, pg, bar);
-                                    if (x == BL - 1) {
-                                        r += BL == 1 ? G : 8;
-                                        x = -1;
-                                    }
-                                }
+                        for (int r = 0, x = 0; r < G; x++) {  // (a box: of 8 positions where there are blocks)
+                            tma_rows(to + lane * (G * 128 * BL) + r * (128 * BL) + x * 1024, map, 64 * x, h, where + r, a.flat ? 0 : page, bar);
+                            if (x == BL - 1) {
+                                r += BL == 1 ? G : 8;
+                                x = -1;
+                            }
                         }
                     }
                     __syncwarp();
