@@ -404,7 +404,7 @@ struct Tm {
     static constexpr int kTileBytes = kTile * HD * 2;  // K or V rows of a tile, and one term of Q
     static constexpr int kQBufs = QT == 1 ? 2 : 1;
     static constexpr int kQ = kQBufs * QT * kTileBytes;
-    static constexpr int kFixed = 1024 + 15360;  // alignment, then barriers and small tables
+    static constexpr int kFixed = 1024 + 19456;  // alignment, then barriers and small tables
     static constexpr int kFit = (kSharedSmemMax - kFixed - kQ) / kTileBytes;
     static constexpr int kStages = kFit > 8 ? 8 : kFit;
     // V's tiles share the barriers of the two P that they are multiplied with
@@ -413,10 +413,12 @@ struct Tm {
     static constexpr int kAhead = kStages - 2 > 4 ? 4 : kStages - 2;
     static_assert(kStages >= 3, "three tiles must fit");
     static constexpr int kTotal = kFixed + kQ + (kStagesK + kStagesV) * kTileBytes;
-    // tensor memory: two S (P over it, a third term behind it), then T
+    // tensor memory: two S, three where they fit beside two T (P over it, a third term behind it), then T.
+    // (Three S and one T for 128 dimensions: 64 rows behind 32K 147 -> 142 us, but a prompt 128 -> 143.)
     static constexpr int kSCols = PT == 3 ? 192 : 128;
-    static constexpr int kTBufs = 2 * kSCols + 2 * HD <= 512 ? 2 : 1;
-    static_assert(2 * kSCols + kTBufs * HD <= 512, "tensor memory plan");
+    static constexpr int kSBufs = 3 * kSCols + 2 * HD <= 512 ? 3 : 2;
+    static constexpr int kTBufs = kSBufs * kSCols + 2 * HD <= 512 ? 2 : 1;
+    static_assert(kSBufs * kSCols + kTBufs * HD <= 512, "tensor memory plan");
 };
 
 // Tiles [t0, t1) of an item, as the planning warp lays them out for the others.
@@ -429,8 +431,8 @@ constexpr int kPieceStart = 1, kPieceWhole = 2, kPieceOwn = 4, kPieceLast = 8;  
 
 struct SmallShared {
     uint64_t k_full[4], k_empty[4], q_full[2], q_empty[2];
-    uint64_t s_full[2];  // S of tiles j, j + 1 (and where there are two K, their places are free)
-    uint64_t ready[2];   // their P, V and a place for T
+    uint64_t s_full[3];  // S of tiles j, j + 1, j + 2 (and where there are two K, their places are free)
+    uint64_t ready[3];   // their P, V and a place for T
     uint64_t t_full[2];  // their T (and V's places are free)
     uint64_t piece_full[kPieces], piece_empty[kPieces];
     uint32_t tmem;
@@ -438,10 +440,10 @@ struct SmallShared {
     uint32_t bad[8][4];          // positions of a tile whose page does not exist
     Piece piece[kPieces];
     int4 row[kPieces][kTile];    // of a row of the product: first and end position, length, 1 + (all of the row: 2); 0: no row
-    float2 stats[4][kTile];      // m (log2 units) and l of a tile's rows
+    float2 stats[8][kTile];      // m (log2 units) and l of a tile's rows; the exponentials are up to 4 tiles ahead of O
     float factor[kPieces][kTile];  // what an accumulator of S is times for a score
 };
-static_assert(sizeof(SmallShared) <= 15360, "");
+static_assert(sizeof(SmallShared) <= 19456, "");
 
 // Waits for a barrier's phase; by a warp, one answer for all lanes.  A wait that
 // does not end (some 0.1 s at least, 4 s where every try sleeps a microsecond)
@@ -577,7 +579,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
     shared_tiles_kernel(const __grid_constant__ SharedArgs a, const __grid_constant__ CUtensorMap map_k,
                         const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_q) {
     using TM = Tm<HD, QT, PT>;
-    constexpr int NK = TM::kStagesK, NV = TM::kStagesV, NT = TM::kTBufs, QB = TM::kQBufs;
+    constexpr int NK = TM::kStagesK, NV = TM::kStagesV, NS = TM::kSBufs, NT = TM::kTBufs, QB = TM::kQBufs;
     extern __shared__ __align__(1024) uint8_t ssm_raw[];
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ssm_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* const q_sm = base;
@@ -601,9 +603,11 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
         for (int i = 0; i < 2; i++) {
             mbar_init(&s.q_full[i], 1);
             mbar_init(&s.q_empty[i], 1);
+            mbar_init(&s.t_full[i], 1);
+        }
+        for (int i = 0; i < NS; i++) {
             mbar_init(&s.s_full[i], 1);
             mbar_init(&s.ready[i], 4 + kSumWarps + copies);
-            mbar_init(&s.t_full[i], 1);
         }
         for (int i = 0; i < kPieces; i++) {
             mbar_init(&s.piece_full[i], 1);
@@ -634,12 +638,18 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
         // ------------------------------------------------------------ exponentials
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
         const int wg = warp >> 2, quad = warp & 3, m = quad * 32 + lane;
-        const uint32_t s_col = tmem + ((uint32_t)(quad * 32) << 16) + wg * TM::kSCols;
+        const uint32_t s_row = tmem + ((uint32_t)(quad * 32) << 16);
         const float cap = a.softcap;
         const bool plain = !(cap > 0.0f) && !a.slopes;
         float slope = 0.0f;
         if (a.slopes && m % a.hb < hn) slope = a.slopes[head0 + m % a.hb] * kLog2e;
-        int j = 0;
+        int j = 0, sb = 0, lap = 0;
+        auto next_s = [&]() {
+            if (++sb == NS) {
+                sb = 0;
+                lap ^= 1;
+            }
+        };
         Pieces pieces;
         while (const Piece* p = pieces.next(s)) {
             const int slot = (pieces.n - 1) % kPieces;
@@ -647,9 +657,10 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
             const int start = p->start(0), it_hi = p->hi, t1 = p->t1;
             const bool busy = __any_sync(0xffffffffu, row.w != 0);
             bool ok = true;
-            for (int t = p->t0; t < t1; t++, j++) {
+            for (int t = p->t0; t < t1; t++, j++, next_s()) {
                 if ((j & 1) != wg) continue;
-                if (!warp_wait(&s.s_full[wg], (j >> 1) & 1, dead)) {
+                const uint32_t s_col = s_row + sb * TM::kSCols;
+                if (!warp_wait(&s.s_full[sb], lap, dead)) {
                     ok = false;
                     break;
                 }
@@ -752,12 +763,12 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                         for (int c = max(c0, 0); c < min(c1, kTile); c++)
                             if ((bad[c >> 5] >> (c & 31)) & 1) l = __int_as_float(0x7fc00000);
                     }
-                    s.stats[j & 3][m] = make_float2(top, l);
+                    s.stats[j & 7][m] = make_float2(top, l);
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&s.ready[wg]);
+                if (lane == 0) mbar_arrive(&s.ready[sb]);
             }
             if (!ok) break;
             pieces.done(s);
@@ -766,13 +777,19 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
         // ------------------------------------------------------------ O
         constexpr int HC = HD / 2;  // columns of a warp
         const int half = (warp - kSoftWarps) >> 2, quad = warp & 3, m = quad * 32 + lane;
-        const uint32_t t_col = tmem + ((uint32_t)(quad * 32) << 16) + 2 * TM::kSCols + half * HC;
+        const uint32_t t_col = tmem + ((uint32_t)(quad * 32) << 16) + NS * TM::kSCols + half * HC;
         const int rr = m / a.hb, head = head0 + m - rr * a.hb;
         const int d0 = half * HC, dn = min(HC, hd - d0);  // this warp's dimensions
         if (lane == 0)  // (T's places are free)
             for (int i = 0; i < NT; i++) mbar_arrive(&s.ready[i]);
-        int j = 0;
+        int j = 0, freed = NT % NS;  // freed: the tile that gets this one's place for T, of those `ready` knows
         bool ok = true;
+        auto release = [&]() {  // T has been read
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s.ready[freed]);
+            if (++freed == NS) freed = 0;
+        };
         Pieces pieces;
         while (const Piece* p = pieces.next(s)) {
             const int4 row = s.row[(pieces.n - 1) % kPieces][m];
@@ -789,7 +806,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                 if (!ok) continue;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if (busy) {
-                    const float2 st = s.stats[j & 3][m];
+                    const float2 st = s.stats[j & 7][m];
                     const float n = fmaxf(M, st.x), z = n == -INFINITY ? 0.0f : n;
                     const float fo = ex2(M - z), ft = ex2(st.x - z);
                     M = n;
@@ -800,16 +817,16 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                     for (int c = 0; c < HC; c += 16) {
                         uint32_t r[16];
                         tmem_ld16(from + c, r);
+                        if (c + 16 >= HC) release();
 #pragma unroll
                         for (int i = 0; i < 8; i++) {
                             const unsigned long long x = f2_pack(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
                             o[c / 2 + i] = f2_fma(o[c / 2 + i], fo2, f2_mul(x, ft2));
                         }
                     }
+                } else {
+                    release();
                 }
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&s.ready[(j + NT) & 1]);
             }
             const int b = p->row0 + rr, kind = p->kind;
             pieces.done(s);
@@ -934,10 +951,10 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                     const int was = j - slots;
                     if (was >= 0)
                         ok = ok && (value      ? warp_wait(&s.t_full[was & 1], (was >> 1) & 1, dead)
-                                    : NK == 2 ? warp_wait(&s.s_full[was & 1], (was >> 1) & 1, dead)
+                                    : NK == 2 ? warp_wait(&s.s_full[was % NS], (was / NS) & 1, dead)
                                               : warp_wait(&s.k_empty[slot], (was / NK) & 1, dead));
                     if (!ok) break;
-                    uint64_t* bar = value ? &s.ready[j & 1] : &s.k_full[slot];
+                    uint64_t* bar = value ? &s.ready[j % NS] : &s.k_full[slot];
                     const uint32_t to = __shfl_sync(0xffffffffu, ring_s + slot * TM::kTileBytes, 0);
                     const bool one = elected();
                     if (one) {
@@ -999,7 +1016,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                     for (; waiting > leave; waiting--) {
                         const bool v = (kinds >> (waiting - 1)) & 1;
                         const int n = v ? told[1]++ : told[0]++;
-                        if (lane == 0) mbar_arrive(v ? &s.ready[n & 1] : &s.k_full[n % NK]);
+                        if (lane == 0) mbar_arrive(v ? &s.ready[n % NS] : &s.k_full[n % NK]);
                     }
                 };
                 // this lane's rows of a tile: their offset; -1: none there; -2: nor needed
@@ -1025,8 +1042,8 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                 auto issue = [&](const uint16_t* src, const Place& f, bool value) {
                     const int n = value ? issued[1]++ : issued[0]++, slots = value ? NV : NK, slot = n % slots, was = n - slots;
                     if (was >= 0) {
-                        uint64_t* bar = value ? &s.t_full[was & 1] : NK == 2 ? &s.s_full[was & 1] : &s.k_empty[slot];
-                        const uint32_t parity = (value || NK == 2 ? was >> 1 : was / NK) & 1;
+                        uint64_t* bar = value ? &s.t_full[was & 1] : NK == 2 ? &s.s_full[was % NS] : &s.k_empty[slot];
+                        const uint32_t parity = (value ? was >> 1 : NK == 2 ? was / NS : was / NK) & 1;
                         if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
                             cp_wait<0>();  // (what frees it may wait for what is on its way)
                             tell(0);
@@ -1187,19 +1204,22 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
             const int ks = (hd + 15) / 16;
             const uint32_t id_v = uniform(idesc<C>(ks * 16, true)), id_k = uniform(idesc<C>(0, false));
             const uint32_t tm = uniform(tmem);
-            int j = 0, was = 0;  // was: positions of the tile before, in 16s
+            constexpr int LAG = NS - 1;  // S is this many tiles ahead of T
+            int j = 0, was[LAG] = {};    // was: positions of the tiles between, in 16s, the oldest first
+            int sb = 0;                  // S's place
+            int vb = 0, v_lap = 0;       // and that of the next tile whose T is made
             int k_slot = 0, k_lap = 0;
             bool ok = true, k_there = false;  // k_there: the next tile's K was waited for
             auto values = [&](int jj, bool more) {  // T = P V of tile jj
                 // (K first: it is there as a rule, and every wait takes its time)
-                if (more) ok = ok && warp_wait(&s.k_full[k_slot], k_lap & 1, dead);
-                k_there = more;
-                ok = ok && warp_wait(&s.ready[jj & 1], (jj >> 1) & 1, dead);
+                k_there = more && (LAG == 1 || a.box);
+                if (k_there) ok = ok && warp_wait(&s.k_full[k_slot], k_lap & 1, dead);
+                ok = ok && warp_wait(&s.ready[vb], v_lap, dead);
                 if (!ok) return;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t b = uniform(jj & 1), n = uniform(was);
+                const uint32_t b = uniform(jj & 1), n = uniform(was[0]);
                 const uint32_t v = lo_kv + ring_v + (NV == 2 ? b : 0) * (TM::kTileBytes >> 4);
-                const uint32_t pc = tm + b * TM::kSCols, tc = tm + 2 * TM::kSCols + (NT == 2 ? b : 0) * HD;
+                const uint32_t pc = tm + uniform(vb) * TM::kSCols, tc = tm + NS * TM::kSCols + (NT == 2 ? b : 0) * HD;
                 if (elected()) {
                     if (n == kTile / 16) {
 #pragma unroll
@@ -1221,6 +1241,11 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                     mma_commit(&s.t_full[jj & 1]);
                 }
                 __syncwarp();
+                if (++vb == NS) {
+                    vb = 0;
+                    v_lap ^= 1;
+                }
+                for (int i = 0; i + 1 < LAG; i++) was[i] = was[i + 1];
             };
             Pieces pieces;
             while (const Piece* p = pieces.next(s)) {
@@ -1234,8 +1259,8 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                     if (!k_there) ok = ok && warp_wait(&s.k_full[k_slot], k_lap & 1, dead);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t b = uniform(j & 1), ksl = NK == 2 ? b : uniform(k_slot), id = uniform(id_k | (uint32_t)(2 * n16) << 17);
-                    const uint32_t k_sm = lo_kv + ring_k + ksl * (TM::kTileBytes >> 4), sc = tm + b * TM::kSCols;
+                    const uint32_t ksl = uniform(k_slot), id = uniform(id_k | (uint32_t)(2 * n16) << 17);
+                    const uint32_t k_sm = lo_kv + ring_k + ksl * (TM::kTileBytes >> 4), sc = tm + uniform(sb) * TM::kSCols;
                     if (elected()) {
                         if (ks == HD / 16) {
 #pragma unroll
@@ -1258,7 +1283,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                                     acc = 1;
                                 }
                         }
-                        mma_commit(&s.s_full[j & 1]);
+                        mma_commit(&s.s_full[sb]);
                         if (NK != 2) mma_commit(&s.k_empty[k_slot]);
                         if (t == t1 - 1) mma_commit(&s.q_empty[n % QB]);
                     }
@@ -1267,12 +1292,14 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                         k_slot = 0;
                         k_lap++;
                     }
-                    if (j > 0) values(j - 1, t + 1 < t1);
-                    was = n16;
+                    if (++sb == NS) sb = 0;
+                    if (j >= LAG) values(j - LAG, t + 1 < t1);
+                    if (j == 0) was[0] = n16;
+                    else was[LAG - 1] = n16;
                 }
                 if (!ok) break;
             }
-            if (ok && j > 0) values(j - 1, false);
+            for (int i = max(0, j - LAG); ok && i < j; i++) values(i, false);
         }
     }
     if (*dead) {
