@@ -12,6 +12,11 @@
 // Items need not share a maximum either, so a row's pieces (shared, own, and
 // those of an item that was cut) meet in one joining launch.
 //
+// What bounds it: of 64 rows behind 32K shared positions (64 heads on 8 of 128, bf16)
+// 102 GFLOP and 0.13 GB would take 62 us of the tensor cores; the chain of a tile
+// (scores, exponentials, values, one tile's tensor memory waiting for the next) takes
+// 3000 clocks for products of 1100, so 148 us.
+//
 // Split.  The items of the batch, one after another, are a line of units, a
 // tile being one (and an item's start another).  Share s of G takes the units
 // [s W / G, (s + 1) W / G) for every KV head side by side, so the machine is
@@ -28,14 +33,20 @@
 //          j, P being read from tensor memory
 //   0-7    two warpgroups taking tiles in turn: S out of tensor memory, a row to
 //          a thread, the exponentials, P back over S
-//   8-15   O, a half of the dimensions each four: T out of tensor memory, added in fp32 (the tensor cores' own
-//          accumulation cuts instead of rounding, which over a long row pulls
-//          towards zero); at an item's end the result or the piece
+//   8-15   O, a half of the dimensions each four: T out of tensor memory, added in
+//          fp32 (the tensor cores' own accumulation cuts instead of rounding, which
+//          over a long row pulls towards zero); at an item's end the result or the piece
 //
-// Rounding.  As in attention_paged.cu: K and V as they are; fp32 rows scaled per
-// row by a power of two and split into 2 fp16 or 3 bf16 terms; probabilities
-// times 2^14 in 2 terms (3 for fp32 rows over a bf16 cache); sums, maxima and
-// O in fp32, rounded once.
+// Rounding.  K and V as they are; fp32 rows scaled per row by a power of two and
+// split into 2 fp16 or 3 bf16 terms, and their probabilities times 2^14 into as
+// many (22 bits or more: what fp32 results need).  16-bit rows as they are, their
+// probabilities in one term of the cache's type: a weight is off by half a step,
+// and the result, an average, by less than its own rounding.  Sums, maxima and O in
+// fp32, rounded once.
+//
+// Measured (B200, graphs, all three launches): 8 requests of 8 beams over up to 32K, 32 heads
+// on 8 of 128, fp32 rows 103 us (row by row 389); 64 rows behind 32K, 64 heads on 8,
+// bf16 148 (1010); a prompt of 2048 tokens, the same heads 130 (1064).
 //
 // A value that one row of an item sees and another does not meets a weight of 0
 // there, and 0 times infinity or NaN is NaN: a row whose result is not finite is
