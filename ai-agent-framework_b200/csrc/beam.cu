@@ -280,12 +280,13 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
     }
 }
 
+constexpr size_t kPlainSmem = 48 * 1024;  // shared memory that a launch may ask for as it is
+
 template <typename T, int NT>
 cudaError_t go_rows(const BeamArgs& a, int rows, cudaStream_t s) {
     constexpr int W = 16 / sizeof(T);
     auto kern = a.wide ? beam_rows_kernel<T, W, NT> : beam_rows_kernel<T, 1, NT>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(LpShared<NT>));
-    if (e != cudaSuccess) return e;
+    static_assert(sizeof(LpShared<NT>) <= kPlainSmem, "no attribute to set");
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(rows * a.cluster));
     cfg.blockDim = dim3(NT);
@@ -316,11 +317,10 @@ cudaError_t go(const BeamArgs& a, int rows, cudaStream_t s) {
     cudaError_t e = small_ctas<T>(a, rows) ? go_rows<T, 128>(a, rows, s) : go_rows<T, 256>(a, rows, s);
     if (e != cudaSuccess) return e;
     auto kern = beam_merge_kernel<T>;
-    auto smem = [](int list) { return sizeof(MergeShared) + (size_t)list * sizeof(Cand); };
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)smem(kBeamMaxWidth * (kLogprobMaxTop + 1)));
+    const size_t smem = sizeof(MergeShared) + (size_t)a.width * a.k1 * sizeof(Cand);
+    if (smem > kPlainSmem) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
-    return launch_pdl(kern, dim3(rows / a.width), dim3(kMergeThreads), smem(a.width * a.k1), s, a);
+    return launch_pdl(kern, dim3(rows / a.width), dim3(kMergeThreads), smem, s, a);
 }
 
 // entries of a row's list: one more where one of them may be the end token

@@ -159,6 +159,15 @@ def test_attention_shared_thousands_of_rows():
     p.check(*p.call())
 
 
+def test_attention_shared_thousands_of_groups():
+    """More groups than the laying of the line keeps at once, of one or two rows or none."""
+    groups = [([40 + i % 5, 45][:i % 3], 30 + i % 13) for i in range(3100)]
+    p = Shared(groups, 2, 1, 64, 16, "bf16", "bf16")
+    assert len(p.lens) == 3099
+    p.lens, p.prefix, p.starts = p.lens, p.prefix[:-3], p.starts[:-3]  # (fewer groups than rows, else each row runs alone)
+    p.check(*p.call())
+
+
 def test_attention_shared_equals_paged():
     """The same numbers as b2_attention_paged to the rounding of the sums, whatever the groups say is shared."""
     p = Shared([([513 + 5 * i for i in range(20)], 512), ([40], 40)], 16, 4, 128, 16, "f32", "f16")
