@@ -448,7 +448,7 @@ struct SmallShared {
     uint64_t piece_full[kPieces], piece_empty[kPieces];
     uint32_t tmem;
     int dead;                    // a wait gave up
-    uint32_t bad[8][4];          // positions of a tile whose page does not exist
+    alignas(16) uint32_t bad[8][4];          // positions of a tile whose page does not exist
     Piece piece[kPieces];
     int4 row[kPieces][kTile];    // of a row of the product: first and end position, length, 1 + (all of the row: 2); 0: no row
     float2 stats[8][kTile];      // m (log2 units) and l of a tile's rows; the exponentials are up to 4 tiles ahead of O
@@ -659,6 +659,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
         const bool plain = !(cap > 0.0f) && !a.slopes;
         float slope = 0.0f;
         if (a.slopes && m % a.hb < hn) slope = a.slopes[head0 + m % a.hb] * kLog2e;
+        const float f_all = cap > 0.0f ? a.scale / cap : a.scale * kLog2e;
         int j = 0, sb = 0, lap = 0;
         auto next_s = [&]() {
             if (++sb == NS) {
@@ -685,7 +686,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                     const int p0 = start + t * kTile, c0 = row.x - p0, c1 = row.y - p0;
                     const int chunks = (min(kTile, it_hi - p0) + 31) / 32;
                     const bool mask = __any_sync(0xffffffffu, c0 > 0 || c1 < 32 * chunks);
-                    float f = QT == 1 ? (cap > 0.0f ? a.scale / cap : a.scale * kLog2e) : s.factor[slot][m];
+                    float f = QT == 1 ? f_all : s.factor[slot][m];
                     if (!plain) {  // cap and slope
 #pragma unroll 1
                         for (int c = 0; c < 32 * chunks; c += 16) {
@@ -774,7 +775,8 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                     const float2 ls = f2_unpack(l2);
                     float l = ls.x + ls.y;
                     const uint32_t* bad = s.bad[j & 7];
-                    if (bad[0] | bad[1] | bad[2] | bad[3]) {
+                    const uint4 any = *reinterpret_cast<const uint4*>(bad);
+                    if (any.x | any.y | any.z | any.w) {
 #pragma unroll 1
                         for (int c = max(c0, 0); c < min(c1, kTile); c++)
                             if ((bad[c >> 5] >> (c & 31)) & 1) l = __int_as_float(0x7fc00000);
