@@ -13,9 +13,9 @@
 // those of an item that was cut) meet in one joining launch.
 //
 // What bounds it: of 64 rows behind 32K shared positions (64 heads on 8 of 128, bf16)
-// 102 GFLOP and 0.13 GB would take 62 us of the tensor cores; the chain of a tile
+// 70 GFLOP would take 42 us of the tensor cores; the chain of a tile
 // (scores, exponentials, values, one tile's tensor memory waiting for the next) takes
-// 3000 clocks for products of 1100, so 148 us.
+// 3000 clocks for products of 1100, so 145 us.
 //
 // Split.  The items of the batch, one after another, are a line of units, a
 // tile being one (and an item's start another).  Share s of G takes the units
@@ -45,8 +45,8 @@
 // fp32, rounded once.
 //
 // Measured (B200, graphs, all three launches): 8 requests of 8 beams over up to 32K, 32 heads
-// on 8 of 128, fp32 rows 103 us (row by row 389); 64 rows behind 32K, 64 heads on 8,
-// bf16 148 (1010); a prompt of 2048 tokens, the same heads 130 (1064).
+// on 8 of 128, fp32 rows 102 us (row by row 389); 64 rows behind 32K, 64 heads on 8,
+// bf16 145 (1010); a prompt of 2048 tokens, the same heads 128 (1064).
 //
 // A value that one row of an item sees and another does not meets a weight of 0
 // there, and 0 times infinity or NaN is NaN: a row whose result is not finite is

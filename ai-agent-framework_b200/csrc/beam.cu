@@ -12,6 +12,12 @@
 // what reaches the bound is ordered by counting, in 64 bits.  Two beams' log Z
 // are known to fp32 sums; where that leaves the order of two neighbours open
 // (one pair in some 10^4), the CTA takes the two rows' log Z in 64 bits.
+//
+// Bound by the pass: 64 requests of 16 beams over 128256 bf16 logits, 263 MB, take 78 us
+// with the histories' reordering (40 us of HBM; the pass 65, with exponential units and issue
+// slots half busy, the lists 8, the histories 7, overlapped in part); 4 beams of one
+// request over 152064 fp32 14.5 us, launches all of it.  A cluster for each request that shares
+// the sums in 64 bits lost: 105 -> 115 us where one was needed, 14.5 -> 16.5 where none was.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
