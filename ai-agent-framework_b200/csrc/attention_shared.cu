@@ -1664,12 +1664,17 @@ size_t layout(int batch, int nh, int nkv, int hd, int sms, uint8_t* base, Shared
 //   64 / 1, 128, bf16     4 x 4   2080        1         28.8         28.8
 //   32 / 8, 128, fp32     8 x 8   2080        4         76.0         47.3
 //   64 / 8, 128, bf16     1 x 16  8224        4         71.6         37.0
-// With no more rows than groups there is nothing to share: 64 x 1 rows, 64 / 8
-// heads, 2080 positions take 97 us row by row and 129 shared.  What is held
-// against 2^28 is what the table has room for, since the lengths are on the device.
+// Positions: the window, or what the table has room for, since the lengths are on
+// the device (16 requests of 1 to 8 rows, window 4096 of 9336, 14 / 2 heads of 64: 22.6
+// and 37; 139 rows of one sequence, window 3: 12.4 and 22.6).
+// Where groups have fewer than two rows on average there is too little to share,
+// however they lie: rows that share nothing take 1.3 to 1.7 times as long in the
+// tiles (64 x 1 rows of 2080 positions, 64 / 8 heads: 97 and 129; 62 rows in 43 groups,
+// 28 / 4 heads of 64, fp32: 35 and 127).
 bool row_by_row(const b2_paged_kv& kv, const b2_paged_attn_opts& o, int batch, int n_groups) {
-    const double positions = (double)batch * o.max_pages * kv.page_size;
-    return kv.hd > 128 || n_groups >= batch || positions * std::max(o.nh, 8 * kv.nkv) * kv.hd <= (double)(1 << 28);
+    const double room = (double)o.max_pages * kv.page_size;
+    const double positions = batch * (o.window > 0 ? std::min(room, (double)o.window) : room);
+    return kv.hd > 128 || batch < 2LL * n_groups || positions * std::max(o.nh, 8 * kv.nkv) * kv.hd <= (double)(1 << 28);
 }
 
 size_t attention_shared_scratch(int batch, int nh, int nkv, int hd, int sms) {

@@ -609,9 +609,10 @@ int b2_page_compact(int32_t* table, int64_t table_stride, const int32_t* lens, i
  * the products take the probabilities of 16-bit rows rounded to the cache's
  * type (half a step of it in a weight), of fp32 rows in 22 bits or more.  Every
  * row runs for itself, as in b2_attention_paged, where the head dimension is
- * past 128, where there are no more rows than groups, and where batch *
- * max_pages * page_size * hd * max(nh, 8 * nkv) is at most 2^28, below which that is
- * faster; so max_pages should be no more than a step may need.  d_scratch:
+ * past 128, where groups have fewer than two rows on average, and where batch *
+ * positions * hd * max(nh, 8 * nkv) is at most 2^28 (positions: the window, or max_pages
+ * * page_size if that is less), which is faster there; so max_pages should be no
+ * more than a step may need.  d_scratch:
  * b2_attention_shared_scratch_bytes(batch, nh, nkv, hd) bytes on 16 bytes, no
  * contents needed. */
 int64_t b2_attention_shared_scratch_bytes(int32_t batch, int32_t nh, int32_t nkv, int32_t hd);

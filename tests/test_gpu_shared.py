@@ -160,11 +160,10 @@ def test_attention_shared_thousands_of_rows():
 
 
 def test_attention_shared_thousands_of_groups():
-    """More groups than the laying of the line keeps at once, of one or two rows or none."""
-    groups = [([40 + i % 5, 45][:i % 3], 30 + i % 13) for i in range(3100)]
+    """More groups than the laying of the line keeps at once, of up to five rows or none."""
+    groups = [([40 + i % 5, 45, 33, 50, 41][:i % 6], 30 + i % 13) for i in range(2400)]
     p = Shared(groups, 2, 1, 64, 16, "bf16", "bf16")
-    assert len(p.lens) == 3099
-    p.lens, p.prefix, p.starts = p.lens, p.prefix[:-3], p.starts[:-3]  # (fewer groups than rows, else each row runs alone)
+    assert len(p.lens) >= 2 * len(groups)
     p.check(*p.call())
 
 
@@ -178,6 +177,20 @@ def test_attention_shared_equals_paged():
             assert float((o - a).norm() / a.norm()) < 2.0 ** -19 and float((ls - la).abs().max()) < 2.0 ** -17
     p.call(prefix=[512, 40])
     p.check(*p.call(prefix=[512, 40]))
+
+
+@pytest.mark.parametrize("dtype,cache", COMBOS)
+@pytest.mark.parametrize("window,rows", [(64, 700), (300, 150)])
+@pytest.mark.parametrize("one", [False, True])
+def test_attention_shared_windows(dtype, cache, window, rows, one):
+    """Windows in rows enough that they are taken together; pages below every window of a group are not looked at."""
+    lens = [900 + i % 97 for i in range(rows - 60)] if not one else [310 + i for i in range(rows - 60)]
+    groups = [(lens, 890 if not one else max(lens)), ([200 + i for i in range(50)], 250), ([5] * 9 + [0], 5)]
+    p = Shared(groups, 96, 12, 64, 16, dtype, cache, one=one)
+    for r in range(p.R):  # (a table row of the first group)
+        if (r == 0) if one else r < len(lens):
+            p.table[r, :(min(lens) - window) // 16] = 10 ** 6
+    p.check(*p.call(window=window), window=window)
 
 
 def test_attention_shared_values_that_others_do_not_see():
