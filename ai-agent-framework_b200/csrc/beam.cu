@@ -156,7 +156,8 @@ __device__ __forceinline__ double exp64(double x, const double* pow2) {
     return __hiloint2double(__double2hiint(p) + ((k >> 5) << 20), __double2loint(p));
 }
 
-// log Z of a row whose largest logit is m in 64 bits, by the CTA.
+// log Z of a row whose largest logit is m in 64 bits, by the CTA: bound by the
+// SM's 64-bit units, some 20 us for 128256 logits.
 template <typename T>
 __device__ double log_z64(const T* x, int n, bool wide, double m, double* part, const double* pow2) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
