@@ -606,8 +606,8 @@ int b2_page_compact(int32_t* table, int64_t table_stride, const int32_t* lens, i
  * rows that get NaN; no row is touched by another's pages, lengths or values.
  * Rows in no group attend alone.  Groups whose starts do not ascend give rows
  * without meaning, no access out of range.  Scores, softmax and sums are fp32;
- * the products take the probabilities of 16-bit rows rounded to the cache's
- * type (half a step of it in a weight), of fp32 rows in 22 bits or more.  Every
+ * the products take the probabilities of 16-bit rows in two terms of the
+ * cache's type (16 bits of BF16, 22 of F16), of fp32 rows in 22 bits or more.  Every
  * row runs for itself, as in b2_attention_paged, where the head dimension is
  * past 128, where groups have fewer than two rows on average, and where batch *
  * positions * hd * max(nh, 8 * nkv) is at most 2^28 (positions: the window, or max_pages
