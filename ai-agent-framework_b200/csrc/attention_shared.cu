@@ -178,6 +178,8 @@ __device__ __forceinline__ void lay_line(const SharedArgs& a) {
         for (int i = tid; i < a.n_groups; i += kPlanThreads) s.prefix[i] = a.prefix[i];
     }
     auto start_of = [&](int g) { return near ? s.starts[g] : a.starts[g]; };
+    // (at most the longest length there is: kNoLimit marks a row's own positions)
+    auto prefix_of = [&](int g) { return (int)min((long long)max(near ? s.prefix[g] : a.prefix[g], 0), kMaxLen); };
 
     int items = 0;
     long long units = 0;
@@ -198,7 +200,7 @@ __device__ __forceinline__ void lay_line(const SharedArgs& a) {
             if (b < a.batch) {
                 g = last_at(a.n_groups, [&](int x) { return start_of(x) <= b; });
                 if (start_of(g) > b || start_of(g + 1) <= b) g = -1;
-                else prefix = max(near ? s.prefix[g] : a.prefix[g], 0);
+                else prefix = prefix_of(g);
             }
             s.lo[i] = sq[u].lo;
             s.hi[i] = min(sq[u].len, prefix);
@@ -221,7 +223,7 @@ __device__ __forceinline__ void lay_line(const SharedArgs& a) {
             int prefix = 0;
             if (g >= 0) {
                 first[k] = max(start_of(g), 0);
-                prefix = max(near ? s.prefix[g] : a.prefix[g], 0);
+                prefix = prefix_of(g);
                 if ((b - first[k]) % R == 0) {
                     Item x{};
                     x.row0 = b;

@@ -30,3 +30,12 @@ def test_constant_values_come_out_as_they_are(dtype, one, hd):
     p.q[..., 0] = 1
     out, _ = p.call(scale=-math.log(0.5 * (1 + eps / 2)))
     assert bool((out == 1.5).all()), out.unique().tolist()
+
+
+@pytest.mark.parametrize("dtype,cache", [("f32", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("prefix", [2 ** 31 - 1, 2 ** 31 - 2])
+@pytest.mark.parametrize("groups", [[list(range(270, 310)), [40, 41], [700] * 3], [list(range(9000, 9030))]])
+def test_prefix_of_everything(dtype, cache, prefix, groups):
+    """A prefix past every length: all of it is shared, whether an item is written whole (many of them) or in pieces."""
+    p = Shared([(ls, max(ls)) for ls in groups for _ in range(40 if len(groups) > 1 else 1)], 16, 2, 64, 16, dtype, cache, one=True)
+    p.check(*p.call(prefix=[prefix] * len(p.prefix)))
