@@ -133,7 +133,7 @@ struct MergeShared {
     double bound;
     int fine[kBeamMaxWidth];      // log_z is in 64 bits; 2: it has to be
     int live, n, again;
-    Cand best[kLogprobMaxTop + 1];  // in order
+    Cand best[kLogprobMaxTop];      // in order
     Cand cand[1];                   // width x k1 of them
 };
 
@@ -250,17 +250,24 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
             const Cand c = s.cand[i];
             int above = 0;
             for (int j = 0; j < n; j++) above += s.cand[j].before(c);
-            if (above <= k) s.best[above] = c;
+            if (above < k) s.best[above] = c;
         }
         __syncthreads();
-        // neighbours of two beams, too close for what is known of them
-        for (int i = tid; i < min(n - 1, k); i += kMergeThreads) {
-            const int u = (int)(s.best[i].at >> 32), v = (int)(s.best[i + 1].at >> 32);
-            if (u != v && s.best[i].score - s.best[i + 1].score < kClose && (s.fine[u] != 1 || s.fine[v] != 1)) {
+        // two beams too close for what is known of them: neighbours among the k best, and the k-th
+        // with any that comes behind it (a beam's own next ones may lie between)
+        auto close = [&](const Cand& x, const Cand& y) {
+            const int u = (int)(x.at >> 32), v = (int)(y.at >> 32);
+            if (u != v && x.score - y.score < kClose && (s.fine[u] != 1 || s.fine[v] != 1)) {
                 atomicCAS(&s.fine[u], 0, 2);
                 atomicCAS(&s.fine[v], 0, 2);
                 s.again = 1;
             }
+        };
+        for (int i = tid; i < min(n, k) - 1; i += kMergeThreads) close(s.best[i], s.best[i + 1]);
+        if (n > k) {
+            const Cand last = s.best[k - 1];
+            for (int i = tid; i < n; i += kMergeThreads)
+                if (last.before(s.cand[i])) close(last, s.cand[i]);
         }
         __syncthreads();
         if (!s.again) break;
