@@ -498,7 +498,9 @@ int b2_logprobs(const void* logits, int32_t dtype, int32_t n, int32_t rows, int6
  * gives every new beam the block table of the beam that it continues, b2_page_copy
  * copies the pages that the two must not share, in all layers at once, and
  * b2_page_pool lists the pages that no row holds any longer; b2_page_plan and
- * b2_rope_append place the new tokens; b2_attention_shared attends, reading what
+ * b2_rope_append place the new tokens, and b2_page_pool once more (the table
+ * and lengths that the plan wrote) takes the plan's pages off the list, which
+ * the plan leaves as it was; b2_attention_shared attends, reading what
  * the rows of a request share once.  b2_page_compact, now and then, moves the
  * pages in use to the front of the pool.  Conventions as for the paged serving
  * step above: device pointers on the current device, asynchronous, no
