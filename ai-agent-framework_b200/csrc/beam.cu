@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(NT) beam_rows_kernel(const __grid_constant__ B
         cl.sync();
         if (rank == 0) {
             if (warp == 0) {
-                const Sums u = join_lanes(lane < C ? cl.map_shared_rank(&s, lane)->row : Sums{-INFINITY, 0.0f, 0.0f});
+                const Sums u = AccZ::join(lane < C ? cl.map_shared_rank(&s, lane)->row : Sums{-INFINITY, 0.0f, 0.0f});
                 __syncwarp();
                 if (lane == 0) s.row = u;
             }
@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(NT) beam_rows_kernel(const __grid_constant__ B
     }
     const Sums r = s.row;
     const bool ok = fabsf(r.m) < INFINITY && r.S == r.S;
-    const double z = ok ? (double)r.m + log((double)r.S) : nan;
+    const double z = ok ? (double)r.m + log((double)r.S + (double)r.T) : nan;
     for (int i = tid; i < a.k1; i += NT) a.keys[row * a.k1 + i] = s.top[i];
     if (tid == 0) {
         a.log_z[row] = z;
@@ -110,9 +110,9 @@ constexpr int kMergeThreads = 512;
 constexpr int kMergeHeads = 2 * kLogprobMaxTop;                  // entries that give the bound, at most
 
 // How far the first launch's log Z may be off: fp32 terms off by 2 steps and
-// sums by a dozen roundings are 2^-20, the rounding of d (d steps of a term
-// e^d) adds less than that.  Candidates of two beams that are closer than
-// twice this are told apart by log Z in 64 bits.
+// sums by the roundings of those taken together are 2^-20, the rounding of d (d
+// steps of a term e^d) adds less than that.  Candidates of two beams that are closer
+// than twice this are told apart by log Z in 64 bits.
 constexpr double kClose = 2.0 / (1 << 18);
 
 // Candidates in order: score down, then place (row, then token) up.

@@ -56,7 +56,7 @@ __device__ __forceinline__ float max_lanes(float x) {
 }
 
 struct Sums {
-    float m, S, T;  // T in units of log 2: sum (x - m) log2(e) e^(x - m)
+    float m, S, T;  // T in units of log 2: sum (x - m) log2(e) e^(x - m); of an AccZ: what S leaves of its sum
 };
 
 // t with its maximum raised to m
@@ -111,12 +111,21 @@ struct Acc {
         const float2 s = f2_unpack(S), t = f2_unpack(T);
         return Sums{m, s.x + s.y, t.x + t.y};
     }
+    static __device__ __forceinline__ Sums join(Sums t) { return join_lanes(t); }
 };
 
+// a + b, and what its rounding leaves (a + b = s + rest exactly, Knuth's two-sum)
+__device__ __forceinline__ float two_sum(float a, float b, float& rest) {
+    const float s = __fadd_rn(a, b), bb = __fsub_rn(s, a);
+    rest = __fadd_rn(__fsub_rn(a, __fsub_rn(s, bb)), __fsub_rn(b, bb));
+    return s;
+}
+
 // A thread's S alone, closer: elements taken together are summed on their own,
-// in four chains, and that sum enters S with what the rounding leaves kept
-// (a + b = s + e exactly, Knuth's two-sum), so a large element meets a handful
-// of roundings instead of one with every later element.
+// in four chains, and that sum enters S with what the rounding leaves kept, from
+// thread to thread too, so a large element meets a handful of roundings instead
+// of one with every later element, and what is small beside it is not lost: the
+// log of a sum of 1 and little more is that little to its own precision.
 struct AccZ {
     static constexpr bool kClamp = false;
     float m = -INFINITY, S = 0.0f, rest = 0.0f;
@@ -143,12 +152,25 @@ struct AccZ {
     }
     __device__ __forceinline__ void flush() {
         const float2 p = f2_unpack(f2_add(f2_add(part[0], part[1]), f2_add(part[2], part[3])));
-        const float b = p.x + p.y, s = __fadd_rn(S, b), bb = __fsub_rn(s, S);
-        rest += __fadd_rn(__fsub_rn(S, __fsub_rn(s, bb)), __fsub_rn(b, bb));
-        S = s;
+        float left;
+        S = two_sum(S, p.x + p.y, left);
+        rest += left;
         part[0] = part[1] = part[2] = part[3] = 0;
     }
-    __device__ __forceinline__ Sums sums() const { return Sums{m, S + rest, 0.0f}; }
+    __device__ __forceinline__ Sums sums() const { return Sums{m, S, rest}; }
+    // the warp's sum, in every lane (its rest may differ there in the last bits)
+    static __device__ __forceinline__ Sums join(Sums t) {
+        const float nm = max_lanes(t.m), f = lex2(max_nan((t.m - (nm == -INFINITY ? 0.0f : nm)) * kLog2eF, -150.0f));
+        const float p = __fmul_rn(t.S, f);
+        t = Sums{nm, p, fmaf(t.T, f, fmaf(t.S, f, -p))};
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            float left;
+            t.S = two_sum(t.S, __shfl_xor_sync(0xffffffffu, t.S, o), left);
+            t.T += __shfl_xor_sync(0xffffffffu, t.T, o) + left;
+        }
+        return t;
+    }
 };
 
 // 16-bit logits two at a time: the larger (a NaN loses), the larger (a NaN
@@ -343,7 +365,7 @@ __device__ __forceinline__ void slice_sums(const A& acc, int k, LpShared<NT>& s)
         for (int o = 1; o < gl; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
         if (tid % gl == 0) s.gmax[tid / gl] = g;
     }
-    const Sums t = join_lanes(acc.sums());
+    const Sums t = A::join(acc.sums());
     if (lane == 0) s.part[warp] = t;
     __syncthreads();
     if (k == 1 && tid == 0) {
@@ -364,7 +386,7 @@ __device__ __forceinline__ void slice_sums(const A& acc, int k, LpShared<NT>& s)
         if (above == k - 1) s.thr = g;
     }
     if (warp == kWarps - 1) {
-        const Sums u = join_lanes(lane < kWarps ? s.part[lane] : Sums{-INFINITY, 0.0f, 0.0f});
+        const Sums u = A::join(lane < kWarps ? s.part[lane] : Sums{-INFINITY, 0.0f, 0.0f});
         if (lane == 0) s.row = u;
     }
     __syncthreads();

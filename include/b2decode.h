@@ -513,14 +513,16 @@ int b2_logprobs(const void* logits, int32_t dtype, int32_t n, int32_t rows, int6
  * 30), the beams of a request one after another; scores[row] is the sum of a
  * beam's log probabilities so far (NULL: all 0).  The candidate (row, v) has
  *   scores[row] + logits[row][v] - log(sum of e^logits[row]),
- * taken in 64 bits; parent / token / score [n_groups][k] get the k largest in
- * order, equal ones by lowest row, then lowest v (parent: the row, counted
- * over all requests; score rounded once).  Nothing continues with a logit of
+ * and parent / token / score [n_groups][k] get the k largest in order, equal
+ * ones by lowest row, then lowest v (parent: the row, counted over all
+ * requests).  The order is that of sums in 64 bits.  score has fp32
+ * exponentials behind it: off by up to 2^-18, some 1e-8 as a rule and less where
+ * a token is nearly certain, then rounded once.  Nothing continues with a logit of
  * -inf, from a beam whose score is -inf, +inf or NaN, whose logits hold a NaN
  * or +inf or are all -inf; places that are left get -1, -1, -inf.  eos >= 0
- * (below n): no candidate has that token; its own score in every row goes to
- * eos_score[rows] (may be NULL; -inf where the row offers none).  width, k up to 64, k up to
- * n, n up to 2^30.  d_scratch: b2_beam_select_scratch_bytes(...) bytes on 16
+ * (below n): no candidate has that token; its own score in every row, as close,
+ * goes to eos_score[rows] (may be NULL; -inf where the row offers none).
+ * width, k up to 64, k up to n, n up to 2^30.  d_scratch: b2_beam_select_scratch_bytes(...) bytes on 16
  * bytes, no contents needed. */
 int64_t b2_beam_select_scratch_bytes(int32_t n, int32_t n_groups, int32_t width, int32_t k);
 int b2_beam_select(const void* logits, int32_t dtype, int32_t n, int32_t n_groups, int32_t width, int64_t ld,

@@ -1,9 +1,11 @@
 """The beam search's operators where two candidates, two threads or two sizes meet
 at a border."""
+import math
+
 import pytest
 
 from test_gpu_beam import Select
-from test_gpu_paged import DT
+from test_gpu_paged import DT, E32
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -22,3 +24,30 @@ def test_doubled_logits_at_the_last_place(dtype, W, k):
     best = d.amax(1) - torch.logsumexp(d, 1)
     near = 2e-7 * torch.rand(G * W, device="cuda", dtype=torch.float64, generator=g)
     Select(x, n, G, W, k, -1, (near - 1.0 - best).float()).call().check()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("pad", [0, 1])
+def test_scores_of_a_sure_token(dtype, pad):
+    """One logit far above the others, which lie within 1 of 0: log p = -log(1 + r) with r = sum e^(x - m).  Every
+    term of r is off by at most 2 steps in its exponential and in each factor that raises its reference (3 2^-22),
+    and by 2.25 half steps of |d| < 30 in d log2(e) (2^-17.9): 2^-17 in all.  The up to 31 terms that are summed
+    with the largest, some 32 e^2 / n of r at most, may be lost there.  The score is rounded once."""
+    n, G = 65536, 12
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = (2 * torch.rand(G, n + pad, device="cuda", generator=g) - 1).to(DT[dtype][0])
+    at = torch.randint(1, n, (G, 1), device="cuda", generator=g)
+    x.scatter_(1, at, torch.linspace(14, 28, G, device="cuda")[:, None].to(x.dtype))
+    lp = torch.log_softmax(x[:, :n].double(), 1)
+    d = (x[:, :n].double() - x[:, :n].double().amax(1, keepdim=True)).scatter(1, at, -math.inf)
+    want = -torch.log1p(torch.exp(d).sum(1))
+    assert float((want - lp.gather(1, at)[:, 0]).abs().max()) < 1e-12
+    s = Select(x, n, G, 1, 1, 0).call()
+    s.check()
+    tol = want.abs() * (2.0 ** -17 + 32 * math.e ** 2 / n + E32)
+    err = (s.score[:G].double() - want).abs()
+    assert bool((err <= tol).all()), (err / want.abs()).tolist()
+    # the same token as the end token
+    for i in range(G):
+        e = Select(x[i:i + 1], n, 1, 1, 1, int(at[i])).call()
+        assert abs(float(e.eos_score[0]) - float(want[i])) <= float(tol[i])
