@@ -285,6 +285,9 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
         }
         __syncthreads();
     }
+    if (a.eos_score && tid < W && s.fine[tid])  // (a row has one log Z)
+        a.eos_score[row0 + tid] =
+            (float)(s.base[tid] + ((double)lf(static_cast<const T*>(a.x)[(row0 + tid) * a.ld + a.eos]) - s.log_z[tid]));
     const int n = min(s.n, k);
     for (int i = tid; i < k; i += kMergeThreads) {
         const Cand c = i < n ? s.best[i] : Cand{-INFINITY, 0};

@@ -51,3 +51,36 @@ def test_scores_of_a_sure_token(dtype, pad):
     for i in range(G):
         e = Select(x[i:i + 1], n, 1, 1, 1, int(at[i])).call()
         assert abs(float(e.eos_score[0]) - float(want[i])) <= float(tol[i])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_one_log_z_of_a_row(dtype):
+    """Beams with nearly the same logits in other places come close, so their log Z are taken in 64 bits; the end
+    token's score has the same log Z: the value in 64 bits (whose sums are off by some 1e-13), rounded once.
+
+    Which beams: e^d of the end token is 1, the others weigh 0.16 together with |d| near 13, so fp32 log Z are off by
+    0.16 (13 * 2.25 half steps + 3 2^-22) + 8 half steps < 2^-20.  Neighbours of two beams within 2^-18 are then
+    within 2^-18 + 2^-19 for the kernel, which settles what is within 2^-17."""
+    G, W, n, eos = 8, 8, 50000, 77
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn(G, 1, n, device="cuda", generator=g).expand(G, W, n).contiguous()
+    for r in x.view(-1, n):
+        r.copy_(r[torch.randperm(n, device="cuda", generator=g)])
+    x[:, :, eos] = 13.0
+    x = x.view(G * W, n).to(DT[dtype][0])
+    s = Select(x, n, G, W, 4 * W, eos).call()
+    lp = torch.log_softmax(x.double(), 1)
+    want = lp[:, eos].clone()
+    score = lp[s.parent[:-1].long(), s.token[:-1].long()]
+    lp[:, eos] = -math.inf
+    val, at = torch.sort(lp.view(G, W * n), dim=1, descending=True, stable=True)
+    row = (torch.arange(G, device="cuda")[:, None] * W + at // n)[:, :4 * W]
+    near = (row[:, 1:] != row[:, :-1]) & (val[:, :4 * W - 1] - val[:, 1:4 * W] < 2.0 ** -18)
+    settled = torch.zeros(G * W, dtype=torch.bool, device="cuda")
+    settled[row[:, 1:][near]] = True
+    settled[row[:, :-1][near]] = True
+    assert int(settled.sum()) > G * W // 2
+    err = (s.eos_score[:-1].double() - want).abs()
+    assert bool((err <= E32 * want.abs() + 1e-12)[settled].all())
+    err = (s.score[:-1].double() - score).abs()
+    assert bool((err <= E32 * score.abs() + 1e-12)[settled[s.parent[:-1].long()]].all())
