@@ -335,7 +335,9 @@ cudaError_t go(const BeamArgs& a, int rows, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     auto kern = beam_merge_kernel<T>;
     const size_t smem = sizeof(MergeShared) + (size_t)a.width * a.k1 * sizeof(Cand);
-    if (smem > kPlainSmem) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // (the limit is the kernel's, not the call's: always the most, so that no thread lowers it under another's launch)
+    constexpr int most = sizeof(MergeShared) + kBeamMaxWidth * (kLogprobMaxTop + 1) * sizeof(Cand);
+    if (smem > kPlainSmem) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (e != cudaSuccess) return e;
     return launch_pdl(kern, dim3(rows / a.width), dim3(kMergeThreads), smem, s, a);
 }

@@ -1,9 +1,11 @@
 """The beam search's operators where two candidates, two threads or two sizes meet
 at a border."""
 import math
+import threading
 
 import pytest
 
+import b2decode as b2
 from test_gpu_beam import Select
 from test_gpu_paged import DT, E32
 
@@ -84,3 +86,32 @@ def test_one_log_z_of_a_row(dtype):
     assert bool((err <= E32 * want.abs() + 1e-12)[settled].all())
     err = (s.score[:-1].double() - score).abs()
     assert bool((err <= E32 * score.abs() + 1e-12)[settled[s.parent[:-1].long()]].all())
+
+
+def test_threads_of_different_widths():
+    """Threads whose requests want different amounts of shared memory, past what a launch may ask for as it is: no call
+    makes another's launch fail."""
+    n, codes = 200, []
+    x = torch.randn(64, n, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    calls = [Select(x[:w], n, 1, w, 64) for w in (64, 48, 64, 48)]
+    torch.cuda.synchronize()
+    start = threading.Barrier(len(calls))
+
+    def run(s):
+        st = torch.cuda.Stream()
+        f = b2.lib().b2_beam_select
+        a = (s.x.data_ptr(), b2.F32, n, 1, s.W, n, None, 64, -1, s.parent.data_ptr(), s.token.data_ptr(), s.score.data_ptr(), None,
+             s.scratch.data_ptr(), st.cuda_stream)
+        start.wait()
+        for _ in range(8):
+            codes.extend({f(*a) for _ in range(500)})
+            st.synchronize()
+    threads = [threading.Thread(target=run, args=(s,)) for s in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert set(codes) == {0}
+    for s in calls:
+        s.check()
