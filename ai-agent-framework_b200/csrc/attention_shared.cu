@@ -976,6 +976,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                     if (!ok) break;
                     uint64_t* bar = value ? &s.ready[j % NS] : &s.k_full[slot];
                     const uint32_t to = __shfl_sync(0xffffffffu, ring_s + slot * TM::kTileBytes, 0);
+                    __syncwarp();  // (the lanes' s.bad before the arrival that the exponentials wait for)
                     const bool one = elected();
                     if (one) {
                         const uint32_t bytes = __popc(by_box) * G * 128 * BL;

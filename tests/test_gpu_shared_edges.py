@@ -39,3 +39,21 @@ def test_prefix_of_everything(dtype, cache, prefix, groups):
     """A prefix past every length: all of it is shared, whether an item is written whole (many of them) or in pieces."""
     p = Shared([(ls, max(ls)) for ls in groups for _ in range(40 if len(groups) > 1 else 1)], 16, 2, 64, 16, dtype, cache, one=True)
     p.check(*p.call(prefix=[prefix] * len(p.prefix)))
+
+
+@pytest.mark.parametrize("P", [8, 16, 24, 100])
+@pytest.mark.parametrize("dtype,cache", [("f32", "f16"), ("bf16", "bf16")])
+def test_missing_page_at_every_place(P, dtype, cache):
+    """Group i's page i does not exist, in whichever tile and part of it that is, by boxes or row by row: its rows are
+    NaN, and all of a call in which it is whole is as it was."""
+    places = 640 // P
+    p = Shared([([640, 641, 655], 640) for _ in range(places)], 8, 2, 64, P, dtype, cache)
+    want = p.call()[0].clone()
+    keep = p.table.clone()
+    for r in range(len(p.lens)):
+        p.table[r, r // 3] = -1 if r % 2 else p.total
+    for _ in range(5):
+        out, ls = p.call()
+        assert bool(torch.isnan(out).all()) and bool(torch.isnan(ls).all())
+    p.table = keep
+    assert torch.equal(p.call()[0], want)
