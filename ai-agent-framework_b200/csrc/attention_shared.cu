@@ -346,6 +346,16 @@ __device__ __forceinline__ float4 load4(const T* p, bool wide) {
     return make_float4(to_float(t[0]), to_float(t[1]), to_float(t[2]), to_float(t[3]));
 }
 
+// The power of two that takes a row's largest element to [2^10, 2^11), the row
+// four elements a lane.  The exponent field is enough: subnormal rows count as
+// 2^-127; from -117 for the largest finite row to 100, so that 2^e and 2^-e are normal.
+__device__ __forceinline__ int row_exponent(float4 x) {
+    const float mx = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+    const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(mx));  // (none negative: ordered as their bits)
+    return top < 0x7f800000u ? min(100, 137 - (int)(top >> 23)) : 0;
+}
+__device__ __forceinline__ float pow2f(int e) { return __int_as_float((127 + e) << 23); }
+
 // A warp's rows of Q, one after another: largest element to [2^10, 2^11), then
 // 16-bit terms.  (A single term is q itself, copied for its alignment.)
 template <typename T, typename C, int QT>
@@ -370,12 +380,8 @@ __device__ __forceinline__ void make_terms(const SharedArgs& a, long long first,
             const long long r = r0 + u * step;
             if (r >= rows) break;
             if (QT > 1) {
-                const float mx = fmaxf(fmaxf(fabsf(x[u].x), fabsf(x[u].y)), fmaxf(fabsf(x[u].z), fabsf(x[u].w)));
-                const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(mx));  // (none negative: ordered as their bits)
-                // (the exponent field is enough: subnormal rows count as 2^-127; down to
-                // -117 for the largest finite row, so that both factors stay normal)
-                const int e = top < 0x7f800000u ? min(100, 137 - (int)(top >> 23)) : 0;
-                const float up = __int_as_float((127 + e) << 23), f = a.scale * __int_as_float((127 - e) << 23);
+                const int e = row_exponent(x[u]);
+                const float up = pow2f(e), f = a.scale * pow2f(-e);
                 if (lane == 0) a.factor[r] = a.softcap > 0.0f ? f / a.softcap : f * kLog2e;
                 x[u] = make_float4(x[u].x * up, x[u].y * up, x[u].z * up, x[u].w * up);
             }
@@ -1365,6 +1371,12 @@ __device__ __noinline__ Sum row_alone(const SharedArgs& a, int b, int head) {
     const int64_t h_off = (int64_t)(head / a.grp) * a.head_stride;
     const T* q = static_cast<const T*>(a.q) + (int64_t)b * a.q_stride + (int64_t)head * hd;
     const float slope = a.slopes ? a.slopes[head] : 0.0f;
+    float up = 1.0f, scale = a.scale;
+    if (std::is_same<T, float>::value) {  // as the products take it
+        const int e = row_exponent(d < hd ? load4(q + d, a.q_wide) : make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+        up = pow2f(e);
+        scale *= pow2f(-e);
+    }
     Sum r{make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
     bool bad = false;
     for (int p0 = sq.lo; p0 < sq.len; p0 += 32) {
@@ -1377,8 +1389,8 @@ __device__ __noinline__ Sum row_alone(const SharedArgs& a, int b, int head) {
                 off = page * a.page_stride + (int64_t)(pos - pg * a.page_size) * a.pos_stride + h_off;
                 const C* k = reinterpret_cast<const C*>(a.k) + off;
                 float dot = 0.0f;
-                for (int i = 0; i < hd; i++) dot = fmaf(to_float(q[i]), to_float(k[i]), dot);
-                x = dot * a.scale;
+                for (int i = 0; i < hd; i++) dot = fmaf(to_float(q[i]) * up, to_float(k[i]), dot);
+                x = dot * scale;
                 if (a.softcap > 0.0f) x = a.softcap * tanhf(x / a.softcap);
                 x = fmaf(slope, (float)(pos - (sq.len - 1)), x) * kLog2e;
             } else {

@@ -4,7 +4,7 @@ import math
 
 import pytest
 
-from test_gpu_paged import DT
+from test_gpu_paged import DT, assert_within, attend64
 from test_gpu_shared import Shared
 
 pytestmark = pytest.mark.gpu
@@ -57,3 +57,20 @@ def test_missing_page_at_every_place(P, dtype, cache):
         assert bool(torch.isnan(out).all()) and bool(torch.isnan(ls).all())
     p.table = keep
     assert torch.equal(p.call()[0], want)
+
+
+@pytest.mark.parametrize("size", [1.0, 1e30, 3e38])
+@pytest.mark.parametrize("cache", ["f16", "bf16"])
+def test_large_queries_beside_infinite_values(size, cache):
+    """fp32 rows of any magnitude in a group where another row sees an infinite value: those that do not see it get
+    what they get without it."""
+    p = Shared([([100, 128, 200, 90, 330], 330)], 8, 2, 64, 16, "f32", cache, one=True)
+    p.q = p.q / p.q.abs().amax(2, keepdim=True) * size
+    scale = 0.125 if size == 1.0 else 1.0 / size if size < 1e37 else 2.0 ** -126
+    p.vc[int(p.table[0, 150 // 16]), 150 % 16] = math.inf
+    out, ls = p.call(scale=scale)
+    want, lse, to, tl = attend64(p.q, p.kc, p.vc, p.table, p.lens, p.req, 16, 0, scale, 0.0, None)
+    for b in (0, 1, 3):
+        assert_within(out[b], want[b], to[b][:, None].expand_as(want[b]), torch.float32)
+        assert bool(((ls[b].double() - lse[b]).abs() <= tl[b]).all())
+    assert bool((out[[2, 4]] == math.inf).all())
