@@ -133,7 +133,7 @@ __device__ __forceinline__ int page_of(const SharedArgs& a, int n) {
 
 // tiles start on multiples of 16 positions
 __device__ __forceinline__ int base_of(const Item& it) { return it.lo & ~15; }
-__device__ __forceinline__ int tiles_of(const Item& it) { return (it.hi - base_of(it) + kTile - 1) / kTile; }
+__device__ __forceinline__ int tiles_of(const Item& it) { return (it.hi - base_of(it) - 1) / kTile + 1; }  // (it.hi > it.lo, up to 2^31 - 64)
 
 // The last i of a[0 .. n) (ascending, a[0] <= x) with a[i] <= x.
 template <typename F>
@@ -700,7 +700,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                         for (int c = 0; c < 32 * chunks; c += 16) {
                             uint32_t r[16];
                             tmem_ld16(s_col + c, r);
-                            const float p1 = (float)(p0 + c - (row.z - 1));
+                            const float p1 = (float)(p0 - (row.z - 1) + c);
 #pragma unroll
                             for (int i = 0; i < 16; i++) {
                                 float x = __uint_as_float(r[i]) * f;
@@ -939,20 +939,21 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
                     row = a.table + (int64_t)p->tr * a.table_stride;
                 };
                 auto look = [&]() {  // this lane's group: its page (any position of it that is seen names it)
-                    const int at = max(p0 + r0, p_lo);
-                    if (lane >= groups || at >= p_hi || p0 + r0 + G <= p_lo) return -1;
-                    return row[page_of(a, at)];
+                    const int lo = max(p_lo - p0, r0);
+                    if (lane >= groups || lo >= r0 + G || lo >= p_hi - p0) return -1;
+                    return row[page_of(a, p0 + lo)];
                 };
                 enter();
                 int nx = p ? look() : -1;
 #pragma unroll 1
                 while (p) {
-                    const int page = nx, lo_t = p_lo - p0, hi_t = min(kTile, p_hi - p0), in = place(p0 + r0);
-                    p0 += kTile;
+                    const int page = nx, lo_t = p_lo - p0, hi_t = min(kTile, p_hi - p0), in = r0 < hi_t ? place(p0 + r0) : 0;
                     if (--t == 0) {
                         pieces.done(s);
                         p = pieces.next(s);
                         enter();
+                    } else {
+                        p0 += kTile;
                     }
                     if (p) nx = look();  // (the next tile's pages, on their way meanwhile)
                     const bool there = (unsigned)page < (unsigned)a.n_pages;

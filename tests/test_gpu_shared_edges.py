@@ -4,7 +4,8 @@ import math
 
 import pytest
 
-from test_gpu_paged import DT, assert_within, attend64
+import b2decode as b2
+from test_gpu_paged import DT, assert_within, attend64, i32, stream
 from test_gpu_shared import Shared
 
 pytestmark = pytest.mark.gpu
@@ -74,3 +75,37 @@ def test_large_queries_beside_infinite_values(size, cache):
         assert_within(out[b], want[b], to[b][:, None].expand_as(want[b]), torch.float32)
         assert bool(((ls[b].double() - lse[b]).abs() <= tl[b]).all())
     assert bool((out[[2, 4]] == math.inf).all())
+
+
+@pytest.mark.parametrize("dtype,cache", [("f32", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("prefix", [2 ** 31 - 1, 100])
+def test_longest_rows(dtype, cache, prefix):
+    """Two rows of 2^31 - 64 positions and a few less, every page of theirs the same one; their positions together,
+    or each row's own.  A position j of the page weighs as often as it is seen, c_j, so out = sum c_j e^s_j v_j / sum
+    c_j e^s_j and lse = log of that sum.  2^24 tiles go to 148 shares, and a share's sums run over 2^17 tiles (twice
+    as many where there are two rows) in fp32: each addition rounds by half a step, 2^18 2^-24 = 2^-6 of the sum
+    at worst, and twice that in the quotient; the join and the rounding of out are far below."""
+    P, nh, hd = 65536, 8, 64
+    dt, tid = DT[dtype]
+    ct, cid = DT[cache]
+    g = torch.Generator(device="cuda").manual_seed(1)
+    kc = torch.randn(1, P, 1, hd, device="cuda", generator=g).to(ct)
+    vc = (1 + torch.randn(1, P, 1, hd, device="cuda", generator=g)).to(ct)
+    q = torch.randn(2, nh, hd, device="cuda", generator=g).to(dt)
+    lens, pages = [2 ** 31 - 64, 2 ** 31 - 1000], 2 ** 31 // P
+    table = torch.zeros(2, pages, dtype=torch.int32, device="cuda")
+    out, lse = torch.full((2, nh, hd), 5.0, device="cuda", dtype=dt), torch.full((2, nh), 5.0, device="cuda")
+    scratch = torch.empty(b2.attention_shared_scratch_bytes(2, nh, 1, hd), dtype=torch.uint8, device="cuda")
+    kv = b2.paged_kv(kc.data_ptr(), vc.data_ptr(), cid, 1, P, 1, hd)
+    opts = b2.paged_attn_opts(tid, nh, 2, pages)
+    ln, starts, pre = i32(lens), i32([0, 2]), i32([prefix])
+    b2.attention_shared(kv, opts, q.data_ptr(), table.data_ptr(), ln.data_ptr(), 0, 2, starts.data_ptr(), pre.data_ptr(), 1,
+                        out.data_ptr(), lse.data_ptr(), scratch.data_ptr(), stream())
+    k, v = kc[0, :, 0].double(), vc[0, :, 0].double()
+    for b, n in enumerate(lens):
+        c = n // P + (torch.arange(P, device="cuda") < n % P).double()
+        s = q[b].double() @ k.T / 8 + torch.log(c)
+        want = torch.softmax(s, 1) @ v
+        tol = 2.0 ** -5 * v.abs().max()
+        assert_within(out[b], want, tol.expand_as(want), dt)
+        assert bool(((lse[b].double() - torch.logsumexp(s, 1)).abs() <= 2.0 ** -5).all())
