@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(kForkThreads) page_fork_kernel(const __grid_co
     }
     if (status) return;
     const int warp0 = (blockIdx.x * kForkThreads + tid) / 32, n_warps = gridDim.x * kForkThreads / 32;
-    const int pieces = (a.max_pages + kPiece - 1) / kPiece;
+    const int pieces = (a.max_pages - 1) / kPiece + 1;
     const long long items = (long long)R * pieces;
     for (long long it = warp0; it < items; it += n_warps) {
         const int c = (int)(it / R), r = (int)(it - (long long)c * R);
@@ -160,27 +160,29 @@ __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(const __grid_co
     constexpr int kCopyChunks = kCopyThreads * LOADS;
     const int per_pos = a.nkv * a.hc;
     const int turns = (int)(((int64_t)a.page_size * per_pos + kCopyChunks - 1) / kCopyChunks);
-    const int64_t items = (int64_t)n * 2 * a.layers * turns;
+    const unsigned planes = 2u * (unsigned)a.layers;
+    const int64_t items = (int64_t)n * planes * turns;
     const bool narrow = items <= 0x7fffffff;  // divisions of 32 bits where they do
     for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
-        int turn, which, pair;
+        int turn, pair;
+        unsigned which;
         if (narrow) {
             const unsigned i = (unsigned)it, rest = i / (unsigned)turns;
             turn = (int)(i - rest * turns);
-            pair = (int)(rest / (unsigned)(2 * a.layers));
-            which = (int)(rest - (unsigned)pair * (2 * a.layers));
+            pair = (int)(rest / planes);
+            which = rest - (unsigned)pair * planes;
         } else {
             const int64_t rest = it / turns;
             turn = (int)(it - rest * turns);
-            pair = (int)(rest / (2 * a.layers));
-            which = (int)(rest - (int64_t)pair * (2 * a.layers));
+            pair = (int)(rest / planes);
+            which = (unsigned)(rest - (int64_t)pair * planes);
         }
         const int src = a.pairs[3 * (int64_t)pair], dst = a.pairs[3 * (int64_t)pair + 1];
         const int count = min(a.pairs[3 * (int64_t)pair + 2], a.page_size);
         if (src == dst || (unsigned)src >= (unsigned)a.n_pages || (unsigned)dst >= (unsigned)a.n_pages) continue;
         const int64_t chunks = (int64_t)max(count, 0) * per_pos;
         if ((int64_t)turn * kCopyChunks >= chunks) continue;
-        uint16_t* base = (which & 1 ? a.v : a.k) + (which >> 1) * a.layer_stride;
+        uint16_t* base = (which & 1 ? a.v : a.k) + (int64_t)(which >> 1) * a.layer_stride;
         const uint16_t* from = base + src * a.page_stride;
         uint16_t* to = base + dst * a.page_stride;
         uint4 v[LOADS];
@@ -213,7 +215,7 @@ __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(const __grid_co
 // row at a time, by the warps from `warp` on in steps of `n_warps`.
 template <typename A, typename F>
 __device__ __forceinline__ void walk_table(const A& a, int warp, int n_warps, F f) {
-    const int lane = threadIdx.x & 31, pieces = (a.max_pages + kPiece - 1) / kPiece;
+    const int lane = threadIdx.x & 31, pieces = (a.max_pages - 1) / kPiece + 1;
     const long long items = (long long)a.n_req * pieces;
     for (long long it = warp; it < items; it += n_warps) {
         const int c = (int)(it / a.n_req), r = (int)(it - (long long)c * a.n_req);
@@ -244,7 +246,7 @@ struct PoolArgs {
 __global__ void __launch_bounds__(kPoolThreads) pool_zero_kernel(const __grid_constant__ PoolArgs a) {
     pdl_trigger();
     pdl_wait();
-    for (int i = blockIdx.x * kPoolThreads + threadIdx.x; i < a.n_pages; i += gridDim.x * kPoolThreads) a.refs[i] = 0;
+    for (unsigned i = blockIdx.x * kPoolThreads + threadIdx.x; i < (unsigned)a.n_pages; i += gridDim.x * kPoolThreads) a.refs[i] = 0;
 }
 
 __global__ void __launch_bounds__(kPoolThreads) pool_count_kernel(const __grid_constant__ PoolArgs a) {
@@ -290,8 +292,8 @@ __global__ void __launch_bounds__(kPoolThreads) pool_blocks_kernel(const int32_t
     int n = 0;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        const int p = blockIdx.x * kPoolBlock + 4 * threadIdx.x + j;
-        n += p < n_pages && refs[p] == 0;
+        const unsigned p = blockIdx.x * kPoolBlock + 4 * threadIdx.x + j;  // (the last block may pass 2^31)
+        n += p < (unsigned)n_pages && refs[p] == 0;
     }
     int all;
     sum_before<kPoolThreads>(n, warps, &all);
@@ -317,19 +319,19 @@ __global__ void __launch_bounds__(kPoolThreads) pool_list_kernel(const __grid_co
     pdl_wait();
     int total;
     const int before = free_before(a.counts, warps, &total);
-    const int p0 = blockIdx.x * kPoolBlock + 4 * threadIdx.x;
+    const unsigned p0 = blockIdx.x * kPoolBlock + 4 * threadIdx.x, N = a.n_pages;
     int n = 0;
     bool free_[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        free_[j] = p0 + j < a.n_pages && a.refs[p0 + j] == 0;
+        free_[j] = p0 + j < N && a.refs[p0 + j] == 0;
         n += free_[j];
     }
     int all;
     int at = before + sum_before<kPoolThreads>(n, warps, &all);
 #pragma unroll
     for (int j = 0; j < 4; j++)
-        if (free_[j]) a.free_pages[at++] = p0 + j;
+        if (free_[j]) a.free_pages[at++] = (int)(p0 + j);
     if (blockIdx.x == 0 && threadIdx.x == 0) *a.n_free = total;
 }
 
@@ -368,19 +370,19 @@ __global__ void __launch_bounds__(kPoolThreads) compact_rank_kernel(const __grid
     int n_free;
     int before = free_before(a.counts, warps, &n_free);
     const int U = a.n_pages - n_free;
-    const int p0 = blockIdx.x * kPoolBlock + 4 * threadIdx.x;
+    const unsigned p0 = blockIdx.x * kPoolBlock + 4 * threadIdx.x, N = a.n_pages;
     int n = 0;
     bool free_[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        free_[j] = p0 + j < a.n_pages && a.refs[p0 + j] == 0;
+        free_[j] = p0 + j < N && a.refs[p0 + j] == 0;
         n += free_[j];
     }
     int all;
     before += sum_before<kPoolThreads>(n, warps, &all);
 #pragma unroll
     for (int j = 0; j < 4; j++)
-        if (p0 + j < a.n_pages) before = place(a, p0 + j, free_[j], U, before);
+        if (p0 + j < N) before = place(a, (int)(p0 + j), free_[j], U, before);
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         a.info[2] = U;
         if (U == 0) *a.moves = 0;
@@ -416,12 +418,12 @@ __global__ void __launch_bounds__(kPoolThreads) compact_apply_kernel(const __gri
     apply(a, blockIdx.x * kPoolThreads + threadIdx.x, gridDim.x * kPoolThreads, a.info[2]);
 }
 
-int pool_blocks(int n_pages) { return (n_pages + kPoolBlock - 1) / kPoolBlock; }
+int pool_blocks(int n_pages) { return (n_pages - 1) / kPoolBlock + 1; }
 size_t words16(size_t n) { return (n + 3) & ~(size_t)3; }
 
 // CTAs for the rows' entries: a warp for every kPiece of them
 int entry_ctas(int n_req, int max_pages, int threads, int sms) {
-    const long long items = (long long)n_req * ((max_pages + kPiece - 1) / kPiece);
+    const long long items = (long long)n_req * ((max_pages - 1) / kPiece + 1);
     return (int)std::max<long long>(1, std::min<long long>(2048 / threads * sms, (items + threads / 32 - 1) / (threads / 32)));
 }
 
@@ -485,7 +487,7 @@ int launch_page_pool(const int32_t* table, int64_t table_stride, const int32_t* 
         return e == cudaSuccess ? B2_OK : cuda_failed("page pool launch", e, err);
     }
     const int blocks = pool_blocks(n_pages);
-    cudaError_t e = launch_pdl(pool_zero_kernel, dim3(std::min(4 * sms, (n_pages + kPoolThreads - 1) / kPoolThreads)),
+    cudaError_t e = launch_pdl(pool_zero_kernel, dim3(std::min(4 * sms, (n_pages - 1) / kPoolThreads + 1)),
                                dim3(kPoolThreads), 0, s, a);
     if (e == cudaSuccess)
         e = launch_pdl(pool_count_kernel, dim3(entry_ctas(n_req, max_pages, kPoolThreads, sms)), dim3(kPoolThreads), 0, s, a);

@@ -7,7 +7,7 @@ import pytest
 
 import b2decode as b2
 from test_gpu_beam import Select
-from test_gpu_paged import DT, E32
+from test_gpu_paged import DT, E32, i32, stream
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -115,3 +115,38 @@ def test_threads_of_different_widths():
     assert set(codes) == {0}
     for s in calls:
         s.check()
+
+
+def test_pages_up_to_2_31():
+    """A pool of 2^31 - 1 pages and rows of as many entries, few of them in use: counted, listed, forked, compacted."""
+    torch.cuda.empty_cache()
+    N = 2 ** 31 - 1
+    big = lambda n=N: torch.empty(n, dtype=torch.int32, device="cuda")  # noqa: E731
+    table, refs, free, n_free, lens = big(), big(), big(), i32([-9]), i32([70])
+    used = [0, N - 2, 5, 2 ** 30, N - 1]
+    table[:6] = i32(used + [77])
+    refs.fill_(-9)
+    scratch = torch.empty(max(b2.page_pool_scratch_bytes(N), b2.page_compact_scratch_bytes(N)), dtype=torch.uint8, device="cuda")
+
+    def pool(t):
+        b2.page_pool(t.data_ptr(), N, lens.data_ptr(), 1, 16, N, refs.data_ptr(), N, free.data_ptr(), n_free.data_ptr(),
+                     scratch.data_ptr(), stream())
+        assert int(n_free) == N - 5
+    pool(table)
+    assert int(torch.count_nonzero(refs)) == 5 and refs[used].tolist() == [1] * 5
+    gaps = torch.tensor(sorted(used), device="cuda") - torch.arange(5, device="cuda")
+    for at in range(0, N - 5, 1 << 28):  # free[i] = i and the pages in use before it
+        i = torch.arange(at, min(at + (1 << 28), N - 5), device="cuda")
+        assert torch.equal(free[at:at + len(i)].long(), i + torch.bucketize(i, gaps, right=True))
+    parent, new, new_lens, pairs, info = i32([0]), big(), i32([-9, -9]), torch.full((8, 3), -9, dtype=torch.int32, device="cuda"), i32([-9] * 4)
+    b2.page_fork(parent.data_ptr(), 1, table.data_ptr(), N, lens.data_ptr(), 1, 16, refs.data_ptr(), N, free.data_ptr(),
+                 n_free.data_ptr(), new.data_ptr(), N, N, new_lens.data_ptr(), pairs.data_ptr(), info.data_ptr(), stream())
+    assert info.tolist() == [0, 0, 0, 0] and new_lens.tolist() == [70, -9] and new[:5].tolist() == used
+    b2.page_compact(new.data_ptr(), N, lens.data_ptr(), 1, 16, N, refs.data_ptr(), N, pairs.data_ptr(), 7, info.data_ptr(),
+                    scratch.data_ptr(), stream())
+    assert info.tolist() == [0, 4, 5, 5] and new[:5].tolist() == [0, 2, 4, 3, 1]
+    assert pairs.tolist() == [[N - 1, 1, 16], [N - 2, 2, 16], [2 ** 30, 3, 16], [5, 4, 16]] + [[-9] * 3] * 4
+    pool(new)
+    assert refs[:6].tolist() == [1] * 5 + [0] and free[:3].tolist() == [5, 6, 7]
+    del table, refs, free, new, scratch
+    torch.cuda.empty_cache()
