@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <array>
 #include <chrono>
 #include <cmath>
 #include <cstring>
@@ -64,19 +65,24 @@ constexpr int64_t kBeamMaxRows = 1 << 27;  // rows of one beam selection
 
 bool float_type(int32_t t) { return t == 0 || t == 1 || t == 30; }
 
-int aligned(const char* who, std::initializer_list<b2::DevicePtr> ptrs) {
+int aligned(const char* who, const b2::DevicePtr* ptrs, size_t n) {
     std::string err;
-    const int rc = b2::check_alignment(ptrs.begin(), (int)ptrs.size(), &err);
+    const int rc = b2::check_alignment(ptrs, (int)n, &err);
+    return rc == B2_OK ? rc : ret(rc, std::string(who) + ": " + err);
+}
+int aligned(const char* who, std::initializer_list<b2::DevicePtr> ptrs) { return aligned(who, ptrs.begin(), ptrs.size()); }
+
+int devices(const char* who, const b2::DevicePtr* ptrs, size_t n) {
+    std::string err;
+    const int rc = b2::check_device_pointers(ptrs, (int)n, &err);
     return rc == B2_OK ? rc : ret(rc, std::string(who) + ": " + err);
 }
 
-int on_device(const char* who, std::initializer_list<b2::DevicePtr> ptrs) {
-    int rc = aligned(who, ptrs);
-    if (rc != B2_OK) return rc;
-    std::string err;
-    rc = b2::check_device_pointers(ptrs.begin(), (int)ptrs.size(), &err);
-    return rc == B2_OK ? rc : ret(rc, std::string(who) + ": " + err);
+int on_device(const char* who, const b2::DevicePtr* ptrs, size_t n) {
+    const int rc = aligned(who, ptrs, n);
+    return rc == B2_OK ? devices(who, ptrs, n) : rc;
 }
+int on_device(const char* who, std::initializer_list<b2::DevicePtr> ptrs) { return on_device(who, ptrs.begin(), ptrs.size()); }
 
 size_t type_bytes(int32_t t) { return t == 0 ? 4 : 2; }
 
@@ -123,13 +129,14 @@ int paged_attn_args(const char* who, const b2_paged_kv& c, const b2_paged_attn_o
     return B2_OK;
 }
 
-int paged_attn_pointers(const char* who, const b2_paged_kv& c, const b2_paged_attn_opts& o, const void* q,
-                        const int32_t* table, const int32_t* lens, const int32_t* req, const void* out, const float* lse,
-                        const void* scratch, const int32_t* starts, const int32_t* prefix) {
+using AttnPointers = std::array<b2::DevicePtr, 12>;
+AttnPointers paged_attn_pointers(const b2_paged_kv& c, const b2_paged_attn_opts& o, const void* q, const int32_t* table,
+                                 const int32_t* lens, const int32_t* req, const void* out, const float* lse,
+                                 const void* scratch, const int32_t* starts, const int32_t* prefix) {
     const size_t es = type_bytes(o.dtype);
-    return on_device(who, {{"q", q, es}, {"the cache's k", c.k, 16}, {"the cache's v", c.v, 16}, {"table", table, 4},
-                           {"lens", lens, 4}, {"req", req, 4}, {"out", out, es}, {"lse", lse, 4}, {"slopes", o.slopes, 4},
-                           {"scratch", scratch, 16}, {"starts", starts, 4}, {"prefix", prefix, 4}});
+    return {{{"q", q, es}, {"the cache's k", c.k, 16}, {"the cache's v", c.v, 16}, {"table", table, 4}, {"lens", lens, 4},
+             {"req", req, 4}, {"out", out, es}, {"lse", lse, 4}, {"slopes", o.slopes, 4}, {"scratch", scratch, 16},
+             {"starts", starts, 4}, {"prefix", prefix, 4}}};
 }
 
 int rope_rows_args(const char* who, const b2_rope_rows* r, b2_rope_rows* out) {
@@ -818,7 +825,8 @@ int b2_attention_paged(const b2_paged_kv* kv, const b2_paged_attn_opts* opts, co
         if (rc != B2_OK) return rc;
         rc = paged_attn_args("b2_attention_paged", c, opts, q, table, lens, req, batch, out, d_scratch);
         if (rc != B2_OK) return rc;
-        rc = paged_attn_pointers("b2_attention_paged", c, *opts, q, table, lens, req, out, lse, d_scratch, nullptr, nullptr);
+        const AttnPointers p = paged_attn_pointers(c, *opts, q, table, lens, req, out, lse, d_scratch, nullptr, nullptr);
+        rc = on_device("b2_attention_paged", p.data(), p.size());
         if (rc != B2_OK) return rc;
         std::string err;
         rc = b2::launch_attention_paged(c, *opts, q, table, lens, req, batch, out, lse, d_scratch,
@@ -1068,9 +1076,16 @@ int b2_attention_shared(const b2_paged_kv* kv, const b2_paged_attn_opts* opts, c
         rc = paged_attn_args("b2_attention_shared", c, opts, q, table, lens, req, batch, out, d_scratch);
         if (rc != B2_OK) return rc;
         if (!starts || !prefix || n_groups <= 0) return ret(B2_ERR_BAD_ARG, "b2_attention_shared: null argument or no groups");
-        rc = paged_attn_pointers("b2_attention_shared", c, *opts, q, table, lens, req, out, lse, d_scratch, starts, prefix);
+        const AttnPointers p = paged_attn_pointers(c, *opts, q, table, lens, req, out, lse, d_scratch, starts, prefix);
+        rc = aligned("b2_attention_shared", p.data(), p.size());
         if (rc != B2_OK) return rc;
-        std::string err;
+        std::string none;  // (without a device the call is refused below)
+        const int sms = std::max(1, b2::current_sms(&none));
+        std::string err = b2::attention_shared_overlap(c, *opts, q, table, lens, req, batch, starts, prefix, n_groups, out, lse,
+                                                       d_scratch, b2::attention_shared_scratch(batch, opts->nh, c.nkv, c.hd, sms));
+        if (!err.empty()) return ret(B2_ERR_BAD_ARG, "b2_attention_shared: " + err);
+        rc = devices("b2_attention_shared", p.data(), p.size());
+        if (rc != B2_OK) return rc;
         rc = b2::launch_attention_shared(c, *opts, q, table, lens, req, batch, starts, prefix, n_groups, out, lse, d_scratch,
                                          static_cast<cudaStream_t>(stream), &err);
         return ret(rc, err);

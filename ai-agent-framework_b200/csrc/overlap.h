@@ -95,4 +95,35 @@ inline bool kv_places_apart(const b2_paged_kv& kv, int layers = 1, int64_t layer
     return true;
 }
 
+// Rows that lie back to back are one run.
+inline Region rows_of(const char* name, const void* p, __int128 bytes, __int128 rows, __int128 stride) {
+    if (stride == bytes) return {name, p, bytes * rows};
+    return {name, p, bytes, rows, stride};
+}
+
+// The pages of a cache's k or v, each with all that lies between its first and
+// last element.
+inline Region pages_of_cache(const char* name, const b2_paged_kv& kv, const void* p) {
+    const __int128 page = 2 * ((__int128)(kv.page_size - 1) * kv.pos_stride + (__int128)(kv.nkv - 1) * kv.head_stride + kv.hd);
+    return rows_of(name, p, page, kv.n_pages, (__int128)2 * kv.page_stride);
+}
+
+// "<output> overlaps <input>" where what an attention over shared prefixes
+// writes shares memory with what it reads.
+inline std::string attention_shared_overlap(const b2_paged_kv& kv, const b2_paged_attn_opts& o, const void* q,
+                                            const int32_t* table, const int32_t* lens, const int32_t* req, int batch,
+                                            const int32_t* starts, const int32_t* prefix, int n_groups, const void* out,
+                                            const float* lse, const void* scratch, size_t scratch_bytes) {
+    const __int128 es = o.dtype == 0 ? 4 : 2, row = es * o.nh * kv.hd, rows = batch;
+    const Region in[] = {rows_of("q", q, row, rows, o.q_stride ? es * o.q_stride : row),
+                         pages_of_cache("the cache's k", kv, kv.k), pages_of_cache("the cache's v", kv, kv.v),
+                         rows_of("table", table, (__int128)4 * o.max_pages, o.n_req,
+                                 (__int128)4 * (o.table_stride ? o.table_stride : o.max_pages)),
+                         {"lens", lens, 4 * rows}, {"req", req, 4 * rows}, {"starts", starts, (__int128)4 * n_groups + 4},
+                         {"prefix", prefix, (__int128)4 * n_groups}, {"slopes", o.slopes, (__int128)4 * o.nh}};
+    const Region to[] = {rows_of("out", out, row, rows, o.out_stride ? es * o.out_stride : row),
+                         {"lse", lse, 4 * rows * o.nh}, {"scratch", scratch, (__int128)scratch_bytes}};
+    return outputs_overlap(in, 9, to, 3);
+}
+
 }  // namespace b2

@@ -608,7 +608,8 @@ int b2_page_compact(int32_t* table, int64_t table_stride, const int32_t* lens, i
  * sees what it sees in b2_attention_paged, whose other arguments and results
  * these are: lengths, windows, slopes, rows that see nothing (zeros and -inf),
  * rows that get NaN; no row is touched by another's pages, lengths or values.
- * Rows in no group attend alone.  Groups whose starts do not ascend give rows
+ * Rows in no group attend alone.  out, lse or d_scratch on one another or on an
+ * input is refused (B2_ERR_BAD_ARG).  Groups whose starts do not ascend give rows
  * without meaning, no access out of range.  Scores, softmax and sums are fp32;
  * the products take the probabilities of 16-bit rows in two terms of the
  * cache's type (16 bits of BF16, 22 of F16), of fp32 rows in 22 bits or more.  Every
