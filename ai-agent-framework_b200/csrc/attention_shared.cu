@@ -15,7 +15,7 @@
 // What bounds it: of 64 rows behind 32K shared positions (64 heads on 8 of 128, bf16)
 // 70 GFLOP would take 42 us of the tensor cores; the chain of a tile
 // (scores, exponentials, values, one tile's tensor memory waiting for the next) takes
-// 3000 clocks for products of 1100, so 145 us.
+// 3600 clocks for products of 1650 (two terms of P), so 166 us.
 //
 // Split.  The items of the batch, one after another, are a line of units, a
 // tile being one (and an item's start another).  Share s of G takes the units
@@ -41,12 +41,12 @@
 // split into 2 fp16 or 3 bf16 terms, and their probabilities times 2^14 into as
 // many (22 bits or more: what fp32 results need).  16-bit rows as they are, their
 // probabilities in 2 terms, 22 bits of fp16 or 16 of bf16, as row by row: with one
-// term, 15 % faster, weights that round to the same side move the result by up to
+// term, 12 % faster, weights that round to the same side move the result by up to
 // a step.  Sums, maxima and O in fp32, rounded once.
 //
 // Measured (B200, graphs, all three launches): 8 requests of 8 beams over up to 32K, 32 heads
 // on 8 of 128, fp32 rows 102 us (row by row 389); 64 rows behind 32K, 64 heads on 8,
-// bf16 145 (1010); a prompt of 2048 tokens, the same heads 128 (1064).
+// bf16 166 (1010); a prompt of 2048 tokens, the same heads 149 (1064).
 //
 // A value that one row of an item sees and another does not meets a weight of 0
 // there, and 0 times infinity or NaN is NaN: a row whose result is not finite is
@@ -433,7 +433,8 @@ struct Tm {
     static_assert(kStages >= 3, "three tiles must fit");
     static constexpr int kTotal = kFixed + kQ + (kStagesK + kStagesV) * kTileBytes;
     // tensor memory: two S, three where they fit beside two T (P over it, a third term behind it), then T.
-    // (Three S and one T for 128 dimensions: 64 rows behind 32K 147 -> 142 us, but a prompt 128 -> 143.)
+    // (Three S and one T for 128 dimensions: 64 rows behind 32K 166 -> 153 us, a prompt 149 -> 150, but 897
+    // rows of 32 requests, 8 / 2 heads of 96, capped, 69 -> 80, and 692 fp32 rows, pages of 100, 242 -> 256.)
     static constexpr int kSCols = PT == 3 ? 192 : 128;
     static constexpr int kSBufs = 3 * kSCols + 2 * HD <= 512 ? 3 : 2;
     static constexpr int kTBufs = kSBufs * kSCols + 2 * HD <= 512 ? 2 : 1;
@@ -1673,19 +1674,21 @@ size_t layout(int batch, int nh, int nkv, int hd, int sms, uint8_t* base, Shared
 // products' time).  The two meet where the rows' positions times max(heads to a
 // KV head, 8) x KV heads x dimensions come to some 2^28 (134 MB at 8 heads), in us:
 //   heads, dims, type     rows   positions   of 2^28   row by row   shared
-//   32 / 8, 128, fp32     1 x 4   2080        1/4       14.5         29.5
-//   64 / 8, 128, bf16     1 x 16  2080        1         28.8         30.0
-//   32 / 8, 128, fp32     1 x 64   544        1         28.9         34.4
-//   64 / 1, 128, bf16     4 x 4   2080        1         28.8         28.8
-//   32 / 8, 128, fp32     8 x 8   2080        4         76.0         47.3
-//   64 / 8, 128, bf16     1 x 16  8224        4         71.6         37.0
+//   32 / 8, 128, fp32     1 x 4   2080        1/4       14.4         28.8
+//   64 / 8, 128, bf16     1 x 16  2080        1         28.7         29.4
+//   32 / 8, 128, fp32     1 x 64   544        1         28.8         32.9
+//   64 / 1, 128, bf16     4 x 4   2080        1         29.6         28.8
+//   32 / 8, 128, fp32     8 x 8   2080        4         75.9         45.2
+//   64 / 8, 128, bf16     1 x 16  8224        4         70.9         37.0
 // Positions: the window, or what the table has room for, since the lengths are on
 // the device (16 requests of 1 to 8 rows, window 4096 of 9336, 14 / 2 heads of 64: 22.6
-// and 37; 139 rows of one sequence, window 3: 12.4 and 22.6).
+// and 39; 139 rows of one sequence, window 3: 10.3 and 22.5).
 // Where groups have fewer than two rows on average there is too little to share,
-// however they lie: rows that share nothing take 1.3 to 1.7 times as long in the
-// tiles (64 x 1 rows of 2080 positions, 64 / 8 heads: 97 and 129; 62 rows in 43 groups,
-// 28 / 4 heads of 64, fp32: 35 and 127).
+// however they lie: rows that share nothing take 1.5 to 1.9 times as long in the
+// tiles (64 x 1 rows of 2080 positions, 64 / 8 heads: 100 and 146; 81 rows in 43 groups,
+// 28 / 4 heads of 64, fp32: 29 and 55), and a prompt of 512 tokens beside 520 tokens of
+// rows of 500 is 262 and 300 (by itself in tiles 43).  Groups without rows count, so a
+// prompt of 300 in a table of 256 requests takes 65 where tiles would take 41.
 bool row_by_row(const b2_paged_kv& kv, const b2_paged_attn_opts& o, int batch, int n_groups) {
     const double room = (double)o.max_pages * kv.page_size;
     const double positions = batch * (o.window > 0 ? std::min(room, (double)o.window) : room);

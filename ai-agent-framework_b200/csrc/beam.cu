@@ -10,14 +10,15 @@
 // that list.  The second takes a request's lists together: the k-th largest of
 // a few entries off the top of each list bounds the k-th best candidate, and
 // what reaches the bound is ordered by counting, in 64 bits.  Two beams' log Z
-// are known to fp32 sums; where that leaves the order of two neighbours open
-// (one pair in some 10^4), the CTA takes the two rows' log Z in 64 bits.
+// are known to fp32 exponentials; where that leaves the order of two candidates open
+// (a request in some 400), the CTA takes the two rows' log Z in 64 bits.
 //
-// Bound by the pass: 64 requests of 16 beams over 128256 bf16 logits, 263 MB, take 78 us
+// Bound by the pass: 64 requests of 16 beams over 128256 bf16 logits, 263 MB, take 79 us
 // with the histories' reordering (40 us of HBM; the pass 65, with exponential units and issue
-// slots half busy, the lists 8, the histories 7, overlapped in part); 4 beams of one
-// request over 152064 fp32 14.5 us, launches all of it.  A cluster for each request that shares
-// the sums in 64 bits lost: 105 -> 115 us where one was needed, 14.5 -> 16.5 where none was.
+// slots half busy, the lists 11, the histories 7, overlapped in part), or 138 where a request
+// needs sums in 64 bits: 25 us a beam.  Beams that tie all need them: 16 with the same logits and
+// scores 420 us, 64 1640.  4 beams of one request over 151936 fp32 16.5 us, launches all of it.
+// A cluster for each request that shares the sums in 64 bits lost: 105 -> 115 us.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -157,7 +158,7 @@ __device__ __forceinline__ double exp64(double x, const double* pow2) {
 }
 
 // log Z of a row whose largest logit is m in 64 bits, by the CTA: bound by the
-// SM's 64-bit units, some 20 us for 128256 logits.
+// SM's 64-bit units, some 25 us for 128256 logits.
 template <typename T>
 __device__ double log_z64(const T* x, int n, bool wide, double m, double* part, const double* pow2) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
