@@ -261,11 +261,13 @@ int matvec_lean(int qtype, const void* w, const float* x, float* y, int rows, in
         (reinterpret_cast<uintptr_t>(x) & 15))
         return 1;
     const size_t smem = qtype == 8 ? lean_smem_bytes<8>(cols / 32) : lean_smem_bytes<2>(cols / 32);
-    if (smem > 232448) return 1;
+    constexpr int most = 232448;
+    if (smem > most) return 1;
     auto kern = qtype == 8 ? matvec_lean_kernel<8> : matvec_lean_kernel<2>;
     const int warps = qtype == 8 ? LvCfg<8>::kWarps : LvCfg<2>::kWarps;
     const int rw = qtype == 8 ? LvCfg<8>::kRows : LvCfg<2>::kRows;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+    // (the limit is the kernel's, not the call's: always the most, so that no thread lowers it under another's launch)
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess) {
         *err = "matvec: shared-memory attribute refused";
         return B2_ERR_CUDA;
     }
